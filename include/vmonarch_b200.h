@@ -285,6 +285,63 @@ int vmb_quant_e4m3(const void* src, const vmb_view* src_view, void* dst, const v
 int vmb_cast_f32_view(const float* src, const vmb_view* src_view, void* dst, const vmb_view* dst_view, int64_t n1,
                       int64_t n2, int64_t batch, int64_t rows, int64_t cols, int32_t dtype, void* stream);
 
+/*
+ * Attention over packed sequences of different lengths (no reference counterpart): the rows of q
+ * (q_total x heads x dim) and of k, v (k_total x kv_heads x dim) hold the sequences one after
+ * another; query head h reads key / value head h / (heads / kv_heads). With `causal`, local query i of
+ * a sequence of nq queries and nk keys sees its first nk - nq + i + 1 keys. A query that sees no
+ * key has o = 0, lse = -inf and passes no gradient. dim: a multiple of 8, at most 128.
+ *
+ * The work is described by units built on the host from the sequence lengths, in device memory
+ * (int32, 48 bytes each). They are trusted: q_row + q_valid <= q_total, k_row + k_valid <= k_total.
+ *  units    (forward) at most 256 queries of one sequence, key tiles [begin, end) of 128 keys
+ *  q_units  (backward, dQ) the same with at most 128 queries
+ *  kv_units (backward, dK / dV) at most 128 keys; k_row / k_valid are theirs, q_row / q_valid the whole
+ *           sequence's queries, vis0 the local query that first sees the unit's key 0 (a large
+ *           negative number when not causal); [begin, end) steps over (head of the group, 64-query
+ *           tile from max(vis0, 0) / 64 on), heads outermost
+ * For the first two, vis0 is the number of keys that local query 0 of the unit sees, before the limits
+ * 0 and k_valid, and k_row / k_valid are the sequence's keys. stat_row: first row of the unit's
+ * queries (kv_units: of the sequence's) in the backward's statistics, where every sequence starts
+ * at a multiple of 128; stat_rows is their total. part: -1, or the slot (0 .. n_parts - 1) of a
+ * piece of work that is split over its key tiles (dQ, forward) or steps (dK / dV); the pieces of a
+ * split unit take consecutive slots, and `joins` lists them as (first unit, number of pieces).
+ */
+typedef struct vmb_packed_unit {
+  int32_t q_row, q_valid, k_row, k_valid, vis0, begin, end, part, stat_row, reserved[3];
+} vmb_packed_unit;
+
+typedef struct vmb_packed_list {
+  const vmb_packed_unit* units;  /* device */
+  const int32_t* joins;          /* device, (first unit, pieces) pairs; NULL when nothing is split */
+  int32_t n_units, n_joins, n_parts, reserved;
+} vmb_packed_list;
+
+typedef struct vmb_rows {  /* [rows][heads][dim] view: strides of a row and of a head, in elements */
+  void* ptr;
+  int64_t row, head;
+} vmb_rows;
+
+typedef struct vmb_packed_args {
+  vmb_rows q, k, v, o;       /* o: written by the forward, read by the backward     */
+  vmb_rows dout, dq, dk, dv; /* backward                                            */
+  vmb_rows o_low;            /* what o's rounding left out: 16-bit (exact o - o), written by the forward
+                                where ptr is not NULL, required by the backward, whose sums o . dout
+                                need more of o than its own 16 bits */
+  float* lse;                /* [heads][q_total] natural log; NULL allowed (forward) */
+  int64_t q_total, k_total, stat_rows;
+  int32_t heads, kv_heads, dim, dtype, causal;
+  float sm_scale;            /* >= 0 */
+  vmb_packed_list units, q_units, kv_units;
+  void* workspace; int64_t workspace_bytes;  /* 256-byte aligned */
+} vmb_packed_args;
+
+/* Workspace of vmb_packed_fwd (0 unless units are split) and of vmb_packed_bwd; -1: malformed. */
+int64_t vmb_packed_fwd_workspace_bytes(const vmb_packed_args* a);
+int64_t vmb_packed_bwd_workspace_bytes(const vmb_packed_args* a);
+int vmb_packed_fwd(const vmb_packed_args* a, void* stream);
+int vmb_packed_bwd(const vmb_packed_args* a, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -104,6 +104,27 @@ class LstepArgs(ctypes.Structure):
     ]
 
 
+class PackedList(ctypes.Structure):
+    _fields_ = [("units", c_vp), ("joins", c_vp), ("n_units", c_i32), ("n_joins", c_i32), ("n_parts", c_i32),
+                ("reserved", c_i32)]
+
+
+class Rows(ctypes.Structure):
+    """vmb_rows: a (rows, heads, dim) tensor with contiguous columns."""
+    _fields_ = [("ptr", c_vp), ("row", c_i64), ("head", c_i64)]
+
+
+class PackedArgs(ctypes.Structure):
+    _fields_ = [(n, Rows) for n in ("q", "k", "v", "o", "dout", "dq", "dk", "dv", "o_low")] + [
+        ("lse", c_vp),
+        ("q_total", c_i64), ("k_total", c_i64), ("stat_rows", c_i64),
+        ("heads", c_i32), ("kv_heads", c_i32), ("dim", c_i32), ("dtype", c_i32), ("causal", c_i32),
+        ("sm_scale", ctypes.c_float),
+        ("units", PackedList), ("q_units", PackedList), ("kv_units", PackedList),
+        ("workspace", c_vp), ("workspace_bytes", c_i64),
+    ]
+
+
 #: every symbol include/vmonarch_b200.h declares, with its ctypes signature
 SIGNATURES = {
     "vmb_abi_version": (ctypes.c_int, []),
@@ -124,6 +145,10 @@ SIGNATURES = {
                                          c_i64, c_i64, c_i32, c_vp]),
     "vmb_quant_e4m3": (ctypes.c_int, [c_vp, ctypes.POINTER(View), c_vp, ctypes.POINTER(View), c_i64, c_i64, c_i64,
                                       c_i64, c_i64, c_i32, ctypes.c_float, c_vp]),
+    "vmb_packed_fwd_workspace_bytes": (c_i64, [ctypes.POINTER(PackedArgs)]),
+    "vmb_packed_bwd_workspace_bytes": (c_i64, [ctypes.POINTER(PackedArgs)]),
+    "vmb_packed_fwd": (ctypes.c_int, [ctypes.POINTER(PackedArgs), c_vp]),
+    "vmb_packed_bwd": (ctypes.c_int, [ctypes.POINTER(PackedArgs), c_vp]),
 }
 
 

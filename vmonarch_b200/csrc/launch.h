@@ -79,6 +79,16 @@ cudaError_t lstep_tc_launch(const LstepParams& p, bool last, bool bwd, bool bf16
 cudaError_t lstep_tc_status(cudaStream_t st, int* out);
 size_t lstep_smem_bytes(int m, int d, int dw, bool last, bool bwd);
 
+// Packed-sequence attention (packed.h): forward, backward and the kernels' pipeline status.
+struct PackedParams;
+cudaError_t packed_fwd(const PackedParams& p, bool bf16, cudaStream_t st);
+cudaError_t packed_status(cudaStream_t st, int* out);
+// dq: the 128-query units (statistics and dQ), kv: the 128-key units (dK, dV); the rest of the two is alike
+cudaError_t packed_bwd(const PackedParams& dq, const PackedParams& kv, bool bf16, cudaStream_t st);
+cudaError_t packed_bwd_status(cudaStream_t st, int* out);
+
+// Adds n to the library's kernel launch count.
+void count_launches(int n);
 // Records `code` and a printf-style message as the calling thread's last error; returns `code`.
 int set_error(int code, const char* fmt, ...);
 

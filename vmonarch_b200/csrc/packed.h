@@ -1,0 +1,57 @@
+// Parameter blocks of the packed-sequence attention kernels (packed_fwd.cu, packed_bwd.cu).
+#pragma once
+#include <cuda.h>
+#include <stdint.h>
+
+#include "fea_params.h"
+
+namespace vmb {
+
+// One unit of a packed call's work, built on the host from the sequence lengths
+// (vmb_packed_unit of include/vmonarch_b200.h, same layout).
+//  forward and dQ : query rows [q_row, q_row + q_valid) (at most 256 / 128) of a sequence whose keys
+//                   are rows [k_row, k_row + k_valid); local query r sees the keys below
+//                   clamp(vis0 + r * causal, 0, k_valid); the unit walks key tiles [begin, end)
+//                   (128 keys each). stat_row: the unit's first row in the padded statistics.
+//  dK / dV        : key rows [k_row, k_row + k_valid) (at most 128) of a sequence whose queries are
+//                   rows [q_row, q_row + q_valid); local key r is seen by the queries from
+//                   vis0 + r on (all of them when not causal); the unit walks steps [begin, end) of
+//                   its (query head of the group, 64-query tile) pairs, the tiles of a head counted
+//                   from max(vis0, 0) / 64. stat_row: the sequence's first padded statistics row.
+//  part           : -1, or the slot that a split unit's partial result goes to
+struct PackedUnit {
+  int32_t q_row, q_valid, k_row, k_valid, vis0, begin, end, part, stat_row, pad0, pad1, pad2;
+};
+
+struct PackedParams {
+  const PackedUnit* units;
+  int n_units;
+  int heads, kv_heads, group, head_chunk;  // head_chunk: (query or kv) heads whose units run together
+  int dim, causal;
+  int64_t q_total, k_total, stat_rows;     // stat_rows: rows of the padded statistics planes
+  float sm_scale;
+  const void *q, *k, *v, *dout;
+  void *o, *o_low, *dq, *dk, *dv;  // o_low: the 16-bit rest that rounding o left out (may be NULL, forward)
+  float* lse;              // [heads][q_total], natural logarithm
+  float* stats;            // backward: planes nl, nc, each [heads][stat_rows]
+  float *part, *part_ml;   // split units: partial tiles and their (max, sum)
+  View qv, kv, vv, ov, olv, dov, dqv, dkv, dvv;  // rows = tokens, s1 = head stride
+};
+
+// Unit and head of a block: chunks of `chunk` heads outermost (their keys and values stay in L2),
+// inside them the units in the host's order (most work first), heads innermost.
+struct UnitHead {
+  int unit, head;
+};
+#ifdef __CUDACC__
+__host__ __device__ __forceinline__ UnitHead unit_of_block(int64_t block, int n_units, int heads, int chunk) {
+  const int64_t per = (int64_t)n_units * chunk;
+  const int c = (int)(block / per);
+  const int rem = (int)(block - c * per);
+  const int left = heads - c * chunk;
+  const int g = left < chunk ? left : chunk;
+  return UnitHead{rem / g, c * chunk + rem % g};
+}
+#endif
+
+}  // namespace vmb

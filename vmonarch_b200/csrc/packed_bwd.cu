@@ -1,0 +1,648 @@
+// Attention over packed sequences of different lengths, backward, on tcgen05 / TMA (packed_fwd.cu has
+// the forward and its definitions).
+//
+//   P_ij = exp(s_ij - lse_i), D_i = sum_c o_ic do_ic, dS_ij = sm_scale P_ij (do_i . v_j - D_i)
+//   dV_j = sum_i P_ij do_i,   dK_j = sum_i dS_ij q_i,   dQ_i = sum_j dS_ij k_j
+// with the sums over i running over every query head that shares the key head. Three kernels, no
+// atomics, so the gradients are the same from run to run:
+//
+// pre   one row per half-warp: nl = -lse log2(e) and nc = -sm_scale D in planes [head][stat_rows], in
+//       which every sequence starts at a multiple of 128 (rows past its end: P = 0). Then
+//       P = 2^(s c + nl) and dS = P (sm_scale dP + nc): two packed FMAs, one exponential, one product.
+//       D takes o with the 16 bits that its rounding left out (o_low): an error of D is shared by a
+//       whole row of dS, so it does not average out in dQ_i = sum_j dS_ij k_j where keys have a mean
+//       (4000 causal queries, D = 128, bf16: dQ off by 4.1e-3 without it, 2.4e-3 with it, of which its
+//       own rounding is 1.7e-3).
+// dkdv  CTA = 128 keys of one key head; walks (query head, 64-query tile): S^T = K Q^T and
+//       dP^T = V dO^T (SS), P^T and dS^T (16-bit) back to TMEM over them, dV += P^T dO and
+//       dK += dS^T Q (TS). thread = key row; two streams of tiles, two warpgroups each.
+//       TMEM: stream b S^T [128b, +64) dP^T [128b + 64, +64), dK [256, +64 NA), dV after it.
+// dq    CTA = 128 queries of one head; walks 128-key tiles: S, dP (SS), dS over S, dQ += dS K (TS).
+//       thread = query row x 32 keys. TMEM: S0 [0,128) S1 [128,256) dP [256,384) dQ [384, +64 NA).
+// Seven products per tile pair instead of five: TMEM cannot hold S, dP, dK, dV and dQ of one tile at
+// once, and recomputing S and dP costs less than adding dQ through memory.
+//
+// Tiles at a sequence's end hold the next sequence's rows. Their scores are dropped by index, and the
+// rows that enter a sum with weight 0 (Q and dO here, K in dq) are cleared in shared memory first, so
+// that nothing another sequence holds (0 x inf) gets into it. P and dS are 16-bit operands of the tensor
+// cores; sums, statistics and accumulators are 32-bit.
+#include "common.cuh"
+#include "launch.h"
+#include "packed.h"
+#include "sm100.cuh"
+#include "tma_host.h"
+
+namespace vmb {
+
+__device__ int g_packed_bwd_err;
+
+namespace {
+
+using namespace sm100;
+
+constexpr int kAtom = 128 * 128;  // 128 rows x 128 B
+constexpr int kAtom64 = 64 * 128;
+constexpr int kThreads = 64 + 128 * 4;  // producer, MMA issuer, four compute warpgroups
+
+struct KParams {
+  CUtensorMap tm_q, tm_k, tm_v, tm_do;  // dkdv: Q, dO boxes of 64 rows; dq: all of 128
+  PackedParams a;
+  float scale_log2;
+};
+
+// P and dS of two scores, packed to 16 bits.
+__device__ __forceinline__ float2 prob2(uint32_t s0, uint32_t s1, float2 sc2, float2 nl2) {
+  const float2 t = __ffma2_rn(make_float2(__uint_as_float(s0), __uint_as_float(s1)), sc2, nl2);
+  return make_float2(fast_exp2(t.x), fast_exp2(t.y));
+}
+__device__ __forceinline__ float2 dscore2(float2 p, uint32_t d0, uint32_t d1, float2 sm2, float2 nc2) {
+  return __fmul2_rn(p, __ffma2_rn(make_float2(__uint_as_float(d0), __uint_as_float(d1)), sm2, nc2));
+}
+
+// Rows [first, rows) of `atoms` consecutive swizzle atoms of `rows` x 128 B, cleared by nthreads threads.
+__device__ __forceinline__ void clear_rows(uint32_t base, int atoms, int rows, int first, int tid, int nthreads) {
+  const int n = (rows - first) * 8;
+  for (int i = tid; i < n * atoms; i += nthreads) {
+    const int a = i / n, rem = i - a * n;
+    asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(base + a * rows * 128 + (first + (rem >> 3)) * 128 +
+                                                                 (rem & 7) * 16),
+                 "r"(0)
+                 : "memory");
+  }
+}
+
+// 16-bit rows of a [128][64 NA] fp32 accumulator into swizzled staging: 32-column chunks [c0, c1).
+template <typename T>
+__device__ __forceinline__ void stage_rows(uint32_t taddr, uint32_t stage, int row, bool any, int c0, int c1) {
+#pragma unroll 1
+  for (int c = c0; c < c1; ++c) {
+    uint32_t v[32];
+    if (any) {
+      tmem_ld32(taddr + c * 32, v);
+      tmem_wait_ld();
+    } else {
+#pragma unroll
+      for (int i = 0; i < 32; ++i) v[i] = 0u;
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      uint32_t w[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        w[i] = Elem<T>::pack(__uint_as_float(v[8 * k + 2 * i]), __uint_as_float(v[8 * k + 2 * i + 1]));
+      const int chunk = (c & 1) * 4 + k;
+      asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(stage + (c >> 1) * kAtom + row * 128 +
+                                                                   ((chunk ^ (row & 7)) << 4)),
+                   "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3])
+                   : "memory");
+    }
+  }
+}
+// The staged rows [0, rows) to global memory, whole 16-byte chunks below `dim` columns.
+template <typename T, int NA>
+__device__ __forceinline__ void store_rows(uint32_t stage, T* out, int64_t rs, int rows, int dim, int tid, int nthreads) {
+  constexpr int CH = 8 * NA;
+  for (int i = tid; i < rows * CH; i += nthreads) {
+    const int r = i / CH, ch = i % CH;
+    uint32_t x[4];
+    asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3])
+                 : "r"(stage + (ch >> 3) * kAtom + r * 128 + (((ch & 7) ^ (r & 7)) << 4)));
+    if (ch * 8 < dim) *reinterpret_cast<uint4*>(out + (int64_t)r * rs + ch * 8) = make_uint4(x[0], x[1], x[2], x[3]);
+  }
+}
+
+// ------------------------------------------------------------------------------------ statistics
+// Block = one 128-query unit of one head; 16 lanes per row, 16 bytes each of o and dO.
+template <typename T>
+__global__ void __launch_bounds__(256) packed_pre_kernel(const __grid_constant__ PackedParams a) {
+  const UnitHead uh = unit_of_block(blockIdx.x, a.n_units, a.heads, a.heads);
+  const PackedUnit u = a.units[uh.unit];
+  const int head = uh.head, sub = threadIdx.x & 15;
+  float* nl = a.stats + (int64_t)head * a.stat_rows + u.stat_row;
+  float* nc = nl + (int64_t)a.heads * a.stat_rows;
+#pragma unroll 2
+  for (int r = threadIdx.x >> 4; r < 128; r += 16) {
+    const bool valid = r < u.q_valid;
+    float d = 0.f;
+    if (valid && sub * 8 < a.dim) {
+      const int64_t row = u.q_row + r;
+      auto load = [&](const void* t, const View& v) {
+        return *reinterpret_cast<const uint4*>(static_cast<const T*>(t) + row * v.rs + head * v.s1 + sub * 8);
+      };
+      const uint4 x = load(a.o, a.ov), w = load(a.o_low, a.olv), y = load(a.dout, a.dov);
+      const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ws[4] = {w.x, w.y, w.z, w.w}, ys[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 f = Elem<T>::unpack(xs[i]), l = Elem<T>::unpack(ws[i]), g = Elem<T>::unpack(ys[i]);
+        d = fmaf(f.x + l.x, g.x, fmaf(f.y + l.y, g.y, d));
+      }
+    }
+#pragma unroll
+    for (int s = 8; s > 0; s >>= 1) d += __shfl_xor_sync(0xffffffffu, d, s);
+    if (sub == 0) {
+      // finite, so that a row without keys and the rows past the end have P = 2^(finite - 1e30) = 0
+      const float lse = valid ? a.lse[(int64_t)head * a.q_total + u.q_row + r] : -INFINITY;
+      nl[r] = lse == -INFINITY ? -1e30f : -lse * kLog2e;
+      nc[r] = valid ? -a.sm_scale * d : 0.f;
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------------ dK, dV
+template <int NA>
+struct DkdvCfg {
+  static constexpr int RES = 2 * NA * kAtom;         // K | V
+  static constexpr int SLOT_T = 2 * NA * kAtom64;    // Q | dO of 64 queries
+  static constexpr int SLOT = SLOT_T + 1024;         // + nl, nc (256 B each)
+  static constexpr int NQ = NA == 2 ? 4 : 8;
+  static constexpr int SMEM = 1024 + RES + NQ * SLOT;
+  static_assert(SMEM <= 232448 - 1024, "shared memory budget");
+  static_assert(NQ * SLOT >= 2 * NA * kAtom, "the epilogue stages dK and dV in the query slots");
+};
+
+template <typename T, int NA>
+__global__ void __launch_bounds__(kThreads, 1) packed_dkdv_kernel(const __grid_constant__ KParams p) {
+  using C = DkdvCfg<NA>;
+  constexpr int NQ = C::NQ;
+  constexpr bool kBf16 = Elem<T>::is_bf16;
+  constexpr uint32_t IDESC_SP = idesc_f16(kBf16, 128, 64, false, false);        // S^T, dP^T
+  constexpr uint32_t IDESC_ACC = idesc_f16(kBf16, 128, 64 * NA, false, true);   // dK, dV (B MN-major)
+  constexpr uint32_t T_DK = 256, T_DV = 256 + 64 * NA;
+  // column of the packed P^T / dS^T of queries [16 kk, +16) inside a tile's S^T / dP^T: a warpgroup
+  // writes inside the 32 columns that it loaded itself
+  auto pcol = [](int kk) -> uint32_t { return 32 * (kk >> 1) + 8 * (kk & 1); };
+
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ __align__(8) uint64_t bars[6 + 2 * NQ];
+  __shared__ uint32_t tmem_base_sh;
+  __shared__ int abort_sh;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const UnitHead uh = unit_of_block(blockIdx.x, p.a.n_units, p.a.kv_heads, p.a.head_chunk);
+  const PackedUnit u = p.a.units[uh.unit];
+  const int kvh = uh.head;
+  const int t_first = max(u.vis0, 0) >> 6;
+  const int per_head = max(((u.q_valid + 63) >> 6) - t_first, 1);  // tiles of one query head
+  const int n = u.end - u.begin;
+  // step i -> query head and first local query of its tile
+  auto step_head = [&](int i) { return kvh * p.a.group + (u.begin + i) / per_head; };
+  auto step_q0 = [&](int i) { return (t_first + (u.begin + i) % per_head) * 64; };
+
+  const uint32_t sbase = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  const uint32_t sK = sbase, sV = sbase + NA * kAtom, sSlots = sbase + C::RES;
+  auto sQ = [&](int s) { return sSlots + s * C::SLOT; };
+  auto sDO = [&](int s) { return sSlots + s * C::SLOT + NA * kAtom64; };
+  auto sStat = [&](int s) { return sSlots + s * C::SLOT + C::SLOT_T; };
+  const uint32_t bar0 = smem_u32(bars);
+  const uint32_t BAR_KV = bar0, BAR_DONE = bar0 + 8u;
+  auto BAR_SP = [&](int b) { return bar0 + 8u * (2 + b); };
+  auto BAR_PDS = [&](int b) { return bar0 + 8u * (4 + b); };
+  auto BAR_QFULL = [&](int s) { return bar0 + 8u * (6 + s); };
+  auto BAR_QEMPTY = [&](int s) { return bar0 + 8u * (6 + NQ + s); };
+  volatile int* abort = &abort_sh;
+
+  if (threadIdx.x == 0) {
+    abort_sh = 0;
+    mbar_init(BAR_KV, 1);
+    mbar_init(BAR_DONE, 1);
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(BAR_SP(b), 1);
+      mbar_init(BAR_PDS(b), 256);
+    }
+    for (int s = 0; s < NQ; ++s) {
+      mbar_init(BAR_QFULL(s), 1);
+      mbar_init(BAR_QEMPTY(s), 1);
+    }
+    fence_mbar_init();
+  }
+  if (warp == 0) {
+    tmem_alloc(smem_u32(&tmem_base_sh), 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_base_sh;
+
+  if (warp == 0) {
+    // ---------------------------------------------------------------- TMA producer
+    if (lane == 0 && n > 0) {
+      int armed[NQ];
+      for (int s = 0; s < NQ; ++s) armed[s] = 0;
+      prefetch_tmap(&p.tm_q);
+      prefetch_tmap(&p.tm_do);
+      mbar_expect_tx(BAR_KV, C::RES);
+      for (int x = 0; x < NA; ++x) {
+        tma_load(sK + x * kAtom, &p.tm_k, 64 * x, u.k_row, BIdx(kvh, 0, 0), BAR_KV);
+        tma_load(sV + x * kAtom, &p.tm_v, 64 * x, u.k_row, BIdx(kvh, 0, 0), BAR_KV);
+      }
+      for (int i = 0; i < n; ++i) {
+        const int s = i % NQ;
+        if (i >= NQ && !mbar_wait(BAR_QEMPTY(s), ((i / NQ) - 1) & 1, abort, &g_packed_bwd_err, 1)) break;
+        const int h = step_head(i), q0 = step_q0(i);
+        mbar_expect_tx(BAR_QFULL(s), C::SLOT_T + 512);
+        for (int x = 0; x < NA; ++x) {
+          tma_load(sQ(s) + x * kAtom64, &p.tm_q, 64 * x, u.q_row + q0, BIdx(h, 0, 0), BAR_QFULL(s));
+          tma_load(sDO(s) + x * kAtom64, &p.tm_do, 64 * x, u.q_row + q0, BIdx(h, 0, 0), BAR_QFULL(s));
+        }
+        const float* st = p.a.stats + (int64_t)h * p.a.stat_rows + u.stat_row + q0;
+        bulk_load(sStat(s), st, 256, BAR_QFULL(s));
+        bulk_load(sStat(s) + 256, st + (int64_t)p.a.heads * p.a.stat_rows, 256, BAR_QFULL(s));
+        if (i + NQ < n) {  // the tile one ring ahead into L2
+          const int ha = step_head(i + NQ), qa = u.q_row + step_q0(i + NQ);
+          for (int x = 0; x < NA; ++x) {
+            tma_prefetch(&p.tm_q, 64 * x, qa, BIdx(ha, 0, 0));
+            tma_prefetch(&p.tm_do, 64 * x, qa, BIdx(ha, 0, 0));
+          }
+        }
+        armed[s] = i / NQ + 1;
+      }
+      mbar_wait_drain(BAR_KV, 0);
+      for (int s = 0; s < NQ; ++s)
+        if (armed[s] > 0) mbar_wait_drain(BAR_QFULL(s), (armed[s] - 1) & 1);
+    }
+  } else if (warp == 1) {
+    // ---------------------------------------------------------------- MMA issuer
+    const uint32_t leader = elect_one() ? 1u : 0u;
+    auto wwait = [&](uint32_t bar, uint32_t parity, int code) -> bool {
+      return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort, &g_packed_bwd_err, code));
+    };
+    auto issue_sp = [&](int i) -> bool {
+      const int s = i % NQ;
+      if (!wwait(BAR_QFULL(s), (i / NQ) & 1, 2)) return false;
+      tc_fence_after();
+      const uint32_t tb = tmem + 128 * (i & 1);
+#pragma unroll
+      for (int kk = 0; kk < 4 * NA; ++kk) {  // S^T = K Q^T
+        const uint32_t oa = (kk >> 2) * kAtom + (kk & 3) * 32, ob = (kk >> 2) * kAtom64 + (kk & 3) * 32;
+        mma_ss_if(leader, tb, smem_desc_sw128(sK + oa, 16, 1024), smem_desc_sw128(sQ(s) + ob, 16, 1024), IDESC_SP, kk > 0);
+      }
+#pragma unroll
+      for (int kk = 0; kk < 4 * NA; ++kk) {  // dP^T = V dO^T
+        const uint32_t oa = (kk >> 2) * kAtom + (kk & 3) * 32, ob = (kk >> 2) * kAtom64 + (kk & 3) * 32;
+        mma_ss_if(leader, tb + 64, smem_desc_sw128(sV + oa, 16, 1024), smem_desc_sw128(sDO(s) + ob, 16, 1024), IDESC_SP,
+                  kk > 0);
+      }
+      mma_commit_if(leader, BAR_SP(i & 1));
+      return true;
+    };
+    bool ok = n <= 0 || wwait(BAR_KV, 0, 2);
+    if (ok && n > 0) ok = issue_sp(0);
+    if (ok && n > 1) ok = issue_sp(1);
+    for (int i = 0; ok && i < n; ++i) {
+      if (!wwait(BAR_PDS(i & 1), (i >> 1) & 1, 4)) break;
+      tc_fence_after();
+      const int s = i % NQ;
+      const uint32_t pt = tmem + 128 * (i & 1), dst = pt + 64;
+#pragma unroll
+      for (int kk = 0; kk < 4; ++kk)  // dK += dS^T Q over 64 queries
+        mma_ts_if(leader, tmem + T_DK, dst + pcol(kk), smem_desc_sw128(sQ(s) + kk * 2048, kAtom64, 1024), IDESC_ACC,
+                  (i > 0 || kk > 0) ? 1u : 0u);
+#pragma unroll
+      for (int kk = 0; kk < 4; ++kk)  // dV += P^T dO
+        mma_ts_if(leader, tmem + T_DV, pt + pcol(kk), smem_desc_sw128(sDO(s) + kk * 2048, kAtom64, 1024), IDESC_ACC,
+                  (i > 0 || kk > 0) ? 1u : 0u);
+      mma_commit_if(leader, BAR_QEMPTY(s));
+      if (i + 2 < n) ok = issue_sp(i + 2);
+    }
+    if (elect_one()) {
+      mma_commit(BAR_DONE);
+      mbar_wait_drain(BAR_DONE, 0);
+    }
+    __syncwarp();
+  } else {
+    // ---------------------------------------------------------------- compute: thread = key row
+    const int wg = (warp - 2) >> 2;
+    const int stm = wg >> 1, half = wg & 1;  // stream (step parity), 32-query half of its tiles
+    const int quad = warp & 3;
+    const int row = quad * 32 + lane;
+    const uint32_t lane_off = (uint32_t)(quad * 32) << 16;
+    const int tid = (wg & 1) * 128 + (threadIdx.x - 64) % 128;  // within the stream's 256 threads
+    auto warp_wait = [&](uint32_t bar, uint32_t parity, int code) -> bool {
+      return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort, &g_packed_bwd_err, code));
+    };
+    const uint32_t ts = tmem + lane_off + 128 * stm, tdp = ts + 64;
+    const float2 sc2 = make_float2(p.scale_log2, p.scale_log2), sm2 = make_float2(p.a.sm_scale, p.a.sm_scale);
+    bool ok = true;
+    for (int i = stm; i < n; i += 2) {
+      const int s = i % NQ;
+      if (!warp_wait(BAR_SP(stm), (i >> 1) & 1, 8)) { ok = false; break; }
+      if (!warp_wait(BAR_QFULL(s), (i / NQ) & 1, 8)) { ok = false; break; }
+      tc_fence_after();
+      const int q0 = step_q0(i), left = u.q_valid - q0;
+      // key `row` is seen by the tile's queries [c_lo, left)
+      const bool masked = left < 64 || u.vis0 + 127 > q0;
+      const int c_lo = u.vis0 + row - q0;
+      if (left < 64) {  // S^T and dP^T of the tile are complete: only dK and dV still read the slot
+        clear_rows(sQ(s), 2 * NA, 64, left, tid, 256);
+        fence_proxy_async_smem();
+      }
+      const uint32_t st = sStat(s);
+#pragma unroll 1
+      for (int qc = 2 * half; qc < 2 * half + 2; ++qc) {  // 16-query chunks
+        uint32_t sv[16], dv[16];
+        tmem_ld16(ts + 16 * qc, sv);
+        tmem_ld16(tdp + 16 * qc, dv);
+        tmem_wait_ld();
+        uint32_t pk[8], dk[8];
+#pragma unroll
+        for (int e = 0; e < 16; e += 4) {
+          const uint32_t so = st + 4 * (16 * qc + e);
+          float4 l4, c4;
+          asm volatile("ld.shared.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(l4.x), "=f"(l4.y), "=f"(l4.z), "=f"(l4.w) : "r"(so));
+          asm volatile("ld.shared.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(c4.x), "=f"(c4.y), "=f"(c4.z), "=f"(c4.w) : "r"(so + 256));
+          float2 p0 = prob2(sv[e], sv[e + 1], sc2, make_float2(l4.x, l4.y));
+          float2 p1 = prob2(sv[e + 2], sv[e + 3], sc2, make_float2(l4.z, l4.w));
+          float2 d0 = dscore2(p0, dv[e], dv[e + 1], sm2, make_float2(c4.x, c4.y));
+          float2 d1 = dscore2(p1, dv[e + 2], dv[e + 3], sm2, make_float2(c4.z, c4.w));
+          if (masked) {
+            const int c = 16 * qc + e;
+            if (c < c_lo || c >= left) p0.x = d0.x = 0.f;
+            if (c + 1 < c_lo || c + 1 >= left) p0.y = d0.y = 0.f;
+            if (c + 2 < c_lo || c + 2 >= left) p1.x = d1.x = 0.f;
+            if (c + 3 < c_lo || c + 3 >= left) p1.y = d1.y = 0.f;
+          }
+          pk[e >> 1] = Elem<T>::pack(p0.x, p0.y);
+          pk[(e >> 1) + 1] = Elem<T>::pack(p1.x, p1.y);
+          dk[e >> 1] = Elem<T>::pack(d0.x, d0.y);
+          dk[(e >> 1) + 1] = Elem<T>::pack(d1.x, d1.y);
+        }
+        tmem_st8(ts + pcol(qc), pk);
+        tmem_st8(tdp + pcol(qc), dk);
+      }
+      tmem_wait_st();
+      tc_fence_before();
+      mbar_arrive(BAR_PDS(stm));
+    }
+    if (ok) ok = warp_wait(BAR_DONE, 0, 8);
+    tc_fence_after();
+    // epilogue: warpgroups 0, 1 stage dK, 2, 3 dV, half of the columns each
+    const int mat = wg >> 1;
+    if (ok)
+      stage_rows<T>(tmem + lane_off + (mat ? T_DV : T_DK), sSlots + mat * NA * kAtom, row, n > 0, (wg & 1) * NA,
+                    ((wg & 1) + 1) * NA);
+    ok = named_bar_and(1, 512, ok && !*abort);
+    if (ok) {
+      T* out = mat ? static_cast<T*>(p.a.dv) + (int64_t)u.k_row * p.a.dvv.rs + (int64_t)kvh * p.a.dvv.s1
+                   : static_cast<T*>(p.a.dk) + (int64_t)u.k_row * p.a.dkv.rs + (int64_t)kvh * p.a.dkv.s1;
+      store_rows<T, NA>(sSlots + mat * NA * kAtom, out, mat ? p.a.dvv.rs : p.a.dkv.rs, u.k_valid, p.a.dim, tid, 256);
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 0) tmem_dealloc(tmem, 512);
+}
+
+// ------------------------------------------------------------------------------------ dQ
+template <int NA>
+struct DqCfg {
+  static constexpr int TILE = NA * kAtom;
+  static constexpr int NK = NA == 2 ? 3 : 5, NV = NA == 2 ? 2 : 4;
+  static constexpr int SMEM = 1024 + (2 + NK + NV) * TILE;
+  static_assert(SMEM <= 232448 - 1024, "shared memory budget");
+};
+
+template <typename T, int NA>
+__global__ void __launch_bounds__(kThreads, 1) packed_dq_kernel(const __grid_constant__ KParams p) {
+  using C = DqCfg<NA>;
+  constexpr int NK = C::NK, NV = C::NV;
+  constexpr uint32_t TILE = C::TILE;
+  constexpr bool kBf16 = Elem<T>::is_bf16;
+  constexpr uint32_t IDESC_S = idesc_f16(kBf16, 128, 128, false, false);
+  constexpr uint32_t IDESC_DQ = idesc_f16(kBf16, 128, 64 * NA, false, true);
+  constexpr uint32_t T_DP = 256, T_DQ = 384;
+  constexpr int B_Q = 0, B_DONE = 1, B_S = 2, B_DS = 4, B_DP = 6, B_DPFREE = 7, B_KFULL = 8, B_KEMPTY = B_KFULL + NK,
+                B_VFULL = B_KEMPTY + NK, B_VEMPTY = B_VFULL + NV, NBARS = B_VEMPTY + NV;
+
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ __align__(8) uint64_t bars[NBARS];
+  __shared__ uint32_t tmem_base_sh;
+  __shared__ int abort_sh;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const UnitHead uh = unit_of_block(blockIdx.x, p.a.n_units, p.a.heads, p.a.head_chunk);
+  const PackedUnit u = p.a.units[uh.unit];
+  const int head = uh.head, kvh = head / p.a.group;
+  auto limit = [&](int r) { return max(0, min(u.k_valid, p.a.causal ? u.vis0 + r : u.k_valid)); };
+  const int n = u.end - u.begin;
+
+  const uint32_t sbase = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  const uint32_t sQ = sbase, sDO = sbase + TILE, sK = sbase + 2 * TILE, sV = sK + NK * TILE;
+  const uint32_t bar0 = smem_u32(bars);
+  auto BAR = [&](int i) { return bar0 + 8u * (uint32_t)i; };
+  volatile int* abort = &abort_sh;
+
+  if (threadIdx.x == 0) {
+    abort_sh = 0;
+    for (int i = 0; i < NBARS; ++i)
+      mbar_init(BAR(i), i == B_DS || i == B_DS + 1 || i == B_DPFREE ? 512 : 1);
+    fence_mbar_init();
+  }
+  if (warp == 0) {
+    tmem_alloc(smem_u32(&tmem_base_sh), 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_base_sh;
+
+  if (warp == 0) {
+    // ---------------------------------------------------------------- TMA producers: lane 0 Q, dO, K; lane 1 V
+    if (lane < 2 && n > 0) {
+      const bool kl = lane == 0;
+      const int nslot = kl ? NK : NV;
+      const CUtensorMap* map = kl ? &p.tm_k : &p.tm_v;
+      prefetch_tmap(map);
+      if (kl) {
+        mbar_expect_tx(BAR(B_Q), 2 * TILE);
+        for (int x = 0; x < NA; ++x) {
+          tma_load(sQ + x * kAtom, &p.tm_q, 64 * x, u.q_row, BIdx(head, 0, 0), BAR(B_Q));
+          tma_load(sDO + x * kAtom, &p.tm_do, 64 * x, u.q_row, BIdx(head, 0, 0), BAR(B_Q));
+        }
+      }
+      int armed[NK > NV ? NK : NV];
+      for (int s = 0; s < nslot; ++s) armed[s] = 0;
+      for (int j = 0; j < n; ++j) {
+        const int s = j % nslot;
+        if (j >= nslot && !mbar_wait(BAR((kl ? B_KEMPTY : B_VEMPTY) + s), ((j / nslot) - 1) & 1, abort, &g_packed_bwd_err, 16))
+          break;
+        const uint32_t full = BAR((kl ? B_KFULL : B_VFULL) + s);
+        const int row = u.k_row + (u.begin + j) * 128;
+        mbar_expect_tx(full, TILE);
+        for (int x = 0; x < NA; ++x)
+          tma_load((kl ? sK : sV) + s * TILE + x * kAtom, map, 64 * x, row, BIdx(kvh, 0, 0), full);
+        if (j + nslot < n)
+          for (int x = 0; x < NA; ++x) tma_prefetch(map, 64 * x, row + nslot * 128, BIdx(kvh, 0, 0));
+        armed[s] = j / nslot + 1;
+      }
+      if (kl) mbar_wait_drain(BAR(B_Q), 0);
+      for (int s = 0; s < nslot; ++s)
+        if (armed[s] > 0) mbar_wait_drain(BAR((kl ? B_KFULL : B_VFULL) + s), (armed[s] - 1) & 1);
+    }
+  } else if (warp == 1) {
+    // ---------------------------------------------------------------- MMA issuer
+    const uint32_t leader = elect_one() ? 1u : 0u;
+    auto wwait = [&](int bar, uint32_t parity, int code) -> bool {
+      return __all_sync(0xffffffffu, mbar_wait(BAR(bar), parity, abort, &g_packed_bwd_err, code));
+    };
+    auto issue = [&](int j, bool dp) -> bool {  // S(j) = Q K^T, or dP(j) = dO V^T
+      const int s = dp ? j % NV : j % NK;
+      if (!wwait((dp ? B_VFULL : B_KFULL) + s, (j / (dp ? NV : NK)) & 1, 32)) return false;
+      tc_fence_after();
+      const uint32_t ab = dp ? sDO : sQ, bb = (dp ? sV : sK) + s * TILE;
+      const uint32_t d = dp ? tmem + T_DP : tmem + 128u * (uint32_t)(j & 1);
+#pragma unroll
+      for (int kk = 0; kk < 4 * NA; ++kk) {
+        const uint32_t off = (kk >> 2) * kAtom + (kk & 3) * 32;
+        mma_ss_if(leader, d, smem_desc_sw128(ab + off, 16, 1024), smem_desc_sw128(bb + off, 16, 1024), IDESC_S, kk > 0);
+      }
+      mma_commit_if(leader, BAR(dp ? B_DP : B_S + (j & 1)));
+      if (dp) mma_commit_if(leader, BAR(B_VEMPTY + s));
+      return true;
+    };
+    bool ok = n <= 0 || wwait(B_Q, 0, 32);
+    if (ok && n > 0) ok = issue(0, false) && issue(0, true);
+    if (ok && n > 1) ok = issue(1, false);
+    for (int j = 0; ok && j < n; ++j) {
+      if (j + 1 < n && (!wwait(B_DPFREE, j & 1, 64) || !issue(j + 1, true))) break;
+      if (!wwait(B_DS + (j & 1), (j >> 1) & 1, 64)) break;
+      tc_fence_after();
+      const uint32_t kb = sK + (j % NK) * TILE, sb = tmem + 128u * (uint32_t)(j & 1);
+#pragma unroll
+      for (int kk = 0; kk < 8; ++kk)  // dQ += dS K; keys [16 kk, +16) of warpgroup kk / 2
+        mma_ts_if(leader, tmem + T_DQ, sb + 32 * (kk >> 1) + 8 * (kk & 1), smem_desc_sw128(kb + kk * 2048, kAtom, 1024),
+                  IDESC_DQ, (j > 0 || kk > 0) ? 1u : 0u);
+      mma_commit_if(leader, BAR(B_KEMPTY + j % NK));
+      if (j + 2 < n) ok = issue(j + 2, false);
+    }
+    if (elect_one()) {
+      mma_commit(BAR(B_DONE));
+      mbar_wait_drain(BAR(B_DONE), 0);
+    }
+    __syncwarp();
+  } else {
+    // ---------------------------------------------------------------- compute: thread = query row x 32 keys
+    const int wg = (warp - 2) >> 2;
+    const int quad = warp & 3;
+    const int row = quad * 32 + lane;
+    const uint32_t lane_off = (uint32_t)(quad * 32) << 16;
+    const int tid = threadIdx.x - 64;
+    const float* stat = p.a.stats + (int64_t)head * p.a.stat_rows + u.stat_row + row;
+    const float fl = stat[0], fc = stat[(int64_t)p.a.heads * p.a.stat_rows];
+    const float2 nl2 = make_float2(fl, fl), nc2 = make_float2(fc, fc);
+    const float2 sc2 = make_float2(p.scale_log2, p.scale_log2), sm2 = make_float2(p.a.sm_scale, p.a.sm_scale);
+    const int my_lim = limit(row), lim_lo = limit(0);
+    auto warp_wait = [&](int bar, uint32_t parity, int code) -> bool {
+      return __all_sync(0xffffffffu, mbar_wait(BAR(bar), parity, abort, &g_packed_bwd_err, code));
+    };
+    bool ok = true;
+    for (int j = 0; j < n; ++j) {
+      if (!warp_wait(B_S + (j & 1), (j >> 1) & 1, 64) || !warp_wait(B_DP, j & 1, 64)) { ok = false; break; }
+      tc_fence_after();
+      const int k0 = (u.begin + j) * 128;
+      const uint32_t ts = tmem + lane_off + 128u * (uint32_t)(j & 1) + 32 * wg;
+      uint32_t sv[32], dv[32], pk[16];
+      tmem_ld32(ts, sv);
+      tmem_ld32(tmem + lane_off + T_DP + 32 * wg, dv);
+      tmem_wait_ld();
+      tc_fence_before();
+      mbar_arrive(BAR(B_DPFREE));
+      if (u.k_valid - k0 < 128) {  // S(j) is complete: only dQ still reads the key tile
+        clear_rows(sK + (j % NK) * TILE, NA, 128, u.k_valid - k0, tid, 512);
+        fence_proxy_async_smem();
+      }
+      const bool masked = lim_lo - k0 < 128;
+      const int valid = my_lim - k0 - 32 * wg;
+#pragma unroll
+      for (int e = 0; e < 32; e += 2) {
+        float2 d = dscore2(prob2(sv[e], sv[e + 1], sc2, nl2), dv[e], dv[e + 1], sm2, nc2);
+        if (masked) {
+          if (e >= valid) d.x = 0.f;
+          if (e + 1 >= valid) d.y = 0.f;
+        }
+        pk[e >> 1] = Elem<T>::pack(d.x, d.y);
+      }
+      tmem_st16(ts, pk);
+      tmem_wait_st();
+      tc_fence_before();
+      mbar_arrive(BAR(B_DS + (j & 1)));
+    }
+    if (ok) ok = warp_wait(B_DONE, 0, 64);
+    tc_fence_after();
+    // epilogue: 16-bit dQ through the idle K ring; a warpgroup stages 32-column chunks wg, wg + 4, ...
+    if (ok && wg < 2 * NA) stage_rows<T>(tmem + lane_off + T_DQ, sK, row, n > 0, wg, wg + 1);
+    ok = named_bar_and(1, 512, ok && !*abort);
+    if (ok)
+      store_rows<T, NA>(sK, static_cast<T*>(p.a.dq) + (int64_t)u.q_row * p.a.dqv.rs + (int64_t)head * p.a.dqv.s1, p.a.dqv.rs,
+                        u.q_valid, p.a.dim, tid, 512);
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 0) tmem_dealloc(tmem, 512);
+}
+
+template <typename Kern>
+cudaError_t run(Kern kern, int smem, int64_t blocks, const KParams& p, cudaStream_t st) {
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return e;
+  if (blocks > 0x7fffffff) return cudaErrorInvalidConfiguration;
+  kern<<<(unsigned)blocks, kThreads, smem, st>>>(p);
+  return cudaGetLastError();
+}
+
+template <typename T, int NA>
+cudaError_t launch(const PackedParams& dq, const PackedParams& kv, cudaStream_t st) {
+  constexpr bool bf16 = Elem<T>::is_bf16;
+  if (dq.n_units > 0) {
+    const int64_t blocks = (int64_t)dq.n_units * dq.heads;
+    if (blocks > 0x7fffffff) return cudaErrorInvalidConfiguration;
+    packed_pre_kernel<T><<<(unsigned)blocks, 256, 0, st>>>(dq);
+    cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) return e;
+  }
+  KParams p{};
+  p.scale_log2 = dq.sm_scale * kLog2e;
+  auto map = [&](CUtensorMap* m, const void* base, int64_t rows, int heads, const View& v, int box) {
+    return rows == 0 || tma::make_map_view(m, base, bf16, dq.dim, rows, heads, v, heads, 1, box);
+  };
+  if (!map(&p.tm_k, dq.k, dq.k_total, dq.kv_heads, dq.kv, 128) || !map(&p.tm_v, dq.v, dq.k_total, dq.kv_heads, dq.vv, 128))
+    return cudaErrorInvalidValue;
+  if (kv.n_units > 0) {
+    if (!map(&p.tm_q, kv.q, kv.q_total, kv.heads, kv.qv, 64) || !map(&p.tm_do, kv.dout, kv.q_total, kv.heads, kv.dov, 64))
+      return cudaErrorInvalidValue;
+    p.a = kv;
+    cudaError_t e = run(packed_dkdv_kernel<T, NA>, DkdvCfg<NA>::SMEM, (int64_t)kv.n_units * kv.kv_heads, p, st);
+    if (e != cudaSuccess) return e;
+  }
+  if (dq.n_units > 0) {
+    if (!map(&p.tm_q, dq.q, dq.q_total, dq.heads, dq.qv, 128) || !map(&p.tm_do, dq.dout, dq.q_total, dq.heads, dq.dov, 128))
+      return cudaErrorInvalidValue;
+    p.a = dq;
+    return run(packed_dq_kernel<T, NA>, DqCfg<NA>::SMEM, (int64_t)dq.n_units * dq.heads, p, st);
+  }
+  return cudaSuccess;
+}
+
+}  // namespace
+
+cudaError_t packed_bwd(const PackedParams& dq, const PackedParams& kv, bool bf16, cudaStream_t st) {
+  if (dq.dim > 64) return bf16 ? launch<__nv_bfloat16, 2>(dq, kv, st) : launch<__half, 2>(dq, kv, st);
+  return bf16 ? launch<__nv_bfloat16, 1>(dq, kv, st) : launch<__half, 1>(dq, kv, st);
+}
+
+cudaError_t packed_bwd_status(cudaStream_t st, int* out) {
+  int zero = 0;
+  cudaError_t e = cudaMemcpyFromSymbolAsync(out, g_packed_bwd_err, sizeof(int), 0, cudaMemcpyDeviceToHost, st);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(st);
+  if (e == cudaSuccess && *out) e = cudaMemcpyToSymbolAsync(g_packed_bwd_err, &zero, sizeof(int), 0, cudaMemcpyHostToDevice, st);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(st);
+  return e;
+}
+
+}  // namespace vmb
