@@ -342,6 +342,46 @@ int64_t vmb_packed_bwd_workspace_bytes(const vmb_packed_args* a);
 int vmb_packed_fwd(const vmb_packed_args* a, void* stream);
 int vmb_packed_bwd(const vmb_packed_args* a, void* stream);
 
+/*
+ * Paged key / value caches (no reference counterpart). A pool holds num_pages pages of page_size slots;
+ * a page of one tensor is [kv_heads][page_size][dim], anywhere its strides put it (elements, multiples
+ * of 8; 16-byte aligned base). dim: a multiple of 8, at most 128.
+ */
+typedef struct vmb_pages {
+  void* ptr;
+  int64_t page, head, slot;  /* strides in elements */
+} vmb_pages;
+
+/* Attention of one new token per sequence: q, o [batch][heads][dim]; token t of sequence b lies in slot
+ * t % page_size of page table[b * table_stride + t / page_size], t < lengths[b]. A sequence of length 0
+ * has o = 0, lse = -inf. Lengths above table_width * page_size are cut to it and page ids outside the
+ * pool read as zeros (their content is on the device, where a call cannot refuse it). */
+typedef struct vmb_paged_args {
+  vmb_rows q, o;
+  vmb_pages k, v;
+  const int32_t* table;    /* [batch][table_stride], device */
+  const int32_t* lengths;  /* [batch], device */
+  float* lse;              /* [batch][heads] natural logarithm, or NULL */
+  int64_t batch, table_stride, table_width, num_pages;
+  int32_t heads, kv_heads, dim, page_size, dtype;
+  float sm_scale;
+  void* workspace; int64_t workspace_bytes;  /* 256-byte aligned, of vmb_paged_workspace_bytes */
+} vmb_paged_args;
+
+int64_t vmb_paged_workspace_bytes(const vmb_paged_args* a);  /* -1: malformed sizes */
+int vmb_paged_attention(const vmb_paged_args* a, void* stream);
+
+/* Row i of k_new, v_new [count][kv_heads][dim] into slot slots[i] % page_size of page
+ * slots[i] / page_size of each pool. Slots outside the pool (negative ones: padding) are skipped; no slot may be
+ * named twice. 16-bit elements of any kind. */
+int vmb_append_pages(const vmb_rows* k_new, const vmb_rows* v_new, const vmb_pages* k, const vmb_pages* v,
+                     const int32_t* slots, int64_t count, int64_t num_pages, int32_t kv_heads, int32_t dim,
+                     int32_t page_size, void* stream);
+/* Page src[i] to page dst[i], i < count, in both pools. Pairs with a page outside the pool are skipped; no
+ * destination may be another pair's source or destination. */
+int vmb_copy_pages(const vmb_pages* k, const vmb_pages* v, const int32_t* src, const int32_t* dst, int64_t count,
+                   int64_t num_pages, int32_t kv_heads, int32_t dim, int32_t page_size, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,11 +1,12 @@
 """B200-native (sm_100a) VMonarch attention: a drop-in for ``video_monarch_attention``.
 
 Exports the reference's three names (reference ``video_monarch_attention/__init__.py:1-4``) and, beside
-them, attention over packed sequences of different lengths.
+them, attention over packed sequences of different lengths and over a paged key / value cache.
 Importing loads the in-tree CUDA library through its C ABI and raises if it is missing.
 """
 from .kernel import flash_entropy_attention
 from .packed import PackedSequences, packed_attention  # noqa: F401
+from .paged import PagedKVCache, append_pages, copy_pages, paged_attention  # noqa: F401
 from .vmonarch import VMonarchAttention, vmonarch_attention
 
 # the drop-in names: `from vmonarch_b200 import *` brings in what the reference's package does

@@ -125,6 +125,22 @@ class PackedArgs(ctypes.Structure):
     ]
 
 
+class Pages(ctypes.Structure):
+    """vmb_pages: a (pages, kv_heads, page_size, dim) pool with contiguous columns."""
+    _fields_ = [("ptr", c_vp), ("page", c_i64), ("head", c_i64), ("slot", c_i64)]
+
+
+class PagedArgs(ctypes.Structure):
+    _fields_ = [
+        ("q", Rows), ("o", Rows), ("k", Pages), ("v", Pages),
+        ("table", c_vp), ("lengths", c_vp), ("lse", c_vp),
+        ("batch", c_i64), ("table_stride", c_i64), ("table_width", c_i64), ("num_pages", c_i64),
+        ("heads", c_i32), ("kv_heads", c_i32), ("dim", c_i32), ("page_size", c_i32), ("dtype", c_i32),
+        ("sm_scale", ctypes.c_float),
+        ("workspace", c_vp), ("workspace_bytes", c_i64),
+    ]
+
+
 #: every symbol include/vmonarch_b200.h declares, with its ctypes signature
 SIGNATURES = {
     "vmb_abi_version": (ctypes.c_int, []),
@@ -149,6 +165,12 @@ SIGNATURES = {
     "vmb_packed_bwd_workspace_bytes": (c_i64, [ctypes.POINTER(PackedArgs)]),
     "vmb_packed_fwd": (ctypes.c_int, [ctypes.POINTER(PackedArgs), c_vp]),
     "vmb_packed_bwd": (ctypes.c_int, [ctypes.POINTER(PackedArgs), c_vp]),
+    "vmb_paged_workspace_bytes": (c_i64, [ctypes.POINTER(PagedArgs)]),
+    "vmb_paged_attention": (ctypes.c_int, [ctypes.POINTER(PagedArgs), c_vp]),
+    "vmb_append_pages": (ctypes.c_int, [ctypes.POINTER(Rows), ctypes.POINTER(Rows), ctypes.POINTER(Pages),
+                                        ctypes.POINTER(Pages), c_vp, c_i64, c_i64, c_i32, c_i32, c_i32, c_vp]),
+    "vmb_copy_pages": (ctypes.c_int, [ctypes.POINTER(Pages), ctypes.POINTER(Pages), c_vp, c_vp, c_i64, c_i64, c_i32,
+                                      c_i32, c_i32, c_vp]),
 }
 
 

@@ -1,0 +1,454 @@
+// Attention of one new token per sequence over a paged key / value cache.
+//
+//   o_b,h = sum_t p_t v_t / sum_t p_t,  p_t = exp(sm_scale q_b,h . k_t - m),  t < lengths[b],
+// where token t of sequence b lies in slot t % page_size of page table[b][t / page_size].
+//
+// Every cached key and value is read once for all the query heads that share it, so the work is bound
+// by memory: 4 D bytes and 4 D group flops a token and key head. The work items (sequence, key
+// head, chunk of up to 8 NT query heads), each a run of 64-token tiles, are laid end to end and every
+// block takes an equal share of the tiles, whatever the sequences' lengths. An item that lies in one
+// block is finished there; one that is cut leaves a partial (max, sum, 32-bit accumulators) per block, which
+// a second kernel joins. Two blocks per SM, about 128 KB of keys and values in flight on each SM.
+//
+// A warp owns 16 tokens of every tile and its own ring of cp.async stages, so the loop has no block-wide
+// synchronisation; the page ids of a stage are fetched one stage before they are needed. Matrix
+// products (mma.sync, m = 16 tokens, n = 8 heads, so a group of up to 8 wastes nothing):
+//   S^T = K Q^T (A from shared memory, B = Q in registers), P^T moved to operand layout by movmatrix,
+//   O^T += V^T P^T (A by transposing loads).
+// The four warps meet at the end of an item. P is rounded to 16 bits for the product; scores,
+// exponentials, sums and accumulators are 32-bit.
+//
+// Tokens past the length are not read: their slots arrive as zeros and their scores are dropped, as
+// are the columns between D and the padded width. Page ids outside the pool read as zeros, too.
+#include "common.cuh"
+#include "launch.h"
+#include "paged.h"
+
+namespace vmb {
+namespace {
+
+constexpr int kTile = 64;     // tokens per tile: 16 per warp
+constexpr int kWarps = 4;
+constexpr int kMinTiles = 4;  // a block's least share: below it the join costs more than the split gains
+
+template <int DP, int NT>
+struct Cfg {
+  static constexpr int STAGES = DP == 128 ? 3 : 6;
+  static constexpr int STAGE = 2 * 16 * DP * 2;  // K and V of 16 tokens
+  static constexpr int RING = kWarps * STAGES * STAGE;
+  static constexpr int LD = DP + 4;              // joined accumulators: 8 heads per warp at a time
+  static constexpr int SMEM = RING + kWarps * 8 * LD * 4 + kWarps * 8 * 2 * 4;
+};
+
+__device__ __forceinline__ uint32_t movmatrix(uint32_t x) {
+  uint32_t y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+__device__ __forceinline__ int tiles_of(int len) { return len > 0 ? (len + kTile - 1) / kTile : 1; }
+__device__ __forceinline__ int seq_len(const PagedParams& p, int b) {
+  return max(0, min(p.lengths[b], p.max_len));
+}
+
+// The flat order of tiles: sequences, then items (key head, head chunk) of a sequence, then its tiles.
+// Warp-collective: total tiles of one item row summed over sequences, and the sequence that holds `at`.
+__device__ __forceinline__ long long total_tiles(const PagedParams& p, int lane) {
+  long long sum = 0;
+  for (int b = lane; b < p.batch; b += 32) sum += tiles_of(seq_len(p, b));
+#pragma unroll
+  for (int s = 16; s > 0; s >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
+  return sum;
+}
+// Blocks that take part: every one has at least kMinTiles tiles.
+__device__ __forceinline__ long long parts_of(const PagedParams& p, long long total) {
+  const long long most = (total + kMinTiles - 1) / kMinTiles;
+  return most < p.blocks ? most : p.blocks;
+}
+
+struct Cursor {
+  int seq, item, tile, tiles, len;
+};
+__device__ __forceinline__ void seek(const PagedParams& p, long long at, int lane, Cursor& c) {
+  long long before = 0;
+  for (int b0 = 0; b0 < p.batch; b0 += 32) {
+    const int b = b0 + lane;
+    const int t = b < p.batch ? tiles_of(seq_len(p, b)) : 0;
+    int incl = t;
+#pragma unroll
+    for (int s = 1; s < 32; s <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, incl, s);
+      if (lane >= s) incl += y;
+    }
+    const bool here = at < (before + incl) * p.items;
+    const unsigned m = __ballot_sync(0xffffffffu, here);
+    if (m) {
+      const int l = __ffs(m) - 1;
+      c.seq = b0 + l;
+      c.tiles = __shfl_sync(0xffffffffu, t, l);
+      const long long rel = at - (before + __shfl_sync(0xffffffffu, incl - t, l)) * p.items;
+      c.item = (int)(rel / c.tiles);
+      c.tile = (int)(rel % c.tiles);
+      c.len = seq_len(p, c.seq);
+      return;
+    }
+    before += __shfl_sync(0xffffffffu, incl, 31);
+  }
+  c = Cursor{0, 0, 0, 1, 0};  // not reached: at < total * items
+}
+__device__ __forceinline__ void advance(const PagedParams& p, Cursor& c) {
+  if (++c.tile < c.tiles) return;
+  c.tile = 0;
+  if (++c.item < p.items) return;
+  c.item = 0;
+  if (++c.seq < p.batch) {
+    c.len = seq_len(p, c.seq);
+    c.tiles = tiles_of(c.len);
+  }
+}
+
+template <typename T, int DP, int NT>
+__global__ void __launch_bounds__(32 * kWarps, 2) paged_decode_kernel(const __grid_constant__ PagedParams p) {
+  using C = Cfg<DP, NT>;
+  constexpr int CH = DP / 8;  // 16-byte chunks per row
+  constexpr int KS = DP / 16;
+  constexpr int HEADS = 8 * NT;
+  extern __shared__ __align__(128) uint8_t smem[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t ring = smem_u32(smem) + warp * C::STAGES * C::STAGE;
+  float* join = reinterpret_cast<float*>(smem + C::RING);          // [warp][8 heads][LD]
+  float* join_ml = join + kWarps * 8 * C::LD;                       // [warp][8 heads][max, sum]
+
+  asm volatile("griddepcontrol.launch_dependents;");
+  long long first, last;  // flat tiles of this block
+  if (p.whole_items) {    // one block per item (short caches): no cut, no join
+    first = last = 0;
+  } else {
+    const long long total = total_tiles(p, lane) * p.items;
+    const long long parts = parts_of(p, total);
+    if (blockIdx.x >= parts) return;
+    first = total * blockIdx.x / parts;
+    last = total * (blockIdx.x + 1) / parts;
+  }
+  Cursor cc;
+  if (p.whole_items) {
+    cc.seq = blockIdx.x / p.items;
+    cc.item = blockIdx.x % p.items;
+    cc.tile = 0;
+    cc.len = seq_len(p, cc.seq);
+    cc.tiles = tiles_of(cc.len);
+    last = cc.tiles;
+  } else {
+    seek(p, first, lane, cc);
+  }
+  const int n = (int)(last - first);
+
+  // ---- loading: lane l < 16 knows the page and slot of row l of the stage that is issued next
+  Cursor lc = cc;
+  int page = -1, slot = 0;
+  auto look_up = [&](const Cursor& c) {
+    const int t = c.tile * kTile + 16 * warp + (lane & 15);
+    page = -1;
+    if (t < c.len) {
+      const int i = t / p.page_size;
+      slot = t - i * p.page_size;
+      page = p.table[(int64_t)c.seq * p.table_stride + i];
+      if ((unsigned)page >= (unsigned)p.num_pages) page = -1;
+    }
+  };
+  auto issue = [&](int it) {  // stage it % STAGES <- this warp's rows of lc, then on to the next tile
+    if (it < n) {
+      const uint32_t st = ring + (it % C::STAGES) * C::STAGE;
+      const int h = lc.item / p.chunks;
+      const T* kh = static_cast<const T*>(p.k) + (int64_t)h * p.k_head;
+      const T* vh = static_cast<const T*>(p.v) + (int64_t)h * p.v_head;
+      const int chunk = lane % CH;
+#pragma unroll
+      for (int i = 0; i < CH / 2; ++i) {
+        const int r = i * (32 / CH) + lane / CH;
+        const int pg = __shfl_sync(0xffffffffu, page, r), sl = __shfl_sync(0xffffffffu, slot, r);
+        const bool on = pg >= 0 && chunk * 8 < p.dim;
+        const int64_t pg0 = on ? pg : 0, sl0 = on ? sl : 0, c0 = on ? chunk * 8 : 0;
+        const uint32_t dst = st + swz<CH>(r, chunk) * 2;
+        cp_async16(dst, kh + pg0 * p.k_page + sl0 * p.k_slot + c0, on ? 16 : 0);
+        cp_async16(dst + 16 * DP * 2, vh + pg0 * p.v_page + sl0 * p.v_slot + c0, on ? 16 : 0);
+      }
+      advance(p, lc);
+      if (it + 1 < n) look_up(lc);
+    }
+    cp_async_commit();
+  };
+  look_up(lc);
+#pragma unroll
+  for (int s = 0; s < C::STAGES - 1; ++s) issue(s);
+
+  uint32_t qf[NT][KS][2];
+  float acc[NT][KS][4], m[NT][2], l[NT][2];
+  bool fresh = true, from_start = cc.tile == 0;
+  for (int it = 0; it < n; ++it) {
+    if (fresh) {
+      // a new item: its query heads as B fragments (head = lane / 4, columns 2 (lane % 4) ...)
+      fresh = false;
+      const int h = cc.item / p.chunks, g0 = (cc.item % p.chunks) * HEADS;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        const int g = g0 + 8 * nt + lane / 4;
+        const T* q = static_cast<const T*>(p.q) + (int64_t)cc.seq * p.q_row + (int64_t)(h * p.group + g) * p.q_head;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int c = 16 * ks + 8 * e + 2 * (lane % 4);
+            qf[nt][ks][e] = g < p.group && c < p.dim ? *reinterpret_cast<const uint32_t*>(q + c) : 0u;
+          }
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[nt][ks][e] = 0.f;
+        m[nt][0] = m[nt][1] = -1e30f;
+        l[nt][0] = l[nt][1] = 0.f;
+      }
+    }
+    cp_async_wait<C::STAGES - 2>();
+    __syncwarp();
+    const uint32_t ks_base = ring + (it % C::STAGES) * C::STAGE, vs_base = ks_base + 16 * DP * 2;
+    const int left = cc.len - cc.tile * kTile - 16 * warp;  // tokens of this warp's rows
+    if (left > 0) {
+      float s[NT][4];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[nt][e] = 0.f;
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        uint32_t a[4];
+        ldsm_x4(ks_base + swz<CH>(lane & 15, 2 * ks + (lane >> 4)) * 2, a[0], a[1], a[2], a[3]);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) mma16816<T>(s[nt], a, qf[nt][ks][0], qf[nt][ks][1]);
+      }
+      uint32_t pb[NT][2];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        // rows: tokens lane / 4 and + 8; columns: heads 2 (lane % 4) and + 1
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          s[nt][e] *= p.scale_log2;
+          if (lane / 4 + 8 * (e >> 1) >= left) s[nt][e] = -INFINITY;
+        }
+        float mx[2] = {fmaxf(s[nt][0], s[nt][2]), fmaxf(s[nt][1], s[nt][3])};
+#pragma unroll
+        for (int x = 4; x < 32; x <<= 1) {
+          mx[0] = fmaxf(mx[0], __shfl_xor_sync(0xffffffffu, mx[0], x));
+          mx[1] = fmaxf(mx[1], __shfl_xor_sync(0xffffffffu, mx[1], x));
+        }
+        if (__any_sync(0xffffffffu, mx[0] > m[nt][0] || mx[1] > m[nt][1])) {
+          float al[2];
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float mn = fmaxf(m[nt][e], mx[e]);
+            al[e] = fast_exp2(m[nt][e] - mn);
+            m[nt][e] = mn;
+            l[nt][e] *= al[e];
+          }
+#pragma unroll
+          for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[nt][ks][e] *= al[e & 1];
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[nt][e] = fast_exp2(s[nt][e] - m[nt][e & 1]);
+        l[nt][0] += s[nt][0] + s[nt][2];
+        l[nt][1] += s[nt][1] + s[nt][3];
+        pb[nt][0] = movmatrix(Elem<T>::pack(s[nt][0], s[nt][1]));
+        pb[nt][1] = movmatrix(Elem<T>::pack(s[nt][2], s[nt][3]));
+      }
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        // V^T: rows d, columns tokens; matrices (tokens 0-7, 8-15) x (d, d + 8)
+        uint32_t a[4];
+        ldsm_x4_t(vs_base + swz<CH>((lane & 7) + 8 * (lane >> 4), 2 * ks + ((lane >> 3) & 1)) * 2, a[0], a[1], a[2], a[3]);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) mma16816<T>(acc[nt][ks], a, pb[nt][0], pb[nt][1]);
+      }
+    }
+    __syncwarp();  // every lane is done with the stage that the next issue refills
+    issue(it + C::STAGES - 1);
+
+    const bool to_end = cc.tile + 1 == cc.tiles;
+    if (to_end || it + 1 == n) {
+      // ---- the four warps' parts of this item (or of this block's share of it)
+      const int h = cc.item / p.chunks, g0 = (cc.item % p.chunks) * HEADS;
+      const bool whole = from_start && to_end;
+      const int64_t part = (int64_t)blockIdx.x * 2 + (from_start ? 1 : 0);
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+#pragma unroll
+          for (int x = 4; x < 32; x <<= 1) l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], x);
+          if (lane < 4) {
+            join_ml[(warp * 8 + 2 * lane + e) * 2] = m[nt][e];
+            join_ml[(warp * 8 + 2 * lane + e) * 2 + 1] = l[nt][e];
+          }
+        }
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            join[(warp * 8 + 2 * (lane % 4) + (e & 1)) * C::LD + 16 * ks + lane / 4 + 8 * (e >> 1)] = acc[nt][ks][e];
+        __syncthreads();
+        for (int i = threadIdx.x; i < 8 * DP; i += 32 * kWarps) {
+          const int r = i / DP, d = i % DP, g = g0 + 8 * nt + r;
+          if (g >= p.group) continue;
+          float mm = -1e30f, sum = 0.f, o = 0.f;
+#pragma unroll
+          for (int w = 0; w < kWarps; ++w) mm = fmaxf(mm, join_ml[(w * 8 + r) * 2]);
+#pragma unroll
+          for (int w = 0; w < kWarps; ++w) {
+            const float f = fast_exp2(join_ml[(w * 8 + r) * 2] - mm);
+            sum = fmaf(f, join_ml[(w * 8 + r) * 2 + 1], sum);
+            o = fmaf(f, join[(w * 8 + r) * C::LD + d], o);
+          }
+          const int64_t head = h * p.group + g;
+          if (whole) {
+            if (d < p.dim) static_cast<T*>(p.o)[(int64_t)cc.seq * p.o_row + head * p.o_head + d] =
+                Elem<T>::from_f(sum == 0.f ? 0.f : o / sum);
+            if (d == 0 && p.lse) p.lse[(int64_t)cc.seq * p.heads + head] = sum == 0.f ? -INFINITY : (mm + log2f(sum)) * kLn2;
+          } else {
+            p.part[(part * HEADS + 8 * nt + r) * DP + d] = o;
+            if (d == 0) *reinterpret_cast<float2*>(p.part_ml + (part * HEADS + 8 * nt + r) * 2) = make_float2(mm, sum);
+          }
+        }
+        __syncthreads();
+      }
+      fresh = true;
+      from_start = true;
+    }
+    advance(p, cc);
+  }
+  cp_async_wait<0>();
+}
+
+// Joins the parts of one (sequence, query head): 8 groups of 32 lanes over the parts, 4 columns a lane.
+template <typename T, int DP, int NT>
+__global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__ PagedParams p) {
+  constexpr int HEADS = 8 * NT, LANES = DP / 4, GROUPS = 256 / LANES;
+  __shared__ float4 sum_o[GROUPS][LANES];
+  __shared__ float2 sum_ml[GROUPS];
+  const int lane = threadIdx.x & 31;
+  const int seq = blockIdx.x / p.heads, head = blockIdx.x % p.heads;
+  const int h = head / p.group, g = head % p.group;
+  const int item = h * p.chunks + g / HEADS, r = g % HEADS;
+  // where the item lies among the blocks' shares (lengths are inputs: readable before the wait)
+  long long total = 0, before = 0;
+  for (int b = lane; b < p.batch; b += 32) {
+    const int t = tiles_of(seq_len(p, b));
+    total += t;
+    if (b < seq) before += t;
+  }
+#pragma unroll
+  for (int s = 16; s > 0; s >>= 1) {
+    total += __shfl_xor_sync(0xffffffffu, total, s);
+    before += __shfl_xor_sync(0xffffffffu, before, s);
+  }
+  total *= p.items;
+  const int tiles = tiles_of(seq_len(p, seq));
+  const long long parts = parts_of(p, total), t0 = before * p.items + (long long)item * tiles;
+  const int c0 = (int)(((t0 + 1) * parts - 1) / total), c1 = (int)(((t0 + tiles) * parts - 1) / total);
+  // every block waits, those without work too: the stream's next kernel must find the first one done
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (c0 == c1) return;  // finished by its block
+  // block c0 holds the item's start (its second slot), the others continue it (their first)
+  const int grp = threadIdx.x / LANES, d4 = threadIdx.x % LANES;
+  auto at = [&](int c) { return ((int64_t)c * 2 + (c == c0 ? 1 : 0)) * HEADS + r; };
+  float m = -1e30f, l = 0.f;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (int c = c0 + grp; c <= c1; c += GROUPS) {
+    const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + at(c) * 2);
+    const float4 v = reinterpret_cast<const float4*>(p.part + at(c) * DP)[d4];
+    const float mn = fmaxf(m, ml.x), fa = fast_exp2(m - mn), fb = fast_exp2(ml.x - mn);
+    l = l * fa + ml.y * fb;
+    o.x = o.x * fa + v.x * fb;
+    o.y = o.y * fa + v.y * fb;
+    o.z = o.z * fa + v.z * fb;
+    o.w = o.w * fa + v.w * fb;
+    m = mn;
+  }
+  sum_o[grp][d4] = o;
+  if (d4 == 0) sum_ml[grp] = make_float2(m, l);
+  __syncthreads();
+  if (grp) return;
+  for (int i = 0; i < GROUPS; ++i) m = fmaxf(m, sum_ml[i].x);
+  l = 0.f;
+  o = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int i = 0; i < GROUPS; ++i) {
+    const float f = fast_exp2(sum_ml[i].x - m);
+    l += sum_ml[i].y * f;
+    o.x += sum_o[i][d4].x * f;
+    o.y += sum_o[i][d4].y * f;
+    o.z += sum_o[i][d4].z * f;
+    o.w += sum_o[i][d4].w * f;
+  }
+  if (4 * d4 < p.dim) {
+    uint2 w;
+    w.x = Elem<T>::pack(o.x / l, o.y / l);
+    w.y = Elem<T>::pack(o.z / l, o.w / l);
+    *reinterpret_cast<uint2*>(static_cast<T*>(p.o) + (int64_t)seq * p.o_row + (int64_t)head * p.o_head + 4 * d4) = w;
+  }
+  if (d4 == 0 && p.lse) p.lse[(int64_t)seq * p.heads + head] = (m + log2f(l)) * kLn2;
+}
+
+template <typename T, int DP, int NT>
+cudaError_t launch(PagedParams p, cudaStream_t st) {
+  using C = Cfg<DP, NT>;
+  auto kern = paged_decode_kernel<T, DP, NT>;
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+  if (e != cudaSuccess) return e;
+  kern<<<(unsigned)p.blocks, 32 * kWarps, C::SMEM, st>>>(p);
+  e = cudaGetLastError();
+  if (e != cudaSuccess || p.whole_items) return e;
+  // the join starts while the last blocks still run and waits on the device for what they wrote
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)(p.batch * p.heads));
+  cfg.blockDim = dim3(256);
+  cfg.stream = st;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, paged_join_kernel<T, DP, NT>, p);
+}
+
+template <typename T>
+cudaError_t launch_dim(const PagedParams& p, cudaStream_t st) {
+  if (p.dim > 64) return p.nt == 2 ? launch<T, 128, 2>(p, st) : launch<T, 128, 1>(p, st);
+  return p.nt == 2 ? launch<T, 64, 2>(p, st) : launch<T, 64, 1>(p, st);
+}
+
+}  // namespace
+
+void paged_plan(PagedParams& p) {
+  p.group = p.heads / p.kv_heads;
+  p.nt = p.group > 8 ? 2 : 1;  // 8 or 16 query heads share a pass over their keys
+  p.chunks = (p.group + 8 * p.nt - 1) / (8 * p.nt);
+  p.items = p.kv_heads * p.chunks;
+  const int64_t tiles = (p.max_len + kTile - 1) / kTile;  // most that an item can have
+  p.whole_items = tiles <= kMinTiles;
+  const int64_t most = (int64_t)p.batch * p.items * (tiles > 0 ? tiles : 1);
+  p.blocks = p.whole_items ? (int64_t)p.batch * p.items : (most < 2 * 148 ? most : 2 * 148);
+}
+
+int64_t paged_workspace(const PagedParams& p) {
+  if (p.whole_items) return 0;
+  const int64_t rows = p.blocks * 2 * 8 * p.nt;
+  return rows * (p.dim > 64 ? 128 : 64) * 4 + rows * 2 * 4;
+}
+
+cudaError_t paged_decode(PagedParams p, void* workspace, bool bf16, cudaStream_t st) {
+  p.part = static_cast<float*>(workspace);
+  p.part_ml = p.part + p.blocks * 2 * 8 * p.nt * (p.dim > 64 ? 128 : 64);
+  return bf16 ? launch_dim<__nv_bfloat16>(p, st) : launch_dim<__half>(p, st);
+}
+
+}  // namespace vmb

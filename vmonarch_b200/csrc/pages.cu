@@ -1,0 +1,60 @@
+// Moves of a paged key / value cache: new rows into their slots, whole pages to other pages. Both are
+// copies bound by memory: every byte is read once and written once, 16 bytes a thread and tensor,
+// neighbouring threads on neighbouring bytes of a row (a page of one head is contiguous in the usual
+// layout, so the rows of a copy follow one another).
+#include "common.cuh"
+#include "launch.h"
+#include "paged.h"
+
+namespace vmb {
+namespace {
+
+constexpr int kThreads = 256;
+
+__device__ __forceinline__ uint4 load16(const void* base, int64_t elem) {
+  return __ldcs(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(base) + elem));
+}
+__device__ __forceinline__ void store16(void* base, int64_t elem, uint4 v) {
+  *reinterpret_cast<uint4*>(static_cast<uint16_t*>(base) + elem) = v;
+}
+
+// COPY: rows are (pair, head, slot); else (row, head).
+template <bool COPY>
+__global__ void __launch_bounds__(kThreads) page_move_kernel(const __grid_constant__ PageMoveParams p) {
+  const uint32_t ch = p.dim / 8, inner = (uint32_t)(COPY ? p.page_size : 1) * ch, per = (uint32_t)p.kv_heads * inner;
+  const int64_t idx = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+  const int64_t i = idx / per;
+  if (i >= p.count) return;
+  const uint32_t rem = (uint32_t)(idx - i * per), h = rem / inner, in = rem - h * inner, slot = in / ch, c = (in - slot * ch) * 8;
+  if (COPY) {
+    const int s = p.src[i], d = p.dst[i];
+    if ((unsigned)s >= (unsigned)p.num_pages || (unsigned)d >= (unsigned)p.num_pages) return;
+    const int64_t ko = h * p.k_head + slot * p.k_slot + c, vo = h * p.v_head + slot * p.v_slot + c;
+    const uint4 k = load16(p.k, s * p.k_page + ko), v = load16(p.v, s * p.v_page + vo);
+    store16(p.k, d * p.k_page + ko, k);
+    store16(p.v, d * p.v_page + vo, v);
+  } else {
+    const int at = p.dst[i];
+    if (at < 0 || at / p.page_size >= p.num_pages) return;
+    const int64_t page = at / p.page_size, sl = at % p.page_size;
+    const uint4 k = load16(p.k_src, i * p.k_row + h * p.k_shead + c), v = load16(p.v_src, i * p.v_row + h * p.v_shead + c);
+    store16(p.k, page * p.k_page + h * p.k_head + sl * p.k_slot + c, k);
+    store16(p.v, page * p.v_page + h * p.v_head + sl * p.v_slot + c, v);
+  }
+}
+
+template <bool COPY>
+cudaError_t launch(const PageMoveParams& p, cudaStream_t st) {
+  const int64_t n = p.count * p.kv_heads * (COPY ? p.page_size : 1) * (p.dim / 8);
+  const int64_t blocks = (n + kThreads - 1) / kThreads;
+  if (blocks > 0x7fffffff) return cudaErrorInvalidConfiguration;
+  page_move_kernel<COPY><<<(unsigned)blocks, kThreads, 0, st>>>(p);
+  return cudaGetLastError();
+}
+
+}  // namespace
+
+cudaError_t append_pages(const PageMoveParams& p, cudaStream_t st) { return launch<false>(p, st); }
+cudaError_t copy_pages(const PageMoveParams& p, cudaStream_t st) { return launch<true>(p, st); }
+
+}  // namespace vmb
