@@ -382,6 +382,42 @@ int vmb_append_pages(const vmb_rows* k_new, const vmb_rows* v_new, const vmb_pag
 int vmb_copy_pages(const vmb_pages* k, const vmb_pages* v, const int32_t* src, const int32_t* dst, int64_t count,
                    int64_t num_pages, int32_t kv_heads, int32_t dim, int32_t page_size, void* stream);
 
+/*
+ * Gated residual with norms around a block (no reference counterpart), over rows of `cols` elements that
+ * belong to `seqs` sequences one after another (seq_start[s]: first row of sequence s, device int32;
+ * NULL with one sequence):
+ *   y^ = y / sqrt(mean(y^2) + eps) * post_weight   (without post_weight: y)
+ *   x_new = x + gate y^,   h = norm(x_new) weight (1 + scale) + shift
+ * norm: x / sqrt(mean(x^2) + eps), or with `layer` (x - mean) / sqrt(var + eps), of the unrounded x_new.
+ * gate, scale, shift [seqs][cols], weight, post_weight [cols], each NULL for 1, 0, 0, 1 and no norm of
+ * y; dtype is the rows', param_dtype the parameters': the same, or VMB_DTYPE_F32. y NULL: h alone is formed.
+ * cols: a multiple of 8, at most 8192. Parameters and outputs are dense, 16-byte aligned.
+ */
+#define VMB_DTYPE_F32 2
+typedef struct vmb_matrix {  /* [rows][cols], row stride in elements (a multiple of 8) */
+  void* ptr;
+  int64_t row;
+} vmb_matrix;
+
+typedef struct vmb_gated_norm_args {
+  vmb_matrix x, y;                   /* y.ptr NULL: no block output */
+  void *x_new, *h;                   /* forward outputs; x_new unused without y */
+  const void *gate, *scale, *shift, *weight, *post_weight;
+  float* stats;                      /* [3][rows]: written by the forward (NULL: not), read by the backward */
+  const int32_t* seq_start;
+  vmb_matrix dx_new, dh;             /* backward: gradients in, ptr NULL for zero */
+  void *dx, *dy;                     /* backward outputs; dy unused without y */
+  void *dgate, *dscale, *dshift, *dweight, *dpost_weight;  /* of param_dtype, each NULL if not wanted */
+  int64_t rows;
+  int32_t cols, seqs, dtype, param_dtype, layer;
+  float eps;
+  void* workspace; int64_t workspace_bytes;  /* backward, 256-byte aligned */
+} vmb_gated_norm_args;
+
+int64_t vmb_gated_norm_bwd_workspace_bytes(const vmb_gated_norm_args* a);  /* -1: malformed sizes */
+int vmb_gated_norm_fwd(const vmb_gated_norm_args* a, void* stream);
+int vmb_gated_norm_bwd(const vmb_gated_norm_args* a, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,7 +1,7 @@
 """Attention over packed sequences against its definition in 64 bits.
 
-Errors are relative in the Frobenius norm, in units u of the element type's rounding (2^-9 bf16,
-2^-12 ... 2^-11 fp16). Forward: P rounded (u) and the output rounded (u): at most 2 u. Gradients: dS
+Errors are relative in the Frobenius norm, in units u of 2^-9 for bf16 (half of a rounding's
+bound, above its root mean square) and 2^-11 for fp16. Forward: P rounded (u) and the output rounded (u): at most 2 u. Gradients: dS
 or P rounded (u), the rounded o inside D = sum o dO (u, relative to |o| |dO|, which cancellation in
 dP - D can double), the output rounded (u): at most 4 u. Where a reference is zero the result must be.
 """

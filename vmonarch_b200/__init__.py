@@ -1,9 +1,11 @@
 """B200-native (sm_100a) VMonarch attention: a drop-in for ``video_monarch_attention``.
 
 Exports the reference's three names (reference ``video_monarch_attention/__init__.py:1-4``) and, beside
-them, attention over packed sequences of different lengths and over a paged key / value cache.
+them, attention over packed sequences of different lengths and over a paged key / value
+cache, and the gated residual norm between a transformer's blocks.
 Importing loads the in-tree CUDA library through its C ABI and raises if it is missing.
 """
+from .gated_norm import gated_residual_norm  # noqa: F401
 from .kernel import flash_entropy_attention
 from .packed import PackedSequences, packed_attention  # noqa: F401
 from .paged import PagedKVCache, append_pages, copy_pages, paged_attention  # noqa: F401

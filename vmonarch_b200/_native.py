@@ -16,6 +16,7 @@ LIB_PATH = Path(os.environ.get("VMONARCH_B200_LIB", Path(__file__).resolve().par
 
 VMB_DTYPE_BF16 = 0
 VMB_DTYPE_F16 = 1
+VMB_DTYPE_F32 = 2  # parameters of vmb_gated_norm only
 VMB_OK = 0
 _ERRNAMES = {1: "EINVAL", 2: "ENOTSUP", 3: "ECUDA"}
 
@@ -141,6 +142,25 @@ class PagedArgs(ctypes.Structure):
     ]
 
 
+class Matrix(ctypes.Structure):
+    """vmb_matrix: a (rows, cols) tensor with contiguous columns."""
+    _fields_ = [("ptr", c_vp), ("row", c_i64)]
+
+
+class GatedNormArgs(ctypes.Structure):
+    _fields_ = [
+        ("x", Matrix), ("y", Matrix), ("x_new", c_vp), ("h", c_vp),
+        ("gate", c_vp), ("scale", c_vp), ("shift", c_vp), ("weight", c_vp), ("post_weight", c_vp),
+        ("stats", c_vp), ("seq_start", c_vp),
+        ("dx_new", Matrix), ("dh", Matrix), ("dx", c_vp), ("dy", c_vp),
+        ("dgate", c_vp), ("dscale", c_vp), ("dshift", c_vp), ("dweight", c_vp), ("dpost_weight", c_vp),
+        ("rows", c_i64),
+        ("cols", c_i32), ("seqs", c_i32), ("dtype", c_i32), ("param_dtype", c_i32), ("layer", c_i32),
+        ("eps", ctypes.c_float),
+        ("workspace", c_vp), ("workspace_bytes", c_i64),
+    ]
+
+
 #: every symbol include/vmonarch_b200.h declares, with its ctypes signature
 SIGNATURES = {
     "vmb_abi_version": (ctypes.c_int, []),
@@ -165,6 +185,9 @@ SIGNATURES = {
     "vmb_packed_bwd_workspace_bytes": (c_i64, [ctypes.POINTER(PackedArgs)]),
     "vmb_packed_fwd": (ctypes.c_int, [ctypes.POINTER(PackedArgs), c_vp]),
     "vmb_packed_bwd": (ctypes.c_int, [ctypes.POINTER(PackedArgs), c_vp]),
+    "vmb_gated_norm_bwd_workspace_bytes": (c_i64, [ctypes.POINTER(GatedNormArgs)]),
+    "vmb_gated_norm_fwd": (ctypes.c_int, [ctypes.POINTER(GatedNormArgs), c_vp]),
+    "vmb_gated_norm_bwd": (ctypes.c_int, [ctypes.POINTER(GatedNormArgs), c_vp]),
     "vmb_paged_workspace_bytes": (c_i64, [ctypes.POINTER(PagedArgs)]),
     "vmb_paged_attention": (ctypes.c_int, [ctypes.POINTER(PagedArgs), c_vp]),
     "vmb_append_pages": (ctypes.c_int, [ctypes.POINTER(Rows), ctypes.POINTER(Rows), ctypes.POINTER(Pages),

@@ -75,6 +75,13 @@ class PackedSequences:
     def __repr__(self):
         return f"PackedSequences({self.num_sequences} sequences, {self.total_q} queries, {self.total_k} keys)"
 
+    def _starts(self):
+        """First query row of every sequence, int32 on the device."""
+        hit = self._cache.get("starts")
+        if hit is None:
+            hit = self._cache["starts"] = torch.from_numpy(self.q_start.astype(np.int32)).to(self.device)
+        return hit
+
     # ------------------------------------------------------------------------------ work lists
     def _query_units(self, rows, causal):
         """Units of `rows` queries for the forward and dQ kernels, and their key tiles."""
