@@ -246,4 +246,8 @@ def device_status(device: torch.device) -> int:
 
 
 def stream_ptr(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+    return raw_stream(device.index if device.index is not None else torch.cuda.current_device())
+
+
+#: handle of a device's current stream, by device index (torch.cuda.current_stream builds a Stream object around it)
+raw_stream = torch._C._cuda_getCurrentRawStream

@@ -31,6 +31,7 @@ namespace vmb {
 namespace {
 
 constexpr int kMaxWarps = 32;
+constexpr int kSmemLimit = 220 * 1024;  // dynamic shared memory of an SM's blocks together
 
 template <typename T, typename P>
 struct Io;  // 8 elements of a parameter as floats
@@ -535,8 +536,8 @@ Shape shape_of(int cols, int64_t rows, int nparam, int nin, int r, int regs_cap_
   const int stage = s.threads * 16 * nin * r, par = nparam * cols * 4;
   // blocks per SM that registers allow (regs_cap_threads threads resident), each with its part of shared memory
   int per_sm = std::max(1, regs_cap_threads / s.threads);
-  while (per_sm > 1 && par + 2 * stage > 220 * 1024 / per_sm) --per_sm;
-  s.stages = std::max(2, std::min(4, (220 * 1024 / per_sm - par) / stage));
+  while (per_sm > 1 && par + 2 * stage > kSmemLimit / per_sm) --per_sm;
+  s.stages = std::max(2, std::min(4, (kSmemLimit / per_sm - par) / stage));
   // the groups' column sums pass through three rows of the shared memory
   s.smem = std::max(par + s.stages * stage, groups > 1 ? 3 * cols * 4 : 0);
   s.blocks = (int)std::min<int64_t>((rows + groups * r - 1) / (groups * r), (int64_t)148 * per_sm);
@@ -548,8 +549,8 @@ Shape backward_shape(const GatedNormParams& p) {
 }
 
 template <typename Kern>
-cudaError_t run(Kern kern, const Shape& s, const GatedNormParams& p, cudaStream_t st) {
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, s.smem);
+cudaError_t run(Kern kern, std::atomic<uint64_t>& ready, const Shape& s, const GatedNormParams& p, cudaStream_t st) {
+  cudaError_t e = allow_smem(kern, kSmemLimit, ready);
   if (e != cudaSuccess) return e;
   kern<<<s.blocks, s.threads, s.smem, st>>>(p);
   return cudaGetLastError();
@@ -561,7 +562,8 @@ cudaError_t forward(GatedNormParams p, cudaStream_t st) {
   const Shape s = shape_of(p.cols, p.rows, 3, HAS_Y ? 2 : 1, R, MAXT > 640 ? 1024 : 768);
   p.tpr = s.tpr;
   p.stages = s.stages;
-  return run(gated_norm_fwd_kernel<T, P, HAS_Y, R, MAXT>, s, p, st);
+  static std::atomic<uint64_t> ready{0};
+  return run(gated_norm_fwd_kernel<T, P, HAS_Y, R, MAXT>, ready, s, p, st);
 }
 
 template <typename T, typename P, bool HAS_Y, int MAXT>
@@ -570,7 +572,8 @@ cudaError_t backward(GatedNormParams p, cudaStream_t st) {
   p.tpr = s.tpr;
   p.stages = s.stages;
   if (p.rows > 0) {
-    cudaError_t e = run(gated_norm_bwd_kernel<T, P, HAS_Y, 1, MAXT>, s, p, st);
+    static std::atomic<uint64_t> ready{0};
+    cudaError_t e = run(gated_norm_bwd_kernel<T, P, HAS_Y, 1, MAXT>, ready, s, p, st);
     if (e != cudaSuccess) return e;
   }
   if (!p.part) return cudaSuccess;

@@ -2,6 +2,7 @@
 #pragma once
 #include <cuda_runtime.h>
 #include <stdint.h>
+#include <atomic>
 #include "fea_params.h"
 
 struct vmb_fea_bwd_args;
@@ -86,6 +87,19 @@ cudaError_t packed_status(cudaStream_t st, int* out);
 // dq: the 128-query units (statistics and dQ), kv: the 128-key units (dK, dV); the rest of the two is alike
 cudaError_t packed_bwd(const PackedParams& dq, const PackedParams& kv, bool bf16, cudaStream_t st);
 cudaError_t packed_bwd_status(cudaStream_t st, int* out);
+
+// Raises a kernel's dynamic shared memory limit, once per device (`done`: a bit each, static beside the launch).
+template <typename Kern>
+cudaError_t allow_smem(Kern kern, int bytes, std::atomic<uint64_t>& done) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const uint64_t bit = uint64_t(1) << (dev & 63);
+  if (dev < 64 && (done.load(std::memory_order_relaxed) & bit)) return cudaSuccess;
+  e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess && dev < 64) done.fetch_or(bit, std::memory_order_relaxed);
+  return e;
+}
 
 // Adds n to the library's kernel launch count.
 void count_launches(int n);

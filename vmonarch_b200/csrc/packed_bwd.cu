@@ -588,8 +588,8 @@ __global__ void __launch_bounds__(kThreads, 1) packed_dq_kernel(const __grid_con
 }
 
 template <typename Kern>
-cudaError_t run(Kern kern, int smem, int64_t blocks, const KParams& p, cudaStream_t st) {
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+cudaError_t run(Kern kern, int smem, std::atomic<uint64_t>& ready, int64_t blocks, const KParams& p, cudaStream_t st) {
+  cudaError_t e = allow_smem(kern, smem, ready);
   if (e != cudaSuccess) return e;
   if (blocks > 0x7fffffff) return cudaErrorInvalidConfiguration;
   kern<<<(unsigned)blocks, kThreads, smem, st>>>(p);
@@ -606,6 +606,7 @@ cudaError_t launch(const PackedParams& dq, const PackedParams& kv, cudaStream_t 
     cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return e;
   }
+  static std::atomic<uint64_t> ready_kv{0}, ready_q{0};
   KParams p{};
   p.scale_log2 = dq.sm_scale * kLog2e;
   auto map = [&](CUtensorMap* m, const void* base, int64_t rows, int heads, const View& v, int box) {
@@ -617,14 +618,14 @@ cudaError_t launch(const PackedParams& dq, const PackedParams& kv, cudaStream_t 
     if (!map(&p.tm_q, kv.q, kv.q_total, kv.heads, kv.qv, 64) || !map(&p.tm_do, kv.dout, kv.q_total, kv.heads, kv.dov, 64))
       return cudaErrorInvalidValue;
     p.a = kv;
-    cudaError_t e = run(packed_dkdv_kernel<T, NA>, DkdvCfg<NA>::SMEM, (int64_t)kv.n_units * kv.kv_heads, p, st);
+    cudaError_t e = run(packed_dkdv_kernel<T, NA>, DkdvCfg<NA>::SMEM, ready_kv, (int64_t)kv.n_units * kv.kv_heads, p, st);
     if (e != cudaSuccess) return e;
   }
   if (dq.n_units > 0) {
     if (!map(&p.tm_q, dq.q, dq.q_total, dq.heads, dq.qv, 128) || !map(&p.tm_do, dq.dout, dq.q_total, dq.heads, dq.dov, 128))
       return cudaErrorInvalidValue;
     p.a = dq;
-    return run(packed_dq_kernel<T, NA>, DqCfg<NA>::SMEM, (int64_t)dq.n_units * dq.heads, p, st);
+    return run(packed_dq_kernel<T, NA>, DqCfg<NA>::SMEM, ready_q, (int64_t)dq.n_units * dq.heads, p, st);
   }
   return cudaSuccess;
 }

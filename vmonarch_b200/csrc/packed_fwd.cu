@@ -505,7 +505,8 @@ __global__ void __launch_bounds__(kThreads, 1) packed_fwd_kernel(const __grid_co
 template <typename T, int NA>
 cudaError_t launch(const KParams& p, cudaStream_t st) {
   auto kern = packed_fwd_kernel<T, NA>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<NA>::SMEM);
+  static std::atomic<uint64_t> ready{0};
+  cudaError_t e = allow_smem(kern, Cfg<NA>::SMEM, ready);
   if (e != cudaSuccess) return e;
   const int64_t blocks = (int64_t)p.a.n_units * p.a.heads;
   if (blocks > 0x7fffffff) return cudaErrorInvalidConfiguration;

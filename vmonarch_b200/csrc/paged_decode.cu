@@ -402,7 +402,8 @@ template <typename T, int DP, int NT>
 cudaError_t launch(PagedParams p, cudaStream_t st) {
   using C = Cfg<DP, NT>;
   auto kern = paged_decode_kernel<T, DP, NT>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+  static std::atomic<uint64_t> ready{0};
+  cudaError_t e = allow_smem(kern, C::SMEM, ready);
   if (e != cudaSuccess) return e;
   kern<<<(unsigned)p.blocks, 32 * kWarps, C::SMEM, st>>>(p);
   e = cudaGetLastError();

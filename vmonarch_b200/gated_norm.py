@@ -4,6 +4,7 @@ counterpart): a norm after the block, its gate, the residual, and the modulated 
 from __future__ import annotations
 
 import ctypes
+import struct
 
 import torch
 
@@ -14,60 +15,67 @@ from .kernel import SUPPORTED_DTYPES
 MAX_WIDTH = 8192
 
 
-def _rows_in_place(t):
-    """`t` (T, C) when the kernels can address it: contiguous columns, 16-byte aligned rows."""
-    if t.stride(1) == 1 and t.data_ptr() % 16 == 0 and (t.size(0) <= 1 or t.stride(0) >= 0 and t.stride(0) % 8 == 0):
-        return t
-    return t.contiguous()
+def _place(t):
+    """`t` (T, C), or a dense copy where the kernels cannot address it in place (contiguous columns, 16-byte
+    aligned rows), and its vmb_matrix."""
+    ptr, (row, col) = t.data_ptr(), t.stride()
+    n, c = t.shape
+    if n <= 1:
+        row = c
+    if col != 1 or row < 0 or row & 7 or ptr & 15:
+        t = _dense(t.contiguous())
+        ptr, row = t.data_ptr(), c
+    return t, ptr, row
 
 
 def _dense(t):
-    return t if t is None or (t.is_contiguous() and t.data_ptr() % 16 == 0) else t.clone(memory_format=torch.contiguous_format)
-
-
-def _matrix(t):
-    return N.Matrix(t.data_ptr(), t.stride(0) if t.size(0) > 1 else t.size(1))
-
-
-def _args(x, y, params, seqs, norm, eps):
-    a = N.GatedNormArgs()
-    a.x = _matrix(x)
-    if y is not None:
-        a.y = _matrix(y)
-    a.param_dtype = a.dtype = N.dtype_code(x.dtype)
-    for name, t in zip(_PARAMS, params):
-        if t is not None:
-            setattr(a, name, t.data_ptr())
-            a.param_dtype = N.VMB_DTYPE_F32 if t.dtype == torch.float32 else a.dtype
-    a.rows, a.cols, a.seqs = x.size(0), x.size(1), seqs.num_sequences if seqs is not None else 1
-    if a.seqs > 1:
-        a.seq_start = seqs._starts().data_ptr()
-    a.layer, a.eps = norm == "layer", eps
-    return a
+    return t if t.is_contiguous() and not t.data_ptr() & 15 else t.clone(memory_format=torch.contiguous_format)
 
 
 _PARAMS = ("gate", "scale", "shift", "weight", "post_weight")
+# vmb_gated_norm_args up to its workspace: x, y, x_new, h, five parameters, stats, seq_start | dx_new, dh, dx, dy,
+# five gradients | sizes
+_ARGS = struct.Struct("25q5if")
+assert _ARGS.size == N.GatedNormArgs.workspace.offset
+_NO_GRADS = (0,) * 11
 
 
-def _forward(x, y, params, seqs, norm, eps, want_stats):
-    x, y = _rows_in_place(x), y if y is None else _rows_in_place(y)
-    params = [_dense(t) for t in params]
-    x_new = torch.empty(x.shape, dtype=x.dtype, device=x.device) if y is not None else None
-    h = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    stats = torch.empty((3, x.size(0)), dtype=torch.float32, device=x.device) if want_stats else None
-    a = _args(x, y, params, seqs, norm, eps)
-    a.x_new, a.h = N.ptr(x_new), h.data_ptr()
-    a.stats = N.ptr(stats)
-    N.check(N.lib.vmb_gated_norm_fwd(ctypes.byref(a), N.stream_ptr(x.device)), "vmb_gated_norm_fwd")
-    return x, y, params, x_new, h, stats
+def _sizes(x, params, seqs, norm, eps):
+    dtype = N.dtype_code(x.dtype)
+    fp32 = any(t is not None and t.dtype == torch.float32 for t in params)
+    rows, cols = x.shape
+    return rows, cols, 1 if seqs is None else seqs.num_sequences, dtype, N.VMB_DTYPE_F32 if fp32 else dtype, norm == "layer", eps
+
+
+def _starts(seqs):
+    return seqs._starts().data_ptr() if seqs is not None and seqs.num_sequences > 1 else 0
+
+
+def _forward(x, y, params, seqs, norm, eps, stats):
+    x, *xr = _place(x)
+    yr = (0, 0)
+    if y is not None:
+        y, *yr = _place(y)
+    params = [t if t is None else _dense(t) for t in params]
+    x_new = torch.empty_like(x, memory_format=torch.contiguous_format) if y is not None else None
+    h = torch.empty_like(x, memory_format=torch.contiguous_format)
+    a = N.GatedNormArgs()
+    _ARGS.pack_into(a, 0, *xr, *yr, 0 if x_new is None else x_new.data_ptr(), h.data_ptr(),
+                    *[0 if t is None else t.data_ptr() for t in params], 0 if stats is None else stats.data_ptr(),
+                    _starts(seqs), *_NO_GRADS, *_sizes(x, params, seqs, norm, eps))
+    rc = N.lib.vmb_gated_norm_fwd(ctypes.byref(a), N.raw_stream(x.device.index))
+    if rc:
+        N.check(rc, "vmb_gated_norm_fwd")
+    return x, y, params, x_new, h
 
 
 class _GatedNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, y, seqs, norm, eps, *params):
         shapes = [None if t is None else t.shape for t in params]
-        xs, ys, dense, x_new, h, stats = _forward(x, y, params, seqs, norm, eps, True)
-        ctx.save_for_backward(xs, ys, stats, *dense)
+        stats = torch.empty((3, x.size(0)), dtype=torch.float32, device=x.device)
+        x, y_in, dense, x_new, h = _forward(x, y, params, seqs, norm, eps, stats)
+        ctx.save_for_backward(x, y_in, stats, *dense)
         ctx.meta = seqs, norm, eps, shapes
         ctx.set_materialize_grads(False)
         return (h,) if y is None else (x_new, h)
@@ -78,26 +86,28 @@ class _GatedNorm(torch.autograd.Function):
         x, y, stats, *params = ctx.saved_tensors
         seqs, norm, eps, shapes = ctx.meta
         dx_new, dh = grads if y is not None else (None, *grads)
-        a = _args(x, y, params, seqs, norm, eps)
-        dx_new, dh = (None if t is None else _rows_in_place(t) for t in (dx_new, dh))
+        dxr = dhr = yr = (0, 0)
         if dx_new is not None:
-            a.dx_new = _matrix(dx_new)
+            dx_new, *dxr = _place(dx_new)
         if dh is not None:
-            a.dh = _matrix(dh)
-        a.stats = stats.data_ptr()
-        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        dy = torch.empty(x.shape, dtype=x.dtype, device=x.device) if y is not None else None
-        a.dx, a.dy = dx.data_ptr(), N.ptr(dy)
-        out = []
-        for name, t, need, shape in zip(_PARAMS, params, ctx.needs_input_grad[5:], shapes):
-            g = torch.empty(shape, dtype=t.dtype, device=x.device) if t is not None and need else None
-            setattr(a, "d" + name, N.ptr(g))
-            out.append(g)
-        nbytes = N.lib.vmb_gated_norm_bwd_workspace_bytes(ctypes.byref(a))
-        if nbytes > 0:
-            ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
-            a.workspace, a.workspace_bytes = ws.data_ptr(), nbytes
-        N.check(N.lib.vmb_gated_norm_bwd(ctypes.byref(a), N.stream_ptr(x.device)), "vmb_gated_norm_bwd")
+            dh, *dhr = _place(dh)
+        if y is not None:
+            yr = _place(y)[1:]
+        dx = torch.empty_like(x, memory_format=torch.contiguous_format)
+        dy = torch.empty_like(x, memory_format=torch.contiguous_format) if y is not None else None
+        out = [torch.empty(shape, dtype=t.dtype, device=x.device) if t is not None and need else None
+               for t, need, shape in zip(params, ctx.needs_input_grad[5:], shapes)]
+        a = N.GatedNormArgs()
+        _ARGS.pack_into(a, 0, *_place(x)[1:], *yr, 0, 0, *[0 if t is None else t.data_ptr() for t in params],
+                        stats.data_ptr(), _starts(seqs), *dxr, *dhr, dx.data_ptr(), 0 if dy is None else dy.data_ptr(),
+                        *[0 if t is None else t.data_ptr() for t in out], *_sizes(x, params, seqs, norm, eps))
+        size = N.lib.vmb_gated_norm_bwd_workspace_bytes(ctypes.byref(a))
+        if size > 0:
+            ws = torch.empty(size, dtype=torch.uint8, device=x.device)
+            a.workspace, a.workspace_bytes = ws.data_ptr(), size
+        rc = N.lib.vmb_gated_norm_bwd(ctypes.byref(a), N.raw_stream(x.device.index))
+        if rc:
+            N.check(rc, "vmb_gated_norm_bwd")
         return (dx, dy, None, None, None, *out)
 
 
@@ -152,5 +162,5 @@ def gated_residual_norm(x, y=None, *, gate=None, scale=None, shift=None, weight=
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, y, *params)):
         out = _GatedNorm.apply(x, y, seqs, norm, eps, *params)
         return (x, out[0]) if y is None else out
-    _, _, _, x_new, h, _ = _forward(x, y, params, seqs, norm, eps, False)
+    x_new, h = _forward(x, y, params, seqs, norm, eps, None)[3:]
     return (x if y is None else x_new), h

@@ -8,6 +8,7 @@ a :class:`PackedSequences`, which every layer of a step then shares.
 from __future__ import annotations
 
 import ctypes
+import struct
 
 import numpy as np
 import torch
@@ -124,70 +125,115 @@ class PackedSequences:
             hit = self._cache[key] = (N.PackedList(dev.data_ptr(), None, len(u), 0, 0, 0), dev)
         return hit[0]
 
-
-def _in_place(t):
-    """`t` when the kernels can address it: contiguous columns, 16-byte aligned rows and heads."""
-    if t.stride(2) == 1 or t.size(2) == 1:
-        if t.data_ptr() % 16 == 0 and all(
-                n <= 1 or (s > 0 and s % 8 == 0) for n, s in zip(t.shape[:2], t.stride()[:2])):
-            return t
-    return t.contiguous()
-
-
-def _rows(t):
-    return N.Rows(t.data_ptr(), t.stride(0) if t.size(0) > 1 else t.size(1) * t.size(2),
-                  t.stride(1) if t.size(1) > 1 else t.size(2))
-
-
-def _args(q, k, v, o, o_low, lse, seqs, causal, sm_scale):
-    a = N.PackedArgs()
-    a.q, a.k, a.v, a.o = _rows(q), _rows(k), _rows(v), _rows(o)
-    a.lse = lse.data_ptr() if lse is not None else None
-    if o_low is not None:
-        a.o_low = _rows(o_low)
-    a.q_total, a.k_total, a.stat_rows = seqs.total_q, seqs.total_k, seqs.stat_rows
-    a.heads, a.kv_heads, a.dim = q.size(1), k.size(1), q.size(2)
-    a.dtype, a.causal, a.sm_scale = N.dtype_code(q.dtype), causal, sm_scale
-    return a
+    def _template(self, key):
+        """vmb_packed_args of a kind of call, everything but the tensors, and its workspace size."""
+        hit = self._cache.get(key)
+        if hit is None:
+            backward, causal, sm_scale, dtype, heads, kv_heads, dim = key
+            a = N.PackedArgs()
+            a.q_total, a.k_total, a.stat_rows = self.total_q, self.total_k, self.stat_rows
+            a.heads, a.kv_heads, a.dim = heads, kv_heads, dim
+            a.dtype, a.causal, a.sm_scale = N.dtype_code(dtype), causal, sm_scale
+            if backward:
+                a.q_units = self._list("dq", causal, heads, heads // kv_heads)
+                a.kv_units = self._list("kv", causal, heads, heads // kv_heads)
+                size = N.lib.vmb_packed_bwd_workspace_bytes(ctypes.byref(a))
+            else:
+                a.units = self._list("fwd", causal, heads, heads // kv_heads)
+                size = N.lib.vmb_packed_fwd_workspace_bytes(ctypes.byref(a))
+            hit = self._cache[key] = bytes(a), size
+        return hit
 
 
-def _forward(q, k, v, seqs, causal, sm_scale, want_lse, want_low=False):
-    q, k, v = _in_place(q), _in_place(k), _in_place(v)
-    o = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    o_low = torch.empty_like(o) if want_low else None
-    lse = torch.empty((q.size(1), q.size(0)), dtype=torch.float32, device=q.device) if want_lse else None
-    if o.numel():
-        a = _args(q, k, v, o, o_low, lse, seqs, causal, sm_scale)
-        a.units = seqs._list("fwd", causal, q.size(1), q.size(1) // k.size(1))
-        N.check(N.lib.vmb_packed_fwd(ctypes.byref(a), N.stream_ptr(q.device)), "vmb_packed_fwd")
-    return q, k, v, o, o_low, lse
+# vmb_packed_args begins with the vmb_rows of q, k, v, o, dout, dq, dk, dv, o_low and lse
+_FWD_TENSORS = struct.Struct("12q")
+_REST = struct.Struct("16q")
+_REST_AT = _FWD_TENSORS.size
+_WORKSPACE = struct.Struct("2q")
+_WORKSPACE_AT = N.PackedArgs.workspace.offset
+
+
+def _place(t):
+    """`t` (rows, heads, dim), or a dense copy where the kernels cannot address it in place (contiguous
+    columns, 16-byte aligned rows and heads), and its vmb_rows."""
+    ptr, (row, head, col) = t.data_ptr(), t.stride()
+    if col == 1 and row > 0 and head > 0 and not (row | head) & 7 and not ptr & 15:
+        return t, ptr, row, head
+    n, h, d = t.shape
+    row, head = row if n > 1 else h * d, head if h > 1 else d  # strides of single rows and heads do not count
+    if not (col == 1 or d == 1) or row <= 0 or head <= 0 or (row | head) & 7 or ptr & 15:
+        t = t.contiguous()
+        if t.data_ptr() & 15:
+            t = t.clone(memory_format=torch.contiguous_format)
+        ptr, row, head = t.data_ptr(), h * d, d
+    return t, ptr, row, head
+
+
+def _forward(q, k, v, seqs, key, device, lse=None, aux=None):
+    """Runs the forward into a new o. `aux`: the bytes kept for a backward, o_low and then (unless `lse` is
+    given) the statistics."""
+    q, *qr = _place(q)
+    k, *kr = _place(k)
+    v, *vr = _place(v)
+    o = torch.empty_like(q, memory_format=torch.contiguous_format)
+    template, size = seqs._template(key)
+    a = N.PackedArgs.from_buffer_copy(template)
+    heads, dim = key[4], key[6]
+    row = heads * dim
+    _FWD_TENSORS.pack_into(a, 0, *qr, *kr, *vr, o.data_ptr(), row, dim)
+    if aux is not None or lse is not None:
+        low = aux.data_ptr() if aux is not None else 0
+        stat = lse.data_ptr() if lse is not None else low + 2 * seqs.total_q * row
+        _REST.pack_into(a, _REST_AT, *_NO_ROWS, low, row, dim, stat)
+    if size:
+        ws = torch.empty(size, dtype=torch.uint8, device=device)
+        _WORKSPACE.pack_into(a, _WORKSPACE_AT, ws.data_ptr(), size)
+    rc = N.lib.vmb_packed_fwd(ctypes.byref(a), N.raw_stream(device.index))
+    if rc:
+        N.check(rc, "vmb_packed_fwd")
+    return q, k, v, o
+
+
+_NO_ROWS = (0,) * 12  # dout, dq, dk, dv of a forward
 
 
 class _PackedAttention(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, seqs, causal, sm_scale):
-        q, k, v, o, o_low, lse = _forward(q, k, v, seqs, causal, sm_scale, True, True)
-        ctx.save_for_backward(q, k, v, o, o_low, lse)
-        ctx.meta = seqs, causal, sm_scale
+    def forward(ctx, q, k, v, seqs, key, return_lse):
+        device, rows, heads, dim = q.device, seqs.total_q, key[4], key[6]
+        lse = torch.empty((heads, rows), dtype=torch.float32, device=device) if return_lse else None
+        # o_low (16-bit) and the statistics behind it, in one buffer
+        aux = torch.empty(rows * heads * (2 * dim + (0 if return_lse else 4)), dtype=torch.uint8, device=device)
+        q, k, v, o = _forward(q, k, v, seqs, key, device, lse, aux)
+        ctx.save_for_backward(q, k, v, o, aux, *([lse] if return_lse else []))
+        ctx.meta = seqs, key
+        if not return_lse:
+            return o
         ctx.mark_non_differentiable(lse)
         return o, lse
 
     @staticmethod
     @torch.autograd.function.once_differentiable
-    def backward(ctx, do, _):
-        q, k, v, o, o_low, lse = ctx.saved_tensors
-        seqs, causal, sm_scale = ctx.meta
-        do = _in_place(do)
-        dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
-        a = _args(q, k, v, o, o_low, lse, seqs, causal, sm_scale)
-        a.dout, a.dq, a.dk, a.dv = _rows(do), _rows(dq), _rows(dk), _rows(dv)
-        heads, group = q.size(1), q.size(1) // k.size(1)
-        a.q_units = seqs._list("dq", causal, heads, group)
-        a.kv_units = seqs._list("kv", causal, heads, group)
-        nbytes = N.lib.vmb_packed_bwd_workspace_bytes(ctypes.byref(a))
-        ws = torch.empty(max(nbytes, 1), dtype=torch.uint8, device=q.device)
-        a.workspace, a.workspace_bytes = ws.data_ptr(), nbytes
-        N.check(N.lib.vmb_packed_bwd(ctypes.byref(a), N.stream_ptr(q.device)), "vmb_packed_bwd")
+    def backward(ctx, do, _=None):
+        q, k, v, o, aux, *lse = ctx.saved_tensors
+        seqs, key = ctx.meta
+        heads, kv_heads, dim = key[4:]
+        row, kv_row, device = heads * dim, kv_heads * dim, q.device
+        do, *dor = _place(do)
+        dq, dk, dv = (torch.empty_like(t, memory_format=torch.contiguous_format) for t in (q, k, v))
+        template, size = seqs._template((True, *key[1:]))
+        a = N.PackedArgs.from_buffer_copy(template)
+        _FWD_TENSORS.pack_into(a, 0, *_place(q)[1:], *_place(k)[1:], *_place(v)[1:], o.data_ptr(), row, dim)
+        low = aux.data_ptr()
+        stat = lse[0].data_ptr() if lse else low + 2 * seqs.total_q * row
+        _REST.pack_into(a, _REST_AT, *dor, dq.data_ptr(), row, dim, dk.data_ptr(), kv_row, dim, dv.data_ptr(), kv_row, dim,
+                        low, row, dim, stat)
+        if size:
+            ws = torch.empty(size, dtype=torch.uint8, device=device)
+            _WORKSPACE.pack_into(a, _WORKSPACE_AT, ws.data_ptr(), size)
+        rc = N.lib.vmb_packed_bwd(ctypes.byref(a), N.raw_stream(device.index))
+        if rc:
+            N.check(rc, "vmb_packed_bwd")
         return dq, dk, dv, None, None, None
 
 
@@ -212,22 +258,25 @@ def packed_attention(q, k, v, seqs, *, causal=False, sm_scale=None, return_lse=F
     sequences' rows, while within a sequence a value that is not finite reaches the gradients of its
     whole 64- or 128-row tile.
     """
-    assert q.dtype in SUPPORTED_DTYPES, f"unsupported dtype {q.dtype}"
-    assert k.dtype == q.dtype and v.dtype == q.dtype, "q, k and v must share a dtype"
+    dtype = q.dtype
+    assert dtype in SUPPORTED_DTYPES, f"unsupported dtype {dtype}"
+    assert k.dtype == dtype and v.dtype == dtype, "q, k and v must share a dtype"
     assert q.dim() == 3 and k.dim() == 3 and v.shape == k.shape and q.size(2) == k.size(2), \
         "q must be (total_q, H, D), k and v (total_k, Hk, D)"
-    d = q.size(2)
+    rows, heads, d = q.shape
+    kv_rows, kv_heads, _ = k.shape
     assert 8 <= d <= MAX_DIM and d % 8 == 0, f"head dim {d} is not a multiple of 8 up to {MAX_DIM}"
-    assert k.size(1) >= 1 and q.size(1) >= 1 and q.size(1) % k.size(1) == 0, "H must be a multiple of Hk"
-    assert q.is_cuda and k.device == q.device and v.device == q.device and seqs.device == q.device, \
+    assert kv_heads >= 1 and heads >= 1 and heads % kv_heads == 0, "H must be a multiple of Hk"
+    device = q.device
+    assert q.is_cuda and k.device == device and v.device == device and seqs.device == device, \
         "q, k, v and seqs must be on one CUDA device"
-    assert q.size(0) == seqs.total_q and k.size(0) == seqs.total_k, \
-        f"q and k have {q.size(0)} and {k.size(0)} rows, the sequences {seqs.total_q} and {seqs.total_k}"
+    assert rows == seqs.total_q and kv_rows == seqs.total_k, \
+        f"q and k have {rows} and {kv_rows} rows, the sequences {seqs.total_q} and {seqs.total_k}"
     sm_scale = d ** -0.5 if sm_scale is None else float(sm_scale)
     assert 0 <= sm_scale < float("inf"), "sm_scale must be finite and not negative"
-    causal = bool(causal)
+    key = (False, bool(causal), sm_scale, dtype, heads, kv_heads, d)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
-        o, lse = _PackedAttention.apply(q, k, v, seqs, causal, sm_scale)
-    else:
-        *_, o, _, lse = _forward(q, k, v, seqs, causal, sm_scale, return_lse)
+        return _PackedAttention.apply(q, k, v, seqs, key, return_lse)
+    lse = torch.empty((heads, rows), dtype=torch.float32, device=device) if return_lse else None
+    o = _forward(q, k, v, seqs, key, device, lse)[3]
     return (o, lse) if return_lse else o

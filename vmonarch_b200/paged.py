@@ -9,30 +9,37 @@ from; :class:`PagedKVCache` holds the pools of a model's layers and keeps the bo
 from __future__ import annotations
 
 import ctypes
+import struct
 
 import numpy as np
 import torch
 
 from . import _native as N
 from .kernel import SUPPORTED_DTYPES
-from .packed import MAX_DIM, _in_place, _rows
+from .packed import MAX_DIM, _place
 
 
 def _pages(t):
-    """vmb_pages of a pool whose pages the kernels can address."""
-    assert t.stride(3) == 1 or t.size(3) == 1, "pools need contiguous columns"
-    st = [s if n > 1 else 0 for n, s in zip(t.shape[:3], t.stride()[:3])]
-    assert t.data_ptr() % 16 == 0 and all(s % 8 == 0 for s in st), "pools need 16-byte aligned rows"
-    return N.Pages(t.data_ptr(), *st)
+    """vmb_pages of a pool (pages, heads, slots, dim), which the kernels address in place."""
+    ptr, (page, head, slot, col) = t.data_ptr(), t.stride()
+    n, h, ps, d = t.shape
+    page, head, slot = page if n > 1 else 0, head if h > 1 else 0, slot if ps > 1 else 0
+    assert col == 1 or d == 1, "pools need contiguous columns"
+    assert not ptr & 15 and page >= 0 and head >= 0 and slot >= 0 and not (page | head | slot) & 7, \
+        "pools need 16-byte aligned rows"
+    return ptr, page, head, slot
 
 
 def _check_pools(k_pages, v_pages):
+    """(pages, heads, page size, dim, dtype, device) of a pair of pools."""
     assert k_pages.dim() == 4 and v_pages.shape == k_pages.shape, "pools must be (num_pages, Hk, page_size, D)"
-    assert k_pages.dtype in SUPPORTED_DTYPES and v_pages.dtype == k_pages.dtype, f"unsupported dtype {k_pages.dtype}"
-    d = k_pages.size(3)
+    dtype, device = k_pages.dtype, k_pages.device
+    assert dtype in SUPPORTED_DTYPES and v_pages.dtype == dtype, f"unsupported dtype {dtype}"
+    n, h, ps, d = k_pages.shape
     assert 8 <= d <= MAX_DIM and d % 8 == 0, f"head dim {d} is not a multiple of 8 up to {MAX_DIM}"
-    assert k_pages.size(1) >= 1 and k_pages.size(2) >= 1, "pools need at least one head and one slot"
-    assert k_pages.is_cuda and v_pages.device == k_pages.device, "pools must be on one CUDA device"
+    assert h >= 1 and ps >= 1, "pools need at least one head and one slot"
+    assert k_pages.is_cuda and v_pages.device == device, "pools must be on one CUDA device"
+    return n, h, ps, d, dtype, device
 
 
 def _check_index(t, name, dim, device):
@@ -60,37 +67,42 @@ def paged_attention(q, k_pages, v_pages, page_table, lengths, *, sm_scale=None, 
     Table and lengths stay on the device: the call does not wait for it and can be captured in a CUDA
     graph whose replays see other lengths.
     """
-    _check_pools(k_pages, v_pages)
-    b, h, d = q.shape
-    assert q.dtype == k_pages.dtype and d == k_pages.size(3) and q.device == k_pages.device, \
+    num, hk, page_size, d, dtype, device = _check_pools(k_pages, v_pages)
+    assert q.dim() == 3 and q.dtype == dtype and q.size(2) == d and q.device == device, \
         "q must be (B, H, D) with the pools' D, dtype and device"
-    assert h >= 1 and h % k_pages.size(1) == 0, "H must be a multiple of Hk"
-    _check_index(page_table, "page_table", 2, q.device)
-    _check_index(lengths, "lengths", 1, q.device)
-    assert page_table.size(0) == b and lengths.size(0) == b, "page_table and lengths must have a row per sequence"
+    b, h, _ = q.shape
+    assert h >= 1 and h % hk == 0, "H must be a multiple of Hk"
+    _check_index(page_table, "page_table", 2, device)
+    _check_index(lengths, "lengths", 1, device)
+    rows, width = page_table.shape
+    assert rows == b and lengths.size(0) == b, "page_table and lengths must have a row per sequence"
     sm_scale = d ** -0.5 if sm_scale is None else float(sm_scale)
     assert 0 <= sm_scale < float("inf"), "sm_scale must be finite and not negative"
-    q, lengths = _in_place(q.detach()), lengths.contiguous()
-    if page_table.size(1) > 1 and page_table.stride(1) != 1 or b > 1 and page_table.stride(0) < page_table.size(1):
-        page_table = page_table.contiguous()
-    o = torch.empty((b, h, d), dtype=q.dtype, device=q.device)
-    lse = torch.empty((b, h), dtype=torch.float32, device=q.device) if return_lse else None
+    q, *qr = _place(q)
+    stride, col = page_table.stride()
+    if width > 1 and col != 1 or b > 1 and stride < width:
+        page_table, stride = page_table.contiguous(), width
+    lengths = lengths.contiguous()
+    o = torch.empty((b, h, d), dtype=dtype, device=device)
+    lse = torch.empty((b, h), dtype=torch.float32, device=device) if return_lse else None
     if b:
         a = N.PagedArgs()
-        a.q, a.o, a.k, a.v = _rows(q), _rows(o), _pages(k_pages), _pages(v_pages)
-        a.table, a.lengths = page_table.data_ptr(), lengths.data_ptr()
-        a.lse = lse.data_ptr() if return_lse else None
-        a.batch, a.table_width = b, page_table.size(1)
-        a.table_stride = page_table.stride(0) if b > 1 else page_table.size(1)
-        a.num_pages, a.page_size = k_pages.size(0), k_pages.size(2)
-        a.heads, a.kv_heads, a.dim = h, k_pages.size(1), d
-        a.dtype, a.sm_scale = N.dtype_code(q.dtype), sm_scale
-        nbytes = N.lib.vmb_paged_workspace_bytes(ctypes.byref(a))
-        if nbytes > 0:
-            ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
-            a.workspace, a.workspace_bytes = ws.data_ptr(), nbytes
-        N.check(N.lib.vmb_paged_attention(ctypes.byref(a), N.stream_ptr(q.device)), "vmb_paged_attention")
+        _PAGED.pack_into(a, 0, *qr, o.data_ptr(), h * d, d, *_pages(k_pages), *_pages(v_pages), page_table.data_ptr(),
+                         lengths.data_ptr(), lse.data_ptr() if return_lse else 0, b, stride if b > 1 else width, width, num,
+                         h, hk, d, page_size, N.dtype_code(dtype), sm_scale)
+        size = N.lib.vmb_paged_workspace_bytes(ctypes.byref(a))
+        if size > 0:
+            ws = torch.empty(size, dtype=torch.uint8, device=device)
+            a.workspace, a.workspace_bytes = ws.data_ptr(), size
+        rc = N.lib.vmb_paged_attention(ctypes.byref(a), N.raw_stream(device.index))
+        if rc:
+            N.check(rc, "vmb_paged_attention")
     return (o, lse) if return_lse else o
+
+
+# vmb_paged_args up to its workspace
+_PAGED = struct.Struct("21q5if")
+assert _PAGED.size == N.PagedArgs.workspace.offset
 
 
 def append_pages(k, v, k_pages, v_pages, slots):
@@ -103,21 +115,22 @@ def append_pages(k, v, k_pages, v_pages, slots):
         slots: (T,) int32, page * page_size + slot of each row. Slots outside the pool (negative ones, as
             padding) are skipped; no slot may be named twice.
     """
-    _check_pools(k_pages, v_pages)
-    assert k.dim() == 3 and v.shape == k.shape and k.shape[1:] == (k_pages.size(1), k_pages.size(3)), \
-        "k and v must be (T, Hk, D) with the pools' Hk and D"
-    assert k.dtype == k_pages.dtype and v.dtype == k.dtype, "k and v must have the pools' dtype"
-    assert k.device == k_pages.device and v.device == k.device, "k and v must be on the pools' device"
-    _check_index(slots, "slots", 1, k.device)
-    assert slots.size(0) == k.size(0), "slots must name one slot per row"
-    assert k_pages.size(0) * k_pages.size(2) < 2 ** 31, "slots are 32-bit: the pool has too many"
-    if k.size(0) == 0:
+    num, hk, page_size, d, dtype, device = _check_pools(k_pages, v_pages)
+    assert k.dim() == 3 and v.shape == k.shape and k.shape[1:] == (hk, d), "k and v must be (T, Hk, D) with the pools' Hk and D"
+    assert k.dtype == dtype and v.dtype == dtype, "k and v must have the pools' dtype"
+    assert k.device == device and v.device == device, "k and v must be on the pools' device"
+    _check_index(slots, "slots", 1, device)
+    n = k.size(0)
+    assert slots.size(0) == n, "slots must name one slot per row"
+    assert num * page_size < 2 ** 31, "slots are 32-bit: the pool has too many"
+    if n == 0:
         return
-    k, v, slots = _in_place(k.detach()), _in_place(v.detach()), slots.contiguous()
-    N.check(N.lib.vmb_append_pages(
-        ctypes.byref(_rows(k)), ctypes.byref(_rows(v)), ctypes.byref(_pages(k_pages)), ctypes.byref(_pages(v_pages)),
-        slots.data_ptr(), k.size(0), k_pages.size(0), k_pages.size(1), k_pages.size(3), k_pages.size(2),
-        N.stream_ptr(k.device)), "vmb_append_pages")
+    k, *kr = _place(k)
+    v, *vr = _place(v)
+    slots = slots.contiguous()
+    N.check(N.lib.vmb_append_pages(N.Rows(*kr), N.Rows(*vr), N.Pages(*_pages(k_pages)), N.Pages(*_pages(v_pages)),
+                                   slots.data_ptr(), n, num, hk, d, page_size, N.raw_stream(device.index)),
+            "vmb_append_pages")
 
 
 def copy_pages(k_pages, v_pages, src, dst):
@@ -129,17 +142,16 @@ def copy_pages(k_pages, v_pages, src, dst):
         src, dst: (n,) int32 page ids. Pairs with a page outside the pool are skipped; no destination may be
             another pair's source or destination.
     """
-    _check_pools(k_pages, v_pages)
-    _check_index(src, "src", 1, k_pages.device)
-    _check_index(dst, "dst", 1, k_pages.device)
-    assert src.size(0) == dst.size(0), "src and dst must have the same length"
-    if src.size(0) == 0:
+    num, hk, page_size, d, dtype, device = _check_pools(k_pages, v_pages)
+    _check_index(src, "src", 1, device)
+    _check_index(dst, "dst", 1, device)
+    n = src.size(0)
+    assert dst.size(0) == n, "src and dst must have the same length"
+    if n == 0:
         return
     src, dst = src.contiguous(), dst.contiguous()
-    N.check(N.lib.vmb_copy_pages(
-        ctypes.byref(_pages(k_pages)), ctypes.byref(_pages(v_pages)), src.data_ptr(), dst.data_ptr(), src.size(0),
-        k_pages.size(0), k_pages.size(1), k_pages.size(3), k_pages.size(2), N.stream_ptr(k_pages.device)),
-        "vmb_copy_pages")
+    N.check(N.lib.vmb_copy_pages(N.Pages(*_pages(k_pages)), N.Pages(*_pages(v_pages)), src.data_ptr(), dst.data_ptr(), n,
+                                 num, hk, d, page_size, N.raw_stream(device.index)), "vmb_copy_pages")
 
 
 class PagedKVCache:
