@@ -11,7 +11,7 @@ namespace {
 using vmb::set_error;
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
-bool matrix_ok(const vmb_matrix& m) { return aligned16(m.ptr) && m.row >= 0 && m.row % 8 == 0; }
+bool matrix_ok(const vmb_matrix& m) { return aligned16(m.ptr) && m.row >= 0 && m.row <= 0x7fffffff && m.row % 8 == 0; }
 int64_t up256(int64_t x) { return (x + 255) / 256 * 256; }
 
 int fill(const vmb_gated_norm_args* a, const char* what, vmb::GatedNormParams& p) {
@@ -32,13 +32,13 @@ int fill(const vmb_gated_norm_args* a, const char* what, vmb::GatedNormParams& p
   if (!matrix_ok(a->x) || !matrix_ok(a->y) || !matrix_ok(a->dx_new) || !matrix_ok(a->dh))
     return set_error(VMB_EINVAL, "%s: rows must be 16-byte aligned", what);
   if (a->rows > 0 && !a->y.ptr && (a->gate || a->post_weight)) return set_error(VMB_EINVAL, "%s: gate and post_weight need y", what);
-  p.x = a->x.ptr; p.y = a->y.ptr; p.x_row = a->x.row; p.y_row = a->y.row;
+  p.x = a->x.ptr; p.y = a->y.ptr; p.x_row = (int)a->x.row; p.y_row = (int)a->y.row;
   p.x_new = a->x_new; p.h = a->h;
   p.gate = a->gate; p.scale = a->scale; p.shift = a->shift; p.weight = a->weight; p.post_weight = a->post_weight;
   p.stats = a->stats;
   p.seq_start = a->seqs > 1 ? a->seq_start : nullptr;
-  p.dx_new = a->dx_new.ptr; p.dx_new_row = a->dx_new.row;
-  p.dh = a->dh.ptr; p.dh_row = a->dh.row;
+  p.dx_new = a->dx_new.ptr; p.dx_new_row = (int)a->dx_new.row;
+  p.dh = a->dh.ptr; p.dh_row = (int)a->dh.row;
   p.dx = a->dx; p.dy = a->dy;
   p.dgate = a->dgate; p.dscale = a->dscale; p.dshift = a->dshift; p.dweight = a->dweight; p.dpost_weight = a->dpost_weight;
   p.rows = a->rows; p.cols = a->cols; p.seqs = a->seqs; p.layer = a->layer ? 1 : 0;

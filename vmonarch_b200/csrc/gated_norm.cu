@@ -15,8 +15,9 @@
 // bytes than reading the rounded x' would); all arithmetic is 32-bit, rounded once at each output.
 //
 // Bound by memory: 8 bytes an element forward (x, y in, x', h out), 12 backward. A block takes an equal
-// share of all rows; TPR threads hold a row, 8 columns each, and go through the share R rows at a time
-// behind a ring of cp.async stages, in which every thread reads back only what it loaded itself. What the
+// share of all rows; groups of TPR threads hold a row each, 8 VPT columns a thread, and go through the share
+// behind a ring of cp.async stages, in which every thread reads back only what it loaded itself; a group's
+// warps meet at a barrier of their own, so one group's sums run beside another's arithmetic. What the
 // row-wise work needs of the parameters (gate post_weight, weight (1 + scale), shift) is combined once per
 // sequence into shared memory: from L2 it would be more than the rows' own traffic. The column sums
 // of the backward stay in registers over a block's rows of a sequence; each (block, sequence) leaves one
@@ -30,73 +31,100 @@
 namespace vmb {
 namespace {
 
-constexpr int kMaxWarps = 32;
 constexpr int kSmemLimit = 220 * 1024;  // dynamic shared memory of an SM's blocks together
 
+// Eight columns as four pairs: the packed f32x2 instructions do two products or sums at once.
+struct V8 {
+  float2 v[4];
+};
+__device__ __forceinline__ float2 pair(float a) { return make_float2(a, a); }
+__device__ __forceinline__ V8 splat(float a) { return V8{{pair(a), pair(a), pair(a), pair(a)}}; }
+template <typename T>
+__device__ __forceinline__ V8 unpack8(uint4 x) {
+  return V8{{Elem<T>::unpack(x.x), Elem<T>::unpack(x.y), Elem<T>::unpack(x.z), Elem<T>::unpack(x.w)}};
+}
+template <typename T>
+__device__ __forceinline__ uint4 pack8(const V8& f) {
+  return make_uint4(Elem<T>::pack(f.v[0].x, f.v[0].y), Elem<T>::pack(f.v[1].x, f.v[1].y),
+                    Elem<T>::pack(f.v[2].x, f.v[2].y), Elem<T>::pack(f.v[3].x, f.v[3].y));
+}
+__device__ __forceinline__ void put8(float* s, const V8& f) {
+  reinterpret_cast<float4*>(s)[0] = make_float4(f.v[0].x, f.v[0].y, f.v[1].x, f.v[1].y);
+  reinterpret_cast<float4*>(s)[1] = make_float4(f.v[2].x, f.v[2].y, f.v[3].x, f.v[3].y);
+}
+__device__ __forceinline__ V8 get8(const float* s) {
+  const float4 a = reinterpret_cast<const float4*>(s)[0], b = reinterpret_cast<const float4*>(s)[1];
+  return V8{{make_float2(a.x, a.y), make_float2(a.z, a.w), make_float2(b.x, b.y), make_float2(b.z, b.w)}};
+}
+__device__ __forceinline__ float sum8(const V8& f) {
+  const float2 a = __fadd2_rn(__fadd2_rn(f.v[0], f.v[1]), __fadd2_rn(f.v[2], f.v[3]));
+  return a.x + a.y;
+}
+__device__ __forceinline__ float dot8(const V8& f, const V8& g) {
+  const float2 a = __ffma2_rn(f.v[0], g.v[0], __fmul2_rn(f.v[1], g.v[1]));
+  const float2 b = __ffma2_rn(f.v[2], g.v[2], __fmul2_rn(f.v[3], g.v[3]));
+  return (a.x + b.x) + (a.y + b.y);
+}
 template <typename T, typename P>
-struct Io;  // 8 elements of a parameter as floats
+struct Io;  // 8 elements of a parameter
 template <typename T>
 struct Io<T, float> {
-  static __device__ __forceinline__ void load(const void* base, int64_t at, float* f) {
-    const float4 a = *reinterpret_cast<const float4*>(static_cast<const float*>(base) + at);
-    const float4 b = *reinterpret_cast<const float4*>(static_cast<const float*>(base) + at + 4);
-    f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w;
-    f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
-  }
+  static __device__ __forceinline__ V8 load(const void* base, int64_t at) { return get8(static_cast<const float*>(base) + at); }
 };
-template <typename T>
-__device__ __forceinline__ void unpack8(uint4 v, float* f) {
-  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float2 p = Elem<T>::unpack(w[i]);
-    f[2 * i] = p.x;
-    f[2 * i + 1] = p.y;
-  }
-}
-template <typename T>
-__device__ __forceinline__ uint4 pack8(const float* f) {
-  return make_uint4(Elem<T>::pack(f[0], f[1]), Elem<T>::pack(f[2], f[3]), Elem<T>::pack(f[4], f[5]), Elem<T>::pack(f[6], f[7]));
-}
 template <typename T>
 struct Io<T, T> {
-  static __device__ __forceinline__ void load(const void* base, int64_t at, float* f) {
-    unpack8<T>(*reinterpret_cast<const uint4*>(static_cast<const T*>(base) + at), f);
+  static __device__ __forceinline__ V8 load(const void* base, int64_t at) {
+    return unpack8<T>(*reinterpret_cast<const uint4*>(static_cast<const T*>(base) + at));
   }
 };
 
-__device__ __forceinline__ void put8(float* s, const float* f) {
-  reinterpret_cast<float4*>(s)[0] = make_float4(f[0], f[1], f[2], f[3]);
-  reinterpret_cast<float4*>(s)[1] = make_float4(f[4], f[5], f[6], f[7]);
-}
-__device__ __forceinline__ void get8(const float* s, float* f) {
-  const float4 a = reinterpret_cast<const float4*>(s)[0], b = reinterpret_cast<const float4*>(s)[1];
-  f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w;
-  f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int s = 16; s > 0; s >>= 1) v += __shfl_xor_sync(0xffffffffu, v, s);
+  return v;
 }
 
-// Sums N values over the `wpr` warps of a row's threads. sums: [2][N][kMaxWarps + pad], alternating.
-template <int N>
-__device__ __forceinline__ void row_sum(float (&v)[N], float* sums, int& flip, int group, int wpr) {
-#pragma unroll
-  for (int s = 16; s > 0; s >>= 1)
-#pragma unroll
-    for (int i = 0; i < N; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], s);
-  if (wpr == 1) return;
-  // two buffers in turn: a thread that writes one again has passed the barrier of the other since
-  float* b = sums + flip * (4 * kMaxWarps);
-  flip ^= 1;
-  if ((threadIdx.x & 31) == 0)
-#pragma unroll
-    for (int i = 0; i < N; ++i) b[i * kMaxWarps + (threadIdx.x >> 5)] = v[i];
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    float t = 0.f;
-    for (int w = 0; w < wpr; ++w) t += b[i * kMaxWarps + group * wpr + w];
-    v[i] = t;
+// Where the warps of a row meet: two buffers in turn of up to two values a warp (a thread that writes one again
+// has passed the barrier of the other since). A group's slots begin at a multiple of four and are padded
+// with zeros to 4 N4, the most warps that a row of this instance has.
+template <int N4>
+struct Meet {
+  float* buf;  // [2][2][kSlots]
+  int group, tpr, slot, base;
+  static constexpr int kSlots = 64;
+  __device__ __forceinline__ Meet(float* shared, int tpr_) : buf(shared), tpr(tpr_) {
+    group = threadIdx.x / tpr;
+    base = group * 4 * N4;
+    slot = base + (threadIdx.x - group * tpr) / 32;
+    for (int i = threadIdx.x; i < 4 * kSlots; i += blockDim.x) buf[i] = 0.f;
+    __syncthreads();
   }
-}
+  template <int N>
+  __device__ __forceinline__ void sum(float (&v)[N], int& flip) const {
+    static_assert(N <= 2, "two values a meeting");
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = warp_sum(v[i]);
+    if constexpr (N4 > 0) {
+      float* b = buf + flip;
+      flip ^= 2 * kSlots;
+      if ((threadIdx.x & 31) == 0)
+#pragma unroll
+        for (int i = 0; i < N; ++i) b[i * kSlots + slot] = v[i];
+      asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "r"(tpr) : "memory");
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        float2 a = make_float2(0.f, 0.f), c = a;
+#pragma unroll
+        for (int w = 0; w < N4; ++w) {
+          const float4 x = *reinterpret_cast<const float4*>(b + i * kSlots + base + 4 * w);
+          a = __fadd2_rn(a, make_float2(x.x, x.y));
+          c = __fadd2_rn(c, make_float2(x.z, x.w));
+        }
+        v[i] = (a.x + c.x) + (a.y + c.y);
+      }
+    }
+  }
+};
 
 struct Share {
   int64_t r0, r1;  // rows of this block
@@ -105,316 +133,315 @@ struct Share {
 __device__ __forceinline__ int64_t seq_begin(const GatedNormParams& p, int s) {
   return p.seq_start ? p.seq_start[s] : (s == 0 ? 0 : p.rows);
 }
+// The last sequence that begins at or before `row`, 32 candidates a step (every warp for itself).
+__device__ __forceinline__ int seq_of(const GatedNormParams& p, int64_t row) {
+  int lo = 0, n = p.seqs;  // the answer is in [lo, lo + n)
+  while (n > 1) {
+    const int step = (n + 31) / 32, at = (threadIdx.x & 31) * step;
+    const unsigned hit = __ballot_sync(0xffffffffu, at < n && seq_begin(p, lo + at) <= row);
+    const int k = hit ? 31 - __clz(hit) : 0;  // begins only grow: the hits are the first lanes
+    lo += k * step;
+    n = min(step, n - k * step);
+  }
+  return lo;
+}
 __device__ __forceinline__ Share share_of_block(const GatedNormParams& p) {
   Share s;
   s.r0 = p.rows * blockIdx.x / gridDim.x;
   s.r1 = p.rows * (blockIdx.x + 1) / gridDim.x;
-  int lo = 0, hi = p.seqs;  // last sequence that begins at or before r0
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) / 2;
-    if (seq_begin(p, mid) <= s.r0) lo = mid;
-    else hi = mid;
-  }
-  s.seq = lo;
+  s.seq = seq_of(p, s.r0);
   return s;
 }
 
-// NIN row tensors, R rows a stage and group: the ring of this thread's 16-byte pieces.
-template <int NIN, int R>
-struct Ring {
-  uint8_t* base;
-  int stages;
-  __device__ __forceinline__ uint4* at(int stage, int r, int in) const {
-    return reinterpret_cast<uint4*>(base) + ((stage * R + r) * NIN + in) * blockDim.x + threadIdx.x;
-  }
-};
 __device__ __forceinline__ void wait_stages(int pending) {
   if (pending >= 3) cp_async_wait<3>();
   else if (pending == 2) cp_async_wait<2>();
   else if (pending == 1) cp_async_wait<1>();
   else cp_async_wait<0>();
 }
+template <typename T>
+__device__ __forceinline__ T* at(const void* base, int row, int stride, int col) {
+  return const_cast<T*>(static_cast<const T*>(base)) + (int64_t)row * stride + col;
+}
+__device__ __forceinline__ uint4 ld_shared16(uint32_t at) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at));
+  return v;
+}
 
 // The parameters of a sequence, combined: [gate post | weight (1 + scale) | shift], 8 columns a thread.
 template <typename T, typename P>
 __device__ __forceinline__ void load_params(const GatedNormParams& p, int seq, int col, bool on, float* gw, float* sw,
                                             float* sh) {
-  float a[8], b[8];
-  auto one = [&](float (&f)[8]) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = 1.f;
-  };
   if (!on) return;
   const int64_t row = (int64_t)seq * p.cols + col;
-  one(a);
-  one(b);
-  if (p.gate) Io<T, P>::load(p.gate, row, a);
-  if (p.post_weight) Io<T, P>::load(p.post_weight, col, b);
+  V8 gate = splat(1.f), post = gate, weight = gate, scale = splat(0.f), shift = scale;
+  if (p.gate) gate = Io<T, P>::load(p.gate, row);
+  if (p.post_weight) post = Io<T, P>::load(p.post_weight, col);
+  if (p.weight) weight = Io<T, P>::load(p.weight, col);
+  if (p.scale) scale = Io<T, P>::load(p.scale, row);
+  if (sh && p.shift) shift = Io<T, P>::load(p.shift, row);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) a[i] *= b[i];
-  put8(gw + col, a);
-  one(a);
-  one(b);
-  if (p.weight) Io<T, P>::load(p.weight, col, a);
-  if (p.scale) {
-    Io<T, P>::load(p.scale, row, b);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) b[i] += 1.f;
+  for (int i = 0; i < 4; ++i) {
+    gate.v[i] = __fmul2_rn(gate.v[i], post.v[i]);
+    weight.v[i] = __fmul2_rn(weight.v[i], __fadd2_rn(scale.v[i], pair(1.f)));
   }
-#pragma unroll
-  for (int i = 0; i < 8; ++i) a[i] *= b[i];
-  put8(sw + col, a);
-  if (sh) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) a[i] = 0.f;
-    if (p.shift) Io<T, P>::load(p.shift, row, a);
-    put8(sh + col, a);
-  }
+  put8(gw + col, gate);
+  put8(sw + col, weight);
+  if (sh) put8(sh + col, shift);
 }
 
-template <typename T, typename P, bool HAS_Y, int R, int MAXT>
+template <typename T, typename P, bool HAS_Y, int VPT, int N4, int MAXT>
 __global__ void __launch_bounds__(MAXT) gated_norm_fwd_kernel(const __grid_constant__ GatedNormParams p) {
   constexpr int NIN = HAS_Y ? 2 : 1;
   extern __shared__ __align__(16) uint8_t smem[];
-  __shared__ float sums[2 * 4 * kMaxWarps];
-  const int tpr = p.tpr, wpr = tpr >> 5, group = threadIdx.x / tpr, groups = blockDim.x / tpr;
-  const int col = (threadIdx.x % tpr) * 8;
-  const bool on = col < p.cols;
+  __shared__ __align__(16) float meeting[4 * Meet<N4>::kSlots];
+  const int tpr = p.tpr, groups = blockDim.x / tpr;
+  const Meet<N4> meet(meeting, tpr);
+  int flip = 0, col[VPT];
+  bool on[VPT];
+#pragma unroll
+  for (int v = 0; v < VPT; ++v) {
+    col[v] = (v * tpr + (int)threadIdx.x - meet.group * tpr) * 8;
+    on[v] = col[v] < p.cols;
+  }
   float* gw = reinterpret_cast<float*>(smem);
   float *sw = gw + p.cols, *sh = sw + p.cols;
-  const Ring<NIN, R> ring{reinterpret_cast<uint8_t*>(sh + p.cols), p.stages};
+  const uint32_t ring = smem_u32(sh + p.cols) + threadIdx.x * 16, piece = blockDim.x * 16, stage = NIN * VPT * piece;
   const float inv_c = 1.f / (float)p.cols;
   const bool post = HAS_Y && p.post_weight != nullptr, layer = p.layer != 0;
-  int flip = 0;
 
   const Share s = share_of_block(p);
   int seq = s.seq;
   for (int64_t a = s.r0; a < s.r1;) {
     while (seq + 1 < p.seqs && seq_begin(p, seq + 1) <= a) ++seq;
     const int64_t b = min(s.r1, seq + 1 < p.seqs ? seq_begin(p, seq + 1) : p.rows);
-    const int n = (int)((b - a + (int64_t)groups * R - 1) / (groups * R));  // stages of this run of rows
-    auto row_of = [&](int it, int r) { return a + ((int64_t)it * groups + group) * R + r; };
-    auto issue = [&](int it) {
-      if (it < n && on)
+    // rows of this group: a + group, a + group + groups, ...
+    const int n = (int)max((b - a - meet.group + groups - 1) / groups, (int64_t)0);
+    int to_load = n, load_row = (int)a + meet.group;
+    uint32_t put = ring, get = ring;
+    const uint32_t end = ring + p.stages * stage;
+    auto issue = [&]() {
+      if (to_load > 0) {
+        --to_load;
 #pragma unroll
-        for (int r = 0; r < R; ++r) {
-          const int64_t row = row_of(it, r);
-          if (row >= b) continue;
-          cp_async16(smem_u32(ring.at(it % p.stages, r, 0)), static_cast<const T*>(p.x) + row * p.x_row + col, 16);
-          if (HAS_Y) cp_async16(smem_u32(ring.at(it % p.stages, r, NIN - 1)), static_cast<const T*>(p.y) + row * p.y_row + col, 16);
-        }
+        for (int v = 0; v < VPT; ++v)
+          if (on[v]) {
+            cp_async16(put + v * piece, at<T>(p.x, load_row, p.x_row, col[v]), 16);
+            if (HAS_Y) cp_async16(put + (VPT + v) * piece, at<T>(p.y, load_row, p.y_row, col[v]), 16);
+          }
+        load_row += groups;
+        put = put + stage == end ? ring : put + stage;
+      }
       cp_async_commit();
     };
-    for (int i = 0; i < p.stages - 1; ++i) issue(i);
+    for (int i = 0; i < p.stages - 1; ++i) issue();
     __syncthreads();  // the last run's parameters are no longer read
-    if (group == 0) load_params<T, P>(p, seq, col, on, gw, sw, sh);
+    if (meet.group == 0)
+#pragma unroll
+      for (int v = 0; v < VPT; ++v) load_params<T, P>(p, seq, col[v], on[v], gw, sw, sh);
     __syncthreads();
-    for (int it = 0; it < n; ++it) {
+    int row = (int)a + meet.group;
+    for (int it = 0; it < n; ++it, row += groups) {
       wait_stages(p.stages - 2);
-      float x[R][8], y[HAS_Y ? R : 1][8], acc[R];
+      V8 x[VPT], y[HAS_Y ? VPT : 1];
 #pragma unroll
-      for (int r = 0; r < R; ++r) {
-        const bool live = on && row_of(it, r) < b;
-        const uint4 zero = make_uint4(0, 0, 0, 0);
-        unpack8<T>(live ? *ring.at(it % p.stages, r, 0) : zero, x[r]);
-        if constexpr (HAS_Y) unpack8<T>(live ? *ring.at(it % p.stages, r, 1) : zero, y[r]);
+      for (int v = 0; v < VPT; ++v) {
+        x[v] = splat(0.f);
+        if (on[v]) x[v] = unpack8<T>(ld_shared16(get + v * piece));
+        if constexpr (HAS_Y) {
+          y[v] = splat(0.f);
+          if (on[v]) y[v] = unpack8<T>(ld_shared16(get + (VPT + v) * piece));
+        }
       }
-      issue(it + p.stages - 1);
-      float ry[R], mean[R], rx[R];
-#pragma unroll
-      for (int r = 0; r < R; ++r) ry[r] = 1.f, mean[r] = 0.f;
+      get = get + stage == end ? ring : get + stage;
+      issue();
+      float ry[1] = {1.f}, mean[1] = {0.f}, rx[1] = {0.f};
       if constexpr (HAS_Y) {
         if (post) {
+          ry[0] = 0.f;
 #pragma unroll
-          for (int r = 0; r < R; ++r) {
-            acc[r] = 0.f;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) acc[r] = fmaf(y[r][i], y[r][i], acc[r]);
-          }
-          row_sum<R>(acc, sums, flip, group, wpr);
-#pragma unroll
-          for (int r = 0; r < R; ++r) ry[r] = rsqrtf(fmaf(acc[r], inv_c, p.eps));
+          for (int v = 0; v < VPT; ++v) ry[0] += dot8(y[v], y[v]);
+          meet.sum(ry, flip);
+          ry[0] = rsqrtf(fmaf(ry[0], inv_c, p.eps));
         }
-        float g[8];
-        if (on) get8(gw + col, g);
 #pragma unroll
-        for (int r = 0; r < R; ++r)
+        for (int v = 0; v < VPT; ++v)
+          if (on[v]) {
+            const V8 g = get8(gw + col[v]);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) x[r][i] = on ? fmaf(g[i], y[r][i] * ry[r], x[r][i]) : 0.f;
+            for (int i = 0; i < 4; ++i) x[v].v[i] = __ffma2_rn(g.v[i], __fmul2_rn(y[v].v[i], pair(ry[0])), x[v].v[i]);
+            *reinterpret_cast<uint4*>(at<T>(p.x_new, row, p.cols, col[v])) = pack8<T>(x[v]);
+          }
       }
       if (layer) {
+        // the mean first, then squares of differences: no cancellation where the mean is large
 #pragma unroll
-        for (int r = 0; r < R; ++r) {
-          acc[r] = 0.f;
+        for (int v = 0; v < VPT; ++v) mean[0] += sum8(x[v]);
+        meet.sum(mean, flip);
+        mean[0] *= inv_c;
 #pragma unroll
-          for (int i = 0; i < 8; ++i) acc[r] += x[r][i];
-        }
-        row_sum<R>(acc, sums, flip, group, wpr);
+        for (int v = 0; v < VPT; ++v)
+          if (on[v])
 #pragma unroll
-        for (int r = 0; r < R; ++r) mean[r] = acc[r] * inv_c;
+            for (int i = 0; i < 4; ++i) x[v].v[i] = __fadd2_rn(x[v].v[i], pair(-mean[0]));
       }
 #pragma unroll
-      for (int r = 0; r < R; ++r) {
-        acc[r] = 0.f;
+      for (int v = 0; v < VPT; ++v) rx[0] += dot8(x[v], x[v]);
+      meet.sum(rx, flip);
+      rx[0] = rsqrtf(fmaf(rx[0], inv_c, p.eps));
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float d = on ? x[r][i] - mean[r] : 0.f;
-          acc[r] = fmaf(d, d, acc[r]);
-        }
-      }
-      row_sum<R>(acc, sums, flip, group, wpr);
+      for (int v = 0; v < VPT; ++v)
+        if (on[v]) {
+          const V8 w = get8(sw + col[v]), t = get8(sh + col[v]);
+          V8 h;
 #pragma unroll
-      for (int r = 0; r < R; ++r) rx[r] = rsqrtf(fmaf(acc[r], inv_c, p.eps));
-      if (on) {
-        float w[8], t[8];
-        get8(sw + col, w);
-        get8(sh + col, t);
-#pragma unroll
-        for (int r = 0; r < R; ++r) {
-          const int64_t row = row_of(it, r);
-          if (row >= b) continue;
-          if (HAS_Y) *reinterpret_cast<uint4*>(static_cast<T*>(p.x_new) + row * p.cols + col) = pack8<T>(x[r]);
-          float h[8];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) h[i] = fmaf((x[r][i] - mean[r]) * rx[r], w[i], t[i]);
-          *reinterpret_cast<uint4*>(static_cast<T*>(p.h) + row * p.cols + col) = pack8<T>(h);
-          if (p.stats && col == 0) {
-            p.stats[row] = ry[r];
-            p.stats[p.rows + row] = mean[r];
-            p.stats[2 * p.rows + row] = rx[r];
+          for (int i = 0; i < 4; ++i) h.v[i] = __ffma2_rn(__fmul2_rn(x[v].v[i], pair(rx[0])), w.v[i], t.v[i]);
+          *reinterpret_cast<uint4*>(at<T>(p.h, row, p.cols, col[v])) = pack8<T>(h);
+          if (p.stats && col[v] == 0) {
+            p.stats[row] = ry[0];
+            p.stats[p.rows + row] = mean[0];
+            p.stats[2 * p.rows + row] = rx[0];
           }
         }
-      }
     }
     cp_async_wait<0>();
     a = b;
   }
 }
 
-template <typename T, typename P, bool HAS_Y, int R, int MAXT>
+// AGAIN: a row's values are read from the ring once more behind the first meeting instead of living through it
+// in registers (rows of more than 640 threads, which have 64 registers each).
+template <typename T, typename P, bool HAS_Y, int N4, int MAXT, bool AGAIN>
 __global__ void __launch_bounds__(MAXT) gated_norm_bwd_kernel(const __grid_constant__ GatedNormParams p) {
   constexpr int NIN = HAS_Y ? 4 : 3;  // x, dh, dx', y
   extern __shared__ __align__(16) uint8_t smem[];
-  __shared__ float sums[2 * 4 * kMaxWarps];
-  static_assert(2 * R <= 4, "row_sum's buffers hold four sums");
-  const int tpr = p.tpr, wpr = tpr >> 5, group = threadIdx.x / tpr, groups = blockDim.x / tpr;
-  const int col = (threadIdx.x % tpr) * 8;
+  __shared__ __align__(16) float meeting[4 * Meet<N4>::kSlots];
+  const int tpr = p.tpr, groups = blockDim.x / tpr;
+  const Meet<N4> meet(meeting, tpr);
+  const int group = meet.group, col = ((int)threadIdx.x - group * tpr) * 8;
   const bool on = col < p.cols;
+  int flip = 0;
   float* gw = reinterpret_cast<float*>(smem);
   float* sw = gw + p.cols;
-  const Ring<NIN, R> ring{reinterpret_cast<uint8_t*>(sw + p.cols), p.stages};
+  const uint32_t ring = smem_u32(sw + p.cols) + threadIdx.x * 16, piece = blockDim.x * 16, stage = NIN * piece;
   const float inv_c = 1.f / (float)p.cols;
-  const bool post = HAS_Y && p.post_weight != nullptr, layer = p.layer != 0;
-  int flip = 0;
+  const bool post = HAS_Y && p.post_weight != nullptr;
 
   const Share s = share_of_block(p);
   int seq = s.seq;
   for (int64_t a = s.r0; a < s.r1;) {
     while (seq + 1 < p.seqs && seq_begin(p, seq + 1) <= a) ++seq;
     const int64_t b = min(s.r1, seq + 1 < p.seqs ? seq_begin(p, seq + 1) : p.rows);
-    const int n = (int)((b - a + (int64_t)groups * R - 1) / (groups * R));
-    auto row_of = [&](int it, int r) { return a + ((int64_t)it * groups + group) * R + r; };
-    auto issue = [&](int it) {
-      if (it < n && on)
-#pragma unroll
-        for (int r = 0; r < R; ++r) {
-          const int64_t row = row_of(it, r);
-          if (row >= b) continue;
-          const int st = it % p.stages;
-          cp_async16(smem_u32(ring.at(st, r, 0)), static_cast<const T*>(p.x) + row * p.x_row + col, 16);
-          if (p.dh) cp_async16(smem_u32(ring.at(st, r, 1)), static_cast<const T*>(p.dh) + row * p.dh_row + col, 16);
-          if (p.dx_new) cp_async16(smem_u32(ring.at(st, r, 2)), static_cast<const T*>(p.dx_new) + row * p.dx_new_row + col, 16);
-          if (HAS_Y) cp_async16(smem_u32(ring.at(st, r, NIN - 1)), static_cast<const T*>(p.y) + row * p.y_row + col, 16);
+    const int n = (int)max((b - a - group + groups - 1) / groups, (int64_t)0);
+    int to_load = n, load_row = (int)a + group;
+    uint32_t put = ring, get = ring;
+    const uint32_t end = ring + p.stages * stage;
+    auto issue = [&]() {
+      if (to_load > 0) {
+        --to_load;
+        if (on) {
+          cp_async16(put, at<T>(p.x, load_row, p.x_row, col), 16);
+          if (p.dh) cp_async16(put + piece, at<T>(p.dh, load_row, p.dh_row, col), 16);
+          if (p.dx_new) cp_async16(put + 2 * piece, at<T>(p.dx_new, load_row, p.dx_new_row, col), 16);
+          if (HAS_Y) cp_async16(put + 3 * piece, at<T>(p.y, load_row, p.y_row, col), 16);
         }
+        load_row += groups;
+        put = put + stage == end ? ring : put + stage;
+      }
       cp_async_commit();
     };
-    for (int i = 0; i < p.stages - 1; ++i) issue(i);
+    for (int i = 0; i < p.stages - 1; ++i) issue();
     __syncthreads();  // the last run's parameters and sums are no longer read
     if (group == 0) load_params<T, P>(p, seq, col, on, gw, sw, nullptr);
     __syncthreads();
-    float sa[8], sb[8], sc[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) sa[i] = sb[i] = sc[i] = 0.f;
-    for (int it = 0; it < n; ++it) {
+    V8 sa = splat(0.f), sb = sa, sc = sa;
+    int row = (int)a + group;
+    // the rows' statistics, one row ahead of their use
+    float nry = 0.f, nmean = 0.f, nrx = 0.f;
+    auto load_stats = [&](int r) {
+      nry = p.stats[r];
+      nmean = p.stats[p.rows + r];
+      nrx = p.stats[2 * p.rows + r];
+    };
+    if (n > 0) load_stats(row);
+    for (int it = 0; it < n; ++it, row += groups) {
       wait_stages(p.stages - 2);
-      float xn[R][8], yn[HAS_Y ? R : 1][8], dh[R][8], acc[2 * R], ry[R], rx[R];
-      uint4 dxr[R];
-      float g[8], w[8];
-      if (on) {
-        get8(gw + col, g);
-        get8(sw + col, w);
-      }
-#pragma unroll
-      for (int r = 0; r < R; ++r) {
-        const int64_t row = row_of(it, r);
-        const bool live = on && row < b;
-        const uint4 zero = make_uint4(0, 0, 0, 0);
-        const int st = it % p.stages;
-        float mean = 0.f;
-        ry[r] = rx[r] = 0.f;
-        if (row < b) {
-          ry[r] = p.stats[row];
-          mean = p.stats[p.rows + row];
-          rx[r] = p.stats[2 * p.rows + row];
-        }
-        unpack8<T>(live ? *ring.at(st, r, 0) : zero, xn[r]);
-        unpack8<T>(live && p.dh ? *ring.at(st, r, 1) : zero, dh[r]);
-        dxr[r] = live && p.dx_new ? *ring.at(st, r, 2) : zero;
+      const float ry = nry, mean = nmean, rx = nrx;
+      V8 xn, yn, dh;  // n, y ry and dh of the formulas; columns past the width hold zeros
+      auto read = [&]() {
+        xn = yn = dh = splat(0.f);
+        if (!on) return;
+        xn = unpack8<T>(ld_shared16(get));
+        if (p.dh) dh = unpack8<T>(ld_shared16(get + piece));
         if constexpr (HAS_Y) {
-          unpack8<T>(live ? *ring.at(st, r, NIN - 1) : zero, yn[r]);
+          yn = unpack8<T>(ld_shared16(get + 3 * piece));
+          const V8 g = get8(gw + col);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            yn[r][i] *= ry[r];
-            if (live) xn[r][i] = fmaf(g[i], yn[r][i], xn[r][i]);
+          for (int i = 0; i < 4; ++i) {
+            yn.v[i] = __fmul2_rn(yn.v[i], pair(ry));
+            xn.v[i] = __ffma2_rn(g.v[i], yn.v[i], xn.v[i]);
           }
         }
-        acc[2 * r] = acc[2 * r + 1] = 0.f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          xn[r][i] = live ? (xn[r][i] - mean) * rx[r] : 0.f;
-          sb[i] = fmaf(dh[r][i], xn[r][i], sb[i]);
-          sc[i] += dh[r][i];
-          dh[r][i] = live ? dh[r][i] * w[i] : 0.f;  // g of the formulas
-          acc[2 * r] = fmaf(dh[r][i], xn[r][i], acc[2 * r]);
-          acc[2 * r + 1] += dh[r][i];
-        }
+        for (int i = 0; i < 4; ++i) xn.v[i] = __fmul2_rn(__fadd2_rn(xn.v[i], pair(-mean)), pair(rx));
+      };
+      auto weigh = [&]() {  // dh -> g of the formulas
+        if (!on) return;
+        const V8 w = get8(sw + col);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) dh.v[i] = __fmul2_rn(dh.v[i], w.v[i]);
+      };
+      read();
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        sb.v[i] = __ffma2_rn(dh.v[i], xn.v[i], sb.v[i]);
+        sc.v[i] = __fadd2_rn(sc.v[i], dh.v[i]);
       }
-      issue(it + p.stages - 1);
-      row_sum<2 * R>(acc, sums, flip, group, wpr);
-      float acc2[R];
-#pragma unroll
-      for (int r = 0; r < R; ++r) {
-        const float gn = acc[2 * r] * inv_c, gm = layer ? acc[2 * r + 1] * inv_c : 0.f;
-        float d[8];
-        unpack8<T>(dxr[r], d);
-        acc2[r] = 0.f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          d[i] = fmaf(rx[r], dh[r][i] - gm - xn[r][i] * gn, d[i]);
-          dh[r][i] = on ? d[i] : 0.f;  // dx
-          if constexpr (HAS_Y) {
-            sa[i] = row_of(it, r) < b && on ? fmaf(d[i], yn[r][i], sa[i]) : sa[i];
-            xn[r][i] = on ? d[i] * g[i] : 0.f;  // t
-            acc2[r] = fmaf(xn[r][i], yn[r][i], acc2[r]);
-          }
-        }
+      weigh();
+      float acc[2] = {dot8(dh, xn), sum8(dh)};
+      V8 dx = splat(0.f);
+      auto read_dx = [&]() {
+        if (on && p.dx_new) dx = unpack8<T>(ld_shared16(get + 2 * piece));
+      };
+      auto next = [&]() {
+        get = get + stage == end ? ring : get + stage;
+        issue();
+      };
+      if (!AGAIN) {
+        read_dx();
+        next();
       }
-      if (post) row_sum<R>(acc2, sums, flip, group, wpr);
-      if (on) {
+      if (it + 1 < n) load_stats(row + groups);
+      meet.sum(acc, flip);
+      if (AGAIN) {
+        read();
+        weigh();
+        read_dx();
+        next();
+      }
+      const float2 gn = pair(-acc[0] * inv_c * rx), gm = pair(p.layer ? -acc[1] * inv_c * rx : 0.f);
 #pragma unroll
-        for (int r = 0; r < R; ++r) {
-          const int64_t row = row_of(it, r);
-          if (row >= b) continue;
-          *reinterpret_cast<uint4*>(static_cast<T*>(p.dx) + row * p.cols + col) = pack8<T>(dh[r]);
-          if constexpr (HAS_Y) {
-            if (post) {
-              const float m = acc2[r] * inv_c;
+      for (int i = 0; i < 4; ++i) {
+        dx.v[i] = __fadd2_rn(dx.v[i], __ffma2_rn(dh.v[i], pair(rx), __ffma2_rn(xn.v[i], gn, gm)));
+        if constexpr (HAS_Y) sa.v[i] = __ffma2_rn(dx.v[i], yn.v[i], sa.v[i]);
+      }
+      if (on) *reinterpret_cast<uint4*>(at<T>(p.dx, row, p.cols, col)) = pack8<T>(dx);
+      if constexpr (HAS_Y) {
+        V8 t = splat(0.f);  // t of the formulas
+        if (on) {
+          const V8 g = get8(gw + col);
 #pragma unroll
-              for (int i = 0; i < 8; ++i) xn[r][i] = ry[r] * (xn[r][i] - yn[r][i] * m);
-            }
-            *reinterpret_cast<uint4*>(static_cast<T*>(p.dy) + row * p.cols + col) = pack8<T>(xn[r]);
-          }
+          for (int i = 0; i < 4; ++i) t.v[i] = __fmul2_rn(dx.v[i], g.v[i]);
         }
+        if (post) {
+          float dot[1] = {dot8(t, yn)};
+          meet.sum(dot, flip);
+          const float2 m = pair(-dot[0] * inv_c * ry);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) t.v[i] = __ffma2_rn(yn.v[i], m, __fmul2_rn(t.v[i], pair(ry)));
+        }
+        if (on) *reinterpret_cast<uint4*>(at<T>(p.dy, row, p.cols, col)) = pack8<T>(t);
       }
     }
     cp_async_wait<0>();
@@ -427,14 +454,13 @@ __global__ void __launch_bounds__(MAXT) gated_norm_bwd_kernel(const __grid_const
         for (int g2 = 0; g2 < groups; ++g2) {
           if (group == g2 && on) {
             float* acc3 = reinterpret_cast<float*>(smem);
-            float f[8];
 #pragma unroll
             for (int q = 0; q < 3; ++q) {
-              float* mine = q == 0 ? sa : q == 1 ? sb : sc;
+              V8& mine = q == 0 ? sa : q == 1 ? sb : sc;
               if (g2 > 0) {
-                get8(acc3 + q * p.cols + col, f);
+                const V8 f = get8(acc3 + q * p.cols + col);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) mine[i] += f[i];
+                for (int i = 0; i < 4; ++i) mine.v[i] = __fadd2_rn(mine.v[i], f.v[i]);
               }
               put8(acc3 + q * p.cols + col, mine);
               if (g2 == groups - 1) put8(out + q * p.cols + col, mine);
@@ -520,60 +546,66 @@ __global__ void __launch_bounds__(128) gated_norm_weights_kernel(const __grid_co
 }
 
 // ------------------------------------------------------------------------------------ host
-// Threads that hold a row: 8 columns each, whole warps.
-int row_threads(int cols) { return (cols / 8 + 31) / 32 * 32; }
+// Threads that hold a row of 8 vpt columns each, whole warps.
+int row_threads(int cols, int vpt) { return (cols / (8 * vpt) + (cols % (8 * vpt) ? 1 : 0) + 31) / 32 * 32; }
 
 struct Shape {
   int threads, tpr, stages, blocks, smem;
 };
-// Threads: whole rows of TPR = cols / 8 rounded up to warps, 256 threads or one row. Stages: up to four,
-// what fits beside the combined parameters; blocks: an equal share for every block that is resident.
-Shape shape_of(int cols, int64_t rows, int nparam, int nin, int r, int regs_cap_threads) {
+// `most` threads or one row; as many stages, up to four, as fit beside the combined parameters; every block
+// that is resident gets an equal share of the rows.
+Shape shape_of(int cols, int64_t rows, int vpt, int most, int per_sm, int nparam, int nin) {
   Shape s;
-  s.tpr = row_threads(cols);
-  const int groups = s.tpr <= 128 ? 256 / s.tpr : 1;
+  s.tpr = row_threads(cols, vpt);
+  const int groups = std::min(16, std::max(1, most / s.tpr));
   s.threads = s.tpr * groups;
-  const int stage = s.threads * 16 * nin * r, par = nparam * cols * 4;
-  // blocks per SM that registers allow (regs_cap_threads threads resident), each with its part of shared memory
-  int per_sm = std::max(1, regs_cap_threads / s.threads);
-  while (per_sm > 1 && par + 2 * stage > kSmemLimit / per_sm) --per_sm;
+  const int stage = s.threads * 16 * nin * vpt, par = nparam * cols * 4;
+  while (per_sm > 1 && par + 3 * stage > kSmemLimit / per_sm) --per_sm;
   s.stages = std::max(2, std::min(4, (kSmemLimit / per_sm - par) / stage));
   // the groups' column sums pass through three rows of the shared memory
   s.smem = std::max(par + s.stages * stage, groups > 1 ? 3 * cols * 4 : 0);
-  s.blocks = (int)std::min<int64_t>((rows + groups * r - 1) / (groups * r), (int64_t)148 * per_sm);
+  s.blocks = (int)std::min<int64_t>(rows, (int64_t)148 * per_sm);
   return s;
 }
 
-Shape backward_shape(const GatedNormParams& p) {
-  return shape_of(p.cols, p.rows, 2, p.y ? 4 : 3, 1, row_threads(p.cols) > 640 ? 1024 : 640);
-}
-
 template <typename Kern>
-cudaError_t run(Kern kern, std::atomic<uint64_t>& ready, const Shape& s, const GatedNormParams& p, cudaStream_t st) {
+cudaError_t run(Kern kern, std::atomic<uint64_t>& ready, const Shape& s, GatedNormParams p, cudaStream_t st) {
   cudaError_t e = allow_smem(kern, kSmemLimit, ready);
   if (e != cudaSuccess) return e;
+  p.tpr = s.tpr;
+  p.stages = s.stages;
   kern<<<s.blocks, s.threads, s.smem, st>>>(p);
   return cudaGetLastError();
 }
 
-template <typename T, typename P, bool HAS_Y, int MAXT>
-cudaError_t forward(GatedNormParams p, cudaStream_t st) {
-  constexpr int R = MAXT > 640 ? 1 : 2;
-  const Shape s = shape_of(p.cols, p.rows, 3, HAS_Y ? 2 : 1, R, MAXT > 640 ? 1024 : 768);
-  p.tpr = s.tpr;
-  p.stages = s.stages;
-  static std::atomic<uint64_t> ready{0};
-  return run(gated_norm_fwd_kernel<T, P, HAS_Y, R, MAXT>, ready, s, p, st);
+// Forward: two vectors a thread (a row's sums then cost half as much per column), up to 640 threads: two
+// rows of 5120 columns at a time, twenty of up to 512.
+template <typename T, typename P, bool Y>
+cudaError_t forward(const GatedNormParams& p, cudaStream_t st) {
+  const Shape s = shape_of(p.cols, p.rows, 2, 640, 1, 3, Y ? 2 : 1);
+  static std::atomic<uint64_t> ready[4];
+  if (s.tpr <= 32) return run(gated_norm_fwd_kernel<T, P, Y, 2, 0, 640>, ready[0], s, p, st);
+  if (s.tpr <= 128) return run(gated_norm_fwd_kernel<T, P, Y, 2, 1, 640>, ready[1], s, p, st);
+  if (s.tpr <= 320) return run(gated_norm_fwd_kernel<T, P, Y, 2, 3, 640>, ready[2], s, p, st);
+  return run(gated_norm_fwd_kernel<T, P, Y, 2, 4, 640>, ready[3], s, p, st);
 }
 
-template <typename T, typename P, bool HAS_Y, int MAXT>
-cudaError_t backward(GatedNormParams p, cudaStream_t st) {
+// Backward: one vector a thread (the column sums take 24 registers of it already).
+Shape backward_shape(const GatedNormParams& p) {
+  const int tpr = row_threads(p.cols, 1);
+  return shape_of(p.cols, p.rows, 1, 256, tpr <= 256 ? 2 : 1, 2, p.y ? 4 : 3);
+}
+template <typename T, typename P, bool Y>
+cudaError_t backward(const GatedNormParams& p, cudaStream_t st) {
   const Shape s = backward_shape(p);
-  p.tpr = s.tpr;
-  p.stages = s.stages;
   if (p.rows > 0) {
-    static std::atomic<uint64_t> ready{0};
-    cudaError_t e = run(gated_norm_bwd_kernel<T, P, HAS_Y, 1, MAXT>, ready, s, p, st);
+    static std::atomic<uint64_t> ready[5];
+    cudaError_t e;
+    if (s.tpr <= 32) e = run(gated_norm_bwd_kernel<T, P, Y, 0, 256, false>, ready[0], s, p, st);
+    else if (s.tpr <= 128) e = run(gated_norm_bwd_kernel<T, P, Y, 1, 256, false>, ready[1], s, p, st);
+    else if (s.tpr <= 256) e = run(gated_norm_bwd_kernel<T, P, Y, 2, 256, false>, ready[2], s, p, st);
+    else if (s.tpr <= 640) e = run(gated_norm_bwd_kernel<T, P, Y, 5, 640, false>, ready[3], s, p, st);
+    else e = run(gated_norm_bwd_kernel<T, P, Y, 8, 1024, true>, ready[4], s, p, st);
     if (e != cudaSuccess) return e;
   }
   if (!p.part) return cudaSuccess;
@@ -585,14 +617,8 @@ cudaError_t backward(GatedNormParams p, cudaStream_t st) {
 
 template <typename T, typename P>
 cudaError_t dispatch(const GatedNormParams& p, bool bwd, cudaStream_t st) {
-  const int threads = row_threads(p.cols);
-  auto go = [&](auto has_y) {
-    constexpr bool Y = decltype(has_y)::value;
-    if (threads <= 256) return bwd ? backward<T, P, Y, 256>(p, st) : forward<T, P, Y, 256>(p, st);
-    if (threads <= 640) return bwd ? backward<T, P, Y, 640>(p, st) : forward<T, P, Y, 640>(p, st);
-    return bwd ? backward<T, P, Y, 1024>(p, st) : forward<T, P, Y, 1024>(p, st);
-  };
-  return p.y ? go(std::true_type{}) : go(std::false_type{});
+  if (bwd) return p.y ? backward<T, P, true>(p, st) : backward<T, P, false>(p, st);
+  return p.y ? forward<T, P, true>(p, st) : forward<T, P, false>(p, st);
 }
 template <typename T>
 cudaError_t dispatch_params(const GatedNormParams& p, bool f32, bool bwd, cudaStream_t st) {

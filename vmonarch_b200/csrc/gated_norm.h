@@ -16,7 +16,8 @@ struct GatedNormParams {
   void *dx, *dy;                     // [rows][cols] dense
   void *dgate, *dscale, *dshift, *dweight, *dpost_weight;  // any may be NULL
   float *part, *seq_part;            // column sums: [blocks + seqs][3][cols], [seqs][cols][2]; NULL: not wanted
-  int64_t rows, x_row, y_row, dx_new_row, dh_row;
+  int64_t rows;                      // below 2^31, as the strides
+  int x_row, y_row, dx_new_row, dh_row;
   int cols, seqs, layer;
   float eps;
   int tpr, stages;                   // set at launch
