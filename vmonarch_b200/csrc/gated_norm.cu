@@ -84,29 +84,29 @@ __device__ __forceinline__ float warp_sum(float v) {
   return v;
 }
 
-// Where the warps of a row meet: two buffers in turn of up to two values a warp (a thread that writes one again
+// Where the warps of a row meet: two buffers in turn of up to three values a warp (a thread that writes one again
 // has passed the barrier of the other since). A group's slots begin at a multiple of four and are padded
 // with zeros to 4 N4, the most warps that a row of this instance has.
 template <int N4>
 struct Meet {
-  float* buf;  // [2][2][kSlots]
+  float* buf;  // [2][3][kSlots]
   int group, tpr, slot, base;
   static constexpr int kSlots = 64;
   __device__ __forceinline__ Meet(float* shared, int tpr_) : buf(shared), tpr(tpr_) {
     group = threadIdx.x / tpr;
     base = group * 4 * N4;
     slot = base + (threadIdx.x - group * tpr) / 32;
-    for (int i = threadIdx.x; i < 4 * kSlots; i += blockDim.x) buf[i] = 0.f;
+    for (int i = threadIdx.x; i < 6 * kSlots; i += blockDim.x) buf[i] = 0.f;
     __syncthreads();
   }
   template <int N>
   __device__ __forceinline__ void sum(float (&v)[N], int& flip) const {
-    static_assert(N <= 2, "two values a meeting");
+    static_assert(N <= 3, "three values a meeting");
 #pragma unroll
     for (int i = 0; i < N; ++i) v[i] = warp_sum(v[i]);
     if constexpr (N4 > 0) {
       float* b = buf + flip;
-      flip ^= 2 * kSlots;
+      flip ^= 3 * kSlots;
       if ((threadIdx.x & 31) == 0)
 #pragma unroll
         for (int i = 0; i < N; ++i) b[i * kSlots + slot] = v[i];
@@ -195,7 +195,7 @@ template <typename T, typename P, bool HAS_Y, int VPT, int N4, int MAXT>
 __global__ void __launch_bounds__(MAXT) gated_norm_fwd_kernel(const __grid_constant__ GatedNormParams p) {
   constexpr int NIN = HAS_Y ? 2 : 1;
   extern __shared__ __align__(16) uint8_t smem[];
-  __shared__ __align__(16) float meeting[4 * Meet<N4>::kSlots];
+  __shared__ __align__(16) float meeting[6 * Meet<N4>::kSlots];
   const int tpr = p.tpr, groups = blockDim.x / tpr;
   const Meet<N4> meet(meeting, tpr);
   int flip = 0, col[VPT];
@@ -256,36 +256,58 @@ __global__ void __launch_bounds__(MAXT) gated_norm_fwd_kernel(const __grid_const
       }
       get = get + stage == end ? ring : get + stage;
       issue();
-      float ry[1] = {1.f}, mean[1] = {0.f}, rx[1] = {0.f};
+      float ry = 1.f, mean = 0.f, rx[1] = {0.f};
       if constexpr (HAS_Y) {
         if (post) {
-          ry[0] = 0.f;
 #pragma unroll
-          for (int v = 0; v < VPT; ++v) ry[0] += dot8(y[v], y[v]);
-          meet.sum(ry, flip);
-          ry[0] = rsqrtf(fmaf(ry[0], inv_c, p.eps));
+          for (int v = 0; v < VPT; ++v) rx[0] += dot8(y[v], y[v]);
         }
 #pragma unroll
         for (int v = 0; v < VPT; ++v)
           if (on[v]) {
             const V8 g = get8(gw + col[v]);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) x[v].v[i] = __ffma2_rn(g.v[i], __fmul2_rn(y[v].v[i], pair(ry[0])), x[v].v[i]);
+            for (int i = 0; i < 4; ++i) y[v].v[i] = __fmul2_rn(y[v].v[i], g.v[i]);
+          }
+        if (post && layer) {
+          // x' = x + ry (g y) is linear in ry, so its mean comes out of the same meeting as ry
+          float t[3] = {rx[0], 0.f, 0.f};
+#pragma unroll
+          for (int v = 0; v < VPT; ++v) {
+            t[1] += sum8(x[v]);
+            t[2] += sum8(y[v]);
+          }
+          meet.sum(t, flip);
+          ry = rsqrtf(fmaf(t[0], inv_c, p.eps));
+          mean = fmaf(t[2], ry, t[1]) * inv_c;
+        } else if (post) {
+          meet.sum(rx, flip);
+          ry = rsqrtf(fmaf(rx[0], inv_c, p.eps));
+        }
+#pragma unroll
+        for (int v = 0; v < VPT; ++v)
+          if (on[v]) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[v].v[i] = __ffma2_rn(y[v].v[i], pair(ry), x[v].v[i]);
             *reinterpret_cast<uint4*>(at<T>(p.x_new, row, p.cols, col[v])) = pack8<T>(x[v]);
           }
       }
       if (layer) {
         // the mean first, then squares of differences: no cancellation where the mean is large
+        if (!post) {
+          rx[0] = 0.f;
 #pragma unroll
-        for (int v = 0; v < VPT; ++v) mean[0] += sum8(x[v]);
-        meet.sum(mean, flip);
-        mean[0] *= inv_c;
+          for (int v = 0; v < VPT; ++v) rx[0] += sum8(x[v]);
+          meet.sum(rx, flip);
+          mean = rx[0] * inv_c;
+        }
 #pragma unroll
         for (int v = 0; v < VPT; ++v)
           if (on[v])
 #pragma unroll
-            for (int i = 0; i < 4; ++i) x[v].v[i] = __fadd2_rn(x[v].v[i], pair(-mean[0]));
+            for (int i = 0; i < 4; ++i) x[v].v[i] = __fadd2_rn(x[v].v[i], pair(-mean));
       }
+      rx[0] = 0.f;
 #pragma unroll
       for (int v = 0; v < VPT; ++v) rx[0] += dot8(x[v], x[v]);
       meet.sum(rx, flip);
@@ -299,8 +321,8 @@ __global__ void __launch_bounds__(MAXT) gated_norm_fwd_kernel(const __grid_const
           for (int i = 0; i < 4; ++i) h.v[i] = __ffma2_rn(__fmul2_rn(x[v].v[i], pair(rx[0])), w.v[i], t.v[i]);
           *reinterpret_cast<uint4*>(at<T>(p.h, row, p.cols, col[v])) = pack8<T>(h);
           if (p.stats && col[v] == 0) {
-            p.stats[row] = ry[0];
-            p.stats[p.rows + row] = mean[0];
+            p.stats[row] = ry;
+            p.stats[p.rows + row] = mean;
             p.stats[2 * p.rows + row] = rx[0];
           }
         }
@@ -316,7 +338,7 @@ template <typename T, typename P, bool HAS_Y, int N4, int MAXT, bool AGAIN>
 __global__ void __launch_bounds__(MAXT) gated_norm_bwd_kernel(const __grid_constant__ GatedNormParams p) {
   constexpr int NIN = HAS_Y ? 4 : 3;  // x, dh, dx', y
   extern __shared__ __align__(16) uint8_t smem[];
-  __shared__ __align__(16) float meeting[4 * Meet<N4>::kSlots];
+  __shared__ __align__(16) float meeting[6 * Meet<N4>::kSlots];
   const int tpr = p.tpr, groups = blockDim.x / tpr;
   const Meet<N4> meet(meeting, tpr);
   const int group = meet.group, col = ((int)threadIdx.x - group * tpr) * 8;
@@ -557,9 +579,11 @@ struct Shape {
 Shape shape_of(int cols, int64_t rows, int vpt, int most, int per_sm, int nparam, int nin) {
   Shape s;
   s.tpr = row_threads(cols, vpt);
-  const int groups = std::min(16, std::max(1, most / s.tpr));
+  int groups = std::min(16, std::max(1, most / s.tpr));
+  const int row = s.tpr * 16 * nin * vpt, par = nparam * cols * 4;
+  while (groups > 1 && par + 2 * groups * row > kSmemLimit) --groups;
   s.threads = s.tpr * groups;
-  const int stage = s.threads * 16 * nin * vpt, par = nparam * cols * 4;
+  const int stage = groups * row;
   while (per_sm > 1 && par + 3 * stage > kSmemLimit / per_sm) --per_sm;
   s.stages = std::max(2, std::min(4, (kSmemLimit / per_sm - par) / stage));
   // the groups' column sums pass through three rows of the shared memory
@@ -578,16 +602,26 @@ cudaError_t run(Kern kern, std::atomic<uint64_t>& ready, const Shape& s, GatedNo
   return cudaGetLastError();
 }
 
-// Forward: two vectors a thread (a row's sums then cost half as much per column), up to 640 threads: two
-// rows of 5120 columns at a time, twenty of up to 512.
+// Forward. Few rows (a serving step: one a block at most): one vector a thread, the shortest way through a row
+// (24 rows of 5120: 5.5 us, with four vectors 7.6 us). Else four vectors a thread: a row's sums then cost a
+// quarter per column, and four rows of 5120 columns are under way on an SM with 640 threads (16576 rows, layer
+// norm with a post norm: 141 us; two vectors and two or three rows 152 us; the floor is 104 us).
 template <typename T, typename P, bool Y>
 cudaError_t forward(const GatedNormParams& p, cudaStream_t st) {
-  const Shape s = shape_of(p.cols, p.rows, 2, 640, 1, 3, Y ? 2 : 1);
-  static std::atomic<uint64_t> ready[4];
-  if (s.tpr <= 32) return run(gated_norm_fwd_kernel<T, P, Y, 2, 0, 640>, ready[0], s, p, st);
-  if (s.tpr <= 128) return run(gated_norm_fwd_kernel<T, P, Y, 2, 1, 640>, ready[1], s, p, st);
-  if (s.tpr <= 320) return run(gated_norm_fwd_kernel<T, P, Y, 2, 3, 640>, ready[2], s, p, st);
-  return run(gated_norm_fwd_kernel<T, P, Y, 2, 4, 640>, ready[3], s, p, st);
+  static std::atomic<uint64_t> ready[8];
+  const int nin = Y ? 2 : 1;
+  if (p.rows <= 148) {
+    const Shape s = shape_of(p.cols, p.rows, 1, 1, 1, 3, nin);
+    if (s.tpr <= 32) return run(gated_norm_fwd_kernel<T, P, Y, 1, 0, 1024>, ready[0], s, p, st);
+    if (s.tpr <= 128) return run(gated_norm_fwd_kernel<T, P, Y, 1, 1, 1024>, ready[1], s, p, st);
+    if (s.tpr <= 256) return run(gated_norm_fwd_kernel<T, P, Y, 1, 2, 1024>, ready[2], s, p, st);
+    if (s.tpr <= 640) return run(gated_norm_fwd_kernel<T, P, Y, 1, 5, 1024>, ready[3], s, p, st);
+    return run(gated_norm_fwd_kernel<T, P, Y, 1, 8, 1024>, ready[4], s, p, st);
+  }
+  const Shape s = shape_of(p.cols, p.rows, 4, 640, 1, 3, nin);
+  if (s.tpr <= 32) return run(gated_norm_fwd_kernel<T, P, Y, 4, 0, 640>, ready[5], s, p, st);
+  if (s.tpr <= 128) return run(gated_norm_fwd_kernel<T, P, Y, 4, 1, 640>, ready[6], s, p, st);
+  return run(gated_norm_fwd_kernel<T, P, Y, 4, 2, 640>, ready[7], s, p, st);
 }
 
 // Backward: one vector a thread (the column sums take 24 registers of it already).
