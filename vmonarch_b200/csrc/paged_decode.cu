@@ -5,10 +5,10 @@
 //
 // Every cached key and value is read once for all the query heads that share it, so the work is bound
 // by memory: 4 D bytes and 4 D group flops a token and key head. The work items (sequence, key
-// head, chunk of up to 8 NT query heads), each a run of 64-token tiles, are laid end to end and every
-// block takes an equal share of the tiles, whatever the sequences' lengths. An item that lies in one
-// block is finished there; one that is cut leaves a partial (max, sum, 32-bit accumulators) per block, which
-// a second kernel joins. Two blocks per SM, about 128 KB of keys and values in flight on each SM.
+// head, chunk of up to 8 NT query heads), each a run of 64-token tiles behind kItemCost units for its start
+// and end, are laid end to end and every block takes an equal share of the units, whatever the
+// sequences' lengths. An item that lies in one block is finished there; one that is cut leaves a partial
+// (max, sum, 32-bit accumulators) per block, which a second kernel joins. Two blocks per SM, about 128 KB of keys and values in flight on each SM.
 //
 // A warp owns 16 tokens of every tile and its own ring of cp.async stages, so the loop has no block-wide
 // synchronisation; the page ids of a stage are fetched one stage before they are needed. Matrix
@@ -29,6 +29,7 @@ namespace {
 
 constexpr int kTile = 64;     // tokens per tile: 16 per warp
 constexpr int kWarps = 4;
+constexpr int kItemCost = 3;  // what an item costs beside its tiles, in tiles
 constexpr int kMinTiles = 4;  // a block's least share: below it the join costs more than the split gains
 
 template <int DP, int NT>
@@ -50,54 +51,62 @@ __device__ __forceinline__ int seq_len(const PagedParams& p, int b) {
   return max(0, min(p.lengths[b], p.max_len));
 }
 
-// The flat order of tiles: sequences, then items (key head, head chunk) of a sequence, then its tiles.
-// Warp-collective: total tiles of one item row summed over sequences, and the sequence that holds `at`.
-__device__ __forceinline__ long long total_tiles(const PagedParams& p, int lane) {
+// The flat order of units: sequences, then items (key head, head chunk) of a sequence, then kItemCost units
+// and the item's tiles.
+__device__ __forceinline__ int units_of(int len) { return kItemCost + tiles_of(len); }
+// Units of one item of every sequence, summed (warp-collective).
+__device__ __forceinline__ long long total_units(const PagedParams& p, int lane) {
   long long sum = 0;
-  for (int b = lane; b < p.batch; b += 32) sum += tiles_of(seq_len(p, b));
+  for (int b = lane; b < p.batch; b += 32) sum += units_of(seq_len(p, b));
 #pragma unroll
   for (int s = 16; s > 0; s >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
   return sum;
 }
-// Blocks that take part: every one has at least kMinTiles tiles.
+// Blocks that take part: every one has at least kMinTiles units.
 __device__ __forceinline__ long long parts_of(const PagedParams& p, long long total) {
   const long long most = (total + kMinTiles - 1) / kMinTiles;
   return most < p.blocks ? most : p.blocks;
 }
 
+// A walk over a block's tiles: `left` units from the tile it stands at to the end of the block's share.
 struct Cursor {
   int seq, item, tile, tiles, len;
+  int left;
 };
-__device__ __forceinline__ void seek(const PagedParams& p, long long at, int lane, Cursor& c) {
+// The first tile at or behind unit `at` (warp-collective).
+__device__ __forceinline__ void seek(const PagedParams& p, long long at, int left, int lane, Cursor& c) {
   long long before = 0;
+  c = Cursor{0, 0, 0, 1, 0, 0};
   for (int b0 = 0; b0 < p.batch; b0 += 32) {
     const int b = b0 + lane;
-    const int t = b < p.batch ? tiles_of(seq_len(p, b)) : 0;
+    const int t = b < p.batch ? units_of(seq_len(p, b)) : 0;
     int incl = t;
 #pragma unroll
     for (int s = 1; s < 32; s <<= 1) {
       const int y = __shfl_up_sync(0xffffffffu, incl, s);
       if (lane >= s) incl += y;
     }
-    const bool here = at < (before + incl) * p.items;
-    const unsigned m = __ballot_sync(0xffffffffu, here);
+    const unsigned m = __ballot_sync(0xffffffffu, at < (before + incl) * p.items);
     if (m) {
-      const int l = __ffs(m) - 1;
-      c.seq = b0 + l;
-      c.tiles = __shfl_sync(0xffffffffu, t, l);
+      const int l = __ffs(m) - 1, units = __shfl_sync(0xffffffffu, t, l);
       const long long rel = at - (before + __shfl_sync(0xffffffffu, incl - t, l)) * p.items;
-      c.item = (int)(rel / c.tiles);
-      c.tile = (int)(rel % c.tiles);
+      const int in = (int)(rel % units) - kItemCost;  // negative: the item's own cost comes first
+      c.seq = b0 + l;
+      c.item = (int)(rel / units);
       c.len = seq_len(p, c.seq);
+      c.tiles = tiles_of(c.len);
+      c.tile = in > 0 ? in : 0;
+      c.left = left + (in < 0 ? in : 0);
       return;
     }
     before += __shfl_sync(0xffffffffu, incl, 31);
   }
-  c = Cursor{0, 0, 0, 1, 0};  // not reached: at < total * items
 }
 __device__ __forceinline__ void advance(const PagedParams& p, Cursor& c) {
+  --c.left;
   if (++c.tile < c.tiles) return;
   c.tile = 0;
+  c.left -= kItemCost;
   if (++c.item < p.items) return;
   c.item = 0;
   if (++c.seq < p.batch) {
@@ -119,28 +128,19 @@ __global__ void __launch_bounds__(32 * kWarps, 2) paged_decode_kernel(const __gr
   float* join_ml = join + kWarps * 8 * C::LD;                       // [warp][8 heads][max, sum]
 
   asm volatile("griddepcontrol.launch_dependents;");
-  long long first, last;  // flat tiles of this block
-  if (p.whole_items) {    // one block per item (short caches): no cut, no join
-    first = last = 0;
-  } else {
-    const long long total = total_tiles(p, lane) * p.items;
-    const long long parts = parts_of(p, total);
-    if (blockIdx.x >= parts) return;
-    first = total * blockIdx.x / parts;
-    last = total * (blockIdx.x + 1) / parts;
-  }
   Cursor cc;
-  if (p.whole_items) {
+  if (p.whole_items) {  // one block per item (short caches): no cut, no join
     cc.seq = blockIdx.x / p.items;
     cc.item = blockIdx.x % p.items;
     cc.tile = 0;
     cc.len = seq_len(p, cc.seq);
-    cc.tiles = tiles_of(cc.len);
-    last = cc.tiles;
+    cc.tiles = cc.left = tiles_of(cc.len);
   } else {
-    seek(p, first, lane, cc);
+    const long long total = total_units(p, lane) * p.items, parts = parts_of(p, total);
+    if (blockIdx.x >= parts) return;
+    const long long first = total * blockIdx.x / parts, last = total * (blockIdx.x + 1) / parts;
+    seek(p, first, (int)(last - first), lane, cc);
   }
-  const int n = (int)(last - first);
 
   // ---- loading: lane l < 16 knows the page and slot of row l of the stage that is issued next
   Cursor lc = cc;
@@ -156,7 +156,7 @@ __global__ void __launch_bounds__(32 * kWarps, 2) paged_decode_kernel(const __gr
     }
   };
   auto issue = [&](int it) {  // stage it % STAGES <- this warp's rows of lc, then on to the next tile
-    if (it < n) {
+    if (lc.left > 0) {
       const uint32_t st = ring + (it % C::STAGES) * C::STAGE;
       const int h = lc.item / p.chunks;
       const T* kh = static_cast<const T*>(p.k) + (int64_t)h * p.k_head;
@@ -173,41 +173,47 @@ __global__ void __launch_bounds__(32 * kWarps, 2) paged_decode_kernel(const __gr
         cp_async16(dst + 16 * DP * 2, vh + pg0 * p.v_page + sl0 * p.v_slot + c0, on ? 16 : 0);
       }
       advance(p, lc);
-      if (it + 1 < n) look_up(lc);
+      if (lc.left > 0) look_up(lc);
     }
     cp_async_commit();
   };
-  look_up(lc);
+  if (lc.left > 0) look_up(lc);
 #pragma unroll
   for (int s = 0; s < C::STAGES - 1; ++s) issue(s);
 
   uint32_t qf[NT][KS][2];
   float acc[NT][KS][4], m[NT][2], l[NT][2];
-  bool fresh = true, from_start = cc.tile == 0;
-  for (int it = 0; it < n; ++it) {
-    if (fresh) {
-      // a new item: its query heads as B fragments (head = lane / 4, columns 2 (lane % 4) ...)
-      fresh = false;
-      const int h = cc.item / p.chunks, g0 = (cc.item % p.chunks) * HEADS;
+  // an item's query heads as B fragments (head = lane / 4, columns 2 (lane % 4) ...)
+  auto load_q = [&](const Cursor& c) {
+    const int h = c.item / p.chunks, g0 = (c.item % p.chunks) * HEADS;
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        const int g = g0 + 8 * nt + lane / 4;
-        const T* q = static_cast<const T*>(p.q) + (int64_t)cc.seq * p.q_row + (int64_t)(h * p.group + g) * p.q_head;
+    for (int nt = 0; nt < NT; ++nt) {
+      const int g = g0 + 8 * nt + lane / 4;
+      const T* q = static_cast<const T*>(p.q) + (int64_t)c.seq * p.q_row + (int64_t)(h * p.group + g) * p.q_head;
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks)
+      for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int c = 16 * ks + 8 * e + 2 * (lane % 4);
-            qf[nt][ks][e] = g < p.group && c < p.dim ? *reinterpret_cast<const uint32_t*>(q + c) : 0u;
-          }
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) acc[nt][ks][e] = 0.f;
-        m[nt][0] = m[nt][1] = -1e30f;
-        l[nt][0] = l[nt][1] = 0.f;
-      }
+        for (int e = 0; e < 2; ++e) {
+          const int col = 16 * ks + 8 * e + 2 * (lane % 4);
+          qf[nt][ks][e] = g < p.group && col < p.dim ? *reinterpret_cast<const uint32_t*>(q + col) : 0u;
+        }
     }
+  };
+  auto clear = [&]() {
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[nt][ks][e] = 0.f;
+      m[nt][0] = m[nt][1] = -1e30f;
+      l[nt][0] = l[nt][1] = 0.f;
+    }
+  };
+  bool from_start = cc.tile == 0;
+  if (cc.left > 0) load_q(cc);
+  clear();
+  for (int it = 0; cc.left > 0; ++it) {
     cp_async_wait<C::STAGES - 2>();
     __syncwarp();
     const uint32_t ks_base = ring + (it % C::STAGES) * C::STAGE, vs_base = ks_base + 16 * DP * 2;
@@ -273,10 +279,13 @@ __global__ void __launch_bounds__(32 * kWarps, 2) paged_decode_kernel(const __gr
     __syncwarp();  // every lane is done with the stage that the next issue refills
     issue(it + C::STAGES - 1);
 
-    const bool to_end = cc.tile + 1 == cc.tiles;
-    if (to_end || it + 1 == n) {
+    const Cursor done = cc;
+    advance(p, cc);
+    const bool to_end = cc.tile == 0;
+    if (to_end || cc.left <= 0) {
       // ---- the four warps' parts of this item (or of this block's share of it)
-      const int h = cc.item / p.chunks, g0 = (cc.item % p.chunks) * HEADS;
+      if (cc.left > 0) load_q(cc);  // of the next item, on its way meanwhile
+      const int h = done.item / p.chunks, g0 = (done.item % p.chunks) * HEADS;
       const bool whole = from_start && to_end;
       const int64_t part = (int64_t)blockIdx.x * 2 + (from_start ? 1 : 0);
 #pragma unroll
@@ -298,7 +307,7 @@ __global__ void __launch_bounds__(32 * kWarps, 2) paged_decode_kernel(const __gr
         __syncthreads();
         for (int i = threadIdx.x; i < 8 * DP; i += 32 * kWarps) {
           const int r = i / DP, d = i % DP, g = g0 + 8 * nt + r;
-          if (g >= p.group) continue;
+          if (g >= p.group) break;  // rows only grow
           float mm = -1e30f, sum = 0.f, o = 0.f;
 #pragma unroll
           for (int w = 0; w < kWarps; ++w) mm = fmaxf(mm, join_ml[(w * 8 + r) * 2]);
@@ -310,9 +319,9 @@ __global__ void __launch_bounds__(32 * kWarps, 2) paged_decode_kernel(const __gr
           }
           const int64_t head = h * p.group + g;
           if (whole) {
-            if (d < p.dim) static_cast<T*>(p.o)[(int64_t)cc.seq * p.o_row + head * p.o_head + d] =
+            if (d < p.dim) static_cast<T*>(p.o)[(int64_t)done.seq * p.o_row + head * p.o_head + d] =
                 Elem<T>::from_f(sum == 0.f ? 0.f : o / sum);
-            if (d == 0 && p.lse) p.lse[(int64_t)cc.seq * p.heads + head] = sum == 0.f ? -INFINITY : (mm + log2f(sum)) * kLn2;
+            if (d == 0 && p.lse) p.lse[(int64_t)done.seq * p.heads + head] = sum == 0.f ? -INFINITY : (mm + log2f(sum)) * kLn2;
           } else {
             p.part[(part * HEADS + 8 * nt + r) * DP + d] = o;
             if (d == 0) *reinterpret_cast<float2*>(p.part_ml + (part * HEADS + 8 * nt + r) * 2) = make_float2(mm, sum);
@@ -320,10 +329,9 @@ __global__ void __launch_bounds__(32 * kWarps, 2) paged_decode_kernel(const __gr
         }
         __syncthreads();
       }
-      fresh = true;
+      clear();
       from_start = true;
     }
-    advance(p, cc);
   }
   cp_async_wait<0>();
 }
@@ -341,7 +349,7 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__
   // where the item lies among the blocks' shares (lengths are inputs: readable before the wait)
   long long total = 0, before = 0;
   for (int b = lane; b < p.batch; b += 32) {
-    const int t = tiles_of(seq_len(p, b));
+    const int t = units_of(seq_len(p, b));
     total += t;
     if (b < seq) before += t;
   }
@@ -352,7 +360,7 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__
   }
   total *= p.items;
   const int tiles = tiles_of(seq_len(p, seq));
-  const long long parts = parts_of(p, total), t0 = before * p.items + (long long)item * tiles;
+  const long long parts = parts_of(p, total), t0 = before * p.items + (long long)item * (kItemCost + tiles) + kItemCost;
   const int c0 = (int)(((t0 + 1) * parts - 1) / total), c1 = (int)(((t0 + tiles) * parts - 1) / total);
   // every block waits, those without work too: the stream's next kernel must find the first one done
   asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -436,8 +444,7 @@ void paged_plan(PagedParams& p) {
   p.items = p.kv_heads * p.chunks;
   const int64_t tiles = (p.max_len + kTile - 1) / kTile;  // most that an item can have
   p.whole_items = tiles <= kMinTiles;
-  const int64_t most = (int64_t)p.batch * p.items * (tiles > 0 ? tiles : 1);
-  p.blocks = p.whole_items ? (int64_t)p.batch * p.items : (most < 2 * 148 ? most : 2 * 148);
+  p.blocks = p.whole_items ? (int64_t)p.batch * p.items : 2 * 148;
 }
 
 int64_t paged_workspace(const PagedParams& p) {
