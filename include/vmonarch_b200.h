@@ -343,7 +343,7 @@ int vmb_packed_fwd(const vmb_packed_args* a, void* stream);
 int vmb_packed_bwd(const vmb_packed_args* a, void* stream);
 
 /*
- * Paged key / value caches (no reference counterpart). A pool holds num_pages pages of page_size slots;
+ * Paged key / value caches (no reference counterpart). A pool holds num_pages >= 1 pages of page_size slots;
  * a page of one tensor is [kv_heads][page_size][dim], anywhere its strides put it (elements, multiples
  * of 8; 16-byte aligned base). dim: a multiple of 8, at most 128.
  */

@@ -89,7 +89,7 @@ def paged(**over):
 
 @pytest.mark.parametrize("over, code", [
     (dict(dtype=2), 1), (dict(dim=12), 2), (dict(dim=256), 2), (dict(heads=5), 1), (dict(kv_heads=0), 1), (dict(page_size=0), 1),
-    (dict(num_pages=-1), 1), (dict(batch=-1), 1), (dict(table_stride=3), 1), (dict(sm_scale=float("inf")), 1),
+    (dict(num_pages=-1), 1), (dict(num_pages=0), 1), (dict(batch=-1), 1), (dict(table_stride=3), 1), (dict(sm_scale=float("inf")), 1),
     (dict(q=N.Rows(8, 256, 64)), 1), (dict(k=N.Pages(256, 2048, 1024, 63)), 1), (dict(lengths=None), 1), (dict(table=None), 1),
     (dict(), 1),  # tables this wide need a workspace
 ])

@@ -26,7 +26,7 @@ bool pages_ok(const vmb_pages& r) {
 int check_pool(const char* what, int64_t num_pages, int kv_heads, int dim, int page_size) {
   if (dim < 8 || dim > 128 || dim % 8)
     return set_error(VMB_ENOTSUP, "%s: head dim %d is not a multiple of 8 up to 128", what, dim);
-  if (kv_heads < 1 || page_size < 1 || num_pages < 0 || num_pages > 0x7fffffff ||
+  if (kv_heads < 1 || page_size < 1 || num_pages < 1 || num_pages > 0x7fffffff ||
       (int64_t)page_size * kv_heads * dim > 0x7fffffff)
     return set_error(VMB_EINVAL, "%s: bad pool sizes", what);
   return VMB_OK;

@@ -10,35 +10,56 @@
 // sequences' lengths. An item that lies in one block is finished there; one that is cut leaves a partial
 // (max, sum, 32-bit accumulators) per block, which a second kernel joins. Two blocks per SM, about 128 KB of keys and values in flight on each SM.
 //
-// A warp owns 16 tokens of every tile and its own ring of cp.async stages, so the loop has no block-wide
-// synchronisation; the page ids of a stage are fetched one stage before they are needed. Matrix
+// A warp owns 16 tokens of every tile and its own ring of TMA stages, so the loop has no block-wide
+// synchronisation. A stage is as few TMA boxes as the page size allows (64 columns x gcd(16, page size) rows: four
+// of them at D = 128 and pages of 16), each issued by a lane that has looked up its page one stage ahead;
+// with per-thread 16-byte copies the addresses cost more issue slots than the arithmetic. Matrix
 // products (mma.sync, m = 16 tokens, n = 8 heads, so a group of up to 8 wastes nothing):
 //   S^T = K Q^T (A from shared memory, B = Q in registers), P^T moved to operand layout by movmatrix,
 //   O^T += V^T P^T (A by transposing loads).
+// tcgen05 would pad a group of 8 heads to 128 rows and pass every score through TMEM; the products here
+// are 16 flops a byte at most, far below what mma.sync does.
 // The four warps meet at the end of an item. P is rounded to 16 bits for the product; scores,
 // exponentials, sums and accumulators are 32-bit.
 //
-// Tokens past the length are not read: their slots arrive as zeros and their scores are dropped, as
-// are the columns between D and the padded width. Page ids outside the pool read as zeros, too.
+// Scores of tokens past the length are dropped; the slots of a last page that hold no token may hold
+// anything, so their value rows are cleared before the product (0 x inf). Pages past the last, page ids outside
+// the pool and columns past D arrive as zeros (coordinates outside the tensor map).
+//
+// Waits for a stage are bounded (sm100.cuh): a block that gives up records a code, drains its copies and
+// leaves its outputs invalid.
+#include <numeric>
+
 #include "common.cuh"
 #include "launch.h"
 #include "paged.h"
+#include "sm100.cuh"
+#include "tma_host.h"
 
 namespace vmb {
+
+__device__ int g_paged_err;
+
 namespace {
+
+using namespace sm100;
 
 constexpr int kTile = 64;     // tokens per tile: 16 per warp
 constexpr int kWarps = 4;
-constexpr int kItemCost = 3;  // what an item costs beside its tiles, in tiles
+constexpr int kItemCost = 2;  // what an item costs beside its tiles, in tiles
 constexpr int kMinTiles = 4;  // a block's least share: below it the join costs more than the split gains
 
 template <int DP, int NT>
 struct Cfg {
   static constexpr int STAGES = DP == 128 ? 3 : 6;
-  static constexpr int STAGE = 2 * 16 * DP * 2;  // K and V of 16 tokens
+  static constexpr int ATOM = 16 * 128;             // 16 tokens x 64 columns, 128-byte swizzle
+  static constexpr int NA = DP / 64;
+  static constexpr int STAGE = 2 * NA * ATOM;       // K atoms, V atoms
   static constexpr int RING = kWarps * STAGES * STAGE;
   static constexpr int LD = DP + 4;              // joined accumulators: 8 heads per warp at a time
-  static constexpr int SMEM = RING + kWarps * 8 * LD * 4 + kWarps * 8 * 2 * 4;
+  static constexpr int JOIN = kWarps * 8 * LD * 4 + kWarps * 8 * 2 * 4;  // accumulators, (max, sum)
+  static constexpr int SMEM = RING + JOIN + kWarps * STAGES * 8 + 16;       // + barriers, abort flag
+  static_assert(2 * (SMEM + 1024) <= 233472, "two blocks per SM");
 };
 
 __device__ __forceinline__ uint32_t movmatrix(uint32_t x) {
@@ -115,19 +136,34 @@ __device__ __forceinline__ void advance(const PagedParams& p, Cursor& c) {
   }
 }
 
+struct KParams {
+  CUtensorMap tm_k, tm_v;  // boxes of 64 columns x box_rows slots; coordinates (column, slot, head, page, 0)
+  PagedParams p;
+};
+
 template <typename T, int DP, int NT>
-__global__ void __launch_bounds__(32 * kWarps, 2) paged_decode_kernel(const __grid_constant__ PagedParams p) {
+__global__ void __launch_bounds__(32 * kWarps, 2) paged_decode_kernel(const __grid_constant__ KParams kp) {
   using C = Cfg<DP, NT>;
-  constexpr int CH = DP / 8;  // 16-byte chunks per row
   constexpr int KS = DP / 16;
   constexpr int HEADS = 8 * NT;
-  extern __shared__ __align__(128) uint8_t smem[];
+  const PagedParams& p = kp.p;
+  extern __shared__ __align__(1024) uint8_t smem[];  // everything shared is in here, so that it starts on an atom
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t ring = smem_u32(smem) + warp * C::STAGES * C::STAGE;
+  const uint32_t bar0 = smem_u32(smem + C::RING + C::JOIN) + 8u * warp * C::STAGES;
   float* join = reinterpret_cast<float*>(smem + C::RING);          // [warp][8 heads][LD]
   float* join_ml = join + kWarps * 8 * C::LD;                       // [warp][8 heads][max, sum]
+  volatile int* abort = reinterpret_cast<int*>(smem + C::RING + C::JOIN + kWarps * C::STAGES * 8);
 
   asm volatile("griddepcontrol.launch_dependents;");
+  if (lane == 0) {
+    if (warp == 0) *abort = 0;
+    for (int s = 0; s < C::STAGES; ++s) mbar_init(bar0 + 8u * s, 1);
+    fence_mbar_init();
+    prefetch_tmap(&kp.tm_k);
+    prefetch_tmap(&kp.tm_v);
+  }
+  __syncthreads();
   Cursor cc;
   if (p.whole_items) {  // one block per item (short caches): no cut, no join
     cc.seq = blockIdx.x / p.items;
@@ -142,40 +178,43 @@ __global__ void __launch_bounds__(32 * kWarps, 2) paged_decode_kernel(const __gr
     seek(p, first, (int)(last - first), lane, cc);
   }
 
-  // ---- loading: lane l < 16 knows the page and slot of row l of the stage that is issued next
+  // ---- loading. A stage's boxes: (row group of box_rows tokens) x (K, V) x atoms; lane i issues boxes i, i + 32.
+  const int boxes = 16 / p.box_rows * 2 * C::NA;
   Cursor lc = cc;
-  int page = -1, slot = 0;
+  int issued = 0;
+  int page[2], slot[2];  // of this lane's boxes of the stage that is issued next
   auto look_up = [&](const Cursor& c) {
-    const int t = c.tile * kTile + 16 * warp + (lane & 15);
-    page = -1;
-    if (t < c.len) {
-      const int i = t / p.page_size;
-      slot = t - i * p.page_size;
-      page = p.table[(int64_t)c.seq * p.table_stride + i];
-      if ((unsigned)page >= (unsigned)p.num_pages) page = -1;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const int box = lane + 32 * k;
+      const int t = c.tile * kTile + 16 * warp + box / (2 * C::NA) * p.box_rows;
+      page[k] = p.num_pages;  // outside the map: zeros
+      slot[k] = 0;
+      if (box < boxes && t < c.len) {
+        const int i = t / p.page_size;
+        slot[k] = t - i * p.page_size;
+        page[k] = p.table[(int64_t)c.seq * p.table_stride + i];
+        if ((unsigned)page[k] >= (unsigned)p.num_pages) page[k] = p.num_pages;
+      }
     }
   };
   auto issue = [&](int it) {  // stage it % STAGES <- this warp's rows of lc, then on to the next tile
-    if (lc.left > 0) {
-      const uint32_t st = ring + (it % C::STAGES) * C::STAGE;
-      const int h = lc.item / p.chunks;
-      const T* kh = static_cast<const T*>(p.k) + (int64_t)h * p.k_head;
-      const T* vh = static_cast<const T*>(p.v) + (int64_t)h * p.v_head;
-      const int chunk = lane % CH;
+    if (lc.left <= 0) return;
+    const uint32_t st = ring + (it % C::STAGES) * C::STAGE, bar = bar0 + 8u * (it % C::STAGES);
+    if (lane == 0) mbar_expect_tx(bar, C::STAGE);
+    ++issued;
+    __syncwarp();
 #pragma unroll
-      for (int i = 0; i < CH / 2; ++i) {
-        const int r = i * (32 / CH) + lane / CH;
-        const int pg = __shfl_sync(0xffffffffu, page, r), sl = __shfl_sync(0xffffffffu, slot, r);
-        const bool on = pg >= 0 && chunk * 8 < p.dim;
-        const int64_t pg0 = on ? pg : 0, sl0 = on ? sl : 0, c0 = on ? chunk * 8 : 0;
-        const uint32_t dst = st + swz<CH>(r, chunk) * 2;
-        cp_async16(dst, kh + pg0 * p.k_page + sl0 * p.k_slot + c0, on ? 16 : 0);
-        cp_async16(dst + 16 * DP * 2, vh + pg0 * p.v_page + sl0 * p.v_slot + c0, on ? 16 : 0);
+    for (int k = 0; k < 2; ++k) {
+      const int box = lane + 32 * k;
+      if (box < boxes) {
+        const int part = box % (2 * C::NA);  // K atoms, then V atoms
+        tma_load(st + part * C::ATOM + box / (2 * C::NA) * p.box_rows * 128, part < C::NA ? &kp.tm_k : &kp.tm_v,
+                 64 * (part % C::NA), slot[k], BIdx(lc.item / p.chunks, page[k], 0), bar);
       }
-      advance(p, lc);
-      if (lc.left > 0) look_up(lc);
     }
-    cp_async_commit();
+    advance(p, lc);
+    if (lc.left > 0) look_up(lc);
   };
   if (lc.left > 0) look_up(lc);
 #pragma unroll
@@ -210,41 +249,55 @@ __global__ void __launch_bounds__(32 * kWarps, 2) paged_decode_kernel(const __gr
       l[nt][0] = l[nt][1] = 0.f;
     }
   };
-  bool from_start = cc.tile == 0;
+  bool from_start = cc.tile == 0, ok = true;
   if (cc.left > 0) load_q(cc);
   clear();
   for (int it = 0; cc.left > 0; ++it) {
-    cp_async_wait<C::STAGES - 2>();
-    __syncwarp();
-    const uint32_t ks_base = ring + (it % C::STAGES) * C::STAGE, vs_base = ks_base + 16 * DP * 2;
+    if (!__all_sync(0xffffffffu, mbar_wait(bar0 + 8u * (it % C::STAGES), (it / C::STAGES) & 1, abort, &g_paged_err, 1))) {
+      ok = false;
+      break;
+    }
+    const uint32_t ks_base = ring + (it % C::STAGES) * C::STAGE, vs_base = ks_base + C::NA * C::ATOM;
     const int left = cc.len - cc.tile * kTile - 16 * warp;  // tokens of this warp's rows
     if (left > 0) {
-      float s[NT][4];
+      if (left < 16) {  // slots without a token: their values enter the product with weight 0
+        for (int i = lane; i < (16 - left) * 8 * C::NA; i += 32) {
+          const int r = left + i / (8 * C::NA), c = i % (8 * C::NA);
+          asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(vs_base + (c >> 3) * C::ATOM + r * 128 + (c & 7) * 16),
+                       "r"(0)
+                       : "memory");
+        }
+        fence_proxy_async_smem();  // the next copy into this stage comes through the async proxy
+        __syncwarp();
+      }
+      float s[NT][2][4];  // two chains of products each
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[nt][e] = 0.f;
+        for (int e = 0; e < 4; ++e) s[nt][0][e] = s[nt][1][e] = 0.f;
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
         uint32_t a[4];
-        ldsm_x4(ks_base + swz<CH>(lane & 15, 2 * ks + (lane >> 4)) * 2, a[0], a[1], a[2], a[3]);
+        const int r = lane & 15, c = (2 * ks + (lane >> 4)) & 7;
+        ldsm_x4(ks_base + (ks >> 2) * C::ATOM + r * 128 + ((c ^ (r & 7)) << 4), a[0], a[1], a[2], a[3]);
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) mma16816<T>(s[nt], a, qf[nt][ks][0], qf[nt][ks][1]);
+        for (int nt = 0; nt < NT; ++nt) mma16816<T>(s[nt][ks & 1], a, qf[nt][ks][0], qf[nt][ks][1]);
       }
       uint32_t pb[NT][2];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         // rows: tokens lane / 4 and + 8; columns: heads 2 (lane % 4) and + 1
+        float x[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          s[nt][e] *= p.scale_log2;
-          if (lane / 4 + 8 * (e >> 1) >= left) s[nt][e] = -INFINITY;
+          x[e] = (s[nt][0][e] + s[nt][1][e]) * p.scale_log2;
+          if (lane / 4 + 8 * (e >> 1) >= left) x[e] = -INFINITY;
         }
-        float mx[2] = {fmaxf(s[nt][0], s[nt][2]), fmaxf(s[nt][1], s[nt][3])};
+        float mx[2] = {fmaxf(x[0], x[2]), fmaxf(x[1], x[3])};
 #pragma unroll
-        for (int x = 4; x < 32; x <<= 1) {
-          mx[0] = fmaxf(mx[0], __shfl_xor_sync(0xffffffffu, mx[0], x));
-          mx[1] = fmaxf(mx[1], __shfl_xor_sync(0xffffffffu, mx[1], x));
+        for (int w = 4; w < 32; w <<= 1) {
+          mx[0] = fmaxf(mx[0], __shfl_xor_sync(0xffffffffu, mx[0], w));
+          mx[1] = fmaxf(mx[1], __shfl_xor_sync(0xffffffffu, mx[1], w));
         }
         if (__any_sync(0xffffffffu, mx[0] > m[nt][0] || mx[1] > m[nt][1])) {
           float al[2];
@@ -261,17 +314,18 @@ __global__ void __launch_bounds__(32 * kWarps, 2) paged_decode_kernel(const __gr
             for (int e = 0; e < 4; ++e) acc[nt][ks][e] *= al[e & 1];
         }
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[nt][e] = fast_exp2(s[nt][e] - m[nt][e & 1]);
-        l[nt][0] += s[nt][0] + s[nt][2];
-        l[nt][1] += s[nt][1] + s[nt][3];
-        pb[nt][0] = movmatrix(Elem<T>::pack(s[nt][0], s[nt][1]));
-        pb[nt][1] = movmatrix(Elem<T>::pack(s[nt][2], s[nt][3]));
+        for (int e = 0; e < 4; ++e) x[e] = fast_exp2(x[e] - m[nt][e & 1]);
+        l[nt][0] += x[0] + x[2];
+        l[nt][1] += x[1] + x[3];
+        pb[nt][0] = movmatrix(Elem<T>::pack(x[0], x[1]));
+        pb[nt][1] = movmatrix(Elem<T>::pack(x[2], x[3]));
       }
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
         // V^T: rows d, columns tokens; matrices (tokens 0-7, 8-15) x (d, d + 8)
         uint32_t a[4];
-        ldsm_x4_t(vs_base + swz<CH>((lane & 7) + 8 * (lane >> 4), 2 * ks + ((lane >> 3) & 1)) * 2, a[0], a[1], a[2], a[3]);
+        const int r = (lane & 7) + 8 * (lane >> 4), c = (2 * ks + ((lane >> 3) & 1)) & 7;
+        ldsm_x4_t(vs_base + (ks >> 2) * C::ATOM + r * 128 + ((c ^ (r & 7)) << 4), a[0], a[1], a[2], a[3]);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) mma16816<T>(acc[nt][ks], a, pb[nt][0], pb[nt][1]);
       }
@@ -333,7 +387,9 @@ __global__ void __launch_bounds__(32 * kWarps, 2) paged_decode_kernel(const __gr
       from_start = true;
     }
   }
-  cp_async_wait<0>();
+  if (!ok) {  // a stage did not arrive in time: the copies under way must land before the block ends
+    for (int i = max(issued - C::STAGES, 0); i < issued; ++i) mbar_wait_drain(bar0 + 8u * (i % C::STAGES), (i / C::STAGES) & 1);
+  }
 }
 
 // Joins the parts of one (sequence, query head): 8 groups of 32 lanes over the parts, 4 columns a lane.
@@ -407,13 +463,21 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__
 }
 
 template <typename T, int DP, int NT>
-cudaError_t launch(PagedParams p, cudaStream_t st) {
+cudaError_t launch(const PagedParams& p, cudaStream_t st) {
   using C = Cfg<DP, NT>;
+  KParams kp{};
+  kp.p = p;
+  auto map = [&](CUtensorMap* m, const void* base, int64_t page, int64_t head, int64_t slot) {
+    return tma::make_map_view(m, base, Elem<T>::is_bf16, p.dim, p.page_size, (int64_t)p.kv_heads * p.num_pages,
+                              View{slot > 0 ? slot : p.dim, head, page, 0}, p.kv_heads, p.num_pages, p.box_rows);
+  };
+  if (!map(&kp.tm_k, p.k, p.k_page, p.k_head, p.k_slot) || !map(&kp.tm_v, p.v, p.v_page, p.v_head, p.v_slot))
+    return cudaErrorInvalidValue;
   auto kern = paged_decode_kernel<T, DP, NT>;
   static std::atomic<uint64_t> ready{0};
   cudaError_t e = allow_smem(kern, C::SMEM, ready);
   if (e != cudaSuccess) return e;
-  kern<<<(unsigned)p.blocks, 32 * kWarps, C::SMEM, st>>>(p);
+  kern<<<(unsigned)p.blocks, 32 * kWarps, C::SMEM, st>>>(kp);
   e = cudaGetLastError();
   if (e != cudaSuccess || p.whole_items) return e;
   // the join starts while the last blocks still run and waits on the device for what they wrote
@@ -442,6 +506,7 @@ void paged_plan(PagedParams& p) {
   p.nt = p.group > 8 ? 2 : 1;  // 8 or 16 query heads share a pass over their keys
   p.chunks = (p.group + 8 * p.nt - 1) / (8 * p.nt);
   p.items = p.kv_heads * p.chunks;
+  p.box_rows = std::gcd(16, p.page_size);
   const int64_t tiles = (p.max_len + kTile - 1) / kTile;  // most that an item can have
   p.whole_items = tiles <= kMinTiles;
   p.blocks = p.whole_items ? (int64_t)p.batch * p.items : 2 * 148;
@@ -457,6 +522,15 @@ cudaError_t paged_decode(PagedParams p, void* workspace, bool bf16, cudaStream_t
   p.part = static_cast<float*>(workspace);
   p.part_ml = p.part + p.blocks * 2 * 8 * p.nt * (p.dim > 64 ? 128 : 64);
   return bf16 ? launch_dim<__nv_bfloat16>(p, st) : launch_dim<__half>(p, st);
+}
+
+cudaError_t paged_status(cudaStream_t st, int* out) {
+  int zero = 0;
+  cudaError_t e = cudaMemcpyFromSymbolAsync(out, g_paged_err, sizeof(int), 0, cudaMemcpyDeviceToHost, st);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(st);
+  if (e == cudaSuccess && *out) e = cudaMemcpyToSymbolAsync(g_paged_err, &zero, sizeof(int), 0, cudaMemcpyHostToDevice, st);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(st);
+  return e;
 }
 
 }  // namespace vmb

@@ -37,7 +37,7 @@ def _check_pools(k_pages, v_pages):
     assert dtype in SUPPORTED_DTYPES and v_pages.dtype == dtype, f"unsupported dtype {dtype}"
     n, h, ps, d = k_pages.shape
     assert 8 <= d <= MAX_DIM and d % 8 == 0, f"head dim {d} is not a multiple of 8 up to {MAX_DIM}"
-    assert h >= 1 and ps >= 1, "pools need at least one head and one slot"
+    assert n >= 1 and h >= 1 and ps >= 1, "pools need at least one page, head and slot"
     assert k_pages.is_cuda and v_pages.device == device, "pools must be on one CUDA device"
     return n, h, ps, d, dtype, device
 
