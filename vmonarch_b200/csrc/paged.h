@@ -17,7 +17,7 @@ struct PagedParams {
   int batch, heads, kv_heads, dim, page_size, num_pages, max_len;
   float scale_log2;
   // set by paged_plan
-  int group, nt, chunks, items, whole_items, box_rows;
+  int group, nt, chunks, items, whole_items, box_rows, join_blocks;
   int64_t blocks;
   float *part, *part_ml;
 };

@@ -392,16 +392,19 @@ __global__ void __launch_bounds__(32 * kWarps, 2) paged_decode_kernel(const __gr
   }
 }
 
-// Joins the parts of one (sequence, query head): 8 groups of 32 lanes over the parts, 4 columns a lane.
+// Joins the parts of one (sequence, query head), or where that would be more blocks than fit at once, of all
+// heads of a (sequence, item): those without work (items in one block, most of a batch's) then cost no
+// second wave. DP / 4 lanes hold a row's columns, four each; the 512 threads' groups of lanes are dealt over the
+// heads, and a head's groups over the parts.
 template <typename T, int DP, int NT>
-__global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__ PagedParams p) {
-  constexpr int HEADS = 8 * NT, LANES = DP / 4, GROUPS = 256 / LANES;
+__global__ void __launch_bounds__(512) paged_join_kernel(const __grid_constant__ PagedParams p) {
+  constexpr int HEADS = 8 * NT, LANES = DP / 4, GROUPS = 512 / LANES;
   __shared__ float4 sum_o[GROUPS][LANES];
   __shared__ float2 sum_ml[GROUPS];
   const int lane = threadIdx.x & 31;
-  const int seq = blockIdx.x / p.heads, head = blockIdx.x % p.heads;
-  const int h = head / p.group, g = head % p.group;
-  const int item = h * p.chunks + g / HEADS, r = g % HEADS;
+  const int seq = blockIdx.x / p.join_blocks, in_seq = blockIdx.x % p.join_blocks;
+  const bool one = p.join_blocks == p.heads;  // a block per head
+  const int item = one ? in_seq / p.group * p.chunks + in_seq % p.group / HEADS : in_seq;
   // where the item lies among the blocks' shares (lengths are inputs: readable before the wait)
   long long total = 0, before = 0;
   for (int b = lane; b < p.batch; b += 32) {
@@ -421,43 +424,49 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__
   // every block waits, those without work too: the stream's next kernel must find the first one done
   asm volatile("griddepcontrol.wait;" ::: "memory");
   if (c0 == c1) return;  // finished by its block
+  const int h = item / p.chunks, g0 = (item % p.chunks) * HEADS, rows = one ? 1 : min(HEADS, p.group - g0);
+  const int grp = threadIdx.x / LANES, d4 = threadIdx.x % LANES, per = GROUPS / rows;
+  const int r = one ? in_seq % p.group - g0 : grp % rows;
+  const int64_t head = (int64_t)h * p.group + g0 + r;
   // block c0 holds the item's start (its second slot), the others continue it (their first)
-  const int grp = threadIdx.x / LANES, d4 = threadIdx.x % LANES;
   auto at = [&](int c) { return ((int64_t)c * 2 + (c == c0 ? 1 : 0)) * HEADS + r; };
   float m = -1e30f, l = 0.f;
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (grp < per * rows) {
 #pragma unroll 4
-  for (int c = c0 + grp; c <= c1; c += GROUPS) {
-    const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + at(c) * 2);
-    const float4 v = reinterpret_cast<const float4*>(p.part + at(c) * DP)[d4];
-    const float mn = fmaxf(m, ml.x), fa = fast_exp2(m - mn), fb = fast_exp2(ml.x - mn);
-    l = l * fa + ml.y * fb;
-    o.x = o.x * fa + v.x * fb;
-    o.y = o.y * fa + v.y * fb;
-    o.z = o.z * fa + v.z * fb;
-    o.w = o.w * fa + v.w * fb;
-    m = mn;
+    for (int c = c0 + grp / rows; c <= c1; c += per) {
+      const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + at(c) * 2);
+      const float4 v = reinterpret_cast<const float4*>(p.part + at(c) * DP)[d4];
+      const float mn = fmaxf(m, ml.x), fa = fast_exp2(m - mn), fb = fast_exp2(ml.x - mn);
+      l = l * fa + ml.y * fb;
+      o.x = o.x * fa + v.x * fb;
+      o.y = o.y * fa + v.y * fb;
+      o.z = o.z * fa + v.z * fb;
+      o.w = o.w * fa + v.w * fb;
+      m = mn;
+    }
   }
   sum_o[grp][d4] = o;
   if (d4 == 0) sum_ml[grp] = make_float2(m, l);
   __syncthreads();
-  if (grp) return;
-  for (int i = 0; i < GROUPS; ++i) m = fmaxf(m, sum_ml[i].x);
+  if (grp >= rows) return;
+  for (int i = 1; i < per; ++i) m = fmaxf(m, sum_ml[grp + i * rows].x);
   l = 0.f;
   o = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int i = 0; i < GROUPS; ++i) {
-    const float f = fast_exp2(sum_ml[i].x - m);
-    l += sum_ml[i].y * f;
-    o.x += sum_o[i][d4].x * f;
-    o.y += sum_o[i][d4].y * f;
-    o.z += sum_o[i][d4].z * f;
-    o.w += sum_o[i][d4].w * f;
+  for (int i = 0; i < per; ++i) {
+    const float f = fast_exp2(sum_ml[grp + i * rows].x - m);
+    const float4 v = sum_o[grp + i * rows][d4];
+    l += sum_ml[grp + i * rows].y * f;
+    o.x += v.x * f;
+    o.y += v.y * f;
+    o.z += v.z * f;
+    o.w += v.w * f;
   }
   if (4 * d4 < p.dim) {
     uint2 w;
     w.x = Elem<T>::pack(o.x / l, o.y / l);
     w.y = Elem<T>::pack(o.z / l, o.w / l);
-    *reinterpret_cast<uint2*>(static_cast<T*>(p.o) + (int64_t)seq * p.o_row + (int64_t)head * p.o_head + 4 * d4) = w;
+    *reinterpret_cast<uint2*>(static_cast<T*>(p.o) + (int64_t)seq * p.o_row + head * p.o_head + 4 * d4) = w;
   }
   if (d4 == 0 && p.lse) p.lse[(int64_t)seq * p.heads + head] = (m + log2f(l)) * kLn2;
 }
@@ -482,8 +491,8 @@ cudaError_t launch(const PagedParams& p, cudaStream_t st) {
   if (e != cudaSuccess || p.whole_items) return e;
   // the join starts while the last blocks still run and waits on the device for what they wrote
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)(p.batch * p.heads));
-  cfg.blockDim = dim3(256);
+  cfg.gridDim = dim3((unsigned)(p.batch * p.join_blocks));
+  cfg.blockDim = dim3(512);
   cfg.stream = st;
   cudaLaunchAttribute attr{};
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -506,6 +515,7 @@ void paged_plan(PagedParams& p) {
   p.nt = p.group > 8 ? 2 : 1;  // 8 or 16 query heads share a pass over their keys
   p.chunks = (p.group + 8 * p.nt - 1) / (8 * p.nt);
   p.items = p.kv_heads * p.chunks;
+  p.join_blocks = (int64_t)p.batch * p.heads <= 4 * 148 ? p.heads : p.items;  // four blocks of 512 threads an SM
   p.box_rows = std::gcd(16, p.page_size);
   const int64_t tiles = (p.max_len + kTile - 1) / kTile;  // most that an item can have
   p.whole_items = tiles <= kMinTiles;
