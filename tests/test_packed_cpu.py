@@ -13,8 +13,21 @@ LENS = [([130], None), ([1, 0, 300, 7], None), ([1, 5, 257, 128, 513], [0, 200, 
 def units(seqs, kind, causal, heads, group):
     """A kernel's unit list as the device holds it (the lists live on the sequences' device)."""
     seqs._list(kind, causal, heads, group)
-    (dev,) = [v[1] for k, v in seqs._cache.items() if k[:2] == (kind, causal)]
-    return dev.numpy().reshape(-1, 12)
+    info, dev = seqs._cache[(kind, causal, heads, group)]
+    u, joins = dev.numpy()[:12 * info.n_units].reshape(-1, 12), dev.numpy()[12 * info.n_units:].reshape(-1, 2)
+    assert len(joins) == info.n_joins and (not len(joins) or info.joins == info.units + 48 * info.n_units)
+    # pieces of cut units: consecutive parts and ranges, each unit joined once; reported as one
+    parts, whole = [], [x for x in u if x[7] < 0]
+    for first, n in joins:
+        mine = sorted((x for x in u if u[first][7] <= x[7] < u[first][7] + n), key=lambda x: x[7])
+        assert len(mine) == n > 1 and all((x[[0, 1, 2, 3, 4, 8]] == mine[0][[0, 1, 2, 3, 4, 8]]).all() for x in mine)
+        assert all(a[6] == b[5] and a[6] > a[5] for a, b in zip(mine, mine[1:]))
+        parts += [x[7] for x in mine]
+        one = mine[0].copy()
+        one[6], one[7] = mine[-1][6], -1
+        whole.append(one)
+    assert sorted(parts) == list(range(info.n_parts))
+    return np.array(whole).reshape(-1, 12)
 
 
 @pytest.mark.parametrize("causal", [False, True])
@@ -64,11 +77,21 @@ def test_key_units_cover_keys_and_the_queries_that_see_them(ql, kl, causal):
     assert (seen == 1).all()
 
 
-def test_longest_work_first():
-    for kind in ("fwd", "dq", "kv"):
-        u = units(PackedSequences([5, 900, 40, 333], device="cpu"), kind, True, 2, 2)
-        work = u[:, 6] - u[:, 5]
-        assert (np.diff(work) <= 0).all()
+def test_longest_work_first_and_cut_to_the_share():
+    """No piece is much above the SMs' fair share of a call's steps, nor below the least worth a piece."""
+    from vmonarch_b200.packed import _LEAST
+    for lens in ([5, 900, 40, 333], [30000], [8000, 100], [200] * 60):
+        for kind in ("fwd", "dq", "kv"):
+            for heads, group in ((2, 2), (40, 5), (1, 1)):
+                seqs = PackedSequences(lens, device="cpu")
+                info = seqs._list(kind, True, heads, group)
+                u = seqs._cache[(kind, True, heads, group)][1].numpy()[:12 * info.n_units].reshape(-1, 12)
+                work = u[:, 6] - u[:, 5]
+                assert (np.diff(work) <= 0).all()
+                blocks = heads // group if kind == "kv" else heads
+                share = max(_LEAST[kind], -(-int(work.sum()) * blocks // 148))
+                assert work.max() <= share + share // 4
+                assert not (u[:, 7] >= 0).any() or work[u[:, 7] >= 0].min() >= share // 2
 
 
 @pytest.mark.parametrize("bad", [dict(lengths=[]), dict(lengths=[3, -1]), dict(lengths=[3], kv_lengths=[1, 2]),

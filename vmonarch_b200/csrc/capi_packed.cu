@@ -13,6 +13,12 @@ namespace {
 
 using vmb::set_error;
 
+int64_t up256(int64_t x);
+// Partial tiles of split units: [parts][heads][rows][64 or 128] fp32, or with dim 0 a (max, sum) pair a row.
+int64_t part_bytes(int64_t parts, int64_t heads, int rows, int dim) {
+  return up256(parts * heads * rows * (dim == 0 ? 2 : dim > 64 ? 128 : 64) * 4);
+}
+
 int64_t up256(int64_t x) { return (x + 255) / 256 * 256; }
 
 int cuda_rc(cudaError_t e, const char* what) {
@@ -58,12 +64,20 @@ int check(const vmb_packed_args* a, const char* what, bool bwd) {
   return VMB_OK;
 }
 
+int workspace(const vmb_packed_args* a, const char* what, int64_t need) {
+  if (need > 0 && (!a->workspace || a->workspace_bytes < need || (reinterpret_cast<uintptr_t>(a->workspace) & 255)))
+    return set_error(VMB_EINVAL, "%s: a 256-byte aligned workspace of %lld bytes needed", what, (long long)need);
+  return VMB_OK;
+}
+
 // Heads whose keys and values (or queries and output gradients) are walked together: as many as keep
 // about 48 MB between them, so that the blocks in flight share them in L2 (126 MB on B200).
 int head_chunk(int64_t bytes_per_head, int heads) {
   const int64_t n = (int64_t(48) << 20) / std::max<int64_t>(bytes_per_head, 1);
   return (int)std::max<int64_t>(1, std::min<int64_t>(n, heads));
 }
+
+int64_t stat_bytes(const vmb_packed_args* a) { return up256(2 * a->heads * a->stat_rows * 4); }
 
 vmb::PackedParams params(const vmb_packed_args* a) {
   vmb::PackedParams p{};
@@ -89,8 +103,8 @@ vmb::PackedParams params(const vmb_packed_args* a) {
 extern "C" {
 
 int64_t vmb_packed_fwd_workspace_bytes(const vmb_packed_args* a) {
-  if (!a || a->heads < 1 || a->units.n_parts < 0) return -1;
-  return 0;
+  if (!a || a->heads < 1 || a->units.n_parts < 0 || a->dim > 128) return -1;
+  return part_bytes(a->units.n_parts, a->heads, 256, a->dim) + part_bytes(a->units.n_parts, a->heads, 256, 0);
 }
 
 int vmb_packed_fwd(const vmb_packed_args* a, void* stream) {
@@ -101,22 +115,28 @@ int vmb_packed_fwd(const vmb_packed_args* a, void* stream) {
   p.units = reinterpret_cast<const vmb::PackedUnit*>(a->units.units);
   p.n_units = a->units.n_units;
   p.head_chunk = std::min(a->heads, p.group * head_chunk(4 * a->k_total * a->dim, a->kv_heads));
-  vmb::count_launches(1);
+  if ((rc = workspace(a, "vmb_packed_fwd", vmb_packed_fwd_workspace_bytes(a)))) return rc;
+  if (a->units.n_parts > 0) {
+    p.joins = a->units.joins;
+    p.n_joins = a->units.n_joins;
+    p.part = static_cast<float*>(a->workspace);
+    p.part_ml = p.part + part_bytes(a->units.n_parts, a->heads, 256, a->dim) / 4;
+  }
+  vmb::count_launches(p.n_joins > 0 ? 2 : 1);
   return cuda_rc(vmb::packed_fwd(p, a->dtype == VMB_DTYPE_BF16, static_cast<cudaStream_t>(stream)), "vmb_packed_fwd");
 }
 
 int64_t vmb_packed_bwd_workspace_bytes(const vmb_packed_args* a) {
-  if (!a || a->heads < 1 || a->stat_rows < 0) return -1;
-  return up256(2 * a->heads * a->stat_rows * 4);
+  if (!a || a->heads < 1 || a->kv_heads < 1 || a->stat_rows < 0 || a->q_units.n_parts < 0 || a->kv_units.n_parts < 0) return -1;
+  return stat_bytes(a) + part_bytes(a->q_units.n_parts, a->heads, 128, a->dim) +
+         part_bytes(a->kv_units.n_parts, 2 * a->kv_heads, 128, a->dim);
 }
 
 int vmb_packed_bwd(const vmb_packed_args* a, void* stream) {
   int rc = check(a, "vmb_packed_bwd", true);
   if (rc) return rc;
   if (a->q_units.n_units == 0 && a->kv_units.n_units == 0) return VMB_OK;
-  const int64_t need = vmb_packed_bwd_workspace_bytes(a);
-  if ((need > 0 && !a->workspace) || a->workspace_bytes < need || (reinterpret_cast<uintptr_t>(a->workspace) & 255))
-    return set_error(VMB_EINVAL, "vmb_packed_bwd: a 256-byte aligned workspace of %lld bytes needed", (long long)need);
+  if ((rc = workspace(a, "vmb_packed_bwd", vmb_packed_bwd_workspace_bytes(a)))) return rc;
   vmb::PackedParams dq = params(a), kv = dq;
   dq.stats = kv.stats = static_cast<float*>(a->workspace);
   dq.units = reinterpret_cast<const vmb::PackedUnit*>(a->q_units.units);
@@ -125,7 +145,13 @@ int vmb_packed_bwd(const vmb_packed_args* a, void* stream) {
   kv.units = reinterpret_cast<const vmb::PackedUnit*>(a->kv_units.units);
   kv.n_units = a->kv_units.n_units;
   kv.head_chunk = head_chunk(4 * a->q_total * a->dim * dq.group, a->kv_heads);
-  vmb::count_launches((dq.n_units > 0 ? 2 : 0) + (kv.n_units > 0 ? 1 : 0));
+  dq.joins = a->q_units.joins;
+  dq.n_joins = a->q_units.n_parts > 0 ? a->q_units.n_joins : 0;
+  dq.part = dq.stats + stat_bytes(a) / 4;
+  kv.joins = a->kv_units.joins;
+  kv.n_joins = a->kv_units.n_parts > 0 ? a->kv_units.n_joins : 0;
+  kv.part = dq.part + part_bytes(a->q_units.n_parts, a->heads, 128, a->dim) / 4;
+  vmb::count_launches((dq.n_units > 0 ? 2 : 0) + (kv.n_units > 0 ? 1 : 0) + (dq.n_joins > 0) + (kv.n_joins > 0));
   return cuda_rc(vmb::packed_bwd(dq, kv, a->dtype == VMB_DTYPE_BF16, static_cast<cudaStream_t>(stream)),
                  "vmb_packed_bwd");
 }

@@ -25,7 +25,8 @@ struct PackedUnit {
 
 struct PackedParams {
   const PackedUnit* units;
-  int n_units;
+  const int32_t* joins;    // (first unit, pieces) of cut units
+  int n_units, n_joins;
   int heads, kv_heads, group, head_chunk;  // head_chunk: (query or kv) heads whose units run together
   int dim, causal;
   int64_t q_total, k_total, stat_rows;     // stat_rows: rows of the padded statistics planes

@@ -112,6 +112,68 @@ __device__ __forceinline__ void store_rows(uint32_t stage, T* out, int64_t rs, i
   }
 }
 
+// 32-column chunks [c0, c1) of an accumulator row to a cut unit's 32-bit partial.
+__device__ __forceinline__ void store_part(uint32_t taddr, float* to, bool any, int c0, int c1) {
+#pragma unroll 1
+  for (int c = c0; c < c1; ++c) {
+    uint32_t v[32];
+    if (any) {
+      tmem_ld32(taddr + c * 32, v);
+      tmem_wait_ld();
+    } else {
+#pragma unroll
+      for (int i = 0; i < 32; ++i) v[i] = 0u;
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      *reinterpret_cast<uint4*>(to + c * 32 + 4 * k) = make_uint4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
+  }
+}
+
+// Adds the pieces of cut units in order: block = (unit, head, matrix, 32 rows), 8 lanes a row, 8 NA columns a
+// lane. KV: dK and dV of key units, else dQ of query units. Partials [part][head][matrix][128][64 NA].
+template <typename T, int NA, bool KV>
+__global__ void __launch_bounds__(256) packed_sum_kernel(const __grid_constant__ PackedParams a) {
+  constexpr int MATS = KV ? 2 : 1;
+  const int heads = KV ? a.kv_heads : a.heads;
+  int64_t b = blockIdx.x;
+  const int rows0 = (int)(b & 3) * 32;
+  b >>= 2;
+  const int mat = (int)(b % MATS);
+  b /= MATS;
+  const int head = (int)(b % heads), join = (int)(b / heads);
+  const PackedUnit u = a.units[a.joins[2 * join]];
+  const int pieces = a.joins[2 * join + 1];
+  const int row = rows0 + (threadIdx.x >> 3), sub = threadIdx.x & 7;
+  if (row >= (KV ? u.k_valid : u.q_valid)) return;
+  float o[8 * NA];
+#pragma unroll
+  for (int i = 0; i < 8 * NA; ++i) o[i] = 0.f;
+#pragma unroll 2
+  for (int k = 0; k < pieces; ++k) {
+    const float4* v = reinterpret_cast<const float4*>(
+        a.part + ((((int64_t)(u.part + k) * heads + head) * MATS + mat) * 128 + row) * (64 * NA) + sub * 8 * NA);
+#pragma unroll
+    for (int i = 0; i < 2 * NA; ++i) {
+      const float4 x = v[i];
+      o[4 * i] += x.x;
+      o[4 * i + 1] += x.y;
+      o[4 * i + 2] += x.z;
+      o[4 * i + 3] += x.w;
+    }
+  }
+  const View& v = !KV ? a.dqv : mat ? a.dvv : a.dkv;
+  T* out = static_cast<T*>(!KV ? a.dq : mat ? a.dv : a.dk) + ((KV ? u.k_row : u.q_row) + row) * v.rs + head * v.s1;
+#pragma unroll
+  for (int g = 0; g < NA; ++g) {
+    const int col = sub * 8 * NA + 8 * g;
+    if (col < a.dim)
+      *reinterpret_cast<uint4*>(out + col) =
+          make_uint4(Elem<T>::pack(o[8 * g], o[8 * g + 1]), Elem<T>::pack(o[8 * g + 2], o[8 * g + 3]),
+                     Elem<T>::pack(o[8 * g + 4], o[8 * g + 5]), Elem<T>::pack(o[8 * g + 6], o[8 * g + 7]));
+  }
+}
+
 // ------------------------------------------------------------------------------------ statistics
 // Block = one 128-query unit of one head; 16 lanes per row, 16 bytes each of o and dO.
 template <typename T>
@@ -379,11 +441,15 @@ __global__ void __launch_bounds__(kThreads, 1) packed_dkdv_kernel(const __grid_c
     tc_fence_after();
     // epilogue: warpgroups 0, 1 stage dK, 2, 3 dV, half of the columns each
     const int mat = wg >> 1;
-    if (ok)
+    if (ok && u.part >= 0)
+      store_part(tmem + lane_off + (mat ? T_DV : T_DK),
+                 p.a.part + ((((int64_t)u.part * p.a.kv_heads + kvh) * 2 + mat) * 128 + row) * (64 * NA), n > 0, (wg & 1) * NA,
+                 ((wg & 1) + 1) * NA);
+    else if (ok)
       stage_rows<T>(tmem + lane_off + (mat ? T_DV : T_DK), sSlots + mat * NA * kAtom, row, n > 0, (wg & 1) * NA,
                     ((wg & 1) + 1) * NA);
     ok = named_bar_and(1, 512, ok && !*abort);
-    if (ok) {
+    if (ok && u.part < 0) {
       T* out = mat ? static_cast<T*>(p.a.dv) + (int64_t)u.k_row * p.a.dvv.rs + (int64_t)kvh * p.a.dvv.s1
                    : static_cast<T*>(p.a.dk) + (int64_t)u.k_row * p.a.dkv.rs + (int64_t)kvh * p.a.dkv.s1;
       store_rows<T, NA>(sSlots + mat * NA * kAtom, out, mat ? p.a.dvv.rs : p.a.dkv.rs, u.k_valid, p.a.dim, tid, 256);
@@ -574,9 +640,15 @@ __global__ void __launch_bounds__(kThreads, 1) packed_dq_kernel(const __grid_con
     if (ok) ok = warp_wait(B_DONE, 0, 64);
     tc_fence_after();
     // epilogue: 16-bit dQ through the idle K ring; a warpgroup stages 32-column chunks wg, wg + 4, ...
-    if (ok && wg < 2 * NA) stage_rows<T>(tmem + lane_off + T_DQ, sK, row, n > 0, wg, wg + 1);
+    if (ok && wg < 2 * NA) {
+      if (u.part >= 0)
+        store_part(tmem + lane_off + T_DQ, p.a.part + (((int64_t)u.part * p.a.heads + head) * 128 + row) * (64 * NA), n > 0, wg,
+                   wg + 1);
+      else
+        stage_rows<T>(tmem + lane_off + T_DQ, sK, row, n > 0, wg, wg + 1);
+    }
     ok = named_bar_and(1, 512, ok && !*abort);
-    if (ok)
+    if (ok && u.part < 0)
       store_rows<T, NA>(sK, static_cast<T*>(p.a.dq) + (int64_t)u.q_row * p.a.dqv.rs + (int64_t)head * p.a.dqv.s1, p.a.dqv.rs,
                         u.q_valid, p.a.dim, tid, 512);
   }
@@ -602,7 +674,7 @@ cudaError_t launch(const PackedParams& dq, const PackedParams& kv, cudaStream_t 
   if (dq.n_units > 0) {
     const int64_t blocks = (int64_t)dq.n_units * dq.heads;
     if (blocks > 0x7fffffff) return cudaErrorInvalidConfiguration;
-    packed_pre_kernel<T><<<(unsigned)blocks, 256, 0, st>>>(dq);
+    packed_pre_kernel<T><<<(unsigned)blocks, 256, 0, st>>>(dq);  // pieces of a cut unit write the same values
     cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return e;
   }
@@ -620,12 +692,17 @@ cudaError_t launch(const PackedParams& dq, const PackedParams& kv, cudaStream_t 
     p.a = kv;
     cudaError_t e = run(packed_dkdv_kernel<T, NA>, DkdvCfg<NA>::SMEM, ready_kv, (int64_t)kv.n_units * kv.kv_heads, p, st);
     if (e != cudaSuccess) return e;
+    if (kv.n_joins > 0) packed_sum_kernel<T, NA, true><<<(unsigned)(kv.n_joins * kv.kv_heads * 8), 256, 0, st>>>(kv);
+    if ((e = cudaGetLastError()) != cudaSuccess) return e;
   }
   if (dq.n_units > 0) {
     if (!map(&p.tm_q, dq.q, dq.q_total, dq.heads, dq.qv, 128) || !map(&p.tm_do, dq.dout, dq.q_total, dq.heads, dq.dov, 128))
       return cudaErrorInvalidValue;
     p.a = dq;
-    return run(packed_dq_kernel<T, NA>, DqCfg<NA>::SMEM, ready_q, (int64_t)dq.n_units * dq.heads, p, st);
+    cudaError_t e = run(packed_dq_kernel<T, NA>, DqCfg<NA>::SMEM, ready_q, (int64_t)dq.n_units * dq.heads, p, st);
+    if (e != cudaSuccess) return e;
+    if (dq.n_joins > 0) packed_sum_kernel<T, NA, false><<<(unsigned)(dq.n_joins * dq.heads * 4), 256, 0, st>>>(dq);
+    return cudaGetLastError();
   }
   return cudaSuccess;
 }

@@ -6,14 +6,20 @@
 // nk - nq + i + 1 (the last query sees the last key). A query that sees no key has o = 0 and
 // lse = -inf.
 //
-// CTA = one head and one unit of up to 256 queries (two 128-row tiles, one per softmax warpgroup) of
-// one sequence. 10 warps: TMA producer, MMA issuer, two warpgroups of softmax and epilogue, thread =
-// query row. The two streams walk the same ring of 128-key tiles and never wait for one another, so
-// one's exponentials run beside the other's matrix products. Online softmax with a lazily raised
+// Work item = one head and one unit of up to 256 queries (two 128-row tiles, one per softmax warpgroup) of
+// one sequence, or a piece of its key tiles. 10 warps: TMA producers, MMA issuer, two warpgroups of softmax and
+// epilogue, thread = query row. The two streams walk the same ring of 128-key tiles and never wait for one
+// another, so one's exponentials run beside the other's matrix products. Online softmax with a lazily raised
 // reference: the exponentials of an unmasked tile go against the current reference and are redone
 // only when a 64-key half's sum passes 2^14. P is 16-bit (the rounding the tensor cores need; l sums
 // the unrounded p), everything else 32-bit.
 // TMEM (512 columns): S_0 [0,128), S_1 [128,256), O_0 [256, +64 NA), O_1 [256 + 64 NA, +64 NA).
+//
+// The grid has a block per work item, and a running block takes over blocks that have not started
+// (clusterlaunchcontrol), most work first: the next item's queries, keys and first scores are under way while the
+// softmax warps write the last item's output straight from registers, and the set-up is paid once per SM.
+// An item that is cut leaves 32-bit partials (max, sum, O), joined by a second kernel; the host cuts
+// where few items would leave SMs without work.
 //
 // The sequences share one tensor, so a tile's rows past the sequence end are the next sequence's.
 // Scores past the end (or after the diagonal) are dropped by index. A value row that no query of the
@@ -53,8 +59,44 @@ struct Cfg {
   static constexpr int NK = NA == 2 ? 3 : 5, NV = NA == 2 ? 2 : 4;
   static constexpr int SMEM = 1024 + (2 + NK + NV) * TILE;
   static_assert(SMEM <= 232448 - 1024, "shared memory budget");
-  static_assert(NK + NV >= 4, "the epilogue stages O and what its rounding leaves, both streams, in the rings");
 };
+
+// 32 bytes to a 32-byte aligned global address (one sector, one store)
+__device__ __forceinline__ void st_global_v8(void* ptr, const uint32_t* v) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(ptr), "r"(v[0]), "r"(v[1]), "r"(v[2]),
+               "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+               : "memory");
+}
+// 32 columns of a row, as 16 packed words; whole sectors where rows are 32-byte aligned. dim: a multiple of 8.
+__device__ __forceinline__ void store_row32(uint16_t* row, int col, int dim, bool sectors, const uint32_t* x) {
+  if (sectors && col + 32 <= dim) {
+    st_global_v8(row + col, x);
+    st_global_v8(row + col + 16, x + 8);
+  } else {
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (col + 8 * k < dim) *reinterpret_cast<uint4*>(row + col + 8 * k) = make_uint4(x[4 * k], x[4 * k + 1], x[4 * k + 2], x[4 * k + 3]);
+  }
+}
+
+// Asks for a block of the grid that has not started: 16 bytes of answer, completing on `bar`.
+__device__ __forceinline__ void request_block(uint32_t answer, uint32_t bar) {
+  asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(answer),
+               "r"(bar)
+               : "memory");
+}
+// The block that the answer names, or -1 when there is none left.
+__device__ __forceinline__ int answered_block(uint32_t answer) {
+  int id;
+  asm volatile(
+      "{\n\t.reg .b128 h;\n\t.reg .pred p;\n\tld.shared.b128 h, [%1];\n\t"
+      "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, h;\n\tmov.b32 %0, -1;\n\t"
+      "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %0, h;\n\t}"
+      : "=r"(id)
+      : "r"(answer)
+      : "memory");
+  return id;
+}
 
 __device__ __forceinline__ float fmax3(float a, float b, float c) {
   float r;
@@ -138,6 +180,24 @@ __device__ __forceinline__ bool clean_row(uint32_t tile, int row) {
   return true;
 }
 
+// A work item as every role sees it: its unit and the key tiles of the two streams.
+struct Item {
+  PackedUnit u;
+  int head, kvh, n_kt[2], n_max, causal;
+  // keys that local query r sees
+  __device__ __forceinline__ int limit(int r) const { return max(0, min(u.k_valid, causal ? u.vis0 + r : u.k_valid)); }
+  __device__ __forceinline__ Item(const PackedParams& a, const PackedUnit& unit, int h) : u(unit), head(h), kvh(h / a.group) {
+    causal = a.causal;
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {  // tiles that stream w's last query sees
+      const int rows = min(u.q_valid - 128 * w, 128);
+      const int tiles = rows > 0 ? (limit(128 * w + rows - 1) + 127) >> 7 : 0;
+      n_kt[w] = max(0, min(tiles, u.end) - u.begin);
+    }
+    n_max = max(n_kt[0], n_kt[1]);
+  }
+};
+
 template <typename T, int NA>
 __global__ void __launch_bounds__(kThreads, 1) packed_fwd_kernel(const __grid_constant__ KParams p) {
   using C = Cfg<NA>;
@@ -148,61 +208,37 @@ __global__ void __launch_bounds__(kThreads, 1) packed_fwd_kernel(const __grid_co
   constexpr uint32_t IDESC_S32 = idesc_f16(kBf16, 128, 32, false, false);  // a last tile of <= 32 keys
   constexpr uint32_t IDESC_PV = idesc_f16(kBf16, 128, 64 * NA, false, true);
   constexpr uint32_t T_O = 256;
+  // barriers: queries full / free, slots full / free, per stream S, first half of P, P, first half of P V, O full,
+  // O free, and the work ring: answer, block known, block read
+  constexpr int B_QFULL = 0, B_QFREE = 1, B_KFULL = 2, B_KFREE = B_KFULL + NK, B_VFULL = B_KFREE + NK, B_VFREE = B_VFULL + NV,
+                B_S = B_VFREE + NV, B_PHALF = B_S + 2, B_PFULL = B_PHALF + 2, B_PVH = B_PFULL + 2, B_OFULL = B_PVH + 2,
+                B_OFREE = B_OFULL + 2, B_ANSWER = B_OFREE + 2, B_WFULL = B_ANSWER + 1, B_WFREE = B_WFULL + 2,
+                NBARS = B_WFREE + 2;
 
   extern __shared__ uint8_t smem_raw[];
-  __shared__ __align__(8) uint64_t bars[11 + 2 * (NK + NV)];
+  __shared__ __align__(16) uint4 answer_sh;
+  __shared__ __align__(8) uint64_t bars[NBARS];
   __shared__ uint32_t tmem_base_sh;
-  __shared__ int abort_sh, dirty_sh;
+  __shared__ int abort_sh, dirty_sh[2];
+  __shared__ struct Work {
+    PackedUnit u;
+    int head;  // -1: no more work
+  } work_sh[2];
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const UnitHead uh = unit_of_block(blockIdx.x, p.a.n_units, p.a.heads, p.a.head_chunk);
-  const PackedUnit u = p.a.units[uh.unit];
-  const int head = uh.head, kvh = head / p.a.group;
-  // keys that local query r sees
-  auto limit = [&](int r) { return max(0, min(u.k_valid, p.a.causal ? u.vis0 + r : u.k_valid)); };
-  // key tiles of stream w: those that its last query sees
-  int n_kt[2];
-#pragma unroll
-  for (int w = 0; w < 2; ++w) {
-    const int rows = min(u.q_valid - 128 * w, 128);
-    const int tiles = rows > 0 ? (limit(128 * w + rows - 1) + 127) >> 7 : 0;
-    n_kt[w] = max(0, min(tiles, u.end) - u.begin);
-  }
-  const int n_max = max(n_kt[0], n_kt[1]);
-  const uint32_t streams = (n_kt[0] > 0) + (n_kt[1] > 0);
-
   const uint32_t sbase = (smem_u32(smem_raw) + 1023u) & ~1023u;
   const uint32_t sQ = sbase, sK = sbase + 2 * TILE, sV = sK + NK * TILE;
   const uint32_t bar0 = smem_u32(bars);
-  const uint32_t BAR_Q = bar0, BAR_DONE = bar0 + 8u;
-  auto BAR_KFULL = [&](int s) { return bar0 + 8u * (2 + s); };
-  auto BAR_VFULL = [&](int s) { return bar0 + 8u * (2 + NK + s); };
-  auto BAR_KEMPTY = [&](int s) { return bar0 + 8u * (2 + NK + NV + s); };
-  auto BAR_VEMPTY = [&](int s) { return bar0 + 8u * (2 + 2 * NK + NV + s); };
-  auto BAR_SFULL = [&](int w) { return bar0 + 8u * (2 + 2 * (NK + NV) + w); };
-  auto BAR_PHALF = [&](int w) { return bar0 + 8u * (4 + 2 * (NK + NV) + w); };
-  auto BAR_PFULL = [&](int w) { return bar0 + 8u * (6 + 2 * (NK + NV) + w); };
-  auto BAR_PVH = [&](int w) { return bar0 + 8u * (8 + 2 * (NK + NV) + w); };
+  auto BAR = [&](int i) { return bar0 + 8u * (uint32_t)i; };
   volatile int* abort = &abort_sh;
 
   if (threadIdx.x == 0) {
     abort_sh = 0;
-    dirty_sh = 0;
-    mbar_init(BAR_Q, 1);
-    mbar_init(BAR_DONE, 1);
-    for (int s = 0; s < NK; ++s) {
-      mbar_init(BAR_KFULL(s), 1);
-      mbar_init(BAR_KEMPTY(s), max(streams, 1u));
-    }
-    for (int s = 0; s < NV; ++s) {
-      mbar_init(BAR_VFULL(s), 1);
-      mbar_init(BAR_VEMPTY(s), max(streams, 1u));
-    }
-    for (int w = 0; w < 2; ++w) {
-      mbar_init(BAR_SFULL(w), 1);
-      mbar_init(BAR_PHALF(w), 128);
-      mbar_init(BAR_PFULL(w), 128);
-      mbar_init(BAR_PVH(w), 1);
+    dirty_sh[0] = dirty_sh[1] = 0;
+    for (int i = 0; i < NBARS; ++i) {
+      const bool rows = (i >= B_PHALF && i < B_PVH) || i == B_OFREE || i == B_OFREE + 1;
+      // a block id is read by the V producer, the MMA warp and eight softmax warps
+      mbar_init(BAR(i), rows ? 128 : i >= B_WFREE ? 10 : 1);
     }
     fence_mbar_init();
   }
@@ -215,93 +251,172 @@ __global__ void __launch_bounds__(kThreads, 1) packed_fwd_kernel(const __grid_co
   tc_fence_after();
   const uint32_t tmem = tmem_base_sh;
 
+  // Item 0 is this block's own, from global memory; the K producer hands the others on through work_sh.
+  auto own_work = [&](int block) -> Work {
+    const UnitHead uh = unit_of_block(block, p.a.n_units, p.a.heads, p.a.head_chunk);
+    return Work{p.a.units[uh.unit], uh.head};
+  };
+  auto work_wait = [&](int i, int code) -> bool {
+    return mbar_wait(BAR(B_WFULL + (i & 1)), ((i - 1) >> 1) & 1, abort, &g_packed_err, code);
+  };
+  // for a whole warp; head -1: no more work (or a failed wait)
+  auto next_work = [&](int i, int code) -> Work {
+    if (i == 0) return own_work(blockIdx.x);
+    if (!__all_sync(0xffffffffu, work_wait(i, code))) return Work{PackedUnit{}, -1};
+    const Work w = work_sh[i & 1];
+    __syncwarp();
+    if (lane == 0) mbar_arrive(BAR(B_WFREE + (i & 1)));
+    return w;
+  };
+
   if (warp == 0) {
     // ------------------------------------------------------------------ TMA producers
-    // lane 0: Q, then the K ring; lane 1: the V ring
-    if (lane < 2 && n_max > 0) {
+    // lane 0: work ring, Q and the K ring; lane 1: the V ring
+    if (lane < 2) {
       const bool kl = lane == 0;
       const int nslot = kl ? NK : NV;
       const CUtensorMap* map = kl ? &p.tm_k : &p.tm_v;
       prefetch_tmap(map);
-      if (kl) {
-        mbar_expect_tx(BAR_Q, streams * TILE);
-        for (int w = 0; w < 2; ++w)
-          if (n_kt[w] > 0)
-            for (int a = 0; a < NA; ++a)
-              tma_load(sQ + w * TILE + a * kAtom, &p.tm_q, 64 * a, u.q_row + 128 * w, BIdx(head, 0, 0), BAR_Q);
+      int tiles = 0, queries = 0, asked = 0;  // loaded so far by this lane; answers asked for
+      bool ok = true;
+      Work work = own_work(blockIdx.x);
+      for (int i = 0; ok && work.head >= 0; ++i) {
+        if (kl) {  // ask for the item after this one, long before it is needed
+          fence_proxy_async_smem();
+          mbar_expect_tx(BAR(B_ANSWER), 16);
+          request_block(smem_u32(&answer_sh), BAR(B_ANSWER));
+          ++asked;
+        }
+        const Item it(p.a, work.u, work.head);
+        if (kl && it.n_max > 0) {
+          if (queries > 0) ok = mbar_wait(BAR(B_QFREE), (queries - 1) & 1, abort, &g_packed_err, 1);
+          if (!ok) break;
+          mbar_expect_tx(BAR(B_QFULL), ((it.n_kt[0] > 0) + (it.n_kt[1] > 0)) * TILE);
+          for (int w = 0; w < 2; ++w)
+            if (it.n_kt[w] > 0)
+              for (int a = 0; a < NA; ++a)
+                tma_load(sQ + w * TILE + a * kAtom, &p.tm_q, 64 * a, it.u.q_row + 128 * w, BIdx(it.head, 0, 0), BAR(B_QFULL));
+          ++queries;
+        }
+        for (int t = 0; t < it.n_max; ++t, ++tiles) {
+          const int s = tiles % nslot;
+          if (tiles >= nslot &&
+              !mbar_wait(BAR((kl ? B_KFREE : B_VFREE) + s), ((tiles / nslot) - 1) & 1, abort, &g_packed_err, 1)) {
+            ok = false;
+            break;
+          }
+          const uint32_t full = BAR((kl ? B_KFULL : B_VFULL) + s), slot = (kl ? sK : sV) + s * TILE;
+          const int row = it.u.k_row + (it.u.begin + t) * 128;
+          mbar_expect_tx(full, TILE);
+          for (int a = 0; a < NA; ++a) tma_load(slot + a * kAtom, map, 64 * a, row, BIdx(it.kvh, 0, 0), full);
+          if (t + nslot < it.n_max)  // the tile one ring ahead into L2
+            for (int a = 0; a < NA; ++a) tma_prefetch(map, 64 * a, row + nslot * 128, BIdx(it.kvh, 0, 0));
+        }
+        if (!ok) break;
+        if (kl) {
+          const int n = i + 1;
+          ok = mbar_wait(BAR(B_ANSWER), i & 1, abort, &g_packed_err, 1) &&
+               (n < 3 || mbar_wait(BAR(B_WFREE + (n & 1)), ((n - 3) >> 1) & 1, abort, &g_packed_err, 1));
+          if (!ok) break;
+          const int block = answered_block(smem_u32(&answer_sh));
+          work.head = -1;
+          if (block >= 0) work = own_work(block);
+          work_sh[n & 1] = work;
+          mbar_arrive(BAR(B_WFULL + (n & 1)));
+        } else {
+          if (!(ok = work_wait(i + 1, 1))) break;
+          work = work_sh[(i + 1) & 1];
+          mbar_arrive(BAR(B_WFREE + ((i + 1) & 1)));
+        }
       }
-      int armed[NK > NV ? NK : NV];
-      for (int s = 0; s < nslot; ++s) armed[s] = 0;
-      for (int t = 0; t < n_max; ++t) {
-        const int s = t % nslot;
-        if (t >= nslot && !mbar_wait(kl ? BAR_KEMPTY(s) : BAR_VEMPTY(s), ((t / nslot) - 1) & 1, abort, &g_packed_err, 1))
-          break;
-        const uint32_t full = kl ? BAR_KFULL(s) : BAR_VFULL(s);
-        const uint32_t slot = (kl ? sK : sV) + s * TILE;
-        const int row = u.k_row + (u.begin + t) * 128;
-        mbar_expect_tx(full, TILE);
-        for (int a = 0; a < NA; ++a) tma_load(slot + a * kAtom, map, 64 * a, row, BIdx(kvh, 0, 0), full);
-        if (t + nslot < n_max)  // the tile one ring ahead into L2
-          for (int a = 0; a < NA; ++a) tma_prefetch(map, 64 * a, row + nslot * 128, BIdx(kvh, 0, 0));
-        armed[s] = t / nslot + 1;
-      }
-      // drain: every armed phase must have landed before the CTA may exit
-      if (kl) mbar_wait_drain(BAR_Q, 0);
-      for (int s = 0; s < nslot; ++s)
-        if (armed[s] > 0) mbar_wait_drain(kl ? BAR_KFULL(s) : BAR_VFULL(s), (armed[s] - 1) & 1);
+      // drain: what was asked for must have landed before the CTA may exit
+      if (kl && queries > 0) mbar_wait_drain(BAR(B_QFULL), (queries - 1) & 1);
+      if (kl && asked > 0) mbar_wait_drain(BAR(B_ANSWER), (asked - 1) & 1);
+      for (int t = max(tiles - nslot, 0); t < tiles; ++t)
+        mbar_wait_drain(BAR((kl ? B_KFULL : B_VFULL) + t % nslot), (t / nslot) & 1);
     }
   } else if (warp == 1) {
     // ------------------------------------------------------------------ MMA issuer
     const uint32_t leader = elect_one() ? 1u : 0u;
-    auto wwait = [&](uint32_t bar, uint32_t parity, int code) -> bool {
-      return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort, &g_packed_err, code));
+    auto wwait = [&](int bar, uint32_t parity, int code) -> bool {
+      return __all_sync(0xffffffffu, mbar_wait(BAR(bar), parity, abort, &g_packed_err, code));
     };
-    // keys of stream w's tile t that some of its queries sees (MMAs of <= 32 keys are shortened)
-    auto tile_keys = [&](int w, int t) {
-      return limit(min(u.q_valid, 128 * (w + 1)) - 1) - (u.begin + t) * 128;
-    };
-    auto issue_s = [&](int w, int t) -> bool {
-      const int s = t % NK;
-      if (!wwait(BAR_KFULL(s), (t / NK) & 1, 2)) return false;
-      tc_fence_after();
-      const uint32_t kb = sK + s * TILE, qb = sQ + w * TILE;
-      const uint32_t idesc = tile_keys(w, t) <= 32 ? IDESC_S32 : IDESC_S;
+    int ring = 0, queries = 0, steps[2] = {0, 0}, outs[2] = {0, 0};  // tiles, units and per-stream tiles and units so far
+    bool ok = true;
+    for (int i = 0; ok; ++i) {
+      const Work work = next_work(i, 2);
+      if (work.head < 0) break;
+      const Item it(p.a, work.u, work.head);
+      if (it.n_max == 0) continue;
+      // keys of stream w's tile t that some of its queries sees (MMAs of <= 32 keys are shortened)
+      auto tile_keys = [&](int w, int t) {
+        return it.limit(min(it.u.q_valid, 128 * (w + 1)) - 1) - (it.u.begin + t) * 128;
+      };
+      auto last_of = [&](int w, int t) { return w == 1 || t >= it.n_kt[1]; };  // no later stream uses tile t
+      auto issue_s = [&](int w, int t) -> bool {
+        const int s = (ring + t) % NK;
+        if (!wwait(B_KFULL + s, ((ring + t) / NK) & 1, 2)) return false;
+        tc_fence_after();
+        const uint32_t kb = sK + s * TILE, qb = sQ + w * TILE;
+        const uint32_t idesc = tile_keys(w, t) <= 32 ? IDESC_S32 : IDESC_S;
 #pragma unroll
-      for (int kk = 0; kk < 4 * NA; ++kk) {
-        const uint32_t off = (kk >> 2) * kAtom + (kk & 3) * 32;
-        mma_ss_if(leader, tmem + 128 * w, smem_desc_sw128(qb + off, 16, 1024), smem_desc_sw128(kb + off, 16, 1024), idesc,
-                  kk > 0);
+        for (int kk = 0; kk < 4 * NA; ++kk) {
+          const uint32_t off = (kk >> 2) * kAtom + (kk & 3) * 32;
+          mma_ss_if(leader, tmem + 128 * w, smem_desc_sw128(qb + off, 16, 1024), smem_desc_sw128(kb + off, 16, 1024), idesc,
+                    kk > 0);
+        }
+        mma_commit_if(leader, BAR(B_S + w));
+        if (last_of(w, t)) {
+          mma_commit_if(leader, BAR(B_KFREE + s));
+          if (t + 1 == it.n_max) mma_commit_if(leader, BAR(B_QFREE));
+        }
+        return true;
+      };
+      ok = wwait(B_QFULL, queries & 1, 2);
+      ++queries;
+      for (int w = 0; w < 2; ++w)
+        if (ok && it.n_kt[w] > 0) ok = issue_s(w, 0);
+      for (int j = 0; ok && j < 2 * it.n_max; ++j) {
+        const int w = j & 1, t = j >> 1;
+        if (t >= it.n_kt[w]) continue;
+        const int c = steps[w] + t, sv = (ring + t) % NV;
+        const uint32_t vb = sV + sv * TILE;
+        const uint32_t a_tm = tmem + 128 * w, o_tm = tmem + T_O + 64 * NA * w;
+        const int ksteps = tile_keys(w, t) <= 32 ? 2 : 8;  // 16 keys per step
+        if (!(ok = wwait(B_PHALF + w, c & 1, 4) && wwait(B_VFULL + sv, ((ring + t) / NV) & 1, 4))) break;
+        // the stream's O of the last unit has been read
+        if (t == 0 && outs[w] > 0 && !(ok = wwait(B_OFREE + w, (outs[w] - 1) & 1, 4))) break;
+        tc_fence_after();
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk)
+          mma_ts_if(leader & (kk < ksteps ? 1u : 0u), o_tm, a_tm + kk * 8, smem_desc_sw128(vb + kk * 2048, kAtom, 1024),
+                    IDESC_PV, (t > 0 || kk > 0) ? 1u : 0u);
+        mma_commit_if(leader, BAR(B_PVH + w));  // a softmax that rescales O mid-tile waits for it
+        if (!(ok = wwait(B_PFULL + w, c & 1, 4))) break;
+        tc_fence_after();
+#pragma unroll
+        for (int kk = 4; kk < 8; ++kk)
+          mma_ts_if(leader & (kk < ksteps ? 1u : 0u), o_tm, a_tm + kk * 8, smem_desc_sw128(vb + kk * 2048, kAtom, 1024),
+                    IDESC_PV, 1u);
+        if (last_of(w, t)) mma_commit_if(leader, BAR(B_VFREE + sv));
+        if (t + 1 < it.n_kt[w]) ok = issue_s(w, t + 1);
+        else mma_commit_if(leader, BAR(B_OFULL + w));
       }
-      mma_commit_if(leader, BAR_SFULL(w));
-      return true;
-    };
-    bool ok = n_max == 0 || wwait(BAR_Q, 0, 2);
-    for (int w = 0; w < 2; ++w)
-      if (ok && n_kt[w] > 0) ok = issue_s(w, 0);
-    for (int j = 0; ok && j < 2 * n_max; ++j) {
-      const int w = j & 1, t = j >> 1;
-      if (t >= n_kt[w]) continue;
-      const uint32_t vb = sV + (t % NV) * TILE;
-      const uint32_t a_tm = tmem + 128 * w, o_tm = tmem + T_O + 64 * NA * w;
-      const int ksteps = tile_keys(w, t) <= 32 ? 2 : 8;  // 16 keys per step
-      if (!wwait(BAR_PHALF(w), t & 1, 4) || !wwait(BAR_VFULL(t % NV), (t / NV) & 1, 4)) break;
-      tc_fence_after();
-#pragma unroll
-      for (int kk = 0; kk < 4; ++kk)
-        mma_ts_if(leader & (kk < ksteps ? 1u : 0u), o_tm, a_tm + kk * 8, smem_desc_sw128(vb + kk * 2048, kAtom, 1024),
-                  IDESC_PV, (t > 0 || kk > 0) ? 1u : 0u);
-      mma_commit_if(leader, BAR_PVH(w));  // a softmax that rescales O mid-tile waits for it
-      if (!wwait(BAR_PFULL(w), t & 1, 4)) break;
-      tc_fence_after();
-#pragma unroll
-      for (int kk = 4; kk < 8; ++kk)
-        mma_ts_if(leader & (kk < ksteps ? 1u : 0u), o_tm, a_tm + kk * 8, smem_desc_sw128(vb + kk * 2048, kAtom, 1024),
-                  IDESC_PV, 1u);
-      if (t + 1 < n_kt[w]) ok = issue_s(w, t + 1);
+      ring += it.n_max;
+      for (int w = 0; w < 2; ++w) {
+        steps[w] += it.n_kt[w];
+        outs[w] += it.n_kt[w] > 0;
+      }
     }
-    if (elect_one()) {  // DONE: every MMA complete (the epilogue reads O; TMEM may be freed)
-      mma_commit(BAR_DONE);
-      mbar_wait_drain(BAR_DONE, 0);
+    // every MMA issued must be complete before TMEM can be freed: one more round of the queries' barrier
+    __syncwarp();
+    if (elect_one()) {
+      __shared__ __align__(8) uint64_t done_sh;
+      const uint32_t done = smem_u32(&done_sh);
+      mbar_init(done, 1);
+      fence_mbar_init();
+      mma_commit(done);
+      mbar_wait_drain(done, 0);
     }
     __syncwarp();
   } else {
@@ -311,188 +426,190 @@ __global__ void __launch_bounds__(kThreads, 1) packed_fwd_kernel(const __grid_co
     const int row = quad * 32 + lane;
     const uint32_t lane_off = (uint32_t)(quad * 32) << 16;
     const uint32_t tS = tmem + lane_off + 128 * w, tO = tmem + lane_off + T_O + 64 * NA * w;
-    const int my_lim = limit(128 * w + row);
-    const int lim_lo = limit(128 * w), lim_hi = limit(min(u.q_valid, 128 * (w + 1)) - 1);
-    float m_ref = -1e30f, l = 0.f;
+    auto warp_wait = [&](int bar, uint32_t parity, int code) -> bool {
+      return __all_sync(0xffffffffu, mbar_wait(BAR(bar), parity, abort, &g_packed_err, code));
+    };
+    const bool sectors = ((p.a.ov.rs | p.a.ov.s1 | p.a.olv.rs | p.a.olv.s1) & 15) == 0 &&
+                         ((reinterpret_cast<uintptr_t>(p.a.o) | reinterpret_cast<uintptr_t>(p.a.o_low)) & 31) == 0;
+    int steps = 0, outs = 0, ring = 0;  // tiles and units of this stream so far, tiles of the ring
     bool ok = true;
-    auto warp_wait = [&](uint32_t bar, uint32_t parity, int code) -> bool {
-      return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort, &g_packed_err, code));
-    };
-    // O and l to the reference max(m_ref, mx). Warp-uniform; no P V into O_w may be in flight.
-    auto rescale = [&](float mx) {
-      const float m_new = fmaxf(m_ref, mx);
-      const float alpha = fast_exp2(m_ref - m_new);
+    for (int i = 0; ok; ++i) {
+      const Work work = next_work(i, 8);
+      if (work.head < 0) break;
+      const Item it(p.a, work.u, work.head);
+      const PackedUnit& u = it.u;
+      const int n_kt = it.n_kt[w];
+      const int my_lim = it.limit(128 * w + row);
+      const int lim_lo = it.limit(128 * w), lim_hi = it.limit(min(u.q_valid, 128 * (w + 1)) - 1);
+      float m_ref = -1e30f, l = 0.f;
+      // O and l to the reference max(m_ref, mx). Warp-uniform; no P V into O_w may be in flight.
+      auto rescale = [&](float mx) {
+        const float m_new = fmaxf(m_ref, mx);
+        const float alpha = fast_exp2(m_ref - m_new);
 #pragma unroll 1
-      for (int c = 0; c < 2 * NA; ++c) {
-        uint32_t o[32];
-        tmem_ld32(tO + c * 32, o);
-        tmem_wait_ld();
-#pragma unroll
-        for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
-        tmem_st32(tO + c * 32, o);
-      }
-      tmem_wait_st();
-      l *= alpha;
-      m_ref = m_new;
-    };
-
-    for (int t = 0; t < n_kt[w]; ++t) {
-      if (!warp_wait(BAR_SFULL(w), t & 1, 8)) { ok = false; break; }
-      tc_fence_after();
-      if (warp == 2 + 4 * w && lane == 0) {
-        // S_w(t) complete, so is P V_w(t - 1) before it: K(t) and V(t - 1) are free of this stream
-        mbar_arrive(BAR_KEMPTY(t % NK));
-        if (t >= 1) mbar_arrive(BAR_VEMPTY((t - 1) % NV));
-      }
-      const int k0 = (u.begin + t) * 128;
-      const bool full = lim_lo - k0 >= 128;  // no query of the stream misses a key of the tile
-      if (t > 0 && full) {
-        // the exponentials against the current reference; a half past the threshold is redone from
-        // the scores in registers, after the rescale
-#pragma unroll
-        for (int hf = 0; hf < 2; ++hf) {
-          uint32_t s[64], pk[32];
-          tmem_ld32(tS + 64 * hf, s);
-          tmem_ld32(tS + 64 * hf + 32, s + 32);
-          tmem_wait_ld();
-          float lt = probs<T, 64, false>(s, pk, p.scale_log2, m_ref, 64);
-          if (__any_sync(0xffffffffu, !(lt <= kSumThreshold))) {
-            // first half: S_w(t) complete implies every earlier P V is; second: the first half's P V
-            if (hf == 1 && !warp_wait(BAR_PVH(w), t & 1, 16)) { ok = false; break; }
-            tc_fence_after();
-            rescale(row_max<64, false>(s, 64) * p.scale_log2);
-            lt = probs<T, 64, false>(s, pk, p.scale_log2, m_ref, 64);
-          }
-          l += lt;
-          tmem_st32(tS + 32 * hf, pk);
-          if (hf == 0) {
-            tmem_wait_st();
-            tc_fence_before();
-            mbar_arrive(BAR_PHALF(w));
-          }
-        }
-        if (!ok) break;
-      } else {
-        // the first tile (sets the reference) and the masked ones: the maximum first
-        const int valid = my_lim - k0;
-        uint32_t sr[128];
-        tmem_ld32(tS, sr);
-        tmem_ld32(tS + 32, sr + 32);
-        tmem_ld32(tS + 64, sr + 64);
-        tmem_ld32(tS + 96, sr + 96);
-        if (!full) {
-          // values that some query must not see: clear what is not finite (thread = key row)
-          if (!warp_wait(BAR_VFULL(t % NV), (t / NV) & 1, 8)) { ok = false; break; }
-          if (clean_row<T, NA>(sV + (t % NV) * TILE, row)) dirty_sh = 1;
-        }
-        tmem_wait_ld();
-        const float mx = (full ? row_max<128, false>(sr, 128) : row_max<128, true>(sr, valid)) * p.scale_log2;
-        if (t == 0) m_ref = mx;
-        else if (__any_sync(0xffffffffu, mx > m_ref + kRescaleThreshold)) rescale(mx);
-        {
-          const uint32_t(&sh)[64] = *reinterpret_cast<const uint32_t(*)[64]>(&sr[0]);
-          uint32_t pk[32];
-          if (full) l += probs<T, 64, false>(sh, pk, p.scale_log2, m_ref, 64);
-          else l += probs<T, 64, true>(sh, pk, p.scale_log2, m_ref, valid);
-          tmem_st32(tS, pk);
-          tmem_wait_st();
-          tc_fence_before();
-          mbar_arrive(BAR_PHALF(w));
-        }
-        {
-          // the second half is loaded again (only its own P overwrites it), so that the first half's
-          // scores alone live through the exponentials
-          uint32_t pk[32];
-          if (lim_hi - k0 > 64) {
-            uint32_t sh[64];
-            tmem_ld32(tS + 64, sh);
-            tmem_ld32(tS + 96, sh + 32);
-            tmem_wait_ld();
-            if (full) l += probs<T, 64, false>(sh, pk, p.scale_log2, m_ref, 64);
-            else l += probs<T, 64, true>(sh, pk, p.scale_log2, m_ref, valid - 64);
-          } else {
-#pragma unroll
-            for (int i = 0; i < 32; ++i) pk[i] = 0u;
-          }
-          tmem_st32(tS + 32, pk);
-        }
-      }
-      tmem_wait_st();
-      tc_fence_before();
-      mbar_arrive(BAR_PFULL(w));
-    }
-
-    // epilogue: O / l in 16 bits (and for a backward the rest that the rounding leaves, 16 bits more)
-    // through the idle rings, whole rows to global memory
-    if (ok) ok = warp_wait(BAR_DONE, 0, 8);
-    tc_fence_after();
-    const uint32_t stage = sK + (uint32_t)w * TILE;
-    const int rows = min(u.q_valid - 128 * w, 128);
-    const bool any = n_kt[w] > 0;
-    if (ok && rows > 0) {
-      const float inv = l == 0.f ? 0.f : 1.f / l;
-      const bool dirty = *reinterpret_cast<volatile int*>(&dirty_sh) != 0;
-#pragma unroll 1
-      for (int c = 0; c < 2 * NA; ++c) {
-        uint32_t o[32];
-        if (any) {
+        for (int c = 0; c < 2 * NA; ++c) {
+          uint32_t o[32];
           tmem_ld32(tO + c * 32, o);
           tmem_wait_ld();
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+          tmem_st32(tO + c * 32, o);
+        }
+        tmem_wait_st();
+        l *= alpha;
+        m_ref = m_new;
+      };
+
+      for (int t = 0; t < n_kt; ++t, ++steps) {
+        if (!(ok = warp_wait(B_S + w, steps & 1, 8))) break;
+        tc_fence_after();
+        const int k0 = (u.begin + t) * 128;
+        const bool full = lim_lo - k0 >= 128;  // no query of the stream misses a key of the tile
+        if (t > 0 && full) {
+          // the exponentials against the current reference; a half past the threshold is redone from
+          // the scores in registers, after the rescale
+#pragma unroll
+          for (int hf = 0; hf < 2; ++hf) {
+            uint32_t s[64], pk[32];
+            tmem_ld32(tS + 64 * hf, s);
+            tmem_ld32(tS + 64 * hf + 32, s + 32);
+            tmem_wait_ld();
+            float lt = probs<T, 64, false>(s, pk, p.scale_log2, m_ref, 64);
+            if (__any_sync(0xffffffffu, !(lt <= kSumThreshold))) {
+              // first half: S_w(t) complete implies every earlier P V is; second: the first half's P V
+              if (hf == 1 && !(ok = warp_wait(B_PVH + w, steps & 1, 16))) break;
+              tc_fence_after();
+              rescale(row_max<64, false>(s, 64) * p.scale_log2);
+              lt = probs<T, 64, false>(s, pk, p.scale_log2, m_ref, 64);
+            }
+            l += lt;
+            tmem_st32(tS + 32 * hf, pk);
+            if (hf == 0) {
+              tmem_wait_st();
+              tc_fence_before();
+              mbar_arrive(BAR(B_PHALF + w));
+            }
+          }
+          if (!ok) break;
+        } else {
+          // the first tile (sets the reference) and the masked ones: the maximum first
+          const int valid = my_lim - k0;
+          uint32_t sr[128];
+          tmem_ld32(tS, sr);
+          tmem_ld32(tS + 32, sr + 32);
+          tmem_ld32(tS + 64, sr + 64);
+          tmem_ld32(tS + 96, sr + 96);
+          if (!full) {
+            // values that some query must not see: clear what is not finite (thread = key row)
+            const int sv = (ring + t) % NV;
+            if (!(ok = warp_wait(B_VFULL + sv, ((ring + t) / NV) & 1, 8))) break;
+            if (clean_row<T, NA>(sV + sv * TILE, row)) dirty_sh[i & 1] = i + 1;
+          }
+          tmem_wait_ld();
+          const float mx = (full ? row_max<128, false>(sr, 128) : row_max<128, true>(sr, valid)) * p.scale_log2;
+          if (t == 0) m_ref = mx;
+          else if (__any_sync(0xffffffffu, mx > m_ref + kRescaleThreshold)) rescale(mx);
+          {
+            const uint32_t(&sh)[64] = *reinterpret_cast<const uint32_t(*)[64]>(&sr[0]);
+            uint32_t pk[32];
+            if (full) l += probs<T, 64, false>(sh, pk, p.scale_log2, m_ref, 64);
+            else l += probs<T, 64, true>(sh, pk, p.scale_log2, m_ref, valid);
+            tmem_st32(tS, pk);
+            tmem_wait_st();
+            tc_fence_before();
+            mbar_arrive(BAR(B_PHALF + w));
+          }
+          {
+            // the second half is loaded again (only its own P overwrites it), so that the first half's
+            // scores alone live through the exponentials
+            uint32_t pk[32];
+            if (lim_hi - k0 > 64) {
+              uint32_t sh[64];
+              tmem_ld32(tS + 64, sh);
+              tmem_ld32(tS + 96, sh + 32);
+              tmem_wait_ld();
+              if (full) l += probs<T, 64, false>(sh, pk, p.scale_log2, m_ref, 64);
+              else l += probs<T, 64, true>(sh, pk, p.scale_log2, m_ref, valid - 64);
+            } else {
+#pragma unroll
+              for (int e = 0; e < 32; ++e) pk[e] = 0u;
+            }
+            tmem_st32(tS + 32, pk);
+          }
+        }
+        tmem_wait_st();
+        tc_fence_before();
+        mbar_arrive(BAR(B_PFULL + w));
+      }
+      if (!ok) break;
+      ring += it.n_max;
+
+      // epilogue: O / l in 16 bits (and for a backward the rest that the rounding leaves, 16 bits more), or a
+      // piece's O, m and l in 32; whole rows from registers to global memory
+      if (n_kt > 0) {
+        if (!(ok = warp_wait(B_OFULL + w, outs & 1, 8))) break;
+        ++outs;
+        tc_fence_after();
+      }
+      const int rows = min(u.q_valid - 128 * w, 128);
+      const bool live = row < rows;
+      const bool dirty = *reinterpret_cast<volatile int*>(&dirty_sh[i & 1]) == i + 1;
+      const float inv = u.part >= 0 ? 1.f : l == 0.f ? 0.f : 1.f / l;
+      const int64_t grow = u.q_row + 128 * w + row;
+      uint16_t* out = static_cast<uint16_t*>(p.a.o) + grow * p.a.ov.rs + (int64_t)it.head * p.a.ov.s1;
+      uint16_t* low = static_cast<uint16_t*>(p.a.o_low) + grow * p.a.olv.rs + (int64_t)it.head * p.a.olv.s1;
+      const int64_t prow = ((int64_t)u.part * p.a.heads + it.head) * 256 + 128 * w + row;  // row of a piece's partial
+#pragma unroll 1
+      for (int c = 0; c < 2 * NA; ++c) {
+        uint32_t o[32];
+        __syncwarp();
+        if (n_kt > 0) {
+          tmem_ld32(tO + c * 32, o);
+          tmem_wait_ld();
+          if (c + 1 == 2 * NA) {  // O is in registers: the next item's products may overwrite it
+            tc_fence_before();
+            mbar_arrive(BAR(B_OFREE + w));
+          }
         } else {
 #pragma unroll
-          for (int i = 0; i < 32; ++i) o[i] = 0u;
+          for (int e = 0; e < 32; ++e) o[e] = 0u;
         }
-        if (dirty && any) {
+        if (!live) continue;
+        if (dirty && n_kt > 0) {
           // values of the masked tiles that were cleared: back to the queries that see them
-          const T* v = static_cast<const T*>(p.a.v) + (int64_t)u.k_row * p.a.vv.rs + (int64_t)kvh * p.a.vv.s1;
-          const int j0 = max(limit(0) & ~127, u.begin * 128), j1 = min(my_lim, u.end * 128);
+          const T* v = static_cast<const T*>(p.a.v) + (int64_t)u.k_row * p.a.vv.rs + (int64_t)it.kvh * p.a.vv.s1;
+          const int j0 = max(it.limit(0) & ~127, u.begin * 128), j1 = min(my_lim, u.end * 128);
 #pragma unroll 1
           for (int j = j0; j < j1; ++j)
 #pragma unroll
-            for (int i = 0; i < 32; ++i) {
-              const float x = c * 32 + i < p.a.dim ? Elem<T>::to_f(v[(int64_t)j * p.a.vv.rs + c * 32 + i]) : 0.f;
-              if (!isfinite(x)) o[i] = __float_as_uint(__uint_as_float(o[i]) + x);
+            for (int e = 0; e < 32; ++e) {
+              const float x = c * 32 + e < p.a.dim ? Elem<T>::to_f(v[(int64_t)j * p.a.vv.rs + c * 32 + e]) : 0.f;
+              if (!isfinite(x)) o[e] = __float_as_uint(__uint_as_float(o[e]) + x);
             }
         }
+        if (u.part >= 0) {
+          float* to = p.a.part + prow * (64 * NA) + c * 32;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          uint32_t x[4], y[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float a = __uint_as_float(o[8 * k + 2 * i]) * inv, b = __uint_as_float(o[8 * k + 2 * i + 1]) * inv;
-            x[i] = Elem<T>::pack(a, b);
-            const float2 r = Elem<T>::unpack(x[i]);
-            y[i] = Elem<T>::pack(a - r.x, b - r.y);
-          }
-          const uint32_t at = stage + (c >> 1) * kAtom + row * 128 + ((((c & 1) * 4 + k) ^ (row & 7)) << 4);
-          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3])
-                       : "memory");
-          if (p.a.o_low)
-            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at + 2 * TILE), "r"(y[0]), "r"(y[1]), "r"(y[2]),
-                         "r"(y[3])
-                         : "memory");
+          for (int k = 0; k < 4; ++k) st_global_v8(to + 8 * k, o + 8 * k);
+          continue;
         }
+        uint32_t x[16], y[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const float a = __uint_as_float(o[2 * e]) * inv, b = __uint_as_float(o[2 * e + 1]) * inv;
+          x[e] = Elem<T>::pack(a, b);
+          const float2 r = Elem<T>::unpack(x[e]);
+          y[e] = Elem<T>::pack(a - r.x, b - r.y);
+        }
+        store_row32(out, c * 32, p.a.dim, sectors, x);
+        if (p.a.o_low) store_row32(low, c * 32, p.a.dim, sectors, y);
       }
-      if (p.a.lse && row < rows)
-        p.a.lse[(int64_t)head * p.a.q_total + u.q_row + 128 * w + row] =
-            l == 0.f ? __int_as_float(0xff800000) : (m_ref + log2f(l)) * kLn2;
-    }
-    ok = named_bar_and(2 + w, 128, ok && !*abort);
-    if (ok && rows > 0) {
-      constexpr int CH = 8 * NA;  // 16-byte chunks per row
-      auto store = [&](void* t, const View& v, uint32_t from) {
-        T* out = static_cast<T*>(t) + (int64_t)(u.q_row + 128 * w) * v.rs + (int64_t)head * v.s1;
-        for (int i = row; i < rows * CH; i += 128) {
-          const int r = i / CH, ch = i % CH;
-          uint32_t x[4];
-          asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];"
-                       : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3])
-                       : "r"(from + (ch >> 3) * kAtom + r * 128 + (((ch & 7) ^ (r & 7)) << 4)));
-          if (ch * 8 < p.a.dim) *reinterpret_cast<uint4*>(out + (int64_t)r * v.rs + ch * 8) = make_uint4(x[0], x[1], x[2], x[3]);
-        }
-      };
-      store(p.a.o, p.a.ov, stage);
-      if (p.a.o_low) store(p.a.o_low, p.a.olv, stage + 2 * TILE);
+      if (live) {
+        if (u.part >= 0)
+          reinterpret_cast<float2*>(p.a.part_ml)[prow] = make_float2(m_ref, l);
+        else if (p.a.lse)
+          p.a.lse[(int64_t)it.head * p.a.q_total + grow] = l == 0.f ? __int_as_float(0xff800000) : (m_ref + log2f(l)) * kLn2;
+      }
     }
   }
 
@@ -500,6 +617,57 @@ __global__ void __launch_bounds__(kThreads, 1) packed_fwd_kernel(const __grid_co
   __syncthreads();
   tc_fence_after();
   if (warp == 0) tmem_dealloc(tmem, 512);
+}
+
+// Joins the pieces of cut units: block = (unit, head, 32 rows), 8 lanes a row, 8 NA columns a lane.
+template <typename T, int NA>
+__global__ void __launch_bounds__(256) packed_fwd_join_kernel(const __grid_constant__ PackedParams a) {
+  const int64_t uh = blockIdx.x >> 3;
+  const int join = (int)(uh / a.heads), head = (int)(uh % a.heads);
+  const PackedUnit u = a.units[a.joins[2 * join]];
+  const int pieces = a.joins[2 * join + 1];
+  const int row = (blockIdx.x & 7) * 32 + (threadIdx.x >> 3), sub = threadIdx.x & 7;
+  if (row >= u.q_valid) return;
+  auto at = [&](int k) { return ((int64_t)(u.part + k) * a.heads + head) * 256 + row; };
+  float m = -1e30f, l = 0.f;
+  for (int k = 0; k < pieces; ++k) m = fmaxf(m, reinterpret_cast<const float2*>(a.part_ml)[at(k)].x);
+  float o[8 * NA];
+#pragma unroll
+  for (int i = 0; i < 8 * NA; ++i) o[i] = 0.f;
+  for (int k = 0; k < pieces; ++k) {
+    const float2 ml = reinterpret_cast<const float2*>(a.part_ml)[at(k)];
+    const float f = fast_exp2(ml.x - m);
+    l = fmaf(ml.y, f, l);
+    const float4* v = reinterpret_cast<const float4*>(a.part + at(k) * (64 * NA) + sub * 8 * NA);
+#pragma unroll
+    for (int i = 0; i < 2 * NA; ++i) {
+      const float4 x = v[i];
+      o[4 * i] = fmaf(x.x, f, o[4 * i]);
+      o[4 * i + 1] = fmaf(x.y, f, o[4 * i + 1]);
+      o[4 * i + 2] = fmaf(x.z, f, o[4 * i + 2]);
+      o[4 * i + 3] = fmaf(x.w, f, o[4 * i + 3]);
+    }
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  const int64_t grow = u.q_row + row;
+#pragma unroll
+  for (int g = 0; g < NA; ++g) {
+    const int col = sub * 8 * NA + 8 * g;
+    if (col >= a.dim) continue;
+    uint32_t x[4], y[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float p = o[8 * g + 2 * i] * inv, q = o[8 * g + 2 * i + 1] * inv;
+      x[i] = Elem<T>::pack(p, q);
+      const float2 r = Elem<T>::unpack(x[i]);
+      y[i] = Elem<T>::pack(p - r.x, q - r.y);
+    }
+    *reinterpret_cast<uint4*>(static_cast<T*>(a.o) + grow * a.ov.rs + head * a.ov.s1 + col) = make_uint4(x[0], x[1], x[2], x[3]);
+    if (a.o_low)
+      *reinterpret_cast<uint4*>(static_cast<T*>(a.o_low) + grow * a.olv.rs + head * a.olv.s1 + col) = make_uint4(y[0], y[1], y[2], y[3]);
+  }
+  if (sub == 0 && a.lse)
+    a.lse[(int64_t)head * a.q_total + grow] = l == 0.f ? __int_as_float(0xff800000) : (m + log2f(l)) * kLn2;
 }
 
 template <typename T, int NA>
@@ -511,6 +679,11 @@ cudaError_t launch(const KParams& p, cudaStream_t st) {
   const int64_t blocks = (int64_t)p.a.n_units * p.a.heads;
   if (blocks > 0x7fffffff) return cudaErrorInvalidConfiguration;
   kern<<<(unsigned)blocks, kThreads, Cfg<NA>::SMEM, st>>>(p);
+  e = cudaGetLastError();
+  if (e != cudaSuccess || p.a.n_joins == 0) return e;
+  const int64_t joins = (int64_t)p.a.n_joins * p.a.heads * 8;
+  if (joins > 0x7fffffff) return cudaErrorInvalidConfiguration;
+  packed_fwd_join_kernel<T, NA><<<(unsigned)joins, 256, 0, st>>>(p.a);
   return cudaGetLastError();
 }
 

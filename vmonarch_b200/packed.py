@@ -21,6 +21,9 @@ MAX_DIM = 128
 _FWD_ROWS, _DQ_ROWS, _KV_ROWS, _STEP = 256, 128, 128, 64
 _FIELDS = 12  # int32 per vmb_packed_unit
 _NEVER_MASKED = -(1 << 30)
+_SMS = 148
+# least steps of a piece when a unit is cut: below it, set-up and join cost more than the cut gains
+_LEAST = {"fwd": 8, "dq": 8, "kv": 16}
 
 
 def _lengths(x, what):
@@ -39,6 +42,31 @@ def _tiles(lens, rows):
     seq = np.repeat(np.arange(len(lens)), count)
     first = (np.arange(len(seq)) - np.repeat(np.cumsum(count) - count, count)) * rows
     return seq, first
+
+
+def _cut(u, heads, least):
+    """Cuts units of a list that would still run when the SMs' fair share of all work is done into equal
+    pieces of at least `least` steps; returns the list and its number of pieces (parts)."""
+    steps = u[:, 6] - u[:, 5]
+    share = max(least, -(-int(steps.sum()) * heads // _SMS))
+    pieces = np.where(steps > share + share // 4, -(-steps // share), 1)
+    if not len(u) or pieces.max() == 1:
+        return u, 0
+    which = np.repeat(np.arange(len(u)), pieces)
+    k = np.arange(len(which)) - np.repeat(np.cumsum(pieces) - pieces, pieces)  # piece of its unit
+    out = u[which]
+    out[:, 5] = u[which, 5] + steps[which] * k // pieces[which]
+    out[:, 6] = u[which, 5] + steps[which] * (k + 1) // pieces[which]
+    is_part = pieces[which] > 1
+    out[is_part, 7] = np.arange(int(is_part.sum()))
+    out[:, 9] = np.where(k == 0, pieces[which], 0)  # for _joins; the kernels do not read it
+    return out, int(is_part.sum())
+
+
+def _joins(u):
+    """(first unit, pieces) of every cut unit of a list."""
+    first = np.nonzero((u[:, 7] >= 0) & (u[:, 9] > 0))[0]
+    return np.stack([first, u[first, 9]], 1).astype(np.int32)
 
 
 class PackedSequences:
@@ -114,15 +142,23 @@ class PackedSequences:
         return u
 
     def _list(self, kind, causal, heads, group):
-        """The device list of a kernel's units, most work first (blocks start in list order)."""
-        key = (kind, causal, group if kind == "kv" else 0)
+        """The device list of a kernel's units, most work first (blocks start in list order), then the joins
+        of those that are cut."""
+        key = (kind, causal, heads, group)
         hit = self._cache.get(key)
         if hit is None:
-            u = self._key_units(causal, group) if kind == "kv" else \
-                self._query_units(_FWD_ROWS if kind == "fwd" else _DQ_ROWS, causal)
+            if kind == "kv":
+                u = self._key_units(causal, group)
+                u, parts = _cut(u, heads // group, _LEAST[kind])
+            else:
+                u = self._query_units(_FWD_ROWS if kind == "fwd" else _DQ_ROWS, causal)
+                u, parts = _cut(u, heads, _LEAST[kind])
             u = u[np.argsort(u[:, 5] - u[:, 6], kind="stable")]
-            dev = torch.from_numpy(np.ascontiguousarray(u)).to(self.device)
-            hit = self._cache[key] = (N.PackedList(dev.data_ptr(), None, len(u), 0, 0, 0), dev)
+            joins = _joins(u)
+            dev = torch.from_numpy(np.concatenate([u.reshape(-1), joins.reshape(-1)])).to(self.device)
+            at = dev.data_ptr()
+            hit = self._cache[key] = (
+                N.PackedList(at, at + u.nbytes if len(joins) else None, len(u), len(joins), parts, 0), dev)
         return hit[0]
 
     def _template(self, key):
