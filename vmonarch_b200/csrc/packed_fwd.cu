@@ -11,7 +11,7 @@
 // epilogue, thread = query row. The two streams walk the same ring of 128-key tiles and never wait for one
 // another, so one's exponentials run beside the other's matrix products. Online softmax with a lazily raised
 // reference: the exponentials of an unmasked tile go against the current reference and are redone
-// only when a 64-key half's sum passes 2^14. P is 16-bit (the rounding the tensor cores need; l sums
+// only when a 64-key half's sum passes 2^14; a warp skips the keys that none of its queries sees. P is 16-bit (the rounding the tensor cores need; l sums
 // the unrounded p), everything else 32-bit.
 // TMEM (512 columns): S_0 [0,128), S_1 [128,256), O_0 [256, +64 NA), O_1 [256 + 64 NA, +64 NA).
 //
@@ -44,7 +44,6 @@ using namespace sm100;
 
 constexpr int kAtom = 128 * 128;  // one swizzle atom column block: 128 rows x 128 B
 constexpr int kThreads = 320;
-constexpr float kRescaleThreshold = 8.0f;
 constexpr float kSumThreshold = 16384.0f;
 
 struct KParams {
@@ -158,11 +157,11 @@ template <typename T, int NA>
 __device__ __forceinline__ bool clean_row(uint32_t tile, int row) {
   uint32_t acc = 0;
 #pragma unroll
-  for (int c = 0; c < 8 * NA; ++c) {
+  for (int c = 0; c < 8 * NA; ++c) {  // neighbouring rows begin at different chunks: no bank conflicts
     uint32_t x[4];
     asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];"
                  : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3])
-                 : "r"(tile + (c >> 3) * kAtom + row * 128 + (c & 7) * 16));
+                 : "r"(tile + (c >> 3) * kAtom + row * 128 + ((c + row) & 7) * 16));
 #pragma unroll
     for (int e = 0; e < 4; ++e) acc = zero_fma2<T>(x[e], acc);
   }
@@ -439,8 +438,10 @@ __global__ void __launch_bounds__(kThreads, 1) packed_fwd_kernel(const __grid_co
       const Item it(p.a, work.u, work.head);
       const PackedUnit& u = it.u;
       const int n_kt = it.n_kt[w];
-      const int my_lim = it.limit(128 * w + row);
-      const int lim_lo = it.limit(128 * w), lim_hi = it.limit(min(u.q_valid, 128 * (w + 1)) - 1);
+      // rows past the unit's last query are not stored: they take its limit, and no part in the reference
+      const int rows = min(u.q_valid - 128 * w, 128);
+      const bool live = row < rows;
+      const int my_lim = it.limit(min(128 * w + row, u.q_valid - 1)), lim_lo = it.limit(128 * w);
       float m_ref = -1e30f, l = 0.f;
       // O and l to the reference max(m_ref, mx). Warp-uniform; no P V into O_w may be in flight.
       auto rescale = [&](float mx) {
@@ -464,79 +465,65 @@ __global__ void __launch_bounds__(kThreads, 1) packed_fwd_kernel(const __grid_co
         if (!(ok = warp_wait(B_S + w, steps & 1, 8))) break;
         tc_fence_after();
         const int k0 = (u.begin + t) * 128;
-        const bool full = lim_lo - k0 >= 128;  // no query of the stream misses a key of the tile
-        if (t > 0 && full) {
-          // the exponentials against the current reference; a half past the threshold is redone from
-          // the scores in registers, after the rescale
+        if (lim_lo - k0 < 128) {
+          // values that some query of the stream must not see: clear what is not finite (thread = key row)
+          const int sv = (ring + t) % NV;
+          if (!(ok = warp_wait(B_VFULL + sv, ((ring + t) / NV) & 1, 8))) break;
+          if (clean_row<T, NA>(sV + sv * TILE, row)) dirty_sh[i & 1] = i + 1;
+        }
+        // Two 64-key halves; a half's P lets its P V start. The exponentials go against the current reference (the
+        // unit's first half sets it); a half past the threshold is redone from the scores in registers.
 #pragma unroll
-          for (int hf = 0; hf < 2; ++hf) {
-            uint32_t s[64], pk[32];
+        for (int hf = 0; hf < 2; ++hf) {
+          const int seen = my_lim - k0 - 64 * hf;               // keys of the half that this query sees,
+          const int least = __shfl_sync(0xffffffffu, seen, 0);  // the warp's first query (limits only grow)
+          const int most = __shfl_sync(0xffffffffu, seen, 31);  // and its last
+          uint32_t pk[32];
+          if (most <= 0) {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) pk[e] = 0u;
+          } else {
+            uint32_t s[64];
             tmem_ld32(tS + 64 * hf, s);
             tmem_ld32(tS + 64 * hf + 32, s + 32);
             tmem_wait_ld();
-            float lt = probs<T, 64, false>(s, pk, p.scale_log2, m_ref, 64);
-            if (__any_sync(0xffffffffu, !(lt <= kSumThreshold))) {
+            auto top = [&]() { return (least >= 64 ? row_max<64, false>(s, 64) : row_max<64, true>(s, seen)) * p.scale_log2; };
+            auto exps = [&]() -> float {
+              if (least >= 64) return probs<T, 64, false>(s, pk, p.scale_log2, m_ref, 64);
+              // masked, 32 keys at a time: a warp computes only those that one of its queries sees
+              const uint32_t(&s0)[32] = *reinterpret_cast<const uint32_t(*)[32]>(&s[0]);
+              const uint32_t(&s1)[32] = *reinterpret_cast<const uint32_t(*)[32]>(&s[32]);
+              uint32_t(&p0)[16] = *reinterpret_cast<uint32_t(*)[16]>(&pk[0]);
+              uint32_t(&p1)[16] = *reinterpret_cast<uint32_t(*)[16]>(&pk[16]);
+              float lt = least >= 32 ? probs<T, 32, false>(s0, p0, p.scale_log2, m_ref, 32)
+                                     : probs<T, 32, true>(s0, p0, p.scale_log2, m_ref, seen);
+              if (most > 32) {
+                lt += probs<T, 32, true>(s1, p1, p.scale_log2, m_ref, seen - 32);
+              } else {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) p1[e] = 0u;
+              }
+              return lt;
+            };
+            if (hf == 0 && t == 0) m_ref = top();
+            float lt = exps();
+            if (__any_sync(0xffffffffu, live && !(lt <= kSumThreshold))) {
               // first half: S_w(t) complete implies every earlier P V is; second: the first half's P V
               if (hf == 1 && !(ok = warp_wait(B_PVH + w, steps & 1, 16))) break;
               tc_fence_after();
-              rescale(row_max<64, false>(s, 64) * p.scale_log2);
-              lt = probs<T, 64, false>(s, pk, p.scale_log2, m_ref, 64);
+              rescale(top());
+              lt = exps();
             }
             l += lt;
-            tmem_st32(tS + 32 * hf, pk);
-            if (hf == 0) {
-              tmem_wait_st();
-              tc_fence_before();
-              mbar_arrive(BAR(B_PHALF + w));
-            }
           }
-          if (!ok) break;
-        } else {
-          // the first tile (sets the reference) and the masked ones: the maximum first
-          const int valid = my_lim - k0;
-          uint32_t sr[128];
-          tmem_ld32(tS, sr);
-          tmem_ld32(tS + 32, sr + 32);
-          tmem_ld32(tS + 64, sr + 64);
-          tmem_ld32(tS + 96, sr + 96);
-          if (!full) {
-            // values that some query must not see: clear what is not finite (thread = key row)
-            const int sv = (ring + t) % NV;
-            if (!(ok = warp_wait(B_VFULL + sv, ((ring + t) / NV) & 1, 8))) break;
-            if (clean_row<T, NA>(sV + sv * TILE, row)) dirty_sh[i & 1] = i + 1;
-          }
-          tmem_wait_ld();
-          const float mx = (full ? row_max<128, false>(sr, 128) : row_max<128, true>(sr, valid)) * p.scale_log2;
-          if (t == 0) m_ref = mx;
-          else if (__any_sync(0xffffffffu, mx > m_ref + kRescaleThreshold)) rescale(mx);
-          {
-            const uint32_t(&sh)[64] = *reinterpret_cast<const uint32_t(*)[64]>(&sr[0]);
-            uint32_t pk[32];
-            if (full) l += probs<T, 64, false>(sh, pk, p.scale_log2, m_ref, 64);
-            else l += probs<T, 64, true>(sh, pk, p.scale_log2, m_ref, valid);
-            tmem_st32(tS, pk);
+          tmem_st32(tS + 32 * hf, pk);
+          if (hf == 0) {
             tmem_wait_st();
             tc_fence_before();
             mbar_arrive(BAR(B_PHALF + w));
           }
-          {
-            // the second half is loaded again (only its own P overwrites it), so that the first half's
-            // scores alone live through the exponentials
-            uint32_t pk[32];
-            if (lim_hi - k0 > 64) {
-              uint32_t sh[64];
-              tmem_ld32(tS + 64, sh);
-              tmem_ld32(tS + 96, sh + 32);
-              tmem_wait_ld();
-              if (full) l += probs<T, 64, false>(sh, pk, p.scale_log2, m_ref, 64);
-              else l += probs<T, 64, true>(sh, pk, p.scale_log2, m_ref, valid - 64);
-            } else {
-#pragma unroll
-              for (int e = 0; e < 32; ++e) pk[e] = 0u;
-            }
-            tmem_st32(tS + 32, pk);
-          }
         }
+        if (!ok) break;
         tmem_wait_st();
         tc_fence_before();
         mbar_arrive(BAR(B_PFULL + w));
@@ -551,8 +538,6 @@ __global__ void __launch_bounds__(kThreads, 1) packed_fwd_kernel(const __grid_co
         ++outs;
         tc_fence_after();
       }
-      const int rows = min(u.q_valid - 128 * w, 128);
-      const bool live = row < rows;
       const bool dirty = *reinterpret_cast<volatile int*>(&dirty_sh[i & 1]) == i + 1;
       const float inv = u.part >= 0 ? 1.f : l == 0.f ? 0.f : 1.f / l;
       const int64_t grow = u.q_row + 128 * w + row;
