@@ -236,8 +236,9 @@ __global__ void __launch_bounds__(kThreads, 1) packed_fwd_kernel(const __grid_co
     dirty_sh[0] = dirty_sh[1] = 0;
     for (int i = 0; i < NBARS; ++i) {
       const bool rows = (i >= B_PHALF && i < B_PVH) || i == B_OFREE || i == B_OFREE + 1;
+      const bool slots = (i >= B_KFREE && i < B_VFULL) || (i >= B_VFREE && i < B_S);  // freed by both streams
       // a block id is read by the V producer, the MMA warp and eight softmax warps
-      mbar_init(BAR(i), rows ? 128 : i >= B_WFREE ? 10 : 1);
+      mbar_init(BAR(i), rows ? 128 : i >= B_WFREE ? 10 : slots ? 2 : 1);
     }
     fence_mbar_init();
   }
@@ -340,24 +341,26 @@ __global__ void __launch_bounds__(kThreads, 1) packed_fwd_kernel(const __grid_co
     auto wwait = [&](int bar, uint32_t parity, int code) -> bool {
       return __all_sync(0xffffffffu, mbar_wait(BAR(bar), parity, abort, &g_packed_err, code));
     };
-    int ring = 0, queries = 0, steps[2] = {0, 0}, outs[2] = {0, 0};  // tiles, units and per-stream tiles and units so far
+    // ring positions of the K tile that is scored next and of the V tile that is weighed next (every tile is loaded
+    // once for both streams), per-stream tiles and units so far
+    int queries = 0, steps[2] = {0, 0}, outs[2] = {0, 0}, ks0 = 0, kp0 = 0, vs0 = 0, vp0 = 0;
     bool ok = true;
     for (int i = 0; ok; ++i) {
       const Work work = next_work(i, 2);
       if (work.head < 0) break;
       const Item it(p.a, work.u, work.head);
       if (it.n_max == 0) continue;
-      // keys of stream w's tile t that some of its queries sees (MMAs of <= 32 keys are shortened)
-      auto tile_keys = [&](int w, int t) {
-        return it.limit(min(it.u.q_valid, 128 * (w + 1)) - 1) - (it.u.begin + t) * 128;
-      };
-      auto last_of = [&](int w, int t) { return w == 1 || t >= it.n_kt[1]; };  // no later stream uses tile t
-      auto issue_s = [&](int w, int t) -> bool {
-        const int s = (ring + t) % NK;
-        if (!wwait(B_KFULL + s, ((ring + t) / NK) & 1, 2)) return false;
+      // a stream's last tile of <= 32 keys: shorter products
+      bool brief[2];
+#pragma unroll
+      for (int w = 0; w < 2; ++w)
+        brief[w] = it.limit(min(it.u.q_valid, 128 * (w + 1)) - 1) - (it.u.begin + it.n_kt[w] - 1) * 128 <= 32;
+      // S of stream w's tile t, whose K tile is in slot s since its phase `parity`
+      auto issue_s = [&](int w, int t, int s, uint32_t parity) -> bool {
+        if (!wwait(B_KFULL + s, parity, 2)) return false;
         tc_fence_after();
         const uint32_t kb = sK + s * TILE, qb = sQ + w * TILE;
-        const uint32_t idesc = tile_keys(w, t) <= 32 ? IDESC_S32 : IDESC_S;
+        const uint32_t idesc = brief[w] && t + 1 == it.n_kt[w] ? IDESC_S32 : IDESC_S;
 #pragma unroll
         for (int kk = 0; kk < 4 * NA; ++kk) {
           const uint32_t off = (kk >> 2) * kAtom + (kk & 3) * 32;
@@ -365,43 +368,42 @@ __global__ void __launch_bounds__(kThreads, 1) packed_fwd_kernel(const __grid_co
                     kk > 0);
         }
         mma_commit_if(leader, BAR(B_S + w));
-        if (last_of(w, t)) {
-          mma_commit_if(leader, BAR(B_KFREE + s));
-          if (t + 1 == it.n_max) mma_commit_if(leader, BAR(B_QFREE));
-        }
         return true;
       };
       ok = wwait(B_QFULL, queries & 1, 2);
       ++queries;
       for (int w = 0; w < 2; ++w)
-        if (ok && it.n_kt[w] > 0) ok = issue_s(w, 0);
-      for (int j = 0; ok && j < 2 * it.n_max; ++j) {
-        const int w = j & 1, t = j >> 1;
-        if (t >= it.n_kt[w]) continue;
-        const int c = steps[w] + t, sv = (ring + t) % NV;
-        const uint32_t vb = sV + sv * TILE;
-        const uint32_t a_tm = tmem + 128 * w, o_tm = tmem + T_O + 64 * NA * w;
-        const int ksteps = tile_keys(w, t) <= 32 ? 2 : 8;  // 16 keys per step
-        if (!(ok = wwait(B_PHALF + w, c & 1, 4) && wwait(B_VFULL + sv, ((ring + t) / NV) & 1, 4))) break;
-        // the stream's O of the last unit has been read
-        if (t == 0 && outs[w] > 0 && !(ok = wwait(B_OFREE + w, (outs[w] - 1) & 1, 4))) break;
-        tc_fence_after();
+        if (ok && it.n_kt[w] > 0) ok = issue_s(w, 0, ks0, kp0);
+      for (int t = 0; ok && t < it.n_max; ++t) {
+        if (++ks0 == NK) ks0 = 0, kp0 ^= 1;  // the next K tile
 #pragma unroll
-        for (int kk = 0; kk < 4; ++kk)
-          mma_ts_if(leader & (kk < ksteps ? 1u : 0u), o_tm, a_tm + kk * 8, smem_desc_sw128(vb + kk * 2048, kAtom, 1024),
-                    IDESC_PV, (t > 0 || kk > 0) ? 1u : 0u);
-        mma_commit_if(leader, BAR(B_PVH + w));  // a softmax that rescales O mid-tile waits for it
-        if (!(ok = wwait(B_PFULL + w, c & 1, 4))) break;
-        tc_fence_after();
+        for (int w = 0; w < 2; ++w) {
+          if (!ok || t >= it.n_kt[w]) continue;
+          const int c = steps[w] + t;
+          const uint32_t vb = sV + vs0 * TILE;
+          const uint32_t a_tm = tmem + 128 * w, o_tm = tmem + T_O + 64 * NA * w;
+          const int ksteps = brief[w] && t + 1 == it.n_kt[w] ? 2 : 8;  // 16 keys per step
+          if (!(ok = wwait(B_PHALF + w, c & 1, 4) && wwait(B_VFULL + vs0, vp0, 4))) break;
+          // the stream's O of the last unit has been read
+          if (t == 0 && outs[w] > 0 && !(ok = wwait(B_OFREE + w, (outs[w] - 1) & 1, 4))) break;
+          tc_fence_after();
 #pragma unroll
-        for (int kk = 4; kk < 8; ++kk)
-          mma_ts_if(leader & (kk < ksteps ? 1u : 0u), o_tm, a_tm + kk * 8, smem_desc_sw128(vb + kk * 2048, kAtom, 1024),
-                    IDESC_PV, 1u);
-        if (last_of(w, t)) mma_commit_if(leader, BAR(B_VFREE + sv));
-        if (t + 1 < it.n_kt[w]) ok = issue_s(w, t + 1);
-        else mma_commit_if(leader, BAR(B_OFULL + w));
+          for (int kk = 0; kk < 4; ++kk)
+            mma_ts_if(leader & (kk < ksteps ? 1u : 0u), o_tm, a_tm + kk * 8, smem_desc_sw128(vb + kk * 2048, kAtom, 1024),
+                      IDESC_PV, (t > 0 || kk > 0) ? 1u : 0u);
+          mma_commit_if(leader, BAR(B_PVH + w));  // a softmax that rescales O mid-tile waits for it
+          if (!(ok = wwait(B_PFULL + w, c & 1, 4))) break;
+          tc_fence_after();
+#pragma unroll
+          for (int kk = 4; kk < 8; ++kk)
+            mma_ts_if(leader & (kk < ksteps ? 1u : 0u), o_tm, a_tm + kk * 8, smem_desc_sw128(vb + kk * 2048, kAtom, 1024),
+                      IDESC_PV, 1u);
+          if (t + 1 < it.n_kt[w]) ok = issue_s(w, t + 1, ks0, kp0);
+          else mma_commit_if(leader, BAR(B_OFULL + w));
+        }
+        if (++vs0 == NV) vs0 = 0, vp0 ^= 1;
       }
-      ring += it.n_max;
+      if (ok) mma_commit_if(leader, BAR(B_QFREE));
       for (int w = 0; w < 2; ++w) {
         steps[w] += it.n_kt[w];
         outs[w] += it.n_kt[w] > 0;
@@ -431,6 +433,7 @@ __global__ void __launch_bounds__(kThreads, 1) packed_fwd_kernel(const __grid_co
     const bool sectors = ((p.a.ov.rs | p.a.ov.s1 | p.a.olv.rs | p.a.olv.s1) & 15) == 0 &&
                          ((reinterpret_cast<uintptr_t>(p.a.o) | reinterpret_cast<uintptr_t>(p.a.o_low)) & 31) == 0;
     int steps = 0, outs = 0, ring = 0;  // tiles and units of this stream so far, tiles of the ring
+    const bool leads = warp == 2 + 4 * w && lane == 0;  // frees ring slots for the stream
     bool ok = true;
     for (int i = 0; ok; ++i) {
       const Work work = next_work(i, 8);
@@ -464,63 +467,93 @@ __global__ void __launch_bounds__(kThreads, 1) packed_fwd_kernel(const __grid_co
       for (int t = 0; t < n_kt; ++t, ++steps) {
         if (!(ok = warp_wait(B_S + w, steps & 1, 8))) break;
         tc_fence_after();
-        const int k0 = (u.begin + t) * 128;
-        if (lim_lo - k0 < 128) {
-          // values that some query of the stream must not see: clear what is not finite (thread = key row)
-          const int sv = (ring + t) % NV;
-          if (!(ok = warp_wait(B_VFULL + sv, ((ring + t) / NV) & 1, 8))) break;
-          if (clean_row<T, NA>(sV + sv * TILE, row)) dirty_sh[i & 1] = i + 1;
+        if (leads) {
+          // S_w(t) complete, so is P V_w(t - 1) before it: K(t) and V(t - 1) are free of this stream
+          mbar_arrive(BAR(B_KFREE + (ring + t) % NK));
+          if (t >= 1) mbar_arrive(BAR(B_VFREE + (ring + t - 1) % NV));
         }
+        const int k0 = (u.begin + t) * 128;
         // Two 64-key halves; a half's P lets its P V start. The exponentials go against the current reference (the
-        // unit's first half sets it); a half past the threshold is redone from the scores in registers.
+        // unit's first half sets it); a half past the threshold is redone from the scores in registers, once
+        // no P V into O is under way: S_w(t) complete implies that every earlier one is done, and in the second
+        // half the first half's is waited for.
+        if (t > 0 && lim_lo - k0 >= 128) {  // no query of the stream misses a key of the tile
 #pragma unroll
-        for (int hf = 0; hf < 2; ++hf) {
-          const int seen = my_lim - k0 - 64 * hf;               // keys of the half that this query sees,
-          const int least = __shfl_sync(0xffffffffu, seen, 0);  // the warp's first query (limits only grow)
-          const int most = __shfl_sync(0xffffffffu, seen, 31);  // and its last
-          uint32_t pk[32];
-          if (most <= 0) {
-#pragma unroll
-            for (int e = 0; e < 32; ++e) pk[e] = 0u;
-          } else {
-            uint32_t s[64];
+          for (int hf = 0; hf < 2; ++hf) {
+            uint32_t s[64], pk[32];
             tmem_ld32(tS + 64 * hf, s);
             tmem_ld32(tS + 64 * hf + 32, s + 32);
             tmem_wait_ld();
-            auto top = [&]() { return (least >= 64 ? row_max<64, false>(s, 64) : row_max<64, true>(s, seen)) * p.scale_log2; };
-            auto exps = [&]() -> float {
-              if (least >= 64) return probs<T, 64, false>(s, pk, p.scale_log2, m_ref, 64);
-              // masked, 32 keys at a time: a warp computes only those that one of its queries sees
-              const uint32_t(&s0)[32] = *reinterpret_cast<const uint32_t(*)[32]>(&s[0]);
-              const uint32_t(&s1)[32] = *reinterpret_cast<const uint32_t(*)[32]>(&s[32]);
-              uint32_t(&p0)[16] = *reinterpret_cast<uint32_t(*)[16]>(&pk[0]);
-              uint32_t(&p1)[16] = *reinterpret_cast<uint32_t(*)[16]>(&pk[16]);
-              float lt = least >= 32 ? probs<T, 32, false>(s0, p0, p.scale_log2, m_ref, 32)
-                                     : probs<T, 32, true>(s0, p0, p.scale_log2, m_ref, seen);
-              if (most > 32) {
-                lt += probs<T, 32, true>(s1, p1, p.scale_log2, m_ref, seen - 32);
-              } else {
-#pragma unroll
-                for (int e = 0; e < 16; ++e) p1[e] = 0u;
-              }
-              return lt;
-            };
-            if (hf == 0 && t == 0) m_ref = top();
-            float lt = exps();
+            float lt = probs<T, 64, false>(s, pk, p.scale_log2, m_ref, 64);
             if (__any_sync(0xffffffffu, live && !(lt <= kSumThreshold))) {
-              // first half: S_w(t) complete implies every earlier P V is; second: the first half's P V
               if (hf == 1 && !(ok = warp_wait(B_PVH + w, steps & 1, 16))) break;
               tc_fence_after();
-              rescale(top());
-              lt = exps();
+              rescale(row_max<64, false>(s, 64) * p.scale_log2);
+              lt = probs<T, 64, false>(s, pk, p.scale_log2, m_ref, 64);
             }
             l += lt;
+            tmem_st32(tS + 32 * hf, pk);
+            if (hf == 0) {
+              tmem_wait_st();
+              tc_fence_before();
+              mbar_arrive(BAR(B_PHALF + w));
+            }
           }
-          tmem_st32(tS + 32 * hf, pk);
-          if (hf == 0) {
-            tmem_wait_st();
-            tc_fence_before();
-            mbar_arrive(BAR(B_PHALF + w));
+        } else {
+          if (lim_lo - k0 < 128) {
+            // values that some query of the stream must not see: clear what is not finite (thread = key row)
+            const int sv = (ring + t) % NV;
+            if (!(ok = warp_wait(B_VFULL + sv, ((ring + t) / NV) & 1, 8))) break;
+            if (clean_row<T, NA>(sV + sv * TILE, row)) dirty_sh[i & 1] = i + 1;
+          }
+#pragma unroll 1
+          for (int hf = 0; hf < 2; ++hf) {
+            const int seen = my_lim - k0 - 64 * hf;               // keys of the half that this query sees,
+            const int least = __shfl_sync(0xffffffffu, seen, 0);  // the warp's first query (limits only grow)
+            const int most = __shfl_sync(0xffffffffu, seen, 31);  // and its last
+            uint32_t pk[32];
+            if (most <= 0) {
+#pragma unroll
+              for (int e = 0; e < 32; ++e) pk[e] = 0u;
+            } else {
+              uint32_t s[64];
+              tmem_ld32(tS + 64 * hf, s);
+              tmem_ld32(tS + 64 * hf + 32, s + 32);
+              tmem_wait_ld();
+              if (hf == 0 && t == 0) m_ref = row_max<64, true>(s, seen) * p.scale_log2;
+              float lt = 0.f;
+#pragma unroll 1
+              for (int pass = 0; pass < 2; ++pass) {
+                if (least >= 64) {
+                  lt = probs<T, 64, false>(s, pk, p.scale_log2, m_ref, 64);
+                } else {
+                  // masked, 32 keys at a time: a warp computes only those that one of its queries sees
+                  const uint32_t(&s0)[32] = *reinterpret_cast<const uint32_t(*)[32]>(&s[0]);
+                  const uint32_t(&s1)[32] = *reinterpret_cast<const uint32_t(*)[32]>(&s[32]);
+                  uint32_t(&p0)[16] = *reinterpret_cast<uint32_t(*)[16]>(&pk[0]);
+                  uint32_t(&p1)[16] = *reinterpret_cast<uint32_t(*)[16]>(&pk[16]);
+                  lt = probs<T, 32, true>(s0, p0, p.scale_log2, m_ref, seen);
+                  if (most > 32) {
+                    lt += probs<T, 32, true>(s1, p1, p.scale_log2, m_ref, seen - 32);
+                  } else {
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) p1[e] = 0u;
+                  }
+                }
+                if (pass || !__any_sync(0xffffffffu, live && !(lt <= kSumThreshold))) break;
+                if (hf == 1 && !(ok = warp_wait(B_PVH + w, steps & 1, 16))) break;
+                tc_fence_after();
+                rescale(row_max<64, true>(s, seen) * p.scale_log2);
+              }
+              if (!ok) break;
+              l += lt;
+            }
+            tmem_st32(tS + 32 * hf, pk);
+            if (hf == 0) {
+              tmem_wait_st();
+              tc_fence_before();
+              mbar_arrive(BAR(B_PHALF + w));
+            }
           }
         }
         if (!ok) break;
@@ -529,7 +562,6 @@ __global__ void __launch_bounds__(kThreads, 1) packed_fwd_kernel(const __grid_co
         mbar_arrive(BAR(B_PFULL + w));
       }
       if (!ok) break;
-      ring += it.n_max;
 
       // epilogue: O / l in 16 bits (and for a backward the rest that the rounding leaves, 16 bits more), or a
       // piece's O, m and l in 32; whole rows from registers to global memory
@@ -538,6 +570,21 @@ __global__ void __launch_bounds__(kThreads, 1) packed_fwd_kernel(const __grid_co
         ++outs;
         tc_fence_after();
       }
+      if (leads) {
+        // the stream's last V tile, and the tiles that only the other stream uses: each once it has landed, so
+        // that this stream's word for a slot never runs ahead of the slot's phase
+        if (n_kt > 0) mbar_arrive(BAR(B_VFREE + (ring + n_kt - 1) % NV));
+        for (int t = n_kt; ok && t < it.n_max; ++t) {
+          const int r = ring + t;
+          ok = mbar_wait(BAR(B_KFULL + r % NK), (r / NK) & 1, abort, &g_packed_err, 8) &&
+               mbar_wait(BAR(B_VFULL + r % NV), (r / NV) & 1, abort, &g_packed_err, 8);
+          if (!ok) break;
+          mbar_arrive(BAR(B_KFREE + r % NK));
+          mbar_arrive(BAR(B_VFREE + r % NV));
+        }
+      }
+      if (!(ok = __all_sync(0xffffffffu, ok))) break;
+      ring += it.n_max;
       const bool dirty = *reinterpret_cast<volatile int*>(&dirty_sh[i & 1]) == i + 1;
       const float inv = u.part >= 0 ? 1.f : l == 0.f ? 0.f : 1.f / l;
       const int64_t grow = u.q_row + 128 * w + row;
