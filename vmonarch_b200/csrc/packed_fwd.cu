@@ -251,22 +251,9 @@ __global__ void __launch_bounds__(kThreads, 1) packed_fwd_kernel(const __grid_co
   tc_fence_after();
   const uint32_t tmem = tmem_base_sh;
 
-  // Item 0 is this block's own, from global memory; the K producer hands the others on through work_sh.
-  auto own_work = [&](int block) -> Work {
-    const UnitHead uh = unit_of_block(block, p.a.n_units, p.a.heads, p.a.head_chunk);
-    return Work{p.a.units[uh.unit], uh.head};
-  };
+  // The K producer hands the items on through work_sh: item i in place i & 1 until its ten readers are done with it.
   auto work_wait = [&](int i, int code) -> bool {
-    return mbar_wait(BAR(B_WFULL + (i & 1)), ((i - 1) >> 1) & 1, abort, &g_packed_err, code);
-  };
-  // for a whole warp; head -1: no more work (or a failed wait)
-  auto next_work = [&](int i, int code) -> Work {
-    if (i == 0) return own_work(blockIdx.x);
-    if (!__all_sync(0xffffffffu, work_wait(i, code))) return Work{PackedUnit{}, -1};
-    const Work w = work_sh[i & 1];
-    __syncwarp();
-    if (lane == 0) mbar_arrive(BAR(B_WFREE + (i & 1)));
-    return w;
+    return mbar_wait(BAR(B_WFULL + (i & 1)), (i >> 1) & 1, abort, &g_packed_err, code);
   };
 
   if (warp == 0) {
@@ -279,8 +266,24 @@ __global__ void __launch_bounds__(kThreads, 1) packed_fwd_kernel(const __grid_co
       prefetch_tmap(map);
       int tiles = 0, queries = 0, asked = 0;  // loaded so far by this lane; answers asked for
       bool ok = true;
-      Work work = own_work(blockIdx.x);
-      for (int i = 0; ok && work.head >= 0; ++i) {
+      Work work;
+      int block = blockIdx.x;
+      for (int i = 0; ok; ++i) {
+        if (kl) {
+          work.head = -1;
+          if (block >= 0) {
+            const UnitHead uh = unit_of_block(block, p.a.n_units, p.a.heads, p.a.head_chunk);
+            work = Work{p.a.units[uh.unit], uh.head};
+          }
+          if (i >= 2 && !(ok = mbar_wait(BAR(B_WFREE + (i & 1)), ((i - 2) >> 1) & 1, abort, &g_packed_err, 1))) break;
+          work_sh[i & 1] = work;
+          mbar_arrive(BAR(B_WFULL + (i & 1)));
+        } else {
+          if (!(ok = work_wait(i, 1))) break;
+          work = work_sh[i & 1];
+          mbar_arrive(BAR(B_WFREE + (i & 1)));
+        }
+        if (work.head < 0) break;
         if (kl) {  // ask for the item after this one, long before it is needed
           fence_proxy_async_smem();
           mbar_expect_tx(BAR(B_ANSWER), 16);
@@ -314,19 +317,8 @@ __global__ void __launch_bounds__(kThreads, 1) packed_fwd_kernel(const __grid_co
         }
         if (!ok) break;
         if (kl) {
-          const int n = i + 1;
-          ok = mbar_wait(BAR(B_ANSWER), i & 1, abort, &g_packed_err, 1) &&
-               (n < 3 || mbar_wait(BAR(B_WFREE + (n & 1)), ((n - 3) >> 1) & 1, abort, &g_packed_err, 1));
-          if (!ok) break;
-          const int block = answered_block(smem_u32(&answer_sh));
-          work.head = -1;
-          if (block >= 0) work = own_work(block);
-          work_sh[n & 1] = work;
-          mbar_arrive(BAR(B_WFULL + (n & 1)));
-        } else {
-          if (!(ok = work_wait(i + 1, 1))) break;
-          work = work_sh[(i + 1) & 1];
-          mbar_arrive(BAR(B_WFREE + ((i + 1) & 1)));
+          if (!(ok = mbar_wait(BAR(B_ANSWER), i & 1, abort, &g_packed_err, 1))) break;
+          block = answered_block(smem_u32(&answer_sh));
         }
       }
       // drain: what was asked for must have landed before the CTA may exit
@@ -346,9 +338,12 @@ __global__ void __launch_bounds__(kThreads, 1) packed_fwd_kernel(const __grid_co
     int queries = 0, steps[2] = {0, 0}, outs[2] = {0, 0}, ks0 = 0, kp0 = 0, vs0 = 0, vp0 = 0;
     bool ok = true;
     for (int i = 0; ok; ++i) {
-      const Work work = next_work(i, 2);
-      if (work.head < 0) break;
-      const Item it(p.a, work.u, work.head);
+      if (!(ok = __all_sync(0xffffffffu, work_wait(i, 2)))) break;
+      const int head = work_sh[i & 1].head;
+      const Item it(p.a, work_sh[i & 1].u, head);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(BAR(B_WFREE + (i & 1)));
+      if (head < 0) break;
       if (it.n_max == 0) continue;
       // a stream's last tile of <= 32 keys: shorter products
       bool brief[2];
@@ -436,15 +431,20 @@ __global__ void __launch_bounds__(kThreads, 1) packed_fwd_kernel(const __grid_co
     const bool leads = warp == 2 + 4 * w && lane == 0;  // frees ring slots for the stream
     bool ok = true;
     for (int i = 0; ok; ++i) {
-      const Work work = next_work(i, 8);
-      if (work.head < 0) break;
-      const Item it(p.a, work.u, work.head);
-      const PackedUnit& u = it.u;
-      const int n_kt = it.n_kt[w];
-      // rows past the unit's last query are not stored: they take its limit, and no part in the reference
-      const int rows = min(u.q_valid - 128 * w, 128);
-      const bool live = row < rows;
-      const int my_lim = it.limit(min(128 * w + row, u.q_valid - 1)), lim_lo = it.limit(128 * w);
+      if (!(ok = __all_sync(0xffffffffu, work_wait(i, 8)))) break;
+      if (work_sh[i & 1].head < 0) break;
+      // what the loop over the tiles needs; the epilogue reads the rest again (the loop wants the registers)
+      int n_kt, begin, my_lim, lim_lo;
+      bool live;
+      {
+        const Item it(p.a, work_sh[i & 1].u, work_sh[i & 1].head);
+        n_kt = it.n_kt[w];
+        begin = it.u.begin;
+        // rows past the unit's last query are not stored: they take its limit, and no part in the reference
+        live = 128 * w + row < it.u.q_valid;
+        my_lim = it.limit(min(128 * w + row, it.u.q_valid - 1));
+        lim_lo = it.limit(128 * w);
+      }
       float m_ref = -1e30f, l = 0.f;
       // O and l to the reference max(m_ref, mx). Warp-uniform; no P V into O_w may be in flight.
       auto rescale = [&](float mx) {
@@ -472,7 +472,7 @@ __global__ void __launch_bounds__(kThreads, 1) packed_fwd_kernel(const __grid_co
           mbar_arrive(BAR(B_KFREE + (ring + t) % NK));
           if (t >= 1) mbar_arrive(BAR(B_VFREE + (ring + t - 1) % NV));
         }
-        const int k0 = (u.begin + t) * 128;
+        const int k0 = (begin + t) * 128;
         // Two 64-key halves; a half's P lets its P V start. The exponentials go against the current reference (the
         // unit's first half sets it); a half past the threshold is redone from the scores in registers, once
         // no P V into O is under way: S_w(t) complete implies that every earlier one is done, and in the second
@@ -570,6 +570,8 @@ __global__ void __launch_bounds__(kThreads, 1) packed_fwd_kernel(const __grid_co
         ++outs;
         tc_fence_after();
       }
+      const Item it(p.a, work_sh[i & 1].u, work_sh[i & 1].head);
+      const PackedUnit& u = it.u;
       if (leads) {
         // the stream's last V tile, and the tiles that only the other stream uses: each once it has landed, so
         // that this stream's word for a slot never runs ahead of the slot's phase
@@ -642,6 +644,8 @@ __global__ void __launch_bounds__(kThreads, 1) packed_fwd_kernel(const __grid_co
         else if (p.a.lse)
           p.a.lse[(int64_t)it.head * p.a.q_total + grow] = l == 0.f ? __int_as_float(0xff800000) : (m_ref + log2f(l)) * kLn2;
       }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(BAR(B_WFREE + (i & 1)));
     }
   }
 
