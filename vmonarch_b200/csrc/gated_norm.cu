@@ -56,6 +56,18 @@ __device__ __forceinline__ V8 get8(const float* s) {
   const float4 a = reinterpret_cast<const float4*>(s)[0], b = reinterpret_cast<const float4*>(s)[1];
   return V8{{make_float2(a.x, a.y), make_float2(a.z, a.w), make_float2(b.x, b.y), make_float2(b.z, b.w)}};
 }
+// The same in shared rows that are read 8 columns a thread: the halves of all vectors apart ([2][cols / 8] of four
+// floats), so that neighbouring threads read neighbouring 16 bytes.
+__device__ __forceinline__ void put_apart(float* s, int cols, int col, const V8& f) {
+  float4* q = reinterpret_cast<float4*>(s) + (col >> 3);
+  q[0] = make_float4(f.v[0].x, f.v[0].y, f.v[1].x, f.v[1].y);
+  q[cols >> 3] = make_float4(f.v[2].x, f.v[2].y, f.v[3].x, f.v[3].y);
+}
+__device__ __forceinline__ V8 get_apart(const float* s, int cols, int col) {
+  const float4* q = reinterpret_cast<const float4*>(s) + (col >> 3);
+  const float4 a = q[0], b = q[cols >> 3];
+  return V8{{make_float2(a.x, a.y), make_float2(a.z, a.w), make_float2(b.x, b.y), make_float2(b.z, b.w)}};
+}
 __device__ __forceinline__ float sum8(const V8& f) {
   const float2 a = __fadd2_rn(__fadd2_rn(f.v[0], f.v[1]), __fadd2_rn(f.v[2], f.v[3]));
   return a.x + a.y;
@@ -78,51 +90,63 @@ struct Io<T, T> {
   }
 };
 
-__device__ __forceinline__ float warp_sum(float v) {
+// Sums N <= 8 values over a warp with about log2(32) + N shuffles instead of 5 N: while there are several
+// values, a step hands half of them to the other half of the lanes. NP: N rounded up to a power of two;
+// afterwards the lanes [i 32 / NP, +32 / NP) hold value i's sum in v[0].
+template <int NP>
+__device__ __forceinline__ void warp_sums(float (&v)[NP]) {
+  int width = 16;
 #pragma unroll
-  for (int s = 16; s > 0; s >>= 1) v += __shfl_xor_sync(0xffffffffu, v, s);
-  return v;
+  for (int n = NP / 2; n > 0; n >>= 1, width >>= 1) {
+    const bool hi = threadIdx.x & width;
+#pragma unroll
+    for (int i = 0; i < n; ++i) {
+      const float send = hi ? v[i] : v[i + n], keep = hi ? v[i + n] : v[i];
+      v[i] = keep + __shfl_xor_sync(0xffffffffu, send, width);
+    }
+  }
+#pragma unroll
+  for (; width > 0; width >>= 1) v[0] += __shfl_xor_sync(0xffffffffu, v[0], width);
 }
 
-// Where the warps of a row meet: two buffers in turn of up to three values a warp (a thread that writes one again
+// Where the warps of a row meet: two buffers in turn of up to eight values a warp (a thread that writes one again
 // has passed the barrier of the other since). A group's slots begin at a multiple of four and are padded
 // with zeros to 4 N4, the most warps that a row of this instance has.
 template <int N4>
 struct Meet {
-  float* buf;  // [2][3][kSlots]
+  static constexpr int kSlots = 64, kFloats = 2 * 8 * kSlots;
+  float* buf;  // [2][8][kSlots]
   int group, tpr, slot, base;
-  static constexpr int kSlots = 64;
   __device__ __forceinline__ Meet(float* shared, int tpr_) : buf(shared), tpr(tpr_) {
     group = threadIdx.x / tpr;
     base = group * 4 * N4;
     slot = base + (threadIdx.x - group * tpr) / 32;
-    for (int i = threadIdx.x; i < 6 * kSlots; i += blockDim.x) buf[i] = 0.f;
+    for (int i = threadIdx.x; i < kFloats; i += blockDim.x) buf[i] = 0.f;
     __syncthreads();
   }
+  // v[i] = its sum over the row's threads
   template <int N>
   __device__ __forceinline__ void sum(float (&v)[N], int& flip) const {
-    static_assert(N <= 3, "three values a meeting");
+    constexpr int NP = N <= 1 ? 1 : N <= 2 ? 2 : N <= 4 ? 4 : 8, LANES = 32 / NP;
+    const int lane = threadIdx.x & 31;
+    float t[NP];
 #pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = warp_sum(v[i]);
+    for (int i = 0; i < NP; ++i) t[i] = i < N ? v[i] : 0.f;
+    warp_sums<NP>(t);
     if constexpr (N4 > 0) {
       float* b = buf + flip;
-      flip ^= 3 * kSlots;
-      if ((threadIdx.x & 31) == 0)
-#pragma unroll
-        for (int i = 0; i < N; ++i) b[i * kSlots + slot] = v[i];
+      flip ^= 8 * kSlots;
+      if (lane % LANES == 0) b[(lane / LANES) * kSlots + slot] = t[0];
       asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "r"(tpr) : "memory");
+      const float* from = b + (lane / LANES) * kSlots + base + lane % LANES;
+      t[0] = 0.f;
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        float2 a = make_float2(0.f, 0.f), c = a;
+      for (int w = 0; w < 4 * N4; w += LANES) t[0] += w + LANES <= 4 * N4 || w + lane % LANES < 4 * N4 ? from[w] : 0.f;
 #pragma unroll
-        for (int w = 0; w < N4; ++w) {
-          const float4 x = *reinterpret_cast<const float4*>(b + i * kSlots + base + 4 * w);
-          a = __fadd2_rn(a, make_float2(x.x, x.y));
-          c = __fadd2_rn(c, make_float2(x.z, x.w));
-        }
-        v[i] = (a.x + c.x) + (a.y + c.y);
-      }
+      for (int x = LANES / 2; x > 0; x >>= 1) t[0] += __shfl_xor_sync(0xffffffffu, t[0], x);
     }
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = NP == 1 ? t[0] : __shfl_sync(0xffffffffu, t[0], i * LANES);
   }
 };
 
@@ -186,16 +210,16 @@ __device__ __forceinline__ void load_params(const GatedNormParams& p, int seq, i
     gate.v[i] = __fmul2_rn(gate.v[i], post.v[i]);
     weight.v[i] = __fmul2_rn(weight.v[i], __fadd2_rn(scale.v[i], pair(1.f)));
   }
-  put8(gw + col, gate);
-  put8(sw + col, weight);
-  if (sh) put8(sh + col, shift);
+  put_apart(gw, p.cols, col, gate);
+  put_apart(sw, p.cols, col, weight);
+  if (sh) put_apart(sh, p.cols, col, shift);
 }
 
 template <typename T, typename P, bool HAS_Y, int VPT, int N4, int MAXT>
 __global__ void __launch_bounds__(MAXT) gated_norm_fwd_kernel(const __grid_constant__ GatedNormParams p) {
   constexpr int NIN = HAS_Y ? 2 : 1;
   extern __shared__ __align__(16) uint8_t smem[];
-  __shared__ __align__(16) float meeting[6 * Meet<N4>::kSlots];
+  __shared__ __align__(16) float meeting[Meet<N4>::kFloats];
   const int tpr = p.tpr, groups = blockDim.x / tpr;
   const Meet<N4> meet(meeting, tpr);
   int flip = 0, col[VPT];
@@ -265,7 +289,7 @@ __global__ void __launch_bounds__(MAXT) gated_norm_fwd_kernel(const __grid_const
 #pragma unroll
         for (int v = 0; v < VPT; ++v)
           if (on[v]) {
-            const V8 g = get8(gw + col[v]);
+            const V8 g = get_apart(gw, p.cols, col[v]);
 #pragma unroll
             for (int i = 0; i < 4; ++i) y[v].v[i] = __fmul2_rn(y[v].v[i], g.v[i]);
           }
@@ -315,7 +339,7 @@ __global__ void __launch_bounds__(MAXT) gated_norm_fwd_kernel(const __grid_const
 #pragma unroll
       for (int v = 0; v < VPT; ++v)
         if (on[v]) {
-          const V8 w = get8(sw + col[v]), t = get8(sh + col[v]);
+          const V8 w = get_apart(sw, p.cols, col[v]), t = get_apart(sh, p.cols, col[v]);
           V8 h;
 #pragma unroll
           for (int i = 0; i < 4; ++i) h.v[i] = __ffma2_rn(__fmul2_rn(x[v].v[i], pair(rx[0])), w.v[i], t.v[i]);
@@ -338,7 +362,7 @@ template <typename T, typename P, bool HAS_Y, int N4, int MAXT, bool AGAIN>
 __global__ void __launch_bounds__(MAXT) gated_norm_bwd_kernel(const __grid_constant__ GatedNormParams p) {
   constexpr int NIN = HAS_Y ? 4 : 3;  // x, dh, dx', y
   extern __shared__ __align__(16) uint8_t smem[];
-  __shared__ __align__(16) float meeting[6 * Meet<N4>::kSlots];
+  __shared__ __align__(16) float meeting[Meet<N4>::kFloats];
   const int tpr = p.tpr, groups = blockDim.x / tpr;
   const Meet<N4> meet(meeting, tpr);
   const int group = meet.group, col = ((int)threadIdx.x - group * tpr) * 8;
@@ -398,7 +422,7 @@ __global__ void __launch_bounds__(MAXT) gated_norm_bwd_kernel(const __grid_const
         if (p.dh) dh = unpack8<T>(ld_shared16(get + piece));
         if constexpr (HAS_Y) {
           yn = unpack8<T>(ld_shared16(get + 3 * piece));
-          const V8 g = get8(gw + col);
+          const V8 g = get_apart(gw, p.cols, col);
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             yn.v[i] = __fmul2_rn(yn.v[i], pair(ry));
@@ -410,7 +434,7 @@ __global__ void __launch_bounds__(MAXT) gated_norm_bwd_kernel(const __grid_const
       };
       auto weigh = [&]() {  // dh -> g of the formulas
         if (!on) return;
-        const V8 w = get8(sw + col);
+        const V8 w = get_apart(sw, p.cols, col);
 #pragma unroll
         for (int i = 0; i < 4; ++i) dh.v[i] = __fmul2_rn(dh.v[i], w.v[i]);
       };
@@ -452,7 +476,7 @@ __global__ void __launch_bounds__(MAXT) gated_norm_bwd_kernel(const __grid_const
       if constexpr (HAS_Y) {
         V8 t = splat(0.f);  // t of the formulas
         if (on) {
-          const V8 g = get8(gw + col);
+          const V8 g = get_apart(gw, p.cols, col);
 #pragma unroll
           for (int i = 0; i < 4; ++i) t.v[i] = __fmul2_rn(dx.v[i], g.v[i]);
         }
