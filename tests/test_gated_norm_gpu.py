@@ -95,6 +95,14 @@ def test_rows(lens):
         check(lens, 5120, torch.float16, torch.float16, "rms", seqs=False)
 
 
+@pytest.mark.parametrize("norm", ["rms", "layer"])
+@pytest.mark.parametrize("c", [80, 256, 264, 512, 520, 1040, 2048, 4096, 5120, 5128, 7000, 8192])
+def test_many_rows(c, norm):
+    """More rows than blocks, in runs that cross sequences: the other layout of the forward's threads."""
+    check([301, 0, 1, 90], c, torch.bfloat16, torch.float32, norm)
+    check([301, 0, 1, 90], c, torch.float16, torch.float16, norm, ("post_weight",))
+
+
 @pytest.mark.parametrize("use", [(True, False), (False, True)])
 def test_one_output_unused(use):
     check([30, 4], 320, torch.bfloat16, torch.float32, "layer", use=use)

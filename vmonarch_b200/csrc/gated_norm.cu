@@ -356,9 +356,7 @@ __global__ void __launch_bounds__(MAXT) gated_norm_fwd_kernel(const __grid_const
   }
 }
 
-// AGAIN: a row's values are read from the ring once more behind the first meeting instead of living through it
-// in registers (rows of more than 640 threads, which have 64 registers each).
-template <typename T, typename P, bool HAS_Y, int N4, int MAXT, bool AGAIN>
+template <typename T, typename P, bool HAS_Y, int N4, int MAXT>
 __global__ void __launch_bounds__(MAXT) gated_norm_bwd_kernel(const __grid_constant__ GatedNormParams p) {
   constexpr int NIN = HAS_Y ? 4 : 3;  // x, dh, dx', y
   extern __shared__ __align__(16) uint8_t smem[];
@@ -454,18 +452,10 @@ __global__ void __launch_bounds__(MAXT) gated_norm_bwd_kernel(const __grid_const
         get = get + stage == end ? ring : get + stage;
         issue();
       };
-      if (!AGAIN) {
-        read_dx();
-        next();
-      }
+      read_dx();
+      next();
       if (it + 1 < n) load_stats(row + groups);
       meet.sum(acc, flip);
-      if (AGAIN) {
-        read();
-        weigh();
-        read_dx();
-        next();
-      }
       const float2 gn = pair(-acc[0] * inv_c * rx), gm = pair(p.layer ? -acc[1] * inv_c * rx : 0.f);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -518,6 +508,182 @@ __global__ void __launch_bounds__(MAXT) gated_norm_bwd_kernel(const __grid_const
         put8(out + col, sa);
         put8(out + p.cols + col, sb);
         put8(out + 2 * p.cols + col, sc);
+      }
+    }
+    a = b;
+  }
+}
+
+// The same for wide rows. A row is read from the ring twice: once for its five sums (dx = dx' + rx (g - mean(g) - n mean(g n)) is linear in its
+// two means, so with the sums of u (dx' + rx g), u and u n, u = y ry gate post_weight, the sum over t y ry comes out
+// of the same meeting), once for the outputs; only the column sums live in registers throughout.
+template <typename T, typename P, bool HAS_Y, int VPT, int N4, int MAXT>
+__global__ void __launch_bounds__(MAXT) gated_norm_bwd_wide_kernel(const __grid_constant__ GatedNormParams p) {
+  constexpr int NIN = HAS_Y ? 4 : 3;  // x, dh, dx', y
+  extern __shared__ __align__(16) uint8_t smem[];
+  __shared__ __align__(16) float meeting[Meet<N4>::kFloats];
+  const int tpr = p.tpr, groups = blockDim.x / tpr;
+  const Meet<N4> meet(meeting, tpr);
+  const int group = meet.group;
+  int flip = 0, col[VPT];
+  bool on[VPT];
+#pragma unroll
+  for (int v = 0; v < VPT; ++v) {
+    col[v] = (v * tpr + (int)threadIdx.x - group * tpr) * 8;
+    on[v] = col[v] < p.cols;
+  }
+  float* gw = reinterpret_cast<float*>(smem);
+  float* sw = gw + p.cols;
+  const uint32_t ring = smem_u32(sw + p.cols) + threadIdx.x * 16, piece = blockDim.x * 16, stage = NIN * VPT * piece;
+  const float inv_c = 1.f / (float)p.cols;
+  const bool post = HAS_Y && p.post_weight != nullptr;
+
+  const Share s = share_of_block(p);
+  int seq = s.seq;
+  for (int64_t a = s.r0; a < s.r1;) {
+    while (seq + 1 < p.seqs && seq_begin(p, seq + 1) <= a) ++seq;
+    const int64_t b = min(s.r1, seq + 1 < p.seqs ? seq_begin(p, seq + 1) : p.rows);
+    const int n = (int)max((b - a - group + groups - 1) / groups, (int64_t)0);
+    int to_load = n, load_row = (int)a + group;
+    uint32_t put = ring, get = ring;
+    const uint32_t end = ring + p.stages * stage;
+    auto issue = [&]() {
+      if (to_load > 0) {
+        --to_load;
+#pragma unroll
+        for (int v = 0; v < VPT; ++v)
+          if (on[v]) {
+            cp_async16(put + v * piece, at<T>(p.x, load_row, p.x_row, col[v]), 16);
+            if (p.dh) cp_async16(put + (VPT + v) * piece, at<T>(p.dh, load_row, p.dh_row, col[v]), 16);
+            if (p.dx_new) cp_async16(put + (2 * VPT + v) * piece, at<T>(p.dx_new, load_row, p.dx_new_row, col[v]), 16);
+            if (HAS_Y) cp_async16(put + (3 * VPT + v) * piece, at<T>(p.y, load_row, p.y_row, col[v]), 16);
+          }
+        load_row += groups;
+        put = put + stage == end ? ring : put + stage;
+      }
+      cp_async_commit();
+    };
+    for (int i = 0; i < p.stages - 1; ++i) issue();
+    __syncthreads();  // the last run's parameters and sums are no longer read
+    if (group == 0)
+#pragma unroll
+      for (int v = 0; v < VPT; ++v) load_params<T, P>(p, seq, col[v], on[v], gw, sw, nullptr);
+    __syncthreads();
+    V8 sa[VPT], sb[VPT], sc[VPT];
+#pragma unroll
+    for (int v = 0; v < VPT; ++v) sa[v] = sb[v] = sc[v] = splat(0.f);
+    int row = (int)a + group;
+    // the rows' statistics, one row ahead of their use
+    float nry = 0.f, nmean = 0.f, nrx = 0.f;
+    auto load_stats = [&](int r) {
+      nry = p.stats[r];
+      nmean = p.stats[p.rows + r];
+      nrx = p.stats[2 * p.rows + r];
+    };
+    if (n > 0) load_stats(row);
+    for (int it = 0; it < n; ++it, row += groups) {
+      issue();  // into the stage that the last row was read from
+      wait_stages(p.stages - 1);
+      const float ry = nry, mean = nmean, rx = nrx;
+      // n, y ry, dh and dx' of the formulas, gate post_weight, weight (1 + scale), for one vector of columns
+      V8 xn, yn, dh, dx, g, w;
+      auto read = [&](int v) {
+        xn = unpack8<T>(ld_shared16(get + v * piece));
+        dh = dx = splat(0.f);
+        if (p.dh) dh = unpack8<T>(ld_shared16(get + (VPT + v) * piece));
+        if (p.dx_new) dx = unpack8<T>(ld_shared16(get + (2 * VPT + v) * piece));
+        w = get_apart(sw, p.cols, col[v]);
+        if constexpr (HAS_Y) {
+          yn = unpack8<T>(ld_shared16(get + (3 * VPT + v) * piece));
+          g = get_apart(gw, p.cols, col[v]);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            yn.v[i] = __fmul2_rn(yn.v[i], pair(ry));
+            xn.v[i] = __ffma2_rn(g.v[i], yn.v[i], xn.v[i]);
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) xn.v[i] = __fmul2_rn(__fadd2_rn(xn.v[i], pair(-mean)), pair(rx));
+      };
+      float acc[5] = {0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int v = 0; v < VPT; ++v)
+        if (on[v]) {
+          read(v);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            sb[v].v[i] = __ffma2_rn(dh.v[i], xn.v[i], sb[v].v[i]);
+            sc[v].v[i] = __fadd2_rn(sc[v].v[i], dh.v[i]);
+            dh.v[i] = __fmul2_rn(dh.v[i], w.v[i]);  // g of the formulas
+          }
+          acc[0] += dot8(dh, xn);
+          acc[1] += sum8(dh);
+          if (post) {
+            V8 u;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              u.v[i] = __fmul2_rn(yn.v[i], g.v[i]);
+              dx.v[i] = __ffma2_rn(dh.v[i], pair(rx), dx.v[i]);
+            }
+            acc[2] += dot8(u, dx);
+            acc[3] += sum8(u);
+            acc[4] += dot8(u, xn);
+          }
+        }
+      if (it + 1 < n) load_stats(row + groups);
+      if (post) {
+        meet.sum(acc, flip);
+      } else {
+        float two[2] = {acc[0], acc[1]};
+        meet.sum(two, flip);
+        acc[0] = two[0];
+        acc[1] = two[1];
+      }
+      const float gn = -acc[0] * inv_c * rx, gm = p.layer ? -acc[1] * inv_c * rx : 0.f;
+      const float m = -fmaf(gm, acc[3], fmaf(gn, acc[4], acc[2])) * inv_c;  // -mean(t y ry)
+#pragma unroll
+      for (int v = 0; v < VPT; ++v)
+        if (on[v]) {
+          read(v);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            dh.v[i] = __fmul2_rn(dh.v[i], w.v[i]);
+            dx.v[i] = __fadd2_rn(dx.v[i], __ffma2_rn(dh.v[i], pair(rx), __ffma2_rn(xn.v[i], pair(gn), pair(gm))));
+            if constexpr (HAS_Y) {
+              sa[v].v[i] = __ffma2_rn(dx.v[i], yn.v[i], sa[v].v[i]);
+              dh.v[i] = __fmul2_rn(dx.v[i], g.v[i]);  // t of the formulas
+              if (post) dh.v[i] = __fmul2_rn(__ffma2_rn(yn.v[i], pair(m), dh.v[i]), pair(ry));
+            }
+          }
+          *reinterpret_cast<uint4*>(at<T>(p.dx, row, p.cols, col[v])) = pack8<T>(dx);
+          if constexpr (HAS_Y) *reinterpret_cast<uint4*>(at<T>(p.dy, row, p.cols, col[v])) = pack8<T>(dh);
+        }
+      get = get + stage == end ? ring : get + stage;
+    }
+    cp_async_wait<0>();
+    if (p.part) {
+      // this block's column sums of the sequence: slot blockIdx + seq (both only grow, so no two share one). The
+      // groups' sums one after another through shared memory (the parameters' place and the ring behind it)
+      float* out = p.part + ((int64_t)blockIdx.x + seq) * 3 * p.cols;
+      float* sums = reinterpret_cast<float*>(smem);
+      if (groups > 1) __syncthreads();
+      for (int g2 = 0; g2 < groups; ++g2) {
+        if (group == g2)
+#pragma unroll
+          for (int v = 0; v < VPT; ++v)
+            if (on[v])
+#pragma unroll
+              for (int q = 0; q < 3; ++q) {
+                V8& mine = q == 0 ? sa[v] : q == 1 ? sb[v] : sc[v];
+                if (g2 > 0) {
+                  const V8 f = get_apart(sums + q * p.cols, p.cols, col[v]);
+#pragma unroll
+                  for (int i = 0; i < 4; ++i) mine.v[i] = __fadd2_rn(mine.v[i], f.v[i]);
+                }
+                if (g2 == groups - 1) put8(out + q * p.cols + col[v], mine);
+                else put_apart(sums + q * p.cols, p.cols, col[v], mine);
+              }
+        if (groups > 1) __syncthreads();
       }
     }
     a = b;
@@ -629,29 +795,37 @@ cudaError_t run(Kern kern, std::atomic<uint64_t>& ready, const Shape& s, GatedNo
 // Forward. Few rows (a serving step: one a block at most): one vector a thread, the shortest way through a row
 // (24 rows of 5120: 5.5 us, with four vectors 7.6 us). Else four vectors a thread: a row's sums then cost a
 // quarter per column, and four rows of 5120 columns are under way on an SM with 640 threads (16576 rows, layer
-// norm with a post norm: 141 us; two vectors and two or three rows 152 us; the floor is 104 us).
+// norm with a post norm: 119 us, two vectors 130 us; the floor is 104 us). Rows that would leave lanes
+// without a vector take fewer, and so do rows so wide that four vectors would leave an SM less than 512 threads.
 template <typename T, typename P, bool Y>
 cudaError_t forward(const GatedNormParams& p, cudaStream_t st) {
-  static std::atomic<uint64_t> ready[8];
+  static std::atomic<uint64_t> ready[10];
   const int nin = Y ? 2 : 1;
-  if (p.rows <= 148) {
-    const Shape s = shape_of(p.cols, p.rows, 1, 1, 1, 3, nin);
+  if (p.rows <= 148 || p.cols <= 256) {
+    const Shape s = shape_of(p.cols, p.rows, 1, p.rows <= 148 ? 1 : 640, 1, 3, nin);
     if (s.tpr <= 32) return run(gated_norm_fwd_kernel<T, P, Y, 1, 0, 1024>, ready[0], s, p, st);
     if (s.tpr <= 128) return run(gated_norm_fwd_kernel<T, P, Y, 1, 1, 1024>, ready[1], s, p, st);
     if (s.tpr <= 256) return run(gated_norm_fwd_kernel<T, P, Y, 1, 2, 1024>, ready[2], s, p, st);
     if (s.tpr <= 640) return run(gated_norm_fwd_kernel<T, P, Y, 1, 5, 1024>, ready[3], s, p, st);
     return run(gated_norm_fwd_kernel<T, P, Y, 1, 8, 1024>, ready[4], s, p, st);
   }
+  if (p.cols <= 512) return run(gated_norm_fwd_kernel<T, P, Y, 2, 0, 640>, ready[5], shape_of(p.cols, p.rows, 2, 640, 1, 3, nin), p, st);
   const Shape s = shape_of(p.cols, p.rows, 4, 640, 1, 3, nin);
-  if (s.tpr <= 32) return run(gated_norm_fwd_kernel<T, P, Y, 4, 0, 640>, ready[5], s, p, st);
-  if (s.tpr <= 128) return run(gated_norm_fwd_kernel<T, P, Y, 4, 1, 640>, ready[6], s, p, st);
-  return run(gated_norm_fwd_kernel<T, P, Y, 4, 2, 640>, ready[7], s, p, st);
+  if (s.tpr <= 32) return run(gated_norm_fwd_kernel<T, P, Y, 4, 0, 640>, ready[6], s, p, st);
+  if (s.tpr <= 128) return run(gated_norm_fwd_kernel<T, P, Y, 4, 1, 640>, ready[7], s, p, st);
+  if (s.threads < 512) return run(gated_norm_fwd_kernel<T, P, Y, 2, 4, 640>, ready[8], shape_of(p.cols, p.rows, 2, 640, 1, 3, nin), p, st);
+  return run(gated_norm_fwd_kernel<T, P, Y, 4, 2, 640>, ready[9], s, p, st);
 }
 
-// Backward: one vector a thread (the column sums take 24 registers of it already).
+// Backward: one vector a thread, whose row lives in registers between its two readings (16576 rows of 5120
+// columns: 213 us, read twice with two vectors a thread 283 us; the floor is 157 us). Rows of more than 640
+// threads would spill at one vector: two vectors a thread there, read twice (10360 rows of 8192 columns: 245 us, the
+// other way 485 us).
+bool wide(const GatedNormParams& p) { return row_threads(p.cols, 1) > 640; }
 Shape backward_shape(const GatedNormParams& p) {
-  const int tpr = row_threads(p.cols, 1);
-  return shape_of(p.cols, p.rows, 1, 256, tpr <= 256 ? 2 : 1, 2, p.y ? 4 : 3);
+  const int nin = p.y ? 4 : 3;
+  if (wide(p)) return shape_of(p.cols, p.rows, 2, 512, 1, 2, nin);
+  return shape_of(p.cols, p.rows, 1, 256, row_threads(p.cols, 1) <= 256 ? 2 : 1, 2, nin);
 }
 template <typename T, typename P, bool Y>
 cudaError_t backward(const GatedNormParams& p, cudaStream_t st) {
@@ -659,11 +833,11 @@ cudaError_t backward(const GatedNormParams& p, cudaStream_t st) {
   if (p.rows > 0) {
     static std::atomic<uint64_t> ready[5];
     cudaError_t e;
-    if (s.tpr <= 32) e = run(gated_norm_bwd_kernel<T, P, Y, 0, 256, false>, ready[0], s, p, st);
-    else if (s.tpr <= 128) e = run(gated_norm_bwd_kernel<T, P, Y, 1, 256, false>, ready[1], s, p, st);
-    else if (s.tpr <= 256) e = run(gated_norm_bwd_kernel<T, P, Y, 2, 256, false>, ready[2], s, p, st);
-    else if (s.tpr <= 640) e = run(gated_norm_bwd_kernel<T, P, Y, 5, 640, false>, ready[3], s, p, st);
-    else e = run(gated_norm_bwd_kernel<T, P, Y, 8, 1024, true>, ready[4], s, p, st);
+    if (wide(p)) e = run(gated_norm_bwd_wide_kernel<T, P, Y, 2, 4, 512>, ready[4], s, p, st);
+    else if (s.tpr <= 32) e = run(gated_norm_bwd_kernel<T, P, Y, 0, 256>, ready[0], s, p, st);
+    else if (s.tpr <= 128) e = run(gated_norm_bwd_kernel<T, P, Y, 1, 256>, ready[1], s, p, st);
+    else if (s.tpr <= 256) e = run(gated_norm_bwd_kernel<T, P, Y, 2, 256>, ready[2], s, p, st);
+    else e = run(gated_norm_bwd_kernel<T, P, Y, 5, 640>, ready[3], s, p, st);
     if (e != cudaSuccess) return e;
   }
   if (!p.part) return cudaSuccess;
