@@ -305,10 +305,12 @@ int vmb_cast_f32_view(const float* src, const vmb_view* src_view, void* dst, con
  * queries (kv_units: of the sequence's) in the backward's statistics, where every sequence starts
  * at a multiple of 128; stat_rows is their total. part: -1, or the slot (0 .. n_parts - 1) of a
  * piece of work that is split over its key tiles (dQ, forward) or steps (dK / dV); the pieces of a
- * split unit take consecutive slots, and `joins` lists them as (first unit, number of pieces).
+ * split unit take consecutive slots, and `joins` lists them as (first unit, number of pieces). lone
+ * (kv_units): the sequence's queries below it see one key at most, so their dS is zero; 0 where that is
+ * not known. pieces: the host's own.
  */
 typedef struct vmb_packed_unit {
-  int32_t q_row, q_valid, k_row, k_valid, vis0, begin, end, part, stat_row, reserved[3];
+  int32_t q_row, q_valid, k_row, k_valid, vis0, begin, end, part, stat_row, pieces, lone, reserved;
 } vmb_packed_unit;
 
 typedef struct vmb_packed_list {

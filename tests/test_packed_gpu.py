@@ -194,3 +194,30 @@ def test_refusals():
     for scale in (-1.0, float("inf"), float("nan")):
         with pytest.raises(AssertionError, match="sm_scale"):
             packed_attention(q, k, v, PackedSequences([8]), sm_scale=scale)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("ql, kl, causal", [([1, 1, 1], None, True), ([70, 1, 3], [1, 1, 1], False), ([200, 90], [1, 1], True)])
+def test_one_visible_key_passes_no_score_gradient(ql, kl, causal, dtype):
+    """A softmax over one key is constant: the gradients of q and k are zeros, not roundings of zero."""
+    kl = kl or ql
+    q, k, v, do = make(ql, kl, 4, 2, 64, dtype)
+    seqs = PackedSequences(ql, kl)
+    _, dq, dk, dv = grads(lambda *x: packed_attention(*x, seqs, causal=causal), (q, k, v), do)
+    assert not dq.any() and not dk.any() and dv.any()
+
+
+@pytest.mark.parametrize("size", [2.0 ** -14, 1.0, 2.0 ** 10])
+def test_fp16_gradients_of_many_keys(size):
+    """P of 6000 keys and dS of small gradients lie below fp16's normal range: 4 u as in the module's docstring
+    (outputs that are themselves below it excepted: their spacing is 2^-24)."""
+    ql, kl = [64], [6000]
+    q, k, v, do = make(ql, kl, 2, 1, 64, torch.float16)
+    do = (do * size).to(torch.float16)
+    do[:5] = 0
+    seqs = PackedSequences(ql, kl)
+    got = grads(lambda *x: packed_attention(*x, seqs), (q, k, v), do)
+    want = grads(lambda *x: packed_reference(*x, ql, kl, False, 64 ** -0.5)[0], [t.double() for t in (q, k, v)], do)
+    for x, ref in zip(got[1:], want[1:]):
+        err = (x.double() - ref).norm().item()
+        assert err <= 4 * U[torch.float16] * ref.norm().item() + 2.0 ** -25 * x.numel() ** 0.5

@@ -77,7 +77,12 @@ int head_chunk(int64_t bytes_per_head, int heads) {
   return (int)std::max<int64_t>(1, std::min<int64_t>(n, heads));
 }
 
-int64_t stat_bytes(const vmb_packed_args* a) { return up256(2 * a->heads * a->stat_rows * 4); }
+// Statistics of a backward: three planes of rows, a value per 128 rows and head, 128 per 128 rows and key head.
+int64_t plane_bytes(const vmb_packed_args* a) { return up256(3 * a->heads * a->stat_rows * 4); }
+int64_t tile_bytes(const vmb_packed_args* a) { return up256(a->heads * (a->stat_rows / 128) * 4); }
+int64_t stat_bytes(const vmb_packed_args* a) {
+  return plane_bytes(a) + tile_bytes(a) + up256(a->kv_heads * (a->stat_rows / 128) * 128 * 4);
+}
 
 vmb::PackedParams params(const vmb_packed_args* a) {
   vmb::PackedParams p{};
@@ -139,6 +144,8 @@ int vmb_packed_bwd(const vmb_packed_args* a, void* stream) {
   if ((rc = workspace(a, "vmb_packed_bwd", vmb_packed_bwd_workspace_bytes(a)))) return rc;
   vmb::PackedParams dq = params(a), kv = dq;
   dq.stats = kv.stats = static_cast<float*>(a->workspace);
+  dq.tile_scale = kv.tile_scale = dq.stats + plane_bytes(a) / 4;
+  dq.centre = kv.centre = dq.tile_scale + tile_bytes(a) / 4;
   dq.units = reinterpret_cast<const vmb::PackedUnit*>(a->q_units.units);
   dq.n_units = a->q_units.n_units;
   dq.head_chunk = std::min(a->heads, dq.group * head_chunk(4 * a->k_total * a->dim, a->kv_heads));

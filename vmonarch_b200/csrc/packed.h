@@ -18,9 +18,10 @@ namespace vmb {
 //                   vis0 + r on (all of them when not causal); the unit walks steps [begin, end) of
 //                   its (query head of the group, 64-query tile) pairs, the tiles of a head counted
 //                   from max(vis0, 0) / 64. stat_row: the sequence's first padded statistics row.
+//                   The sequence's queries below `lone` see one key at most.
 //  part           : -1, or the slot that a split unit's partial result goes to
 struct PackedUnit {
-  int32_t q_row, q_valid, k_row, k_valid, vis0, begin, end, part, stat_row, pad0, pad1, pad2;
+  int32_t q_row, q_valid, k_row, k_valid, vis0, begin, end, part, stat_row, pieces, lone, pad;
 };
 
 struct PackedParams {
@@ -34,7 +35,9 @@ struct PackedParams {
   const void *q, *k, *v, *dout;
   void *o, *o_low, *dq, *dk, *dv;  // o_low: the 16-bit rest that rounding o left out (may be NULL, forward)
   float* lse;              // [heads][q_total], natural logarithm
-  float* stats;            // backward: planes nl, nc, each [heads][stat_rows]
+  float* stats;            // backward: planes nl, nc, row scales, each [heads][stat_rows]
+  float* tile_scale;       // backward: least row scale of 128 rows, [heads][stat_rows / 128]
+  float* centre;           // backward: mean of a sequence's first keys, [kv_heads][stat_rows / 128][128]
   float *part, *part_ml;   // split units: partial tiles and their (max, sum)
   View qv, kv, vv, ov, olv, dov, dqv, dkv, dvv;  // rows = tokens, s1 = head stride
 };

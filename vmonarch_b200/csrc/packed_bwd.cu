@@ -7,7 +7,8 @@
 // atomics, so the gradients are the same from run to run:
 //
 // pre   one row per half-warp: nl = -lse log2(e) and nc = -sm_scale D in planes [head][stat_rows], in
-//       which every sequence starts at a multiple of 128 (rows past its end: P = 0). Then
+//       which every sequence starts at a multiple of 128 (rows past its end: P = 0), and the mean
+//       of the sequence's first keys for dq. Then
 //       P = 2^(s c + nl) and dS = P (sm_scale dP + nc): two packed FMAs, one exponential, one product.
 //       D takes o with the 16 bits that its rounding left out (o_low): an error of D is shared by a
 //       whole row of dS, so it does not average out in dQ_i = sum_j dS_ij k_j where keys have a mean
@@ -21,7 +22,9 @@
 //       thread = query row x 32 keys. A row of dS sums to zero, its rounded values do not quite, and what they
 //       leave would weigh the mean that keys share: dQ_i = sum_j dS_ij (k_j - c) for any c, so the sum of the
 //       rounded values times the mean of the sequence's first keys is taken off at the end (15600 causal queries
-//       around a mean of 0.3, D = 128, bf16: error of dQ 1.49 -> 1.4x times that of its own rounding). TMEM: S0 [0,128) S1 [128,256) dP [256,384) dQ [384, +64 NA).
+//       around a mean of 0.3, D = 128, bf16: error of dQ 1.49 -> 1.43 times that of its own rounding).
+//       TMEM: S0 [0,128) S1 [128,256) dP [256,384) dQ [384, +64 NA).
+// A query that sees one key has dS = 0 by its index, where dP - D would leave a rounding.
 // Seven products per tile pair instead of five: TMEM cannot hold S, dP, dK, dV and dQ of one tile at
 // once, and recomputing S and dP costs less than adding dQ through memory.
 //
@@ -52,6 +55,15 @@ struct KParams {
   PackedParams a;
   float scale_log2;
 };
+
+// Below 2^-14 fp16 loses bits, which P of a few thousand keys, and dS of small dO, would reach: P is held as 2^8 P, and
+// dS as 2^8 s dS with the power of two s that brings sm_scale |dO| into (2^-6, 2^-5], of a row in dq, of the largest of
+// the rows that meet in one dK in dkdv. |2^8 s dS| <= 2^8 2^-5 2 |v| stays in range while |v| < 4094; 16000 keys of
+// |v| = sqrt(D) lie around 2^-12 (14061 keys, D = 96: errors of dQ and dK 1.51 and 1.53 -> 1.42 and 1.44 times those of
+// their own rounding). bf16 has the range, s = 1.
+template <typename T>
+constexpr float kPScale = Elem<T>::is_bf16 ? 1.f : 256.f;
+constexpr float kMaxScale = 1152921504606846976.f;  // 2^60, the scale of rows that need none
 
 // P and dS of two scores, packed to 16 bits.
 __device__ __forceinline__ float2 prob2(uint32_t s0, uint32_t s1, float2 sc2, float2 nl2) {
@@ -190,15 +202,49 @@ __global__ void __launch_bounds__(256) packed_sum_kernel(const __grid_constant__
 // Block = one 128-query unit of one head; 16 lanes per row, 16 bytes each of o and dO.
 template <typename T>
 __global__ void __launch_bounds__(256) packed_pre_kernel(const __grid_constant__ PackedParams a) {
+  __shared__ float4 sums[16][32];
+  __shared__ float least[16];
   const UnitHead uh = unit_of_block(blockIdx.x, a.n_units, a.heads, a.heads);
   const PackedUnit u = a.units[uh.unit];
   const int head = uh.head, sub = threadIdx.x & 15;
   float* nl = a.stats + (int64_t)head * a.stat_rows + u.stat_row;
   float* nc = nl + (int64_t)a.heads * a.stat_rows;
+  float* ns = nc + (int64_t)a.heads * a.stat_rows;
+  if (head % a.group == 0) {
+    // the mean of up to 128 first keys of the unit's sequence (for dq)
+    const int keys = min(u.k_valid, 128), kvh = head / a.group;
+    float f[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = 0.f;
+    if (sub * 8 < a.dim) {
+      const T* k = static_cast<const T*>(a.k) + (int64_t)u.k_row * a.kv.rs + (int64_t)kvh * a.kv.s1 + sub * 8;
+#pragma unroll 8
+      for (int r = threadIdx.x >> 4; r < keys; r += 16) {
+        const uint4 x = *reinterpret_cast<const uint4*>(k + (int64_t)r * a.kv.rs);
+        const uint32_t xs[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float2 v = Elem<T>::unpack(xs[i]);
+          f[2 * i] += v.x;
+          f[2 * i + 1] += v.y;
+        }
+      }
+    }
+    sums[threadIdx.x >> 4][2 * sub] = make_float4(f[0], f[1], f[2], f[3]);
+    sums[threadIdx.x >> 4][2 * sub + 1] = make_float4(f[4], f[5], f[6], f[7]);
+    __syncthreads();
+    if (threadIdx.x < 128) {
+      float s = 0.f;
+#pragma unroll
+      for (int g = 0; g < 16; ++g) s += reinterpret_cast<const float*>(sums[g])[threadIdx.x];
+      a.centre[((int64_t)kvh * (a.stat_rows >> 7) + (u.stat_row >> 7)) * 128 + threadIdx.x] = keys > 0 ? s / (float)keys : 0.f;
+    }
+  }
+  float low = kMaxScale;
 #pragma unroll 2
   for (int r = threadIdx.x >> 4; r < 128; r += 16) {
     const bool valid = r < u.q_valid;
-    float d = 0.f;
+    float d = 0.f, norm = 0.f;
     if (valid && sub * 8 < a.dim) {
       const int64_t row = u.q_row + r;
       auto load = [&](const void* t, const View& v) {
@@ -210,15 +256,36 @@ __global__ void __launch_bounds__(256) packed_pre_kernel(const __grid_constant__
       for (int i = 0; i < 4; ++i) {
         const float2 f = Elem<T>::unpack(xs[i]), l = Elem<T>::unpack(ws[i]), g = Elem<T>::unpack(ys[i]);
         d = fmaf(f.x + l.x, g.x, fmaf(f.y + l.y, g.y, d));
+        norm = fmaf(g.x, g.x, fmaf(g.y, g.y, norm));
       }
     }
 #pragma unroll
-    for (int s = 8; s > 0; s >>= 1) d += __shfl_xor_sync(0xffffffffu, d, s);
+    for (int s = 8; s > 0; s >>= 1) {
+      d += __shfl_xor_sync(0xffffffffu, d, s);
+      if (!Elem<T>::is_bf16) norm += __shfl_xor_sync(0xffffffffu, norm, s);
+    }
+    if (!Elem<T>::is_bf16) {
+      // rows without a gradient and those past the end do not count
+      const float size = a.sm_scale * sqrtf(norm);
+      const float s = valid && size > 0.f && isfinite(size) ? exp2f(fminf(fmaxf(-5.f - ceilf(log2f(size)), -60.f), 60.f))
+                                                            : kMaxScale;
+      low = fminf(low, s);
+      if (sub == 0) ns[r] = s;
+    }
     if (sub == 0) {
       // finite, so that a row without keys and the rows past the end have P = 2^(finite - 1e30) = 0
       const float lse = valid ? a.lse[(int64_t)head * a.q_total + u.q_row + r] : -INFINITY;
-      nl[r] = lse == -INFINITY ? -1e30f : -lse * kLog2e;
+      nl[r] = lse == -INFINITY ? -1e30f : fmaf(-lse, kLog2e, Elem<T>::is_bf16 ? 0.f : 8.f);
       nc[r] = valid ? -a.sm_scale * d : 0.f;
+    }
+  }
+  if (!Elem<T>::is_bf16) {
+    if (sub == 0) least[threadIdx.x >> 4] = low;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+#pragma unroll
+      for (int g = 1; g < 16; ++g) low = fminf(low, least[g]);
+      a.tile_scale[(int64_t)head * (a.stat_rows >> 7) + (u.stat_row >> 7)] = low;
     }
   }
 }
@@ -398,6 +465,17 @@ __global__ void __launch_bounds__(kThreads, 1) packed_dkdv_kernel(const __grid_c
     };
     const uint32_t ts = tmem + lane_off + 128 * stm, tdp = ts + 64;
     const float2 sc2 = make_float2(p.scale_log2, p.scale_log2), sm2 = make_float2(p.a.sm_scale, p.a.sm_scale);
+    float ds_scale = 1.f;  // fp16: of all the rows that meet in this unit's dK
+    if (!kBf16) {
+      const int tiles = (u.q_valid + 127) >> 7;
+      ds_scale = kMaxScale;
+      for (int i = lane; i < tiles * p.a.group; i += 32)
+        ds_scale = fminf(ds_scale, p.a.tile_scale[((int64_t)kvh * p.a.group + i / tiles) * (p.a.stat_rows >> 7) +
+                                                  (u.stat_row >> 7) + i % tiles]);
+#pragma unroll
+      for (int x = 16; x > 0; x >>= 1) ds_scale = fminf(ds_scale, __shfl_xor_sync(0xffffffffu, ds_scale, x));
+    }
+    const float2 ss2 = make_float2(ds_scale, ds_scale);
     bool ok = true;
     for (int i = stm; i < n; i += 2) {
       const int s = i % NQ;
@@ -406,8 +484,8 @@ __global__ void __launch_bounds__(kThreads, 1) packed_dkdv_kernel(const __grid_c
       tc_fence_after();
       const int q0 = step_q0(i), left = u.q_valid - q0;
       // key `row` is seen by the tile's queries [c_lo, left)
-      const bool masked = left < 64 || u.vis0 + 127 > q0;
-      const int c_lo = u.vis0 + row - q0;
+      const bool masked = left < 64 || u.vis0 + 127 > q0 || u.lone > q0;
+      const int c_lo = u.vis0 + row - q0, c_ds = max(c_lo, u.lone - q0);
       if (left < 64) {  // S^T and dP^T of the tile are complete: only dK and dV still read the slot
         clear_rows(sQ(s), 2 * NA, 64, left, tid, 256);
         fence_proxy_async_smem();
@@ -428,14 +506,18 @@ __global__ void __launch_bounds__(kThreads, 1) packed_dkdv_kernel(const __grid_c
           asm volatile("ld.shared.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(c4.x), "=f"(c4.y), "=f"(c4.z), "=f"(c4.w) : "r"(so + 256));
           float2 p0 = prob2(sv[e], sv[e + 1], sc2, make_float2(l4.x, l4.y));
           float2 p1 = prob2(sv[e + 2], sv[e + 3], sc2, make_float2(l4.z, l4.w));
-          float2 d0 = dscore2(p0, dv[e], dv[e + 1], sm2, make_float2(c4.x, c4.y));
-          float2 d1 = dscore2(p1, dv[e + 2], dv[e + 3], sm2, make_float2(c4.z, c4.w));
+          float2 d0 = dscore2(kBf16 ? p0 : __fmul2_rn(p0, ss2), dv[e], dv[e + 1], sm2, make_float2(c4.x, c4.y));
+          float2 d1 = dscore2(kBf16 ? p1 : __fmul2_rn(p1, ss2), dv[e + 2], dv[e + 3], sm2, make_float2(c4.z, c4.w));
           if (masked) {
             const int c = 16 * qc + e;
-            if (c < c_lo || c >= left) p0.x = d0.x = 0.f;
-            if (c + 1 < c_lo || c + 1 >= left) p0.y = d0.y = 0.f;
-            if (c + 2 < c_lo || c + 2 >= left) p1.x = d1.x = 0.f;
-            if (c + 3 < c_lo || c + 3 >= left) p1.y = d1.y = 0.f;
+            if (c < c_lo || c >= left) p0.x = 0.f;
+            if (c + 1 < c_lo || c + 1 >= left) p0.y = 0.f;
+            if (c + 2 < c_lo || c + 2 >= left) p1.x = 0.f;
+            if (c + 3 < c_lo || c + 3 >= left) p1.y = 0.f;
+            if (c < c_ds || c >= left) d0.x = 0.f;
+            if (c + 1 < c_ds || c + 1 >= left) d0.y = 0.f;
+            if (c + 2 < c_ds || c + 2 >= left) d1.x = 0.f;
+            if (c + 3 < c_ds || c + 3 >= left) d1.y = 0.f;
           }
           pk[e >> 1] = Elem<T>::pack(p0.x, p0.y);
           pk[(e >> 1) + 1] = Elem<T>::pack(p1.x, p1.y);
@@ -453,13 +535,14 @@ __global__ void __launch_bounds__(kThreads, 1) packed_dkdv_kernel(const __grid_c
     tc_fence_after();
     // epilogue: warpgroups 0, 1 stage dK, 2, 3 dV, half of the columns each
     const int mat = wg >> 1;
+    const float unscale = (mat ? 1.f : 1.f / ds_scale) / kPScale<T>;
     if (ok && u.part >= 0)
       store_part(tmem + lane_off + (mat ? T_DV : T_DK),
                  p.a.part + ((((int64_t)u.part * p.a.kv_heads + kvh) * 2 + mat) * 128 + row) * (64 * NA), n > 0, (wg & 1) * NA,
-                 ((wg & 1) + 1) * NA, 1.f);
+                 ((wg & 1) + 1) * NA, unscale);
     else if (ok)
       stage_rows<T>(tmem + lane_off + (mat ? T_DV : T_DK), sSlots + mat * NA * kAtom, row, n > 0, (wg & 1) * NA,
-                    ((wg & 1) + 1) * NA, 1.f);
+                    ((wg & 1) + 1) * NA, unscale);
     ok = named_bar_and(1, 512, ok && !*abort);
     if (ok && u.part < 0) {
       T* out = mat ? static_cast<T*>(p.a.dv) + (int64_t)u.k_row * p.a.dvv.rs + (int64_t)kvh * p.a.dvv.s1
@@ -611,24 +694,17 @@ __global__ void __launch_bounds__(kThreads, 1) packed_dq_kernel(const __grid_con
     const uint32_t lane_off = (uint32_t)(quad * 32) << 16;
     const int tid = threadIdx.x - 64;
     const float* stat = p.a.stats + (int64_t)head * p.a.stat_rows + u.stat_row + row;
-    const float fl = stat[0], fc = stat[(int64_t)p.a.heads * p.a.stat_rows];
-    const float2 nl2 = make_float2(fl, fl), nc2 = make_float2(fc, fc);
-    const float2 sc2 = make_float2(p.scale_log2, p.scale_log2), sm2 = make_float2(p.a.sm_scale, p.a.sm_scale);
+    const int64_t plane = (int64_t)p.a.heads * p.a.stat_rows;
+    const float row_scale = kBf16 ? 1.f : stat[2 * plane];
     const int my_lim = limit(row), lim_lo = limit(0);
+    const float ds_scale = my_lim > 1 ? row_scale : 0.f;  // a softmax over one key has no gradient
+    const float fl = stat[0], fc = stat[plane] * ds_scale, fs = p.a.sm_scale * ds_scale;
+    const float2 nl2 = make_float2(fl, fl), nc2 = make_float2(fc, fc);
+    const float2 sc2 = make_float2(p.scale_log2, p.scale_log2), sm2 = make_float2(fs, fs);
     auto warp_wait = [&](int bar, uint32_t parity, int code) -> bool {
       return __all_sync(0xffffffffu, mbar_wait(BAR(bar), parity, abort, &g_packed_bwd_err, code));
     };
-    // The mean of up to 128 first keys of the sequence (the same for every piece of a cut unit), a column a thread.
-    if (tid < 64 * NA) {
-      const int keys = min(u.k_valid, 128);
-      const T* k = static_cast<const T*>(p.a.k) + (int64_t)u.k_row * p.a.kv.rs + (int64_t)kvh * p.a.kv.s1 + tid;
-      float s = 0.f;
-      if (tid < p.a.dim) {
-#pragma unroll 8
-        for (int r = 0; r < keys; ++r) s += Elem<T>::to_f(k[(int64_t)r * p.a.kv.rs]);
-      }
-      centre_sh[tid] = keys > 0 ? s / (float)keys : 0.f;
-    }
+    if (tid < 64 * NA) centre_sh[tid] = p.a.centre[((int64_t)kvh * (p.a.stat_rows >> 7) + (u.stat_row >> 7)) * 128 + tid];
     float sum = 0.f;  // of this thread's rounded dS
     bool ok = true;
     for (int j = 0; j < n; ++j) {
@@ -677,12 +753,13 @@ __global__ void __launch_bounds__(kThreads, 1) packed_dq_kernel(const __grid_con
     // epilogue: 16-bit dQ through the idle K ring; a warpgroup stages 32-column chunks wg, wg + 4, ...
     ok = named_bar_and(1, 512, ok);
     if (ok && wg < 2 * NA) {
+      const float unscale = 1.f / (row_scale * kPScale<T>);
       const float off = (sums[row] + sums[128 + row]) + (sums[256 + row] + sums[384 + row]);
       if (u.part >= 0)
         store_part(tmem + lane_off + T_DQ, p.a.part + (((int64_t)u.part * p.a.heads + head) * 128 + row) * (64 * NA), n > 0, wg,
-                   wg + 1, 1.f, off, centre_sh);
+                   wg + 1, unscale, off, centre_sh);
       else
-        stage_rows<T>(tmem + lane_off + T_DQ, sK, row, n > 0, wg, wg + 1, 1.f, off, centre_sh);
+        stage_rows<T>(tmem + lane_off + T_DQ, sK, row, n > 0, wg, wg + 1, unscale, off, centre_sh);
     }
     ok = named_bar_and(1, 512, ok && !*abort);
     if (ok && u.part < 0)

@@ -139,6 +139,8 @@ class PackedSequences:
         u[:, 6] = group * np.maximum(-(-nq // _STEP) - np.maximum(vis0, 0) // _STEP, 0)
         u[:, 7] = -1
         u[:, 8] = self.stat_start[seq]
+        # queries below this one see one key at most, and a softmax over one key has no gradient
+        u[:, 10] = np.maximum(nq - nk + 1, 0) if causal else np.where(nk == 1, nq, 0)
         return u
 
     def _list(self, kind, causal, heads, group):
@@ -292,7 +294,7 @@ def packed_attention(q, k, v, seqs, *, causal=False, sm_scale=None, return_lse=F
     projection) are read in place, others through a dense copy. Rows of other sequences and keys that
     a query does not see take no part, whatever they hold; in the backward pass that covers other
     sequences' rows, while within a sequence a value that is not finite reaches the gradients of its
-    whole 64- or 128-row tile.
+    whole 64- or 128-row tile. The fp16 backward needs value rows with a norm below 4094.
     """
     dtype = q.dtype
     assert dtype in SUPPORTED_DTYPES, f"unsupported dtype {dtype}"
