@@ -251,3 +251,12 @@ def stream_ptr(device: torch.device) -> int:
 
 #: handle of a device's current stream, by device index (torch.cuda.current_stream builds a Stream object around it)
 raw_stream = torch._C._cuda_getCurrentRawStream
+
+
+def once_differentiable(backward):
+    """torch's decorator of that name, whose bookkeeping is left out while no graph of the gradients is recorded."""
+    recorded = torch.autograd.function.once_differentiable(backward)
+
+    def run(ctx, *grads):
+        return (recorded if torch.is_grad_enabled() else backward)(ctx, *grads)
+    return run

@@ -15,16 +15,15 @@ from .kernel import SUPPORTED_DTYPES
 MAX_WIDTH = 8192
 
 
-def _place(t):
-    """`t` (T, C), or a dense copy where the kernels cannot address it in place (contiguous columns, 16-byte
+def _place(t, rows, cols):
+    """`t` (rows, cols), or a dense copy where the kernels cannot address it in place (contiguous columns, 16-byte
     aligned rows), and its vmb_matrix."""
     ptr, (row, col) = t.data_ptr(), t.stride()
-    n, c = t.shape
-    if n <= 1:
-        row = c
+    if rows <= 1:
+        row = cols
     if col != 1 or row < 0 or row & 7 or ptr & 15:
         t = _dense(t.contiguous())
-        ptr, row = t.data_ptr(), c
+        ptr, row = t.data_ptr(), cols
     return t, ptr, row
 
 
@@ -38,31 +37,20 @@ _PARAMS = ("gate", "scale", "shift", "weight", "post_weight")
 _ARGS = struct.Struct("25q5if")
 assert _ARGS.size == N.GatedNormArgs.workspace.offset
 _NO_GRADS = (0,) * 11
+_NO_ROWS = None, 0, 0
 
 
-def _sizes(x, params, seqs, norm, eps):
-    dtype = N.dtype_code(x.dtype)
-    fp32 = any(t is not None and t.dtype == torch.float32 for t in params)
-    rows, cols = x.shape
-    return rows, cols, 1 if seqs is None else seqs.num_sequences, dtype, N.VMB_DTYPE_F32 if fp32 else dtype, norm == "layer", eps
-
-
-def _starts(seqs):
-    return seqs._starts().data_ptr() if seqs is not None and seqs.num_sequences > 1 else 0
-
-
-def _forward(x, y, params, seqs, norm, eps, stats):
-    x, *xr = _place(x)
-    yr = (0, 0)
-    if y is not None:
-        y, *yr = _place(y)
-    params = [t if t is None else _dense(t) for t in params]
-    x_new = torch.empty_like(x, memory_format=torch.contiguous_format) if y is not None else None
+def _forward(x, y, params, seqs, sizes, stats):
+    rows, cols = sizes[:2]
+    x, x_ptr, x_row = _place(x, rows, cols)
+    y, y_ptr, y_row = _NO_ROWS if y is None else _place(y, rows, cols)
+    params = [None if t is None else _dense(t) for t in params]
+    x_new = None if y is None else torch.empty_like(x, memory_format=torch.contiguous_format)
     h = torch.empty_like(x, memory_format=torch.contiguous_format)
     a = N.GatedNormArgs()
-    _ARGS.pack_into(a, 0, *xr, *yr, 0 if x_new is None else x_new.data_ptr(), h.data_ptr(),
+    _ARGS.pack_into(a, 0, x_ptr, x_row, y_ptr, y_row, 0 if x_new is None else x_new.data_ptr(), h.data_ptr(),
                     *[0 if t is None else t.data_ptr() for t in params], 0 if stats is None else stats.data_ptr(),
-                    _starts(seqs), *_NO_GRADS, *_sizes(x, params, seqs, norm, eps))
+                    seqs._starts().data_ptr() if sizes[2] > 1 else 0, *_NO_GRADS, *sizes)
     rc = N.lib.vmb_gated_norm_fwd(ctypes.byref(a), N.raw_stream(x.device.index))
     if rc:
         N.check(rc, "vmb_gated_norm_fwd")
@@ -71,36 +59,33 @@ def _forward(x, y, params, seqs, norm, eps, stats):
 
 class _GatedNorm(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, y, seqs, norm, eps, *params):
-        shapes = [None if t is None else t.shape for t in params]
-        stats = torch.empty((3, x.size(0)), dtype=torch.float32, device=x.device)
-        x, y_in, dense, x_new, h = _forward(x, y, params, seqs, norm, eps, stats)
-        ctx.save_for_backward(x, y_in, stats, *dense)
-        ctx.meta = seqs, norm, eps, shapes
+    def forward(ctx, x, y, seqs, sizes, *params):
+        stats = torch.empty(3 * sizes[0], dtype=torch.float32, device=x.device)
+        x, y, params, x_new, h = _forward(x, y, params, seqs, sizes, stats)
+        ctx.save_for_backward(x, y, stats, *params)
+        ctx.meta = seqs, sizes
         ctx.set_materialize_grads(False)
         return (h,) if y is None else (x_new, h)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @N.once_differentiable
     def backward(ctx, *grads):
         x, y, stats, *params = ctx.saved_tensors
-        seqs, norm, eps, shapes = ctx.meta
-        dx_new, dh = grads if y is not None else (None, *grads)
-        dxr = dhr = yr = (0, 0)
-        if dx_new is not None:
-            dx_new, *dxr = _place(dx_new)
-        if dh is not None:
-            dh, *dhr = _place(dh)
-        if y is not None:
-            yr = _place(y)[1:]
+        seqs, sizes = ctx.meta
+        rows, cols = sizes[:2]
+        dx_new, dh = (None, *grads) if y is None else grads
+        dx_new, dxn_ptr, dxn_row = _NO_ROWS if dx_new is None else _place(dx_new, rows, cols)
+        dh, dh_ptr, dh_row = _NO_ROWS if dh is None else _place(dh, rows, cols)
+        _, x_ptr, x_row = _place(x, rows, cols)
+        _, y_ptr, y_row = _NO_ROWS if y is None else _place(y, rows, cols)
         dx = torch.empty_like(x, memory_format=torch.contiguous_format)
-        dy = torch.empty_like(x, memory_format=torch.contiguous_format) if y is not None else None
-        out = [torch.empty(shape, dtype=t.dtype, device=x.device) if t is not None and need else None
-               for t, need, shape in zip(params, ctx.needs_input_grad[5:], shapes)]
+        dy = None if y is None else torch.empty_like(x, memory_format=torch.contiguous_format)
+        out = [torch.empty_like(t) if need and t is not None else None for t, need in zip(params, ctx.needs_input_grad[4:])]
         a = N.GatedNormArgs()
-        _ARGS.pack_into(a, 0, *_place(x)[1:], *yr, 0, 0, *[0 if t is None else t.data_ptr() for t in params],
-                        stats.data_ptr(), _starts(seqs), *dxr, *dhr, dx.data_ptr(), 0 if dy is None else dy.data_ptr(),
-                        *[0 if t is None else t.data_ptr() for t in out], *_sizes(x, params, seqs, norm, eps))
+        _ARGS.pack_into(a, 0, x_ptr, x_row, y_ptr, y_row, 0, 0, *[0 if t is None else t.data_ptr() for t in params],
+                        stats.data_ptr(), seqs._starts().data_ptr() if sizes[2] > 1 else 0, dxn_ptr, dxn_row, dh_ptr, dh_row,
+                        dx.data_ptr(), 0 if dy is None else dy.data_ptr(),
+                        *[0 if t is None else t.data_ptr() for t in out], *sizes)
         size = N.lib.vmb_gated_norm_bwd_workspace_bytes(ctypes.byref(a))
         if size > 0:
             ws = torch.empty(size, dtype=torch.uint8, device=x.device)
@@ -108,7 +93,7 @@ class _GatedNorm(torch.autograd.Function):
         rc = N.lib.vmb_gated_norm_bwd(ctypes.byref(a), N.raw_stream(x.device.index))
         if rc:
             N.check(rc, "vmb_gated_norm_bwd")
-        return (dx, dy, None, None, None, *out)
+        return (dx, dy, None, None, *out)
 
 
 def gated_residual_norm(x, y=None, *, gate=None, scale=None, shift=None, weight=None, post_weight=None, norm="rms",
@@ -132,35 +117,43 @@ def gated_residual_norm(x, y=None, *, gate=None, scale=None, shift=None, weight=
         (x_new, h), both (T, C) in x's dtype; with y None (x, h)
     All arithmetic is 32-bit; h is formed from x_new before its rounding.
     """
-    assert x.dtype in SUPPORTED_DTYPES, f"unsupported dtype {x.dtype}"
-    assert x.dim() == 2, "x must be (T, C)"
-    c = x.size(1)
+    kind, device, shape = x.dtype, x.device, x.shape
+    assert kind in SUPPORTED_DTYPES, f"unsupported dtype {kind}"
+    assert len(shape) == 2, "x must be (T, C)"
+    rows, c = shape
     assert 8 <= c <= MAX_WIDTH and c % 8 == 0, f"width {c} is not a multiple of 8 up to {MAX_WIDTH}"
-    assert y is None or (y.shape == x.shape and y.dtype == x.dtype and y.device == x.device), "y must be like x"
+    assert y is None or (y.shape == shape and y.dtype == kind and y.device == device), "y must be like x"
     assert y is not None or (gate is None and post_weight is None), "gate and post_weight need y"
     assert norm in ("rms", "layer"), f"norm must be 'rms' or 'layer', not {norm!r}"
     eps = float(eps)
     assert 0 <= eps < float("inf"), "eps must be finite and not negative"
     assert x.is_cuda, "vmonarch_b200 needs CUDA tensors"
+    count = 1
     if seqs is not None:
-        assert seqs.device == x.device, "x and seqs must be on one CUDA device"
-        assert seqs.total_q == x.size(0), f"x has {x.size(0)} rows, the sequences {seqs.total_q}"
-        assert seqs.num_sequences <= 65535, "at most 65535 sequences"
+        count = seqs.num_sequences
+        assert seqs.device == device, "x and seqs must be on one CUDA device"
+        assert seqs.total_q == rows, f"x has {rows} rows, the sequences {seqs.total_q}"
+        assert count <= 65535, "at most 65535 sequences"
     params = (gate, scale, shift, weight, post_weight)
-    dtype = None
+    dtype, needed = None, x.requires_grad or (y is not None and y.requires_grad)
     for name, t in zip(_PARAMS, params):
         if t is None:
             continue
-        assert t.device == x.device, f"{name} must be on x's device"
-        assert t.dtype in (x.dtype, torch.float32) and t.dtype == (dtype or t.dtype), \
-            "the parameters must share one dtype, x's or fp32"
-        dtype = t.dtype
-        if name in ("weight", "post_weight") or seqs is None:
-            assert t.shape == (c,) or (seqs is None and t.shape == (1, c)), f"{name} must be ({c},)"
+        assert t.device == device, f"{name} must be on x's device"
+        if t.dtype != dtype:
+            assert dtype is None and t.dtype in (kind, torch.float32), "the parameters must share one dtype, x's or fp32"
+            dtype = t.dtype
+        if seqs is None:
+            assert t.shape == (c,) or t.shape == (1, c), f"{name} must be ({c},)"
+        elif name in ("weight", "post_weight"):
+            assert t.shape == (c,), f"{name} must be ({c},)"
         else:
-            assert t.shape == (seqs.num_sequences, c), f"{name} must be ({seqs.num_sequences}, {c})"
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, y, *params)):
-        out = _GatedNorm.apply(x, y, seqs, norm, eps, *params)
+            assert t.shape == (count, c), f"{name} must be ({count}, {c})"
+        needed = needed or t.requires_grad
+    code = N.dtype_code(kind)
+    sizes = (rows, c, count, code, N.VMB_DTYPE_F32 if dtype == torch.float32 else code, norm == "layer", eps)
+    if needed and torch.is_grad_enabled():
+        out = _GatedNorm.apply(x, y, seqs, sizes, *params)
         return (x, out[0]) if y is None else out
-    x_new, h = _forward(x, y, params, seqs, norm, eps, None)[3:]
+    x_new, h = _forward(x, y, params, seqs, sizes, None)[3:]
     return (x if y is None else x_new), h

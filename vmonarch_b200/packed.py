@@ -251,7 +251,7 @@ class _PackedAttention(torch.autograd.Function):
         return o, lse
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @N.once_differentiable
     def backward(ctx, do, _=None):
         q, k, v, o, aux, *lse = ctx.saved_tensors
         seqs, key = ctx.meta
