@@ -369,6 +369,7 @@ __global__ void __launch_bounds__(kThreads, 1) packed_fwd_kernel(const __grid_co
       ++queries;
       for (int w = 0; w < 2; ++w)
         if (ok && it.n_kt[w] > 0) ok = issue_s(w, 0, ks0, kp0);
+      if (ok && it.n_max == 1) mma_commit_if(leader, BAR(B_QFREE));
       for (int t = 0; ok && t < it.n_max; ++t) {
         if (++ks0 == NK) ks0 = 0, kp0 ^= 1;  // the next K tile
 #pragma unroll
@@ -396,9 +397,9 @@ __global__ void __launch_bounds__(kThreads, 1) packed_fwd_kernel(const __grid_co
           if (t + 1 < it.n_kt[w]) ok = issue_s(w, t + 1, ks0, kp0);
           else mma_commit_if(leader, BAR(B_OFULL + w));
         }
+        if (ok && t + 2 == it.n_max) mma_commit_if(leader, BAR(B_QFREE));  // the last scores are on their way
         if (++vs0 == NV) vs0 = 0, vp0 ^= 1;
       }
-      if (ok) mma_commit_if(leader, BAR(B_QFREE));
       for (int w = 0; w < 2; ++w) {
         steps[w] += it.n_kt[w];
         outs[w] += it.n_kt[w] > 0;
