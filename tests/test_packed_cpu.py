@@ -77,21 +77,26 @@ def test_key_units_cover_keys_and_the_queries_that_see_them(ql, kl, causal):
     assert (seen == 1).all()
 
 
-def test_longest_work_first_and_cut_to_the_share():
-    """No piece is much above the SMs' fair share of a call's steps, nor below the least worth a piece."""
-    from vmonarch_b200.packed import _LEAST
-    for lens in ([5, 900, 40, 333], [30000], [8000, 100], [200] * 60):
+def test_longest_work_first_and_cut_where_the_sms_finish_sooner():
+    """Pieces are never below half the least worth a piece, and a cut list is done before the uncut one, its join
+    included; large lists hold no unit much above the SMs' fair share."""
+    from vmonarch_b200.packed import _JOIN, _JOINED, _LEAST, _MANY, _PIECE, _SETUP, _span
+    for lens in ([5, 900, 40, 333], [30000], [8000, 100], [200] * 60, [3677], [130]):
         for kind in ("fwd", "dq", "kv"):
             for heads, group in ((2, 2), (40, 5), (1, 1)):
                 seqs = PackedSequences(lens, device="cpu")
                 info = seqs._list(kind, True, heads, group)
                 u = seqs._cache[(kind, True, heads, group)][1].numpy()[:12 * info.n_units].reshape(-1, 12)
-                work = u[:, 6] - u[:, 5]
+                work, part = u[:, 6] - u[:, 5], u[:, 7] >= 0
                 assert (np.diff(work) <= 0).all()
                 blocks = heads // group if kind == "kv" else heads
-                share = max(_LEAST[kind], -(-int(work.sum()) * blocks // 148))
-                assert work.max() <= share + share // 4
-                assert not (u[:, 7] >= 0).any() or work[u[:, 7] >= 0].min() >= share // 2
+                whole = seqs._key_units(True, group) if kind == "kv" else seqs._query_units(256 if kind == "fwd" else 128, True)
+                if part.any():
+                    assert work[part].min() >= _LEAST[kind] // 2
+                    after = _span(np.sort(-work - _PIECE * part), blocks, _SETUP[kind]) + _JOIN + part.sum() * blocks // _JOINED
+                    assert after < _span(np.sort(-whole[:, 6]), blocks, _SETUP[kind])
+                if len(whole) * blocks > _MANY:
+                    assert work.max() <= max(_LEAST[kind], -(-int(work.sum()) * blocks // 148)) * 5 // 4 + 1
 
 
 @pytest.mark.parametrize("bad", [dict(lengths=[]), dict(lengths=[3, -1]), dict(lengths=[3], kv_lengths=[1, 2]),

@@ -70,7 +70,7 @@ int workspace(const vmb_packed_args* a, const char* what, int64_t need) {
   return VMB_OK;
 }
 
-// Heads whose keys and values (or queries and output gradients) are walked together: as many as keep
+// Heads whose keys and values are walked together: as many as keep
 // about 48 MB between them, so that the blocks in flight share them in L2 (126 MB on B200).
 int head_chunk(int64_t bytes_per_head, int heads) {
   const int64_t n = (int64_t(48) << 20) / std::max<int64_t>(bytes_per_head, 1);
@@ -151,7 +151,7 @@ int vmb_packed_bwd(const vmb_packed_args* a, void* stream) {
   dq.head_chunk = std::min(a->heads, dq.group * head_chunk(4 * a->k_total * a->dim, a->kv_heads));
   kv.units = reinterpret_cast<const vmb::PackedUnit*>(a->kv_units.units);
   kv.n_units = a->kv_units.n_units;
-  kv.head_chunk = head_chunk(4 * a->q_total * a->dim * dq.group, a->kv_heads);
+  kv.head_chunk = a->kv_heads;  // all of them: units of a second chunk would start too late to end evenly
   dq.joins = a->q_units.joins;
   dq.n_joins = a->q_units.n_parts > 0 ? a->q_units.n_joins : 0;
   dq.part = dq.stats + stat_bytes(a) / 4;

@@ -8,6 +8,7 @@ a :class:`PackedSequences`, which every layer of a step then shares.
 from __future__ import annotations
 
 import ctypes
+import heapq
 import struct
 
 import numpy as np
@@ -24,6 +25,11 @@ _NEVER_MASKED = -(1 << 30)
 _SMS = 148
 # least steps of a piece when a unit is cut: below it, set-up and join cost more than the cut gains
 _LEAST = {"fwd": 8, "dq": 8, "kv": 16}
+# measured, in steps (of 1.1 to 2 us): what a unit costs beside its own and what a piece of one costs more, and the
+# kernel that joins the pieces: its launch, and how many pieces it joins in a step
+_SETUP, _PIECE, _JOIN, _JOINED = {"fwd": 3, "dq": 5, "kv": 8}, 3, 3, 40
+# lists of more blocks than this (eight for each SM) are even enough without looking
+_MANY = 8 * _SMS
 
 
 def _lengths(x, what):
@@ -44,22 +50,59 @@ def _tiles(lens, rows):
     return seq, first
 
 
-def _cut(u, heads, least):
-    """Cuts units of a list that would still run when the SMs' fair share of all work is done into equal
-    pieces of at least `least` steps; returns the list and its number of pieces (parts)."""
-    steps = u[:, 6] - u[:, 5]
-    share = max(least, -(-int(steps.sum()) * heads // _SMS))
-    pieces = np.where(steps > share + share // 4, -(-steps // share), 1)
-    if not len(u) or pieces.max() == 1:
-        return u, 0
-    which = np.repeat(np.arange(len(u)), pieces)
+def _span(steps, heads, setup):
+    """Steps until the last SM is done, when units of -`steps` steps start in list order wherever an SM is free."""
+    load = [0] * _SMS
+    for n in steps.tolist():
+        n = setup - n
+        for _ in range(heads):
+            heapq.heapreplace(load, load[0] + n)
+    return max(load)
+
+
+def _pieces(steps, limit):
+    """How many equal pieces of about `limit` steps each unit makes."""
+    return np.maximum(-(-steps // limit), 1)
+
+
+def _piece_steps(steps, pieces):
+    which = np.repeat(np.arange(len(steps)), pieces)
     k = np.arange(len(which)) - np.repeat(np.cumsum(pieces) - pieces, pieces)  # piece of its unit
+    n, total = pieces[which], steps[which]
+    return which, k, total * k // n, total * (k + 1) // n
+
+
+def _cut(u, heads, kind):
+    """Cuts the units of a list into equal pieces, so far as the SMs finish sooner by it: the pieces' set-up
+    and their join included. Returns the list and its number of pieces (parts)."""
+    steps = u[:, 6].astype(np.int64)
+    if not len(u):
+        return u, 0
+    least, setup = _LEAST[kind], _SETUP[kind]
+    share = max(-(-int(steps.sum()) * heads // _SMS), 1)
+    limits = [max(least, -(-share * n // 8)) for n in (11, 10, 9, 8, 4, 2)]
+    best = _pieces(steps, limits[1])  # a unit far above everybody's fair share is cut in any case
+    if len(u) * heads <= _MANY:
+        best, best_cost = None, 0
+        for limit in dict.fromkeys([int(steps.max()) + 1, *limits]):
+            pieces = _pieces(steps, limit)
+            if best is not None and (best_cost <= 1.03 * (share + setup) or pieces.max() == 1):
+                continue
+            which, _, begin, end = _piece_steps(steps, pieces)
+            cut = pieces[which] > 1
+            cost = _span(np.sort(begin - end - _PIECE * cut), heads, setup)
+            if cut.any():
+                cost += _JOIN + int(cut.sum()) * heads // _JOINED
+            if best is None or cost < 0.98 * best_cost:
+                best, best_cost = pieces, cost
+    if best.max() == 1:
+        return u, 0
+    which, k, begin, end = _piece_steps(steps, best)
     out = u[which]
-    out[:, 5] = u[which, 5] + steps[which] * k // pieces[which]
-    out[:, 6] = u[which, 5] + steps[which] * (k + 1) // pieces[which]
-    is_part = pieces[which] > 1
+    out[:, 5], out[:, 6] = begin, end
+    is_part = best[which] > 1
     out[is_part, 7] = np.arange(int(is_part.sum()))
-    out[:, 9] = np.where(k == 0, pieces[which], 0)  # for _joins; the kernels do not read it
+    out[:, 9] = np.where(k == 0, best[which], 0)  # for _joins; the kernels do not read it
     return out, int(is_part.sum())
 
 
@@ -151,10 +194,10 @@ class PackedSequences:
         if hit is None:
             if kind == "kv":
                 u = self._key_units(causal, group)
-                u, parts = _cut(u, heads // group, _LEAST[kind])
+                u, parts = _cut(u, heads // group, kind)
             else:
                 u = self._query_units(_FWD_ROWS if kind == "fwd" else _DQ_ROWS, causal)
-                u, parts = _cut(u, heads, _LEAST[kind])
+                u, parts = _cut(u, heads, kind)
             u = u[np.argsort(u[:, 5] - u[:, 6], kind="stable")]
             joins = _joins(u)
             dev = torch.from_numpy(np.concatenate([u.reshape(-1), joins.reshape(-1)])).to(self.device)
