@@ -315,7 +315,7 @@ __global__ void __launch_bounds__(kThreads, 1) packed_dkdv_kernel(const __grid_c
   auto pcol = [](int kk) -> uint32_t { return 32 * (kk >> 1) + 8 * (kk & 1); };
 
   extern __shared__ uint8_t smem_raw[];
-  __shared__ __align__(8) uint64_t bars[6 + 2 * NQ];
+  __shared__ __align__(8) uint64_t bars[10 + 2 * NQ];
   __shared__ uint32_t tmem_base_sh;
   __shared__ int abort_sh;
 
@@ -337,10 +337,12 @@ __global__ void __launch_bounds__(kThreads, 1) packed_dkdv_kernel(const __grid_c
   auto sStat = [&](int s) { return sSlots + s * C::SLOT + C::SLOT_T; };
   const uint32_t bar0 = smem_u32(bars);
   const uint32_t BAR_KV = bar0, BAR_DONE = bar0 + 8u;
-  auto BAR_SP = [&](int b) { return bar0 + 8u * (2 + b); };
-  auto BAR_PDS = [&](int b) { return bar0 + 8u * (4 + b); };
-  auto BAR_QFULL = [&](int s) { return bar0 + 8u * (6 + s); };
-  auto BAR_QEMPTY = [&](int s) { return bar0 + 8u * (6 + NQ + s); };
+  auto BAR_S = [&](int b) { return bar0 + 8u * (2 + b); };
+  auto BAR_DP = [&](int b) { return bar0 + 8u * (4 + b); };
+  auto BAR_P = [&](int b) { return bar0 + 8u * (6 + b); };
+  auto BAR_DS = [&](int b) { return bar0 + 8u * (8 + b); };
+  auto BAR_QFULL = [&](int s) { return bar0 + 8u * (10 + s); };
+  auto BAR_QEMPTY = [&](int s) { return bar0 + 8u * (10 + NQ + s); };
   volatile int* abort = &abort_sh;
 
   if (threadIdx.x == 0) {
@@ -348,8 +350,10 @@ __global__ void __launch_bounds__(kThreads, 1) packed_dkdv_kernel(const __grid_c
     mbar_init(BAR_KV, 1);
     mbar_init(BAR_DONE, 1);
     for (int b = 0; b < 2; ++b) {
-      mbar_init(BAR_SP(b), 1);
-      mbar_init(BAR_PDS(b), 256);
+      mbar_init(BAR_S(b), 1);
+      mbar_init(BAR_DP(b), 1);
+      mbar_init(BAR_P(b), 256);
+      mbar_init(BAR_DS(b), 256);
     }
     for (int s = 0; s < NQ; ++s) {
       mbar_init(BAR_QFULL(s), 1);
@@ -409,43 +413,49 @@ __global__ void __launch_bounds__(kThreads, 1) packed_dkdv_kernel(const __grid_c
     auto wwait = [&](uint32_t bar, uint32_t parity, int code) -> bool {
       return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort, &g_packed_bwd_err, code));
     };
-    auto issue_sp = [&](int i) -> bool {
-      const int s = i % NQ;
-      if (!wwait(BAR_QFULL(s), (i / NQ) & 1, 2)) return false;
+    // S^T = K Q^T or dP^T = V dO^T of step i, whose slot has landed
+    auto issue = [&](int i, bool dp) {
+      const uint32_t tb = tmem + 128 * (i & 1) + (dp ? 64 : 0), sa = dp ? sV : sK, sb = dp ? sDO(i % NQ) : sQ(i % NQ);
+#pragma unroll
+      for (int kk = 0; kk < 4 * NA; ++kk) {
+        const uint32_t oa = (kk >> 2) * kAtom + (kk & 3) * 32, ob = (kk >> 2) * kAtom64 + (kk & 3) * 32;
+        mma_ss_if(leader, tb, smem_desc_sw128(sa + oa, 16, 1024), smem_desc_sw128(sb + ob, 16, 1024), IDESC_SP, kk > 0);
+      }
+      mma_commit_if(leader, dp ? BAR_DP(i & 1) : BAR_S(i & 1));
+    };
+    auto landed = [&](int i) -> bool {
+      if (!wwait(BAR_QFULL(i % NQ), (i / NQ) & 1, 2)) return false;
       tc_fence_after();
-      const uint32_t tb = tmem + 128 * (i & 1);
-#pragma unroll
-      for (int kk = 0; kk < 4 * NA; ++kk) {  // S^T = K Q^T
-        const uint32_t oa = (kk >> 2) * kAtom + (kk & 3) * 32, ob = (kk >> 2) * kAtom64 + (kk & 3) * 32;
-        mma_ss_if(leader, tb, smem_desc_sw128(sK + oa, 16, 1024), smem_desc_sw128(sQ(s) + ob, 16, 1024), IDESC_SP, kk > 0);
-      }
-#pragma unroll
-      for (int kk = 0; kk < 4 * NA; ++kk) {  // dP^T = V dO^T
-        const uint32_t oa = (kk >> 2) * kAtom + (kk & 3) * 32, ob = (kk >> 2) * kAtom64 + (kk & 3) * 32;
-        mma_ss_if(leader, tb + 64, smem_desc_sw128(sV + oa, 16, 1024), smem_desc_sw128(sDO(s) + ob, 16, 1024), IDESC_SP,
-                  kk > 0);
-      }
-      mma_commit_if(leader, BAR_SP(i & 1));
       return true;
     };
     bool ok = n <= 0 || wwait(BAR_KV, 0, 2);
-    if (ok && n > 0) ok = issue_sp(0);
-    if (ok && n > 1) ok = issue_sp(1);
+    for (int i = 0; ok && i < min(n, 2); ++i) {
+      if (!(ok = landed(i))) break;
+      issue(i, false);
+      issue(i, true);
+    }
+    // A stream's S^T of step i + 2 runs while its warps still work on dS^T of step i, its dP^T while they work on P^T
     for (int i = 0; ok && i < n; ++i) {
-      if (!wwait(BAR_PDS(i & 1), (i >> 1) & 1, 4)) break;
-      tc_fence_after();
       const int s = i % NQ;
       const uint32_t pt = tmem + 128 * (i & 1), dst = pt + 64;
+      if (!wwait(BAR_P(i & 1), (i >> 1) & 1, 4)) break;
+      tc_fence_after();
 #pragma unroll
-      for (int kk = 0; kk < 4; ++kk)  // dK += dS^T Q over 64 queries
-        mma_ts_if(leader, tmem + T_DK, dst + pcol(kk), smem_desc_sw128(sQ(s) + kk * 2048, kAtom64, 1024), IDESC_ACC,
-                  (i > 0 || kk > 0) ? 1u : 0u);
-#pragma unroll
-      for (int kk = 0; kk < 4; ++kk)  // dV += P^T dO
+      for (int kk = 0; kk < 4; ++kk)  // dV += P^T dO over 64 queries
         mma_ts_if(leader, tmem + T_DV, pt + pcol(kk), smem_desc_sw128(sDO(s) + kk * 2048, kAtom64, 1024), IDESC_ACC,
                   (i > 0 || kk > 0) ? 1u : 0u);
+      if (i + 2 < n) {
+        if (!landed(i + 2)) break;
+        issue(i + 2, false);
+      }
+      if (!wwait(BAR_DS(i & 1), (i >> 1) & 1, 4)) break;
+      tc_fence_after();
+#pragma unroll
+      for (int kk = 0; kk < 4; ++kk)  // dK += dS^T Q
+        mma_ts_if(leader, tmem + T_DK, dst + pcol(kk), smem_desc_sw128(sQ(s) + kk * 2048, kAtom64, 1024), IDESC_ACC,
+                  (i > 0 || kk > 0) ? 1u : 0u);
       mma_commit_if(leader, BAR_QEMPTY(s));
-      if (i + 2 < n) ok = issue_sp(i + 2);
+      if (i + 2 < n) issue(i + 2, true);
     }
     if (elect_one()) {
       mma_commit(BAR_DONE);
@@ -479,57 +489,76 @@ __global__ void __launch_bounds__(kThreads, 1) packed_dkdv_kernel(const __grid_c
     bool ok = true;
     for (int i = stm; i < n; i += 2) {
       const int s = i % NQ;
-      if (!warp_wait(BAR_SP(stm), (i >> 1) & 1, 8)) { ok = false; break; }
-      if (!warp_wait(BAR_QFULL(s), (i / NQ) & 1, 8)) { ok = false; break; }
+      if (!warp_wait(BAR_S(stm), (i >> 1) & 1, 8) || !warp_wait(BAR_QFULL(s), (i / NQ) & 1, 8)) { ok = false; break; }
       tc_fence_after();
       const int q0 = step_q0(i), left = u.q_valid - q0;
       // key `row` is seen by the tile's queries [c_lo, left)
       const bool masked = left < 64 || u.vis0 + 127 > q0 || u.lone > q0;
-      const int c_lo = u.vis0 + row - q0, c_ds = max(c_lo, u.lone - q0);
-      if (left < 64) {  // S^T and dP^T of the tile are complete: only dK and dV still read the slot
+      const int c_lo = u.vis0 + row - q0 - 32 * half, c_hi = left - 32 * half;
+      if (left < 64) {
+        // S^T is complete, and what dP^T still reads only goes into queries past the end: clear for dK and dV
         clear_rows(sQ(s), 2 * NA, 64, left, tid, 256);
         fence_proxy_async_smem();
       }
-      const uint32_t st = sStat(s);
-#pragma unroll 1
-      for (int qc = 2 * half; qc < 2 * half + 2; ++qc) {  // 16-query chunks
-        uint32_t sv[16], dv[16];
-        tmem_ld16(ts + 16 * qc, sv);
-        tmem_ld16(tdp + 16 * qc, dv);
+      const uint32_t st = sStat(s) + 128 * half;
+      float2 pr[16];  // P^T of the thread's 32 queries
+      {
+        uint32_t sv[32], pk[16];
+        tmem_ld32(ts + 32 * half, sv);
         tmem_wait_ld();
-        uint32_t pk[8], dk[8];
 #pragma unroll
-        for (int e = 0; e < 16; e += 4) {
-          const uint32_t so = st + 4 * (16 * qc + e);
-          float4 l4, c4;
-          asm volatile("ld.shared.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(l4.x), "=f"(l4.y), "=f"(l4.z), "=f"(l4.w) : "r"(so));
-          asm volatile("ld.shared.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(c4.x), "=f"(c4.y), "=f"(c4.z), "=f"(c4.w) : "r"(so + 256));
+        for (int e = 0; e < 32; e += 4) {
+          float4 l4;
+          asm volatile("ld.shared.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(l4.x), "=f"(l4.y), "=f"(l4.z), "=f"(l4.w) : "r"(st + 4 * e));
           float2 p0 = prob2(sv[e], sv[e + 1], sc2, make_float2(l4.x, l4.y));
           float2 p1 = prob2(sv[e + 2], sv[e + 3], sc2, make_float2(l4.z, l4.w));
-          float2 d0 = dscore2(kBf16 ? p0 : __fmul2_rn(p0, ss2), dv[e], dv[e + 1], sm2, make_float2(c4.x, c4.y));
-          float2 d1 = dscore2(kBf16 ? p1 : __fmul2_rn(p1, ss2), dv[e + 2], dv[e + 3], sm2, make_float2(c4.z, c4.w));
           if (masked) {
-            const int c = 16 * qc + e;
-            if (c < c_lo || c >= left) p0.x = 0.f;
-            if (c + 1 < c_lo || c + 1 >= left) p0.y = 0.f;
-            if (c + 2 < c_lo || c + 2 >= left) p1.x = 0.f;
-            if (c + 3 < c_lo || c + 3 >= left) p1.y = 0.f;
-            if (c < c_ds || c >= left) d0.x = 0.f;
-            if (c + 1 < c_ds || c + 1 >= left) d0.y = 0.f;
-            if (c + 2 < c_ds || c + 2 >= left) d1.x = 0.f;
-            if (c + 3 < c_ds || c + 3 >= left) d1.y = 0.f;
+            if (e < c_lo || e >= c_hi) p0.x = 0.f;
+            if (e + 1 < c_lo || e + 1 >= c_hi) p0.y = 0.f;
+            if (e + 2 < c_lo || e + 2 >= c_hi) p1.x = 0.f;
+            if (e + 3 < c_lo || e + 3 >= c_hi) p1.y = 0.f;
           }
           pk[e >> 1] = Elem<T>::pack(p0.x, p0.y);
           pk[(e >> 1) + 1] = Elem<T>::pack(p1.x, p1.y);
-          dk[e >> 1] = Elem<T>::pack(d0.x, d0.y);
-          dk[(e >> 1) + 1] = Elem<T>::pack(d1.x, d1.y);
+          pr[e >> 1] = kBf16 ? p0 : __fmul2_rn(p0, ss2);
+          pr[(e >> 1) + 1] = kBf16 ? p1 : __fmul2_rn(p1, ss2);
         }
-        tmem_st8(ts + pcol(qc), pk);
-        tmem_st8(tdp + pcol(qc), dk);
+        tmem_st16(ts + pcol(2 * half), pk);
       }
       tmem_wait_st();
       tc_fence_before();
-      mbar_arrive(BAR_PDS(stm));
+      mbar_arrive(BAR_P(stm));
+      if (!warp_wait(BAR_DP(stm), (i >> 1) & 1, 8)) { ok = false; break; }
+      tc_fence_after();
+      const int d_lo = max(c_lo, u.lone - q0 - 32 * half);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        uint32_t dv[16], dk[8];
+        tmem_ld16(tdp + 32 * half + 16 * h, dv);
+        tmem_wait_ld();
+#pragma unroll
+        for (int e = 0; e < 16; e += 4) {
+          float4 c4;
+          asm volatile("ld.shared.v4.f32 {%0,%1,%2,%3}, [%4];"
+                       : "=f"(c4.x), "=f"(c4.y), "=f"(c4.z), "=f"(c4.w)
+                       : "r"(st + 256 + 64 * h + 4 * e));
+          float2 d0 = dscore2(pr[8 * h + (e >> 1)], dv[e], dv[e + 1], sm2, make_float2(c4.x, c4.y));
+          float2 d1 = dscore2(pr[8 * h + (e >> 1) + 1], dv[e + 2], dv[e + 3], sm2, make_float2(c4.z, c4.w));
+          if (masked) {
+            const int c = 16 * h + e;
+            if (c < d_lo || c >= c_hi) d0.x = 0.f;
+            if (c + 1 < d_lo || c + 1 >= c_hi) d0.y = 0.f;
+            if (c + 2 < d_lo || c + 2 >= c_hi) d1.x = 0.f;
+            if (c + 3 < d_lo || c + 3 >= c_hi) d1.y = 0.f;
+          }
+          dk[e >> 1] = Elem<T>::pack(d0.x, d0.y);
+          dk[(e >> 1) + 1] = Elem<T>::pack(d1.x, d1.y);
+        }
+        tmem_st8(tdp + pcol(2 * half + h), dk);
+      }
+      tmem_wait_st();
+      tc_fence_before();
+      mbar_arrive(BAR_DS(stm));
     }
     if (ok) ok = warp_wait(BAR_DONE, 0, 8);
     tc_fence_after();
