@@ -32,6 +32,8 @@
 // rows that enter a sum with weight 0 (Q and dO here, K in dq) are cleared in shared memory first, so
 // that nothing another sequence holds (0 x inf) gets into it. P and dS are 16-bit operands of the tensor
 // cores; sums, statistics and accumulators are 32-bit.
+#include <type_traits>
+
 #include "common.cuh"
 #include "launch.h"
 #include "packed.h"
@@ -502,7 +504,7 @@ __global__ void __launch_bounds__(kThreads, 1) packed_dkdv_kernel(const __grid_c
       }
       const uint32_t st = sStat(s) + 128 * half;
       float2 pr[16];  // P^T of the thread's 32 queries
-      {
+      auto p_phase = [&](auto mask) {
         uint32_t sv[32], pk[16];
         tmem_ld32(ts + 32 * half, sv);
         tmem_wait_ld();
@@ -512,7 +514,7 @@ __global__ void __launch_bounds__(kThreads, 1) packed_dkdv_kernel(const __grid_c
           asm volatile("ld.shared.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(l4.x), "=f"(l4.y), "=f"(l4.z), "=f"(l4.w) : "r"(st + 4 * e));
           float2 p0 = prob2(sv[e], sv[e + 1], sc2, make_float2(l4.x, l4.y));
           float2 p1 = prob2(sv[e + 2], sv[e + 3], sc2, make_float2(l4.z, l4.w));
-          if (masked) {
+          if (mask) {
             if (e < c_lo || e >= c_hi) p0.x = 0.f;
             if (e + 1 < c_lo || e + 1 >= c_hi) p0.y = 0.f;
             if (e + 2 < c_lo || e + 2 >= c_hi) p1.x = 0.f;
@@ -524,15 +526,16 @@ __global__ void __launch_bounds__(kThreads, 1) packed_dkdv_kernel(const __grid_c
           pr[(e >> 1) + 1] = kBf16 ? p1 : __fmul2_rn(p1, ss2);
         }
         tmem_st16(ts + pcol(2 * half), pk);
-      }
+      };
+      if (masked) p_phase(std::true_type{});
+      else p_phase(std::false_type{});
       tmem_wait_st();
       tc_fence_before();
       mbar_arrive(BAR_P(stm));
       if (!warp_wait(BAR_DP(stm), (i >> 1) & 1, 8)) { ok = false; break; }
       tc_fence_after();
       const int d_lo = max(c_lo, u.lone - q0 - 32 * half);
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
+      auto ds_phase = [&](int h, auto mask) {
         uint32_t dv[16], dk[8];
         tmem_ld16(tdp + 32 * half + 16 * h, dv);
         tmem_wait_ld();
@@ -544,7 +547,7 @@ __global__ void __launch_bounds__(kThreads, 1) packed_dkdv_kernel(const __grid_c
                        : "r"(st + 256 + 64 * h + 4 * e));
           float2 d0 = dscore2(pr[8 * h + (e >> 1)], dv[e], dv[e + 1], sm2, make_float2(c4.x, c4.y));
           float2 d1 = dscore2(pr[8 * h + (e >> 1) + 1], dv[e + 2], dv[e + 3], sm2, make_float2(c4.z, c4.w));
-          if (masked) {
+          if (mask) {
             const int c = 16 * h + e;
             if (c < d_lo || c >= c_hi) d0.x = 0.f;
             if (c + 1 < d_lo || c + 1 >= c_hi) d0.y = 0.f;
@@ -555,6 +558,13 @@ __global__ void __launch_bounds__(kThreads, 1) packed_dkdv_kernel(const __grid_c
           dk[(e >> 1) + 1] = Elem<T>::pack(d1.x, d1.y);
         }
         tmem_st8(tdp + pcol(2 * half + h), dk);
+      };
+      if (masked) {
+        ds_phase(0, std::true_type{});
+        ds_phase(1, std::true_type{});
+      } else {
+        ds_phase(0, std::false_type{});
+        ds_phase(1, std::false_type{});
       }
       tmem_wait_st();
       tc_fence_before();
@@ -753,15 +763,19 @@ __global__ void __launch_bounds__(kThreads, 1) packed_dq_kernel(const __grid_con
       }
       const bool masked = lim_lo - k0 < 128;
       const int valid = my_lim - k0 - 32 * wg;
+      auto scores = [&](auto mask) {
 #pragma unroll
-      for (int e = 0; e < 32; e += 2) {
-        float2 d = dscore2(prob2(sv[e], sv[e + 1], sc2, nl2), dv[e], dv[e + 1], sm2, nc2);
-        if (masked) {
-          if (e >= valid) d.x = 0.f;
-          if (e + 1 >= valid) d.y = 0.f;
+        for (int e = 0; e < 32; e += 2) {
+          float2 d = dscore2(prob2(sv[e], sv[e + 1], sc2, nl2), dv[e], dv[e + 1], sm2, nc2);
+          if (mask) {
+            if (e >= valid) d.x = 0.f;
+            if (e + 1 >= valid) d.y = 0.f;
+          }
+          pk[e >> 1] = Elem<T>::pack(d.x, d.y);
         }
-        pk[e >> 1] = Elem<T>::pack(d.x, d.y);
-      }
+      };
+      if (masked) scores(std::true_type{});
+      else scores(std::false_type{});
       tmem_st16(ts, pk);
       float2 s0 = make_float2(0.f, 0.f), s1 = s0;
 #pragma unroll
