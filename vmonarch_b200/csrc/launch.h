@@ -102,6 +102,30 @@ cudaError_t allow_smem(Kern kern, int bytes, std::atomic<uint64_t>& done) {
   return e;
 }
 
+#ifdef __CUDACC__
+// Launches a kernel that may be set up while the stream's kernel before it still runs. Every block of it calls
+// wait_for_kernel_before() before it touches global memory.
+template <typename... Params, typename... Args>
+cudaError_t launch_early(void (*kern)(Params...), int64_t blocks, int threads, int smem, cudaStream_t st, const Args&... args) {
+  if (blocks > 0x7fffffff) return cudaErrorInvalidConfiguration;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)blocks);
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.dynamicSmemBytes = (size_t)smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kern, args...);
+}
+// Waits until the stream's kernel before this one is done and its writes are visible.
+__device__ __forceinline__ void wait_for_kernel_before() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+// From here on (all blocks here, or done) the stream's next kernel may be set up, if it was launched for that.
+__device__ __forceinline__ void let_next_kernel_start() { asm volatile("griddepcontrol.launch_dependents;"); }
+#endif
+
 // Adds n to the library's kernel launch count.
 void count_launches(int n);
 // Records `code` and a printf-style message as the calling thread's last error; returns `code`.

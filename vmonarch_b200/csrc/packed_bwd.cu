@@ -160,6 +160,8 @@ __device__ __forceinline__ void store_part(uint32_t taddr, float* to, bool any, 
 // lane. KV: dK and dV of key units, else dQ of query units. Partials [part][head][matrix][128][64 NA].
 template <typename T, int NA, bool KV>
 __global__ void __launch_bounds__(256) packed_sum_kernel(const __grid_constant__ PackedParams a) {
+  wait_for_kernel_before();
+  let_next_kernel_start();
   constexpr int MATS = KV ? 2 : 1;
   const int heads = KV ? a.kv_heads : a.heads;
   int64_t b = blockIdx.x;
@@ -206,6 +208,8 @@ template <typename T>
 __global__ void __launch_bounds__(256) packed_pre_kernel(const __grid_constant__ PackedParams a) {
   __shared__ float4 sums[16][32];
   __shared__ float least[16];
+  wait_for_kernel_before();
+  let_next_kernel_start();
   const UnitHead uh = unit_of_block(blockIdx.x, a.n_units, a.heads, a.heads);
   const PackedUnit u = a.units[uh.unit];
   const int head = uh.head, sub = threadIdx.x & 15;
@@ -322,16 +326,6 @@ __global__ void __launch_bounds__(kThreads, 1) packed_dkdv_kernel(const __grid_c
   __shared__ int abort_sh;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const UnitHead uh = unit_of_block(blockIdx.x, p.a.n_units, p.a.kv_heads, p.a.head_chunk);
-  const PackedUnit u = p.a.units[uh.unit];
-  const int kvh = uh.head;
-  const int t_first = max(u.vis0, 0) >> 6;
-  const int per_head = max(((u.q_valid + 63) >> 6) - t_first, 1);  // tiles of one query head
-  const int n = u.end - u.begin;
-  // step i -> query head and first local query of its tile
-  auto step_head = [&](int i) { return kvh * p.a.group + (u.begin + i) / per_head; };
-  auto step_q0 = [&](int i) { return (t_first + (u.begin + i) % per_head) * 64; };
-
   const uint32_t sbase = (smem_u32(smem_raw) + 1023u) & ~1023u;
   const uint32_t sK = sbase, sV = sbase + NA * kAtom, sSlots = sbase + C::RES;
   auto sQ = [&](int s) { return sSlots + s * C::SLOT; };
@@ -371,6 +365,18 @@ __global__ void __launch_bounds__(kThreads, 1) packed_dkdv_kernel(const __grid_c
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tmem_base_sh;
+  wait_for_kernel_before();
+  let_next_kernel_start();
+
+  const UnitHead uh = unit_of_block(blockIdx.x, p.a.n_units, p.a.kv_heads, p.a.head_chunk);
+  const PackedUnit u = p.a.units[uh.unit];
+  const int kvh = uh.head;
+  const int t_first = max(u.vis0, 0) >> 6;
+  const int per_head = max(((u.q_valid + 63) >> 6) - t_first, 1);  // tiles of one query head
+  const int n = u.end - u.begin;
+  // step i -> query head and first local query of its tile
+  auto step_head = [&](int i) { return kvh * p.a.group + (u.begin + i) / per_head; };
+  auto step_q0 = [&](int i) { return (t_first + (u.begin + i) % per_head) * 64; };
 
   if (warp == 0) {
     // ---------------------------------------------------------------- TMA producer
@@ -624,12 +630,6 @@ __global__ void __launch_bounds__(kThreads, 1) packed_dq_kernel(const __grid_con
   __shared__ __align__(16) float centre_sh[64 * NA];  // mean of the sequence's first keys
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const UnitHead uh = unit_of_block(blockIdx.x, p.a.n_units, p.a.heads, p.a.head_chunk);
-  const PackedUnit u = p.a.units[uh.unit];
-  const int head = uh.head, kvh = head / p.a.group;
-  auto limit = [&](int r) { return max(0, min(u.k_valid, p.a.causal ? u.vis0 + r : u.k_valid)); };
-  const int n = u.end - u.begin;
-
   const uint32_t sbase = (smem_u32(smem_raw) + 1023u) & ~1023u;
   const uint32_t sQ = sbase, sDO = sbase + TILE, sK = sbase + 2 * TILE, sV = sK + NK * TILE;
   const uint32_t bar0 = smem_u32(bars);
@@ -650,6 +650,14 @@ __global__ void __launch_bounds__(kThreads, 1) packed_dq_kernel(const __grid_con
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tmem_base_sh;
+  wait_for_kernel_before();
+  let_next_kernel_start();
+
+  const UnitHead uh = unit_of_block(blockIdx.x, p.a.n_units, p.a.heads, p.a.head_chunk);
+  const PackedUnit u = p.a.units[uh.unit];
+  const int head = uh.head, kvh = head / p.a.group;
+  auto limit = [&](int r) { return max(0, min(u.k_valid, p.a.causal ? u.vis0 + r : u.k_valid)); };
+  const int n = u.end - u.begin;
 
   if (warp == 0) {
     // ---------------------------------------------------------------- TMA producers: lane 0 Q, dO, K; lane 1 V
@@ -820,19 +828,15 @@ template <typename Kern>
 cudaError_t run(Kern kern, int smem, std::atomic<uint64_t>& ready, int64_t blocks, const KParams& p, cudaStream_t st) {
   cudaError_t e = allow_smem(kern, smem, ready);
   if (e != cudaSuccess) return e;
-  if (blocks > 0x7fffffff) return cudaErrorInvalidConfiguration;
-  kern<<<(unsigned)blocks, kThreads, smem, st>>>(p);
-  return cudaGetLastError();
+  return launch_early(kern, blocks, kThreads, smem, st, p);
 }
 
 template <typename T, int NA>
 cudaError_t launch(const PackedParams& dq, const PackedParams& kv, cudaStream_t st) {
   constexpr bool bf16 = Elem<T>::is_bf16;
   if (dq.n_units > 0) {
-    const int64_t blocks = (int64_t)dq.n_units * dq.heads;
-    if (blocks > 0x7fffffff) return cudaErrorInvalidConfiguration;
-    packed_pre_kernel<T><<<(unsigned)blocks, 256, 0, st>>>(dq);  // pieces of a cut unit write the same values
-    cudaError_t e = cudaGetLastError();
+    // pieces of a cut unit write the same values
+    cudaError_t e = launch_early(packed_pre_kernel<T>, (int64_t)dq.n_units * dq.heads, 256, 0, st, dq);
     if (e != cudaSuccess) return e;
   }
   static std::atomic<uint64_t> ready_kv{0}, ready_q{0};
@@ -849,8 +853,9 @@ cudaError_t launch(const PackedParams& dq, const PackedParams& kv, cudaStream_t 
     p.a = kv;
     cudaError_t e = run(packed_dkdv_kernel<T, NA>, DkdvCfg<NA>::SMEM, ready_kv, (int64_t)kv.n_units * kv.kv_heads, p, st);
     if (e != cudaSuccess) return e;
-    if (kv.n_joins > 0) packed_sum_kernel<T, NA, true><<<(unsigned)(kv.n_joins * kv.kv_heads * 8), 256, 0, st>>>(kv);
-    if ((e = cudaGetLastError()) != cudaSuccess) return e;
+    if (kv.n_joins > 0 &&
+        (e = launch_early(packed_sum_kernel<T, NA, true>, (int64_t)kv.n_joins * kv.kv_heads * 8, 256, 0, st, kv)) != cudaSuccess)
+      return e;
   }
   if (dq.n_units > 0) {
     if (!map(&p.tm_q, dq.q, dq.q_total, dq.heads, dq.qv, 128) || !map(&p.tm_do, dq.dout, dq.q_total, dq.heads, dq.dov, 128))
@@ -858,8 +863,7 @@ cudaError_t launch(const PackedParams& dq, const PackedParams& kv, cudaStream_t 
     p.a = dq;
     cudaError_t e = run(packed_dq_kernel<T, NA>, DqCfg<NA>::SMEM, ready_q, (int64_t)dq.n_units * dq.heads, p, st);
     if (e != cudaSuccess) return e;
-    if (dq.n_joins > 0) packed_sum_kernel<T, NA, false><<<(unsigned)(dq.n_joins * dq.heads * 4), 256, 0, st>>>(dq);
-    return cudaGetLastError();
+    if (dq.n_joins > 0) return launch_early(packed_sum_kernel<T, NA, false>, (int64_t)dq.n_joins * dq.heads * 4, 256, 0, st, dq);
   }
   return cudaSuccess;
 }

@@ -250,6 +250,8 @@ __global__ void __launch_bounds__(kThreads, 1) packed_fwd_kernel(const __grid_co
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tmem_base_sh;
+  wait_for_kernel_before();
+  let_next_kernel_start();
 
   // The K producer hands the items on through work_sh: item i in place i & 1 until its ten readers are done with it.
   auto work_wait = [&](int i, int code) -> bool {
@@ -659,6 +661,8 @@ __global__ void __launch_bounds__(kThreads, 1) packed_fwd_kernel(const __grid_co
 // Joins the pieces of cut units: block = (unit, head, 32 rows), 8 lanes a row, 8 NA columns a lane.
 template <typename T, int NA>
 __global__ void __launch_bounds__(256) packed_fwd_join_kernel(const __grid_constant__ PackedParams a) {
+  wait_for_kernel_before();
+  let_next_kernel_start();
   const int64_t uh = blockIdx.x >> 3;
   const int join = (int)(uh / a.heads), head = (int)(uh % a.heads);
   const PackedUnit u = a.units[a.joins[2 * join]];
@@ -713,15 +717,9 @@ cudaError_t launch(const KParams& p, cudaStream_t st) {
   static std::atomic<uint64_t> ready{0};
   cudaError_t e = allow_smem(kern, Cfg<NA>::SMEM, ready);
   if (e != cudaSuccess) return e;
-  const int64_t blocks = (int64_t)p.a.n_units * p.a.heads;
-  if (blocks > 0x7fffffff) return cudaErrorInvalidConfiguration;
-  kern<<<(unsigned)blocks, kThreads, Cfg<NA>::SMEM, st>>>(p);
-  e = cudaGetLastError();
+  e = launch_early(kern, (int64_t)p.a.n_units * p.a.heads, kThreads, Cfg<NA>::SMEM, st, p);
   if (e != cudaSuccess || p.a.n_joins == 0) return e;
-  const int64_t joins = (int64_t)p.a.n_joins * p.a.heads * 8;
-  if (joins > 0x7fffffff) return cudaErrorInvalidConfiguration;
-  packed_fwd_join_kernel<T, NA><<<(unsigned)joins, 256, 0, st>>>(p.a);
-  return cudaGetLastError();
+  return launch_early(packed_fwd_join_kernel<T, NA>, (int64_t)p.a.n_joins * p.a.heads * 8, 256, 0, st, p.a);
 }
 
 template <typename T>

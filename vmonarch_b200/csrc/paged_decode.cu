@@ -155,7 +155,7 @@ __global__ void __launch_bounds__(32 * kWarps, 2) paged_decode_kernel(const __gr
   float* join_ml = join + kWarps * 8 * C::LD;                       // [warp][8 heads][max, sum]
   volatile int* abort = reinterpret_cast<int*>(smem + C::RING + C::JOIN + kWarps * C::STAGES * 8);
 
-  asm volatile("griddepcontrol.launch_dependents;");
+  let_next_kernel_start();
   if (lane == 0) {
     if (warp == 0) *abort = 0;
     for (int s = 0; s < C::STAGES; ++s) mbar_init(bar0 + 8u * s, 1);
@@ -422,7 +422,7 @@ __global__ void __launch_bounds__(512) paged_join_kernel(const __grid_constant__
   const long long parts = parts_of(p, total), t0 = before * p.items + (long long)item * (kItemCost + tiles) + kItemCost;
   const int c0 = (int)(((t0 + 1) * parts - 1) / total), c1 = (int)(((t0 + tiles) * parts - 1) / total);
   // every block waits, those without work too: the stream's next kernel must find the first one done
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  wait_for_kernel_before();
   if (c0 == c1) return;  // finished by its block
   const int h = item / p.chunks, g0 = (item % p.chunks) * HEADS, rows = one ? 1 : min(HEADS, p.group - g0);
   const int grp = threadIdx.x / LANES, d4 = threadIdx.x % LANES, per = GROUPS / rows;
@@ -490,16 +490,7 @@ cudaError_t launch(const PagedParams& p, cudaStream_t st) {
   e = cudaGetLastError();
   if (e != cudaSuccess || p.whole_items) return e;
   // the join starts while the last blocks still run and waits on the device for what they wrote
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)(p.batch * p.join_blocks));
-  cfg.blockDim = dim3(512);
-  cfg.stream = st;
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, paged_join_kernel<T, DP, NT>, p);
+  return launch_early(paged_join_kernel<T, DP, NT>, (int64_t)p.batch * p.join_blocks, 512, 0, st, p);
 }
 
 template <typename T>
