@@ -32,6 +32,7 @@ def _dense(t):
 
 
 _PARAMS = ("gate", "scale", "shift", "weight", "post_weight")
+_WEIGHTS = ("weight", "post_weight")
 # vmb_gated_norm_args up to its workspace: x, y, x_new, h, five parameters, stats, seq_start | dx_new, dh, dx, dy,
 # five gradients | sizes
 _ARGS = struct.Struct("25q5if")
@@ -44,7 +45,6 @@ def _forward(x, y, params, seqs, sizes, stats):
     rows, cols = sizes[:2]
     x, x_ptr, x_row = _place(x, rows, cols)
     y, y_ptr, y_row = _NO_ROWS if y is None else _place(y, rows, cols)
-    params = [None if t is None else _dense(t) for t in params]
     x_new = None if y is None else torch.empty_like(x, memory_format=torch.contiguous_format)
     h = torch.empty_like(x, memory_format=torch.contiguous_format)
     a = N.GatedNormArgs()
@@ -54,14 +54,14 @@ def _forward(x, y, params, seqs, sizes, stats):
     rc = N.lib.vmb_gated_norm_fwd(ctypes.byref(a), N.raw_stream(x.device.index))
     if rc:
         N.check(rc, "vmb_gated_norm_fwd")
-    return x, y, params, x_new, h
+    return x, y, x_new, h
 
 
 class _GatedNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, y, seqs, sizes, *params):
         stats = torch.empty(3 * sizes[0], dtype=torch.float32, device=x.device)
-        x, y, params, x_new, h = _forward(x, y, params, seqs, sizes, stats)
+        x, y, x_new, h = _forward(x, y, params, seqs, sizes, stats)
         ctx.save_for_backward(x, y, stats, *params)
         ctx.meta = seqs, sizes
         ctx.set_materialize_grads(False)
@@ -134,26 +134,28 @@ def gated_residual_norm(x, y=None, *, gate=None, scale=None, shift=None, weight=
         assert seqs.device == device, "x and seqs must be on one CUDA device"
         assert seqs.total_q == rows, f"x has {rows} rows, the sequences {seqs.total_q}"
         assert count <= 65535, "at most 65535 sequences"
-    params = (gate, scale, shift, weight, post_weight)
-    dtype, needed = None, x.requires_grad or (y is not None and y.requires_grad)
-    for name, t in zip(_PARAMS, params):
-        if t is None:
-            continue
-        assert t.device == device, f"{name} must be on x's device"
-        if t.dtype != dtype:
-            assert dtype is None and t.dtype in (kind, torch.float32), "the parameters must share one dtype, x's or fp32"
-            dtype = t.dtype
-        if seqs is None:
-            assert t.shape == (c,) or t.shape == (1, c), f"{name} must be ({c},)"
-        elif name in ("weight", "post_weight"):
-            assert t.shape == (c,), f"{name} must be ({c},)"
-        else:
-            assert t.shape == (count, c), f"{name} must be ({count}, {c})"
-        needed = needed or t.requires_grad
+    needed = x.requires_grad or (y is not None and y.requires_grad)
+    params, dtype, wide, tall = [], None, (c,), (count, c)
+    for name, t in zip(_PARAMS, (gate, scale, shift, weight, post_weight)):
+        if t is not None:
+            assert t.device == device, f"{name} must be on x's device"
+            if t.dtype != dtype:
+                assert dtype is None and t.dtype in (kind, torch.float32), "the parameters must share one dtype, x's or fp32"
+                dtype = t.dtype
+            if seqs is None:
+                assert t.shape == wide or t.shape == tall, f"{name} must be ({c},)"
+            elif name in _WEIGHTS:
+                assert t.shape == wide, f"{name} must be ({c},)"
+            else:
+                assert t.shape == tall, f"{name} must be ({count}, {c})"
+            needed = needed or t.requires_grad
+            if t.data_ptr() & 15 or not t.is_contiguous():
+                t = _dense(t)
+        params.append(t)
     code = N.dtype_code(kind)
     sizes = (rows, c, count, code, N.VMB_DTYPE_F32 if dtype == torch.float32 else code, norm == "layer", eps)
     if needed and torch.is_grad_enabled():
         out = _GatedNorm.apply(x, y, seqs, sizes, *params)
         return (x, out[0]) if y is None else out
-    x_new, h = _forward(x, y, params, seqs, sizes, None)[3:]
+    x_new, h = _forward(x, y, params, seqs, sizes, None)[2:]
     return (x if y is None else x_new), h

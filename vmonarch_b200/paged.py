@@ -19,11 +19,11 @@ from .kernel import SUPPORTED_DTYPES
 from .packed import MAX_DIM, _place
 
 
-def _pages(t):
-    """vmb_pages of a pool (pages, heads, slots, dim), which the kernels address in place."""
+def _pages(t, n, h, ps, d):
+    """vmb_pages of a pool (n pages, h heads, ps slots, d columns), which the kernels address in place."""
     ptr, (page, head, slot, col) = t.data_ptr(), t.stride()
-    n, h, ps, d = t.shape
-    page, head, slot = page if n > 1 else 0, head if h > 1 else 0, slot if ps > 1 else 0
+    if n == 1 or h == 1 or ps == 1:  # such strides do not count
+        page, head, slot = page if n > 1 else 0, head if h > 1 else 0, slot if ps > 1 else 0
     assert col == 1 or d == 1, "pools need contiguous columns"
     assert not ptr & 15 and page >= 0 and head >= 0 and slot >= 0 and not (page | head | slot) & 7, \
         "pools need 16-byte aligned rows"
@@ -32,10 +32,10 @@ def _pages(t):
 
 def _check_pools(k_pages, v_pages):
     """(pages, heads, page size, dim, dtype, device) of a pair of pools."""
-    assert k_pages.dim() == 4 and v_pages.shape == k_pages.shape, "pools must be (num_pages, Hk, page_size, D)"
-    dtype, device = k_pages.dtype, k_pages.device
+    shape, dtype, device = k_pages.shape, k_pages.dtype, k_pages.device
+    assert len(shape) == 4 and v_pages.shape == shape, "pools must be (num_pages, Hk, page_size, D)"
     assert dtype in SUPPORTED_DTYPES and v_pages.dtype == dtype, f"unsupported dtype {dtype}"
-    n, h, ps, d = k_pages.shape
+    n, h, ps, d = shape
     assert 8 <= d <= MAX_DIM and d % 8 == 0, f"head dim {d} is not a multiple of 8 up to {MAX_DIM}"
     assert n >= 1 and h >= 1 and ps >= 1, "pools need at least one page, head and slot"
     assert k_pages.is_cuda and v_pages.device == device, "pools must be on one CUDA device"
@@ -68,9 +68,10 @@ def paged_attention(q, k_pages, v_pages, page_table, lengths, *, sm_scale=None, 
     graph whose replays see other lengths.
     """
     num, hk, page_size, d, dtype, device = _check_pools(k_pages, v_pages)
-    assert q.dim() == 3 and q.dtype == dtype and q.size(2) == d and q.device == device, \
+    shape = q.shape
+    assert len(shape) == 3 and q.dtype == dtype and shape[2] == d and q.device == device, \
         "q must be (B, H, D) with the pools' D, dtype and device"
-    b, h, _ = q.shape
+    b, h, _ = shape
     assert h >= 1 and h % hk == 0, "H must be a multiple of Hk"
     _check_index(page_table, "page_table", 2, device)
     _check_index(lengths, "lengths", 1, device)
@@ -83,11 +84,11 @@ def paged_attention(q, k_pages, v_pages, page_table, lengths, *, sm_scale=None, 
     if width > 1 and col != 1 or b > 1 and stride < width:
         page_table, stride = page_table.contiguous(), width
     lengths = lengths.contiguous()
-    o = torch.empty((b, h, d), dtype=dtype, device=device)
+    o = torch.empty_like(q, memory_format=torch.contiguous_format)
     lse = torch.empty((b, h), dtype=torch.float32, device=device) if return_lse else None
     if b:
         a = N.PagedArgs()
-        _PAGED.pack_into(a, 0, *qr, o.data_ptr(), h * d, d, *_pages(k_pages), *_pages(v_pages), page_table.data_ptr(),
+        _PAGED.pack_into(a, 0, *qr, o.data_ptr(), h * d, d, *_pages(k_pages, num, hk, page_size, d), *_pages(v_pages, num, hk, page_size, d), page_table.data_ptr(),
                          lengths.data_ptr(), lse.data_ptr() if return_lse else 0, b, stride if b > 1 else width, width, num,
                          h, hk, d, page_size, N.dtype_code(dtype), sm_scale)
         size = N.lib.vmb_paged_workspace_bytes(ctypes.byref(a))
@@ -128,9 +129,10 @@ def append_pages(k, v, k_pages, v_pages, slots):
     k, *kr = _place(k)
     v, *vr = _place(v)
     slots = slots.contiguous()
-    N.check(N.lib.vmb_append_pages(N.Rows(*kr), N.Rows(*vr), N.Pages(*_pages(k_pages)), N.Pages(*_pages(v_pages)),
-                                   slots.data_ptr(), n, num, hk, d, page_size, N.raw_stream(device.index)),
-            "vmb_append_pages")
+    pool = num, hk, page_size, d
+    N.check(N.lib.vmb_append_pages(N.Rows(*kr), N.Rows(*vr), N.Pages(*_pages(k_pages, *pool)),
+                                   N.Pages(*_pages(v_pages, *pool)), slots.data_ptr(), n, num, hk, d, page_size,
+                                   N.raw_stream(device.index)), "vmb_append_pages")
 
 
 def copy_pages(k_pages, v_pages, src, dst):
@@ -150,8 +152,9 @@ def copy_pages(k_pages, v_pages, src, dst):
     if n == 0:
         return
     src, dst = src.contiguous(), dst.contiguous()
-    N.check(N.lib.vmb_copy_pages(N.Pages(*_pages(k_pages)), N.Pages(*_pages(v_pages)), src.data_ptr(), dst.data_ptr(), n,
-                                 num, hk, d, page_size, N.raw_stream(device.index)), "vmb_copy_pages")
+    pool = num, hk, page_size, d
+    N.check(N.lib.vmb_copy_pages(N.Pages(*_pages(k_pages, *pool)), N.Pages(*_pages(v_pages, *pool)), src.data_ptr(),
+                                 dst.data_ptr(), n, num, hk, d, page_size, N.raw_stream(device.index)), "vmb_copy_pages")
 
 
 class PagedKVCache:
