@@ -183,19 +183,27 @@ __device__ __forceinline__ bool clean_row(uint32_t tile, int row) {
   return true;
 }
 
-// A work item as every role sees it: its unit and the key tiles of the two streams.
+// A work item, made by the K producer and read by every role from shared memory.
 struct Item {
   PackedUnit u;
-  int head, kvh, n_kt[2], n_max, causal;
+  int head, kvh;     // head -1: no more work
+  int n_kt[2], n_max;  // key tiles of the two streams
+  int brief;         // bit w: stream w's last tile has at most 32 keys that count
+  int causal;
   // keys that local query r sees
   __device__ __forceinline__ int limit(int r) const { return max(0, min(u.k_valid, causal ? u.vis0 + r : u.k_valid)); }
-  __device__ __forceinline__ Item(const PackedParams& a, const PackedUnit& unit, int h) : u(unit), head(h), kvh(h / a.group) {
+  __device__ __forceinline__ void set(const PackedParams& a, const PackedUnit& unit, int h) {
+    u = unit;
+    head = h;
+    kvh = h / a.group;
     causal = a.causal;
+    brief = 0;
 #pragma unroll
     for (int w = 0; w < 2; ++w) {  // tiles that stream w's last query sees
       const int rows = min(u.q_valid - 128 * w, 128);
-      const int tiles = rows > 0 ? (limit(128 * w + rows - 1) + 127) >> 7 : 0;
-      n_kt[w] = max(0, min(tiles, u.end) - u.begin);
+      const int last = rows > 0 ? limit(128 * w + rows - 1) : 0;
+      n_kt[w] = max(0, min((last + 127) >> 7, u.end) - u.begin);
+      if (last - (u.begin + n_kt[w] - 1) * 128 <= 32) brief |= 1 << w;
     }
     n_max = max(n_kt[0], n_kt[1]);
   }
@@ -223,10 +231,7 @@ __global__ void __launch_bounds__(kThreads, 1) packed_fwd_kernel(const __grid_co
   __shared__ __align__(8) uint64_t bars[NBARS];
   __shared__ uint32_t tmem_base_sh;
   __shared__ int abort_sh, dirty_sh[2];
-  __shared__ struct Work {
-    PackedUnit u;
-    int head;  // -1: no more work
-  } work_sh[2];
+  __shared__ Item work_sh[2];
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t sbase = (smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -272,31 +277,30 @@ __global__ void __launch_bounds__(kThreads, 1) packed_fwd_kernel(const __grid_co
       prefetch_tmap(map);
       int tiles = 0, queries = 0, asked = 0;  // loaded so far by this lane; answers asked for
       bool ok = true;
-      Work work;
+      Item it;
       int block = blockIdx.x;
       for (int i = 0; ok; ++i) {
         if (kl) {
-          work.head = -1;
+          it.head = -1;
           if (block >= 0) {
             const UnitHead uh = unit_of_block(block, p.a.n_units, p.a.heads, p.a.head_chunk);
-            work = Work{p.a.units[uh.unit], uh.head};
+            it.set(p.a, p.a.units[uh.unit], uh.head);
           }
           if (i >= 2 && !(ok = mbar_wait(BAR(B_WFREE + (i & 1)), ((i - 2) >> 1) & 1, abort, &g_packed_err, 1))) break;
-          work_sh[i & 1] = work;
+          work_sh[i & 1] = it;
           mbar_arrive(BAR(B_WFULL + (i & 1)));
         } else {
           if (!(ok = work_wait(i, 1))) break;
-          work = work_sh[i & 1];
+          it = work_sh[i & 1];
           mbar_arrive(BAR(B_WFREE + (i & 1)));
         }
-        if (work.head < 0) break;
+        if (it.head < 0) break;
         if (kl) {  // ask for the item after this one, long before it is needed
           fence_proxy_async_smem();
           mbar_expect_tx(BAR(B_ANSWER), 16);
           request_block(smem_u32(&answer_sh), BAR(B_ANSWER));
           ++asked;
         }
-        const Item it(p.a, work.u, work.head);
         if (kl && it.n_max > 0) {
           if (queries > 0) ok = mbar_wait(BAR(B_QFREE), (queries - 1) & 1, abort, &g_packed_err, 1);
           if (!ok) break;
@@ -345,23 +349,20 @@ __global__ void __launch_bounds__(kThreads, 1) packed_fwd_kernel(const __grid_co
     bool ok = true;
     for (int i = 0; ok; ++i) {
       if (!(ok = __all_sync(0xffffffffu, work_wait(i, 2)))) break;
-      const int head = work_sh[i & 1].head;
-      const Item it(p.a, work_sh[i & 1].u, head);
+      const int head = work_sh[i & 1].head, n_max = work_sh[i & 1].n_max;
+      const int n_kt[2] = {work_sh[i & 1].n_kt[0], work_sh[i & 1].n_kt[1]};
+      // a stream's last tile of <= 32 keys: shorter products
+      const bool brief[2] = {(work_sh[i & 1].brief & 1) != 0, (work_sh[i & 1].brief & 2) != 0};
       __syncwarp();
       if (lane == 0) mbar_arrive(BAR(B_WFREE + (i & 1)));
       if (head < 0) break;
-      if (it.n_max == 0) continue;
-      // a stream's last tile of <= 32 keys: shorter products
-      bool brief[2];
-#pragma unroll
-      for (int w = 0; w < 2; ++w)
-        brief[w] = it.limit(min(it.u.q_valid, 128 * (w + 1)) - 1) - (it.u.begin + it.n_kt[w] - 1) * 128 <= 32;
+      if (n_max == 0) continue;
       // S of stream w's tile t, whose K tile is in slot s since its phase `parity`
       auto issue_s = [&](int w, int t, int s, uint32_t parity) -> bool {
         if (!wwait(B_KFULL + s, parity, 2)) return false;
         tc_fence_after();
         const uint32_t kb = sK + s * TILE, qb = sQ + w * TILE;
-        const uint32_t idesc = brief[w] && t + 1 == it.n_kt[w] ? IDESC_S32 : IDESC_S;
+        const uint32_t idesc = brief[w] && t + 1 == n_kt[w] ? IDESC_S32 : IDESC_S;
 #pragma unroll
         for (int kk = 0; kk < 4 * NA; ++kk) {
           const uint32_t off = (kk >> 2) * kAtom + (kk & 3) * 32;
@@ -374,17 +375,17 @@ __global__ void __launch_bounds__(kThreads, 1) packed_fwd_kernel(const __grid_co
       ok = wwait(B_QFULL, queries & 1, 2);
       ++queries;
       for (int w = 0; w < 2; ++w)
-        if (ok && it.n_kt[w] > 0) ok = issue_s(w, 0, ks0, kp0);
-      if (ok && it.n_max == 1) mma_commit_if(leader, BAR(B_QFREE));
-      for (int t = 0; ok && t < it.n_max; ++t) {
+        if (ok && n_kt[w] > 0) ok = issue_s(w, 0, ks0, kp0);
+      if (ok && n_max == 1) mma_commit_if(leader, BAR(B_QFREE));
+      for (int t = 0; ok && t < n_max; ++t) {
         if (++ks0 == NK) ks0 = 0, kp0 ^= 1;  // the next K tile
 #pragma unroll
         for (int w = 0; w < 2; ++w) {
-          if (!ok || t >= it.n_kt[w]) continue;
+          if (!ok || t >= n_kt[w]) continue;
           const int c = steps[w] + t;
           const uint32_t vb = sV + vs0 * TILE;
           const uint32_t a_tm = tmem + 128 * w, o_tm = tmem + T_O + 64 * NA * w;
-          const int ksteps = brief[w] && t + 1 == it.n_kt[w] ? 2 : 8;  // 16 keys per step
+          const int ksteps = brief[w] && t + 1 == n_kt[w] ? 2 : 8;  // 16 keys per step
           if (!(ok = wwait(B_PHALF + w, c & 1, 4) && wwait(B_VFULL + vs0, vp0, 4))) break;
           // the stream's O of the last unit has been read
           if (t == 0 && outs[w] > 0 && !(ok = wwait(B_OFREE + w, (outs[w] - 1) & 1, 4))) break;
@@ -400,15 +401,15 @@ __global__ void __launch_bounds__(kThreads, 1) packed_fwd_kernel(const __grid_co
           for (int kk = 4; kk < 8; ++kk)
             mma_ts_if(leader & (kk < ksteps ? 1u : 0u), o_tm, a_tm + kk * 8, smem_desc_sw128(vb + kk * 2048, kAtom, 1024),
                       IDESC_PV, 1u);
-          if (t + 1 < it.n_kt[w]) ok = issue_s(w, t + 1, ks0, kp0);
+          if (t + 1 < n_kt[w]) ok = issue_s(w, t + 1, ks0, kp0);
           else mma_commit_if(leader, BAR(B_OFULL + w));
         }
-        if (ok && t + 2 == it.n_max) mma_commit_if(leader, BAR(B_QFREE));  // the last scores are on their way
+        if (ok && t + 2 == n_max) mma_commit_if(leader, BAR(B_QFREE));  // the last scores are on their way
         if (++vs0 == NV) vs0 = 0, vp0 ^= 1;
       }
       for (int w = 0; w < 2; ++w) {
-        steps[w] += it.n_kt[w];
-        outs[w] += it.n_kt[w] > 0;
+        steps[w] += n_kt[w];
+        outs[w] += n_kt[w] > 0;
       }
     }
     // every MMA issued must be complete before TMEM can be freed: one more round of the queries' barrier
@@ -444,7 +445,7 @@ __global__ void __launch_bounds__(kThreads, 1) packed_fwd_kernel(const __grid_co
       int n_kt, begin, my_lim, lim_lo;
       bool live;
       {
-        const Item it(p.a, work_sh[i & 1].u, work_sh[i & 1].head);
+        const Item& it = work_sh[i & 1];
         n_kt = it.n_kt[w];
         begin = it.u.begin;
         // rows past the unit's last query are not stored: they take its limit, and no part in the reference
@@ -527,7 +528,7 @@ __global__ void __launch_bounds__(kThreads, 1) packed_fwd_kernel(const __grid_co
               tmem_ld32(tS + 64 * hf, s);
               tmem_ld32(tS + 64 * hf + 32, s + 32);
               tmem_wait_ld();
-              if (hf == 0 && t == 0) m_ref = row_max<64, true>(s, seen) * p.scale_log2;
+              if (hf == 0 && t == 0) m_ref = (least >= 64 ? row_max<64, false>(s, 64) : row_max<64, true>(s, seen)) * p.scale_log2;
               float lt = 0.f;
 #pragma unroll 1
               for (int pass = 0; pass < 2; ++pass) {
@@ -577,7 +578,7 @@ __global__ void __launch_bounds__(kThreads, 1) packed_fwd_kernel(const __grid_co
         ++outs;
         tc_fence_after();
       }
-      const Item it(p.a, work_sh[i & 1].u, work_sh[i & 1].head);
+      const Item& it = work_sh[i & 1];
       const PackedUnit& u = it.u;
       if (leads) {
         // the stream's last V tile, and the tiles that only the other stream uses: each once it has landed, so
@@ -634,16 +635,23 @@ __global__ void __launch_bounds__(kThreads, 1) packed_fwd_kernel(const __grid_co
           for (int k = 0; k < 4; ++k) st_global_v8(to + 8 * k, o + 8 * k);
           continue;
         }
-        uint32_t x[16], y[16];
+        uint32_t x[16];
+        const float2 inv2 = make_float2(inv, inv);
+        auto scaled = [&](int e) { return __fmul2_rn(make_float2(__uint_as_float(o[2 * e]), __uint_as_float(o[2 * e + 1])), inv2); };
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-          const float a = __uint_as_float(o[2 * e]) * inv, b = __uint_as_float(o[2 * e + 1]) * inv;
-          x[e] = Elem<T>::pack(a, b);
-          const float2 r = Elem<T>::unpack(x[e]);
-          y[e] = Elem<T>::pack(a - r.x, b - r.y);
+          const float2 a = scaled(e);
+          x[e] = Elem<T>::pack(a.x, a.y);
         }
         store_row32(out, c * 32, p.a.dim, sectors, x);
-        if (p.a.o_low) store_row32(low, c * 32, p.a.dim, sectors, y);
+        if (p.a.o_low) {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const float2 a = scaled(e), r = Elem<T>::unpack(x[e]);
+            x[e] = Elem<T>::pack(a.x - r.x, a.y - r.y);
+          }
+          store_row32(low, c * 32, p.a.dim, sectors, x);
+        }
       }
       if (live) {
         if (u.part >= 0)
