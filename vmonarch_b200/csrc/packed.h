@@ -56,6 +56,28 @@ __host__ __device__ __forceinline__ UnitHead unit_of_block(int64_t block, int n_
   const int g = left < chunk ? left : chunk;
   return UnitHead{rem / g, c * chunk + rem % g};
 }
+
+// 32 bytes to a 32-byte aligned global address (one sector, one store)
+__device__ __forceinline__ void st_global_v8(void* ptr, const uint32_t* v) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(ptr), "r"(v[0]), "r"(v[1]), "r"(v[2]),
+               "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+               : "memory");
+}
+// 32 columns of a row, as 16 packed words; whole sectors where rows are 32-byte aligned. dim: a multiple of 8.
+__device__ __forceinline__ void store_row32(uint16_t* row, int col, int dim, bool sectors, const uint32_t* x) {
+  if (sectors && col + 32 <= dim) {
+    st_global_v8(row + col, x);
+    st_global_v8(row + col + 16, x + 8);
+  } else {
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (col + 8 * k < dim) *reinterpret_cast<uint4*>(row + col + 8 * k) = make_uint4(x[4 * k], x[4 * k + 1], x[4 * k + 2], x[4 * k + 3]);
+  }
+}
+// Whether the rows of a 16-bit tensor start at whole 32-byte sectors.
+__device__ __forceinline__ bool whole_sectors(const void* t, const View& v) {
+  return ((v.rs | v.s1) & 15) == 0 && (reinterpret_cast<uintptr_t>(t) & 31) == 0;
+}
 #endif
 
 }  // namespace vmb

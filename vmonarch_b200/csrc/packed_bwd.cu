@@ -113,39 +113,17 @@ __device__ __forceinline__ void result_row(uint32_t taddr, int c, bool any, floa
     for (int i = 0; i < 32; ++i) v[i] = 0u;
   }
 }
-// 16-bit rows of a [128][64 NA] fp32 accumulator into swizzled staging: 32-column chunks [c0, c1).
+// 32-column chunks [c0, c1) of an accumulator row to a row of 16-bit values.
 template <typename T>
-__device__ __forceinline__ void stage_rows(uint32_t taddr, uint32_t stage, int row, bool any, int c0, int c1, float scale,
-                                           float off = 0.f, const float* centre = nullptr) {
+__device__ __forceinline__ void store_result(uint32_t taddr, T* out, bool live, bool sectors, int dim, bool any, int c0, int c1,
+                                             float scale, float off = 0.f, const float* centre = nullptr) {
 #pragma unroll 1
   for (int c = c0; c < c1; ++c) {
-    uint32_t v[32];
+    uint32_t v[32], x[16];
     result_row(taddr, c, any, scale, off, centre, v);
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      uint32_t w[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        w[i] = Elem<T>::pack(__uint_as_float(v[8 * k + 2 * i]), __uint_as_float(v[8 * k + 2 * i + 1]));
-      const int chunk = (c & 1) * 4 + k;
-      asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(stage + (c >> 1) * kAtom + row * 128 +
-                                                                   ((chunk ^ (row & 7)) << 4)),
-                   "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3])
-                   : "memory");
-    }
-  }
-}
-// The staged rows [0, rows) to global memory, whole 16-byte chunks below `dim` columns.
-template <typename T, int NA>
-__device__ __forceinline__ void store_rows(uint32_t stage, T* out, int64_t rs, int rows, int dim, int tid, int nthreads) {
-  constexpr int CH = 8 * NA;
-  for (int i = tid; i < rows * CH; i += nthreads) {
-    const int r = i / CH, ch = i % CH;
-    uint32_t x[4];
-    asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];"
-                 : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3])
-                 : "r"(stage + (ch >> 3) * kAtom + r * 128 + (((ch & 7) ^ (r & 7)) << 4)));
-    if (ch * 8 < dim) *reinterpret_cast<uint4*>(out + (int64_t)r * rs + ch * 8) = make_uint4(x[0], x[1], x[2], x[3]);
+    for (int i = 0; i < 16; ++i) x[i] = Elem<T>::pack(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]));
+    if (live) store_row32(reinterpret_cast<uint16_t*>(out), c * 32, dim, sectors, x);
   }
 }
 
@@ -311,7 +289,6 @@ struct DkdvCfg {
   static constexpr int NQ = NA == 2 ? 4 : 8;
   static constexpr int SMEM = 1024 + RES + NQ * SLOT;
   static_assert(SMEM <= 232448 - 1024, "shared memory budget");
-  static_assert(NQ * SLOT >= 2 * NA * kAtom, "the epilogue stages dK and dV in the query slots");
 };
 
 template <typename T, int NA>
@@ -584,21 +561,19 @@ __global__ void __launch_bounds__(kThreads, 1) packed_dkdv_kernel(const __grid_c
     }
     if (ok) ok = warp_wait(BAR_DONE, 0, 8);
     tc_fence_after();
-    // epilogue: warpgroups 0, 1 stage dK, 2, 3 dV, half of the columns each
+    // epilogue: warpgroups 0, 1 take dK, 2, 3 dV, half of the columns each
     const int mat = wg >> 1;
     const float unscale = (mat ? 1.f : 1.f / ds_scale) / kPScale<T>;
-    if (ok && u.part >= 0)
-      store_part(tmem + lane_off + (mat ? T_DV : T_DK),
-                 p.a.part + ((((int64_t)u.part * p.a.kv_heads + kvh) * 2 + mat) * 128 + row) * (64 * NA), n > 0, (wg & 1) * NA,
-                 ((wg & 1) + 1) * NA, unscale);
-    else if (ok)
-      stage_rows<T>(tmem + lane_off + (mat ? T_DV : T_DK), sSlots + mat * NA * kAtom, row, n > 0, (wg & 1) * NA,
-                    ((wg & 1) + 1) * NA, unscale);
     ok = named_bar_and(1, 512, ok && !*abort);
-    if (ok && u.part < 0) {
-      T* out = mat ? static_cast<T*>(p.a.dv) + (int64_t)u.k_row * p.a.dvv.rs + (int64_t)kvh * p.a.dvv.s1
-                   : static_cast<T*>(p.a.dk) + (int64_t)u.k_row * p.a.dkv.rs + (int64_t)kvh * p.a.dkv.s1;
-      store_rows<T, NA>(sSlots + mat * NA * kAtom, out, mat ? p.a.dvv.rs : p.a.dkv.rs, u.k_valid, p.a.dim, tid, 256);
+    const uint32_t acc = tmem + lane_off + (mat ? T_DV : T_DK);
+    if (ok && u.part >= 0) {
+      store_part(acc, p.a.part + ((((int64_t)u.part * p.a.kv_heads + kvh) * 2 + mat) * 128 + row) * (64 * NA), n > 0,
+                 (wg & 1) * NA, ((wg & 1) + 1) * NA, unscale);
+    } else if (ok) {
+      const View& v = mat ? p.a.dvv : p.a.dkv;
+      T* out = static_cast<T*>(mat ? p.a.dv : p.a.dk);
+      store_result<T>(acc, out + (int64_t)(u.k_row + row) * v.rs + (int64_t)kvh * v.s1, row < u.k_valid, whole_sectors(out, v),
+                      p.a.dim, n > 0, (wg & 1) * NA, ((wg & 1) + 1) * NA, unscale);
     }
   }
 
@@ -807,21 +782,19 @@ __global__ void __launch_bounds__(kThreads, 1) packed_dq_kernel(const __grid_con
     if (ok) sums[wg * 128 + row] = sum;
     if (ok) ok = warp_wait(B_DONE, 0, 64);
     tc_fence_after();
-    // epilogue: 16-bit dQ through the idle K ring; a warpgroup stages 32-column chunks wg, wg + 4, ...
-    ok = named_bar_and(1, 512, ok);
+    // epilogue: a warpgroup takes 32 columns
+    ok = named_bar_and(1, 512, ok && !*abort);
     if (ok && wg < 2 * NA) {
       const float unscale = 1.f / (row_scale * kPScale<T>);
       const float off = (sums[row] + sums[128 + row]) + (sums[256 + row] + sums[384 + row]);
+      T* out = static_cast<T*>(p.a.dq);
       if (u.part >= 0)
         store_part(tmem + lane_off + T_DQ, p.a.part + (((int64_t)u.part * p.a.heads + head) * 128 + row) * (64 * NA), n > 0, wg,
                    wg + 1, unscale, off, centre_sh);
       else
-        stage_rows<T>(tmem + lane_off + T_DQ, sK, row, n > 0, wg, wg + 1, unscale, off, centre_sh);
+        store_result<T>(tmem + lane_off + T_DQ, out + (int64_t)(u.q_row + row) * p.a.dqv.rs + (int64_t)head * p.a.dqv.s1,
+                        row < u.q_valid, whole_sectors(out, p.a.dqv), p.a.dim, n > 0, wg, wg + 1, unscale, off, centre_sh);
     }
-    ok = named_bar_and(1, 512, ok && !*abort);
-    if (ok && u.part < 0)
-      store_rows<T, NA>(sK, static_cast<T*>(p.a.dq) + (int64_t)u.q_row * p.a.dqv.rs + (int64_t)head * p.a.dqv.s1, p.a.dqv.rs,
-                        u.q_valid, p.a.dim, tid, 512);
   }
 
   tc_fence_before();

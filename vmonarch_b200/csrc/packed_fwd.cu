@@ -64,24 +64,6 @@ struct Cfg {
   static_assert(SMEM <= 232448 - 1024, "shared memory budget");
 };
 
-// 32 bytes to a 32-byte aligned global address (one sector, one store)
-__device__ __forceinline__ void st_global_v8(void* ptr, const uint32_t* v) {
-  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(ptr), "r"(v[0]), "r"(v[1]), "r"(v[2]),
-               "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
-               : "memory");
-}
-// 32 columns of a row, as 16 packed words; whole sectors where rows are 32-byte aligned. dim: a multiple of 8.
-__device__ __forceinline__ void store_row32(uint16_t* row, int col, int dim, bool sectors, const uint32_t* x) {
-  if (sectors && col + 32 <= dim) {
-    st_global_v8(row + col, x);
-    st_global_v8(row + col + 16, x + 8);
-  } else {
-#pragma unroll
-    for (int k = 0; k < 4; ++k)
-      if (col + 8 * k < dim) *reinterpret_cast<uint4*>(row + col + 8 * k) = make_uint4(x[4 * k], x[4 * k + 1], x[4 * k + 2], x[4 * k + 3]);
-  }
-}
-
 // Asks for a block of the grid that has not started: 16 bytes of answer, completing on `bar`.
 __device__ __forceinline__ void request_block(uint32_t answer, uint32_t bar) {
   asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(answer),
@@ -433,8 +415,7 @@ __global__ void __launch_bounds__(kThreads, 1) packed_fwd_kernel(const __grid_co
     auto warp_wait = [&](int bar, uint32_t parity, int code) -> bool {
       return __all_sync(0xffffffffu, mbar_wait(BAR(bar), parity, abort, &g_packed_err, code));
     };
-    const bool sectors = ((p.a.ov.rs | p.a.ov.s1 | p.a.olv.rs | p.a.olv.s1) & 15) == 0 &&
-                         ((reinterpret_cast<uintptr_t>(p.a.o) | reinterpret_cast<uintptr_t>(p.a.o_low)) & 31) == 0;
+    const bool sectors = whole_sectors(p.a.o, p.a.ov) && whole_sectors(p.a.o_low, p.a.olv);
     int steps = 0, outs = 0, ring = 0;  // tiles and units of this stream so far, tiles of the ring
     const bool leads = warp == 2 + 4 * w && lane == 0;  // frees ring slots for the stream
     bool ok = true;
