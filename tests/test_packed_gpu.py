@@ -221,3 +221,41 @@ def test_fp16_gradients_of_many_keys(size):
     for x, ref in zip(got[1:], want[1:]):
         err = (x.double() - ref).norm().item()
         assert err <= 4 * U[torch.float16] * ref.norm().item() + 2.0 ** -25 * x.numel() ** 0.5
+
+
+def test_captured_step():
+    """A captured forward and backward follows the values in its inputs; its kernels start early as uncaptured ones do."""
+    seqs = PackedSequences([200, 3, 700])
+    q, k, v, do = make([200, 3, 700], [200, 3, 700], 4, 2, 64, torch.bfloat16)
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+
+    def step():
+        o = packed_attention(*leaves, seqs, causal=True)
+        return [o.detach(), *torch.autograd.grad(o, leaves, do)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    new = make([200, 3, 700], [200, 3, 700], 4, 2, 64, torch.bfloat16, seed=1)
+    with torch.no_grad():
+        for t, x in zip((*leaves, do), new):
+            t.copy_(x)
+    for _ in range(3):
+        graph.replay()
+    torch.cuda.synchronize()
+    for x, ref in zip(out, step()):
+        assert torch.equal(x, ref)
+
+
+def test_gradients_carry_no_gradient():
+    q, k, v, _ = make([20], [20], 2, 1, 64, torch.bfloat16)
+    q.requires_grad_()
+    o = packed_attention(q, k, v, PackedSequences([20]))
+    dq, = torch.autograd.grad(o.float().sum(), q, create_graph=True)
+    with pytest.raises(RuntimeError):
+        dq.float().sum().backward()

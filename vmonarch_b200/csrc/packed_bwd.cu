@@ -32,7 +32,7 @@
 // once, and recomputing S and dP costs less than adding dQ through memory.
 // Bound by the tensor products (operands from shared memory) and the latencies between them. 15600 + 1289 + 409 + 1
 // causal tokens, 16/4 heads, D = 128, bf16: pre 48 us, dkdv 1650 us (1.22 PFLOP/s of its four products), dq 1160 us
-// (1.30 PFLOP/s of its three); five products at the measured dense rate (1.67 PFLOP/s) would take 1500 us.
+// (1.30 PFLOP/s of its three), 2690 us with the set-ups overlapped; five products at the measured dense rate (1.67 PFLOP/s) would take 1500 us.
 //
 // Tiles at a sequence's end hold the next sequence's rows. Their scores are dropped by index, and the
 // rows that enter a sum with weight 0 (Q and dO here, K in dq) are cleared in shared memory first, so

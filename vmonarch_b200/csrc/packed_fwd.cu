@@ -19,9 +19,9 @@
 // (clusterlaunchcontrol), most work first: the next item's queries, keys and first scores are under way while the
 // softmax warps write the last item's output straight from registers, and the set-up is paid once per SM.
 // Bound by the instructions of the softmax warps (part of the exponentials as polynomials gained nothing):
-// 2 us a 256 x 128 tile at D = 128, 5.3 us an item beside its tiles. 32760 causal tokens, 16/4 heads, D = 128, bf16:
-// 3460 us, 1.27 PFLOP/s in short runs, 1.07 under the power cap; 16 prompts of 1 to 4093 tokens, 40/8 heads: 425 us,
-// 0.80 PFLOP/s (the measured dense rate is 1.67).
+// 2 us a 256 x 128 tile at D = 128, 4.2 us an item beside its tiles. 32760 causal tokens, 16/4 heads, D = 128, bf16:
+// 3460 us, 1.27 PFLOP/s in short runs, 1.07 under the power cap; 16 prompts of 1 to 4093 tokens, 40/8 heads: 414 us,
+// 0.82 PFLOP/s (the measured dense rate is 1.67).
 // An item that is cut leaves 32-bit partials (max, sum, O), joined by a second kernel; the host cuts
 // where few items would leave SMs without work.
 //
