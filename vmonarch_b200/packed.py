@@ -79,7 +79,8 @@ def _cut(u, heads, kind):
     if not len(u):
         return u, 0
     least, setup = _LEAST[kind], _SETUP[kind]
-    share = max(-(-int(steps.sum()) * heads // _SMS), 1)
+    total = int(steps.sum()) * heads
+    share = max(-(-total // _SMS), 1)
     limits = [max(least, -(-share * n // 8)) for n in (11, 10, 9, 8, 4, 2)]
     best = _pieces(steps, limits[1])  # a unit far above everybody's fair share is cut in any case
     if len(u) * heads <= _MANY:
@@ -88,11 +89,13 @@ def _cut(u, heads, kind):
             pieces = _pieces(steps, limit)
             if best is not None and (best_cost <= 1.03 * (share + setup) or pieces.max() == 1):
                 continue
+            cuts = int(pieces[pieces > 1].sum()) * heads
+            join = _JOIN + cuts // _JOINED if cuts else 0
+            evenly = (total + setup * int(pieces.sum()) * heads + _PIECE * cuts) // _SMS + join
+            if best is not None and evenly >= 0.98 * best_cost:
+                continue  # even if it ended evenly
             which, _, begin, end = _piece_steps(steps, pieces)
-            cut = pieces[which] > 1
-            cost = _span(np.sort(begin - end - _PIECE * cut), heads, setup)
-            if cut.any():
-                cost += _JOIN + int(cut.sum()) * heads // _JOINED
+            cost = _span(np.sort(begin - end - _PIECE * (pieces[which] > 1)), heads, setup) + join
             if best is None or cost < 0.98 * best_cost:
                 best, best_cost = pieces, cost
     if best.max() == 1:
