@@ -259,3 +259,18 @@ def test_gradients_carry_no_gradient():
     dq, = torch.autograd.grad(o.float().sum(), q, create_graph=True)
     with pytest.raises(RuntimeError):
         dq.float().sum().backward()
+
+
+@pytest.mark.parametrize("ql, kl, causal", [([300, 2, 40], None, True), ([130], [3], False)])
+def test_fp16_gradients_of_large_values(ql, kl, causal):
+    """Value rows near the documented limit of the fp16 backward (a norm of 4094): 4 u as in the module's docstring."""
+    kl = kl or ql
+    q, k, v, do = make(ql, kl, 4, 2, 64, torch.float16)
+    v = (v.float() * (4000 / v.float().norm(dim=-1, keepdim=True))).to(torch.float16)
+    do = (do * 0.125).to(torch.float16)
+    seqs = PackedSequences(ql, kl)
+    got = grads(lambda *x: packed_attention(*x, seqs, causal=causal), (q, k, v), do)
+    want = grads(lambda *x: packed_reference(*x, ql, kl, causal, 64 ** -0.5)[0], [t.double() for t in (q, k, v)], do)
+    assert max(w.abs().max().item() for w in want) < 60000  # the results themselves are in range
+    for x, ref in zip(got, want):
+        assert rel(x, ref) <= 4 * U[torch.float16]
