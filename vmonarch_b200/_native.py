@@ -241,7 +241,7 @@ def ptr(t: torch.Tensor | None) -> int | None:
 def device_status(device: torch.device) -> int:
     """OR of the pipeline-timeout codes recorded by the kernels since the last call (0 = none)."""
     out = ctypes.c_int32(0)
-    check(lib.vmb_device_status(stream_ptr(device), ctypes.byref(out)), "vmb_device_status")
+    launch("vmb_device_status", lambda stream: lib.vmb_device_status(stream, ctypes.byref(out)), device)
     return out.value
 
 
@@ -251,6 +251,22 @@ def stream_ptr(device: torch.device) -> int:
 
 #: handle of a device's current stream, by device index (torch.cuda.current_stream builds a Stream object around it)
 raw_stream = torch._C._cuda_getCurrentRawStream
+#: index of the current device
+current_device = torch._C._cuda_getDevice
+
+
+def launch(what: str, fn, device: torch.device, *args) -> None:
+    """Calls a C entry with `args` and the current stream of `device`, which is made the current device for the call
+    where it is not: the entries set up and launch kernels on the current device, and a stream handle alone does not
+    name one (every device's default stream has the handle 0)."""
+    index = current_device() if device.index is None else device.index
+    if index == current_device():
+        rc = fn(*args, raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, raw_stream(index))
+    if rc:
+        check(rc, what)
 
 
 def once_differentiable(backward):

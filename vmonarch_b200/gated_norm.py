@@ -51,9 +51,7 @@ def _forward(x, y, params, seqs, sizes, stats):
     _ARGS.pack_into(a, 0, x_ptr, x_row, y_ptr, y_row, 0 if x_new is None else x_new.data_ptr(), h.data_ptr(),
                     *[0 if t is None else t.data_ptr() for t in params], 0 if stats is None else stats.data_ptr(),
                     seqs._starts().data_ptr() if sizes[2] > 1 else 0, *_NO_GRADS, *sizes)
-    rc = N.lib.vmb_gated_norm_fwd(ctypes.byref(a), N.raw_stream(x.device.index))
-    if rc:
-        N.check(rc, "vmb_gated_norm_fwd")
+    N.launch("vmb_gated_norm_fwd", N.lib.vmb_gated_norm_fwd, x.device, ctypes.byref(a))
     return x, y, x_new, h
 
 
@@ -90,9 +88,7 @@ class _GatedNorm(torch.autograd.Function):
         if size > 0:
             ws = torch.empty(size, dtype=torch.uint8, device=x.device)
             a.workspace, a.workspace_bytes = ws.data_ptr(), size
-        rc = N.lib.vmb_gated_norm_bwd(ctypes.byref(a), N.raw_stream(x.device.index))
-        if rc:
-            N.check(rc, "vmb_gated_norm_bwd")
+        N.launch("vmb_gated_norm_bwd", N.lib.vmb_gated_norm_bwd, x.device, ctypes.byref(a))
         return (dx, dy, None, None, *out)
 
 

@@ -43,10 +43,10 @@ def kernel_launches() -> int:
 
 def _call(name: str, fn, arg, dev) -> None:
     if _timer is None:
-        N.check(fn(ctypes.byref(arg), N.stream_ptr(dev)), name)
+        N.launch(name, fn, dev, ctypes.byref(arg))
         return
     with _timer(name, arg):
-        N.check(fn(ctypes.byref(arg), N.stream_ptr(dev)), name)
+        N.launch(name, fn, dev, ctypes.byref(arg))
 
 
 # ----------------------------------------------------------------------------------------- layouts
@@ -321,9 +321,8 @@ def quant_e4m3(src: torch.Tensor, scale: float = 1.0) -> torch.Tensor:
     src = src if viewable(src) else src.contiguous()
     n1, n2 = _split(bshape)
     sv, dv = _view(src, nb), _view(dst, nb)
-    N.check(N.lib.vmb_quant_e4m3(src.data_ptr(), ctypes.byref(sv), dst.data_ptr(), ctypes.byref(dv), n1, n2,
-                                 math.prod(bshape), src.size(-2), src.size(-1), N.dtype_code(src.dtype), float(scale),
-                                 N.stream_ptr(src.device)), "vmb_quant_e4m3")
+    N.launch("vmb_quant_e4m3", N.lib.vmb_quant_e4m3, src.device, src.data_ptr(), ctypes.byref(sv), dst.data_ptr(),
+             ctypes.byref(dv), n1, n2, math.prod(bshape), src.size(-2), src.size(-1), N.dtype_code(src.dtype), float(scale))
     return dst
 
 
@@ -338,6 +337,5 @@ def cast_f32(src: torch.Tensor, dst: torch.Tensor) -> None:
         return
     n1, n2 = _split(bshape)
     sv, dv = _view(src, nb), _view(dst, nb)
-    N.check(N.lib.vmb_cast_f32_view(src.data_ptr(), ctypes.byref(sv), dst.data_ptr(), ctypes.byref(dv), n1, n2,
-                                    math.prod(bshape), src.size(-2), src.size(-1), N.dtype_code(dst.dtype),
-                                    N.stream_ptr(src.device)), "vmb_cast_f32_view")
+    N.launch("vmb_cast_f32_view", N.lib.vmb_cast_f32_view, src.device, src.data_ptr(), ctypes.byref(sv), dst.data_ptr(),
+             ctypes.byref(dv), n1, n2, math.prod(bshape), src.size(-2), src.size(-1), N.dtype_code(dst.dtype))

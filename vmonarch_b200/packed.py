@@ -272,9 +272,7 @@ def _forward(q, k, v, seqs, key, device, lse=None, aux=None):
     if size:
         ws = torch.empty(size, dtype=torch.uint8, device=device)
         _WORKSPACE.pack_into(a, _WORKSPACE_AT, ws.data_ptr(), size)
-    rc = N.lib.vmb_packed_fwd(ctypes.byref(a), N.raw_stream(device.index))
-    if rc:
-        N.check(rc, "vmb_packed_fwd")
+    N.launch("vmb_packed_fwd", N.lib.vmb_packed_fwd, device, ctypes.byref(a))
     return q, k, v, o
 
 
@@ -315,9 +313,7 @@ class _PackedAttention(torch.autograd.Function):
         if size:
             ws = torch.empty(size, dtype=torch.uint8, device=device)
             _WORKSPACE.pack_into(a, _WORKSPACE_AT, ws.data_ptr(), size)
-        rc = N.lib.vmb_packed_bwd(ctypes.byref(a), N.raw_stream(device.index))
-        if rc:
-            N.check(rc, "vmb_packed_bwd")
+        N.launch("vmb_packed_bwd", N.lib.vmb_packed_bwd, device, ctypes.byref(a))
         return dq, dk, dv, None, None, None
 
 

@@ -95,9 +95,7 @@ def paged_attention(q, k_pages, v_pages, page_table, lengths, *, sm_scale=None, 
         if size > 0:
             ws = torch.empty(size, dtype=torch.uint8, device=device)
             a.workspace, a.workspace_bytes = ws.data_ptr(), size
-        rc = N.lib.vmb_paged_attention(ctypes.byref(a), N.raw_stream(device.index))
-        if rc:
-            N.check(rc, "vmb_paged_attention")
+        N.launch("vmb_paged_attention", N.lib.vmb_paged_attention, device, ctypes.byref(a))
     return (o, lse) if return_lse else o
 
 
@@ -130,9 +128,8 @@ def append_pages(k, v, k_pages, v_pages, slots):
     v, *vr = _place(v)
     slots = slots.contiguous()
     pool = num, hk, page_size, d
-    N.check(N.lib.vmb_append_pages(N.Rows(*kr), N.Rows(*vr), N.Pages(*_pages(k_pages, *pool)),
-                                   N.Pages(*_pages(v_pages, *pool)), slots.data_ptr(), n, num, hk, d, page_size,
-                                   N.raw_stream(device.index)), "vmb_append_pages")
+    N.launch("vmb_append_pages", N.lib.vmb_append_pages, device, N.Rows(*kr), N.Rows(*vr), N.Pages(*_pages(k_pages, *pool)),
+             N.Pages(*_pages(v_pages, *pool)), slots.data_ptr(), n, num, hk, d, page_size)
 
 
 def copy_pages(k_pages, v_pages, src, dst):
@@ -153,8 +150,8 @@ def copy_pages(k_pages, v_pages, src, dst):
         return
     src, dst = src.contiguous(), dst.contiguous()
     pool = num, hk, page_size, d
-    N.check(N.lib.vmb_copy_pages(N.Pages(*_pages(k_pages, *pool)), N.Pages(*_pages(v_pages, *pool)), src.data_ptr(),
-                                 dst.data_ptr(), n, num, hk, d, page_size, N.raw_stream(device.index)), "vmb_copy_pages")
+    N.launch("vmb_copy_pages", N.lib.vmb_copy_pages, device, N.Pages(*_pages(k_pages, *pool)),
+             N.Pages(*_pages(v_pages, *pool)), src.data_ptr(), dst.data_ptr(), n, num, hk, d, page_size)
 
 
 class PagedKVCache:
