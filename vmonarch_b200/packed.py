@@ -10,6 +10,7 @@ from __future__ import annotations
 import ctypes
 import heapq
 import struct
+import threading
 
 import numpy as np
 import torch
@@ -30,6 +31,8 @@ _LEAST = {"fwd": 8, "dq": 8, "kv": 16}
 _SETUP, _PIECE, _JOIN, _JOINED = {"fwd": 3, "dq": 5, "kv": 8}, 3, 3, 40
 # lists of more blocks than this (eight for each SM) are even enough without looking
 _MANY = 8 * _SMS
+# held while something is added to what a PackedSequences keeps: two threads that made the same list would each hold one
+_making = threading.RLock()
 
 
 def _lengths(x, what):
@@ -126,7 +129,7 @@ class PackedSequences:
         device: where the tensors of the sequences live.
 
     The object holds device copies of its work lists, made at the first call that needs them; keep it
-    for as long as the lengths stand, e.g. for all layers of a step. It may be used on any stream.
+    for as long as the lengths stand, e.g. for all layers of a step. It may be used on any stream and by several threads.
     """
 
     def __init__(self, lengths, kv_lengths=None, device="cuda"):
@@ -150,12 +153,22 @@ class PackedSequences:
     def __repr__(self):
         return f"PackedSequences({self.num_sequences} sequences, {self.total_q} queries, {self.total_k} keys)"
 
+    def _kept(self, key, make, *args):
+        """What is kept under `key`, made by make(*args) at the first call."""
+        hit = self._cache.get(key)
+        if hit is None:
+            with _making:
+                hit = self._cache.get(key)
+                if hit is None:
+                    hit = self._cache[key] = make(*args)
+        return hit
+
+    def _on_device(self, array):
+        return torch.from_numpy(array).to(self.device)
+
     def _starts(self):
         """First query row of every sequence, int32 on the device."""
-        hit = self._cache.get("starts")
-        if hit is None:
-            hit = self._cache["starts"] = torch.from_numpy(self.q_start.astype(np.int32)).to(self.device)
-        return hit
+        return self._kept("starts", lambda: self._on_device(self.q_start.astype(np.int32)))
 
     # ------------------------------------------------------------------------------ work lists
     def _query_units(self, rows, causal):
@@ -189,44 +202,43 @@ class PackedSequences:
         u[:, 10] = np.maximum(nq - nk + 1, 0) if causal else np.where(nk == 1, nq, 0)
         return u
 
-    def _list(self, kind, causal, heads, group):
+    def _list(self, *key):
         """The device list of a kernel's units, most work first (blocks start in list order), then the joins
-        of those that are cut."""
-        key = (kind, causal, heads, group)
-        hit = self._cache.get(key)
-        if hit is None:
-            if kind == "kv":
-                u = self._key_units(causal, group)
-                u, parts = _cut(u, heads // group, kind)
-            else:
-                u = self._query_units(_FWD_ROWS if kind == "fwd" else _DQ_ROWS, causal)
-                u, parts = _cut(u, heads, kind)
-            u = u[np.argsort(u[:, 5] - u[:, 6], kind="stable")]
-            joins = _joins(u)
-            dev = torch.from_numpy(np.concatenate([u.reshape(-1), joins.reshape(-1)])).to(self.device)
-            at = dev.data_ptr()
-            hit = self._cache[key] = (
-                N.PackedList(at, at + u.nbytes if len(joins) else None, len(u), len(joins), parts, 0), dev)
-        return hit[0]
+        of those that are cut. key: kind, causal, heads, group."""
+        return self._kept(key, self._make_list, *key)[0]
+
+    def _make_list(self, kind, causal, heads, group):
+        if kind == "kv":
+            u = self._key_units(causal, group)
+            u, parts = _cut(u, heads // group, kind)
+        else:
+            u = self._query_units(_FWD_ROWS if kind == "fwd" else _DQ_ROWS, causal)
+            u, parts = _cut(u, heads, kind)
+        u = u[np.argsort(u[:, 5] - u[:, 6], kind="stable")]
+        joins = _joins(u)
+        dev = self._on_device(np.concatenate([u.reshape(-1), joins.reshape(-1)]))
+        at = dev.data_ptr()
+        return N.PackedList(at, at + u.nbytes if len(joins) else None, len(u), len(joins), parts, 0), dev
 
     def _template(self, key):
-        """vmb_packed_args of a kind of call, everything but the tensors, and its workspace size."""
+        """vmb_packed_args of a kind of call, everything but the tensors, its workspace size, and the device lists
+        that it names."""
         hit = self._cache.get(key)
-        if hit is None:
-            backward, causal, sm_scale, dtype, heads, kv_heads, dim = key
-            a = N.PackedArgs()
-            a.q_total, a.k_total, a.stat_rows = self.total_q, self.total_k, self.stat_rows
-            a.heads, a.kv_heads, a.dim = heads, kv_heads, dim
-            a.dtype, a.causal, a.sm_scale = N.dtype_code(dtype), causal, sm_scale
-            if backward:
-                a.q_units = self._list("dq", causal, heads, heads // kv_heads)
-                a.kv_units = self._list("kv", causal, heads, heads // kv_heads)
-                size = N.lib.vmb_packed_bwd_workspace_bytes(ctypes.byref(a))
-            else:
-                a.units = self._list("fwd", causal, heads, heads // kv_heads)
-                size = N.lib.vmb_packed_fwd_workspace_bytes(ctypes.byref(a))
-            hit = self._cache[key] = bytes(a), size
-        return hit
+        return self._kept(key, self._make_template, *key) if hit is None else hit
+
+    def _make_template(self, backward, causal, sm_scale, dtype, heads, kv_heads, dim):
+        a = N.PackedArgs()
+        a.q_total, a.k_total, a.stat_rows = self.total_q, self.total_k, self.stat_rows
+        a.heads, a.kv_heads, a.dim = heads, kv_heads, dim
+        a.dtype, a.causal, a.sm_scale = N.dtype_code(dtype), causal, sm_scale
+        lists = [(kind, causal, heads, heads // kv_heads) for kind in (("dq", "kv") if backward else ("fwd",))]
+        if backward:
+            a.q_units, a.kv_units = (self._list(*x) for x in lists)
+            size = N.lib.vmb_packed_bwd_workspace_bytes(ctypes.byref(a))
+        else:
+            a.units = self._list(*lists[0])
+            size = N.lib.vmb_packed_fwd_workspace_bytes(ctypes.byref(a))
+        return bytes(a), size, tuple(self._cache[x][1] for x in lists)
 
 
 # vmb_packed_args begins with the vmb_rows of q, k, v, o, dout, dq, dk, dv, o_low and lse
@@ -260,7 +272,7 @@ def _forward(q, k, v, seqs, key, device, lse=None, aux=None):
     k, *kr = _place(k)
     v, *vr = _place(v)
     o = torch.empty_like(q, memory_format=torch.contiguous_format)
-    template, size = seqs._template(key)
+    template, size, _ = seqs._template(key)
     a = N.PackedArgs.from_buffer_copy(template)
     heads, dim = key[4], key[6]
     row = heads * dim
@@ -303,7 +315,7 @@ class _PackedAttention(torch.autograd.Function):
         row, kv_row, device = heads * dim, kv_heads * dim, q.device
         do, *dor = _place(do)
         dq, dk, dv = (torch.empty_like(t, memory_format=torch.contiguous_format) for t in (q, k, v))
-        template, size = seqs._template((True, *key[1:]))
+        template, size, _ = seqs._template((True, *key[1:]))
         a = N.PackedArgs.from_buffer_copy(template)
         _FWD_TENSORS.pack_into(a, 0, *_place(q)[1:], *_place(k)[1:], *_place(v)[1:], o.data_ptr(), row, dim)
         low = aux.data_ptr()
