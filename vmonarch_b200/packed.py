@@ -145,6 +145,7 @@ class PackedSequences:
         stat = -(-self.q_lens // _DQ_ROWS) * _DQ_ROWS
         self.stat_start, self.stat_rows = np.cumsum(stat) - stat, int(stat.sum())
         self._cache = {}
+        self._home = None  # the stream on which all that is kept was allocated; None: there is none, or several
 
     @property
     def num_sequences(self) -> int:
@@ -163,12 +164,28 @@ class PackedSequences:
                     hit = self._cache[key] = make(*args)
         return hit
 
+    def _stream(self):
+        """Handle of the device's current stream."""
+        return N.raw_stream(self.device.index) if self.device.type == "cuda" else 0
+
     def _on_device(self, array):
+        stream = self._stream()
+        self._home = stream if not self._cache or stream == self._home else None
         return torch.from_numpy(array).to(self.device)
+
+    def _use(self, *tensors):
+        """Kept tensors that the current stream is about to read: where they belong to another, the allocator learns that
+        their memory stays in use here, whenever the object goes."""
+        if self._stream() != self._home:
+            stream = torch.cuda.current_stream(self.device)
+            for t in tensors:
+                t.record_stream(stream)
 
     def _starts(self):
         """First query row of every sequence, int32 on the device."""
-        return self._kept("starts", lambda: self._on_device(self.q_start.astype(np.int32)))
+        starts = self._kept("starts", lambda: self._on_device(self.q_start.astype(np.int32)))
+        self._use(starts)
+        return starts
 
     # ------------------------------------------------------------------------------ work lists
     def _query_units(self, rows, causal):
@@ -272,7 +289,8 @@ def _forward(q, k, v, seqs, key, device, lse=None, aux=None):
     k, *kr = _place(k)
     v, *vr = _place(v)
     o = torch.empty_like(q, memory_format=torch.contiguous_format)
-    template, size, _ = seqs._template(key)
+    template, size, lists = seqs._template(key)
+    seqs._use(*lists)
     a = N.PackedArgs.from_buffer_copy(template)
     heads, dim = key[4], key[6]
     row = heads * dim
@@ -315,7 +333,8 @@ class _PackedAttention(torch.autograd.Function):
         row, kv_row, device = heads * dim, kv_heads * dim, q.device
         do, *dor = _place(do)
         dq, dk, dv = (torch.empty_like(t, memory_format=torch.contiguous_format) for t in (q, k, v))
-        template, size, _ = seqs._template((True, *key[1:]))
+        template, size, lists = seqs._template((True, *key[1:]))
+        seqs._use(*lists)
         a = N.PackedArgs.from_buffer_copy(template)
         _FWD_TENSORS.pack_into(a, 0, *_place(q)[1:], *_place(k)[1:], *_place(v)[1:], o.data_ptr(), row, dim)
         low = aux.data_ptr()
