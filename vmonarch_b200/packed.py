@@ -128,8 +128,10 @@ class PackedSequences:
             prompt behind a cached prefix); default: `lengths`.
         device: where the tensors of the sequences live.
 
-    The object holds device copies of its work lists, made at the first call that needs them; keep it
-    for as long as the lengths stand, e.g. for all layers of a step. It may be used on any stream and by several threads.
+    The object holds device copies of its work lists, made at the first call of each kind (direction, causal, head
+    counts), which waits for the copy; keep it for as long as the lengths stand, e.g. for all layers of a step. It may
+    be used on any stream and by several threads. A captured graph reads the lists where they are: make one call of
+    each kind before the capture, and keep the object for as long as the graph.
     """
 
     def __init__(self, lengths, kv_lengths=None, device="cuda"):
@@ -169,6 +171,8 @@ class PackedSequences:
         return N.raw_stream(self.device.index) if self.device.type == "cuda" else 0
 
     def _on_device(self, array):
+        assert self.device.type != "cuda" or not torch.cuda.is_current_stream_capturing(), \
+            "the first call of a kind with these sequences copies their lists: make one before the capture"
         stream = self._stream()
         self._home = stream if not self._cache or stream == self._home else None
         return torch.from_numpy(array).to(self.device)
