@@ -11,6 +11,7 @@ import os
 from pathlib import Path
 
 import torch
+from torch.autograd import forward_ad
 
 LIB_PATH = Path(os.environ.get("VMONARCH_B200_LIB", Path(__file__).resolve().parent / "libvmonarch_b200.so"))
 
@@ -267,6 +268,12 @@ def launch(what: str, fn, device: torch.device, *args) -> None:
             rc = fn(*args, raw_stream(index))
     if rc:
         check(rc, what)
+
+
+def derived(*tensors) -> bool:
+    """Whether a call on these tensors (or None) goes through its autograd function: one of them requires a gradient, or
+    a level of forward-mode derivatives is open, whose dual tensors the function refuses."""
+    return forward_ad._current_level >= 0 or torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
 def once_differentiable(backward):

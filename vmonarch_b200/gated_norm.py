@@ -95,7 +95,7 @@ class _GatedNorm(torch.autograd.Function):
 def gated_residual_norm(x, y=None, *, gate=None, scale=None, shift=None, weight=None, post_weight=None, norm="rms",
                         eps=1e-6, seqs=None):
     """
-    x_new = x + gate * y', h = norm(x_new) * weight * (1 + scale) + shift; differentiable in every tensor.
+    x_new = x + gate * y', h = norm(x_new) * weight * (1 + scale) + shift; differentiable in every tensor (backward only).
 
     Args:
         x: (T, C) residual stream, bf16 or fp16, C a multiple of 8 up to 8192
@@ -130,7 +130,6 @@ def gated_residual_norm(x, y=None, *, gate=None, scale=None, shift=None, weight=
         assert seqs.device == device, "x and seqs must be on one CUDA device"
         assert seqs.total_q == rows, f"x has {rows} rows, the sequences {seqs.total_q}"
         assert count <= 65535, "at most 65535 sequences"
-    needed = x.requires_grad or (y is not None and y.requires_grad)
     params, dtype, wide, tall = [], None, (c,), (count, c)
     for name, t in zip(_PARAMS, (gate, scale, shift, weight, post_weight)):
         if t is not None:
@@ -144,13 +143,12 @@ def gated_residual_norm(x, y=None, *, gate=None, scale=None, shift=None, weight=
                 assert t.shape == wide, f"{name} must be ({c},)"
             else:
                 assert t.shape == tall, f"{name} must be ({count}, {c})"
-            needed = needed or t.requires_grad
             if t.data_ptr() & 15 or not t.is_contiguous():
                 t = _dense(t)
         params.append(t)
     code = N.dtype_code(kind)
     sizes = (rows, c, count, code, N.VMB_DTYPE_F32 if dtype == torch.float32 else code, norm == "layer", eps)
-    if needed and torch.is_grad_enabled():
+    if N.derived(x, y, *params):
         out = _GatedNorm.apply(x, y, seqs, sizes, *params)
         return (x, out[0]) if y is None else out
     x_new, h = _forward(x, y, params, seqs, sizes, None)[2:]

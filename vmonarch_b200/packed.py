@@ -354,7 +354,7 @@ class _PackedAttention(torch.autograd.Function):
 
 def packed_attention(q, k, v, seqs, *, causal=False, sm_scale=None, return_lse=False):
     """
-    Softmax attention over packed sequences, differentiable in q, k and v.
+    Softmax attention over packed sequences, differentiable in q, k and v (backward only).
 
     Args:
         q: (total_q, H, D), bf16 or fp16, D a multiple of 8 up to 128
@@ -390,7 +390,7 @@ def packed_attention(q, k, v, seqs, *, causal=False, sm_scale=None, return_lse=F
     sm_scale = d ** -0.5 if sm_scale is None else float(sm_scale)
     assert 0 <= sm_scale < float("inf"), "sm_scale must be finite and not negative"
     key = (False, bool(causal), sm_scale, dtype, heads, kv_heads, d)
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+    if N.derived(q, k, v):
         return _PackedAttention.apply(q, k, v, seqs, key, return_lse)
     lse = torch.empty((heads, rows), dtype=torch.float32, device=device) if return_lse else None
     o = _forward(q, k, v, seqs, key, device, lse)[3]
