@@ -138,9 +138,10 @@ __device__ __forceinline__ bool finite16(uint32_t h) {  // one element in the lo
   return (h & kExp) != kExp;
 }
 
-// Clears what is not finite in row `row` of a [128][64 NA] tile; true if there was any.
+// Clears what is not finite in row `row` of a [128][64 NA] tile, once `*dirty` is `mark`. Both streams may do so to one
+// tile at a time: each finds a value or its clearing, and the mark with the latter.
 template <typename T, int NA>
-__device__ __forceinline__ bool clean_row(uint32_t tile, int row) {
+__device__ __forceinline__ void clean_row(uint32_t tile, int row, volatile int* dirty, int mark) {
   uint32_t acc = 0;
 #pragma unroll
   for (int c = 0; c < 8 * NA; ++c) {  // neighbouring rows begin at different chunks: no bank conflicts
@@ -151,18 +152,21 @@ __device__ __forceinline__ bool clean_row(uint32_t tile, int row) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) acc = zero_fma2<T>(x[e], acc);
   }
-  if (finite16<T>(acc) && finite16<T>(acc >> 16)) return false;
+  const bool clean = finite16<T>(acc) && finite16<T>(acc >> 16);
+  if (!clean) *dirty = mark;
+  __threadfence_block();
+  if (!clean) {
 #pragma unroll 1
-  for (int w = 0; w < 32 * NA; ++w) {
-    const uint32_t at = tile + (w >> 5) * kAtom + row * 128 + (w & 31) * 4;
-    uint32_t x;
-    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(x) : "r"(at));
-    if (!finite16<T>(x)) x &= 0xffff0000u;
-    if (!finite16<T>(x >> 16)) x &= 0x0000ffffu;
-    asm volatile("st.shared.b32 [%0], %1;" ::"r"(at), "r"(x) : "memory");
+    for (int w = 0; w < 32 * NA; ++w) {
+      const uint32_t at = tile + (w >> 5) * kAtom + row * 128 + (w & 31) * 4;
+      uint32_t x;
+      asm volatile("ld.shared.b32 %0, [%1];" : "=r"(x) : "r"(at));
+      if (!finite16<T>(x)) x &= 0xffff0000u;
+      if (!finite16<T>(x >> 16)) x &= 0x0000ffffu;
+      asm volatile("st.shared.b32 [%0], %1;" ::"r"(at), "r"(x) : "memory");
+    }
   }
-  fence_proxy_async_smem();  // read by the P V MMA (async proxy)
-  return true;
+  fence_proxy_async_smem();  // read by the P V MMA (async proxy), whichever thread cleared it
 }
 
 // A work item, made by the K producer and read by every role from shared memory.
@@ -432,7 +436,7 @@ __global__ void __launch_bounds__(kThreads, 1) packed_fwd_kernel(const __grid_co
         // rows past the unit's last query are not stored: they take its limit, and no part in the reference
         live = 128 * w + row < it.u.q_valid;
         my_lim = it.limit(min(128 * w + row, it.u.q_valid - 1));
-        lim_lo = it.limit(128 * w);
+        lim_lo = it.limit(0);  // of the unit's first query, for both streams
       }
       float m_ref = -1e30f, l = 0.f;
       // O and l to the reference max(m_ref, mx). Warp-uniform; no P V into O_w may be in flight.
@@ -466,7 +470,7 @@ __global__ void __launch_bounds__(kThreads, 1) packed_fwd_kernel(const __grid_co
         // unit's first half sets it); a half past the threshold is redone from the scores in registers, once
         // no P V into O is under way: S_w(t) complete implies that every earlier one is done, and in the second
         // half the first half's is waited for.
-        if (t > 0 && lim_lo - k0 >= 128) {  // no query of the stream misses a key of the tile
+        if (t > 0 && lim_lo - k0 >= 128) {  // no query of the unit misses a key of the tile
 #pragma unroll
           for (int hf = 0; hf < 2; ++hf) {
             uint32_t s[64], pk[32];
@@ -490,10 +494,12 @@ __global__ void __launch_bounds__(kThreads, 1) packed_fwd_kernel(const __grid_co
           }
         } else {
           if (lim_lo - k0 < 128) {
-            // values that some query of the stream must not see: clear what is not finite (thread = key row)
+            // Values that some query of the unit must not see: clear what is not finite (thread = key row). Both streams
+            // look, also the one whose queries see the whole tile: the other's clearing may come before its product or
+            // after, and the epilogue adds back what was cleared in the tiles from here on.
             const int sv = (ring + t) % NV;
             if (!(ok = warp_wait(B_VFULL + sv, ((ring + t) / NV) & 1, 8))) break;
-            if (clean_row<T, NA>(sV + sv * TILE, row)) dirty_sh[i & 1] = i + 1;
+            clean_row<T, NA>(sV + sv * TILE, row, &dirty_sh[i & 1], i + 1);
           }
 #pragma unroll 1
           for (int hf = 0; hf < 2; ++hf) {
