@@ -260,20 +260,20 @@ def launch(what: str, fn, device: torch.device, *args) -> None:
     """Calls a C entry with `args` and the current stream of `device`, which is made the current device for the call
     where it is not: the entries set up and launch kernels on the current device, and a stream handle alone does not
     name one (every device's default stream has the handle 0)."""
-    index = current_device() if device.index is None else device.index
+    index = device.index
     if index == current_device():
         rc = fn(*args, raw_stream(index))
     else:
-        with torch.cuda.device(index):
-            rc = fn(*args, raw_stream(index))
+        with torch.cuda.device(current_device() if index is None else index):
+            rc = fn(*args, raw_stream(current_device()))
     if rc:
         check(rc, what)
 
 
-def derived(*tensors) -> bool:
-    """Whether a call on these tensors (or None) goes through its autograd function: one of them requires a gradient, or
-    a level of forward-mode derivatives is open, whose dual tensors the function refuses."""
-    return forward_ad._current_level >= 0 or torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+def derived(needed: bool) -> bool:
+    """Whether a call goes through its autograd function: an input requires a gradient (`needed`), or a level of
+    forward-mode derivatives is open, whose dual tensors the function refuses."""
+    return forward_ad._current_level >= 0 or needed and torch.is_grad_enabled()
 
 
 def once_differentiable(backward):

@@ -130,6 +130,7 @@ def gated_residual_norm(x, y=None, *, gate=None, scale=None, shift=None, weight=
         assert seqs.device == device, "x and seqs must be on one CUDA device"
         assert seqs.total_q == rows, f"x has {rows} rows, the sequences {seqs.total_q}"
         assert count <= 65535, "at most 65535 sequences"
+    needed = x.requires_grad or (y is not None and y.requires_grad)
     params, dtype, wide, tall = [], None, (c,), (count, c)
     for name, t in zip(_PARAMS, (gate, scale, shift, weight, post_weight)):
         if t is not None:
@@ -143,12 +144,13 @@ def gated_residual_norm(x, y=None, *, gate=None, scale=None, shift=None, weight=
                 assert t.shape == wide, f"{name} must be ({c},)"
             else:
                 assert t.shape == tall, f"{name} must be ({count}, {c})"
+            needed = needed or t.requires_grad
             if t.data_ptr() & 15 or not t.is_contiguous():
                 t = _dense(t)
         params.append(t)
     code = N.dtype_code(kind)
     sizes = (rows, c, count, code, N.VMB_DTYPE_F32 if dtype == torch.float32 else code, norm == "layer", eps)
-    if N.derived(x, y, *params):
+    if N.derived(needed):
         out = _GatedNorm.apply(x, y, seqs, sizes, *params)
         return (x, out[0]) if y is None else out
     x_new, h = _forward(x, y, params, seqs, sizes, None)[2:]

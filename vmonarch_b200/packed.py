@@ -141,6 +141,7 @@ class PackedSequences:
         self.device = torch.device(device)
         if self.device.type == "cuda" and self.device.index is None:
             self.device = torch.device("cuda", torch.cuda.current_device())
+        self._index = self.device.index if self.device.type == "cuda" else None
         self.total_q, self.total_k = int(self.q_lens.sum()), int(self.k_lens.sum())
         self.q_start = np.cumsum(self.q_lens) - self.q_lens
         self.k_start = np.cumsum(self.k_lens) - self.k_lens
@@ -168,7 +169,7 @@ class PackedSequences:
 
     def _stream(self):
         """Handle of the device's current stream."""
-        return N.raw_stream(self.device.index) if self.device.type == "cuda" else 0
+        return 0 if self._index is None else N.raw_stream(self._index)
 
     def _on_device(self, array):
         assert self.device.type != "cuda" or not torch.cuda.is_current_stream_capturing(), \
@@ -177,7 +178,7 @@ class PackedSequences:
         self._home = stream if not self._cache or stream == self._home else None
         return torch.from_numpy(array).to(self.device)
 
-    def _use(self, *tensors):
+    def _use(self, tensors):
         """Kept tensors that the current stream is about to read: where they belong to another, the allocator learns that
         their memory stays in use here, whenever the object goes."""
         if self._stream() != self._home:
@@ -187,8 +188,10 @@ class PackedSequences:
 
     def _starts(self):
         """First query row of every sequence, int32 on the device."""
-        starts = self._kept("starts", lambda: self._on_device(self.q_start.astype(np.int32)))
-        self._use(starts)
+        starts = self._cache.get("starts")
+        if starts is None:
+            starts = self._kept("starts", lambda: self._on_device(self.q_start.astype(np.int32)))
+        self._use((starts,))
         return starts
 
     # ------------------------------------------------------------------------------ work lists
@@ -294,7 +297,7 @@ def _forward(q, k, v, seqs, key, device, lse=None, aux=None):
     v, *vr = _place(v)
     o = torch.empty_like(q, memory_format=torch.contiguous_format)
     template, size, lists = seqs._template(key)
-    seqs._use(*lists)
+    seqs._use(lists)
     a = N.PackedArgs.from_buffer_copy(template)
     heads, dim = key[4], key[6]
     row = heads * dim
@@ -338,7 +341,7 @@ class _PackedAttention(torch.autograd.Function):
         do, *dor = _place(do)
         dq, dk, dv = (torch.empty_like(t, memory_format=torch.contiguous_format) for t in (q, k, v))
         template, size, lists = seqs._template((True, *key[1:]))
-        seqs._use(*lists)
+        seqs._use(lists)
         a = N.PackedArgs.from_buffer_copy(template)
         _FWD_TENSORS.pack_into(a, 0, *_place(q)[1:], *_place(k)[1:], *_place(v)[1:], o.data_ptr(), row, dim)
         low = aux.data_ptr()
@@ -390,7 +393,7 @@ def packed_attention(q, k, v, seqs, *, causal=False, sm_scale=None, return_lse=F
     sm_scale = d ** -0.5 if sm_scale is None else float(sm_scale)
     assert 0 <= sm_scale < float("inf"), "sm_scale must be finite and not negative"
     key = (False, bool(causal), sm_scale, dtype, heads, kv_heads, d)
-    if N.derived(q, k, v):
+    if N.derived(q.requires_grad or k.requires_grad or v.requires_grad):
         return _PackedAttention.apply(q, k, v, seqs, key, return_lse)
     lse = torch.empty((heads, rows), dtype=torch.float32, device=device) if return_lse else None
     o = _forward(q, k, v, seqs, key, device, lse)[3]
