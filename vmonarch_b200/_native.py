@@ -208,7 +208,9 @@ def _load() -> ctypes.CDLL:
         raise ImportError(f"vmonarch_b200: {LIB_PATH} has ABI version {lib.vmb_abi_version()}, the binding expects "
                           f"{ABI_VERSION}; rebuild it with `python vmonarch_b200/build.py`")
     for name, (res, args) in SIGNATURES.items():
-        fn = getattr(lib, name)
+        fn = getattr(lib, name, None)
+        if fn is None:  # calls are added without a new ABI version
+            raise ImportError(f"vmonarch_b200: {LIB_PATH} does not have {name}; rebuild it with `python vmonarch_b200/build.py`")
         fn.restype = res
         fn.argtypes = args
     return lib
