@@ -41,7 +41,8 @@ int check(const vmb_packed_args* a, const char* what, bool bwd) {
   if (!a) return set_error(VMB_EINVAL, "%s: null args", what);
   if (a->dtype != VMB_DTYPE_BF16 && a->dtype != VMB_DTYPE_F16)
     return set_error(VMB_EINVAL, "%s: unknown dtype %d", what, a->dtype);
-  if (a->q_total < 0 || a->k_total < 0 || a->q_total > 0x7fffffff || a->k_total > 0x7fffffff || a->stat_rows < 0)
+  if (a->q_total < 0 || a->k_total < 0 || a->q_total > 0x7fffffff || a->k_total > 0x7fffffff || a->stat_rows < 0 ||
+      (bwd && a->stat_rows > 0x7fffffff))
     return set_error(VMB_EINVAL, "%s: bad row counts", what);
   if (a->heads < 1 || a->kv_heads < 1 || a->heads % a->kv_heads)
     return set_error(VMB_EINVAL, "%s: heads=%d is not a multiple of kv_heads=%d", what, a->heads, a->kv_heads);

@@ -251,6 +251,8 @@ class PackedSequences:
         return self._kept(key, self._make_template, *key) if hit is None else hit
 
     def _make_template(self, backward, causal, sm_scale, dtype, heads, kv_heads, dim):
+        assert not backward or self.stat_rows < 2 ** 31, \
+            f"the backward's statistics have 32-bit rows: {self.num_sequences} sequences padded to 128 rows each are too many"
         a = N.PackedArgs()
         a.q_total, a.k_total, a.stat_rows = self.total_q, self.total_k, self.stat_rows
         a.heads, a.kv_heads, a.dim = heads, kv_heads, dim
