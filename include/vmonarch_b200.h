@@ -50,11 +50,13 @@ const char* vmb_last_error(void);
 int vmb_device_status(void* stream, int32_t* out);
 
 /* Test hook of the pipeline-timeout path; no counterpart in the reference. wait_cycles > 0
- * shortens the tcgen05 forward kernels' pipeline wait limit to that many SM cycles; hold_loads != 0
- * (only with 0 < wait_cycles <= 1e8) makes their load producers issue no copy, so the consumers'
- * first waits run out: the kernels record their codes (vmb_device_status), drain, free their
- * tensor memory and exit with their outputs invalid. (0, 0) restores normal operation. The
- * setting is process-wide and read at each vmb_fea_fwd call; it exists for tests only. */
+ * shortens the pipeline wait limit of the tcgen05 forward kernels and of the packed and paged attention
+ * kernels to that many SM cycles; hold_loads != 0 (only with 0 < wait_cycles <= 1e8) makes their
+ * load producers (paged: one of a block's four warps) issue no copy, so the consumers' first waits
+ * run out: the kernels record their codes (vmb_device_status), drain, free their tensor memory and
+ * exit with their outputs invalid. (0, 0) restores normal operation. The setting is process-wide and
+ * read at each vmb_fea_fwd, vmb_packed_fwd, vmb_packed_bwd and vmb_paged_attention call; it exists
+ * for tests only. */
 int vmb_test_pipeline_timeout(int64_t wait_cycles, int32_t hold_loads);
 
 /* Number of kernels this library has launched in the process so far (all threads, all devices).

@@ -14,7 +14,7 @@ namespace {
 
 thread_local std::string g_last_error;
 std::atomic<uint64_t> g_launches{0};
-// vmb_test_pipeline_timeout: shortened wait limit and load hold of the tcgen05 forward kernels
+// vmb_test_pipeline_timeout: shortened wait limit and load hold of the kernels with a pipeline of loads
 std::atomic<int64_t> g_test_wait_cycles{0};
 std::atomic<int> g_test_hold_loads{0};
 
@@ -100,6 +100,10 @@ int set_error(int code, const char* fmt, ...) {
   return code;
 }
 void count_launches(int n) { count(n); }
+void test_timeout(long long* wait_limit, int* hold_loads) {
+  *wait_limit = g_test_wait_cycles.load(std::memory_order_relaxed);
+  *hold_loads = g_test_hold_loads.load(std::memory_order_relaxed);
+}
 }  // namespace vmb
 
 extern "C" {
@@ -190,8 +194,7 @@ int vmb_fea_fwd(const vmb_fea_fwd_args* a, void* stream) {
   p.e4m3 = e4m3;
   p.n_q = (int)a->n_q; p.n_kv = (int)a->n_kv; p.dv1 = a->dv1;
   p.scale_log2 = a->sm_scale * kLog2eHost;
-  p.wait_limit = g_test_wait_cycles.load(std::memory_order_relaxed);
-  p.hold_loads = g_test_hold_loads.load(std::memory_order_relaxed);
+  vmb::test_timeout(&p.wait_limit, &p.hold_loads);
   p.work = a->workspace;
   p.work_bytes = a->workspace ? a->workspace_bytes : 0;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);

@@ -99,6 +99,7 @@ vmb::PackedParams params(const vmb_packed_args* a) {
   p.q = a->q.ptr; p.k = a->k.ptr; p.v = a->v.ptr; p.o = a->o.ptr; p.o_low = a->o_low.ptr;
   p.dout = a->dout.ptr; p.dq = a->dq.ptr; p.dk = a->dk.ptr; p.dv = a->dv.ptr;
   p.lse = a->lse;
+  vmb::test_timeout(&p.wait_limit, &p.hold_loads);
   p.qv = view(a->q); p.kv = view(a->k); p.vv = view(a->v); p.ov = view(a->o); p.olv = view(a->o_low);
   p.dov = view(a->dout); p.dqv = view(a->dq); p.dkv = view(a->dk); p.dvv = view(a->dv);
   return p;

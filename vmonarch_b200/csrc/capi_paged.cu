@@ -47,6 +47,7 @@ int fill(const vmb_paged_args* a, vmb::PagedParams& p) {
     return set_error(VMB_EINVAL, "%s: sm_scale must be finite and not negative", what);
   p.q = a->q.ptr; p.k = a->k.ptr; p.v = a->v.ptr; p.o = a->o.ptr;
   p.lse = a->lse;
+  vmb::test_timeout(&p.wait_limit, &p.hold_loads);
   p.table = a->table;
   p.lengths = a->lengths;
   p.q_row = a->q.row; p.q_head = a->q.head; p.o_row = a->o.row; p.o_head = a->o.head;

@@ -126,6 +126,8 @@ __device__ __forceinline__ void wait_for_kernel_before() { asm volatile("griddep
 __device__ __forceinline__ void let_next_kernel_start() { asm volatile("griddepcontrol.launch_dependents;"); }
 #endif
 
+// What vmb_test_pipeline_timeout has set: a pipeline wait limit in cycles (0: the default), and whether loads are held.
+void test_timeout(long long* wait_limit, int* hold_loads);
 // Adds n to the library's kernel launch count.
 void count_launches(int n);
 // Records `code` and a printf-style message as the calling thread's last error; returns `code`.

@@ -40,6 +40,8 @@ struct PackedParams {
   float* centre;           // backward: mean of a sequence's first keys, [kv_heads][stat_rows / 128][128]
   float *part, *part_ml;   // split units: partial tiles and their (max, sum)
   View qv, kv, vv, ov, olv, dov, dqv, dkv, dvv;  // rows = tokens, s1 = head stride
+  long long wait_limit;    // pipeline wait limit in cycles (0: the default ~2 s)
+  int hold_loads;          // test of the timeout path: the producers issue no load
 };
 
 // Unit and head of a block: chunks of `chunk` heads outermost (their keys and values stay in L2),

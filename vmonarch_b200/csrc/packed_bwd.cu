@@ -363,7 +363,7 @@ __global__ void __launch_bounds__(kThreads, 1) packed_dkdv_kernel(const __grid_c
 
   if (warp == 0) {
     // ---------------------------------------------------------------- TMA producer
-    if (lane == 0 && n > 0) {
+    if (lane == 0 && n > 0 && !p.a.hold_loads) {
       int armed[NQ];
       for (int s = 0; s < NQ; ++s) armed[s] = 0;
       prefetch_tmap(&p.tm_q);
@@ -375,7 +375,7 @@ __global__ void __launch_bounds__(kThreads, 1) packed_dkdv_kernel(const __grid_c
       }
       for (int i = 0; i < n; ++i) {
         const int s = i % NQ;
-        if (i >= NQ && !mbar_wait(BAR_QEMPTY(s), ((i / NQ) - 1) & 1, abort, &g_packed_bwd_err, 1)) break;
+        if (i >= NQ && !mbar_wait(BAR_QEMPTY(s), ((i / NQ) - 1) & 1, abort, &g_packed_bwd_err, 1, p.a.wait_limit)) break;
         const int h = step_head(i), q0 = step_q0(i);
         mbar_expect_tx(BAR_QFULL(s), C::SLOT_T + 512);
         for (int x = 0; x < NA; ++x) {
@@ -402,7 +402,7 @@ __global__ void __launch_bounds__(kThreads, 1) packed_dkdv_kernel(const __grid_c
     // ---------------------------------------------------------------- MMA issuer
     const uint32_t leader = elect_one() ? 1u : 0u;
     auto wwait = [&](uint32_t bar, uint32_t parity, int code) -> bool {
-      return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort, &g_packed_bwd_err, code));
+      return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort, &g_packed_bwd_err, code, p.a.wait_limit));
     };
     // S^T = K Q^T or dP^T = V dO^T of step i, whose slot has landed
     auto issue = [&](int i, bool dp) {
@@ -462,7 +462,7 @@ __global__ void __launch_bounds__(kThreads, 1) packed_dkdv_kernel(const __grid_c
     const uint32_t lane_off = (uint32_t)(quad * 32) << 16;
     const int tid = (wg & 1) * 128 + (threadIdx.x - 64) % 128;  // within the stream's 256 threads
     auto warp_wait = [&](uint32_t bar, uint32_t parity, int code) -> bool {
-      return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort, &g_packed_bwd_err, code));
+      return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort, &g_packed_bwd_err, code, p.a.wait_limit));
     };
     const uint32_t ts = tmem + lane_off + 128 * stm, tdp = ts + 64;
     const float2 sc2 = make_float2(p.scale_log2, p.scale_log2), sm2 = make_float2(p.a.sm_scale, p.a.sm_scale);
@@ -642,7 +642,7 @@ __global__ void __launch_bounds__(kThreads, 1) packed_dq_kernel(const __grid_con
 
   if (warp == 0) {
     // ---------------------------------------------------------------- TMA producers: lane 0 Q, dO, K; lane 1 V
-    if (lane < 2 && n > 0) {
+    if (lane < 2 && n > 0 && !p.a.hold_loads) {
       const bool kl = lane == 0;
       const int nslot = kl ? NK : NV;
       const CUtensorMap* map = kl ? &p.tm_k : &p.tm_v;
@@ -658,7 +658,7 @@ __global__ void __launch_bounds__(kThreads, 1) packed_dq_kernel(const __grid_con
       for (int s = 0; s < nslot; ++s) armed[s] = 0;
       for (int j = 0; j < n; ++j) {
         const int s = j % nslot;
-        if (j >= nslot && !mbar_wait(BAR((kl ? B_KEMPTY : B_VEMPTY) + s), ((j / nslot) - 1) & 1, abort, &g_packed_bwd_err, 16))
+        if (j >= nslot && !mbar_wait(BAR((kl ? B_KEMPTY : B_VEMPTY) + s), ((j / nslot) - 1) & 1, abort, &g_packed_bwd_err, 16, p.a.wait_limit))
           break;
         const uint32_t full = BAR((kl ? B_KFULL : B_VFULL) + s);
         const int row = u.k_row + (u.begin + j) * 128;
@@ -677,7 +677,7 @@ __global__ void __launch_bounds__(kThreads, 1) packed_dq_kernel(const __grid_con
     // ---------------------------------------------------------------- MMA issuer
     const uint32_t leader = elect_one() ? 1u : 0u;
     auto wwait = [&](int bar, uint32_t parity, int code) -> bool {
-      return __all_sync(0xffffffffu, mbar_wait(BAR(bar), parity, abort, &g_packed_bwd_err, code));
+      return __all_sync(0xffffffffu, mbar_wait(BAR(bar), parity, abort, &g_packed_bwd_err, code, p.a.wait_limit));
     };
     auto issue = [&](int j, bool dp) -> bool {  // S(j) = Q K^T, or dP(j) = dO V^T
       const int s = dp ? j % NV : j % NK;
@@ -730,7 +730,7 @@ __global__ void __launch_bounds__(kThreads, 1) packed_dq_kernel(const __grid_con
     const float2 nl2 = make_float2(fl, fl), nc2 = make_float2(fc, fc);
     const float2 sc2 = make_float2(p.scale_log2, p.scale_log2), sm2 = make_float2(fs, fs);
     auto warp_wait = [&](int bar, uint32_t parity, int code) -> bool {
-      return __all_sync(0xffffffffu, mbar_wait(BAR(bar), parity, abort, &g_packed_bwd_err, code));
+      return __all_sync(0xffffffffu, mbar_wait(BAR(bar), parity, abort, &g_packed_bwd_err, code, p.a.wait_limit));
     };
     if (tid < 64 * NA) centre_sh[tid] = p.a.centre[((int64_t)kvh * (p.a.stat_rows >> 7) + (u.stat_row >> 7)) * 128 + tid];
     float sum = 0.f;  // of this thread's rounded dS

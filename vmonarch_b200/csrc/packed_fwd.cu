@@ -250,13 +250,15 @@ __global__ void __launch_bounds__(kThreads, 1) packed_fwd_kernel(const __grid_co
 
   // The K producer hands the items on through work_sh: item i in place i & 1 until its ten readers are done with it.
   auto work_wait = [&](int i, int code) -> bool {
-    return mbar_wait(BAR(B_WFULL + (i & 1)), (i >> 1) & 1, abort, &g_packed_err, code);
+    // (the one wait that runs out when loads are held, so the one with a limit that a test can shorten)
+    return mbar_wait(BAR(B_WFULL + (i & 1)), (i >> 1) & 1, abort, &g_packed_err, code, p.a.wait_limit);
   };
 
   if (warp == 0) {
     // ------------------------------------------------------------------ TMA producers
     // lane 0: work ring, Q and the K ring; lane 1: the V ring
-    if (lane < 2) {
+    // (hold_loads, a test of the timeout path: no work is handed on, so every other role's wait runs out)
+    if (lane < 2 && !p.a.hold_loads) {
       const bool kl = lane == 0;
       const int nslot = kl ? NK : NV;
       const CUtensorMap* map = kl ? &p.tm_k : &p.tm_v;

@@ -20,6 +20,8 @@ struct PagedParams {
   int group, nt, chunks, items, whole_items, box_rows, join_blocks;
   int64_t blocks;
   float *part, *part_ml;
+  long long wait_limit;  // pipeline wait limit in cycles (0: the default ~2 s)
+  int hold_loads;        // test of the timeout path: the first warp of a block issues no load
 };
 
 // Pages of [kv_heads][page_size][dim] elements, by strides.

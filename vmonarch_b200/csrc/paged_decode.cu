@@ -30,8 +30,8 @@
 // 64 sequences of up to 8190 tokens, 40/8 heads, D = 128, pages of 16: 44 us, 4.3 TB/s; 3 of up to 262143, 16/4 heads,
 // pages of 64: 92 us, 5.8 TB/s (the measured copy rate is 6.5); one of 201 tokens, 8/2 heads, D = 64: 8.2 us.
 //
-// Waits for a stage are bounded (sm100.cuh): a block that gives up records a code, drains its copies and
-// leaves its outputs invalid.
+// Waits for a stage are bounded (sm100.cuh): a warp that gives up records a code, goes through the rest of its share
+// without loads, waits and products, drains its copies and leaves the block's outputs invalid.
 #include <numeric>
 
 #include "common.cuh"
@@ -185,6 +185,7 @@ __global__ void __launch_bounds__(32 * kWarps, 2) paged_decode_kernel(const __gr
   // ---- loading. A stage's boxes: (row group of box_rows tokens) x (K, V) x atoms; lane i issues boxes i, i + 32.
   const int boxes = 16 / p.box_rows * 2 * C::NA;
   Cursor lc = cc;
+  if (p.hold_loads && warp == 0) lc.left = 0;
   int issued = 0;
   int page[2], slot[2];  // of this lane's boxes of the stage that is issued next
   auto look_up = [&](const Cursor& c) {
@@ -257,12 +258,12 @@ __global__ void __launch_bounds__(32 * kWarps, 2) paged_decode_kernel(const __gr
   if (cc.left > 0) load_q(cc);
   clear();
   for (int it = 0; cc.left > 0; ++it) {
-    if (!__all_sync(0xffffffffu, mbar_wait(bar0 + 8u * (it % C::STAGES), (it / C::STAGES) & 1, abort, &g_paged_err, 1))) {
-      ok = false;
-      break;
+    if (ok && !__all_sync(0xffffffffu, mbar_wait(bar0 + 8u * (it % C::STAGES), (it / C::STAGES) & 1, abort, &g_paged_err, 1, p.wait_limit))) {
+      ok = false;  // no more loads and products, but on to the barriers that the block's warps share
+      lc.left = 0;
     }
     const uint32_t ks_base = ring + (it % C::STAGES) * C::STAGE, vs_base = ks_base + C::NA * C::ATOM;
-    const int left = cc.len - cc.tile * kTile - 16 * warp;  // tokens of this warp's rows
+    const int left = ok ? cc.len - cc.tile * kTile - 16 * warp : 0;  // tokens of this warp's rows
     if (left > 0) {
       if (left < 16) {  // slots without a token: their values enter the product with weight 0
         for (int i = lane; i < (16 - left) * 8 * C::NA; i += 32) {
