@@ -166,7 +166,8 @@ __device__ __forceinline__ void clean_row(uint32_t tile, int row, volatile int* 
       asm volatile("st.shared.b32 [%0], %1;" ::"r"(at), "r"(x) : "memory");
     }
   }
-  fence_proxy_async_smem();  // read by the P V MMA (async proxy), whichever thread cleared it
+  // read by the P V MMA (async proxy), whichever thread cleared it (16 mixed prompts: 408 us with the fence always, 403 so)
+  if (*dirty == mark) fence_proxy_async_smem();
 }
 
 // A work item, made by the K producer and read by every role from shared memory.
