@@ -22,7 +22,8 @@
 // sequence into shared memory: from L2 it would be more than the rows' own traffic. The column sums
 // of the backward stay in registers over a block's rows of a sequence; each (block, sequence) leaves one
 // 32-bit partial row, added in a fixed order by a second kernel. 16637 rows of 5120 columns, layer norm and post norm,
-// fp32 parameters: forward 127 us, backward 218 us with its sums (82 % and 72 % of the measured copy rate); 24 rows: 5.2 us.
+// fp32 parameters: forward 131 us, backward 232 us with its sums, calls in a row (79 % and 67 % of the measured copy rate);
+// 24 rows, two rms norms: 5.2 us, replayed in a graph.
 #include <algorithm>
 
 #include "common.cuh"
@@ -794,7 +795,7 @@ cudaError_t run(Kern kern, std::atomic<uint64_t>& ready, const Shape& s, GatedNo
 }
 
 // Forward. Few rows (a serving step: one a block at most): one vector a thread, the shortest way through a row
-// (24 rows of 5120: 5.5 us, with four vectors 7.6 us). Else four vectors a thread: a row's sums then cost a
+// (24 rows of 5120, two rms norms: 5.2 us, with four vectors 7.4 us, replayed in a graph). Else four vectors a thread: a row's sums then cost a
 // quarter per column, and four rows of 5120 columns are under way on an SM with 640 threads (16576 rows, layer
 // norm with a post norm: 119 us, two vectors 130 us; the floor is 104 us). Rows that would leave lanes
 // without a vector take fewer, and so do rows so wide that four vectors would leave an SM less than 512 threads.

@@ -13,7 +13,7 @@
 //       D takes o with the 16 bits that its rounding left out (o_low): an error of D is shared by a
 //       whole row of dS, so it does not average out in dQ_i = sum_j dS_ij k_j where keys have a mean
 //       (4000 causal queries, D = 128, bf16: dQ off by 4.1e-3 without it, 2.4e-3 with it, of which its
-//       own rounding is 1.7e-3).
+//       own rounding is 1.7e-3). The forward's rounding of P is in o all the same, and so in D.
 // dkdv  CTA = 128 keys of one key head; walks (query head, 64-query tile): S^T = K Q^T and
 //       dP^T = V dO^T (SS), P^T and dS^T (16-bit) back to TMEM over them, dV += P^T dO and
 //       dK += dS^T Q (TS). thread = key row; two streams of tiles, two warpgroups each. P^T is handed over before dS^T is
@@ -28,11 +28,12 @@
 //       around a mean of 0.3, D = 128, bf16: error of dQ 1.49 -> 1.43 times that of its own rounding).
 //       TMEM: S0 [0,128) S1 [128,256) dP [256,384) dQ [384, +64 NA).
 // A query that sees one key has dS = 0 by its index, where dP - D would leave a rounding.
-// Seven products per tile pair instead of five: TMEM cannot hold S, dP, dK, dV and dQ of one tile at
-// once, and recomputing S and dP costs less than adding dQ through memory.
+// Seven products per tile pair instead of five: above D = 64 TMEM cannot hold S, dP, dK, dV and dQ of one tile at
+// once, and recomputing S and dP costs less than adding dQ through memory in 32 bits. (Neither dS kept in memory in 16
+// bits for dQ nor the 128 columns that are idle up to D = 64 have been tried here.)
 // Bound by the tensor products (operands from shared memory) and the latencies between them. 15600 + 1289 + 409 + 1
 // causal tokens, 16/4 heads, D = 128, bf16: pre 48 us, dkdv 1650 us (1.22 PFLOP/s of its four products), dq 1160 us
-// (1.30 PFLOP/s of its three), 2690 us with the set-ups overlapped; five products at the measured dense rate (1.67 PFLOP/s) would take 1500 us.
+// (1.30 PFLOP/s of its three), 2720 us with the set-ups overlapped; five products at the measured dense rate (1.67 PFLOP/s) would take 1500 us.
 //
 // Tiles at a sequence's end hold the next sequence's rows. Their scores are dropped by index, and the
 // rows that enter a sum with weight 0 (Q and dO here, K in dq) are cleared in shared memory first, so

@@ -20,15 +20,15 @@
 // softmax warps write the last item's output straight from registers, and the set-up is paid once per SM.
 // Bound by the instructions of the softmax warps (part of the exponentials as polynomials gained nothing):
 // 2 us a 256 x 128 tile at D = 128, 4.2 us an item beside its tiles. 32760 causal tokens, 16/4 heads, D = 128, bf16:
-// 3460 us, 1.27 PFLOP/s in short runs, 1.07 under the power cap; 16 prompts of 1 to 4093 tokens, 40/8 heads: 414 us,
-// 0.82 PFLOP/s (the measured dense rate is 1.67).
+// 3600 us, 1.22 PFLOP/s in short runs, 4090 us, 1.07 under the power cap; 16 prompts of 1 to 4093 tokens, 40/8 heads: 403 us,
+// 0.84 PFLOP/s in short runs (the measured dense rate is 1.67).
 // An item that is cut leaves 32-bit partials (max, sum, O), joined by a second kernel; the host cuts
 // where few items would leave SMs without work.
 //
 // The sequences share one tensor, so a tile's rows past the sequence end are the next sequence's.
-// Scores past the end (or after the diagonal) are dropped by index. A value row that no query of the
-// tile sees enters P V with p = 0, and 0 x inf = NaN, so in a tile that is masked for some row the
-// threads look the value tile over (one multiply by zero per pair) and clear what is not finite;
+// Scores past the end (or after the diagonal) are dropped by index. A value row that a query does not
+// see enters its P V with p = 0, and 0 x inf = NaN, so in a tile that is masked for some query of the unit the
+// threads of both streams look the value tile over (one multiply by zero per pair) and clear what is not finite;
 // the epilogue then adds those values back, from global memory, to the queries that do see them.
 //
 // Head dims below 64 NA load as zeros past the tensor's columns (TMA) and store only their own.

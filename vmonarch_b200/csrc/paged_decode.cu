@@ -3,8 +3,8 @@
 //   o_b,h = sum_t p_t v_t / sum_t p_t,  p_t = exp(sm_scale q_b,h . k_t - m),  t < lengths[b],
 // where token t of sequence b lies in slot t % page_size of page table[b][t / page_size].
 //
-// Every cached key and value is read once for all the query heads that share it, so the work is bound
-// by memory: 4 D bytes and 4 D group flops a token and key head. The work items (sequence, key
+// Every cached key and value is read once for up to 16 query heads that share it (larger groups go in chunks of 16), so the
+// work is bound by memory: 4 D bytes and 4 D group flops a token and key head. The work items (sequence, key
 // head, chunk of up to 8 NT query heads), each a run of 64-token tiles behind kItemCost units for its start
 // and end, are laid end to end and every block takes an equal share of the units, whatever the
 // sequences' lengths. An item that lies in one block is finished there; one that is cut leaves a partial
@@ -28,7 +28,7 @@
 // the pool and columns past D arrive as zeros (coordinates outside the tensor map).
 //
 // 64 sequences of up to 8190 tokens, 40/8 heads, D = 128, pages of 16: 44 us, 4.3 TB/s; 3 of up to 262143, 16/4 heads,
-// pages of 64: 92 us, 5.8 TB/s (the measured copy rate is 6.5); one of 201 tokens, 8/2 heads, D = 64: 8.2 us.
+// pages of 64: 93 us, 5.8 TB/s (the measured copy rate is 6.5); one of 201 tokens, 8/2 heads, D = 64: 6.5 us, replayed in a graph.
 //
 // Waits for a stage are bounded (sm100.cuh): a warp that gives up records a code, goes through the rest of its share
 // without loads, waits and products, drains its copies and leaves the block's outputs invalid.
@@ -258,7 +258,8 @@ __global__ void __launch_bounds__(32 * kWarps, 2) paged_decode_kernel(const __gr
   if (cc.left > 0) load_q(cc);
   clear();
   for (int it = 0; cc.left > 0; ++it) {
-    if (ok && !__all_sync(0xffffffffu, mbar_wait(bar0 + 8u * (it % C::STAGES), (it / C::STAGES) & 1, abort, &g_paged_err, 1, p.wait_limit))) {
+    if (ok && !__all_sync(0xffffffffu, mbar_wait(bar0 + 8u * (it % C::STAGES), (it / C::STAGES) & 1, abort, &g_paged_err, 1,
+                                                 p.wait_limit))) {
       ok = false;  // no more loads and products, but on to the barriers that the block's warps share
       lc.left = 0;
     }
@@ -491,6 +492,7 @@ cudaError_t launch(const PagedParams& p, cudaStream_t st) {
   static std::atomic<uint64_t> ready{0};
   cudaError_t e = allow_smem(kern, C::SMEM, ready);
   if (e != cudaSuccess) return e;
+  // not launched early: the join behind it reads the lengths before it waits, and this kernel's start is what makes them final
   kern<<<(unsigned)p.blocks, 32 * kWarps, C::SMEM, st>>>(kp);
   e = cudaGetLastError();
   if (e != cudaSuccess || p.whole_items) return e;
