@@ -309,10 +309,10 @@ int vmb_cast_f32_view(const float* src, const vmb_view* src_view, void* dst, con
  * piece of work that is split over its key tiles (dQ, forward) or steps (dK / dV); the pieces of a
  * split unit take consecutive slots, and `joins` lists them as (first unit, number of pieces). lone
  * (kv_units): the sequence's queries below it see one key at most, so their dS is zero; 0 where that is
- * not known. pieces: the host's own.
+ * not known. extra: 0. pieces: the host's own.
  */
 typedef struct vmb_packed_unit {
-  int32_t q_row, q_valid, k_row, k_valid, vis0, begin, end, part, stat_row, pieces, lone, reserved;
+  int32_t q_row, q_valid, k_row, k_valid, vis0, begin, end, part, stat_row, pieces, lone, extra;
 } vmb_packed_unit;
 
 typedef struct vmb_packed_list {
@@ -345,6 +345,14 @@ int64_t vmb_packed_fwd_workspace_bytes(const vmb_packed_args* a);
 int64_t vmb_packed_bwd_workspace_bytes(const vmb_packed_args* a);
 int vmb_packed_fwd(const vmb_packed_args* a, void* stream);
 int vmb_packed_bwd(const vmb_packed_args* a, void* stream);
+/* The same with a window (causal only): of the keys below its limit n a query sees the last `window` >= 1 and the first
+ * `sinks` >= 0. units and q_units leave out the key tiles between the first sinks and the window of the unit's first
+ * query: tile x of [begin, end) is key tile x below lone (the tiles of the sinks; 0 where nothing is left out) and
+ * x + extra from there on. kv_units: the unit's first `extra` keys are sinks; without any the steps of a head end at the
+ * tile of the last query that sees the unit's last key (local query vis0 + k_valid - 2 + window). lone there: all of
+ * the sequence's queries where window + sinks is 1. */
+int vmb_packed_window_fwd(const vmb_packed_args* a, int32_t window, int32_t sinks, void* stream);
+int vmb_packed_window_bwd(const vmb_packed_args* a, int32_t window, int32_t sinks, void* stream);
 
 /*
  * Paged key / value caches (no reference counterpart). A pool holds num_pages >= 1 pages of page_size slots;

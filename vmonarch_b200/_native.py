@@ -186,6 +186,8 @@ SIGNATURES = {
     "vmb_packed_bwd_workspace_bytes": (c_i64, [ctypes.POINTER(PackedArgs)]),
     "vmb_packed_fwd": (ctypes.c_int, [ctypes.POINTER(PackedArgs), c_vp]),
     "vmb_packed_bwd": (ctypes.c_int, [ctypes.POINTER(PackedArgs), c_vp]),
+    "vmb_packed_window_fwd": (ctypes.c_int, [ctypes.POINTER(PackedArgs), c_i32, c_i32, c_vp]),
+    "vmb_packed_window_bwd": (ctypes.c_int, [ctypes.POINTER(PackedArgs), c_i32, c_i32, c_vp]),
     "vmb_gated_norm_bwd_workspace_bytes": (c_i64, [ctypes.POINTER(GatedNormArgs)]),
     "vmb_gated_norm_fwd": (ctypes.c_int, [ctypes.POINTER(GatedNormArgs), c_vp]),
     "vmb_gated_norm_bwd": (ctypes.c_int, [ctypes.POINTER(GatedNormArgs), c_vp]),

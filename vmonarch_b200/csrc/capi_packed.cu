@@ -85,8 +85,21 @@ int64_t stat_bytes(const vmb_packed_args* a) {
   return plane_bytes(a) + tile_bytes(a) + up256(a->kv_heads * (a->stat_rows / 128) * 128 * 4);
 }
 
-vmb::PackedParams params(const vmb_packed_args* a) {
+// With a window, rows are at most this many, so that windows and sinks above it are alike and sums with them stay in 32 bits.
+constexpr int kWide = (1 << 30) - 1024;
+int check_window(const vmb_packed_args* a, int32_t window, int32_t sinks, const char* what) {
+  if (!a) return set_error(VMB_EINVAL, "%s: null args", what);
+  if (!a->causal || window < 1 || sinks < 0)
+    return set_error(VMB_EINVAL, "%s: a window is causal, of one key at least, and sinks are not negative", what);
+  if (a->q_total > kWide || a->k_total > kWide)
+    return set_error(VMB_ENOTSUP, "%s: at most %d rows with a window", what, kWide);
+  return VMB_OK;
+}
+
+vmb::PackedParams params(const vmb_packed_args* a, int32_t window, int32_t sinks) {
   vmb::PackedParams p{};
+  p.window = std::min(window, kWide);
+  p.sinks = std::min(sinks, kWide);
   p.heads = a->heads;
   p.kv_heads = a->kv_heads;
   p.group = a->heads / a->kv_heads;
@@ -114,15 +127,19 @@ int64_t vmb_packed_fwd_workspace_bytes(const vmb_packed_args* a) {
   return part_bytes(a->units.n_parts, a->heads, 256, a->dim) + part_bytes(a->units.n_parts, a->heads, 256, 0);
 }
 
-int vmb_packed_fwd(const vmb_packed_args* a, void* stream) {
-  int rc = check(a, "vmb_packed_fwd", false);
+}  // extern "C"
+
+namespace {
+
+int packed_fwd(const vmb_packed_args* a, int32_t window, int32_t sinks, const char* what, void* stream) {
+  int rc = check(a, what, false);
   if (rc) return rc;
   if (a->units.n_units == 0) return VMB_OK;
-  vmb::PackedParams p = params(a);
+  vmb::PackedParams p = params(a, window, sinks);
   p.units = reinterpret_cast<const vmb::PackedUnit*>(a->units.units);
   p.n_units = a->units.n_units;
   p.head_chunk = std::min(a->heads, p.group * head_chunk(4 * a->k_total * a->dim, a->kv_heads));
-  if ((rc = workspace(a, "vmb_packed_fwd", vmb_packed_fwd_workspace_bytes(a)))) return rc;
+  if ((rc = workspace(a, what, vmb_packed_fwd_workspace_bytes(a)))) return rc;
   if (a->units.n_parts > 0) {
     p.joins = a->units.joins;
     p.n_joins = a->units.n_joins;
@@ -130,7 +147,19 @@ int vmb_packed_fwd(const vmb_packed_args* a, void* stream) {
     p.part_ml = p.part + part_bytes(a->units.n_parts, a->heads, 256, a->dim) / 4;
   }
   vmb::count_launches(p.n_joins > 0 ? 2 : 1);
-  return cuda_rc(vmb::packed_fwd(p, a->dtype == VMB_DTYPE_BF16, static_cast<cudaStream_t>(stream)), "vmb_packed_fwd");
+  return cuda_rc(vmb::packed_fwd(p, a->dtype == VMB_DTYPE_BF16, static_cast<cudaStream_t>(stream)), what);
+}
+
+}  // namespace
+
+extern "C" {
+
+int vmb_packed_fwd(const vmb_packed_args* a, void* stream) { return packed_fwd(a, 0, 0, "vmb_packed_fwd", stream); }
+
+int vmb_packed_window_fwd(const vmb_packed_args* a, int32_t window, int32_t sinks, void* stream) {
+  const char* what = "vmb_packed_window_fwd";
+  const int rc = check_window(a, window, sinks, what);
+  return rc ? rc : packed_fwd(a, window, sinks, what, stream);
 }
 
 int64_t vmb_packed_bwd_workspace_bytes(const vmb_packed_args* a) {
@@ -139,12 +168,16 @@ int64_t vmb_packed_bwd_workspace_bytes(const vmb_packed_args* a) {
          part_bytes(a->kv_units.n_parts, 2 * a->kv_heads, 128, a->dim);
 }
 
-int vmb_packed_bwd(const vmb_packed_args* a, void* stream) {
-  int rc = check(a, "vmb_packed_bwd", true);
+}  // extern "C"
+
+namespace {
+
+int packed_bwd(const vmb_packed_args* a, int32_t window, int32_t sinks, const char* what, void* stream) {
+  int rc = check(a, what, true);
   if (rc) return rc;
   if (a->q_units.n_units == 0 && a->kv_units.n_units == 0) return VMB_OK;
-  if ((rc = workspace(a, "vmb_packed_bwd", vmb_packed_bwd_workspace_bytes(a)))) return rc;
-  vmb::PackedParams dq = params(a), kv = dq;
+  if ((rc = workspace(a, what, vmb_packed_bwd_workspace_bytes(a)))) return rc;
+  vmb::PackedParams dq = params(a, window, sinks), kv = dq;
   dq.stats = kv.stats = static_cast<float*>(a->workspace);
   dq.tile_scale = kv.tile_scale = dq.stats + plane_bytes(a) / 4;
   dq.centre = kv.centre = dq.tile_scale + tile_bytes(a) / 4;
@@ -161,8 +194,19 @@ int vmb_packed_bwd(const vmb_packed_args* a, void* stream) {
   kv.n_joins = a->kv_units.n_parts > 0 ? a->kv_units.n_joins : 0;
   kv.part = dq.part + part_bytes(a->q_units.n_parts, a->heads, 128, a->dim) / 4;
   vmb::count_launches((dq.n_units > 0 ? 2 : 0) + (kv.n_units > 0 ? 1 : 0) + (dq.n_joins > 0) + (kv.n_joins > 0));
-  return cuda_rc(vmb::packed_bwd(dq, kv, a->dtype == VMB_DTYPE_BF16, static_cast<cudaStream_t>(stream)),
-                 "vmb_packed_bwd");
+  return cuda_rc(vmb::packed_bwd(dq, kv, a->dtype == VMB_DTYPE_BF16, static_cast<cudaStream_t>(stream)), what);
+}
+
+}  // namespace
+
+extern "C" {
+
+int vmb_packed_bwd(const vmb_packed_args* a, void* stream) { return packed_bwd(a, 0, 0, "vmb_packed_bwd", stream); }
+
+int vmb_packed_window_bwd(const vmb_packed_args* a, int32_t window, int32_t sinks, void* stream) {
+  const char* what = "vmb_packed_window_bwd";
+  const int rc = check_window(a, window, sinks, what);
+  return rc ? rc : packed_bwd(a, window, sinks, what, stream);
 }
 
 }  // extern "C"

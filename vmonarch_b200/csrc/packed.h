@@ -20,8 +20,14 @@ namespace vmb {
 //                   from max(vis0, 0) / 64. stat_row: the sequence's first padded statistics row.
 //                   The sequence's queries below `lone` see one key at most.
 //  part           : -1, or the slot that a split unit's partial result goes to
+// With a window of W keys and S first keys that stay visible, local query r that sees the keys below `lim` without them
+// sees those of [lim - W, lim) and [0, S).
+//  forward and dQ : tiles [begin, end) are counted without the ones between the sinks and the window: tile x is
+//                   key tile x below lone, x + extra from there on
+//  dK / dV        : the first `extra` key rows are below S; the others are seen by W queries, so the tiles of a head
+//                   end where the unit's last key goes out of sight
 struct PackedUnit {
-  int32_t q_row, q_valid, k_row, k_valid, vis0, begin, end, part, stat_row, pieces, lone, pad;
+  int32_t q_row, q_valid, k_row, k_valid, vis0, begin, end, part, stat_row, pieces, lone, extra;
 };
 
 struct PackedParams {
@@ -30,6 +36,7 @@ struct PackedParams {
   int n_units, n_joins;
   int heads, kv_heads, group, head_chunk;  // head_chunk: (query or kv) heads whose units run together
   int dim, causal;
+  int window, sinks;       // window 0: none
   int64_t q_total, k_total, stat_rows;     // stat_rows: rows of the padded statistics planes
   float sm_scale;
   const void *q, *k, *v, *dout;
@@ -57,6 +64,20 @@ __host__ __device__ __forceinline__ UnitHead unit_of_block(int64_t block, int n_
   const int left = heads - c * chunk;
   const int g = left < chunk ? left : chunk;
   return UnitHead{rem / g, c * chunk + rem % g};
+}
+
+// Which keys a query sees below its limit `lim`, with a window and sinks.
+__device__ __forceinline__ int window_start(int lim, int window) { return max(lim - window, 0); }
+// Bit e: whether key k0 + e is seen, e < N (32 or 64): below lim, and from `lo` on or below `sinks`.
+__device__ __forceinline__ uint32_t bits_below32(int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; }
+__device__ __forceinline__ uint32_t seen32(int k0, int lo, int lim, int sinks) {
+  return bits_below32(lim - k0) & (~bits_below32(lo - k0) | bits_below32(sinks - k0));
+}
+// A unit's tile x as a key tile.
+__device__ __forceinline__ int key_tile(const PackedUnit& u, int x) { return x < u.lone ? x : x + u.extra; }
+// Whether every query of a unit sees all of the keys [k0, k0 + 128): `lim` of its first query, `lo` of its last.
+__device__ __forceinline__ bool sees_tile(int k0, int lo, int lim, int sinks) {
+  return lim - k0 >= 128 && (k0 >= lo || k0 + 128 <= sinks);
 }
 
 // 32 bytes to a 32-byte aligned global address (one sector, one store)

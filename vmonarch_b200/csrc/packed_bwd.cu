@@ -292,7 +292,7 @@ struct DkdvCfg {
   static_assert(SMEM <= 232448 - 1024, "shared memory budget");
 };
 
-template <typename T, int NA>
+template <typename T, int NA, bool WIN>
 __global__ void __launch_bounds__(kThreads, 1) packed_dkdv_kernel(const __grid_constant__ KParams p) {
   using C = DkdvCfg<NA>;
   constexpr int NQ = C::NQ;
@@ -356,7 +356,9 @@ __global__ void __launch_bounds__(kThreads, 1) packed_dkdv_kernel(const __grid_c
   const PackedUnit u = p.a.units[uh.unit];
   const int kvh = uh.head;
   const int t_first = max(u.vis0, 0) >> 6;
-  const int per_head = max(((u.q_valid + 63) >> 6) - t_first, 1);  // tiles of one query head
+  // queries from here on see no key of the unit
+  const int q_end = WIN && u.extra == 0 ? max(min(u.q_valid, u.vis0 + u.k_valid - 1 + p.a.window), 0) : u.q_valid;
+  const int per_head = max(((q_end + 63) >> 6) - t_first, 1);  // tiles of one query head
   const int n = u.end - u.begin;
   // step i -> query head and first local query of its tile
   auto step_head = [&](int i) { return kvh * p.a.group + (u.begin + i) / per_head; };
@@ -484,9 +486,11 @@ __global__ void __launch_bounds__(kThreads, 1) packed_dkdv_kernel(const __grid_c
       if (!warp_wait(BAR_S(stm), (i >> 1) & 1, 8) || !warp_wait(BAR_QFULL(s), (i / NQ) & 1, 8)) { ok = false; break; }
       tc_fence_after();
       const int q0 = step_q0(i), left = u.q_valid - q0;
-      // key `row` is seen by the tile's queries [c_lo, left)
-      const bool masked = left < 64 || u.vis0 + 127 > q0 || u.lone > q0;
-      const int c_lo = u.vis0 + row - q0 - 32 * half, c_hi = left - 32 * half;
+      // key `row` is seen by the tile's queries [c_lo, c_hi): up to its end, or for W of them if it is no sink
+      const bool masked = left < 64 || u.vis0 + 127 > q0 || u.lone > q0 ||
+                          (WIN && u.extra < 128 && u.vis0 + u.extra + p.a.window < q0 + 64);
+      const int c_lo = u.vis0 + row - q0 - 32 * half;
+      const int c_hi = (WIN && row >= u.extra ? min(left, u.vis0 + row + p.a.window - q0) : left) - 32 * half;
       if (left < 64) {
         // S^T is complete, and what dP^T still reads only goes into queries past the end: clear for dK and dV
         clear_rows(sQ(s), 2 * NA, 64, left, tid, 256);
@@ -593,7 +597,7 @@ struct DqCfg {
   static_assert(SMEM <= 232448 - 1024, "shared memory budget");
 };
 
-template <typename T, int NA>
+template <typename T, int NA, bool WIN>
 __global__ void __launch_bounds__(kThreads, 1) packed_dq_kernel(const __grid_constant__ KParams p) {
   using C = DqCfg<NA>;
   constexpr int NK = C::NK, NV = C::NV;
@@ -662,12 +666,14 @@ __global__ void __launch_bounds__(kThreads, 1) packed_dq_kernel(const __grid_con
         if (j >= nslot && !mbar_wait(BAR((kl ? B_KEMPTY : B_VEMPTY) + s), ((j / nslot) - 1) & 1, abort, &g_packed_bwd_err, 16, p.a.wait_limit))
           break;
         const uint32_t full = BAR((kl ? B_KFULL : B_VFULL) + s);
-        const int row = u.k_row + (u.begin + j) * 128;
+        const int row = u.k_row + (WIN ? key_tile(u, u.begin + j) : u.begin + j) * 128;
         mbar_expect_tx(full, TILE);
         for (int x = 0; x < NA; ++x)
           tma_load((kl ? sK : sV) + s * TILE + x * kAtom, map, 64 * x, row, BIdx(kvh, 0, 0), full);
-        if (j + nslot < n)
-          for (int x = 0; x < NA; ++x) tma_prefetch(map, 64 * x, row + nslot * 128, BIdx(kvh, 0, 0));
+        if (j + nslot < n) {
+          const int ahead = WIN ? u.k_row + key_tile(u, u.begin + j + nslot) * 128 : row + nslot * 128;
+          for (int x = 0; x < NA; ++x) tma_prefetch(map, 64 * x, ahead, BIdx(kvh, 0, 0));
+        }
         armed[s] = j / nslot + 1;
       }
       if (kl) mbar_wait_drain(BAR(B_Q), 0);
@@ -726,7 +732,10 @@ __global__ void __launch_bounds__(kThreads, 1) packed_dq_kernel(const __grid_con
     const int64_t plane = (int64_t)p.a.heads * p.a.stat_rows;
     const float row_scale = kBf16 ? 1.f : stat[2 * plane];
     const int my_lim = limit(row), lim_lo = limit(0);
-    const float ds_scale = my_lim > 1 ? row_scale : 0.f;  // a softmax over one key has no gradient
+    const int my_lo = WIN ? window_start(my_lim, p.a.window) : 0;
+    const int lo_hi = WIN ? window_start(limit(u.q_valid - 1), p.a.window) : 0;  // of the unit's last query
+    // a softmax over one key has no gradient
+    const float ds_scale = my_lim > 1 && (!WIN || p.a.window + p.a.sinks > 1) ? row_scale : 0.f;
     const float fl = stat[0], fc = stat[plane] * ds_scale, fs = p.a.sm_scale * ds_scale;
     const float2 nl2 = make_float2(fl, fl), nc2 = make_float2(fc, fc);
     const float2 sc2 = make_float2(p.scale_log2, p.scale_log2), sm2 = make_float2(fs, fs);
@@ -739,7 +748,7 @@ __global__ void __launch_bounds__(kThreads, 1) packed_dq_kernel(const __grid_con
     for (int j = 0; j < n; ++j) {
       if (!warp_wait(B_S + (j & 1), (j >> 1) & 1, 64) || !warp_wait(B_DP, j & 1, 64)) { ok = false; break; }
       tc_fence_after();
-      const int k0 = (u.begin + j) * 128;
+      const int k0 = (WIN ? key_tile(u, u.begin + j) : u.begin + j) * 128;
       const uint32_t ts = tmem + lane_off + 128u * (uint32_t)(j & 1) + 32 * wg;
       uint32_t sv[32], dv[32], pk[16];
       tmem_ld32(ts, sv);
@@ -751,15 +760,16 @@ __global__ void __launch_bounds__(kThreads, 1) packed_dq_kernel(const __grid_con
         clear_rows(sK + (j % NK) * TILE, NA, 128, u.k_valid - k0, tid, 512);
         fence_proxy_async_smem();
       }
-      const bool masked = lim_lo - k0 < 128;
+      const bool masked = WIN ? !sees_tile(k0, lo_hi, lim_lo, p.a.sinks) : lim_lo - k0 < 128;
       const int valid = my_lim - k0 - 32 * wg;
+      const uint32_t seen = WIN ? seen32(k0 + 32 * wg, my_lo, my_lim, p.a.sinks) : 0u;
       auto scores = [&](auto mask) {
 #pragma unroll
         for (int e = 0; e < 32; e += 2) {
           float2 d = dscore2(prob2(sv[e], sv[e + 1], sc2, nl2), dv[e], dv[e + 1], sm2, nc2);
           if (mask) {
-            if (e >= valid) d.x = 0.f;
-            if (e + 1 >= valid) d.y = 0.f;
+            if (WIN ? !((seen >> e) & 1u) : e >= valid) d.x = 0.f;
+            if (WIN ? !((seen >> (e + 1)) & 1u) : e + 1 >= valid) d.y = 0.f;
           }
           pk[e >> 1] = Elem<T>::pack(d.x, d.y);
         }
@@ -811,7 +821,7 @@ cudaError_t run(Kern kern, int smem, std::atomic<uint64_t>& ready, int64_t block
   return launch_early(kern, blocks, kThreads, smem, st, p);
 }
 
-template <typename T, int NA>
+template <typename T, int NA, bool WIN>
 cudaError_t launch(const PackedParams& dq, const PackedParams& kv, cudaStream_t st) {
   constexpr bool bf16 = Elem<T>::is_bf16;
   if (dq.n_units > 0) {
@@ -831,7 +841,7 @@ cudaError_t launch(const PackedParams& dq, const PackedParams& kv, cudaStream_t 
     if (!map(&p.tm_q, kv.q, kv.q_total, kv.heads, kv.qv, 64) || !map(&p.tm_do, kv.dout, kv.q_total, kv.heads, kv.dov, 64))
       return cudaErrorInvalidValue;
     p.a = kv;
-    cudaError_t e = run(packed_dkdv_kernel<T, NA>, DkdvCfg<NA>::SMEM, ready_kv, (int64_t)kv.n_units * kv.kv_heads, p, st);
+    cudaError_t e = run(packed_dkdv_kernel<T, NA, WIN>, DkdvCfg<NA>::SMEM, ready_kv, (int64_t)kv.n_units * kv.kv_heads, p, st);
     if (e != cudaSuccess) return e;
     if (kv.n_joins > 0 &&
         (e = launch_early(packed_sum_kernel<T, NA, true>, (int64_t)kv.n_joins * kv.kv_heads * 8, 256, 0, st, kv)) != cudaSuccess)
@@ -841,7 +851,7 @@ cudaError_t launch(const PackedParams& dq, const PackedParams& kv, cudaStream_t 
     if (!map(&p.tm_q, dq.q, dq.q_total, dq.heads, dq.qv, 128) || !map(&p.tm_do, dq.dout, dq.q_total, dq.heads, dq.dov, 128))
       return cudaErrorInvalidValue;
     p.a = dq;
-    cudaError_t e = run(packed_dq_kernel<T, NA>, DqCfg<NA>::SMEM, ready_q, (int64_t)dq.n_units * dq.heads, p, st);
+    cudaError_t e = run(packed_dq_kernel<T, NA, WIN>, DqCfg<NA>::SMEM, ready_q, (int64_t)dq.n_units * dq.heads, p, st);
     if (e != cudaSuccess) return e;
     if (dq.n_joins > 0) return launch_early(packed_sum_kernel<T, NA, false>, (int64_t)dq.n_joins * dq.heads * 4, 256, 0, st, dq);
   }
@@ -851,8 +861,12 @@ cudaError_t launch(const PackedParams& dq, const PackedParams& kv, cudaStream_t 
 }  // namespace
 
 cudaError_t packed_bwd(const PackedParams& dq, const PackedParams& kv, bool bf16, cudaStream_t st) {
-  if (dq.dim > 64) return bf16 ? launch<__nv_bfloat16, 2>(dq, kv, st) : launch<__half, 2>(dq, kv, st);
-  return bf16 ? launch<__nv_bfloat16, 1>(dq, kv, st) : launch<__half, 1>(dq, kv, st);
+  auto run = [&](auto win) {
+    constexpr bool WIN = decltype(win)::value;
+    if (dq.dim > 64) return bf16 ? launch<__nv_bfloat16, 2, WIN>(dq, kv, st) : launch<__half, 2, WIN>(dq, kv, st);
+    return bf16 ? launch<__nv_bfloat16, 1, WIN>(dq, kv, st) : launch<__half, 1, WIN>(dq, kv, st);
+  };
+  return dq.window ? run(std::true_type{}) : run(std::false_type{});
 }
 
 cudaError_t packed_bwd_status(cudaStream_t st, int* out) {

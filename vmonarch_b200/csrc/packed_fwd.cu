@@ -3,8 +3,8 @@
 //
 //   o_i = sum_j p_ij v_j / sum_j p_ij,  p_ij = exp(s_ij - m_i),  s_ij = sm_scale q_i . k_j,
 // over the keys j of query i's own sequence that it sees: all of them, or with `causal` the first
-// nk - nq + i + 1 (the last query sees the last key). A query that sees no key has o = 0 and
-// lse = -inf.
+// nk - nq + i + 1 (the last query sees the last key), and of these with a window the last `window` and the first `sinks`
+// (WIN). A query that sees no key has o = 0 and lse = -inf.
 //
 // Work item = one head and one unit of up to 256 queries (two 128-row tiles, one per softmax warpgroup) of
 // one sequence, or a piece of its key tiles. 10 warps: TMA producers, MMA issuer, two warpgroups of softmax and
@@ -119,6 +119,32 @@ __device__ __forceinline__ float probs(const uint32_t (&sr)[N], uint32_t (&pk)[N
   return (la[0].x + la[0].y) + (la[1].x + la[1].y);
 }
 
+// The same by a mask: bit e of `seen` says whether key e counts.
+__device__ __forceinline__ float row_max_bits(const uint32_t (&sr)[32], uint32_t seen) {
+  auto at = [&](int i) { return (seen >> i) & 1u ? __uint_as_float(sr[i]) : -1e30f; };
+  float mr[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) mr[k] = fmax3(at(3 * k), at(3 * k + 1), at(3 * k + 2));
+#pragma unroll
+  for (int i = 12; i < 32; i += 2) mr[(i >> 1) & 3] = fmax3(mr[(i >> 1) & 3], at(i), at(i + 1));
+  return fmax3(fmaxf(mr[0], mr[1]), mr[2], mr[3]);
+}
+template <typename T>
+__device__ __forceinline__ float probs_bits(const uint32_t (&sr)[32], uint32_t (&pk)[16], float sc, float m, uint32_t seen) {
+  float2 la[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+  const float2 sc2 = make_float2(sc, sc), nm2 = make_float2(-m, -m);
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    float2 d = __ffma2_rn(make_float2(__uint_as_float(sr[2 * i]), __uint_as_float(sr[2 * i + 1])), sc2, nm2);
+    if (!((seen >> (2 * i)) & 1u)) d.x = -1e30f;
+    if (!((seen >> (2 * i + 1)) & 1u)) d.y = -1e30f;
+    const float2 pp = make_float2(fast_exp2(d.x), fast_exp2(d.y));
+    la[i & 1] = __fadd2_rn(la[i & 1], pp);
+    pk[i] = Elem<T>::pack(pp.x, pp.y);
+  }
+  return (la[0].x + la[0].y) + (la[1].x + la[1].y);
+}
+
 // x * 0 + acc over a pair: NaN once either half was an infinity or NaN.
 template <typename T>
 __device__ __forceinline__ uint32_t zero_fma2(uint32_t x, uint32_t acc) {
@@ -179,6 +205,7 @@ struct Item {
   int causal;
   // keys that local query r sees
   __device__ __forceinline__ int limit(int r) const { return max(0, min(u.k_valid, causal ? u.vis0 + r : u.k_valid)); }
+  template <bool WIN>
   __device__ __forceinline__ void set(const PackedParams& a, const PackedUnit& unit, int h) {
     u = unit;
     head = h;
@@ -189,14 +216,17 @@ struct Item {
     for (int w = 0; w < 2; ++w) {  // tiles that stream w's last query sees
       const int rows = min(u.q_valid - 128 * w, 128);
       const int last = rows > 0 ? limit(128 * w + rows - 1) : 0;
-      n_kt[w] = max(0, min((last + 127) >> 7, u.end) - u.begin);
-      if (last - (u.begin + n_kt[w] - 1) * 128 <= 32) brief |= 1 << w;
+      int to = (last + 127) >> 7;
+      if (WIN && to > u.lone) to = max(to - u.extra, u.lone);
+      n_kt[w] = max(0, min(to, u.end) - u.begin);
+      const int end = u.begin + n_kt[w] - 1;
+      if (last - (WIN ? key_tile(u, end) : end) * 128 <= 32) brief |= 1 << w;
     }
     n_max = max(n_kt[0], n_kt[1]);
   }
 };
 
-template <typename T, int NA>
+template <typename T, int NA, bool WIN>
 __global__ void __launch_bounds__(kThreads, 1) packed_fwd_kernel(const __grid_constant__ KParams p) {
   using C = Cfg<NA>;
   constexpr int NK = C::NK, NV = C::NV;
@@ -273,7 +303,7 @@ __global__ void __launch_bounds__(kThreads, 1) packed_fwd_kernel(const __grid_co
           it.head = -1;
           if (block >= 0) {
             const UnitHead uh = unit_of_block(block, p.a.n_units, p.a.heads, p.a.head_chunk);
-            it.set(p.a, p.a.units[uh.unit], uh.head);
+            it.set<WIN>(p.a, p.a.units[uh.unit], uh.head);
           }
           if (i >= 2 && !(ok = mbar_wait(BAR(B_WFREE + (i & 1)), ((i - 2) >> 1) & 1, abort, &g_packed_err, 1))) break;
           work_sh[i & 1] = it;
@@ -308,11 +338,13 @@ __global__ void __launch_bounds__(kThreads, 1) packed_fwd_kernel(const __grid_co
             break;
           }
           const uint32_t full = BAR((kl ? B_KFULL : B_VFULL) + s), slot = (kl ? sK : sV) + s * TILE;
-          const int row = it.u.k_row + (it.u.begin + t) * 128;
+          const int row = it.u.k_row + (WIN ? key_tile(it.u, it.u.begin + t) : it.u.begin + t) * 128;
           mbar_expect_tx(full, TILE);
           for (int a = 0; a < NA; ++a) tma_load(slot + a * kAtom, map, 64 * a, row, BIdx(it.kvh, 0, 0), full);
-          if (t + nslot < it.n_max)  // the tile one ring ahead into L2
-            for (int a = 0; a < NA; ++a) tma_prefetch(map, 64 * a, row + nslot * 128, BIdx(it.kvh, 0, 0));
+          if (t + nslot < it.n_max) {  // the tile one ring ahead into L2
+            const int ahead = WIN ? it.u.k_row + key_tile(it.u, it.u.begin + t + nslot) * 128 : row + nslot * 128;
+            for (int a = 0; a < NA; ++a) tma_prefetch(map, 64 * a, ahead, BIdx(it.kvh, 0, 0));
+          }
         }
         if (!ok) break;
         if (kl) {
@@ -430,7 +462,7 @@ __global__ void __launch_bounds__(kThreads, 1) packed_fwd_kernel(const __grid_co
       if (!(ok = __all_sync(0xffffffffu, work_wait(i, 8)))) break;
       if (work_sh[i & 1].head < 0) break;
       // what the loop over the tiles needs; the epilogue reads the rest again (the loop wants the registers)
-      int n_kt, begin, my_lim, lim_lo;
+      int n_kt, begin, my_lim, lim_lo, my_lo = 0, lo_hi = 0;
       bool live;
       {
         const Item& it = work_sh[i & 1];
@@ -440,6 +472,10 @@ __global__ void __launch_bounds__(kThreads, 1) packed_fwd_kernel(const __grid_co
         live = 128 * w + row < it.u.q_valid;
         my_lim = it.limit(min(128 * w + row, it.u.q_valid - 1));
         lim_lo = it.limit(0);  // of the unit's first query, for both streams
+        if (WIN) {
+          my_lo = window_start(my_lim, p.a.window);
+          lo_hi = window_start(it.limit(it.u.q_valid - 1), p.a.window);  // of the unit's last query
+        }
       }
       float m_ref = -1e30f, l = 0.f;
       // O and l to the reference max(m_ref, mx). Warp-uniform; no P V into O_w may be in flight.
@@ -468,12 +504,13 @@ __global__ void __launch_bounds__(kThreads, 1) packed_fwd_kernel(const __grid_co
           mbar_arrive(BAR(B_KFREE + (ring + t) % NK));
           if (t >= 1) mbar_arrive(BAR(B_VFREE + (ring + t - 1) % NV));
         }
-        const int k0 = (begin + t) * 128;
+        const int k0 = (WIN ? key_tile(work_sh[i & 1].u, begin + t) : begin + t) * 128;
+        const bool whole = WIN ? sees_tile(k0, lo_hi, lim_lo, p.a.sinks) : lim_lo - k0 >= 128;
         // Two 64-key halves; a half's P lets its P V start. The exponentials go against the current reference (the
         // unit's first half sets it); a half past the threshold is redone from the scores in registers, once
         // no P V into O is under way: S_w(t) complete implies that every earlier one is done, and in the second
         // half the first half's is waited for.
-        if (t > 0 && lim_lo - k0 >= 128) {  // no query of the unit misses a key of the tile
+        if (t > 0 && whole) {  // no query of the unit misses a key of the tile
 #pragma unroll
           for (int hf = 0; hf < 2; ++hf) {
             uint32_t s[64], pk[32];
@@ -496,7 +533,7 @@ __global__ void __launch_bounds__(kThreads, 1) packed_fwd_kernel(const __grid_co
             }
           }
         } else {
-          if (lim_lo - k0 < 128) {
+          if (!whole) {
             // Values that some query of the unit must not see: clear what is not finite (thread = key row). Both streams
             // look, also the one whose queries see the whole tile: the other's clearing may come before its product or
             // after, and the epilogue adds back what was cleared in the tiles from here on.
@@ -506,45 +543,86 @@ __global__ void __launch_bounds__(kThreads, 1) packed_fwd_kernel(const __grid_co
           }
 #pragma unroll 1
           for (int hf = 0; hf < 2; ++hf) {
-            const int seen = my_lim - k0 - 64 * hf;               // keys of the half that this query sees,
-            const int least = __shfl_sync(0xffffffffu, seen, 0);  // the warp's first query (limits only grow)
-            const int most = __shfl_sync(0xffffffffu, seen, 31);  // and its last
             uint32_t pk[32];
-            if (most <= 0) {
+            if constexpr (WIN) {
+              // which of the half's keys this query sees, 32 keys at a time: a warp computes only those that one of its
+              // queries sees
+              const int kh = k0 + 64 * hf;
+              const uint32_t seen0 = seen32(kh, my_lo, my_lim, p.a.sinks), seen1 = seen32(kh + 32, my_lo, my_lim, p.a.sinks);
+              const bool any0 = __any_sync(0xffffffffu, seen0 != 0), any1 = __any_sync(0xffffffffu, seen1 != 0);
+              const bool all = __all_sync(0xffffffffu, (seen0 & seen1) == 0xffffffffu);
 #pragma unroll
               for (int e = 0; e < 32; ++e) pk[e] = 0u;
-            } else {
-              uint32_t s[64];
-              tmem_ld32(tS + 64 * hf, s);
-              tmem_ld32(tS + 64 * hf + 32, s + 32);
-              tmem_wait_ld();
-              if (hf == 0 && t == 0) m_ref = (least >= 64 ? row_max<64, false>(s, 64) : row_max<64, true>(s, seen)) * p.scale_log2;
-              float lt = 0.f;
+              if (any0 || any1) {
+                uint32_t s[64];
+                tmem_ld32(tS + 64 * hf, s);
+                tmem_ld32(tS + 64 * hf + 32, s + 32);
+                tmem_wait_ld();
+                const uint32_t(&s0)[32] = *reinterpret_cast<const uint32_t(*)[32]>(&s[0]);
+                const uint32_t(&s1)[32] = *reinterpret_cast<const uint32_t(*)[32]>(&s[32]);
+                uint32_t(&p0)[16] = *reinterpret_cast<uint32_t(*)[16]>(&pk[0]);
+                uint32_t(&p1)[16] = *reinterpret_cast<uint32_t(*)[16]>(&pk[16]);
+                auto top = [&]() { return fmaxf(row_max_bits(s0, seen0), row_max_bits(s1, seen1)) * p.scale_log2; };
+                // (a query that sees none of these keys keeps the reference of no key)
+                if (hf == 0 && t == 0) m_ref = fmaxf(m_ref, all ? row_max<64, false>(s, 64) * p.scale_log2 : top());
+                float lt = 0.f;
 #pragma unroll 1
-              for (int pass = 0; pass < 2; ++pass) {
-                if (least >= 64) {
-                  lt = probs<T, 64, false>(s, pk, p.scale_log2, m_ref, 64);
-                } else {
-                  // masked, 32 keys at a time: a warp computes only those that one of its queries sees
-                  const uint32_t(&s0)[32] = *reinterpret_cast<const uint32_t(*)[32]>(&s[0]);
-                  const uint32_t(&s1)[32] = *reinterpret_cast<const uint32_t(*)[32]>(&s[32]);
-                  uint32_t(&p0)[16] = *reinterpret_cast<uint32_t(*)[16]>(&pk[0]);
-                  uint32_t(&p1)[16] = *reinterpret_cast<uint32_t(*)[16]>(&pk[16]);
-                  lt = probs<T, 32, true>(s0, p0, p.scale_log2, m_ref, seen);
-                  if (most > 32) {
-                    lt += probs<T, 32, true>(s1, p1, p.scale_log2, m_ref, seen - 32);
+                for (int pass = 0; pass < 2; ++pass) {
+                  if (all) {
+                    lt = probs<T, 64, false>(s, pk, p.scale_log2, m_ref, 64);
                   } else {
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) p1[e] = 0u;
+                    lt = 0.f;
+                    if (any0) lt = probs_bits<T>(s0, p0, p.scale_log2, m_ref, seen0);
+                    if (any1) lt += probs_bits<T>(s1, p1, p.scale_log2, m_ref, seen1);
                   }
+                  if (pass || !__any_sync(0xffffffffu, live && !(lt <= kSumThreshold))) break;
+                  if (hf == 1 && !(ok = warp_wait(B_PVH + w, steps & 1, 16))) break;
+                  tc_fence_after();
+                  rescale(top());
                 }
-                if (pass || !__any_sync(0xffffffffu, live && !(lt <= kSumThreshold))) break;
-                if (hf == 1 && !(ok = warp_wait(B_PVH + w, steps & 1, 16))) break;
-                tc_fence_after();
-                rescale(row_max<64, true>(s, seen) * p.scale_log2);
+                if (!ok) break;
+                l += lt;
               }
-              if (!ok) break;
-              l += lt;
+            } else {
+              const int seen = my_lim - k0 - 64 * hf;               // keys of the half that this query sees,
+              const int least = __shfl_sync(0xffffffffu, seen, 0);  // the warp's first query (limits only grow)
+              const int most = __shfl_sync(0xffffffffu, seen, 31);  // and its last
+              if (most <= 0) {
+  #pragma unroll
+                for (int e = 0; e < 32; ++e) pk[e] = 0u;
+              } else {
+                uint32_t s[64];
+                tmem_ld32(tS + 64 * hf, s);
+                tmem_ld32(tS + 64 * hf + 32, s + 32);
+                tmem_wait_ld();
+                if (hf == 0 && t == 0) m_ref = (least >= 64 ? row_max<64, false>(s, 64) : row_max<64, true>(s, seen)) * p.scale_log2;
+                float lt = 0.f;
+  #pragma unroll 1
+                for (int pass = 0; pass < 2; ++pass) {
+                  if (least >= 64) {
+                    lt = probs<T, 64, false>(s, pk, p.scale_log2, m_ref, 64);
+                  } else {
+                    // masked, 32 keys at a time: a warp computes only those that one of its queries sees
+                    const uint32_t(&s0)[32] = *reinterpret_cast<const uint32_t(*)[32]>(&s[0]);
+                    const uint32_t(&s1)[32] = *reinterpret_cast<const uint32_t(*)[32]>(&s[32]);
+                    uint32_t(&p0)[16] = *reinterpret_cast<uint32_t(*)[16]>(&pk[0]);
+                    uint32_t(&p1)[16] = *reinterpret_cast<uint32_t(*)[16]>(&pk[16]);
+                    lt = probs<T, 32, true>(s0, p0, p.scale_log2, m_ref, seen);
+                    if (most > 32) {
+                      lt += probs<T, 32, true>(s1, p1, p.scale_log2, m_ref, seen - 32);
+                    } else {
+  #pragma unroll
+                      for (int e = 0; e < 16; ++e) p1[e] = 0u;
+                    }
+                  }
+                  if (pass || !__any_sync(0xffffffffu, live && !(lt <= kSumThreshold))) break;
+                  if (hf == 1 && !(ok = warp_wait(B_PVH + w, steps & 1, 16))) break;
+                  tc_fence_after();
+                  rescale(row_max<64, true>(s, seen) * p.scale_log2);
+                }
+                if (!ok) break;
+                l += lt;
+              }
             }
             tmem_st32(tS + 32 * hf, pk);
             if (hf == 0) {
@@ -610,14 +688,27 @@ __global__ void __launch_bounds__(kThreads, 1) packed_fwd_kernel(const __grid_co
         if (dirty && n_kt > 0) {
           // values of the masked tiles that were cleared: back to the queries that see them
           const T* v = static_cast<const T*>(p.a.v) + (int64_t)u.k_row * p.a.vv.rs + (int64_t)it.kvh * p.a.vv.s1;
-          const int j0 = max(it.limit(0) & ~127, u.begin * 128), j1 = min(my_lim, u.end * 128);
-#pragma unroll 1
-          for (int j = j0; j < j1; ++j)
+          auto add_back = [&](int j) {
 #pragma unroll
             for (int e = 0; e < 32; ++e) {
               const float x = c * 32 + e < p.a.dim ? Elem<T>::to_f(v[(int64_t)j * p.a.vv.rs + c * 32 + e]) : 0.f;
               if (!isfinite(x)) o[e] = __float_as_uint(__uint_as_float(o[e]) + x);
             }
+          };
+          if constexpr (WIN) {
+#pragma unroll 1
+            for (int t = 0; t < n_kt; ++t) {
+              const int k0 = key_tile(u, u.begin + t) * 128;
+              if (sees_tile(k0, lo_hi, lim_lo, p.a.sinks)) continue;
+#pragma unroll 1
+              for (int j = k0; j < min(k0 + 128, my_lim); ++j)
+                if (j >= my_lo || j < p.a.sinks) add_back(j);
+            }
+          } else {
+            const int j0 = max(it.limit(0) & ~127, u.begin * 128), j1 = min(my_lim, u.end * 128);
+#pragma unroll 1
+            for (int j = j0; j < j1; ++j) add_back(j);
+          }
         }
         if (u.part >= 0) {
           float* to = p.a.part + prow * (64 * NA) + c * 32;
@@ -713,9 +804,9 @@ __global__ void __launch_bounds__(256) packed_fwd_join_kernel(const __grid_const
     a.lse[(int64_t)head * a.q_total + grow] = l == 0.f ? __int_as_float(0xff800000) : (m + log2f(l)) * kLn2;
 }
 
-template <typename T, int NA>
+template <typename T, int NA, bool WIN>
 cudaError_t launch(const KParams& p, cudaStream_t st) {
-  auto kern = packed_fwd_kernel<T, NA>;
+  auto kern = packed_fwd_kernel<T, NA, WIN>;
   static std::atomic<uint64_t> ready{0};
   cudaError_t e = allow_smem(kern, Cfg<NA>::SMEM, ready);
   if (e != cudaSuccess) return e;
@@ -726,7 +817,8 @@ cudaError_t launch(const KParams& p, cudaStream_t st) {
 
 template <typename T>
 cudaError_t launch_dim(const KParams& p, cudaStream_t st) {
-  return p.a.dim > 64 ? launch<T, 2>(p, st) : launch<T, 1>(p, st);
+  if (p.a.window) return p.a.dim > 64 ? launch<T, 2, true>(p, st) : launch<T, 1, true>(p, st);
+  return p.a.dim > 64 ? launch<T, 2, false>(p, st) : launch<T, 1, false>(p, st);
 }
 
 }  // namespace

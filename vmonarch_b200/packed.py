@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import heapq
+import operator
 import struct
 import threading
 
@@ -23,6 +24,8 @@ MAX_DIM = 128
 _FWD_ROWS, _DQ_ROWS, _KV_ROWS, _STEP = 256, 128, 128, 64
 _FIELDS = 12  # int32 per vmb_packed_unit
 _NEVER_MASKED = -(1 << 30)
+# most rows that a call with a window takes; windows and sinks above it are alike
+_WIDE = (1 << 30) - 1024
 _SMS = 148
 # least steps of a piece when a unit is cut: below it, set-up and join cost more than the cut gains
 _LEAST = {"fwd": 8, "dq": 8, "kv": 16}
@@ -128,7 +131,7 @@ class PackedSequences:
             prompt behind a cached prefix); default: `lengths`.
         device: where the tensors of the sequences live.
 
-    The object holds device copies of its work lists, made at the first call of each kind (direction, causal, head
+    The object holds device copies of its work lists, made at the first call of each kind (direction, mask, head
     counts), which waits for the copy; keep it for as long as the lengths stand, e.g. for all layers of a step. It may
     be used on any stream and by several threads. A captured graph reads the lists where they are: make one call of
     each kind before the capture, and keep the object for as long as the graph.
@@ -195,6 +198,7 @@ class PackedSequences:
         return starts
 
     # ------------------------------------------------------------------------------ work lists
+    # `causal`: False, True, or with a window the pair (window, sinks)
     def _query_units(self, rows, causal):
         """Units of `rows` queries for the forward and dQ kernels, and their key tiles."""
         seq, first = _tiles(self.q_lens, rows)
@@ -208,6 +212,15 @@ class PackedSequences:
         u[:, 6] = -(-seen // 128)
         u[:, 7] = -1
         u[:, 8] = self.stat_start[seq] + first
+        if isinstance(causal, tuple):
+            window, sinks = causal
+            # tiles of the sinks, then those from the first query's window on; the ones between are not counted
+            sink_tiles = -(-np.minimum(sinks, seen) // 128)
+            begin = np.maximum(np.clip(vis0, 0, nk) - window, 0) // 128
+            gap = begin > sink_tiles
+            u[:, 10] = np.where(gap, sink_tiles, 0)
+            u[:, 11] = np.where(gap, begin - sink_tiles, 0)
+            u[:, 6] -= u[:, 11]
         return u
 
     def _key_units(self, causal, group):
@@ -219,11 +232,18 @@ class PackedSequences:
         u[:, 0], u[:, 1] = self.q_start[seq], nq
         u[:, 2], u[:, 3] = self.k_start[seq] + first, np.minimum(nk - first, _KV_ROWS)
         u[:, 4] = vis0
-        u[:, 6] = group * np.maximum(-(-nq // _STEP) - np.maximum(vis0, 0) // _STEP, 0)
+        end = nq  # of the queries that see one of the keys
+        if isinstance(causal, tuple):
+            window, sinks = causal
+            u[:, 11] = np.clip(sinks - first, 0, u[:, 3])
+            end = np.where(u[:, 11] > 0, nq, np.clip(vis0 + u[:, 3] - 1 + window, 0, nq))
+        u[:, 6] = group * np.maximum(-(-end // _STEP) - np.maximum(vis0, 0) // _STEP, 0)
         u[:, 7] = -1
         u[:, 8] = self.stat_start[seq]
         # queries below this one see one key at most, and a softmax over one key has no gradient
         u[:, 10] = np.maximum(nq - nk + 1, 0) if causal else np.where(nk == 1, nq, 0)
+        if causal == (1, 0):
+            u[:, 10] = nq
         return u
 
     def _list(self, *key):
@@ -256,7 +276,7 @@ class PackedSequences:
         a = N.PackedArgs()
         a.q_total, a.k_total, a.stat_rows = self.total_q, self.total_k, self.stat_rows
         a.heads, a.kv_heads, a.dim = heads, kv_heads, dim
-        a.dtype, a.causal, a.sm_scale = N.dtype_code(dtype), causal, sm_scale
+        a.dtype, a.causal, a.sm_scale = N.dtype_code(dtype), bool(causal), sm_scale
         lists = [(kind, causal, heads, heads // kv_heads) for kind in (("dq", "kv") if backward else ("fwd",))]
         if backward:
             a.q_units, a.kv_units = (self._list(*x) for x in lists)
@@ -311,7 +331,10 @@ def _forward(q, k, v, seqs, key, device, lse=None, aux=None):
     if size:
         ws = torch.empty(size, dtype=torch.uint8, device=device)
         _WORKSPACE.pack_into(a, _WORKSPACE_AT, ws.data_ptr(), size)
-    N.launch("vmb_packed_fwd", N.lib.vmb_packed_fwd, device, ctypes.byref(a))
+    if type(key[1]) is tuple:
+        N.launch("vmb_packed_window_fwd", N.lib.vmb_packed_window_fwd, device, ctypes.byref(a), *key[1])
+    else:
+        N.launch("vmb_packed_fwd", N.lib.vmb_packed_fwd, device, ctypes.byref(a))
     return q, k, v, o
 
 
@@ -353,11 +376,24 @@ class _PackedAttention(torch.autograd.Function):
         if size:
             ws = torch.empty(size, dtype=torch.uint8, device=device)
             _WORKSPACE.pack_into(a, _WORKSPACE_AT, ws.data_ptr(), size)
-        N.launch("vmb_packed_bwd", N.lib.vmb_packed_bwd, device, ctypes.byref(a))
+        if type(key[1]) is tuple:
+            N.launch("vmb_packed_window_bwd", N.lib.vmb_packed_window_bwd, device, ctypes.byref(a), *key[1])
+        else:
+            N.launch("vmb_packed_bwd", N.lib.vmb_packed_bwd, device, ctypes.byref(a))
         return dq, dk, dv, None, None, None
 
 
-def packed_attention(q, k, v, seqs, *, causal=False, sm_scale=None, return_lse=False):
+def _window(window, sinks):
+    """(window, sinks) as the kernels take them, None without a window."""
+    if window is None:
+        assert sinks == 0, "sinks need a window"
+        return None
+    window, sinks = operator.index(window), operator.index(sinks)
+    assert window >= 1 and sinks >= 0, "window must be at least 1 and sinks not negative"
+    return min(window, _WIDE), min(sinks, _WIDE)
+
+
+def packed_attention(q, k, v, seqs, *, causal=False, window=None, sinks=0, sm_scale=None, return_lse=False):
     """
     Softmax attention over packed sequences, differentiable in q, k and v (backward only).
 
@@ -366,6 +402,8 @@ def packed_attention(q, k, v, seqs, *, causal=False, sm_scale=None, return_lse=F
         k, v: (total_k, Hk, D), the same dtype, H a multiple of Hk
         seqs: the sequences' lengths, a :class:`PackedSequences` on the same device
         causal: query i of a sequence of nq queries and nk keys sees its first nk - nq + i + 1 keys
+        window: of these only the last `window` (at least 1; None: all), and the sequence's first `sinks`, which stay
+            visible; causal only. The work grows with the window, not with the length.
         sm_scale: softmax scale, not negative; defaults to 1 / sqrt(D)
         return_lse: also return the log of each softmax's sum
     Returns:
@@ -381,6 +419,10 @@ def packed_attention(q, k, v, seqs, *, causal=False, sm_scale=None, return_lse=F
     dtype = q.dtype
     assert dtype in SUPPORTED_DTYPES, f"unsupported dtype {dtype}"
     assert k.dtype == dtype and v.dtype == dtype, "q, k and v must share a dtype"
+    mask = _window(window, sinks) or bool(causal)
+    if window is not None:
+        assert causal, "a window needs causal=True"
+        assert q.size(0) <= _WIDE and k.size(0) <= _WIDE, f"at most {_WIDE} rows with a window"
     assert q.dim() == 3 and k.dim() == 3 and v.shape == k.shape and q.size(2) == k.size(2), \
         "q must be (total_q, H, D), k and v (total_k, Hk, D)"
     rows, heads, d = q.shape
@@ -394,7 +436,7 @@ def packed_attention(q, k, v, seqs, *, causal=False, sm_scale=None, return_lse=F
         f"q and k have {rows} and {kv_rows} rows, the sequences {seqs.total_q} and {seqs.total_k}"
     sm_scale = d ** -0.5 if sm_scale is None else float(sm_scale)
     assert 0 <= sm_scale < float("inf"), "sm_scale must be finite and not negative"
-    key = (False, bool(causal), sm_scale, dtype, heads, kv_heads, d)
+    key = (False, mask, sm_scale, dtype, heads, kv_heads, d)
     if N.derived(q.requires_grad or k.requires_grad or v.requires_grad):
         return _PackedAttention.apply(q, k, v, seqs, key, return_lse)
     lse = torch.empty((heads, rows), dtype=torch.float32, device=device) if return_lse else None
