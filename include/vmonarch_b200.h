@@ -383,6 +383,23 @@ typedef struct vmb_paged_args {
 int64_t vmb_paged_workspace_bytes(const vmb_paged_args* a);  /* -1: malformed sizes */
 int vmb_paged_attention(const vmb_paged_args* a, void* stream);
 
+/* One value per page and key head, device: value x scale[page * s.page + head * s.head]. */
+typedef struct vmb_page_scales {
+  float* ptr;
+  int64_t page, head;
+} vmb_page_scales;
+
+/* The same over other caches: with a window a sequence's new token sees the last `window` >= 1 of its tokens and the first
+ * `sinks` >= 0 (window 0: all, sinks 0), and table entries of pages without a token that it sees are not read. With
+ * k_scale.ptr and v_scale.ptr the pools hold e4m3 values (one byte an element; dim and strides multiples of 16) with a scale
+ * for each page and head, not negative; q and o stay of type dtype. NULL, both of them: 16-bit pools. */
+typedef struct vmb_cache_args {
+  vmb_page_scales k_scale, v_scale;
+  int32_t window, sinks;
+} vmb_cache_args;
+int64_t vmb_cache_workspace_bytes(const vmb_paged_args* a, const vmb_cache_args* c);  /* -1: malformed sizes */
+int vmb_cache_attention(const vmb_paged_args* a, const vmb_cache_args* c, void* stream);
+
 /* Row i of k_new, v_new [count][kv_heads][dim] into slot slots[i] % page_size of page
  * slots[i] / page_size of each pool. Slots outside the pool (negative ones: padding) are skipped; no slot may be
  * named twice. 16-bit elements of any kind. */
@@ -393,6 +410,18 @@ int vmb_append_pages(const vmb_rows* k_new, const vmb_rows* v_new, const vmb_pag
  * destination may be another pair's source or destination. */
 int vmb_copy_pages(const vmb_pages* k, const vmb_pages* v, const int32_t* src, const int32_t* dst, int64_t count,
                    int64_t num_pages, int32_t kv_heads, int32_t dim, int32_t page_size, void* stream);
+/* The same for pools of e4m3 values with scales (vmb_cache_args). Appended rows are of type dtype. For every page, head and
+ * tensor, the call's rows need the least power of two s, 2^-126 at least, with |x| <= 448 s for each of their finite values.
+ * A call that writes slot 0 of a page begins it: its scale becomes s, and what its other slots held is void. Otherwise the
+ * scale becomes the larger of s and what it was, and where it grows the page's other slots are brought to it (rounded to
+ * nearest). Rows are divided by the scale and rounded to nearest even; infinities and NaN become NaN. The rows that go into
+ * one page have to follow one another in the call, skipped ones not between them. */
+int vmb_append_pages_e4m3(const vmb_rows* k_new, const vmb_rows* v_new, const vmb_pages* k, const vmb_pages* v,
+                          const vmb_page_scales* k_scale, const vmb_page_scales* v_scale, const int32_t* slots, int64_t count,
+                          int64_t num_pages, int32_t kv_heads, int32_t dim, int32_t page_size, int32_t dtype, void* stream);
+int vmb_copy_pages_e4m3(const vmb_pages* k, const vmb_pages* v, const vmb_page_scales* k_scale, const vmb_page_scales* v_scale,
+                        const int32_t* src, const int32_t* dst, int64_t count, int64_t num_pages, int32_t kv_heads, int32_t dim,
+                        int32_t page_size, void* stream);
 
 /*
  * Gated residual with norms around a block (no reference counterpart), over rows of `cols` elements that

@@ -143,6 +143,15 @@ class PagedArgs(ctypes.Structure):
     ]
 
 
+class PageScales(ctypes.Structure):
+    """vmb_page_scales: a (pages, kv_heads) tensor of float32."""
+    _fields_ = [("ptr", c_vp), ("page", c_i64), ("head", c_i64)]
+
+
+class CacheArgs(ctypes.Structure):
+    _fields_ = [("k_scale", PageScales), ("v_scale", PageScales), ("window", c_i32), ("sinks", c_i32)]
+
+
 class Matrix(ctypes.Structure):
     """vmb_matrix: a (rows, cols) tensor with contiguous columns."""
     _fields_ = [("ptr", c_vp), ("row", c_i64)]
@@ -193,6 +202,13 @@ SIGNATURES = {
     "vmb_gated_norm_bwd": (ctypes.c_int, [ctypes.POINTER(GatedNormArgs), c_vp]),
     "vmb_paged_workspace_bytes": (c_i64, [ctypes.POINTER(PagedArgs)]),
     "vmb_paged_attention": (ctypes.c_int, [ctypes.POINTER(PagedArgs), c_vp]),
+    "vmb_cache_workspace_bytes": (c_i64, [ctypes.POINTER(PagedArgs), ctypes.POINTER(CacheArgs)]),
+    "vmb_cache_attention": (ctypes.c_int, [ctypes.POINTER(PagedArgs), ctypes.POINTER(CacheArgs), c_vp]),
+    "vmb_append_pages_e4m3": (ctypes.c_int, [ctypes.POINTER(Rows), ctypes.POINTER(Rows), ctypes.POINTER(Pages),
+                                             ctypes.POINTER(Pages), ctypes.POINTER(PageScales), ctypes.POINTER(PageScales),
+                                             c_vp, c_i64, c_i64, c_i32, c_i32, c_i32, c_i32, c_vp]),
+    "vmb_copy_pages_e4m3": (ctypes.c_int, [ctypes.POINTER(Pages), ctypes.POINTER(Pages), ctypes.POINTER(PageScales),
+                                           ctypes.POINTER(PageScales), c_vp, c_vp, c_i64, c_i64, c_i32, c_i32, c_i32, c_vp]),
     "vmb_append_pages": (ctypes.c_int, [ctypes.POINTER(Rows), ctypes.POINTER(Rows), ctypes.POINTER(Pages),
                                         ctypes.POINTER(Pages), c_vp, c_i64, c_i64, c_i32, c_i32, c_i32, c_vp]),
     "vmb_copy_pages": (ctypes.c_int, [ctypes.POINTER(Pages), ctypes.POINTER(Pages), c_vp, c_vp, c_i64, c_i64, c_i32,

@@ -16,6 +16,10 @@ struct PagedParams {
   int64_t table_stride;
   int batch, heads, kv_heads, dim, page_size, num_pages, max_len;
   float scale_log2;
+  int window, sinks;       // window 0: none
+  // pools of e4m3 values: value x scale[page][head]; NULL: 16-bit pools
+  const float *k_scale, *v_scale;
+  int64_t ks_page, ks_head, vs_page, vs_head;
   // set by paged_plan
   int group, nt, chunks, items, whole_items, box_rows, join_blocks;
   int64_t blocks;
@@ -33,6 +37,10 @@ struct PageMoveParams {
   int64_t k_page, k_head, k_slot, v_page, v_head, v_slot;
   int64_t count;             // append: rows; copy: pages
   int kv_heads, dim, page_size, num_pages;
+  float *k_scale, *v_scale;  // pools of e4m3 values: [page][head]
+  int64_t ks_page, ks_head, vs_page, vs_head;
+  // set by append_pages_e4m3: rows whose runs one team of warps takes
+  int group;
 };
 
 void paged_plan(PagedParams& p);
@@ -40,5 +48,7 @@ int64_t paged_workspace(const PagedParams& p);
 cudaError_t paged_decode(PagedParams p, void* workspace, bool bf16, cudaStream_t st);
 cudaError_t append_pages(const PageMoveParams& p, cudaStream_t st);
 cudaError_t copy_pages(const PageMoveParams& p, cudaStream_t st);
+cudaError_t append_pages_e4m3(PageMoveParams p, bool bf16, cudaStream_t st);
+cudaError_t copy_pages_e4m3(PageMoveParams p, cudaStream_t st);
 
 }  // namespace vmb

@@ -3,6 +3,14 @@
 // neighbouring threads on neighbouring bytes of a row (a page of one head is contiguous in the usual
 // layout, so the rows of a copy follow one another). 32760 tokens of 8 heads, D = 128, appended to pages of 16:
 // 47.5 us, 2047 such pages copied: 47 us, 5.7 TB/s (the measured copy rate is 6.5).
+//
+// Rows that go into e4m3 pools (append_e4m3_kernel) share a scale with what their page holds: the least power of two s
+// with |x| <= 448 s, for a page, head and tensor (a power of two costs a floating format no precision, and a page
+// that grows to a larger one keeps its values but for those that become subnormal). Rows of one page follow one another, so a
+// run of them belongs to one team of warps: largest value, scale, the page brought to it where it grows, rows divided and
+// stored, in one pass and without atomics.
+#include <algorithm>
+
 #include "common.cuh"
 #include "launch.h"
 #include "paged.h"
@@ -19,8 +27,8 @@ __device__ __forceinline__ void store16(void* base, int64_t elem, uint4 v) {
   *reinterpret_cast<uint4*>(static_cast<uint16_t*>(base) + elem) = v;
 }
 
-// COPY: rows are (pair, head, slot); else (row, head).
-template <bool COPY>
+// COPY: rows are (pair, head, slot); else (row, head). SCALED: the pages' scales go with them.
+template <bool COPY, bool SCALED>
 __global__ void __launch_bounds__(kThreads) page_move_kernel(const __grid_constant__ PageMoveParams p) {
   const uint32_t ch = p.dim / 8, inner = (uint32_t)(COPY ? p.page_size : 1) * ch, per = (uint32_t)p.kv_heads * inner;
   const int64_t idx = (int64_t)blockIdx.x * kThreads + threadIdx.x;
@@ -34,6 +42,10 @@ __global__ void __launch_bounds__(kThreads) page_move_kernel(const __grid_consta
     const uint4 k = load16(p.k, s * p.k_page + ko), v = load16(p.v, s * p.v_page + vo);
     store16(p.k, d * p.k_page + ko, k);
     store16(p.v, d * p.v_page + vo, v);
+    if (SCALED && in == 0) {
+      p.k_scale[d * p.ks_page + h * p.ks_head] = p.k_scale[s * p.ks_page + h * p.ks_head];
+      p.v_scale[d * p.vs_page + h * p.vs_head] = p.v_scale[s * p.vs_page + h * p.vs_head];
+    }
   } else {
     const int at = p.dst[i];
     if (at < 0 || at / p.page_size >= p.num_pages) return;
@@ -44,16 +56,196 @@ __global__ void __launch_bounds__(kThreads) page_move_kernel(const __grid_consta
   }
 }
 
-template <bool COPY>
+template <bool COPY, bool SCALED = false>
 cudaError_t launch(const PageMoveParams& p, cudaStream_t st) {
   const int64_t n = p.count * p.kv_heads * (COPY ? p.page_size : 1) * (p.dim / 8);
   const int64_t blocks = (n + kThreads - 1) / kThreads;
   if (blocks > 0x7fffffff) return cudaErrorInvalidConfiguration;
-  page_move_kernel<COPY><<<(unsigned)blocks, kThreads, 0, st>>>(p);
+  page_move_kernel<COPY, SCALED><<<(unsigned)blocks, kThreads, 0, st>>>(p);
+  return cudaGetLastError();
+}
+
+// ------------------------------------------------------------------------------------ rows into e4m3 pools
+constexpr int kTeamWarps = 4;  // warps of a block
+constexpr int kHeld = 8;       // 16-byte loads that a lane holds at a time
+
+// The least power of two s >= 2^-126 with top <= 448 s (448 = 1.75 x 2^8), for a finite top >= 0.
+__device__ __forceinline__ float pow2_scale(float top) {
+  const uint32_t b = __float_as_uint(top);
+  const int e = (int)(b >> 23) - ((b & 0x7fffffu) <= 0x600000u ? 8 : 7);  // biased
+  return __uint_as_float((uint32_t)max(e, 1) << 23);
+}
+
+// A team of TW warps (a warp, or the block) takes the runs that begin in its `group` rows, for one head and tensor.
+template <typename T, int TW>
+__global__ void __launch_bounds__(32 * kTeamWarps) append_e4m3_kernel(const __grid_constant__ PageMoveParams p) {
+  __shared__ float tops[2][kTeamWarps];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t team = TW == 1 ? (int64_t)blockIdx.x * kTeamWarps + warp : blockIdx.x;
+  const int pairs = 2 * p.kv_heads;
+  const int64_t row0 = team / pairs * p.group;
+  if (row0 >= p.count) return;
+  const int pair = (int)(team % pairs), head = pair >> 1;
+  const bool is_v = pair & 1;
+  const T* src = static_cast<const T*>(is_v ? p.v_src : p.k_src) + head * (is_v ? p.v_shead : p.k_shead);
+  const int64_t src_row = is_v ? p.v_row : p.k_row, dst_slot = is_v ? p.v_slot : p.k_slot;
+  uint8_t* pool = static_cast<uint8_t*>(is_v ? p.v : p.k) + head * (is_v ? p.v_head : p.k_head);
+  const int64_t dst_page = is_v ? p.v_page : p.k_page;
+  float* scales = is_v ? p.v_scale + head * p.vs_head : p.k_scale + head * p.ks_head;
+  const int64_t scale_page = is_v ? p.vs_page : p.ks_page;
+  // lanes a row: a power of two, eight columns each
+  const int ch = p.dim / 8, lpr = ch > 8 ? 16 : ch > 4 ? 8 : ch > 2 ? 4 : 2;
+  const int per = 32 / lpr * TW;                                // rows a load of the team
+  const int at = (TW == 1 ? 0 : warp * (32 / lpr)) + lane / lpr, c = lane % lpr * 8;
+  const bool live = c < p.dim;
+  const int step = TW == 1 ? lane : threadIdx.x;
+  int turn = 0;
+  auto page_of = [&](int64_t row) -> int {  // -1: skipped, or past the last row
+    if (row < 0 || row >= p.count) return -1;
+    const int s = p.dst[row];
+    if (s < 0) return -1;
+    const int page = s / p.page_size;
+    return page < p.num_pages ? page : -1;
+  };
+  // (group <= 32: a lane looks at a row)
+  const int mine = page_of(row0 + lane), before = page_of(row0 + lane - 1);
+  unsigned starts = __ballot_sync(0xffffffffu, lane < p.group && mine >= 0 && mine != before);
+  const unsigned same = __ballot_sync(0xffffffffu, mine >= 0 && mine == before);
+  for (; starts; starts &= starts - 1) {
+    const int s = __ffs(starts) - 1, page = __shfl_sync(0xffffffffu, mine, s);
+    const int64_t first = row0 + s;
+    int n = __ffs(~((same >> s) >> 1));  // rows of the run among the 32
+    if (s + n > 31) {                     // up to the last of them: it may go on
+      n = 32 - s;
+      for (;;) {
+        const unsigned other = ~__ballot_sync(0xffffffffu, page_of(first + n + lane) == page);
+        if (other) {
+          n += __ffs(other) - 1;
+          break;
+        }
+        n += 32;
+      }
+    }
+    uint4 x[kHeld];
+    bool begins = false;  // slot 0 of the page is among the rows
+    auto load = [&](int r0) {
+#pragma unroll
+      for (int u = 0; u < kHeld; ++u) {
+        const int r = r0 + u * per + at;
+        x[u] = make_uint4(0u, 0u, 0u, 0u);
+        if (r < n && live) x[u] = load16(src, (first + r) * src_row + c);
+      }
+    };
+    // the largest value; infinities, where there are any, left out (NaN are by fmaxf)
+    float top = 0.f;
+    auto largest = [&](bool finite) {
+      top = 0.f;
+      for (int r0 = 0; r0 < n; r0 += kHeld * per) {
+        if (n > kHeld * per || r0 == 0 && !finite) load(r0);
+#pragma unroll
+        for (int u = 0; u < kHeld; ++u) {
+          const uint32_t w[4] = {x[u].x, x[u].y, x[u].z, x[u].w};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float2 f = Elem<T>::unpack(w[i]);
+            const float a = fabsf(f.x), b = fabsf(f.y);
+            top = fmaxf(top, finite && a == INFINITY ? 0.f : a);
+            top = fmaxf(top, finite && b == INFINITY ? 0.f : b);
+          }
+        }
+      }
+      top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
+      if (TW > 1) {
+        if (lane == 0) tops[turn & 1][warp] = top;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < kTeamWarps; ++i) top = fmaxf(top, tops[turn & 1][i]);
+        ++turn;
+      }
+    };
+    largest(false);
+    const bool infinite = top == INFINITY;
+    if (infinite) largest(true);
+    for (int r = lane; r < n; r += 32) begins |= p.dst[first + r] % p.page_size == 0;
+    begins = __any_sync(0xffffffffu, begins);
+    float* scale_at = scales + page * scale_page;
+    const float old = *scale_at, need = pow2_scale(top);
+    const float scale = begins ? need : fmaxf(old, need);
+    uint8_t* to = pool + page * dst_page;
+    if (TW > 1) __syncthreads();  // everybody has read the scale
+    else __syncwarp();
+    if (!begins && !(old >= scale)) {
+      const float by = old / scale;
+      const int chunks = p.dim / 16;
+      for (int i = step; i < p.page_size * chunks; i += 32 * TW) {
+        uint4* q = reinterpret_cast<uint4*>(to + (int64_t)(i / chunks) * dst_slot + i % chunks * 16);
+        uint4 v = *q;
+        uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const __half2_raw lo = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w[k] & 0xffffu), __NV_E4M3);
+          const __half2_raw hi = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w[k] >> 16), __NV_E4M3);
+          const float2 a = __half22float2(__half2(lo)), b = __half22float2(__half2(hi));
+          w[k] = pack_e4m3x2(a.x * by, a.y * by) | pack_e4m3x2(b.x * by, b.y * by) << 16;
+        }
+        *q = make_uint4(w[0], w[1], w[2], w[3]);
+      }
+      if (TW > 1) __syncthreads();
+      else __syncwarp();
+    }
+    if (step == 0) *scale_at = scale;
+    // a power of two is multiplied with (its inverse is one), any other scale, which a caller brought, divided by
+    const bool pow2 = (__float_as_uint(scale) & 0x7fffffu) == 0;
+    const float inv = 1.f / scale;
+    for (int r0 = 0; r0 < n; r0 += kHeld * per) {
+      if (n > kHeld * per) load(r0);
+#pragma unroll
+      for (int u = 0; u < kHeld; ++u) {
+        const int r = r0 + u * per + at;
+        if (r >= n || !live) continue;
+        const uint32_t w[4] = {x[u].x, x[u].y, x[u].z, x[u].w};
+        uint32_t q[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          float2 f = Elem<T>::unpack(w[i]);
+          if (infinite) {  // the conversion would make the largest value of them
+            if (isinf(f.x)) f.x = __int_as_float(0x7fffffff);
+            if (isinf(f.y)) f.y = __int_as_float(0x7fffffff);
+          }
+          q[i] = pow2 ? pack_e4m3x2(f.x * inv, f.y * inv) : pack_e4m3x2(f.x / scale, f.y / scale);
+        }
+        const int slot = p.dst[first + r] % p.page_size;
+        *reinterpret_cast<uint2*>(to + slot * dst_slot + c) = make_uint2(q[0] | q[1] << 16, q[2] | q[3] << 16);
+      }
+    }
+  }
+}
+
+template <typename T>
+cudaError_t launch_e4m3(PageMoveParams p, cudaStream_t st) {
+  const bool block = p.page_size > 32;
+  const int64_t pairs = 2 * p.kv_heads;
+  // one row a team while all teams fit on the GPU at once, up to a page's rows where there are many
+  const int64_t room = block ? 148 * 16 : 148 * 16 * kTeamWarps;
+  p.group = (int)std::min<int64_t>(std::max<int64_t>((p.count * pairs + room - 1) / room, 1), std::min(p.page_size, 32));
+  const int64_t teams = (p.count + p.group - 1) / p.group * pairs, blocks = block ? teams : (teams + kTeamWarps - 1) / kTeamWarps;
+  if (blocks > 0x7fffffff) return cudaErrorInvalidConfiguration;
+  if (block) append_e4m3_kernel<T, kTeamWarps><<<(unsigned)blocks, 32 * kTeamWarps, 0, st>>>(p);
+  else append_e4m3_kernel<T, 1><<<(unsigned)blocks, 32 * kTeamWarps, 0, st>>>(p);
   return cudaGetLastError();
 }
 
 }  // namespace
+
+cudaError_t append_pages_e4m3(PageMoveParams p, bool bf16, cudaStream_t st) {
+  return bf16 ? launch_e4m3<__nv_bfloat16>(p, st) : launch_e4m3<__half>(p, st);
+}
+// bytes move two at a time: sizes and strides are multiples of 16 of them
+cudaError_t copy_pages_e4m3(PageMoveParams p, cudaStream_t st) {
+  for (int64_t* s : {&p.k_page, &p.k_head, &p.k_slot, &p.v_page, &p.v_head, &p.v_slot}) *s /= 2;
+  p.dim /= 2;
+  return launch<true, true>(p, st);
+}
 
 cudaError_t append_pages(const PageMoveParams& p, cudaStream_t st) { return launch<false>(p, st); }
 cudaError_t copy_pages(const PageMoveParams& p, cudaStream_t st) { return launch<true>(p, st); }

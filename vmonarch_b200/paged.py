@@ -1,8 +1,9 @@
 """A paged key / value cache, and attention of one new token per sequence over it (no reference
 counterpart).
 
-The pool of a layer is a pair of tensors (num_pages, Hk, page_size, D). A sequence's tokens fill pages
-listed in its row of a page table: token t lies in slot t % page_size of page table[b, t // page_size].
+The pool of a layer is a pair of tensors (num_pages, Hk, page_size, D), in 16 bits or in 8: then of type
+torch.float8_e4m3fn, with a scale for each page and head, k_scale and v_scale, (num_pages, Hk) float32. A sequence's tokens
+fill pages listed in its row of a page table: token t lies in slot t % page_size of page table[b, t // page_size].
 :func:`append_pages`, :func:`copy_pages` and :func:`paged_attention` work on such tensors, wherever they come
 from; :class:`PagedKVCache` holds the pools of a model's layers and keeps the book of their pages.
 """
@@ -16,27 +17,39 @@ import torch
 
 from . import _native as N
 from .kernel import SUPPORTED_DTYPES
-from .packed import MAX_DIM, _place
+from .packed import MAX_DIM, _place, _window
+
+#: element type of 8-bit pools
+E4M3 = torch.float8_e4m3fn
 
 
-def _pages(t, n, h, ps, d):
-    """vmb_pages of a pool (n pages, h heads, ps slots, d columns), which the kernels address in place."""
+def _pages(t, n, h, ps, d, step=8):
+    """vmb_pages of a pool (n pages, h heads, ps slots, d columns; 16 bytes are `step` elements), which the kernels address in
+    place."""
     ptr, (page, head, slot, col) = t.data_ptr(), t.stride()
     if n == 1 or h == 1 or ps == 1:  # such strides do not count
         page, head, slot = page if n > 1 else 0, head if h > 1 else 0, slot if ps > 1 else 0
     assert col == 1 or d == 1, "pools need contiguous columns"
-    assert not ptr & 15 and page >= 0 and head >= 0 and slot >= 0 and not (page | head | slot) & 7, \
+    assert not ptr & 15 and page >= 0 and head >= 0 and slot >= 0 and not (page | head | slot) & (step - 1), \
         "pools need 16-byte aligned rows"
     return ptr, page, head, slot
 
 
-def _check_pools(k_pages, v_pages):
+def _check_pools(k_pages, v_pages, k_scale=None, v_scale=None):
     """(pages, heads, page size, dim, dtype, device) of a pair of pools."""
     shape, dtype, device = k_pages.shape, k_pages.dtype, k_pages.device
     assert len(shape) == 4 and v_pages.shape == shape, "pools must be (num_pages, Hk, page_size, D)"
-    assert dtype in SUPPORTED_DTYPES and v_pages.dtype == dtype, f"unsupported dtype {dtype}"
+    assert (dtype in SUPPORTED_DTYPES or dtype == E4M3) and v_pages.dtype == dtype, f"unsupported dtype {dtype}"
     n, h, ps, d = shape
-    assert 8 <= d <= MAX_DIM and d % 8 == 0, f"head dim {d} is not a multiple of 8 up to {MAX_DIM}"
+    step = 8
+    if dtype == E4M3 or k_scale is not None or v_scale is not None:
+        step = 16
+        assert dtype == E4M3 and k_scale is not None and v_scale is not None, \
+            "8-bit pools (torch.float8_e4m3fn), and no others, go with k_scale and v_scale"
+        for scale in (k_scale, v_scale):
+            assert scale.shape == (n, h) and scale.dtype == torch.float32 and scale.device == device, \
+                "scales must be (num_pages, Hk), float32 and on the pools' device"
+    assert 8 <= d <= MAX_DIM and d % step == 0, f"head dim {d} is not a multiple of {step} up to {MAX_DIM}"
     assert n >= 1 and h >= 1 and ps >= 1, "pools need at least one page, head and slot"
     assert k_pages.is_cuda and v_pages.device == device, "pools must be on one CUDA device"
     return n, h, ps, d, dtype, device
@@ -47,18 +60,29 @@ def _check_index(t, name, dim, device):
         f"{name} must be int32, {dim}-dimensional and on the pools' device"
 
 
-def paged_attention(q, k_pages, v_pages, page_table, lengths, *, sm_scale=None, return_lse=False):
+def _scales(t):
+    """vmb_page_scales of a (num_pages, Hk) tensor."""
+    page, head = t.stride()
+    return N.PageScales(t.data_ptr(), page if t.size(0) > 1 else 0, head if t.size(1) > 1 else 0)
+
+
+def paged_attention(q, k_pages, v_pages, page_table, lengths, *, k_scale=None, v_scale=None, window=None, sinks=0,
+                    sm_scale=None, return_lse=False):
     """
     Attention of one new token per sequence over a paged cache (inference: carries no gradient).
 
     Args:
         q: (B, H, D), bf16 or fp16, D a multiple of 8 up to 128
         k_pages, v_pages: (num_pages, Hk, page_size, D), the same dtype, H a multiple of Hk; any strides
-            with contiguous columns and 16-byte aligned rows, any page size
+            with contiguous columns and 16-byte aligned rows, any page size. Or torch.float8_e4m3fn, D a multiple of 16
+        k_scale, v_scale: (num_pages, Hk) float32, not negative, with 8-bit pools: a key or value is its element times the
+            scale of its page and head
         page_table: (B, width) int32, the pages of each sequence; entries past its length are not read.
             A page id outside the pool reads as zeros.
         lengths: (B,) int32, the tokens each sequence has cached, the new one's among them if it is to
             see itself; at most width * page_size count
+        window: only the last `window` tokens (at least 1; None: all) and the first `sinks` are seen; table entries of pages
+            without one of them are not read
         sm_scale: softmax scale, not negative; defaults to 1 / sqrt(D)
         return_lse: also return the log of each softmax's sum
     Returns:
@@ -67,10 +91,14 @@ def paged_attention(q, k_pages, v_pages, page_table, lengths, *, sm_scale=None, 
     Table and lengths stay on the device: the call does not wait for it and can be captured in a CUDA
     graph whose replays see other lengths.
     """
-    num, hk, page_size, d, dtype, device = _check_pools(k_pages, v_pages)
+    num, hk, page_size, d, dtype, device = _check_pools(k_pages, v_pages, k_scale, v_scale)
     shape = q.shape
+    if dtype == E4M3:
+        dtype = q.dtype
+        assert dtype in SUPPORTED_DTYPES, f"unsupported dtype {dtype}"
     assert len(shape) == 3 and q.dtype == dtype and shape[2] == d and q.device == device, \
         "q must be (B, H, D) with the pools' D, dtype and device"
+    mask = _window(window, sinks)
     b, h, _ = shape
     assert h >= 1 and h % hk == 0, "H must be a multiple of Hk"
     _check_index(page_table, "page_table", 2, device)
@@ -88,14 +116,25 @@ def paged_attention(q, k_pages, v_pages, page_table, lengths, *, sm_scale=None, 
     lse = torch.empty((b, h), dtype=torch.float32, device=device) if return_lse else None
     if b:
         a = N.PagedArgs()
-        _PAGED.pack_into(a, 0, *qr, o.data_ptr(), h * d, d, *_pages(k_pages, num, hk, page_size, d), *_pages(v_pages, num, hk, page_size, d), page_table.data_ptr(),
+        pool = num, hk, page_size, d, 8 if k_scale is None else 16
+        _PAGED.pack_into(a, 0, *qr, o.data_ptr(), h * d, d, *_pages(k_pages, *pool), *_pages(v_pages, *pool), page_table.data_ptr(),
                          lengths.data_ptr(), lse.data_ptr() if return_lse else 0, b, stride if b > 1 else width, width, num,
                          h, hk, d, page_size, N.dtype_code(dtype), sm_scale)
-        size = N.lib.vmb_paged_workspace_bytes(ctypes.byref(a))
+        if k_scale is None and mask is None:
+            name, args = "vmb_paged_attention", (ctypes.byref(a),)
+            size = N.lib.vmb_paged_workspace_bytes(*args)
+        else:
+            c = N.CacheArgs()
+            if k_scale is not None:
+                c.k_scale, c.v_scale = _scales(k_scale), _scales(v_scale)
+            if mask is not None:
+                c.window, c.sinks = mask
+            name, args = "vmb_cache_attention", (ctypes.byref(a), ctypes.byref(c))
+            size = N.lib.vmb_cache_workspace_bytes(*args)
         if size > 0:
             ws = torch.empty(size, dtype=torch.uint8, device=device)
             a.workspace, a.workspace_bytes = ws.data_ptr(), size
-        N.launch("vmb_paged_attention", N.lib.vmb_paged_attention, device, ctypes.byref(a))
+        N.launch(name, getattr(N.lib, name), device, *args)
     return (o, lse) if return_lse else o
 
 
@@ -104,19 +143,29 @@ _PAGED = struct.Struct("21q5if")
 assert _PAGED.size == N.PagedArgs.workspace.offset
 
 
-def append_pages(k, v, k_pages, v_pages, slots):
+def append_pages(k, v, k_pages, v_pages, slots, *, k_scale=None, v_scale=None):
     """
     Writes new rows into their slots of a pool, in place.
 
     Args:
-        k, v: (T, Hk, D), the pools' dtype
+        k, v: (T, Hk, D), the pools' dtype; bf16 or fp16 with 8-bit pools
         k_pages, v_pages: (num_pages, Hk, page_size, D)
         slots: (T,) int32, page * page_size + slot of each row. Slots outside the pool (negative ones, as
             padding) are skipped; no slot may be named twice.
+        k_scale, v_scale: (num_pages, Hk) float32, with 8-bit pools; written too. Zero for pages that were never used.
+
+    Into 8-bit pools rows are rounded, divided by their page's and head's scale. The call's rows of a page need the least power
+    of two s (2^-126 at least) with |x| <= 448 s. A call that writes a page's slot 0 begins the page: the scale becomes s, and
+    what other slots held is void. Otherwise the scale becomes the larger of s and what it was; where it grows, the page's
+    other slots are brought to it, which changes only values that become subnormal. Infinities and NaN become NaN. The rows that go
+    into one page have to follow one another in the call, as :meth:`PagedKVCache.reserve` and :func:`reserve_pages` list them.
     """
-    num, hk, page_size, d, dtype, device = _check_pools(k_pages, v_pages)
+    num, hk, page_size, d, dtype, device = _check_pools(k_pages, v_pages, k_scale, v_scale)
     assert k.dim() == 3 and v.shape == k.shape and k.shape[1:] == (hk, d), "k and v must be (T, Hk, D) with the pools' Hk and D"
-    assert k.dtype == dtype and v.dtype == dtype, "k and v must have the pools' dtype"
+    if dtype == E4M3:
+        assert k.dtype in SUPPORTED_DTYPES and v.dtype == k.dtype, "k and v must be both bf16 or both fp16"
+    else:
+        assert k.dtype == dtype and v.dtype == dtype, "k and v must have the pools' dtype"
     assert k.device == device and v.device == device, "k and v must be on the pools' device"
     _check_index(slots, "slots", 1, device)
     n = k.size(0)
@@ -128,11 +177,16 @@ def append_pages(k, v, k_pages, v_pages, slots):
     v, *vr = _place(v)
     slots = slots.contiguous()
     pool = num, hk, page_size, d
+    if k_scale is not None:
+        N.launch("vmb_append_pages_e4m3", N.lib.vmb_append_pages_e4m3, device, N.Rows(*kr), N.Rows(*vr),
+                 N.Pages(*_pages(k_pages, *pool, 16)), N.Pages(*_pages(v_pages, *pool, 16)), _scales(k_scale), _scales(v_scale),
+                 slots.data_ptr(), n, num, hk, d, page_size, N.dtype_code(k.dtype))
+        return
     N.launch("vmb_append_pages", N.lib.vmb_append_pages, device, N.Rows(*kr), N.Rows(*vr), N.Pages(*_pages(k_pages, *pool)),
              N.Pages(*_pages(v_pages, *pool)), slots.data_ptr(), n, num, hk, d, page_size)
 
 
-def copy_pages(k_pages, v_pages, src, dst):
+def copy_pages(k_pages, v_pages, src, dst, *, k_scale=None, v_scale=None):
     """
     Copies page src[i] to page dst[i] of both pools, in place.
 
@@ -140,8 +194,9 @@ def copy_pages(k_pages, v_pages, src, dst):
         k_pages, v_pages: (num_pages, Hk, page_size, D)
         src, dst: (n,) int32 page ids. Pairs with a page outside the pool are skipped; no destination may be
             another pair's source or destination.
+        k_scale, v_scale: (num_pages, Hk) float32, with 8-bit pools; copied too
     """
-    num, hk, page_size, d, dtype, device = _check_pools(k_pages, v_pages)
+    num, hk, page_size, d, dtype, device = _check_pools(k_pages, v_pages, k_scale, v_scale)
     _check_index(src, "src", 1, device)
     _check_index(dst, "dst", 1, device)
     n = src.size(0)
@@ -150,6 +205,11 @@ def copy_pages(k_pages, v_pages, src, dst):
         return
     src, dst = src.contiguous(), dst.contiguous()
     pool = num, hk, page_size, d
+    if k_scale is not None:
+        N.launch("vmb_copy_pages_e4m3", N.lib.vmb_copy_pages_e4m3, device, N.Pages(*_pages(k_pages, *pool, 16)),
+                 N.Pages(*_pages(v_pages, *pool, 16)), _scales(k_scale), _scales(v_scale), src.data_ptr(), dst.data_ptr(), n,
+                 num, hk, d, page_size)
+        return
     N.launch("vmb_copy_pages", N.lib.vmb_copy_pages, device, N.Pages(*_pages(k_pages, *pool)),
              N.Pages(*_pages(v_pages, *pool)), src.data_ptr(), dst.data_ptr(), n, num, hk, d, page_size)
 
@@ -167,18 +227,23 @@ class PagedKVCache:
         num_pages, page_size: size of each layer's pools
         kv_heads, head_dim: of the keys and values; head_dim a multiple of 8 up to 128
         layers: number of layers
-        dtype, device: of the pools
+        dtype, device: of the pools. With torch.float8_e4m3fn they hold 8 bits an element (head_dim a multiple of 16), and
+            `k_scale` and `v_scale`, (layers, num_pages, kv_heads), the scales of their pages and heads.
     """
 
     def __init__(self, num_pages, page_size, kv_heads, head_dim, *, layers=1, dtype=torch.bfloat16, device="cuda"):
         assert num_pages >= 1 and page_size >= 1 and kv_heads >= 1 and layers >= 1, "sizes must be positive"
         assert num_pages * page_size < 2 ** 31, "slots are 32-bit: fewer pages or smaller ones"
-        assert dtype in SUPPORTED_DTYPES, f"unsupported dtype {dtype}"
-        assert 8 <= head_dim <= MAX_DIM and head_dim % 8 == 0, f"head dim {head_dim} is not a multiple of 8 up to {MAX_DIM}"
+        assert dtype in SUPPORTED_DTYPES or dtype == E4M3, f"unsupported dtype {dtype}"
+        step = 16 if dtype == E4M3 else 8
+        assert 8 <= head_dim <= MAX_DIM and head_dim % step == 0, f"head dim {head_dim} is not a multiple of {step} up to {MAX_DIM}"
         self.page_size, self.num_pages = page_size, num_pages
         shape = (layers, num_pages, kv_heads, page_size, head_dim)
         self.k = torch.zeros(shape, dtype=dtype, device=device)
         self.v = torch.zeros(shape, dtype=dtype, device=device)
+        self.k_scale = self.v_scale = None
+        if dtype == E4M3:
+            self.k_scale, self.v_scale = torch.zeros((2, layers, num_pages, kv_heads), dtype=torch.float32, device=device)
         self.device = self.k.device
         self._free = list(range(num_pages - 1, -1, -1))  # taken from the end: low pages first
         self._owners = [0] * num_pages
@@ -221,11 +286,15 @@ class PagedKVCache:
     def _ints(self, values):
         return torch.from_numpy(np.asarray(values, dtype=np.int32)).to(self.device)
 
+    def _scales(self, layer):
+        """The scales of a layer's pools, as the calls take them: none with 16-bit pools."""
+        return {} if self.k_scale is None else dict(k_scale=self.k_scale[layer], v_scale=self.v_scale[layer])
+
     def _copy(self, src, dst):
         if src:
             src, dst = self._ints(src), self._ints(dst)
-            for k, v in zip(self.k, self.v):
-                copy_pages(k, v, src, dst)
+            for layer, (k, v) in enumerate(zip(self.k, self.v)):
+                copy_pages(k, v, src, dst, **self._scales(layer))
 
     def reserve(self, seqs, counts) -> torch.Tensor:
         """
@@ -275,7 +344,7 @@ class PagedKVCache:
 
     def write(self, layer: int, k, v, slots) -> None:
         """Rows k, v (T, Hk, D) of one layer into the slots that :meth:`reserve` gave."""
-        append_pages(k, v, self.k[layer], self.v[layer], slots)
+        append_pages(k, v, self.k[layer], self.v[layer], slots, **self._scales(layer))
 
     def tables(self, seqs):
         """(page table, lengths) of the sequences, for :meth:`attend` in every layer."""
@@ -285,9 +354,10 @@ class PagedKVCache:
             table[i, :len(r)] = r
         return self._ints(table), self._ints([self._length[s] for s in seqs])
 
-    def attend(self, layer: int, q, table, lengths, *, sm_scale=None):
+    def attend(self, layer: int, q, table, lengths, *, window=None, sinks=0, sm_scale=None):
         """:func:`paged_attention` of one token per sequence over a layer's pool."""
-        return paged_attention(q, self.k[layer], self.v[layer], table, lengths, sm_scale=sm_scale)
+        return paged_attention(q, self.k[layer], self.v[layer], table, lengths, **self._scales(layer), window=window, sinks=sinks,
+                               sm_scale=sm_scale)
 
     def compact(self) -> int:
         """Moves the pages in use to the lowest ids (tables made before are void) and returns how many
