@@ -424,6 +424,31 @@ int vmb_copy_pages_e4m3(const vmb_pages* k, const vmb_pages* v, const vmb_page_s
                         int32_t page_size, void* stream);
 
 /*
+ * The book of a paged cache on the device (no reference counterpart): sequence b of lengths[b] tokens holds
+ * ceil(lengths[b] / page_size) pages, the first entries of its table row; free_pages[0 .. *num_free) is the stack of the
+ * others. reserve: counts[b] more tokens of every sequence. The new pages of the sequences, in order, are taken from the
+ * stack's end, lengths and *num_free follow, and slots[total] gets the slot of every new token, sequence after sequence, then
+ * -1. truncate: every sequence keeps its first keep[b] tokens (negative: none); the pages beyond go back in the opposite order.
+ * A call that cannot be done changes nothing, adds bits to *failed (1 too few free pages, 2 a table row too narrow, 4 more
+ * tokens than rows or a negative number, 8 more pages than the stack has room for) and gives slots of -1.
+ */
+typedef struct vmb_page_book {
+  int32_t* table;       /* [batch][table_stride], of which table_width entries a row */
+  int32_t* lengths;     /* [batch] */
+  int32_t* free_pages;  /* [num_pages] */
+  int32_t* num_free;    /* [1] */
+  int32_t* failed;      /* [1], or NULL */
+  int64_t table_stride, batch, table_width, num_pages;
+  int32_t page_size;
+} vmb_page_book;
+
+/* Workspace of either call; needed above 1024 sequences, for reserve above 4096 rows, for truncate above 65536 table entries. */
+int64_t vmb_page_book_workspace_bytes(const vmb_page_book* b);  /* -1: malformed sizes */
+int vmb_reserve_pages(const vmb_page_book* b, const int32_t* counts, int32_t* slots, int64_t total, void* workspace,
+                      int64_t workspace_bytes, void* stream);
+int vmb_truncate_pages(const vmb_page_book* b, const int32_t* keep, void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
  * Gated residual with norms around a block (no reference counterpart), over rows of `cols` elements that
  * belong to `seqs` sequences one after another (seq_start[s]: first row of sequence s, device int32;
  * NULL with one sequence):

@@ -152,6 +152,11 @@ class CacheArgs(ctypes.Structure):
     _fields_ = [("k_scale", PageScales), ("v_scale", PageScales), ("window", c_i32), ("sinks", c_i32)]
 
 
+class PageBook(ctypes.Structure):
+    _fields_ = [("table", c_vp), ("lengths", c_vp), ("free_pages", c_vp), ("num_free", c_vp), ("failed", c_vp),
+                ("table_stride", c_i64), ("batch", c_i64), ("table_width", c_i64), ("num_pages", c_i64), ("page_size", c_i32)]
+
+
 class Matrix(ctypes.Structure):
     """vmb_matrix: a (rows, cols) tensor with contiguous columns."""
     _fields_ = [("ptr", c_vp), ("row", c_i64)]
@@ -202,6 +207,9 @@ SIGNATURES = {
     "vmb_gated_norm_bwd": (ctypes.c_int, [ctypes.POINTER(GatedNormArgs), c_vp]),
     "vmb_paged_workspace_bytes": (c_i64, [ctypes.POINTER(PagedArgs)]),
     "vmb_paged_attention": (ctypes.c_int, [ctypes.POINTER(PagedArgs), c_vp]),
+    "vmb_page_book_workspace_bytes": (c_i64, [ctypes.POINTER(PageBook)]),
+    "vmb_reserve_pages": (ctypes.c_int, [ctypes.POINTER(PageBook), c_vp, c_vp, c_i64, c_vp, c_i64, c_vp]),
+    "vmb_truncate_pages": (ctypes.c_int, [ctypes.POINTER(PageBook), c_vp, c_vp, c_i64, c_vp]),
     "vmb_cache_workspace_bytes": (c_i64, [ctypes.POINTER(PagedArgs), ctypes.POINTER(CacheArgs)]),
     "vmb_cache_attention": (ctypes.c_int, [ctypes.POINTER(PagedArgs), ctypes.POINTER(CacheArgs), c_vp]),
     "vmb_append_pages_e4m3": (ctypes.c_int, [ctypes.POINTER(Rows), ctypes.POINTER(Rows), ctypes.POINTER(Pages),

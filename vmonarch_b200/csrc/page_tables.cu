@@ -1,0 +1,211 @@
+// The book of a paged cache on the GPU: which pages hold a sequence's tokens, and which are free.
+//
+// Free pages are a stack, free_pages[0 .. num_free). Sequence b of length n holds ceil(n / page_size) pages, in order, in its
+// row of the table.
+//   reserve   sequence b is to hold c_b more tokens. The new pages of all sequences, in order, come off the stack one by one:
+//             the j-th is free_pages[num_free - 1 - j]. Row i of the packed new tokens (all of sequence 0's, then 1's ...) gets
+//             the slot page * page_size + position % page_size of its token; rows past the last token -1.
+//   truncate  sequence b keeps its first k_b tokens. Pages beyond them go back in the opposite order, so that a truncate
+//             undoes a reserve.
+// A call that cannot be done (too few free pages, a table row too narrow, more tokens than rows) changes nothing, says so in
+// `failed` and gives the slots -1, which the appending kernels skip.
+//
+// The work is a prefix sum over the sequences, a few bytes a token, and bound by latency: the sums are one block's (each
+// thread takes neighbouring sequences), which goes on to the rows or pages by itself where they are few; otherwise it leaves
+// its sums to a second kernel that is launched early. Whole numbers, no atomics on them: the same book from run to run.
+#include "common.cuh"
+#include "launch.h"
+#include "page_tables.h"
+
+namespace vmb {
+namespace {
+
+constexpr int kThreads = 1024;
+constexpr int kOneBatch = 1024;  // most sequences of a call in one block
+constexpr int kOneRows = 4096;   // and rows, or table entries per 16 sequences
+
+enum { kNoPages = 1, kTooWide = 2, kTooMany = 4, kOverfull = 8 };
+
+__device__ __forceinline__ int ceil_div(int64_t a, int b) { return (int)((a + b - 1) / b); }
+
+// What the sums of a call say of each sequence: its length before, the rows and pages before it; and of the call.
+struct Plan {
+  int *len, *rows, *pages, *call;  // [batch], [batch + 1], [batch + 1]; call: done (1) or not, free pages before
+};
+__device__ __forceinline__ Plan plan_at(int32_t* at, int batch) {
+  return Plan{at, at + batch, at + 2 * batch + 1, at + 3 * batch + 2};
+}
+
+// Exclusive sums of two values over the block's threads, and their totals.
+struct Sums {
+  int64_t a, b, total_a, total_b;
+};
+__device__ __forceinline__ Sums block_sums(int64_t a, int64_t b) {
+  __shared__ int64_t warp_a[33], warp_b[33];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+  int64_t ia = a, ib = b;
+#pragma unroll
+  for (int s = 1; s < 32; s <<= 1) {
+    const int64_t x = __shfl_up_sync(0xffffffffu, ia, s), y = __shfl_up_sync(0xffffffffu, ib, s);
+    if (lane >= s) ia += x, ib += y;
+  }
+  if (lane == 31) warp_a[warp] = ia, warp_b[warp] = ib;
+  __syncthreads();
+  if (warp == 0) {
+    int64_t x = lane < warps ? warp_a[lane] : 0, y = lane < warps ? warp_b[lane] : 0;
+    const int64_t x0 = x, y0 = y;
+#pragma unroll
+    for (int s = 1; s < 32; s <<= 1) {
+      const int64_t u = __shfl_up_sync(0xffffffffu, x, s), v = __shfl_up_sync(0xffffffffu, y, s);
+      if (lane >= s) x += u, y += v;
+    }
+    warp_a[lane] = x - x0, warp_b[lane] = y - y0;
+    if (lane == 31) warp_a[32] = x, warp_b[32] = y;
+  }
+  __syncthreads();
+  return Sums{warp_a[warp] + ia - a, warp_b[warp] + ib - b, warp_a[32], warp_b[32]};
+}
+
+// The rows [row, total) in steps of `step`.
+__device__ __forceinline__ void write_slots(const BookParams& p, const Plan& plan, int64_t row, int64_t step) {
+  const bool done = plan.call[0] != 0;
+  const int top = plan.call[1] - 1, last = plan.rows[p.batch];
+  for (; row < p.total; row += step) {
+    int slot = -1;
+    if (done && row < last) {
+      int lo = 0, hi = p.batch;  // the last sequence that begins at or before the row: rows[lo] <= row < rows[hi]
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (plan.rows[mid] <= row) lo = mid;
+        else hi = mid;
+      }
+      const int len = plan.len[lo], at = len + (int)(row - plan.rows[lo]);
+      const int i = at / p.page_size, in = at - i * p.page_size, have = ceil_div(len, p.page_size);
+      int32_t* entry = p.table + lo * p.stride + i;
+      const int page = i < have ? *entry : p.free_pages[top - (plan.pages[lo] + i - have)];
+      if (in == 0) *entry = page;  // (a page's first token is new if the page is)
+      if ((unsigned)page < (unsigned)p.num_pages) slot = page * p.page_size + in;
+    }
+    p.slots[row] = slot;
+  }
+}
+// Sequence b's pages beyond its new length, by threads of which this is the `t`-th of `n`.
+__device__ __forceinline__ void return_pages(const BookParams& p, const Plan& plan, int b, int t, int n) {
+  const int count = plan.pages[b + 1] - plan.pages[b], held = ceil_div(plan.len[b], p.page_size);
+  const int top = plan.call[1] + plan.pages[p.batch] - 1;
+  const int32_t* from = p.table + b * p.stride + held - count;
+  for (int i = t; i < count; i += n) p.free_pages[top - (plan.pages[b] + i)] = from[i];
+}
+
+// RESERVE: counts -> sums, else lengths to keep -> sums. ONE: this block does the rest too.
+template <bool RESERVE, bool ONE>
+__global__ void __launch_bounds__(kThreads) book_kernel(const __grid_constant__ BookParams p) {
+  __shared__ int32_t plan_sh[ONE ? 3 * kOneBatch + 4 : 1];
+  const Plan plan = plan_at(ONE ? plan_sh : p.plan, p.batch);
+  if (!ONE) let_next_kernel_start();
+  const int per = (p.batch + blockDim.x - 1) / blockDim.x;
+  const int b0 = min((int)threadIdx.x * per, p.batch), b1 = min(b0 + per, p.batch);
+  const int64_t room = min((int64_t)p.width * p.page_size, (int64_t)0x7fffffff - 64);  // (what the attention takes)
+  int64_t rows = 0, pages = 0;
+  int bad = 0;
+  // tokens before and behind a call
+  auto lengths = [&](int b, int64_t& len, int64_t& next) {
+    len = p.lengths[b];
+    const int64_t want = p.want[b];
+    next = RESERVE ? len + want : max((int64_t)0, min(len, want));
+    if (len < 0 || (RESERVE && want < 0)) bad |= kTooMany, next = len = max(len, (int64_t)0);
+    if (max(len, next) > room) bad |= kTooWide, next = len = min(len, room);
+  };
+  for (int b = b0; b < b1; ++b) {
+    int64_t len, next;
+    lengths(b, len, next);
+    rows += RESERVE ? next - len : 0;
+    pages += RESERVE ? ceil_div(next, p.page_size) - ceil_div(len, p.page_size) : ceil_div(len, p.page_size) - ceil_div(next, p.page_size);
+  }
+  const int free_before = max(0, min(*p.num_free, p.num_pages));
+  const Sums s = block_sums(rows, pages);
+  if (RESERVE && s.total_b > free_before) bad |= kNoPages;
+  if (RESERVE && s.total_a > p.total) bad |= kTooMany;
+  if (!RESERVE && free_before + s.total_b > p.num_pages) bad |= kOverfull;
+  // (every thread has read the number of free pages)
+  bad = (__syncthreads_or(bad & kNoPages) ? kNoPages : 0) | (__syncthreads_or(bad & kTooWide) ? kTooWide : 0) |
+        (__syncthreads_or(bad & kTooMany) ? kTooMany : 0) | (__syncthreads_or(bad & kOverfull) ? kOverfull : 0);
+  if (threadIdx.x == 0) {
+    plan.call[0] = bad == 0;
+    plan.call[1] = free_before;
+    if (bad && p.failed) *p.failed |= bad;
+    if (!bad) *p.num_free = free_before + (int)(RESERVE ? -s.total_b : s.total_b);
+  }
+  if (!bad) {
+    rows = s.a;
+    pages = s.b;
+    for (int b = b0; b < b1; ++b) {
+      int64_t len, next;
+      lengths(b, len, next);
+      plan.len[b] = (int)len;
+      plan.rows[b] = (int)rows;
+      plan.pages[b] = (int)pages;
+      rows += RESERVE ? next - len : 0;
+      pages += RESERVE ? ceil_div(next, p.page_size) - ceil_div(len, p.page_size) : ceil_div(len, p.page_size) - ceil_div(next, p.page_size);
+      p.lengths[b] = (int)next;
+    }
+    if (threadIdx.x == 0) plan.rows[p.batch] = (int)s.total_a, plan.pages[p.batch] = (int)s.total_b;
+  }
+  if (!ONE) return;
+  __syncthreads();
+  if (RESERVE) {
+    write_slots(p, plan, threadIdx.x, blockDim.x);
+  } else if (!bad) {
+    for (int b = threadIdx.x >> 5; b < p.batch; b += blockDim.x >> 5) return_pages(p, plan, b, threadIdx.x & 31, 32);
+  }
+}
+
+__global__ void __launch_bounds__(256) slots_kernel(const __grid_constant__ BookParams p) {
+  wait_for_kernel_before();
+  let_next_kernel_start();
+  write_slots(p, plan_at(p.plan, p.batch), (int64_t)blockIdx.x * 256 + threadIdx.x, (int64_t)gridDim.x * 256);
+}
+// A warp a sequence.
+__global__ void __launch_bounds__(256) return_kernel(const __grid_constant__ BookParams p) {
+  wait_for_kernel_before();
+  let_next_kernel_start();
+  const Plan plan = plan_at(p.plan, p.batch);
+  const int64_t b = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (b < p.batch && plan.call[0]) return_pages(p, plan, (int)b, threadIdx.x & 31, 32);
+}
+
+// threads of the first kernel: a sequence, and where it does them a row, each, if that many fit
+int threads_for(int64_t n) { return (int)(n >= kThreads ? kThreads : n <= 128 ? 128 : (n + 31) / 32 * 32); }
+
+}  // namespace
+
+int64_t book_plan_ints(int64_t batch) { return 3 * batch + 4; }
+
+bool reserve_in_one(const BookParams& p) { return p.batch <= kOneBatch && p.total <= kOneRows; }
+// (at most the whole table goes back: 64 entries a thread)
+bool truncate_in_one(const BookParams& p) { return p.batch <= kOneBatch && (int64_t)p.batch * p.width <= 16 * kOneRows; }
+
+cudaError_t reserve_pages(const BookParams& p, cudaStream_t st) {
+  if (reserve_in_one(p)) {
+    book_kernel<true, true><<<1, threads_for(p.total > p.batch ? p.total : p.batch), 0, st>>>(p);
+    return cudaGetLastError();
+  }
+  book_kernel<true, false><<<1, threads_for(p.batch), 0, st>>>(p);
+  cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess || p.total == 0) return e;
+  const int64_t blocks = (p.total + 255) / 256;
+  return launch_early(slots_kernel, blocks < 148 * 8 ? blocks : 148 * 8, 256, 0, st, p);
+}
+
+cudaError_t truncate_pages(const BookParams& p, cudaStream_t st) {
+  if (truncate_in_one(p)) {
+    book_kernel<false, true><<<1, threads_for(32 * (int64_t)p.batch), 0, st>>>(p);
+    return cudaGetLastError();
+  }
+  book_kernel<false, false><<<1, threads_for(p.batch), 0, st>>>(p);
+  cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return e;
+  return launch_early(return_kernel, ((int64_t)p.batch + 7) / 8, 256, 0, st, p);
+}
+
+}  // namespace vmb

@@ -18,6 +18,7 @@ import torch
 from . import _native as N
 from .kernel import SUPPORTED_DTYPES
 from .packed import MAX_DIM, _place, _window
+from .page_tables import PageTables
 
 #: element type of 8-bit pools
 E4M3 = torch.float8_e4m3fn
@@ -249,11 +250,27 @@ class PagedKVCache:
         self._owners = [0] * num_pages
         self._pages, self._length = {}, {}
         self._next = 0
+        self._lent = False  # whether pages are a PageTables' now
 
     @property
     def num_free(self) -> int:
         """Pages that no sequence holds."""
         return len(self._free)
+
+    def page_tables(self, batch, width, num_pages=None):
+        """
+        A :class:`PageTables` of `batch` sequences over this cache's pools, with `num_pages` (default: all) of its free pages,
+        which are then no longer this book's. Its slots, table and lengths go to :meth:`write` and :meth:`attend`, beside
+        those of sequences of this book.
+        """
+        num_pages = len(self._free) if num_pages is None else num_pages
+        if num_pages > len(self._free):
+            raise MemoryError(f"paged cache: {num_pages} pages needed, {len(self._free)} of {self.num_pages} free")
+        tables = PageTables(self.num_pages, self.page_size, batch, width, pages=self._free[len(self._free) - num_pages:],
+                            device=self.device)
+        del self._free[len(self._free) - num_pages:]
+        self._lent = self._lent or num_pages > 0
+        return tables
 
     def length(self, seq: int) -> int:
         return self._length[seq]
@@ -362,6 +379,7 @@ class PagedKVCache:
     def compact(self) -> int:
         """Moves the pages in use to the lowest ids (tables made before are void) and returns how many
         are in use. The pools' tails can then be left out of a copy or a snapshot."""
+        assert not self._lent, "pages that a PageTables holds cannot be moved"
         used = [p for p in range(self.num_pages) if self._owners[p]]
         n = len(used)
         holes = [p for p in range(n) if not self._owners[p]]
