@@ -124,15 +124,16 @@ int vmb_test_pipeline_timeout(int64_t wait_cycles, int32_t hold_loads) {
 
 int vmb_device_status(void* stream, int32_t* out) {
   if (!out) return fail(VMB_EINVAL, "vmb_device_status: null output");
-  int v = 0, w = 0, x = 0, y = 0, z = 0, g = 0;
+  int v = 0, w = 0, x = 0, y = 0, z = 0, g = 0, g8 = 0;
   cudaError_t e = vmb::fea_fwd_sm100_status(static_cast<cudaStream_t>(stream), &v);
   if (e == cudaSuccess) e = vmb::fea_bwd_sm100_status(static_cast<cudaStream_t>(stream), &w);
   if (e == cudaSuccess) e = vmb::lstep_tc_status(static_cast<cudaStream_t>(stream), &x);
   if (e == cudaSuccess) e = vmb::packed_status(static_cast<cudaStream_t>(stream), &y);
   if (e == cudaSuccess) e = vmb::packed_bwd_status(static_cast<cudaStream_t>(stream), &z);
   if (e == cudaSuccess) e = vmb::paged_status(static_cast<cudaStream_t>(stream), &g);
+  if (e == cudaSuccess) e = vmb::paged8_status(static_cast<cudaStream_t>(stream), &g8);
   if (e != cudaSuccess) return cuda_status(e, "vmb_device_status");
-  *out = v | (w << 8) | (x << 16) | ((y | z | g) << 24);
+  *out = v | (w << 8) | (x << 16) | ((y | z | g | g8) << 24);
   return VMB_OK;
 }
 

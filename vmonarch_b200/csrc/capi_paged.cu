@@ -71,7 +71,7 @@ int fill(const vmb_paged_args* a, const vmb_cache_args* c, vmb::PagedParams& p, 
   p.heads = a->heads; p.kv_heads = a->kv_heads; p.dim = a->dim; p.page_size = a->page_size;
   p.num_pages = (int)a->num_pages;
   // token positions are 32-bit, a tile past the last one included
-  p.max_len = (int)std::min<int64_t>(a->table_width * a->page_size, 0x7fffffff - 64);
+  p.max_len = (int)std::min<int64_t>(a->table_width * a->page_size, 0x7fffffff - (e4m3 ? vmb::kPagedTile8 : 64));
   p.scale_log2 = a->sm_scale * vmb::kLog2e;
   vmb::paged_plan(p);
   return VMB_OK;

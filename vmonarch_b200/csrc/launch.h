@@ -88,6 +88,7 @@ cudaError_t packed_status(cudaStream_t st, int* out);
 cudaError_t packed_bwd(const PackedParams& dq, const PackedParams& kv, bool bf16, cudaStream_t st);
 cudaError_t packed_bwd_status(cudaStream_t st, int* out);
 cudaError_t paged_status(cudaStream_t st, int* out);
+cudaError_t paged8_status(cudaStream_t st, int* out);
 
 // Raises a kernel's dynamic shared memory limit, once per device (`done`: a bit each, static beside the launch).
 template <typename Kern>

@@ -22,6 +22,7 @@ struct PagedParams {
   int64_t ks_page, ks_head, vs_page, vs_head;
   // set by paged_plan
   int group, nt, chunks, items, whole_items, box_rows, join_blocks;
+  int cols;  // columns that the kernels work on: 64 or 128
   int64_t blocks;
   float *part, *part_ml;
   long long wait_limit;  // pipeline wait limit in cycles (0: the default ~2 s)
@@ -46,6 +47,9 @@ struct PageMoveParams {
 void paged_plan(PagedParams& p);
 int64_t paged_workspace(const PagedParams& p);
 cudaError_t paged_decode(PagedParams p, void* workspace, bool bf16, cudaStream_t st);
+// over e4m3 pools (p planned, with its partials' places): tiles of that many tokens
+constexpr int kPagedTile8 = 128;
+cudaError_t paged_decode8(const PagedParams& p, bool bf16, cudaStream_t st);
 cudaError_t append_pages(const PageMoveParams& p, cudaStream_t st);
 cudaError_t copy_pages(const PageMoveParams& p, cudaStream_t st);
 cudaError_t append_pages_e4m3(PageMoveParams p, bool bf16, cudaStream_t st);

@@ -34,11 +34,12 @@ inline EncodeTiledFn encode_fn() {
 // 5-D map over the view `v` of a [batch][rows][cols] tensor (fea_params.h): dims (cols, rows, n1,
 // n2, batch / (n1 n2)), so a tile of batch entry s is addressed as (x, y, s % n1, s / n1 % n2,
 // s / (n1 n2)). Boxes of `box_cols` columns (128 B, one swizzle row) x `box_rows` rows, 128-byte
-// swizzle. Rows past `rows` read as zeros and are clipped on stores, per batch entry. Strides must
+// swizzle (or 64 B and a 64-byte one). Rows past `rows` read as zeros and are clipped on stores, per batch entry. Strides must
 // be multiples of 16 bytes (token-major head strides of D * 2 bytes are); the stride of an extent-1
 // dimension is never used and is replaced by a valid value.
 inline bool make_map5(CUtensorMap* m, CUtensorMapDataType dt, int esize, const void* base, int64_t cols, int64_t rows,
-                      int64_t batch, const View& v, int n1, int n2, int box_cols, int box_rows) {
+                      int64_t batch, const View& v, int n1, int n2, int box_cols, int box_rows,
+                      CUtensorMapSwizzle swizzle = CU_TENSOR_MAP_SWIZZLE_128B) {
   EncodeTiledFn enc = encode_fn();
   if (!enc || n1 < 1 || n2 < 1 || batch < 1 || batch % ((int64_t)n1 * n2)) return false;
   const int64_t n3 = batch / ((int64_t)n1 * n2);
@@ -55,7 +56,7 @@ inline bool make_map5(CUtensorMap* m, CUtensorMapDataType dt, int esize, const v
   cuuint32_t box[5] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows, 1, 1, 1};
   cuuint32_t estr[5] = {1, 1, 1, 1, 1};
   return enc(m, dt, 5, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
