@@ -23,6 +23,7 @@ struct PagedParams {
   // set by paged_plan
   int group, nt, chunks, items, whole_items, box_rows, join_blocks;
   int cols;  // columns that the kernels work on: 64 or 128
+  uint32_t page_magic, page_shift;  // t / page_size = t * page_magic >> page_shift, t < 2^31
   int64_t blocks;
   float *part, *part_ml;
   long long wait_limit;  // pipeline wait limit in cycles (0: the default ~2 s)

@@ -367,11 +367,15 @@ void paged_plan(PagedParams& p) {
   const int64_t tile = p.k_scale ? kPagedTile8 : kTile, warp_rows = tile / kWarps;
   p.box_rows = std::gcd((int)warp_rows, p.page_size);
   // (a copy's place in shared memory is a multiple of 128 bytes, so boxes of one row of 8-bit values take 128 columns)
+  int bits = 0;  // 2^(bits - 1) < page_size <= 2^bits; the quotient's excess, below 2^-31, never reaches a whole number
+  while ((int64_t(1) << bits) < p.page_size) ++bits;
+  p.page_shift = 31 + bits;
+  p.page_magic = (uint32_t)(((uint64_t(1) << p.page_shift) + p.page_size - 1) / p.page_size);
   p.cols = p.dim > 64 || (p.k_scale && p.box_rows == 1) ? 128 : 64;
   int64_t tiles = (p.max_len + tile - 1) / tile;  // most that an item can have
   if (p.window) tiles = std::min(tiles, (p.sinks + tile - 1) / tile + (p.window + warp_rows - 1 + tile - 1) / tile);
   p.whole_items = tiles <= kMinTiles;
-  p.blocks = p.whole_items ? (int64_t)p.batch * p.items : 2 * 148;
+  p.blocks = p.whole_items ? (int64_t)p.batch * p.items : (p.k_scale && p.nt == 1 ? 3 : 2) * 148;
 }
 
 int64_t paged_workspace(const PagedParams& p) {

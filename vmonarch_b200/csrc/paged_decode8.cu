@@ -35,7 +35,8 @@ static_assert(kRows == 32, "a lane a token");
 
 template <int DP, int NT>
 struct Cfg {
-  static constexpr int STAGES = DP == 128 ? 3 : 6;
+  static constexpr int BLOCKS = NT == 1 ? 3 : 2;     // an SM: registers and shared memory for as many
+  static constexpr int STAGES = (DP == 128 ? 1 : 2) * (BLOCKS == 3 ? 2 : 3);
   static constexpr int MAT = kRows * DP;             // a warp's keys or values: rows of DP bytes, swizzled
   static constexpr int STAGE = 2 * MAT;
   static constexpr int RING = kWarps * STAGES * STAGE;
@@ -43,7 +44,7 @@ struct Cfg {
   static constexpr int JOIN = kWarps * 4 * LD * 4 + kWarps * 4 * 2 * 4;  // accumulators, (max, sum)
   static constexpr int SCALES = kWarps * STAGES * 2 * kRows * 4;
   static constexpr int SMEM = RING + JOIN + SCALES + kWarps * STAGES * 8 + 16;  // + barriers, abort flag
-  static_assert(2 * (SMEM + 1024) <= 233472, "two blocks per SM");
+  static_assert(BLOCKS * (SMEM + 1024) <= 233472, "shared memory of an SM");
 };
 
 // Two e4m3 values (the low or high half of x) as two fp16, exactly.
@@ -79,7 +80,7 @@ struct KParams {
 };
 
 template <typename T, int DP, int NT, bool WIN>
-__global__ void __launch_bounds__(32 * kWarps, 2) paged_decode8_kernel(const __grid_constant__ KParams kp) {
+__global__ void __launch_bounds__(32 * kWarps, Cfg<DP, NT>::BLOCKS) paged_decode8_kernel(const __grid_constant__ KParams kp) {
   using C = Cfg<DP, NT>;
   constexpr int KS = DP / 16;
   constexpr int HEADS = 8 * NT;
@@ -93,7 +94,6 @@ __global__ void __launch_bounds__(32 * kWarps, 2) paged_decode8_kernel(const __g
   const uint32_t bar0 = smem_u32(smem + C::RING + C::JOIN + C::SCALES) + 8u * warp * C::STAGES;
   volatile int* abort = reinterpret_cast<int*>(smem + C::RING + C::JOIN + C::SCALES + kWarps * C::STAGES * 8);
 
-  let_next_kernel_start();
   if (lane == 0) {
     if (warp == 0) *abort = 0;
     for (int s = 0; s < C::STAGES; ++s) mbar_init(bar0 + 8u * s, 1);
@@ -102,6 +102,9 @@ __global__ void __launch_bounds__(32 * kWarps, 2) paged_decode8_kernel(const __g
     prefetch_tmap(&kp.tm_v);
   }
   __syncthreads();
+  // the join reads the lengths before it waits: it may start once every block here knows that all before this kernel is done
+  wait_for_kernel_before();
+  let_next_kernel_start();
   Cursor cc;
   if (p.whole_items) {  // one block per item (short caches): no cut, no join
     cc.seq = blockIdx.x / p.items;
@@ -123,6 +126,16 @@ __global__ void __launch_bounds__(32 * kWarps, 2) paged_decode8_kernel(const __g
   if (p.hold_loads && warp == 0) lc.left = 0;
   int issued = 0;
   int page, slot;  // of this lane's token of the stage that is issued next
+  // of the item that is loaded: its key head, page table row and scales
+  int head;
+  const int32_t* table;
+  const float *k_scales, *v_scales;
+  auto enter = [&]() {
+    head = lc.item / p.chunks;
+    table = p.table + (int64_t)lc.seq * p.table_stride;
+    k_scales = p.k_scale + head * p.ks_head;
+    v_scales = p.v_scale + head * p.vs_head;
+  };
   auto look_up = [&](const Cursor& c) {
     const int t = c.token<WIN, kTile>() + kRows * warp + lane;
     page = p.num_pages;  // outside the map: zeros
@@ -131,9 +144,9 @@ __global__ void __launch_bounds__(32 * kWarps, 2) paged_decode8_kernel(const __g
     bool wanted = t < c.len;
     if (WIN) wanted = wanted && (sees(c, t) || (t & ~(p.box_rows - 1)) + p.box_rows > c.len - p.window);
     if (wanted) {
-      const int i = t / p.page_size;
+      const int i = (int)((uint64_t)t * p.page_magic >> p.page_shift);
       slot = t - i * p.page_size;
-      page = p.table[(int64_t)c.seq * p.table_stride + i];
+      page = table[i];
       if ((unsigned)page >= (unsigned)p.num_pages) page = p.num_pages;
     }
   };
@@ -144,21 +157,26 @@ __global__ void __launch_bounds__(32 * kWarps, 2) paged_decode8_kernel(const __g
       if (lane == 0) mbar_expect_tx(bar, C::STAGE);
       ++issued;
       __syncwarp();
-      const int head = lc.item / p.chunks;
       if ((lane & (p.box_rows - 1)) == 0) {
         tma_load(st + lane * DP, &kp.tm_k, 0, slot, BIdx(head, page, 0), bar);
         tma_load(st + C::MAT + lane * DP, &kp.tm_v, 0, slot, BIdx(head, page, 0), bar);
       }
       const bool valid = page < p.num_pages;
       const int from = valid ? page : 0;
-      cp_async4(sc, p.k_scale + from * p.ks_page + head * p.ks_head, valid);
-      cp_async4(sc + 4 * kRows, p.v_scale + from * p.vs_page + head * p.vs_head, valid);
+      cp_async4(sc, k_scales + from * p.ks_page, valid);
+      cp_async4(sc + 4 * kRows, v_scales + from * p.vs_page, valid);
       advance<WIN, kTile>(p, lc);
-      if (lc.left > 0) look_up(lc);
+      if (lc.left > 0) {
+        if (lc.tile == 0) enter();
+        look_up(lc);
+      }
     }
     cp_async_commit();  // a group a stage, also behind the last
   };
-  if (lc.left > 0) look_up(lc);
+  if (lc.left > 0) {
+    enter();
+    look_up(lc);
+  }
 #pragma unroll
   for (int s = 0; s < C::STAGES - 1; ++s) issue(s);
 
@@ -270,22 +288,28 @@ __global__ void __launch_bounds__(32 * kWarps, 2) paged_decode8_kernel(const __g
       for (int nt = 0; nt < NT; ++nt) {
         // i: rows lane / 4 + 8 i; e: heads 2 (lane % 4) + e
         float x[4][2], y[4][2];  // scores, and those that weigh the values, with their scale
-        float over = -1.f;
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             x[i][e] = s[nt][i >> 1][(i & 1) * 2 + e] * (qs[nt][e] * k_by[i]);
             y[i][e] = x[i][e] + v_log[i];
-            if (!((rows >> (lane / 4 + 8 * i)) & 1u)) x[i][e] = y[i][e] = -INFINITY;
-            over = fmaxf(fmaxf(x[i][e] - m[nt][e], y[i][e] - mv[nt][e]), over);
           }
-        if (__any_sync(0xffffffffu, over > kRaise)) {
-          float mx[2], my[2], al[2];
+        if (rows != 0xffffffffu) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (!((rows >> (lane / 4 + 8 * i)) & 1u)) x[i][0] = y[i][0] = x[i][1] = y[i][1] = -INFINITY;
+        }
+        float mx[2], my[2], al[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          mx[e] = fmaxf(fmaxf(x[0][e], x[1][e]), fmaxf(x[2][e], x[3][e]));
+          my[e] = fmaxf(fmaxf(y[0][e], y[1][e]), fmaxf(y[2][e], y[3][e]));
+        }
+        if (__any_sync(0xffffffffu, fmaxf(fmaxf(mx[0] - m[nt][0], my[0] - mv[nt][0]), fmaxf(mx[1] - m[nt][1], my[1] - mv[nt][1])) >
+                                        kRaise)) {
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            mx[e] = fmaxf(fmaxf(x[0][e], x[1][e]), fmaxf(x[2][e], x[3][e]));
-            my[e] = fmaxf(fmaxf(y[0][e], y[1][e]), fmaxf(y[2][e], y[3][e]));
 #pragma unroll
             for (int w = 4; w < 32; w <<= 1) {
               mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], w));
@@ -407,8 +431,7 @@ cudaError_t launch(const PagedParams& p, cudaStream_t st) {
   static std::atomic<uint64_t> ready{0};
   cudaError_t e = allow_smem(kern, C::SMEM, ready);
   if (e != cudaSuccess) return e;
-  kern<<<(unsigned)p.blocks, 32 * kWarps, C::SMEM, st>>>(kp);  // (not launched early: see paged_decode.cu)
-  e = cudaGetLastError();
+  e = launch_early(kern, p.blocks, 32 * kWarps, C::SMEM, st, kp);
   if (e != cudaSuccess || p.whole_items) return e;
   return launch_early(paged_join_kernel<T, DP, NT, WIN, kTile>, (int64_t)p.batch * p.join_blocks, 512, 0, st, p);
 }
