@@ -85,13 +85,14 @@ def test_cut_units():
 
 
 def test_a_long_window_is_causal_attention():
-    """Where the window takes in everything: the same up to the split of the work, which is the same here."""
+    """Where the window takes in everything: the same but for the order of 64 numbers' sum (64 roundings of 2^-24, so 2^-18 of l,
+    lse and what is made of them), which moves a result to its neighbour at most: one step, 2 u."""
     q, k, v, do = make([300, 40], [300, 700], 4, 2, 64, torch.bfloat16)
     seqs = PackedSequences([300, 40], [300, 700])
     want = grads(lambda *x: packed_attention(*x, seqs, causal=True), (q, k, v), do)
     for window, sinks in ((700, 0), (699, 1), (10 ** 12, 3)):
         for a, b in zip(grads(own(seqs, window, sinks), (q, k, v), do), want):
-            assert torch.equal(a, b)
+            assert rel(a, b) <= 2 * U[torch.bfloat16]
 
 
 @pytest.mark.parametrize("scale", [0.0, 3.0])

@@ -545,35 +545,45 @@ __global__ void __launch_bounds__(kThreads, 1) packed_fwd_kernel(const __grid_co
           for (int hf = 0; hf < 2; ++hf) {
             uint32_t pk[32];
             if constexpr (WIN) {
-              // which of the half's keys this query sees, 32 keys at a time: a warp computes only those that one of its
-              // queries sees
+              // 32 keys at a time: which of them this query sees, and whether the warp's queries see none or all of them
               const int kh = k0 + 64 * hf;
-              const uint32_t seen0 = seen32(kh, my_lo, my_lim, p.a.sinks), seen1 = seen32(kh + 32, my_lo, my_lim, p.a.sinks);
-              const bool any0 = __any_sync(0xffffffffu, seen0 != 0), any1 = __any_sync(0xffffffffu, seen1 != 0);
-              const bool all = __all_sync(0xffffffffu, (seen0 & seen1) == 0xffffffffu);
+              uint32_t seen[2];
+              bool any[2], all[2];
+#pragma unroll
+              for (int c = 0; c < 2; ++c) {
+                seen[c] = seen32(kh + 32 * c, my_lo, my_lim, p.a.sinks);
+                any[c] = __any_sync(0xffffffffu, seen[c] != 0);
+                all[c] = __all_sync(0xffffffffu, seen[c] == 0xffffffffu);
+              }
 #pragma unroll
               for (int e = 0; e < 32; ++e) pk[e] = 0u;
-              if (any0 || any1) {
-                uint32_t s[64];
-                tmem_ld32(tS + 64 * hf, s);
-                tmem_ld32(tS + 64 * hf + 32, s + 32);
-                tmem_wait_ld();
-                const uint32_t(&s0)[32] = *reinterpret_cast<const uint32_t(*)[32]>(&s[0]);
-                const uint32_t(&s1)[32] = *reinterpret_cast<const uint32_t(*)[32]>(&s[32]);
-                uint32_t(&p0)[16] = *reinterpret_cast<uint32_t(*)[16]>(&pk[0]);
-                uint32_t(&p1)[16] = *reinterpret_cast<uint32_t(*)[16]>(&pk[16]);
-                auto top = [&]() { return fmaxf(row_max_bits(s0, seen0), row_max_bits(s1, seen1)) * p.scale_log2; };
+              if (any[0] || any[1]) {
+                // (scores are loaded again where they are needed again: 64 of them beside the rest would spill)
+                auto top = [&]() {
+                  float mx = -1e30f;
+#pragma unroll
+                  for (int c = 0; c < 2; ++c) {
+                    uint32_t s[32];
+                    tmem_ld32(tS + 64 * hf + 32 * c, s);
+                    tmem_wait_ld();
+                    mx = fmaxf(mx, row_max_bits(s, seen[c]));
+                  }
+                  return fmaxf(mx * p.scale_log2, -1e30f);
+                };
                 // (a query that sees none of these keys keeps the reference of no key)
-                if (hf == 0 && t == 0) m_ref = fmaxf(m_ref, all ? row_max<64, false>(s, 64) * p.scale_log2 : top());
+                if (hf == 0 && t == 0) m_ref = fmaxf(m_ref, top());
                 float lt = 0.f;
 #pragma unroll 1
                 for (int pass = 0; pass < 2; ++pass) {
-                  if (all) {
-                    lt = probs<T, 64, false>(s, pk, p.scale_log2, m_ref, 64);
-                  } else {
-                    lt = 0.f;
-                    if (any0) lt = probs_bits<T>(s0, p0, p.scale_log2, m_ref, seen0);
-                    if (any1) lt += probs_bits<T>(s1, p1, p.scale_log2, m_ref, seen1);
+                  lt = 0.f;
+#pragma unroll
+                  for (int c = 0; c < 2; ++c) {
+                    if (!any[c]) continue;
+                    uint32_t s[32];
+                    uint32_t(&pc)[16] = *reinterpret_cast<uint32_t(*)[16]>(&pk[16 * c]);
+                    tmem_ld32(tS + 64 * hf + 32 * c, s);
+                    tmem_wait_ld();
+                    lt += all[c] ? probs<T, 32, false>(s, pc, p.scale_log2, m_ref, 32) : probs_bits<T>(s, pc, p.scale_log2, m_ref, seen[c]);
                   }
                   if (pass || !__any_sync(0xffffffffu, live && !(lt <= kSumThreshold))) break;
                   if (hf == 1 && !(ok = warp_wait(B_PVH + w, steps & 1, 16))) break;
