@@ -416,12 +416,16 @@ int vmb_copy_pages(const vmb_pages* k, const vmb_pages* v, const int32_t* src, c
  * scale becomes the larger of s and what it was, and where it grows the page's other slots are brought to it (rounded to
  * nearest). Rows are divided by the scale and rounded to nearest even; infinities and NaN become NaN. The rows that go into
  * one page have to follow one another in the call, skipped ones not between them. */
-int vmb_append_pages_e4m3(const vmb_rows* k_new, const vmb_rows* v_new, const vmb_pages* k, const vmb_pages* v,
-                          const vmb_page_scales* k_scale, const vmb_page_scales* v_scale, const int32_t* slots, int64_t count,
-                          int64_t num_pages, int32_t kv_heads, int32_t dim, int32_t page_size, int32_t dtype, void* stream);
-int vmb_copy_pages_e4m3(const vmb_pages* k, const vmb_pages* v, const vmb_page_scales* k_scale, const vmb_page_scales* v_scale,
-                        const int32_t* src, const int32_t* dst, int64_t count, int64_t num_pages, int32_t kv_heads, int32_t dim,
-                        int32_t page_size, void* stream);
+typedef struct vmb_move_e4m3_args {
+  vmb_rows k_new, v_new;             /* append */
+  vmb_pages k, v;
+  vmb_page_scales k_scale, v_scale;
+  const int32_t *src, *dst;          /* copy: pages; append: dst are the slots */
+  int64_t count, num_pages;
+  int32_t kv_heads, dim, page_size, dtype;  /* dtype: of appended rows */
+} vmb_move_e4m3_args;
+int vmb_append_pages_e4m3(const vmb_move_e4m3_args* a, void* stream);
+int vmb_copy_pages_e4m3(const vmb_move_e4m3_args* a, void* stream);
 
 /*
  * The book of a paged cache on the device (no reference counterpart): sequence b of lengths[b] tokens holds

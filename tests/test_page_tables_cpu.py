@@ -11,7 +11,8 @@ from test_ops_capi import HEADER
 from vmonarch_b200 import PagedKVCache, PageTables, append_pages, copy_pages, paged_attention, reserve_pages, truncate_pages
 from vmonarch_b200 import _native as N
 
-STRUCTS = {"vmb_page_scales": N.PageScales, "vmb_cache_args": N.CacheArgs, "vmb_page_book": N.PageBook}
+STRUCTS = {"vmb_page_scales": N.PageScales, "vmb_cache_args": N.CacheArgs, "vmb_page_book": N.PageBook,
+           "vmb_move_e4m3_args": N.MoveE4m3Args}
 E4M3 = torch.float8_e4m3fn
 
 
@@ -86,18 +87,24 @@ def test_cache_attention_refusals(args, cache, code):
     assert N.lib.vmb_cache_attention(paged(**args), ctypes.byref(c), None) == code and N.lib.vmb_last_error()
 
 
-def test_e4m3_move_refusals():
+def move8(**over):
     r, p, s = N.Rows(256, 128, 64), N.Pages(256, 2048, 1024, 64), N.PageScales(256, 2, 1)
-    ok = [r, r, p, p, s, s, 256, 3, 10, 2, 64, 16, 0]
-    for at, bad, code in ((0, N.Rows(8, 128, 64), 1), (2, N.Pages(256, 2048, 1024, 72), 1), (4, N.PageScales(None, 2, 1), 1),
-                          (5, N.PageScales(256, -1, 1), 1), (6, None, 1), (7, -1, 1), (8, 0, 1), (10, 40, 2), (10, 144, 2), (12, 2, 1)):
-        args = list(ok)
-        args[at] = bad
-        assert N.lib.vmb_append_pages_e4m3(*args, None) == code
-    for at, bad, code in ((0, N.Pages(264, 2048, 1024, 64), 1), (2, N.PageScales(None, 2, 1), 1), (4, None, 1), (5, None, 1), (9, 40, 2)):
-        args = [p, p, s, s, 256, 256, 3, 10, 2, 64, 16]
-        args[at] = bad
-        assert N.lib.vmb_copy_pages_e4m3(*args, None) == code
+    a = N.MoveE4m3Args(r, r, p, p, s, s, 256, 256, 3, 10, 2, 64, 16, 0)
+    for k, v in over.items():
+        setattr(a, k, v)
+    return ctypes.byref(a)
+
+
+def test_e4m3_move_refusals():
+    both = [(dict(k=N.Pages(256, 2048, 1024, 72)), 1), (dict(v=N.Pages(264, 2048, 1024, 64)), 1), (dict(k_scale=N.PageScales(None, 2, 1)), 1),
+            (dict(v_scale=N.PageScales(256, -1, 1)), 1), (dict(dst=None), 1), (dict(count=-1), 1), (dict(num_pages=0), 1),
+            (dict(dim=40), 2), (dict(dim=144), 2)]
+    for over, code in both + [(dict(k_new=N.Rows(8, 128, 64)), 1), (dict(v_new=N.Rows(None, 128, 64)), 1), (dict(dtype=2), 1)]:
+        assert N.lib.vmb_append_pages_e4m3(move8(**over), None) == code and N.lib.vmb_last_error()
+    for over, code in both + [(dict(src=None), 1)]:
+        assert N.lib.vmb_copy_pages_e4m3(move8(**over), None) == code and N.lib.vmb_last_error()
+    assert N.lib.vmb_append_pages_e4m3(None, None) == N.lib.vmb_copy_pages_e4m3(None, None) == 1
+    assert N.lib.vmb_append_pages_e4m3(move8(count=0), None) == N.lib.vmb_copy_pages_e4m3(move8(count=0), None) == 0
 
 
 def test_page_tables_start_empty():

@@ -152,6 +152,12 @@ class CacheArgs(ctypes.Structure):
     _fields_ = [("k_scale", PageScales), ("v_scale", PageScales), ("window", c_i32), ("sinks", c_i32)]
 
 
+class MoveE4m3Args(ctypes.Structure):
+    _fields_ = [("k_new", Rows), ("v_new", Rows), ("k", Pages), ("v", Pages), ("k_scale", PageScales), ("v_scale", PageScales),
+                ("src", c_vp), ("dst", c_vp), ("count", c_i64), ("num_pages", c_i64),
+                ("kv_heads", c_i32), ("dim", c_i32), ("page_size", c_i32), ("dtype", c_i32)]
+
+
 class PageBook(ctypes.Structure):
     _fields_ = [("table", c_vp), ("lengths", c_vp), ("free_pages", c_vp), ("num_free", c_vp), ("failed", c_vp),
                 ("table_stride", c_i64), ("batch", c_i64), ("table_width", c_i64), ("num_pages", c_i64), ("page_size", c_i32)]
@@ -212,11 +218,8 @@ SIGNATURES = {
     "vmb_truncate_pages": (ctypes.c_int, [ctypes.POINTER(PageBook), c_vp, c_vp, c_i64, c_vp]),
     "vmb_cache_workspace_bytes": (c_i64, [ctypes.POINTER(PagedArgs), ctypes.POINTER(CacheArgs)]),
     "vmb_cache_attention": (ctypes.c_int, [ctypes.POINTER(PagedArgs), ctypes.POINTER(CacheArgs), c_vp]),
-    "vmb_append_pages_e4m3": (ctypes.c_int, [ctypes.POINTER(Rows), ctypes.POINTER(Rows), ctypes.POINTER(Pages),
-                                             ctypes.POINTER(Pages), ctypes.POINTER(PageScales), ctypes.POINTER(PageScales),
-                                             c_vp, c_i64, c_i64, c_i32, c_i32, c_i32, c_i32, c_vp]),
-    "vmb_copy_pages_e4m3": (ctypes.c_int, [ctypes.POINTER(Pages), ctypes.POINTER(Pages), ctypes.POINTER(PageScales),
-                                           ctypes.POINTER(PageScales), c_vp, c_vp, c_i64, c_i64, c_i32, c_i32, c_i32, c_vp]),
+    "vmb_append_pages_e4m3": (ctypes.c_int, [ctypes.POINTER(MoveE4m3Args), c_vp]),
+    "vmb_copy_pages_e4m3": (ctypes.c_int, [ctypes.POINTER(MoveE4m3Args), c_vp]),
     "vmb_append_pages": (ctypes.c_int, [ctypes.POINTER(Rows), ctypes.POINTER(Rows), ctypes.POINTER(Pages),
                                         ctypes.POINTER(Pages), c_vp, c_i64, c_i64, c_i32, c_i32, c_i32, c_vp]),
     "vmb_copy_pages": (ctypes.c_int, [ctypes.POINTER(Pages), ctypes.POINTER(Pages), c_vp, c_vp, c_i64, c_i64, c_i32,

@@ -94,10 +94,10 @@ int move_params(const char* what, const vmb_pages* k, const vmb_pages* v, const 
   return VMB_OK;
 }
 
-int scale_params(const char* what, const vmb_page_scales* k, const vmb_page_scales* v, vmb::PageMoveParams& p) {
-  if (!k || !v || !scales_ok(*k) || !scales_ok(*v)) return set_error(VMB_EINVAL, "%s: e4m3 pools need scales", what);
-  p.k_scale = k->ptr; p.ks_page = k->page; p.ks_head = k->head;
-  p.v_scale = v->ptr; p.vs_page = v->page; p.vs_head = v->head;
+int scale_params(const char* what, const vmb_page_scales& k, const vmb_page_scales& v, vmb::PageMoveParams& p) {
+  if (!scales_ok(k) || !scales_ok(v)) return set_error(VMB_EINVAL, "%s: e4m3 pools need scales", what);
+  p.k_scale = k.ptr; p.ks_page = k.page; p.ks_head = k.head;
+  p.v_scale = v.ptr; p.vs_page = v.page; p.vs_head = v.head;
   return VMB_OK;
 }
 
@@ -166,33 +166,30 @@ int vmb_copy_pages(const vmb_pages* k, const vmb_pages* v, const int32_t* src, c
   return cuda_rc(vmb::copy_pages(p, static_cast<cudaStream_t>(stream)), "vmb_copy_pages");
 }
 
-int vmb_append_pages_e4m3(const vmb_rows* k_new, const vmb_rows* v_new, const vmb_pages* k, const vmb_pages* v,
-                          const vmb_page_scales* k_scale, const vmb_page_scales* v_scale, const int32_t* slots, int64_t count,
-                          int64_t num_pages, int32_t kv_heads, int32_t dim, int32_t page_size, int32_t dtype, void* stream) {
+int vmb_append_pages_e4m3(const vmb_move_e4m3_args* a, void* stream) {
   const char* what = "vmb_append_pages_e4m3";
   vmb::PageMoveParams p{};
-  if (count == 0) return VMB_OK;
-  if (dtype != VMB_DTYPE_BF16 && dtype != VMB_DTYPE_F16) return set_error(VMB_EINVAL, "%s: unknown dtype %d", what, dtype);
-  int rc = move_params(what, k, v, slots, count, num_pages, kv_heads, dim, page_size, p, true);
-  if (rc || (rc = scale_params(what, k_scale, v_scale, p))) return rc;
-  if (!k_new || !v_new || !rows_ok(*k_new) || !rows_ok(*v_new))
-    return set_error(VMB_EINVAL, "%s: new rows need 16-byte alignment", what);
-  p.k_src = k_new->ptr; p.v_src = v_new->ptr;
-  p.k_row = k_new->row; p.k_shead = k_new->head; p.v_row = v_new->row; p.v_shead = v_new->head;
+  if (!a) return set_error(VMB_EINVAL, "%s: null args", what);
+  if (a->count == 0) return VMB_OK;
+  if (a->dtype != VMB_DTYPE_BF16 && a->dtype != VMB_DTYPE_F16) return set_error(VMB_EINVAL, "%s: unknown dtype %d", what, a->dtype);
+  int rc = move_params(what, &a->k, &a->v, a->dst, a->count, a->num_pages, a->kv_heads, a->dim, a->page_size, p, true);
+  if (rc || (rc = scale_params(what, a->k_scale, a->v_scale, p))) return rc;
+  if (!rows_ok(a->k_new) || !rows_ok(a->v_new)) return set_error(VMB_EINVAL, "%s: new rows need 16-byte alignment", what);
+  p.k_src = a->k_new.ptr; p.v_src = a->v_new.ptr;
+  p.k_row = a->k_new.row; p.k_shead = a->k_new.head; p.v_row = a->v_new.row; p.v_shead = a->v_new.head;
   vmb::count_launches(1);
-  return cuda_rc(vmb::append_pages_e4m3(p, dtype == VMB_DTYPE_BF16, static_cast<cudaStream_t>(stream)), what);
+  return cuda_rc(vmb::append_pages_e4m3(p, a->dtype == VMB_DTYPE_BF16, static_cast<cudaStream_t>(stream)), what);
 }
 
-int vmb_copy_pages_e4m3(const vmb_pages* k, const vmb_pages* v, const vmb_page_scales* k_scale, const vmb_page_scales* v_scale,
-                        const int32_t* src, const int32_t* dst, int64_t count, int64_t num_pages, int32_t kv_heads, int32_t dim,
-                        int32_t page_size, void* stream) {
+int vmb_copy_pages_e4m3(const vmb_move_e4m3_args* a, void* stream) {
   const char* what = "vmb_copy_pages_e4m3";
   vmb::PageMoveParams p{};
-  if (count == 0) return VMB_OK;
-  int rc = move_params(what, k, v, dst, count, num_pages, kv_heads, dim, page_size, p, true);
-  if (rc || (rc = scale_params(what, k_scale, v_scale, p))) return rc;
-  if (!src) return set_error(VMB_EINVAL, "%s: null source list", what);
-  p.src = src;
+  if (!a) return set_error(VMB_EINVAL, "%s: null args", what);
+  if (a->count == 0) return VMB_OK;
+  int rc = move_params(what, &a->k, &a->v, a->dst, a->count, a->num_pages, a->kv_heads, a->dim, a->page_size, p, true);
+  if (rc || (rc = scale_params(what, a->k_scale, a->v_scale, p))) return rc;
+  if (!a->src) return set_error(VMB_EINVAL, "%s: null source list", what);
+  p.src = a->src;
   vmb::count_launches(1);
   return cuda_rc(vmb::copy_pages_e4m3(p, static_cast<cudaStream_t>(stream)), what);
 }

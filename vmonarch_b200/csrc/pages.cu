@@ -10,6 +10,7 @@
 // run of them belongs to one team of warps: largest value, scale, the page brought to it where it grows, rows divided and
 // stored, in one pass and without atomics.
 #include <algorithm>
+#include <type_traits>
 
 #include "common.cuh"
 #include "launch.h"
@@ -76,15 +77,59 @@ __device__ __forceinline__ float pow2_scale(float top) {
   return __uint_as_float((uint32_t)max(e, 1) << 23);
 }
 
+__device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("max.u16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+// Four 16-bit words' pairs as e4m3, divided by a scale. POW2: times its inverse, exact in bf16 (fp16's exponents do not reach).
+template <typename T, bool POW2>
+__device__ __forceinline__ uint2 quantized(uint4 x, float scale, float inv) {
+  const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+  uint32_t q[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float2 f;
+    if (POW2 && Elem<T>::is_bf16) {
+      const __nv_bfloat162 y = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&w[i]), __floats2bfloat162_rn(inv, inv));
+      f = Elem<T>::unpack(*reinterpret_cast<const uint32_t*>(&y));
+    } else {
+      f = Elem<T>::unpack(w[i]);
+      f = POW2 ? make_float2(f.x * inv, f.y * inv) : make_float2(f.x / scale, f.y / scale);
+    }
+    q[i] = pack_e4m3x2(f.x, f.y);
+  }
+  return make_uint2(q[0] | q[1] << 16, q[2] | q[3] << 16);
+}
+
 // A team of TW warps (a warp, or the block) takes the runs that begin in its `group` rows, for one head and tensor.
 template <typename T, int TW>
-__global__ void __launch_bounds__(32 * kTeamWarps) append_e4m3_kernel(const __grid_constant__ PageMoveParams p) {
-  __shared__ float tops[2][kTeamWarps];
+__global__ void __launch_bounds__(32 * kTeamWarps, 6) append_e4m3_kernel(const __grid_constant__ PageMoveParams p) {
+  __shared__ uint32_t tops[2][kTeamWarps];
+  constexpr uint32_t kInf = Elem<T>::is_bf16 ? 0x7f80u : 0x7c00u;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t team = TW == 1 ? (int64_t)blockIdx.x * kTeamWarps + warp : blockIdx.x;
   const int pairs = 2 * p.kv_heads;
   const int64_t row0 = team / pairs * p.group;
   if (row0 >= p.count) return;
+  // (group <= 32: a lane looks at a row; page -1: skipped, or past the last row)
+  auto look_at = [&](int64_t row, int& page, int& slot) {
+    page = slot = -1;
+    const int s = row >= 0 && row < p.count ? p.dst[row] : -1;
+    if (s < 0) return;
+    page = s / p.page_size;
+    slot = s - page * p.page_size;
+    if (page >= p.num_pages) page = -1;
+  };
+  int mine, my_slot, before, unused;
+  look_at(row0 + lane, mine, my_slot);
+  look_at(row0 - 1, before, unused);
+  const int above = __shfl_up_sync(0xffffffffu, mine, 1);
+  if (lane > 0) before = above;
+  unsigned starts = __ballot_sync(0xffffffffu, lane < p.group && mine >= 0 && mine != before);
+  if (!starts) return;
+  const unsigned same = __ballot_sync(0xffffffffu, mine >= 0 && mine == before);
+  const unsigned firsts = __ballot_sync(0xffffffffu, my_slot == 0);
   const int pair = (int)(team % pairs), head = pair >> 1;
   const bool is_v = pair & 1;
   const T* src = static_cast<const T*>(is_v ? p.v_src : p.k_src) + head * (is_v ? p.v_shead : p.k_shead);
@@ -100,77 +145,69 @@ __global__ void __launch_bounds__(32 * kTeamWarps) append_e4m3_kernel(const __gr
   const bool live = c < p.dim;
   const int step = TW == 1 ? lane : threadIdx.x;
   int turn = 0;
-  auto page_of = [&](int64_t row) -> int {  // -1: skipped, or past the last row
-    if (row < 0 || row >= p.count) return -1;
-    const int s = p.dst[row];
-    if (s < 0) return -1;
-    const int page = s / p.page_size;
-    return page < p.num_pages ? page : -1;
-  };
-  // (group <= 32: a lane looks at a row)
-  const int mine = page_of(row0 + lane), before = page_of(row0 + lane - 1);
-  unsigned starts = __ballot_sync(0xffffffffu, lane < p.group && mine >= 0 && mine != before);
-  const unsigned same = __ballot_sync(0xffffffffu, mine >= 0 && mine == before);
   for (; starts; starts &= starts - 1) {
     const int s = __ffs(starts) - 1, page = __shfl_sync(0xffffffffu, mine, s);
     const int64_t first = row0 + s;
     int n = __ffs(~((same >> s) >> 1));  // rows of the run among the 32
-    if (s + n > 31) {                     // up to the last of them: it may go on
+    bool begins = (firsts >> s & (n >= 32 ? 0xffffffffu : (1u << n) - 1u)) != 0;  // slot 0 of the page is among the rows
+    if (s + n > 31) {                    // up to the last of them: it may go on
       n = 32 - s;
       for (;;) {
-        const unsigned other = ~__ballot_sync(0xffffffffu, page_of(first + n + lane) == page);
-        if (other) {
-          n += __ffs(other) - 1;
-          break;
-        }
-        n += 32;
+        int next, slot;
+        look_at(first + n + lane, next, slot);
+        const unsigned other = ~__ballot_sync(0xffffffffu, next == page);
+        const int more = other ? __ffs(other) - 1 : 32;
+        begins |= __any_sync(0xffffffffu, lane < more && slot == 0);
+        n += more;
+        if (other) break;
       }
     }
+    float* scale_at = scales + page * scale_page;
+    const float old = *scale_at;
     uint4 x[kHeld];
-    bool begins = false;  // slot 0 of the page is among the rows
+    const T* from = src + (first + at) * src_row + c;
     auto load = [&](int r0) {
 #pragma unroll
       for (int u = 0; u < kHeld; ++u) {
-        const int r = r0 + u * per + at;
         x[u] = make_uint4(0u, 0u, 0u, 0u);
-        if (r < n && live) x[u] = load16(src, (first + r) * src_row + c);
+        if (r0 + u * per + at < n && live) x[u] = load16(from, (r0 + u * per) * src_row);
       }
     };
-    // the largest value; infinities, where there are any, left out (NaN are by fmaxf)
-    float top = 0.f;
-    auto largest = [&](bool finite) {
-      top = 0.f;
+    const bool held = n <= kHeld * per;
+    // the largest magnitude as 16 bits, whose order is that of the values; without what is not finite if asked for
+    auto largest = [&](bool finite) -> uint32_t {
+      uint32_t top = 0;
       for (int r0 = 0; r0 < n; r0 += kHeld * per) {
-        if (n > kHeld * per || r0 == 0 && !finite) load(r0);
+        if (!held) load(r0);
 #pragma unroll
         for (int u = 0; u < kHeld; ++u) {
           const uint32_t w[4] = {x[u].x, x[u].y, x[u].z, x[u].w};
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const float2 f = Elem<T>::unpack(w[i]);
-            const float a = fabsf(f.x), b = fabsf(f.y);
-            top = fmaxf(top, finite && a == INFINITY ? 0.f : a);
-            top = fmaxf(top, finite && b == INFINITY ? 0.f : b);
+            uint32_t a = w[i] & 0x7fff7fffu;
+            if (finite) {
+              if ((a & 0xffffu) >= kInf) a &= 0xffff0000u;
+              if (a >> 16 >= kInf) a &= 0xffffu;
+            }
+            top = max_u16x2(top, a);
           }
         }
       }
-      top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
+      top = __reduce_max_sync(0xffffffffu, max(top & 0xffffu, top >> 16));
       if (TW > 1) {
         if (lane == 0) tops[turn & 1][warp] = top;
         __syncthreads();
 #pragma unroll
-        for (int i = 0; i < kTeamWarps; ++i) top = fmaxf(top, tops[turn & 1][i]);
+        for (int i = 0; i < kTeamWarps; ++i) top = max(top, tops[turn & 1][i]);
         ++turn;
       }
+      return top;
     };
-    largest(false);
-    const bool infinite = top == INFINITY;
-    if (infinite) largest(true);
-    for (int r = lane; r < n; r += 32) begins |= p.dst[first + r] % p.page_size == 0;
-    begins = __any_sync(0xffffffffu, begins);
-    float* scale_at = scales + page * scale_page;
-    const float old = *scale_at, need = pow2_scale(top);
-    const float scale = begins ? need : fmaxf(old, need);
+    if (held) load(0);
+    uint32_t top = largest(false);
+    const bool infinite = top >= kInf;
+    if (infinite) top = largest(true);
+    const float need = pow2_scale(Elem<T>::unpack(top).x), scale = begins ? need : fmaxf(old, need);
     uint8_t* to = pool + page * dst_page;
     if (TW > 1) __syncthreads();  // everybody has read the scale
     else __syncwarp();
@@ -194,28 +231,38 @@ __global__ void __launch_bounds__(32 * kTeamWarps) append_e4m3_kernel(const __gr
       else __syncwarp();
     }
     if (step == 0) *scale_at = scale;
-    // a power of two is multiplied with (its inverse is one), any other scale, which a caller brought, divided by
+    // a power of two is multiplied with its inverse, which is exact; any other scale, which a caller brought, divides
     const bool pow2 = (__float_as_uint(scale) & 0x7fffffu) == 0;
     const float inv = 1.f / scale;
+    auto write = [&](auto exact) {
+#pragma unroll
+      for (int u = 0; u < kHeld; ++u) {
+        const int r = u * per + at;
+        const int slot = __shfl_sync(0xffffffffu, my_slot, (s + r) & 31);
+        if (r < n && live) *reinterpret_cast<uint2*>(to + slot * dst_slot + c) = quantized<T, decltype(exact)::value>(x[u], scale, inv);
+      }
+    };
+    if (held && s + n <= 32 && pow2 && !infinite) {
+      write(std::true_type{});
+      continue;
+    }
+#pragma unroll 1
     for (int r0 = 0; r0 < n; r0 += kHeld * per) {
-      if (n > kHeld * per) load(r0);
+      if (!held) load(r0);
 #pragma unroll
       for (int u = 0; u < kHeld; ++u) {
         const int r = r0 + u * per + at;
         if (r >= n || !live) continue;
-        const uint32_t w[4] = {x[u].x, x[u].y, x[u].z, x[u].w};
-        uint32_t q[4];
+        if (infinite) {  // to NaN: the conversion would make the largest value of an infinity
+          uint32_t* w = &x[u].x;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          float2 f = Elem<T>::unpack(w[i]);
-          if (infinite) {  // the conversion would make the largest value of them
-            if (isinf(f.x)) f.x = __int_as_float(0x7fffffff);
-            if (isinf(f.y)) f.y = __int_as_float(0x7fffffff);
+          for (int i = 0; i < 4; ++i) {
+            if ((w[i] & 0x7fffu) == kInf) w[i] |= 1u;
+            if ((w[i] >> 16 & 0x7fffu) == kInf) w[i] |= 0x10000u;
           }
-          q[i] = pow2 ? pack_e4m3x2(f.x * inv, f.y * inv) : pack_e4m3x2(f.x / scale, f.y / scale);
         }
-        const int slot = p.dst[first + r] % p.page_size;
-        *reinterpret_cast<uint2*>(to + slot * dst_slot + c) = make_uint2(q[0] | q[1] << 16, q[2] | q[3] << 16);
+        const int slot = p.dst[first + r] - page * p.page_size;
+        *reinterpret_cast<uint2*>(to + slot * dst_slot + c) = pow2 ? quantized<T, true>(x[u], scale, inv) : quantized<T, false>(x[u], scale, inv);
       }
     }
   }

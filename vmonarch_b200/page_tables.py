@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes
 import operator
+import struct
 
 import torch
 
@@ -20,27 +21,35 @@ _FAILURES = {1: "not enough free pages", 2: "a sequence is longer than its row o
 
 def _book(page_table, lengths, want, free_pages, num_free, page_size, failed):
     """vmb_page_book of the tensors, and their device."""
-    device = page_table.device
-    for t, name, dim in ((page_table, "page_table", 2), (lengths, "lengths", 1), (want, "counts or lengths to keep", 1),
-                         (free_pages, "free_pages", 1), (num_free, "num_free", 1)):
-        assert t.dtype == torch.int32 and t.dim() == dim and t.device == device, \
-            f"{name} must be int32, {dim}-dimensional and on the page table's device"
+    device, int32 = page_table.device, torch.int32
+    assert page_table.dtype == int32 and page_table.dim() == 2, "page_table must be int32 and 2-dimensional"
     batch, width = page_table.shape
+    assert lengths.dtype == int32 and lengths.device == device and lengths.shape == (batch,), \
+        "lengths must be int32, an entry per row of the page table and on its device"
+    assert want.dtype == int32 and want.device == device and want.shape == (batch,), \
+        "counts, or lengths to keep, must be int32, an entry per row of the page table and on its device"
+    assert free_pages.dtype == int32 and free_pages.device == device and free_pages.dim() == 1, \
+        "free_pages must be int32, 1-dimensional and on the page table's device"
+    assert num_free.dtype == int32 and num_free.device == device and num_free.shape == (1,), \
+        "num_free must be one int32 on the page table's device"
     stride, col = page_table.stride()
     assert width <= 1 or col == 1 and (batch <= 1 or stride >= width), "the page table's rows must be contiguous and apart"
-    assert lengths.size(0) == batch and want.size(0) == batch, "lengths and counts must have an entry per row of the page table"
-    num_pages = free_pages.size(0)
-    page_size = operator.index(page_size)
-    assert page_size >= 1 and num_pages >= 1 and num_free.size(0) == 1, "page_size and free_pages must not be empty, num_free one value"
+    num_pages, page_size = free_pages.size(0), operator.index(page_size)
+    assert page_size >= 1 and num_pages >= 1, "page_size and free_pages must not be empty"
     assert num_pages * page_size < 2 ** 31, "slots are 32-bit: the pool has too many"
-    for t, name in ((lengths, "lengths"), (free_pages, "free_pages")):
-        assert t.is_contiguous(), f"{name} must be contiguous: it is written in place"
+    assert lengths.is_contiguous() and free_pages.is_contiguous(), "lengths and free_pages are written in place and must be contiguous"
     if failed is not None:
-        assert failed.dtype == torch.int32 and failed.numel() == 1 and failed.device == device, "failed must be one int32 on the same device"
+        assert failed.dtype == int32 and failed.device == device and failed.numel() == 1, "failed must be one int32 on the same device"
     assert page_table.is_cuda, "the book must be on a CUDA device"
-    return N.PageBook(page_table.data_ptr(), lengths.data_ptr(), free_pages.data_ptr(), num_free.data_ptr(),
-                      None if failed is None else failed.data_ptr(), stride if batch > 1 else width, batch, width, num_pages,
-                      page_size), device
+    book = N.PageBook()
+    _BOOK.pack_into(book, 0, page_table.data_ptr(), lengths.data_ptr(), free_pages.data_ptr(), num_free.data_ptr(),
+                    0 if failed is None else failed.data_ptr(), stride if batch > 1 else width, batch, width, num_pages, page_size)
+    return book, device, batch, width
+
+
+# vmb_page_book
+_BOOK = struct.Struct("9qi")
+assert _BOOK.size <= ctypes.sizeof(N.PageBook)
 
 
 def _workspace(book, device):
@@ -69,12 +78,12 @@ def reserve_pages(page_table, lengths, counts, free_pages, num_free, *, page_siz
     A call that cannot be done changes nothing but `failed`, and its slots are -1. Nothing waits for the device. Pages have
     one owner here: forks and their shared pages are :class:`PagedKVCache`'s.
     """
-    book, device = _book(page_table, lengths, counts, free_pages, num_free, page_size, failed)
+    book, device, batch, _ = _book(page_table, lengths, counts, free_pages, num_free, page_size, failed)
     total = operator.index(total)
     assert 0 <= total < 2 ** 31, "total must be a number of rows"
     counts = counts.contiguous()
     slots = torch.empty(total, dtype=torch.int32, device=device)
-    ws, size = (None, 0) if book.batch <= 1024 and total <= 4096 else _workspace(book, device)
+    ws, size = (None, 0) if batch <= 1024 and total <= 4096 else _workspace(book, device)
     N.launch("vmb_reserve_pages", N.lib.vmb_reserve_pages, device, ctypes.byref(book), counts.data_ptr(), slots.data_ptr(), total,
              N.ptr(ws), size)
     return slots
@@ -90,11 +99,11 @@ def truncate_pages(page_table, lengths, keep, free_pages, num_free, *, page_size
         table holds, 4 a negative length, 8 more pages than free_pages has room for, which cannot be unless one was returned
         twice. Such a call changes nothing else.
     """
-    book, device = _book(page_table, lengths, keep, free_pages, num_free, page_size, failed)
-    if not book.batch:
+    book, device, batch, width = _book(page_table, lengths, keep, free_pages, num_free, page_size, failed)
+    if not batch:
         return
     keep = keep.contiguous()
-    ws, size = (None, 0) if book.batch <= 1024 and book.batch * book.table_width <= 65536 else _workspace(book, device)
+    ws, size = (None, 0) if batch <= 1024 and batch * width <= 65536 else _workspace(book, device)
     N.launch("vmb_truncate_pages", N.lib.vmb_truncate_pages, device, ctypes.byref(book), keep.data_ptr(), N.ptr(ws), size)
 
 

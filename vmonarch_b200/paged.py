@@ -47,9 +47,10 @@ def _check_pools(k_pages, v_pages, k_scale=None, v_scale=None):
         step = 16
         assert dtype == E4M3 and k_scale is not None and v_scale is not None, \
             "8-bit pools (torch.float8_e4m3fn), and no others, go with k_scale and v_scale"
-        for scale in (k_scale, v_scale):
-            assert scale.shape == (n, h) and scale.dtype == torch.float32 and scale.device == device, \
-                "scales must be (num_pages, Hk), float32 and on the pools' device"
+        each = (n, h)
+        assert k_scale.shape == each and k_scale.dtype == torch.float32 and k_scale.device == device and \
+            v_scale.shape == each and v_scale.dtype == torch.float32 and v_scale.device == device, \
+            "scales must be (num_pages, Hk), float32 and on the pools' device"
     assert 8 <= d <= MAX_DIM and d % step == 0, f"head dim {d} is not a multiple of {step} up to {MAX_DIM}"
     assert n >= 1 and h >= 1 and ps >= 1, "pools need at least one page, head and slot"
     assert k_pages.is_cuda and v_pages.device == device, "pools must be on one CUDA device"
@@ -63,8 +64,7 @@ def _check_index(t, name, dim, device):
 
 def _scales(t):
     """vmb_page_scales of a (num_pages, Hk) tensor."""
-    page, head = t.stride()
-    return N.PageScales(t.data_ptr(), page if t.size(0) > 1 else 0, head if t.size(1) > 1 else 0)
+    return t.data_ptr(), *t.stride()
 
 
 def paged_attention(q, k_pages, v_pages, page_table, lengths, *, k_scale=None, v_scale=None, window=None, sinks=0,
@@ -126,10 +126,8 @@ def paged_attention(q, k_pages, v_pages, page_table, lengths, *, k_scale=None, v
             size = N.lib.vmb_paged_workspace_bytes(*args)
         else:
             c = N.CacheArgs()
-            if k_scale is not None:
-                c.k_scale, c.v_scale = _scales(k_scale), _scales(v_scale)
-            if mask is not None:
-                c.window, c.sinks = mask
+            scales = _NO_SCALES if k_scale is None else (*_scales(k_scale), *_scales(v_scale))
+            _CACHE.pack_into(c, 0, *scales, *(mask or (0, 0)))
             name, args = "vmb_cache_attention", (ctypes.byref(a), ctypes.byref(c))
             size = N.lib.vmb_cache_workspace_bytes(*args)
         if size > 0:
@@ -142,6 +140,11 @@ def paged_attention(q, k_pages, v_pages, page_table, lengths, *, k_scale=None, v
 # vmb_paged_args up to its workspace
 _PAGED = struct.Struct("21q5if")
 assert _PAGED.size == N.PagedArgs.workspace.offset
+_CACHE = struct.Struct("6q2i")
+assert _CACHE.size == ctypes.sizeof(N.CacheArgs)
+_NO_SCALES = (0,) * 6
+_MOVE8 = struct.Struct("24q4i")
+assert _MOVE8.size == ctypes.sizeof(N.MoveE4m3Args)
 
 
 def append_pages(k, v, k_pages, v_pages, slots, *, k_scale=None, v_scale=None):
@@ -179,9 +182,10 @@ def append_pages(k, v, k_pages, v_pages, slots, *, k_scale=None, v_scale=None):
     slots = slots.contiguous()
     pool = num, hk, page_size, d
     if k_scale is not None:
-        N.launch("vmb_append_pages_e4m3", N.lib.vmb_append_pages_e4m3, device, N.Rows(*kr), N.Rows(*vr),
-                 N.Pages(*_pages(k_pages, *pool, 16)), N.Pages(*_pages(v_pages, *pool, 16)), _scales(k_scale), _scales(v_scale),
-                 slots.data_ptr(), n, num, hk, d, page_size, N.dtype_code(k.dtype))
+        a = N.MoveE4m3Args()
+        _MOVE8.pack_into(a, 0, *kr, *vr, *_pages(k_pages, *pool, 16), *_pages(v_pages, *pool, 16), *_scales(k_scale), *_scales(v_scale),
+                         0, slots.data_ptr(), n, num, hk, d, page_size, N.dtype_code(k.dtype))
+        N.launch("vmb_append_pages_e4m3", N.lib.vmb_append_pages_e4m3, device, ctypes.byref(a))
         return
     N.launch("vmb_append_pages", N.lib.vmb_append_pages, device, N.Rows(*kr), N.Rows(*vr), N.Pages(*_pages(k_pages, *pool)),
              N.Pages(*_pages(v_pages, *pool)), slots.data_ptr(), n, num, hk, d, page_size)
@@ -207,9 +211,10 @@ def copy_pages(k_pages, v_pages, src, dst, *, k_scale=None, v_scale=None):
     src, dst = src.contiguous(), dst.contiguous()
     pool = num, hk, page_size, d
     if k_scale is not None:
-        N.launch("vmb_copy_pages_e4m3", N.lib.vmb_copy_pages_e4m3, device, N.Pages(*_pages(k_pages, *pool, 16)),
-                 N.Pages(*_pages(v_pages, *pool, 16)), _scales(k_scale), _scales(v_scale), src.data_ptr(), dst.data_ptr(), n,
-                 num, hk, d, page_size)
+        a = N.MoveE4m3Args()
+        _MOVE8.pack_into(a, 0, *_NO_SCALES, *_pages(k_pages, *pool, 16), *_pages(v_pages, *pool, 16), *_scales(k_scale),
+                         *_scales(v_scale), src.data_ptr(), dst.data_ptr(), n, num, hk, d, page_size, 0)
+        N.launch("vmb_copy_pages_e4m3", N.lib.vmb_copy_pages_e4m3, device, ctypes.byref(a))
         return
     N.launch("vmb_copy_pages", N.lib.vmb_copy_pages, device, N.Pages(*_pages(k_pages, *pool)),
              N.Pages(*_pages(v_pages, *pool)), src.data_ptr(), dst.data_ptr(), n, num, hk, d, page_size)
