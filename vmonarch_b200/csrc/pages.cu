@@ -68,7 +68,7 @@ cudaError_t launch(const PageMoveParams& p, cudaStream_t st) {
 
 // ------------------------------------------------------------------------------------ rows into e4m3 pools
 constexpr int kTeamWarps = 4;  // warps of a block
-constexpr int kHeld = 8;       // 16-byte loads that a lane holds at a time
+constexpr int kHeld = 4;       // pieces of 16 columns that a lane holds at a time
 
 // The least power of two s >= 2^-126 with top <= 448 s (448 = 1.75 x 2^8), for a finite top >= 0.
 __device__ __forceinline__ float pow2_scale(float top) {
@@ -82,13 +82,13 @@ __device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) {
   asm("max.u16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
   return r;
 }
-// Four 16-bit words' pairs as e4m3, divided by a scale. POW2: times its inverse, exact in bf16 (fp16's exponents do not reach).
+// Sixteen values as e4m3, divided by a scale. POW2: times its inverse, exact in bf16 (fp16's exponents do not reach).
 template <typename T, bool POW2>
-__device__ __forceinline__ uint2 quantized(uint4 x, float scale, float inv) {
-  const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-  uint32_t q[4];
+__device__ __forceinline__ uint4 quantized(const uint4 (&x)[2], float scale, float inv) {
+  const uint32_t w[8] = {x[0].x, x[0].y, x[0].z, x[0].w, x[1].x, x[1].y, x[1].z, x[1].w};
+  uint32_t q[8];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < 8; ++i) {
     float2 f;
     if (POW2 && Elem<T>::is_bf16) {
       const __nv_bfloat162 y = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&w[i]), __floats2bfloat162_rn(inv, inv));
@@ -99,7 +99,7 @@ __device__ __forceinline__ uint2 quantized(uint4 x, float scale, float inv) {
     }
     q[i] = pack_e4m3x2(f.x, f.y);
   }
-  return make_uint2(q[0] | q[1] << 16, q[2] | q[3] << 16);
+  return make_uint4(q[0] | q[1] << 16, q[2] | q[3] << 16, q[4] | q[5] << 16, q[6] | q[7] << 16);
 }
 
 // A team of TW warps (a warp, or the block) takes the runs that begin in its `group` rows, for one head and tensor.
@@ -138,11 +138,12 @@ __global__ void __launch_bounds__(32 * kTeamWarps, 6) append_e4m3_kernel(const _
   const int64_t dst_page = is_v ? p.v_page : p.k_page;
   float* scales = is_v ? p.v_scale + head * p.vs_head : p.k_scale + head * p.ks_head;
   const int64_t scale_page = is_v ? p.vs_page : p.ks_page;
-  // lanes a row: a power of two, eight columns each
-  const int ch = p.dim / 8, lpr = ch > 8 ? 16 : ch > 4 ? 8 : ch > 2 ? 4 : 2;
-  const int per = 32 / lpr * TW;                                // rows a load of the team
-  const int at = (TW == 1 ? 0 : warp * (32 / lpr)) + lane / lpr, c = lane % lpr * 8;
+  // lanes a row: a power of two, sixteen columns each
+  const int ch = p.dim / 16, bits = ch > 4 ? 3 : ch > 2 ? 2 : ch > 1 ? 1 : 0;
+  const int per = (32 >> bits) * TW;                            // rows a load of the team
+  const int at = (TW == 1 ? 0 : warp * (32 >> bits)) + (lane >> bits), c = (lane & ((1 << bits) - 1)) * 16;
   const bool live = c < p.dim;
+  const int64_t src_step = per * src_row;
   const int step = TW == 1 ? lane : threadIdx.x;
   int turn = 0;
   for (; starts; starts &= starts - 1) {
@@ -164,13 +165,17 @@ __global__ void __launch_bounds__(32 * kTeamWarps, 6) append_e4m3_kernel(const _
     }
     float* scale_at = scales + page * scale_page;
     const float old = *scale_at;
-    uint4 x[kHeld];
+    uint4 x[kHeld][2];
     const T* from = src + (first + at) * src_row + c;
     auto load = [&](int r0) {
+      const T* q = from + r0 * src_row;
 #pragma unroll
-      for (int u = 0; u < kHeld; ++u) {
-        x[u] = make_uint4(0u, 0u, 0u, 0u);
-        if (r0 + u * per + at < n && live) x[u] = load16(from, (r0 + u * per) * src_row);
+      for (int u = 0; u < kHeld; ++u, q += src_step) {
+        x[u][0] = x[u][1] = make_uint4(0u, 0u, 0u, 0u);
+        if (r0 + u * per + at < n && live) {
+          x[u][0] = load16(q, 0);
+          x[u][1] = load16(q, 8);
+        }
       }
     };
     const bool held = n <= kHeld * per;
@@ -181,9 +186,9 @@ __global__ void __launch_bounds__(32 * kTeamWarps, 6) append_e4m3_kernel(const _
         if (!held) load(r0);
 #pragma unroll
         for (int u = 0; u < kHeld; ++u) {
-          const uint32_t w[4] = {x[u].x, x[u].y, x[u].z, x[u].w};
+          const uint32_t w[8] = {x[u][0].x, x[u][0].y, x[u][0].z, x[u][0].w, x[u][1].x, x[u][1].y, x[u][1].z, x[u][1].w};
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
+          for (int i = 0; i < 8; ++i) {
             uint32_t a = w[i] & 0x7fff7fffu;
             if (finite) {
               if ((a & 0xffffu) >= kInf) a &= 0xffff0000u;
@@ -239,7 +244,7 @@ __global__ void __launch_bounds__(32 * kTeamWarps, 6) append_e4m3_kernel(const _
       for (int u = 0; u < kHeld; ++u) {
         const int r = u * per + at;
         const int slot = __shfl_sync(0xffffffffu, my_slot, (s + r) & 31);
-        if (r < n && live) *reinterpret_cast<uint2*>(to + slot * dst_slot + c) = quantized<T, decltype(exact)::value>(x[u], scale, inv);
+        if (r < n && live) *reinterpret_cast<uint4*>(to + slot * dst_slot + c) = quantized<T, decltype(exact)::value>(x[u], scale, inv);
       }
     };
     if (held && s + n <= 32 && pow2 && !infinite) {
@@ -254,15 +259,15 @@ __global__ void __launch_bounds__(32 * kTeamWarps, 6) append_e4m3_kernel(const _
         const int r = r0 + u * per + at;
         if (r >= n || !live) continue;
         if (infinite) {  // to NaN: the conversion would make the largest value of an infinity
-          uint32_t* w = &x[u].x;
+          uint32_t* w = &x[u][0].x;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
+          for (int i = 0; i < 8; ++i) {
             if ((w[i] & 0x7fffu) == kInf) w[i] |= 1u;
             if ((w[i] >> 16 & 0x7fffu) == kInf) w[i] |= 0x10000u;
           }
         }
         const int slot = p.dst[first + r] - page * p.page_size;
-        *reinterpret_cast<uint2*>(to + slot * dst_slot + c) = pow2 ? quantized<T, true>(x[u], scale, inv) : quantized<T, false>(x[u], scale, inv);
+        *reinterpret_cast<uint4*>(to + slot * dst_slot + c) = pow2 ? quantized<T, true>(x[u], scale, inv) : quantized<T, false>(x[u], scale, inv);
       }
     }
   }
