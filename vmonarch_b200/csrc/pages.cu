@@ -121,6 +121,16 @@ __global__ void __launch_bounds__(32 * kTeamWarps, 6) append_e4m3_kernel(const _
     slot = s - page * p.page_size;
     if (page >= p.num_pages) page = -1;
   };
+  const int pair = (int)(team % pairs), head = pair >> 1;
+  const bool is_v = pair & 1;
+  const T* src = static_cast<const T*>(is_v ? p.v_src : p.k_src) + head * (is_v ? p.v_shead : p.k_shead);
+  const int64_t src_row = is_v ? p.v_row : p.k_row, dst_slot = is_v ? p.v_slot : p.k_slot;
+  // the rows on their way to L2 while the slots are read
+  if (lane < p.group && row0 + lane < p.count) {
+    const T* row = src + (row0 + lane) * src_row;
+    asm volatile("prefetch.global.L2 [%0];" ::"l"(row));
+    if (p.dim > 64) asm volatile("prefetch.global.L2 [%0];" ::"l"(row + p.dim - 1));
+  }
   int mine, my_slot, before, unused;
   look_at(row0 + lane, mine, my_slot);
   look_at(row0 - 1, before, unused);
@@ -130,10 +140,6 @@ __global__ void __launch_bounds__(32 * kTeamWarps, 6) append_e4m3_kernel(const _
   if (!starts) return;
   const unsigned same = __ballot_sync(0xffffffffu, mine >= 0 && mine == before);
   const unsigned firsts = __ballot_sync(0xffffffffu, my_slot == 0);
-  const int pair = (int)(team % pairs), head = pair >> 1;
-  const bool is_v = pair & 1;
-  const T* src = static_cast<const T*>(is_v ? p.v_src : p.k_src) + head * (is_v ? p.v_shead : p.k_shead);
-  const int64_t src_row = is_v ? p.v_row : p.k_row, dst_slot = is_v ? p.v_slot : p.k_slot;
   uint8_t* pool = static_cast<uint8_t*>(is_v ? p.v : p.k) + head * (is_v ? p.v_head : p.k_head);
   const int64_t dst_page = is_v ? p.v_page : p.k_page;
   float* scales = is_v ? p.v_scale + head * p.vs_head : p.k_scale + head * p.ks_head;
