@@ -201,7 +201,7 @@ struct Item {
   PackedUnit u;
   int head, kvh;     // head -1: no more work
   int n_kt[2], n_max;  // key tiles of the two streams
-  int brief;         // bit w: stream w's last tile has at most 32 keys that count
+  int brief;         // bit w: stream w's last tile has at most 32 keys that count; bit 2: the first tile has, sinks
   int causal;
   // keys that local query r sees
   __device__ __forceinline__ int limit(int r) const { return max(0, min(u.k_valid, causal ? u.vis0 + r : u.k_valid)); }
@@ -223,6 +223,7 @@ struct Item {
       if (last - (WIN ? key_tile(u, end) : end) * 128 <= 32) brief |= 1 << w;
     }
     n_max = max(n_kt[0], n_kt[1]);
+    if (WIN && u.lone > 0 && u.begin == 0 && a.sinks <= 32) brief |= 4;
   }
 };
 
@@ -374,6 +375,7 @@ __global__ void __launch_bounds__(kThreads, 1) packed_fwd_kernel(const __grid_co
       const int n_kt[2] = {work_sh[i & 1].n_kt[0], work_sh[i & 1].n_kt[1]};
       // a stream's last tile of <= 32 keys: shorter products
       const bool brief[2] = {(work_sh[i & 1].brief & 1) != 0, (work_sh[i & 1].brief & 2) != 0};
+      const bool brief_first = WIN && (work_sh[i & 1].brief & 4) != 0;
       __syncwarp();
       if (lane == 0) mbar_arrive(BAR(B_WFREE + (i & 1)));
       if (head < 0) break;
@@ -383,7 +385,7 @@ __global__ void __launch_bounds__(kThreads, 1) packed_fwd_kernel(const __grid_co
         if (!wwait(B_KFULL + s, parity, 2)) return false;
         tc_fence_after();
         const uint32_t kb = sK + s * TILE, qb = sQ + w * TILE;
-        const uint32_t idesc = brief[w] && t + 1 == n_kt[w] ? IDESC_S32 : IDESC_S;
+        const uint32_t idesc = brief[w] && t + 1 == n_kt[w] || WIN && brief_first && t == 0 ? IDESC_S32 : IDESC_S;
 #pragma unroll
         for (int kk = 0; kk < 4 * NA; ++kk) {
           const uint32_t off = (kk >> 2) * kAtom + (kk & 3) * 32;
@@ -406,7 +408,7 @@ __global__ void __launch_bounds__(kThreads, 1) packed_fwd_kernel(const __grid_co
           const int c = steps[w] + t;
           const uint32_t vb = sV + vs0 * TILE;
           const uint32_t a_tm = tmem + 128 * w, o_tm = tmem + T_O + 64 * NA * w;
-          const int ksteps = brief[w] && t + 1 == n_kt[w] ? 2 : 8;  // 16 keys per step
+          const int ksteps = brief[w] && t + 1 == n_kt[w] || WIN && brief_first && t == 0 ? 2 : 8;  // 16 keys per step
           if (!(ok = wwait(B_PHALF + w, c & 1, 4) && wwait(B_VFULL + vs0, vp0, 4))) break;
           // the stream's O of the last unit has been read
           if (t == 0 && outs[w] > 0 && !(ok = wwait(B_OFREE + w, (outs[w] - 1) & 1, 4))) break;
