@@ -22,6 +22,7 @@ struct PagedParams {
   int64_t ks_page, ks_head, vs_page, vs_head;
   // set by paged_plan
   int group, nt, chunks, items, whole_items, box_rows, join_blocks;
+  int per_sm;  // blocks of the 8-bit kernel that an SM holds
   int cols;  // columns that the kernels work on: 64 or 128
   uint32_t page_magic, page_shift;  // t / page_size = t * page_magic >> page_shift, t < 2^31
   int64_t blocks;

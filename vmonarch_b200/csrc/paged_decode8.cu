@@ -33,9 +33,8 @@ constexpr int kRows = kTile / kWarps;  // tokens of a tile that a warp owns
 constexpr float kRaise = 8.f;          // a reference is raised once a score passes it by more: P <= 2^8, inside fp16
 static_assert(kRows == 32, "a lane a token");
 
-template <int DP, int NT>
+template <int DP, int NT, int BLOCKS>
 struct Cfg {
-  static constexpr int BLOCKS = NT == 1 ? 3 : 2;     // an SM: registers and shared memory for as many
   static constexpr int STAGES = (DP == 128 ? 1 : 2) * (BLOCKS == 3 ? 2 : 3);
   static constexpr int MAT = kRows * DP;             // a warp's keys or values: rows of DP bytes, swizzled
   static constexpr int STAGE = 2 * MAT;
@@ -79,9 +78,9 @@ struct KParams {
   PagedParams p;
 };
 
-template <typename T, int DP, int NT, bool WIN>
-__global__ void __launch_bounds__(32 * kWarps, Cfg<DP, NT>::BLOCKS) paged_decode8_kernel(const __grid_constant__ KParams kp) {
-  using C = Cfg<DP, NT>;
+template <typename T, int DP, int NT, bool WIN, int BLOCKS>
+__global__ void __launch_bounds__(32 * kWarps, BLOCKS) paged_decode8_kernel(const __grid_constant__ KParams kp) {
+  using C = Cfg<DP, NT, BLOCKS>;
   constexpr int KS = DP / 16;
   constexpr int HEADS = 8 * NT;
   const PagedParams& p = kp.p;
@@ -415,9 +414,9 @@ __global__ void __launch_bounds__(32 * kWarps, Cfg<DP, NT>::BLOCKS) paged_decode
   }
 }
 
-template <typename T, int DP, int NT, bool WIN>
+template <typename T, int DP, int NT, bool WIN, int BLOCKS>
 cudaError_t launch(const PagedParams& p, cudaStream_t st) {
-  using C = Cfg<DP, NT>;
+  using C = Cfg<DP, NT, BLOCKS>;
   KParams kp{};
   kp.p = p;
   auto map = [&](CUtensorMap* m, const void* base, int64_t page, int64_t head, int64_t slot) {
@@ -427,7 +426,7 @@ cudaError_t launch(const PagedParams& p, cudaStream_t st) {
   };
   if (!map(&kp.tm_k, p.k, p.k_page, p.k_head, p.k_slot) || !map(&kp.tm_v, p.v, p.v_page, p.v_head, p.v_slot))
     return cudaErrorInvalidValue;
-  auto kern = paged_decode8_kernel<T, DP, NT, WIN>;
+  auto kern = paged_decode8_kernel<T, DP, NT, WIN, BLOCKS>;
   static std::atomic<uint64_t> ready{0};
   cudaError_t e = allow_smem(kern, C::SMEM, ready);
   if (e != cudaSuccess) return e;
@@ -438,8 +437,9 @@ cudaError_t launch(const PagedParams& p, cudaStream_t st) {
 
 template <typename T, bool WIN>
 cudaError_t launch_dim(const PagedParams& p, cudaStream_t st) {
-  if (p.cols == 128) return p.nt == 2 ? launch<T, 128, 2, WIN>(p, st) : launch<T, 128, 1, WIN>(p, st);
-  return p.nt == 2 ? launch<T, 64, 2, WIN>(p, st) : launch<T, 64, 1, WIN>(p, st);
+  if (p.nt == 2) return p.cols == 128 ? launch<T, 128, 2, WIN, 2>(p, st) : launch<T, 64, 2, WIN, 2>(p, st);
+  if (p.per_sm == 3) return p.cols == 128 ? launch<T, 128, 1, WIN, 3>(p, st) : launch<T, 64, 1, WIN, 3>(p, st);
+  return p.cols == 128 ? launch<T, 128, 1, WIN, 2>(p, st) : launch<T, 64, 1, WIN, 2>(p, st);
 }
 
 }  // namespace
