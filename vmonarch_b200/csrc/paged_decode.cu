@@ -78,7 +78,6 @@ __global__ void __launch_bounds__(32 * kWarps, 2) paged_decode_kernel(const __gr
   float* join_ml = join + kWarps * 8 * C::LD;                       // [warp][8 heads][max, sum]
   volatile int* abort = reinterpret_cast<int*>(smem + C::RING + C::JOIN + kWarps * C::STAGES * 8);
 
-  let_next_kernel_start();
   if (lane == 0) {
     if (warp == 0) *abort = 0;
     for (int s = 0; s < C::STAGES; ++s) mbar_init(bar0 + 8u * s, 1);
@@ -87,6 +86,9 @@ __global__ void __launch_bounds__(32 * kWarps, 2) paged_decode_kernel(const __gr
     prefetch_tmap(&kp.tm_v);
   }
   __syncthreads();
+  // the join reads the lengths before it waits: it may start once every block here knows that all before this kernel is done
+  wait_for_kernel_before();
+  let_next_kernel_start();
   Cursor cc;
   if (p.whole_items) {  // one block per item (short caches): no cut, no join
     cc.seq = blockIdx.x / p.items;
@@ -342,9 +344,7 @@ cudaError_t launch(const PagedParams& p, cudaStream_t st) {
   static std::atomic<uint64_t> ready{0};
   cudaError_t e = allow_smem(kern, C::SMEM, ready);
   if (e != cudaSuccess) return e;
-  // not launched early: the join behind it reads the lengths before it waits, and this kernel's start is what makes them final
-  kern<<<(unsigned)p.blocks, 32 * kWarps, C::SMEM, st>>>(kp);
-  e = cudaGetLastError();
+  e = launch_early(kern, p.blocks, 32 * kWarps, C::SMEM, st, kp);
   if (e != cudaSuccess || p.whole_items) return e;
   // the join starts while the last blocks still run and waits on the device for what they wrote
   return launch_early(paged_join_kernel<T, DP, NT, WIN, kTile>, (int64_t)p.batch * p.join_blocks, 512, 0, st, p);
