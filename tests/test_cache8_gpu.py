@@ -484,3 +484,9 @@ def test_refusals():
             append_pages(*args, **kw)
     with pytest.raises(AssertionError):
         copy_pages(kp, vp, slots, slots)
+    wide = ks[:1].expand(ks.shape)  # may be read, but not written
+    paged_attention(**{**ok, "k_scale": wide})
+    with pytest.raises(AssertionError, match="expanded"):
+        append_pages(rows, rows, kp, vp, slots, k_scale=wide, v_scale=vs)
+    with pytest.raises(AssertionError, match="expanded"):
+        copy_pages(kp, vp, slots, slots, k_scale=ks, v_scale=wide)

@@ -134,6 +134,9 @@ def test_pages_handed_to_tables_on_the_device():
         cache.page_tables(2, 3, 1)
     with pytest.raises(AssertionError, match="moved"):
         cache.compact()
+    for other in (PageTables(10, 4, 2, 3, device="cpu"), object()):
+        with pytest.raises(AssertionError, match="taken back"):
+            cache.take_back(other)
 
 
 def test_8_bit_pools_refuse():

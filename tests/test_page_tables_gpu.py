@@ -206,6 +206,11 @@ def test_captured_decoding(window, sinks, dtype):
     pages = [p for b, n in enumerate(lens) for p in tables.table[b, :-(-n // page)].tolist()]
     pages += tables.free_pages[:int(tables.num_free)].tolist() + cache.pages(kept)
     assert sorted(pages) == list(range(60))
+    cache.take_back(tables)
+    assert cache.num_free == 56 and int(tables.num_free) == 0 and cache.compact() == 4
+    cache.reserve([cache.add()], [56 * page])
+    with pytest.raises(AssertionError):
+        cache.take_back(tables)
 
 
 def test_other_streams_and_devices():

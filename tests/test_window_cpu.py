@@ -83,8 +83,10 @@ def test_pieces_of_windowed_units():
 
 def test_a_window_as_long_as_the_sequences_lists_the_causal_units():
     seqs = PackedSequences([300, 5, 900], [300, 40, 1000], device="cpu")
-    for kind in ("fwd", "dq", "kv"):
-        assert np.array_equal(units(seqs, kind, (1000, 0), 2, 1), units(seqs, kind, True, 2, 1))
+    for kind in ("fwd", "dq", "kv"):  # (of few heads the forward's units are smaller)
+        assert np.array_equal(units(seqs, kind, (1000, 0), 40, 1), units(seqs, kind, True, 40, 1))
+    most = {kind: [units(seqs, kind, mask, 2, 1)[:, 1].max() for mask in ((1000, 0), True)] for kind in ("fwd", "dq")}
+    assert most == {"fwd": [128, 256], "dq": [128, 128]}
 
 
 @pytest.mark.parametrize("kw, why", [

@@ -62,9 +62,11 @@ def _check_index(t, name, dim, device):
         f"{name} must be int32, {dim}-dimensional and on the pools' device"
 
 
-def _scales(t):
+def _scales(t, written=False):
     """vmb_page_scales of a (num_pages, Hk) tensor."""
-    return t.data_ptr(), *t.stride()
+    page, head = t.stride()
+    assert not written or (page or t.size(0) == 1) and (head or t.size(1) == 1), "scales that are written must not be expanded views"
+    return t.data_ptr(), page, head
 
 
 def paged_attention(q, k_pages, v_pages, page_table, lengths, *, k_scale=None, v_scale=None, window=None, sinks=0,
@@ -183,8 +185,8 @@ def append_pages(k, v, k_pages, v_pages, slots, *, k_scale=None, v_scale=None):
     pool = num, hk, page_size, d
     if k_scale is not None:
         a = N.MoveE4m3Args()
-        _MOVE8.pack_into(a, 0, *kr, *vr, *_pages(k_pages, *pool, 16), *_pages(v_pages, *pool, 16), *_scales(k_scale), *_scales(v_scale),
-                         0, slots.data_ptr(), n, num, hk, d, page_size, N.dtype_code(k.dtype))
+        _MOVE8.pack_into(a, 0, *kr, *vr, *_pages(k_pages, *pool, 16), *_pages(v_pages, *pool, 16), *_scales(k_scale, True),
+                         *_scales(v_scale, True), 0, slots.data_ptr(), n, num, hk, d, page_size, N.dtype_code(k.dtype))
         N.launch("vmb_append_pages_e4m3", N.lib.vmb_append_pages_e4m3, device, ctypes.byref(a))
         return
     N.launch("vmb_append_pages", N.lib.vmb_append_pages, device, N.Rows(*kr), N.Rows(*vr), N.Pages(*_pages(k_pages, *pool)),
@@ -212,8 +214,8 @@ def copy_pages(k_pages, v_pages, src, dst, *, k_scale=None, v_scale=None):
     pool = num, hk, page_size, d
     if k_scale is not None:
         a = N.MoveE4m3Args()
-        _MOVE8.pack_into(a, 0, *_NO_SCALES, *_pages(k_pages, *pool, 16), *_pages(v_pages, *pool, 16), *_scales(k_scale),
-                         *_scales(v_scale), src.data_ptr(), dst.data_ptr(), n, num, hk, d, page_size, 0)
+        _MOVE8.pack_into(a, 0, *_NO_SCALES, *_pages(k_pages, *pool, 16), *_pages(v_pages, *pool, 16), *_scales(k_scale, True),
+                         *_scales(v_scale, True), src.data_ptr(), dst.data_ptr(), n, num, hk, d, page_size, 0)
         N.launch("vmb_copy_pages_e4m3", N.lib.vmb_copy_pages_e4m3, device, ctypes.byref(a))
         return
     N.launch("vmb_copy_pages", N.lib.vmb_copy_pages, device, N.Pages(*_pages(k_pages, *pool)),
@@ -255,7 +257,7 @@ class PagedKVCache:
         self._owners = [0] * num_pages
         self._pages, self._length = {}, {}
         self._next = 0
-        self._lent = False  # whether pages are a PageTables' now
+        self._lent = {}  # PageTables that hold pages of this book, by their id
 
     @property
     def num_free(self) -> int:
@@ -266,7 +268,7 @@ class PagedKVCache:
         """
         A :class:`PageTables` of `batch` sequences over this cache's pools, with `num_pages` (default: all) of its free pages,
         which are then no longer this book's. Its slots, table and lengths go to :meth:`write` and :meth:`attend`, beside
-        those of sequences of this book.
+        those of sequences of this book. :meth:`take_back` ends it.
         """
         num_pages = len(self._free) if num_pages is None else num_pages
         if num_pages > len(self._free):
@@ -274,8 +276,17 @@ class PagedKVCache:
         tables = PageTables(self.num_pages, self.page_size, batch, width, pages=self._free[len(self._free) - num_pages:],
                             device=self.device)
         del self._free[len(self._free) - num_pages:]
-        self._lent = self._lent or num_pages > 0
+        self._lent[id(tables)] = tables
         return tables
+
+    def take_back(self, tables) -> None:
+        """Takes the pages of a :class:`PageTables` that :meth:`page_tables` made back into this book, those of its sequences
+        among them. `tables` is empty and of no more use. Waits for the device."""
+        assert self._lent.pop(id(tables), None) is tables, "not a PageTables of this cache, or taken back before"
+        tables.truncate(torch.zeros_like(tables.lengths))
+        tables.check()
+        self._free += tables.free_pages[:int(tables.num_free)].tolist()
+        tables.num_free.zero_()
 
     def length(self, seq: int) -> int:
         return self._length[seq]
