@@ -4,9 +4,10 @@ then continued token by token from a paged cache.
 Every block's attention is ``packed_attention`` (training, prompts) or the cache's ``attend`` (one token at a
 time), and everything between two blocks is one ``gated_residual_norm``: the norm after the block that ends, its
 gate, the residual, and the modulated norm before the one that begins, with gates, scales and shifts that a
-conditioning vector gives each sequence.
+conditioning vector gives each sequence. With a window every token sees the last ones and a few first ones only, while
+training and from the cache, which may hold its keys and values in 8 bits.
 
-    python examples/packed_transformer.py [--steps 60]
+    python examples/packed_transformer.py [--steps 60] [--window 32 --sinks 4] [--cache-bits 8]
 """
 from __future__ import annotations
 
@@ -41,8 +42,9 @@ class Block(nn.Module):
 
 
 class PackedTransformer(nn.Module):
-    def __init__(self, vocab=96, cond=16, dim=256, heads=4, kv_heads=2, layers=2):
+    def __init__(self, vocab=96, cond=16, dim=256, heads=4, kv_heads=2, layers=2, window=None, sinks=0):
         super().__init__()
+        self.sight = dict(window=window, sinks=sinks)
         self.embed = nn.Embedding(vocab, dim)
         self.blocks = nn.ModuleList(Block(dim, heads, kv_heads) for _ in range(layers))
         # one norm before the first block, one after each of the 2 * layers halves (the last one before the head)
@@ -71,11 +73,11 @@ class PackedTransformer(nn.Module):
         return self.head(h)
 
     def forward(self, tokens, cond, seqs):
-        return self.run(tokens, cond, seqs, lambda _, q, k, v: packed_attention(q, k, v, seqs, causal=True))
+        return self.run(tokens, cond, seqs, lambda _, q, k, v: packed_attention(q, k, v, seqs, causal=True, **self.sight))
 
-    def new_cache(self, num_pages, page_size=16):
+    def new_cache(self, num_pages, page_size=16, dtype=None):
         _, kv_heads, d = self.blocks[0].shape
-        return PagedKVCache(num_pages, page_size, kv_heads, d, layers=len(self.blocks), dtype=self.head.weight.dtype,
+        return PagedKVCache(num_pages, page_size, kv_heads, d, layers=len(self.blocks), dtype=dtype or self.head.weight.dtype,
                             device=self.head.weight.device)
 
     @torch.no_grad()
@@ -85,7 +87,7 @@ class PackedTransformer(nn.Module):
 
         def attend(layer, q, k, v):
             cache.write(layer, k, v, slots)
-            return packed_attention(q, k, v, seqs, causal=True)
+            return packed_attention(q, k, v, seqs, causal=True, **self.sight)
 
         return self.run(tokens, cond, seqs, attend)
 
@@ -97,7 +99,7 @@ class PackedTransformer(nn.Module):
 
         def attend(layer, q, k, v):
             cache.write(layer, k, v, slots)
-            return cache.attend(layer, q, table, lengths)
+            return cache.attend(layer, q, table, lengths, **self.sight)
 
         return self.run(tokens, cond, PackedSequences([1] * len(ids), device=tokens.device), attend)
 
@@ -134,15 +136,18 @@ def train(model, steps, device, seed=0, vocab=96, cond=16):
 def main():
     ap = argparse.ArgumentParser()
     ap.add_argument("--steps", type=int, default=60)
+    ap.add_argument("--window", type=int)
+    ap.add_argument("--sinks", type=int, default=0)
+    ap.add_argument("--cache-bits", type=int, choices=(8, 16), default=16)
     args = ap.parse_args()
     device = torch.device("cuda", 0)
     torch.manual_seed(0)
-    model = PackedTransformer().to(device, torch.bfloat16)
+    model = PackedTransformer(window=args.window, sinks=args.sinks).to(device, torch.bfloat16)
     losses = train(model, args.steps, device)
     print(f"loss {losses[0]:.3f} -> {losses[-1]:.3f} over {args.steps} steps")
     tokens, c, lens = clips(3, 40, 96, 16, torch.Generator().manual_seed(1))
     tokens, c = tokens.to(device), c.to(device, torch.bfloat16)
-    cache = model.new_cache(64)
+    cache = model.new_cache(64, dtype=torch.float8_e4m3fn if args.cache_bits == 8 else None)
     ids = [cache.add() for _ in lens]
     last = torch.tensor(lens, device=device).cumsum(0) - 1
     token = model.prompt(tokens, c, PackedSequences(lens, device=device), cache, ids)[last].argmax(-1)

@@ -43,7 +43,7 @@ __device__ __forceinline__ Span span_of(const PagedParams& p, int len) {
 template <bool WIN, int TILE>
 __device__ __forceinline__ int tiles_of(const PagedParams& p, int len) { return span_of<WIN, TILE>(p, len).tiles; }
 __device__ __forceinline__ int seq_len(const PagedParams& p, int b) {
-  return max(0, min(p.lengths[b], p.max_len));
+  return max(0, min(__ldcg(p.lengths + b), p.max_len));  // (from L2: the join reads them before it waits)
 }
 
 // The flat order of units: sequences, then items (key head, head chunk) of a sequence, then kItemCost units

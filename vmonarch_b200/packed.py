@@ -388,14 +388,14 @@ class _PackedAttention(torch.autograd.Function):
         return dq, dk, dv, None, None, None
 
 
-def _window(window, sinks):
-    """(window, sinks) as the kernels take them, None without a window."""
+def _window(window, sinks, most):
+    """(window, sinks) as the kernels take them, `most` for what is more, None without a window."""
     if window is None:
         assert sinks == 0, "sinks need a window"
         return None
     window, sinks = operator.index(window), operator.index(sinks)
     assert window >= 1 and sinks >= 0, "window must be at least 1 and sinks not negative"
-    return min(window, _WIDE), min(sinks, _WIDE)
+    return min(window, most), min(sinks, most)
 
 
 def packed_attention(q, k, v, seqs, *, causal=False, window=None, sinks=0, sm_scale=None, return_lse=False):
@@ -424,7 +424,7 @@ def packed_attention(q, k, v, seqs, *, causal=False, window=None, sinks=0, sm_sc
     dtype = q.dtype
     assert dtype in SUPPORTED_DTYPES, f"unsupported dtype {dtype}"
     assert k.dtype == dtype and v.dtype == dtype, "q, k and v must share a dtype"
-    mask = _window(window, sinks) or bool(causal)
+    mask = _window(window, sinks, _WIDE) or bool(causal)
     if window is not None:
         assert causal, "a window needs causal=True"
         assert q.size(0) <= _WIDE and k.size(0) <= _WIDE, f"at most {_WIDE} rows with a window"

@@ -101,7 +101,7 @@ def paged_attention(q, k_pages, v_pages, page_table, lengths, *, k_scale=None, v
         assert dtype in SUPPORTED_DTYPES, f"unsupported dtype {dtype}"
     assert len(shape) == 3 and q.dtype == dtype and shape[2] == d and q.device == device, \
         "q must be (B, H, D) with the pools' D, dtype and device"
-    mask = _window(window, sinks)
+    mask = _window(window, sinks, 2 ** 31 - 1)  # lengths are 32-bit
     b, h, _ = shape
     assert h >= 1 and h % hk == 0, "H must be a multiple of Hk"
     _check_index(page_table, "page_table", 2, device)
