@@ -26,7 +26,8 @@ constexpr int kOneRows = 4096;   // and rows, or table entries per 16 sequences
 
 enum { kNoPages = 1, kTooWide = 2, kTooMany = 4, kOverfull = 8 };
 
-__device__ __forceinline__ int ceil_div(int64_t a, int b) { return (int)((a + b - 1) / b); }
+// Pages of `a` tokens; a and b below 2^31, so that their sum stays in 32 bits (a 64-bit division costs more than all else here).
+__device__ __forceinline__ int ceil_div(int a, int b) { return (int)(((uint32_t)a + (uint32_t)b - 1u) / (uint32_t)b); }
 
 // What the sums of a call say of each sequence: its length before, the rows and pages before it; and of the call.
 struct Plan {
@@ -66,27 +67,55 @@ __device__ __forceinline__ Sums block_sums(int64_t a, int64_t b) {
   return Sums{warp_a[warp] + ia - a, warp_b[warp] + ib - b, warp_a[32], warp_b[32]};
 }
 
-// The rows [row, total) in steps of `step`.
+// R neighbouring rows from `row` on, then those `step` further on: one search and, inside a page, one look for R of them.
+template <int R>
 __device__ __forceinline__ void write_slots(const BookParams& p, const Plan& plan, int64_t row, int64_t step) {
   const bool done = plan.call[0] != 0;
   const int top = plan.call[1] - 1, last = plan.rows[p.batch];
   for (; row < p.total; row += step) {
-    int slot = -1;
-    if (done && row < last) {
-      int lo = 0, hi = p.batch;  // the last sequence that begins at or before the row: rows[lo] <= row < rows[hi]
-      while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (plan.rows[mid] <= row) lo = mid;
-        else hi = mid;
+    int slots[R];
+    int seq = -1, next = 0, page = 0, in = 0, i = 0;  // of the row before; `next`: where its sequence ends
+#pragma unroll
+    for (int k = 0; k < R; ++k) {
+      const int64_t r = row + k;
+      slots[k] = -1;
+      if (!done || r >= last) continue;
+      bool look = true;
+      if (seq >= 0 && r < next) {
+        look = ++in == p.page_size;
+        if (look) in = 0, ++i;
+      } else {
+        if (seq < 0) {
+          int hi = p.batch;  // the last sequence that begins at or before the row: rows[seq] <= r < rows[hi]
+          seq = 0;
+          while (hi - seq > 1) {
+            const int mid = (seq + hi) >> 1;
+            if (plan.rows[mid] <= r) seq = mid;
+            else hi = mid;
+          }
+        } else {
+          while (plan.rows[seq + 1] <= r) ++seq;
+        }
+        next = plan.rows[seq + 1];
+        const int at = plan.len[seq] + (int)(r - plan.rows[seq]);
+        i = at / p.page_size;
+        in = at - i * p.page_size;
       }
-      const int len = plan.len[lo], at = len + (int)(row - plan.rows[lo]);
-      const int i = at / p.page_size, in = at - i * p.page_size, have = ceil_div(len, p.page_size);
-      int32_t* entry = p.table + lo * p.stride + i;
-      const int page = i < have ? *entry : p.free_pages[top - (plan.pages[lo] + i - have)];
-      if (in == 0) *entry = page;  // (a page's first token is new if the page is)
-      if ((unsigned)page < (unsigned)p.num_pages) slot = page * p.page_size + in;
+      if (look) {
+        const int have = ceil_div(plan.len[seq], p.page_size);
+        int32_t* entry = p.table + seq * p.stride + i;
+        page = i < have ? *entry : p.free_pages[top - (plan.pages[seq] + i - have)];
+        if (in == 0) *entry = page;  // (a page's first token is new if the page is)
+      }
+      if ((unsigned)page < (unsigned)p.num_pages) slots[k] = page * p.page_size + in;
     }
-    p.slots[row] = slot;
+    if (R == 4 && row + R <= p.total && (reinterpret_cast<uintptr_t>(p.slots) & 15) == 0) {
+      *reinterpret_cast<int4*>(p.slots + row) = make_int4(slots[0], slots[1 % R], slots[2 % R], slots[3 % R]);
+    } else {
+#pragma unroll
+      for (int k = 0; k < R; ++k)
+        if (row + k < p.total) p.slots[row + k] = slots[k];
+    }
   }
 }
 // Sequence b's pages beyond its new length, by threads of which this is the `t`-th of `n`.
@@ -116,11 +145,15 @@ __global__ void __launch_bounds__(kThreads) book_kernel(const __grid_constant__ 
     if (len < 0 || (RESERVE && want < 0)) bad |= kTooMany, next = len = max(len, (int64_t)0);
     if (max(len, next) > room) bad |= kTooWide, next = len = min(len, room);
   };
+  auto difference = [&](int len, int next) {
+    const int pages = ceil_div(next, p.page_size) - ceil_div(len, p.page_size);
+    return RESERVE ? pages : -pages;
+  };
   for (int b = b0; b < b1; ++b) {
     int64_t len, next;
     lengths(b, len, next);
     rows += RESERVE ? next - len : 0;
-    pages += RESERVE ? ceil_div(next, p.page_size) - ceil_div(len, p.page_size) : ceil_div(len, p.page_size) - ceil_div(next, p.page_size);
+    pages += difference((int)len, (int)next);
   }
   const int free_before = max(0, min(*p.num_free, p.num_pages));
   const Sums s = block_sums(rows, pages);
@@ -146,7 +179,7 @@ __global__ void __launch_bounds__(kThreads) book_kernel(const __grid_constant__ 
       plan.rows[b] = (int)rows;
       plan.pages[b] = (int)pages;
       rows += RESERVE ? next - len : 0;
-      pages += RESERVE ? ceil_div(next, p.page_size) - ceil_div(len, p.page_size) : ceil_div(len, p.page_size) - ceil_div(next, p.page_size);
+      pages += difference((int)len, (int)next);
       p.lengths[b] = (int)next;
     }
     if (threadIdx.x == 0) plan.rows[p.batch] = (int)s.total_a, plan.pages[p.batch] = (int)s.total_b;
@@ -154,7 +187,7 @@ __global__ void __launch_bounds__(kThreads) book_kernel(const __grid_constant__ 
   if (!ONE) return;
   __syncthreads();
   if (RESERVE) {
-    write_slots(p, plan, threadIdx.x, blockDim.x);
+    write_slots<1>(p, plan, threadIdx.x, blockDim.x);
   } else if (!bad) {
     for (int b = threadIdx.x >> 5; b < p.batch; b += blockDim.x >> 5) return_pages(p, plan, b, threadIdx.x & 31, 32);
   }
@@ -163,7 +196,7 @@ __global__ void __launch_bounds__(kThreads) book_kernel(const __grid_constant__ 
 __global__ void __launch_bounds__(256) slots_kernel(const __grid_constant__ BookParams p) {
   wait_for_kernel_before();
   let_next_kernel_start();
-  write_slots(p, plan_at(p.plan, p.batch), (int64_t)blockIdx.x * 256 + threadIdx.x, (int64_t)gridDim.x * 256);
+  write_slots<4>(p, plan_at(p.plan, p.batch), ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4, (int64_t)gridDim.x * 1024);
 }
 // A warp a sequence.
 __global__ void __launch_bounds__(256) return_kernel(const __grid_constant__ BookParams p) {
@@ -193,7 +226,7 @@ cudaError_t reserve_pages(const BookParams& p, cudaStream_t st) {
   book_kernel<true, false><<<1, threads_for(p.batch), 0, st>>>(p);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess || p.total == 0) return e;
-  const int64_t blocks = (p.total + 255) / 256;
+  const int64_t blocks = (p.total + 1023) / 1024;
   return launch_early(slots_kernel, blocks < 148 * 8 ? blocks : 148 * 8, 256, 0, st, p);
 }
 
