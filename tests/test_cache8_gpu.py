@@ -336,7 +336,11 @@ def test_append_extremes(dtype, page):
                 scale = torch.full((3, hk), old, device="cuda")
                 pools, scales = [codes.clone(), codes.clone()], [scale.clone(), scale.clone()]
                 slots = torch.arange(page + first, page + first + len(rows), dtype=torch.int32, device="cuda")
-                append_pages(x[rows], x[rows], *pools, slots, k_scale=scales[0], v_scale=scales[1])
+                # pages of 64: skipped rows behind, as many as make the call one whose runs are a block's each
+                skipped = 2 * page if page == 64 else 0
+                padded = torch.cat([slots, torch.full((skipped,), -1, dtype=torch.int32, device="cuda")])
+                new = torch.cat([x[rows], x[:1].expand(skipped, hk, d)])
+                append_pages(new, new, *pools, padded, k_scale=scales[0], v_scale=scales[1])
                 ref, sref = codes.double(), scale.double()
                 append_reference(x[rows], ref, sref, slots)
                 for p, s in zip(pools, scales):

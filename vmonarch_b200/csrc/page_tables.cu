@@ -21,8 +21,11 @@ namespace vmb {
 namespace {
 
 constexpr int kThreads = 1024;
-constexpr int kOneBatch = 1024;  // most sequences of a call in one block
-constexpr int kOneRows = 4096;   // and rows, or table entries per 16 sequences
+// Most sequences of a call in one block, and rows (or table entries / 16, of which a call returns few). Both calls, us, in one
+// block and with second kernels: 64 sequences of one new token each 5.9 and 10.2, 256 of four 7.4 and 10.4, 256 of sixteen 11.1 and
+// 10.7, 8 of 1024 13.2 and 8.8.
+constexpr int kOneBatch = 1024;
+constexpr int kOneRows = 4096;
 
 enum { kNoPages = 1, kTooWide = 2, kTooMany = 4, kOverfull = 8 };
 
@@ -67,6 +70,17 @@ __device__ __forceinline__ Sums block_sums(int64_t a, int64_t b) {
   return Sums{warp_a[warp] + ia - a, warp_b[warp] + ib - b, warp_a[32], warp_b[32]};
 }
 
+// The last sequence whose first number is at most x: before[seq] <= x < before[seq + 1].
+__device__ __forceinline__ int sequence_of(const int* before, int batch, int64_t x) {
+  int lo = 0, hi = batch;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (before[mid] <= x) lo = mid;
+    else hi = mid;
+  }
+  return lo;
+}
+
 // R neighbouring rows from `row` on, then those `step` further on: one search and, inside a page, one look for R of them.
 template <int R>
 __device__ __forceinline__ void write_slots(const BookParams& p, const Plan& plan, int64_t row, int64_t step) {
@@ -85,17 +99,9 @@ __device__ __forceinline__ void write_slots(const BookParams& p, const Plan& pla
         look = ++in == p.page_size;
         if (look) in = 0, ++i;
       } else {
-        if (seq < 0) {
-          int hi = p.batch;  // the last sequence that begins at or before the row: rows[seq] <= r < rows[hi]
-          seq = 0;
-          while (hi - seq > 1) {
-            const int mid = (seq + hi) >> 1;
-            if (plan.rows[mid] <= r) seq = mid;
-            else hi = mid;
-          }
-        } else {
+        if (seq < 0) seq = sequence_of(plan.rows, p.batch, r);
+        else
           while (plan.rows[seq + 1] <= r) ++seq;
-        }
         next = plan.rows[seq + 1];
         const int at = plan.len[seq] + (int)(r - plan.rows[seq]);
         i = at / p.page_size;
@@ -118,12 +124,15 @@ __device__ __forceinline__ void write_slots(const BookParams& p, const Plan& pla
     }
   }
 }
-// Sequence b's pages beyond its new length, by threads of which this is the `t`-th of `n`.
-__device__ __forceinline__ void return_pages(const BookParams& p, const Plan& plan, int b, int t, int n) {
-  const int count = plan.pages[b + 1] - plan.pages[b], held = ceil_div(plan.len[b], p.page_size);
-  const int top = plan.call[1] + plan.pages[p.batch] - 1;
-  const int32_t* from = p.table + b * p.stride + held - count;
-  for (int i = t; i < count; i += n) p.free_pages[top - (plan.pages[b] + i)] = from[i];
+// The pages beyond the sequences' new lengths, from the x-th on in steps of `step`.
+__device__ __forceinline__ void return_pages(const BookParams& p, const Plan& plan, int64_t x, int64_t step) {
+  const int number = plan.pages[p.batch], top = plan.call[1] + number - 1;
+  for (; x < number; x += step) {
+    const int b = sequence_of(plan.pages, p.batch, x);
+    // (the last of them is the last that the sequence held)
+    const int held = ceil_div(plan.len[b], p.page_size);
+    p.free_pages[top - x] = p.table[b * p.stride + held - (plan.pages[b + 1] - (int)x)];
+  }
 }
 
 // RESERVE: counts -> sums, else lengths to keep -> sums. ONE: this block does the rest too.
@@ -189,7 +198,7 @@ __global__ void __launch_bounds__(kThreads) book_kernel(const __grid_constant__ 
   if (RESERVE) {
     write_slots<1>(p, plan, threadIdx.x, blockDim.x);
   } else if (!bad) {
-    for (int b = threadIdx.x >> 5; b < p.batch; b += blockDim.x >> 5) return_pages(p, plan, b, threadIdx.x & 31, 32);
+    return_pages(p, plan, threadIdx.x, blockDim.x);
   }
 }
 
@@ -198,13 +207,11 @@ __global__ void __launch_bounds__(256) slots_kernel(const __grid_constant__ Book
   let_next_kernel_start();
   write_slots<4>(p, plan_at(p.plan, p.batch), ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4, (int64_t)gridDim.x * 1024);
 }
-// A warp a sequence.
 __global__ void __launch_bounds__(256) return_kernel(const __grid_constant__ BookParams p) {
   wait_for_kernel_before();
   let_next_kernel_start();
   const Plan plan = plan_at(p.plan, p.batch);
-  const int64_t b = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-  if (b < p.batch && plan.call[0]) return_pages(p, plan, (int)b, threadIdx.x & 31, 32);
+  if (plan.call[0]) return_pages(p, plan, (int64_t)blockIdx.x * 256 + threadIdx.x, (int64_t)gridDim.x * 256);
 }
 
 // threads of the first kernel: a sequence, and where it does them a row, each, if that many fit
@@ -232,13 +239,15 @@ cudaError_t reserve_pages(const BookParams& p, cudaStream_t st) {
 
 cudaError_t truncate_pages(const BookParams& p, cudaStream_t st) {
   if (truncate_in_one(p)) {
-    book_kernel<false, true><<<1, threads_for(32 * (int64_t)p.batch), 0, st>>>(p);
+    book_kernel<false, true><<<1, threads_for(p.batch), 0, st>>>(p);
     return cudaGetLastError();
   }
   book_kernel<false, false><<<1, threads_for(p.batch), 0, st>>>(p);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return e;
-  return launch_early(return_kernel, ((int64_t)p.batch + 7) / 8, 256, 0, st, p);
+  // (as many pages as the table has entries may go back, but hardly ever do)
+  const int64_t blocks = ((int64_t)p.batch * p.width + 255) / 256;
+  return launch_early(return_kernel, blocks < 148 * 8 ? blocks : 148 * 8, 256, 0, st, p);
 }
 
 }  // namespace vmb

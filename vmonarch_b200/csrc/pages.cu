@@ -296,7 +296,10 @@ __global__ void __launch_bounds__(32 * kTeamWarps, kTeamBlocks) append_e4m3_kern
 
 template <typename T>
 cudaError_t launch_e4m3(PageMoveParams p, cudaStream_t st) {
-  const bool block = p.page_size > 32;
+  // A block a run where runs may be long: pages of 64 slots and rows for two of them. 16384 rows of prompts, 8 heads, D = 128, us, with
+  // a warp and with a block: pages of 48 27.3 and 36.5, of 64 34.2 and 28.9, of 256 46.9 and 33.9; 1024 rows, pages of 256 28.5
+  // and 13.1; one row of each of 64 sequences, whatever their pages, 3.3 and 4.8.
+  const bool block = p.page_size >= 64 && p.count >= 2 * (int64_t)p.page_size;
   const int64_t pairs = 2 * p.kv_heads;
   // one row a team while all teams fit on the GPU at once, up to a page's rows where there are many
   const int64_t room = block ? 148 * 16 : 148 * 16 * kTeamWarps;
