@@ -378,7 +378,7 @@ void paged_plan(PagedParams& p) {
   // 8-bit: three blocks an SM with rings of two stages hide the ends of many items, two with three stages keep more copies in
   // flight over few long ones (512 items of 64 sequences: 38.9 us with three, 40.8 with two; 12 items of up to 262143 tokens:
   // 55.7 and 53.8); 16 heads need the registers of two
-  p.per_sm = p.k_scale && p.nt == 1 && (int64_t)p.batch * p.items >= 2 * 148 ? 3 : 2;
+  p.per_sm = !p.k_scale || p.nt == 2 ? 2 : p.cols == 64 ? 4 : (int64_t)p.batch * p.items >= 2 * 148 ? 3 : 2;
   p.blocks = p.whole_items ? (int64_t)p.batch * p.items : p.per_sm * 148;
 }
 

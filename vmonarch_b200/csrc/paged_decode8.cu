@@ -35,7 +35,7 @@ static_assert(kRows == 32, "a lane a token");
 
 template <int DP, int NT, int BLOCKS>
 struct Cfg {
-  static constexpr int STAGES = (DP == 128 ? 1 : 2) * (BLOCKS == 3 ? 2 : 3);
+  static constexpr int STAGES = DP == 128 ? (BLOCKS == 3 ? 2 : 3) : BLOCKS == 4 ? 3 : 6;
   static constexpr int MAT = kRows * DP;             // a warp's keys or values: rows of DP bytes, swizzled
   static constexpr int STAGE = 2 * MAT;
   static constexpr int RING = kWarps * STAGES * STAGE;
@@ -182,27 +182,33 @@ __global__ void __launch_bounds__(32 * kWarps, BLOCKS) paged_decode8_kernel(cons
   uint32_t qf[NT][KS][2];
   float acc[NT][KS][4], m[NT][2], mv[NT][2], l[NT][2];  // mv: the accumulators' reference
   float qs[NT][2];                                       // what a score is multiplied with, for heads 2 (lane % 4) and + 1
-  // an item's query heads as B fragments (head = lane / 4, columns 4 (lane % 4) ...)
+  // an item's query heads as B fragments (head = lane / 4, columns 4 (lane % 4) ...): loaded, and once they are there, scaled
   auto load_q = [&](const Cursor& c) {
     const int h = c.item / p.chunks, g0 = (c.item % p.chunks) * HEADS;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       const int g = g0 + 8 * nt + lane / 4;
       const T* q = static_cast<const T*>(p.q) + (int64_t)c.seq * p.q_row + (int64_t)(h * p.group + g) * p.q_head;
-      float top = 0.f;
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
         const int col = 16 * ks + 4 * (lane % 4);
         const uint2 x = g < p.group && col < p.dim ? *reinterpret_cast<const uint2*>(q + col) : make_uint2(0u, 0u);
         qf[nt][ks][0] = x.x;
         qf[nt][ks][1] = x.y;
-        if (Elem<T>::is_bf16) {
-          const float2 a = Elem<T>::unpack(x.x), b = Elem<T>::unpack(x.y);
-          top = fmaxf(fmaxf(fmaxf(fabsf(a.x), fabsf(a.y)), fmaxf(fabsf(b.x), fabsf(b.y))), top);
-        }
       }
+    }
+  };
+  auto scale_q = [&]() {
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
       float factor = 1.f;
       if (Elem<T>::is_bf16) {
+        float top = 0.f;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+          const float2 a = Elem<T>::unpack(qf[nt][ks][0]), b = Elem<T>::unpack(qf[nt][ks][1]);
+          top = fmaxf(fmaxf(fmaxf(fabsf(a.x), fabsf(a.y)), fmaxf(fabsf(b.x), fabsf(b.y))), top);
+        }
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
         const int e = (int)(__float_as_uint(top) >> 23) - 127;  // top < 2^(e + 1); 128: not finite
@@ -233,7 +239,10 @@ __global__ void __launch_bounds__(32 * kWarps, BLOCKS) paged_decode8_kernel(cons
     }
   };
   bool from_start = cc.tile == 0, ok = true;
-  if (cc.left > 0) load_q(cc);
+  if (cc.left > 0) {
+    load_q(cc);
+    scale_q();
+  }
   clear();
   for (int it = 0; cc.left > 0; ++it) {
     if (ok && !__all_sync(0xffffffffu, mbar_wait(bar0 + 8u * (it % C::STAGES), (it / C::STAGES) & 1, abort, &g_paged8_err, 1,
@@ -404,6 +413,7 @@ __global__ void __launch_bounds__(32 * kWarps, BLOCKS) paged_decode8_kernel(cons
         }
         __syncthreads();
       }
+      if (cc.left > 0) scale_q();
       clear();
       from_start = true;
     }
@@ -438,8 +448,8 @@ cudaError_t launch(const PagedParams& p, cudaStream_t st) {
 template <typename T, bool WIN>
 cudaError_t launch_dim(const PagedParams& p, cudaStream_t st) {
   if (p.nt == 2) return p.cols == 128 ? launch<T, 128, 2, WIN, 2>(p, st) : launch<T, 64, 2, WIN, 2>(p, st);
-  if (p.per_sm == 3) return p.cols == 128 ? launch<T, 128, 1, WIN, 3>(p, st) : launch<T, 64, 1, WIN, 3>(p, st);
-  return p.cols == 128 ? launch<T, 128, 1, WIN, 2>(p, st) : launch<T, 64, 1, WIN, 2>(p, st);
+  if (p.cols == 64) return launch<T, 64, 1, WIN, 4>(p, st);
+  return p.per_sm == 3 ? launch<T, 128, 1, WIN, 3>(p, st) : launch<T, 128, 1, WIN, 2>(p, st);
 }
 
 }  // namespace
