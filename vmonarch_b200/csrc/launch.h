@@ -105,8 +105,7 @@ cudaError_t allow_smem(Kern kern, int bytes, std::atomic<uint64_t>& done) {
 
 #ifdef __CUDACC__
 // Launches a kernel that may be set up while the stream's kernel before it still runs. Every block of it calls
-// wait_for_kernel_before() before it touches global memory. (The join of the paged attention reads the call's lengths
-// before that: the kernel in front of it lets it start only when it has waited itself, so all that wrote them is done by then.)
+// wait_for_kernel_before() before it touches global memory.
 template <typename... Params, typename... Args>
 cudaError_t launch_early(void (*kern)(Params...), int64_t blocks, int threads, int smem, cudaStream_t st, const Args&... args) {
   if (blocks > 0x7fffffff) return cudaErrorInvalidConfiguration;

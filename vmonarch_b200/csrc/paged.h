@@ -27,6 +27,7 @@ struct PagedParams {
   uint32_t page_magic, page_shift;  // t / page_size = t * page_magic >> page_shift, t < 2^31
   int64_t blocks;
   float *part, *part_ml;
+  int2* cuts;            // [batch][items]: the first and last block of an item that is cut, -1 of one that is not
   long long wait_limit;  // pipeline wait limit in cycles (0: the default ~2 s)
   int hold_loads;        // test of the timeout path: the first warp of a block issues no load
 };

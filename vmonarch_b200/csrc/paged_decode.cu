@@ -24,8 +24,8 @@
 // anything, so their value rows are cleared before the product (0 x inf). Pages past the last, page ids outside
 // the pool and columns past D arrive as zeros (coordinates outside the tensor map).
 //
-// 64 sequences of up to 8190 tokens, 40/8 heads, D = 128, pages of 16: 44 us, 4.3 TB/s; 3 of up to 262143, 16/4 heads,
-// pages of 64: 93 us, 5.8 TB/s (the measured copy rate is 6.5); one of 201 tokens, 8/2 heads, D = 64: 6.5 us, replayed in a graph.
+// 64 sequences of up to 8190 tokens, 40/8 heads, D = 128, pages of 16: 41.5 us, 4.6 TB/s; 3 of up to 262143, 16/4 heads,
+// pages of 64: 91 us, 5.9 TB/s (the measured copy rate is 6.5); one of 201 tokens, 8/2 heads, D = 64: 6.5 us, replayed in a graph.
 //
 // Waits for a stage are bounded (sm100.cuh): a warp that gives up records a code, goes through the rest of its share
 // without loads, waits and products, drains its copies and leaves the block's outputs invalid.
@@ -55,7 +55,7 @@ struct Cfg {
   static constexpr int RING = kWarps * STAGES * STAGE;
   static constexpr int LD = DP + 4;              // joined accumulators: 8 heads per warp at a time
   static constexpr int JOIN = kWarps * 8 * LD * 4 + kWarps * 8 * 2 * 4;  // accumulators, (max, sum)
-  static constexpr int SMEM = RING + JOIN + kWarps * STAGES * 8 + 16;       // + barriers, abort flag
+  static constexpr int SMEM = RING + JOIN + kWarps * STAGES * 8 + 32;       // + barriers, abort flag, the share's numbers
   static_assert(2 * (SMEM + 1024) <= 233472, "two blocks per SM");
 };
 
@@ -77,6 +77,7 @@ __global__ void __launch_bounds__(32 * kWarps, 2) paged_decode_kernel(const __gr
   float* join = reinterpret_cast<float*>(smem + C::RING);          // [warp][8 heads][LD]
   float* join_ml = join + kWarps * 8 * C::LD;                       // [warp][8 heads][max, sum]
   volatile int* abort = reinterpret_cast<int*>(smem + C::RING + C::JOIN + kWarps * C::STAGES * 8);
+  long long* share = reinterpret_cast<long long*>(smem + C::RING + C::JOIN + kWarps * C::STAGES * 8 + 8);  // units, blocks that take part
 
   if (lane == 0) {
     if (warp == 0) *abort = 0;
@@ -86,7 +87,6 @@ __global__ void __launch_bounds__(32 * kWarps, 2) paged_decode_kernel(const __gr
     prefetch_tmap(&kp.tm_v);
   }
   __syncthreads();
-  // the join reads the lengths before it waits: it may start once every block here knows that all before this kernel is done
   wait_for_kernel_before();
   let_next_kernel_start();
   Cursor cc;
@@ -99,6 +99,7 @@ __global__ void __launch_bounds__(32 * kWarps, 2) paged_decode_kernel(const __gr
   } else {
     const long long total = total_units<WIN, kTile>(p, lane) * p.items, parts = parts_of(p, total);
     if (blockIdx.x >= parts) return;
+    if (threadIdx.x == 0) share[0] = total, share[1] = parts;
     const long long first = total * blockIdx.x / parts, last = total * (blockIdx.x + 1) / parts;
     seek<WIN, kTile>(p, first, (int)(last - first), lane, cc);
   }
@@ -278,6 +279,8 @@ __global__ void __launch_bounds__(32 * kWarps, 2) paged_decode_kernel(const __gr
       if (cc.left > 0) load_q(cc);  // of the next item, on its way meanwhile
       const int h = done.item / p.chunks, g0 = (done.item % p.chunks) * HEADS;
       const bool whole = from_start && to_end;
+      if (from_start && !p.whole_items && threadIdx.x == 0)
+        p.cuts[(int64_t)done.seq * p.items + done.item] = whole ? make_int2(-1, 0) : cut_behind(share[0], share[1], cc.tiles - cc.tile);
       const int64_t part = (int64_t)blockIdx.x * 2 + (from_start ? 1 : 0);
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
@@ -347,7 +350,7 @@ cudaError_t launch(const PagedParams& p, cudaStream_t st) {
   e = launch_early(kern, p.blocks, 32 * kWarps, C::SMEM, st, kp);
   if (e != cudaSuccess || p.whole_items) return e;
   // the join starts while the last blocks still run and waits on the device for what they wrote
-  return launch_early(paged_join_kernel<T, DP, NT, WIN, kTile>, (int64_t)p.batch * p.join_blocks, 512, 0, st, p);
+  return launch_early(paged_join_kernel<T, DP, NT>, (int64_t)p.batch * p.join_blocks, 512, 0, st, p);
 }
 
 template <typename T, bool WIN>
@@ -376,8 +379,9 @@ void paged_plan(PagedParams& p) {
   if (p.window) tiles = std::min(tiles, (p.sinks + tile - 1) / tile + (p.window + warp_rows - 1 + tile - 1) / tile);
   p.whole_items = tiles <= kMinTiles;
   // 8-bit: three blocks an SM with rings of two stages hide the ends of many items, two with three stages keep more copies in
-  // flight over few long ones (512 items of 64 sequences: 38.9 us with three, 40.8 with two; 12 items of up to 262143 tokens:
-  // 55.7 and 53.8); 16 heads need the registers of two
+  // flight over few long ones (512 items of 64 sequences: 37.9 us with three, 39.3 with two; 12 items of up to 262143 tokens:
+  // 53.4 and 51.4); 16 heads need the registers of two. Up to 64 columns four
+  // fit (the same calls at D = 64: 27.7 and 35.8 us with four, 29.8 with three and 41.9 with two)
   p.per_sm = !p.k_scale || p.nt == 2 ? 2 : p.cols == 64 ? 4 : (int64_t)p.batch * p.items >= 2 * 148 ? 3 : 2;
   p.blocks = p.whole_items ? (int64_t)p.batch * p.items : p.per_sm * 148;
 }
@@ -385,12 +389,13 @@ void paged_plan(PagedParams& p) {
 int64_t paged_workspace(const PagedParams& p) {
   if (p.whole_items) return 0;
   const int64_t rows = p.blocks * 2 * 8 * p.nt;
-  return rows * p.cols * 4 + rows * 2 * 4;
+  return rows * p.cols * 4 + rows * 2 * 4 + (int64_t)p.batch * p.items * (int64_t)sizeof(int2);
 }
 
 cudaError_t paged_decode(PagedParams p, void* workspace, bool bf16, cudaStream_t st) {
   p.part = static_cast<float*>(workspace);
   p.part_ml = p.part + p.blocks * 2 * 8 * p.nt * p.cols;
+  p.cuts = reinterpret_cast<int2*>(p.part_ml + p.blocks * 2 * 8 * p.nt * 2);
   if (p.k_scale) return paged_decode8(p, bf16, st);
   if (p.window) return bf16 ? launch_dim<__nv_bfloat16, true>(p, st) : launch_dim<__half, true>(p, st);
   return bf16 ? launch_dim<__nv_bfloat16, false>(p, st) : launch_dim<__half, false>(p, st);

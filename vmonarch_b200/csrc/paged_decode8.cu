@@ -42,7 +42,7 @@ struct Cfg {
   static constexpr int LD = DP + 4;                  // joined accumulators: 4 heads per warp at a time
   static constexpr int JOIN = kWarps * 4 * LD * 4 + kWarps * 4 * 2 * 4;  // accumulators, (max, sum)
   static constexpr int SCALES = kWarps * STAGES * 2 * kRows * 4;
-  static constexpr int SMEM = RING + JOIN + SCALES + kWarps * STAGES * 8 + 16;  // + barriers, abort flag
+  static constexpr int SMEM = RING + JOIN + SCALES + kWarps * STAGES * 8 + 32;  // + barriers, abort flag, the share's numbers
   static_assert(BLOCKS * (SMEM + 1024) <= 233472, "shared memory of an SM");
 };
 
@@ -92,6 +92,8 @@ __global__ void __launch_bounds__(32 * kWarps, BLOCKS) paged_decode8_kernel(cons
   const uint32_t scales = smem_u32(smem + C::RING + C::JOIN) + warp * C::STAGES * 2 * kRows * 4;  // [stage][K, V][token]
   const uint32_t bar0 = smem_u32(smem + C::RING + C::JOIN + C::SCALES) + 8u * warp * C::STAGES;
   volatile int* abort = reinterpret_cast<int*>(smem + C::RING + C::JOIN + C::SCALES + kWarps * C::STAGES * 8);
+  // units of all, blocks that take part
+  long long* share = reinterpret_cast<long long*>(smem + C::RING + C::JOIN + C::SCALES + kWarps * C::STAGES * 8 + 8);
 
   if (lane == 0) {
     if (warp == 0) *abort = 0;
@@ -101,7 +103,6 @@ __global__ void __launch_bounds__(32 * kWarps, BLOCKS) paged_decode8_kernel(cons
     prefetch_tmap(&kp.tm_v);
   }
   __syncthreads();
-  // the join reads the lengths before it waits: it may start once every block here knows that all before this kernel is done
   wait_for_kernel_before();
   let_next_kernel_start();
   Cursor cc;
@@ -114,6 +115,7 @@ __global__ void __launch_bounds__(32 * kWarps, BLOCKS) paged_decode8_kernel(cons
   } else {
     const long long total = total_units<WIN, kTile>(p, lane) * p.items, parts = parts_of(p, total);
     if (blockIdx.x >= parts) return;
+    if (threadIdx.x == 0) share[0] = total, share[1] = parts;
     const long long first = total * blockIdx.x / parts, last = total * (blockIdx.x + 1) / parts;
     seek<WIN, kTile>(p, first, (int)(last - first), lane, cc);
   }
@@ -376,6 +378,8 @@ __global__ void __launch_bounds__(32 * kWarps, BLOCKS) paged_decode8_kernel(cons
       if (cc.left > 0) load_q(cc);  // of the next item, on its way meanwhile
       const int h = done.item / p.chunks, g0 = (done.item % p.chunks) * HEADS;
       const bool whole = from_start && to_end;
+      if (from_start && !p.whole_items && threadIdx.x == 0)
+        p.cuts[(int64_t)done.seq * p.items + done.item] = whole ? make_int2(-1, 0) : cut_behind(share[0], share[1], cc.tiles - cc.tile);
       const int64_t part = (int64_t)blockIdx.x * 2 + (from_start ? 1 : 0);
 #pragma unroll
       for (int round = 0; round < 2 * NT; ++round) {  // heads 8 nt + 2 r + e, r < 4
@@ -442,7 +446,7 @@ cudaError_t launch(const PagedParams& p, cudaStream_t st) {
   if (e != cudaSuccess) return e;
   e = launch_early(kern, p.blocks, 32 * kWarps, C::SMEM, st, kp);
   if (e != cudaSuccess || p.whole_items) return e;
-  return launch_early(paged_join_kernel<T, DP, NT, WIN, kTile>, (int64_t)p.batch * p.join_blocks, 512, 0, st, p);
+  return launch_early(paged_join_kernel<T, DP, NT>, (int64_t)p.batch * p.join_blocks, 512, 0, st, p);
 }
 
 template <typename T, bool WIN>

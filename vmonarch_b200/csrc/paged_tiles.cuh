@@ -4,7 +4,10 @@
 // The work items (sequence, key head, chunk of up to 8 NT query heads), each a run of tiles of TILE tokens behind kItemCost
 // units for its start and end, are laid end to end and every block takes an equal share of the units, whatever the
 // sequences' lengths. An item that lies in one block is finished there; one that is cut leaves a partial
-// (max, sum, 32-bit accumulators) per block, which a second kernel joins.
+// (max, sum, 32-bit accumulators) per block, which a second kernel joins. That kernel has no room on an SM beside the first
+// one's blocks, so all that it does is paid: the block that starts an item tells it which blocks hold the rest. (Found from the
+// lengths instead, 64 sequences of up to 8190 tokens, 40/8 heads: 44.0 us for 41.5 in 16 bits, 39.8 for 38.5 in 8. A grid of the
+// kernel's blocks, each joining the item that it cut: the same there, but 58.9 us for 51.4 over 12 long items.)
 #pragma once
 #include "common.cuh"
 #include "launch.h"
@@ -43,7 +46,7 @@ __device__ __forceinline__ Span span_of(const PagedParams& p, int len) {
 template <bool WIN, int TILE>
 __device__ __forceinline__ int tiles_of(const PagedParams& p, int len) { return span_of<WIN, TILE>(p, len).tiles; }
 __device__ __forceinline__ int seq_len(const PagedParams& p, int b) {
-  return max(0, min(__ldcg(p.lengths + b), p.max_len));  // (from L2: the join reads them before it waits)
+  return max(0, min(p.lengths[b], p.max_len));
 }
 
 // The flat order of units: sequences, then items (key head, head chunk) of a sequence, then kItemCost units
@@ -123,41 +126,14 @@ __device__ __forceinline__ void advance(const PagedParams& p, Cursor& c) {
   if (++c.seq < p.batch) c.enter<WIN, TILE>(p);
 }
 
-// Joins the parts of one (sequence, query head), or where that would be more blocks than fit at once, of all
-// heads of a (sequence, item): those without work (items in one block, most of a batch's) then cost no
-// second wave. DP / 4 lanes hold a row's columns, four each; the 512 threads' groups of lanes are dealt over the
-// heads, and a head's groups over the parts.
-template <typename T, int DP, int NT, bool WIN, int TILE>
-__global__ void __launch_bounds__(512) paged_join_kernel(const __grid_constant__ PagedParams p) {
+// A block of 512 threads joins `rows` heads of an item from the blocks [c0, c1]: DP / 4 lanes hold a row's columns, four each; the
+// threads' groups of lanes are dealt over the heads (group g has head r of those from g0 on), and a head's groups over the parts.
+template <typename T, int DP, int NT>
+__device__ __forceinline__ void join_parts(const PagedParams& p, int seq, int h, int g0, int r, int rows, int c0, int c1) {
   constexpr int HEADS = 8 * NT, LANES = DP / 4, GROUPS = 512 / LANES;
   __shared__ float4 sum_o[GROUPS][LANES];
   __shared__ float2 sum_ml[GROUPS];
-  const int lane = threadIdx.x & 31;
-  const int seq = blockIdx.x / p.join_blocks, in_seq = blockIdx.x % p.join_blocks;
-  const bool one = p.join_blocks == p.heads;  // a block per head
-  const int item = one ? in_seq / p.group * p.chunks + in_seq % p.group / HEADS : in_seq;
-  // where the item lies among the blocks' shares (lengths are inputs: readable before the wait)
-  long long total = 0, before = 0;
-  for (int b = lane; b < p.batch; b += 32) {
-    const int t = units_of<WIN, TILE>(p, seq_len(p, b));
-    total += t;
-    if (b < seq) before += t;
-  }
-#pragma unroll
-  for (int s = 16; s > 0; s >>= 1) {
-    total += __shfl_xor_sync(0xffffffffu, total, s);
-    before += __shfl_xor_sync(0xffffffffu, before, s);
-  }
-  total *= p.items;
-  const int tiles = tiles_of<WIN, TILE>(p, seq_len(p, seq));
-  const long long parts = parts_of(p, total), t0 = before * p.items + (long long)item * (kItemCost + tiles) + kItemCost;
-  const int c0 = (int)(((t0 + 1) * parts - 1) / total), c1 = (int)(((t0 + tiles) * parts - 1) / total);
-  // every block waits, those without work too: the stream's next kernel must find the first one done
-  wait_for_kernel_before();
-  if (c0 == c1) return;  // finished by its block
-  const int h = item / p.chunks, g0 = (item % p.chunks) * HEADS, rows = one ? 1 : min(HEADS, p.group - g0);
   const int grp = threadIdx.x / LANES, d4 = threadIdx.x % LANES, per = GROUPS / rows;
-  const int r = one ? in_seq % p.group - g0 : grp % rows;
   const int64_t head = (int64_t)h * p.group + g0 + r;
   // block c0 holds the item's start (its second slot), the others continue it (their first)
   auto at = [&](int c) { return ((int64_t)c * 2 + (c == c0 ? 1 : 0)) * HEADS + r; };
@@ -200,6 +176,30 @@ __global__ void __launch_bounds__(512) paged_join_kernel(const __grid_constant__
     *reinterpret_cast<uint2*>(static_cast<T*>(p.o) + (int64_t)seq * p.o_row + head * p.o_head + 4 * d4) = w;
   }
   if (d4 == 0 && p.lse) p.lse[(int64_t)seq * p.heads + head] = (m + log2f(l)) * kLn2;
+}
+
+// Joins the parts of one (sequence, query head), or where that would be more blocks than fit at once, of all
+// heads of a (sequence, item): those without work (items in one block, most of a batch's) then cost no
+// second wave.
+template <typename T, int DP, int NT>
+__global__ void __launch_bounds__(512) paged_join_kernel(const __grid_constant__ PagedParams p) {
+  constexpr int HEADS = 8 * NT;
+  const int seq = blockIdx.x / p.join_blocks, in_seq = blockIdx.x % p.join_blocks;
+  const bool one = p.join_blocks == p.heads;  // a block per head
+  const int item = one ? in_seq / p.group * p.chunks + in_seq % p.group / HEADS : in_seq;
+  const int h = item / p.chunks, g0 = (item % p.chunks) * HEADS, rows = one ? 1 : min(HEADS, p.group - g0);
+  // every block waits, those without work too: the stream's next kernel must find the first one done. (It is not let start before
+  // that: its blocks would take the SMs from this one's.)
+  wait_for_kernel_before();
+  const int2 cut = p.cuts[(int64_t)seq * p.items + item];
+  if (cut.x < 0) return;  // finished by its block
+  join_parts<T, DP, NT>(p, seq, h, g0, one ? in_seq % p.group - g0 : threadIdx.x / (DP / 4) % rows, rows, cut.x, cut.y);
+}
+
+// The blocks of the item that this block has started and the end of its share cuts. `rest`: tiles of the item behind it.
+__device__ __forceinline__ int2 cut_behind(long long total, long long parts, int rest) {
+  const long long last = total * (blockIdx.x + 1) / parts;  // the end of the share, in units
+  return make_int2(blockIdx.x, (int)(((last + rest) * parts - 1) / total));
 }
 
 }  // namespace
