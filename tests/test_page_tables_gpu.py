@@ -99,6 +99,48 @@ def test_truncate_undoes_reserve(batch, page):
     tables.check()
 
 
+@pytest.mark.parametrize("batch, width, page, most", [
+    (1024, 70, 16, 60), (1024, 257, 16, 64), (1024, 257, 16, 70), (3, 40000, 1, 17000), (64, 1100, 7, 1024), (1, 70000, 1, 65536), (2, 33, 64, 2049),
+])
+def test_captured_exchanges(batch, width, page, most):
+    """Sequences given up or cut back and others admitted, captured together: one block's, a cluster's and two kernels' calls."""
+    rng = random.Random(width)
+    pool = batch * width
+    mine = rng.sample(range(pool), pool - 5)
+    tables, book = PageTables(pool, page, batch, width, pages=mine), Book(mine, page, batch, width)
+    keep, counts, total = ints([0] * batch), ints([0] * batch), batch * most
+    slots = [None]
+
+    def step():
+        tables.truncate(keep)
+        slots[0] = tables.reserve(counts, total)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    for turn in range(6):
+        left = [0 if rng.random() < 0.7 else rng.randint(0, n) for n in book.lengths]
+        if turn == 3:
+            left = list(book.lengths)
+        more = [min(rng.choice([0, 1, rng.randint(0, most), most]), width * page - n) for n in left]
+        if turn == 4:
+            more[rng.randrange(batch)] = width * page + 1  # cannot be done: slots of -1, the book as the cut left it
+        keep.copy_(ints(left))
+        counts.copy_(ints(more))
+        book.truncate(left)
+        want, bad = book.reserve(more, total)
+        graph.replay()
+        assert torch.equal(slots[0], ints(want))
+        assert (int(tables.failed) != 0) == bool(bad)
+        tables.failed.zero_()
+        same(tables, book)
+
+
 def test_what_cannot_be_done_changes_nothing():
     tables = PageTables(10, 4, 3, 3)
     tables.reserve(ints([4, 5, 0]), 9)

@@ -22,8 +22,8 @@ int fill(const char* what, const vmb_page_book* a, const int32_t* want, vmb::Boo
   return VMB_OK;
 }
 
-int workspace(const char* what, vmb::BookParams& p, bool in_one, void* ws, int64_t bytes) {
-  const int64_t need = in_one ? 0 : 4 * vmb::book_plan_ints(p.batch);
+int workspace(const char* what, vmb::BookParams& p, bool needed, void* ws, int64_t bytes) {
+  const int64_t need = !needed ? 0 : 4 * vmb::book_plan_ints(p.batch);
   if (need > 0 && (!ws || bytes < need || (reinterpret_cast<uintptr_t>(ws) & 3)))
     return set_error(VMB_EINVAL, "%s: a workspace of %lld bytes needed", what, (long long)need);
   p.plan = static_cast<int32_t*>(ws);
@@ -51,9 +51,8 @@ int vmb_reserve_pages(const vmb_page_book* a, const int32_t* counts, int32_t* sl
   if (total < 0 || total > 0x7fffffff || (total > 0 && !slots)) return set_error(VMB_EINVAL, "%s: bad number of rows, or no slots", what);
   p.slots = slots;
   p.total = total;
-  const bool one = vmb::reserve_in_one(p);
-  if ((rc = workspace(what, p, one, ws, ws_bytes))) return rc;
-  vmb::count_launches(one || total == 0 ? 1 : 2);
+  if ((rc = workspace(what, p, vmb::reserve_needs_workspace(p), ws, ws_bytes))) return rc;
+  vmb::count_launches(vmb::reserve_in_one(p) || total == 0 ? 1 : 2);
   return cuda_rc(vmb::reserve_pages(p, static_cast<cudaStream_t>(stream)), what);
 }
 
@@ -62,9 +61,8 @@ int vmb_truncate_pages(const vmb_page_book* a, const int32_t* keep, void* ws, in
   vmb::BookParams p{};
   int rc = fill(what, a, keep, p);
   if (rc || p.batch == 0) return rc;
-  const bool one = vmb::truncate_in_one(p);
-  if ((rc = workspace(what, p, one, ws, ws_bytes))) return rc;
-  vmb::count_launches(one ? 1 : 2);
+  if ((rc = workspace(what, p, vmb::truncate_needs_workspace(p), ws, ws_bytes))) return rc;
+  vmb::count_launches(vmb::truncate_in_one(p) ? 1 : 2);
   return cuda_rc(vmb::truncate_pages(p, static_cast<cudaStream_t>(stream)), what);
 }
 

@@ -11,8 +11,9 @@
 // `failed` and gives the slots -1, which the appending kernels skip.
 //
 // The work is a prefix sum over the sequences, a few bytes a token, and bound by latency: the sums are one block's (each
-// thread takes neighbouring sequences), which goes on to the rows or pages by itself where they are few; otherwise it leaves
-// its sums to a second kernel that is launched early. Whole numbers, no atomics on them: the same book from run to run.
+// thread takes neighbouring sequences), which goes on to the rows or pages by itself where they are few; where they are more, the
+// eight blocks of a cluster all form the sums and share the rest; otherwise the block leaves its sums to a second kernel that
+// is launched early. Whole numbers, no atomics on them: the same book from run to run.
 #include "common.cuh"
 #include "launch.h"
 #include "page_tables.h"
@@ -21,10 +22,16 @@ namespace vmb {
 namespace {
 
 constexpr int kThreads = 1024;
-// Most sequences of a call in one block, and rows (or table entries / 16, of which a call returns few). Both calls, us, in one
-// block and with second kernels: 64 sequences of one new token each 5.9 and 10.2, 256 of four 7.4 and 10.4, 256 of sixteen 11.1 and
-// 10.7, 8 of 1024 13.2 and 8.8.
+// Most sequences of a call in one block or one cluster, and rows (or table entries / 16, of which a call returns few). us in one
+// block, in a cluster and with a second kernel, reserve: 64 sequences of one new token each 2.1, 4.5 and 5.7, 256 of four 4.5, 4.7 and
+// 5.9, 1024 of four 9.5, 6.7 and 8.2, 8 of 1024 9.5, 5.0 and 4.6, 64 of 1024 64, 6.8 and 5.2, where the second launch costs the host
+// 2.5, 128 of 1024 134, 10.3 and 5.7; truncate, all of their pages: 2.6, 3.7 and 4.9, 3.0, 3.9 and 5.6, 4.6, 5.4 and 7.0, 4.0, 3.9
+// and 4.0, 19, 4.1 and 4.8, 39, 4.3 and 5.3.
 constexpr int kOneBatch = 1024;
+constexpr int kBlockRows = 2048;
+constexpr int kClusterRows = 65536;
+constexpr int kClusterBlocks = 8;
+// Rows up to which no workspace is asked for.
 constexpr int kOneRows = 4096;
 
 enum { kNoPages = 1, kTooWide = 2, kTooMany = 4, kOverfull = 8 };
@@ -135,12 +142,16 @@ __device__ __forceinline__ void return_pages(const BookParams& p, const Plan& pl
   }
 }
 
-// RESERVE: counts -> sums, else lengths to keep -> sums. ONE: this block does the rest too.
-template <bool RESERVE, bool ONE>
-__global__ void __launch_bounds__(kThreads) book_kernel(const __grid_constant__ BookParams p) {
-  __shared__ int32_t plan_sh[ONE ? 3 * kOneBatch + 4 : 1];
-  const Plan plan = plan_at(ONE ? plan_sh : p.plan, p.batch);
-  if (!ONE) let_next_kernel_start();
+// Where the rest of a call is done: by a kernel of its own, by the block that has the sums, or by the blocks of a cluster, which
+// all form the sums.
+enum Rest { kNext, kBlock, kCluster };
+
+// RESERVE: counts -> sums, else lengths to keep -> sums.
+template <bool RESERVE, Rest REST>
+__device__ __forceinline__ void keep_book(const BookParams& p) {
+  __shared__ int32_t plan_sh[REST != kNext ? 3 * kOneBatch + 4 : 1];
+  const Plan plan = plan_at(REST != kNext ? plan_sh : p.plan, p.batch);
+  if (REST == kNext) let_next_kernel_start();
   const int per = (p.batch + blockDim.x - 1) / blockDim.x;
   const int b0 = min((int)threadIdx.x * per, p.batch), b1 = min(b0 + per, p.batch);
   const int64_t room = min((int64_t)p.width * p.page_size, (int64_t)0x7fffffff - 64);  // (what the attention takes)
@@ -175,8 +186,8 @@ __global__ void __launch_bounds__(kThreads) book_kernel(const __grid_constant__ 
   if (threadIdx.x == 0) {
     plan.call[0] = bad == 0;
     plan.call[1] = free_before;
-    if (bad && p.failed) *p.failed |= bad;
-    if (!bad) *p.num_free = free_before + (int)(RESERVE ? -s.total_b : s.total_b);
+    if (bad && p.failed && blockIdx.x == 0) *p.failed |= bad;
+    if (!bad && REST != kCluster) *p.num_free = free_before + (int)(RESERVE ? -s.total_b : s.total_b);
   }
   if (!bad) {
     rows = s.a;
@@ -189,17 +200,36 @@ __global__ void __launch_bounds__(kThreads) book_kernel(const __grid_constant__ 
       plan.pages[b] = (int)pages;
       rows += RESERVE ? next - len : 0;
       pages += difference((int)len, (int)next);
-      p.lengths[b] = (int)next;
+      if (REST != kCluster) p.lengths[b] = (int)next;
     }
     if (threadIdx.x == 0) plan.rows[p.batch] = (int)s.total_a, plan.pages[p.batch] = (int)s.total_b;
   }
-  if (!ONE) return;
-  __syncthreads();
-  if (RESERVE) {
-    write_slots<1>(p, plan, threadIdx.x, blockDim.x);
-  } else if (!bad) {
-    return_pages(p, plan, threadIdx.x, blockDim.x);
+  if (REST == kCluster) {  // every block has read the book before one of them writes it
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    if (blockIdx.x == 0 && !bad) {
+      if (threadIdx.x == 0) *p.num_free = free_before + (int)(RESERVE ? -s.total_b : s.total_b);
+      for (int b = b0; b < b1; ++b) {
+        int64_t len, next;
+        lengths(b, len, next);
+        p.lengths[b] = (int)next;
+      }
+    }
   }
+  if (REST == kNext) return;
+  __syncthreads();
+  const int64_t at = (int64_t)blockIdx.x * blockDim.x + threadIdx.x, step = (int64_t)gridDim.x * blockDim.x;
+  if (RESERVE) {
+    constexpr int R = REST == kBlock ? 1 : 4;
+    write_slots<R>(p, plan, R * at, R * step);
+  } else if (!bad) {
+    return_pages(p, plan, at, step);
+  }
+}
+template <bool RESERVE, Rest REST>
+__global__ void __launch_bounds__(kThreads) book_kernel(const __grid_constant__ BookParams p) { keep_book<RESERVE, REST>(p); }
+template <bool RESERVE>
+__global__ void __cluster_dims__(kClusterBlocks, 1, 1) __launch_bounds__(kThreads) book_cluster_kernel(const __grid_constant__ BookParams p) {
+  keep_book<RESERVE, kCluster>(p);
 }
 
 __global__ void __launch_bounds__(256) slots_kernel(const __grid_constant__ BookParams p) {
@@ -221,16 +251,19 @@ int threads_for(int64_t n) { return (int)(n >= kThreads ? kThreads : n <= 128 ? 
 
 int64_t book_plan_ints(int64_t batch) { return 3 * batch + 4; }
 
-bool reserve_in_one(const BookParams& p) { return p.batch <= kOneBatch && p.total <= kOneRows; }
-// (at most the whole table goes back: 64 entries a thread)
-bool truncate_in_one(const BookParams& p) { return p.batch <= kOneBatch && (int64_t)p.batch * p.width <= 16 * kOneRows; }
+bool reserve_needs_workspace(const BookParams& p) { return p.batch > kOneBatch || p.total > kOneRows; }
+// (at most the whole table goes back: 64 entries a thread, 128 of a cluster's)
+bool truncate_needs_workspace(const BookParams& p) { return p.batch > kOneBatch || (int64_t)p.batch * p.width > 16 * kOneRows; }
+bool reserve_in_one(const BookParams& p) { return p.batch <= kOneBatch && p.total <= kClusterRows; }
+bool truncate_in_one(const BookParams& p) { return p.batch <= kOneBatch && (int64_t)p.batch * p.width <= 16 * kClusterRows; }
 
 cudaError_t reserve_pages(const BookParams& p, cudaStream_t st) {
   if (reserve_in_one(p)) {
-    book_kernel<true, true><<<1, threads_for(p.total > p.batch ? p.total : p.batch), 0, st>>>(p);
+    if (p.total <= kBlockRows) book_kernel<true, kBlock><<<1, threads_for(p.total > p.batch ? p.total : p.batch), 0, st>>>(p);
+    else book_cluster_kernel<true><<<kClusterBlocks, kThreads, 0, st>>>(p);
     return cudaGetLastError();
   }
-  book_kernel<true, false><<<1, threads_for(p.batch), 0, st>>>(p);
+  book_kernel<true, kNext><<<1, threads_for(p.batch), 0, st>>>(p);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess || p.total == 0) return e;
   const int64_t blocks = (p.total + 1023) / 1024;
@@ -239,10 +272,11 @@ cudaError_t reserve_pages(const BookParams& p, cudaStream_t st) {
 
 cudaError_t truncate_pages(const BookParams& p, cudaStream_t st) {
   if (truncate_in_one(p)) {
-    book_kernel<false, true><<<1, threads_for(p.batch), 0, st>>>(p);
+    if (!truncate_needs_workspace(p)) book_kernel<false, kBlock><<<1, threads_for(p.batch), 0, st>>>(p);
+    else book_cluster_kernel<false><<<kClusterBlocks, kThreads, 0, st>>>(p);
     return cudaGetLastError();
   }
-  book_kernel<false, false><<<1, threads_for(p.batch), 0, st>>>(p);
+  book_kernel<false, kNext><<<1, threads_for(p.batch), 0, st>>>(p);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return e;
   // (as many pages as the table has entries may go back, but hardly ever do)

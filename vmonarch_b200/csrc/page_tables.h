@@ -13,10 +13,12 @@ struct BookParams {
   int32_t* slots;             // reserve: [total]
   int64_t stride, total;
   int batch, width, num_pages, page_size;
-  int32_t* plan;              // workspace of book_plan_ints(batch), or NULL where one block does everything
+  int32_t* plan;              // workspace of book_plan_ints(batch), or NULL where a call needs none
 };
 
-// Whether one block does a call's work; otherwise it needs a workspace.
+// Whether a call needs a workspace, and whether one kernel does its work.
+bool reserve_needs_workspace(const BookParams& p);
+bool truncate_needs_workspace(const BookParams& p);
 bool reserve_in_one(const BookParams& p);
 bool truncate_in_one(const BookParams& p);
 int64_t book_plan_ints(int64_t batch);
