@@ -88,6 +88,23 @@ def test_splits():
     check8([40000, 30], 16, 1, 128, 64, torch.float16, window=30000, sinks=100)
 
 
+@pytest.mark.parametrize("h, hk, d", [(8, 2, 128), (4, 4, 64), (16, 1, 128), (6, 3, 48)])
+@pytest.mark.parametrize("lens", [[512], [513, 1], [640, 0, 200], [768] * 5, [1024, 1023] + [1000] * 40, [1500] * 30])
+def test_whole_and_cut(lens, h, hk, d):
+    """Short caches, whose items may stay in one block, and the same ones under a table with room for long ones."""
+    q, kp, vp, ks, vs, table, lengths, o = check8(lens, h, hk, d, 16, torch.bfloat16)
+    wide = torch.full((len(lens), 3000), -7, dtype=torch.int32, device="cuda")
+    wide[:, :table.size(1)] = table
+    scales = dict(k_scale=ks, v_scale=vs)
+    o2, lse2 = paged_attention(q, kp, vp, wide, lengths, return_lse=True, **scales)
+    _, lse = paged_attention(q, kp, vp, table, lengths, return_lse=True, **scales)
+    # each within 2 u of what both stand for
+    for a, b in zip(o, o2):
+        assert (a.double() - b.double()).norm() <= 4 * U[torch.bfloat16] * a.double().norm()
+    live = lse > float("-inf")
+    assert torch.equal(live, lse2 > float("-inf")) and (lse - lse2)[live].abs().max() <= 1e-4
+
+
 @pytest.mark.parametrize("page", [16, 8, 64])
 def test_pages_of_very_different_scales(page):
     """A page whose values are 2^40 times another's, whichever of them is attended to: every sequence to full precision."""

@@ -377,13 +377,18 @@ void paged_plan(PagedParams& p) {
   p.cols = p.dim > 64 || (p.k_scale && p.box_rows == 1) ? 128 : 64;
   int64_t tiles = (p.max_len + tile - 1) / tile;  // most that an item can have
   if (p.window) tiles = std::min(tiles, (p.sinks + tile - 1) / tile + (p.window + warp_rows - 1 + tile - 1) / tile);
-  p.whole_items = tiles <= kMinTiles;
   // 8-bit: three blocks an SM with rings of two stages hide the ends of many items, two with three stages keep more copies in
   // flight over few long ones (512 items of 64 sequences: 37.9 us with three, 39.3 with two; 12 items of up to 262143 tokens:
   // 53.4 and 51.4); 16 heads need the registers of two. Up to 64 columns four
   // fit (the same calls at D = 64: 27.7 and 35.8 us with four, 29.8 with three and 41.9 with two)
   p.per_sm = !p.k_scale || p.nt == 2 ? 2 : p.cols == 64 ? 4 : (int64_t)p.batch * p.items >= 2 * 148 ? 3 : 2;
-  p.blocks = p.whole_items ? (int64_t)p.batch * p.items : p.per_sm * 148;
+  // An item stays whole where its tiles cost no more than the cut with its join, which is about six of them where few items leave
+  // blocks free, and more where fewer are (half of the tiles, for lengths differ). D = 128, us, whole and cut: 2 items
+  // of 257 tokens 8.3 and 10.8 in 16 bits, of 513 12.6 and 10.9, in 8 bits of 513 9.2 and 11.6, of 1025 13.9 and 11.6; 256 items of
+  // 513 tokens 14.9 and 19.7, 11.4 and 17.4. The join's launch and the workspace cost the host 5 beside that.
+  const int64_t count = (int64_t)p.batch * p.items, room = p.per_sm * 148;
+  p.whole_items = tiles <= kMinTiles || (count <= room && tiles * (2 * room - count) <= 12 * room);
+  p.blocks = p.whole_items ? count : room;
 }
 
 int64_t paged_workspace(const PagedParams& p) {
