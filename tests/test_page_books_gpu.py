@@ -1,0 +1,45 @@
+"""The book of a paged cache on the GPU: calls at the ends of what it allows."""
+import pytest
+import torch
+
+from vmonarch_b200 import PagedKVCache
+
+pytestmark = pytest.mark.gpu
+
+
+def ints(x):
+    return torch.tensor(x, dtype=torch.int32, device="cuda")
+
+
+def test_taken_back_after_a_reserve_that_failed():
+    """Too few pages, a sequence too long for its row, too few rows: none of it was done, and every page is free once afterwards."""
+    cache = PagedKVCache(20, 4, 1, 16, device="cuda")
+    kept = cache.add()
+    cache.reserve([kept], [10])
+    tables = cache.page_tables(3, 6, 9)
+    tables.reserve(ints([5, 0, 9]), 14)
+    for counts, total in (([12, 12, 13], 37), ([20, 0, 0], 20), ([1, 1, 1], 2)):
+        assert (tables.reserve(ints(counts), total) == -1).all()
+    assert int(tables.failed) == 7 and tables.lengths.tolist() == [5, 0, 9]
+    cache.take_back(tables)
+    assert cache.num_free == 17 and sorted(cache._free + cache.pages(kept)) == list(range(20))
+    assert not tables.num_free.any() and not tables.lengths.any()
+    with pytest.raises(AssertionError, match="taken back"):
+        cache.take_back(tables)
+    assert cache.compact() == 3
+
+
+def test_a_loan_stays_where_its_truncation_fails():
+    cache = PagedKVCache(20, 4, 1, 16, device="cuda")
+    tables = cache.page_tables(3, 6, 9)
+    tables.reserve(ints([5, 0, 9]), 14)
+    tables.lengths[1] = 25  # what no call of its own leaves
+    for _ in range(2):
+        with pytest.raises(MemoryError, match="longer"):
+            cache.take_back(tables)
+        assert cache.num_free == 11 and tables.lengths.tolist() == [5, 25, 9] and tables.num_free.tolist() == [4]
+        with pytest.raises(AssertionError, match="moved"):
+            cache.compact()
+    tables.lengths[1] = 0
+    cache.take_back(tables)
+    assert sorted(cache._free) == list(range(20)) and cache.compact() == 0

@@ -281,12 +281,15 @@ class PagedKVCache:
 
     def take_back(self, tables) -> None:
         """Takes the pages of a :class:`PageTables` that :meth:`page_tables` made back into this book, those of its sequences
-        among them. `tables` is empty and of no more use. Waits for the device."""
-        assert self._lent.pop(id(tables), None) is tables, "not a PageTables of this cache, or taken back before"
+        among them, whatever its earlier calls could not do. `tables` is empty and of no more use. Raises MemoryError, with the
+        pages still lent, if its sequences cannot be cut (lengths that no call of its own leaves). Waits for the device."""
+        assert self._lent.get(id(tables)) is tables, "not a PageTables of this cache, or taken back before"
+        tables.failed.zero_()  # a call that could not be done changed nothing
         tables.truncate(torch.zeros_like(tables.lengths))
         tables.check()
         self._free += tables.free_pages[:int(tables.num_free)].tolist()
         tables.num_free.zero_()
+        del self._lent[id(tables)]
 
     def length(self, seq: int) -> int:
         return self._length[seq]
