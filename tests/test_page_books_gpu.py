@@ -2,7 +2,8 @@
 import pytest
 import torch
 
-from vmonarch_b200 import PagedKVCache
+from vmonarch_b200 import PagedKVCache, reserve_pages, truncate_pages
+from vmonarch_b200 import _native as N
 
 pytestmark = pytest.mark.gpu
 
@@ -43,3 +44,19 @@ def test_a_loan_stays_where_its_truncation_fails():
     tables.lengths[1] = 0
     cache.take_back(tables)
     assert sorted(cache._free) == list(range(20)) and cache.compact() == 0
+
+
+@pytest.mark.parametrize("batch", [3, 1024, 1025, 2000])
+def test_tables_without_entries(batch):
+    """Rows of no entries: nothing is held, so there is nothing to return, and no token can be taken."""
+    table = torch.empty(batch, 0, dtype=torch.int32, device="cuda")
+    lengths, free, num, failed = ints([0] * batch), ints([3, 2, 1, 0]), ints([4]), ints([0])
+    book = dict(page_size=4, failed=failed)
+    before = N.lib.vmb_kernel_launches()
+    truncate_pages(table, lengths, ints([0] * batch), free, num, **book)
+    truncate_pages(table, lengths, ints([5, -1] * (batch // 2) + [0] * (batch % 2)), free, num, **book)
+    assert N.lib.vmb_kernel_launches() == before + 2
+    assert reserve_pages(table, lengths, ints([0] * batch), free, num, total=6, **book).tolist() == [-1] * 6
+    assert not failed.any()
+    assert (reserve_pages(table, lengths, ints([1] * batch), free, num, total=batch, **book) == -1).all() and int(failed) & 2
+    assert not lengths.any() and num.tolist() == [4] and free.tolist() == [3, 2, 1, 0]

@@ -62,7 +62,7 @@ int vmb_truncate_pages(const vmb_page_book* a, const int32_t* keep, void* ws, in
   int rc = fill(what, a, keep, p);
   if (rc || p.batch == 0) return rc;
   if ((rc = workspace(what, p, vmb::truncate_needs_workspace(p), ws, ws_bytes))) return rc;
-  vmb::count_launches(vmb::truncate_in_one(p) ? 1 : 2);
+  vmb::count_launches(vmb::truncate_in_one(p) || p.width == 0 ? 1 : 2);
   return cuda_rc(vmb::truncate_pages(p, static_cast<cudaStream_t>(stream)), what);
 }
 

@@ -278,7 +278,7 @@ cudaError_t truncate_pages(const BookParams& p, cudaStream_t st) {
   }
   book_kernel<false, kNext><<<1, threads_for(p.batch), 0, st>>>(p);
   cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess) return e;
+  if (e != cudaSuccess || p.width == 0) return e;  // (rows of no entries hold no pages)
   // (as many pages as the table has entries may go back, but hardly ever do)
   const int64_t blocks = ((int64_t)p.batch * p.width + 255) / 256;
   return launch_early(return_kernel, blocks < 148 * 8 ? blocks : 148 * 8, 256, 0, st, p);
