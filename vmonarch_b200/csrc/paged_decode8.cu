@@ -12,8 +12,13 @@
 // byte permutation; V^T's rows are then 2 r and 2 r + 1 where the 16-bit form has r and r + 8). e4m3 converts to fp16 exactly, so
 // the products are fp16 for bf16 queries too: a row of those is scaled by the power of two that brings its largest element
 // below 2^15, which loses nothing above 2^-29 of it. The key scale multiplies the score. The value scale goes into the exponent: the sum takes
-// 2^(x - m), the product 2^(x + log2 vs - m'), each against a reference of its own, so that pages of any scales meet in one
-// accumulator with the precision that they would have alone; the end of an item brings the accumulators from m' to m.
+// 2^(x - m), the product P = 2^(x + log2 vs - m'), each against a reference of its own, so that pages of any scales meet in one
+// 32-bit accumulator; the end of an item brings the accumulators from m' to m. A column in which the largest weights meet small or no
+// values is the sum of small ones, so these keep their bits: the references stay 2^7 below the largest score, which puts fp16's
+// normal numbers at 2^-21 of the largest weight, and a warp with a weight below that takes the tile's product in bf16, in which
+// e4m3 is exact too, with P as the sum of two bf16 values. (GPU time with fp16 alone, of calls without such weights and where every
+// tile has some: 64 sequences of up to 8192 tokens, 40/8 heads, D = 128: 95.2 us, 96.5 and 108; 3 of up to 262143, 16/4 heads: 71.9, 73.3
+// and 85.5. Weights sorted by size into fp16 products with factors of their own: 146 and 116 at scores of 8 nats' deviation.)
 //
 // Waits for a stage are bounded as in paged_decode.cu.
 #include "paged_tiles.cuh"
@@ -30,7 +35,10 @@ using namespace sm100;
 
 constexpr int kTile = kPagedTile8;
 constexpr int kRows = kTile / kWarps;  // tokens of a tile that a warp owns
-constexpr float kRaise = 8.f;          // a reference is raised once a score passes it by more: P <= 2^8, inside fp16
+// A reference is raised, to 2^-kLift of the largest score, once a score passes it by more than 2^kRaise: P <= 2^15, inside fp16.
+constexpr float kLift = 7.f, kRaise = 15.f;
+// Exponents between which a weight is too small for fp16's normal numbers, but not for 32 bits.
+constexpr float kLeast = -14.f, kNone = -126.f;
 static_assert(kRows == 32, "a lane a token");
 
 template <int DP, int NT, int BLOCKS>
@@ -293,74 +301,111 @@ __global__ void __launch_bounds__(32 * kWarps, BLOCKS) paged_decode8_kernel(cons
             for (int nt = 0; nt < NT; ++nt) mma16816<__half>(s[nt][h], a, qf[nt][2 * k2 + e][0], qf[nt][2 * k2 + e][1]);
           }
         }
-      uint32_t pb[NT][2][2];
+      float y[NT][4][2];  // scores that weigh the values, with their scale, then the weights
+      bool wide = false;  // whether some of these are too small for fp16
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         // i: rows lane / 4 + 8 i; e: heads 2 (lane % 4) + e
-        float x[4][2], y[4][2];  // scores, and those that weigh the values, with their scale
+        float x[4][2];
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             x[i][e] = s[nt][i >> 1][(i & 1) * 2 + e] * (qs[nt][e] * k_by[i]);
-            y[i][e] = x[i][e] + v_log[i];
+            y[nt][i][e] = x[i][e] + v_log[i];
           }
         if (rows != 0xffffffffu) {
 #pragma unroll
           for (int i = 0; i < 4; ++i)
-            if (!((rows >> (lane / 4 + 8 * i)) & 1u)) x[i][0] = y[i][0] = x[i][1] = y[i][1] = -INFINITY;
+            if (!((rows >> (lane / 4 + 8 * i)) & 1u)) x[i][0] = y[nt][i][0] = x[i][1] = y[nt][i][1] = -INFINITY;
         }
         float mx[2], my[2], al[2];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           mx[e] = fmaxf(fmaxf(x[0][e], x[1][e]), fmaxf(x[2][e], x[3][e]));
-          my[e] = fmaxf(fmaxf(y[0][e], y[1][e]), fmaxf(y[2][e], y[3][e]));
+          my[e] = fmaxf(fmaxf(y[nt][0][e], y[nt][1][e]), fmaxf(y[nt][2][e], y[nt][3][e]));
         }
-        if (__any_sync(0xffffffffu, fmaxf(fmaxf(mx[0] - m[nt][0], my[0] - mv[nt][0]), fmaxf(mx[1] - m[nt][1], my[1] - mv[nt][1])) >
-                                        kRaise)) {
+        const bool above = fmaxf(fmaxf(mx[0] - m[nt][0], my[0] - mv[nt][0]), fmaxf(mx[1] - m[nt][1], my[1] - mv[nt][1])) > kRaise;
+        float least[2];
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
+        for (int e = 0; e < 2; ++e) least[e] = fminf(fminf(y[nt][0][e], y[nt][1][e]), fminf(y[nt][2][e], y[nt][3][e])) - mv[nt][e];
+        if (__any_sync(0xffffffffu, above || fminf(least[0], least[1]) < kLeast)) {
+          if (__any_sync(0xffffffffu, above)) {
 #pragma unroll
-            for (int w = 4; w < 32; w <<= 1) {
-              mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], w));
-              my[e] = fmaxf(my[e], __shfl_xor_sync(0xffffffffu, my[e], w));
+            for (int e = 0; e < 2; ++e) {
+#pragma unroll
+              for (int w = 4; w < 32; w <<= 1) {
+                mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], w));
+                my[e] = fmaxf(my[e], __shfl_xor_sync(0xffffffffu, my[e], w));
+              }
+              const float mn = fmaxf(m[nt][e], mx[e] - kLift), vn = fmaxf(mv[nt][e], my[e] - kLift);
+              l[nt][e] *= fast_exp2(m[nt][e] - mn);
+              al[e] = fast_exp2(mv[nt][e] - vn);
+              m[nt][e] = mn;
+              mv[nt][e] = vn;
             }
-            const float mn = fmaxf(m[nt][e], mx[e]), vn = fmaxf(mv[nt][e], my[e]);
-            l[nt][e] *= fast_exp2(m[nt][e] - mn);
-            al[e] = fast_exp2(mv[nt][e] - vn);
-            m[nt][e] = mn;
-            mv[nt][e] = vn;
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) acc[nt][ks][e] *= al[e & 1];
           }
+          bool low = false;
 #pragma unroll
-          for (int ks = 0; ks < KS; ++ks)
+          for (int i = 0; i < 4; ++i)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) acc[nt][ks][e] *= al[e & 1];
+            for (int e = 0; e < 2; ++e) low |= y[nt][i][e] - mv[nt][e] < kLeast && y[nt][i][e] - mv[nt][e] >= kNone;
+          wide |= __any_sync(0xffffffffu, low);
         }
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           l[nt][e] += (fast_exp2(x[0][e] - m[nt][e]) + fast_exp2(x[1][e] - m[nt][e])) +
                       (fast_exp2(x[2][e] - m[nt][e]) + fast_exp2(x[3][e] - m[nt][e]));
 #pragma unroll
-          for (int i = 0; i < 4; ++i) y[i][e] = fast_exp2(y[i][e] - mv[nt][e]);
+          for (int i = 0; i < 4; ++i) y[nt][i][e] = fast_exp2(y[nt][i][e] - mv[nt][e]);
         }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) pb[nt][i >> 1][i & 1] = movmatrix(Elem<__half>::pack(y[i][0], y[i][1]));
       }
+      auto times_values = [&](auto type) {  // acc += V^T P, in products of that type; bf16: P as the sum of two values
+        using M = decltype(type);
+        constexpr int PARTS = Elem<M>::is_bf16 ? 2 : 1;
+        uint32_t pb[PARTS][NT][2][2];
 #pragma unroll
-      for (int k2 = 0; k2 < KS / 2; ++k2)
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {  // 16 columns of tokens 0-7, 8-15 of the half, the next 16 of them
-          uint32_t x[4];
-          ldsm_x4_t(vs_base + chunk_at<DP>(16 * h + (lane & 15), 2 * k2 + (lane >> 4)), x[0], x[1], x[2], x[3]);
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            // columns (2 r, 2 r + 1) of two tokens -> two tokens of column 2 r, two of 2 r + 1
-            const uint32_t lo = __byte_perm(x[2 * e], 0, 0x3120), hi = __byte_perm(x[2 * e + 1], 0, 0x3120);
-            const uint32_t a[4] = {f16x2_lo(lo), f16x2_hi(lo), f16x2_lo(hi), f16x2_hi(hi)};
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) mma16816<__half>(acc[nt][2 * k2 + e], a, pb[nt][h][0], pb[nt][h][1]);
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t p0 = Elem<M>::pack(y[nt][i][0], y[nt][i][1]);
+            pb[0][nt][i >> 1][i & 1] = movmatrix(p0);
+            if (PARTS == 2) {
+              const float2 f = Elem<M>::unpack(p0);
+              pb[PARTS - 1][nt][i >> 1][i & 1] = movmatrix(Elem<M>::pack(y[nt][i][0] - f.x, y[nt][i][1] - f.y));
+            }
           }
-        }
+#pragma unroll
+        for (int k2 = 0; k2 < KS / 2; ++k2)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {  // 16 columns of tokens 0-7, 8-15 of the half, the next 16 of them
+            uint32_t x[4];
+            ldsm_x4_t(vs_base + chunk_at<DP>(16 * h + (lane & 15), 2 * k2 + (lane >> 4)), x[0], x[1], x[2], x[3]);
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              // columns (2 r, 2 r + 1) of two tokens -> two tokens of column 2 r, two of 2 r + 1
+              const uint32_t lo = __byte_perm(x[2 * e], 0, 0x3120), hi = __byte_perm(x[2 * e + 1], 0, 0x3120);
+              uint32_t a[4] = {f16x2_lo(lo), f16x2_hi(lo), f16x2_lo(hi), f16x2_hi(hi)};
+              if (Elem<M>::is_bf16) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                  const float2 f = Elem<__half>::unpack(a[i]);
+                  a[i] = Elem<M>::pack(f.x, f.y);
+                }
+              }
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int i = 0; i < PARTS; ++i) mma16816<M>(acc[nt][2 * k2 + e], a, pb[i][nt][h][0], pb[i][nt][h][1]);
+            }
+          }
+      };
+      if (wide) times_values(__nv_bfloat16());
+      else times_values(__half());
     }
     __syncwarp();  // every lane is done with the stage that the next issue refills
     issue(it + C::STAGES - 1);
@@ -370,11 +415,19 @@ __global__ void __launch_bounds__(32 * kWarps, BLOCKS) paged_decode8_kernel(cons
     const bool to_end = cc.tile == 0;
     if (to_end || cc.left <= 0) {
       // ---- the four warps' parts of this item (or of this block's share of it)
-      float to_m[NT][2];
+      // sums and accumulators to the reference m + kLift, the largest score that raised it; the latter's factor in two parts, for scales
+      // near the ends of their range would take it out of its own
+      float to_m[NT][2][2];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int e = 0; e < 2; ++e) to_m[nt][e] = fast_exp2(mv[nt][e] - m[nt][e]);
+        for (int e = 0; e < 2; ++e) {
+          m[nt][e] += kLift;
+          l[nt][e] *= fast_exp2(-kLift);
+          const float by = mv[nt][e] - m[nt][e], half = rintf(0.5f * by);
+          to_m[nt][e][0] = fast_exp2(half);
+          to_m[nt][e][1] = fast_exp2(by - half);
+        }
       if (cc.left > 0) load_q(cc);  // of the next item, on its way meanwhile
       const int h = done.item / p.chunks, g0 = (done.item % p.chunks) * HEADS;
       const bool whole = from_start && to_end;
@@ -391,7 +444,7 @@ __global__ void __launch_bounds__(32 * kWarps, BLOCKS) paged_decode8_kernel(cons
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks)
           *reinterpret_cast<float2*>(join + (warp * 4 + lane % 4) * C::LD + 16 * ks + 2 * (lane / 4)) =
-              make_float2(acc[nt][ks][e] * to_m[nt][e], acc[nt][ks][2 + e] * to_m[nt][e]);
+              make_float2(acc[nt][ks][e] * to_m[nt][e][0] * to_m[nt][e][1], acc[nt][ks][2 + e] * to_m[nt][e][0] * to_m[nt][e][1]);
         __syncthreads();
         for (int i = threadIdx.x; i < 4 * DP; i += 32 * kWarps) {
           const int r = i / DP, d = i % DP, in = 8 * nt + 2 * r + e, g = g0 + in;
