@@ -49,6 +49,11 @@ using namespace sm100;
 constexpr int kAtom = 128 * 128;  // one swizzle atom column block: 128 rows x 128 B
 constexpr int kThreads = 320;
 constexpr float kSumThreshold = 16384.0f;
+// With a window, sinks may hold nearly all of the weight and small values, so that the rest is what counts: in fp16 the reference stays
+// this far below the largest score that set it, and weights down to 2^-21 of the largest keep their bits.
+template <typename T, bool WIN>
+constexpr float kLift = WIN && !Elem<T>::is_bf16 ? 7.f : 0.f;
+static_assert(64 * 128 <= kSumThreshold, "a half's sum against a reference that it has just set");
 
 struct KParams {
   CUtensorMap tm_q, tm_k, tm_v;
@@ -523,7 +528,7 @@ __global__ void __launch_bounds__(kThreads, 1) packed_fwd_kernel(const __grid_co
             if (__any_sync(0xffffffffu, live && !(lt <= kSumThreshold))) {
               if (hf == 1 && !(ok = warp_wait(B_PVH + w, steps & 1, 16))) break;
               tc_fence_after();
-              rescale(row_max<64, false>(s, 64) * p.scale_log2);
+              rescale(row_max<64, false>(s, 64) * p.scale_log2 - kLift<T, WIN>);
               lt = probs<T, 64, false>(s, pk, p.scale_log2, m_ref, 64);
             }
             l += lt;
@@ -570,7 +575,7 @@ __global__ void __launch_bounds__(kThreads, 1) packed_fwd_kernel(const __grid_co
                     tmem_wait_ld();
                     mx = fmaxf(mx, row_max_bits(s, seen[c]));
                   }
-                  return fmaxf(mx * p.scale_log2, -1e30f);
+                  return fmaxf(mx * p.scale_log2 - kLift<T, WIN>, -1e30f);
                 };
                 // (a query that sees none of these keys keeps the reference of no key)
                 if (hf == 0 && t == 0) m_ref = fmaxf(m_ref, top());

@@ -45,6 +45,10 @@ namespace {
 using namespace sm100;
 
 constexpr int kTile = 64;  // tokens per tile: 16 per warp
+// With a window, sinks may hold nearly all of the weight and small values, so that the rest is what counts: in fp16 the reference stays
+// this far below the largest score, P <= 2^15, and weights down to 2^-29 of the largest keep their bits.
+template <typename T, bool WIN>
+constexpr float kLift = WIN && !Elem<T>::is_bf16 ? 15.f : 0.f;
 
 template <int DP, int NT>
 struct Cfg {
@@ -237,6 +241,8 @@ __global__ void __launch_bounds__(32 * kWarps, 2) paged_decode_kernel(const __gr
           mx[0] = fmaxf(mx[0], __shfl_xor_sync(0xffffffffu, mx[0], w));
           mx[1] = fmaxf(mx[1], __shfl_xor_sync(0xffffffffu, mx[1], w));
         }
+        mx[0] -= kLift<T, WIN>;
+        mx[1] -= kLift<T, WIN>;
         if (__any_sync(0xffffffffu, mx[0] > m[nt][0] || mx[1] > m[nt][1])) {
           float al[2];
 #pragma unroll
