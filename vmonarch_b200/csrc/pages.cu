@@ -301,8 +301,10 @@ cudaError_t launch_e4m3(PageMoveParams p, cudaStream_t st) {
   // and 13.1; one row of each of 64 sequences, whatever their pages, 3.3 and 4.8.
   const bool block = p.page_size >= 64 && p.count >= 2 * (int64_t)p.page_size;
   const int64_t pairs = 2 * p.kv_heads;
-  // one row a team while all teams fit on the GPU at once, up to a page's rows where there are many
-  const int64_t room = block ? 148 * 16 : 148 * 16 * kTeamWarps;
+  // one row a team while all teams are on the GPU at once, up to a page's rows where there are many (8 heads, D = 128, us, with this room and
+  // with that of 16 blocks an SM, at which teams of one row took up to three turns: 512 rows of a prompt, pages of 16, 4.1 and 5.4, pages
+  // of 64 4.7 and 5.4; one row of each of 512 sequences, pages of 16, 7.3 and 8.3)
+  const int64_t room = 148 * kTeamBlocks * (block ? 1 : kTeamWarps);
   p.group = (int)std::min<int64_t>(std::max<int64_t>((p.count * pairs + room - 1) / room, 1), std::min(p.page_size, 32));
   const int64_t teams = (p.count + p.group - 1) / p.group * pairs, blocks = block ? teams : (teams + kTeamWarps - 1) / kTeamWarps;
   if (teams > 0x7fffffff) return cudaErrorInvalidConfiguration;
