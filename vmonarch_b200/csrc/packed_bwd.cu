@@ -188,8 +188,9 @@ __global__ void __launch_bounds__(256) packed_sum_kernel(const __grid_constant__
 }
 
 // ------------------------------------------------------------------------------------ statistics
-// With a window: D of a query that sees two to eight keys as sum_j P_j (do . v_j), where `d` is o . do. The rounding of P in o does
-// not average out over so few keys (sequences of one and three tokens, fp16: error of dK 1.53 -> 1.43 times that of its own rounding).
+// With a window, under which all queries may see that few: D of a query that sees two to eight keys as sum_j P_j (do . v_j), where `d` is
+// o . do. The rounding of P in o does not average out over so few keys (400 sequences of one and three tokens, fp16: error of dK
+// 1.49 -> 1.41 times that of its own rounding). Without one only a sequence's first queries do, which keep o . do.
 // 16 lanes a row, eight columns each; warp-collective.
 template <typename T>
 __device__ __forceinline__ float few_keys_d(const PackedParams& a, const PackedUnit& u, int head, int r, int sub, bool valid, float d) {

@@ -605,7 +605,7 @@ __global__ void __launch_bounds__(kThreads, 1) packed_fwd_kernel(const __grid_co
               const int least = __shfl_sync(0xffffffffu, seen, 0);  // the warp's first query (limits only grow)
               const int most = __shfl_sync(0xffffffffu, seen, 31);  // and its last
               if (most <= 0) {
-  #pragma unroll
+#pragma unroll
                 for (int e = 0; e < 32; ++e) pk[e] = 0u;
               } else {
                 uint32_t s[64];
@@ -614,7 +614,7 @@ __global__ void __launch_bounds__(kThreads, 1) packed_fwd_kernel(const __grid_co
                 tmem_wait_ld();
                 if (hf == 0 && t == 0) m_ref = (least >= 64 ? row_max<64, false>(s, 64) : row_max<64, true>(s, seen)) * p.scale_log2;
                 float lt = 0.f;
-  #pragma unroll 1
+#pragma unroll 1
                 for (int pass = 0; pass < 2; ++pass) {
                   if (least >= 64) {
                     lt = probs<T, 64, false>(s, pk, p.scale_log2, m_ref, 64);
@@ -628,7 +628,7 @@ __global__ void __launch_bounds__(kThreads, 1) packed_fwd_kernel(const __grid_co
                     if (most > 32) {
                       lt += probs<T, 32, true>(s1, p1, p.scale_log2, m_ref, seen - 32);
                     } else {
-  #pragma unroll
+#pragma unroll
                       for (int e = 0; e < 16; ++e) p1[e] = 0u;
                     }
                   }

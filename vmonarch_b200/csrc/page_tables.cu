@@ -31,8 +31,10 @@ constexpr int kOneBatch = 1024;
 constexpr int kBlockRows = 2048;
 constexpr int kClusterRows = 65536;
 constexpr int kClusterBlocks = 8;
-// Rows up to which no workspace is asked for.
-constexpr int kOneRows = 4096;
+// Rows, and table entries, up to which no workspace is asked for, though a cluster's calls do not read it.
+constexpr int kOneRows = 4096, kOneEntries = 65536;
+// Table entries up to which one block does a truncate: the whole table may go back, 64 entries a thread.
+constexpr int kBlockEntries = 65536;
 
 enum { kNoPages = 1, kTooWide = 2, kTooMany = 4, kOverfull = 8 };
 
@@ -252,8 +254,7 @@ int threads_for(int64_t n) { return (int)(n >= kThreads ? kThreads : n <= 128 ? 
 int64_t book_plan_ints(int64_t batch) { return 3 * batch + 4; }
 
 bool reserve_needs_workspace(const BookParams& p) { return p.batch > kOneBatch || p.total > kOneRows; }
-// (at most the whole table goes back: 64 entries a thread, 128 of a cluster's)
-bool truncate_needs_workspace(const BookParams& p) { return p.batch > kOneBatch || (int64_t)p.batch * p.width > 16 * kOneRows; }
+bool truncate_needs_workspace(const BookParams& p) { return p.batch > kOneBatch || (int64_t)p.batch * p.width > kOneEntries; }
 bool reserve_in_one(const BookParams& p) { return p.batch <= kOneBatch && p.total <= kClusterRows; }
 bool truncate_in_one(const BookParams& p) { return p.batch <= kOneBatch && (int64_t)p.batch * p.width <= 16 * kClusterRows; }
 
@@ -272,7 +273,7 @@ cudaError_t reserve_pages(const BookParams& p, cudaStream_t st) {
 
 cudaError_t truncate_pages(const BookParams& p, cudaStream_t st) {
   if (truncate_in_one(p)) {
-    if (!truncate_needs_workspace(p)) book_kernel<false, kBlock><<<1, threads_for(p.batch), 0, st>>>(p);
+    if ((int64_t)p.batch * p.width <= kBlockEntries) book_kernel<false, kBlock><<<1, threads_for(p.batch), 0, st>>>(p);
     else book_cluster_kernel<false><<<kClusterBlocks, kThreads, 0, st>>>(p);
     return cudaGetLastError();
   }

@@ -384,9 +384,10 @@ void paged_plan(PagedParams& p) {
   int64_t tiles = (p.max_len + tile - 1) / tile;  // most that an item can have
   if (p.window) tiles = std::min(tiles, (p.sinks + tile - 1) / tile + (p.window + warp_rows - 1 + tile - 1) / tile);
   // 8-bit: three blocks an SM with rings of two stages hide the ends of many items, two with three stages keep more copies in
-  // flight over few long ones (512 items of 64 sequences: 37.9 us with three, 39.3 with two; 12 items of up to 262143 tokens:
-  // 53.4 and 51.4); 16 heads need the registers of two. Up to 64 columns four
-  // fit (the same calls at D = 64: 27.7 and 35.8 us with four, 29.8 with three and 41.9 with two)
+  // flight over few long ones (512 items of 64 sequences: 38.3 us with three, 41.1 with two; 12 items of up to 262143 tokens:
+  // 54.1 and 51.7); 16 heads need the registers of two. Up to 64 columns four
+  // fit (the same calls at D = 64, before small weights took products of their own: 25.5 and 34.9 us with four, 29.8 with three and 41.9 with
+  // two; with them 25.9 and 35.9 with four)
   p.per_sm = !p.k_scale || p.nt == 2 ? 2 : p.cols == 64 ? 4 : (int64_t)p.batch * p.items >= 2 * 148 ? 3 : 2;
   // An item stays whole where its tiles cost no more than the cut with its join, which is about six of them where few items leave
   // blocks free, and more where fewer are (half of the tiles, for lengths differ). D = 128, us, whole and cut: 2 items

@@ -79,7 +79,7 @@ def paged_attention(q, k_pages, v_pages, page_table, lengths, *, k_scale=None, v
         k_pages, v_pages: (num_pages, Hk, page_size, D), the same dtype, H a multiple of Hk; any strides
             with contiguous columns and 16-byte aligned rows, any page size. Or torch.float8_e4m3fn, D a multiple of 16
         k_scale, v_scale: (num_pages, Hk) float32, not negative, with 8-bit pools: a key or value is its element times the
-            scale of its page and head
+            scale of its page and head. Of a bf16 query's elements those below 2^-29 of its largest lose bits then.
         page_table: (B, width) int32, the pages of each sequence; entries past its length are not read.
             A page id outside the pool reads as zeros.
         lengths: (B,) int32, the tokens each sequence has cached, the new one's among them if it is to
