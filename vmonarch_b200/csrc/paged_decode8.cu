@@ -5,7 +5,7 @@
 // where ks_t and vs_t are the scales of token t's page. Half the bytes a token, and so half the time that a block may spend on
 // one: a warp owns 32 tokens of every tile (the loop, the looking up of pages and the softmax's bookkeeping are paid per
 // 32), each lane looks up one token's page and copies its two scales, and the softmax keeps its reference until a score
-// passes it by more than 2^8, which a vote over the warp says without a maximum over lanes.
+// passes the one that set it by more than 2^8, which a vote over the warp says without a maximum over lanes.
 //
 // Operands. ldmatrix moves pairs of bytes: it leaves a lane with four neighbouring columns of a key (a permutation of the
 // contraction index, in which the queries are loaded too) and, transposed, with two neighbouring columns of two tokens (a
@@ -35,7 +35,8 @@ using namespace sm100;
 
 constexpr int kTile = kPagedTile8;
 constexpr int kRows = kTile / kWarps;  // tokens of a tile that a warp owns
-// A reference is raised, to 2^-kLift of the largest score, once a score passes it by more than 2^kRaise: P <= 2^15, inside fp16.
+// A reference is raised, to 2^-kLift of the largest score, once a score passes it by more than 2^kRaise: P <= 2^15, inside fp16, and the
+// score that set it is passed by 2^(kRaise - kLift).
 constexpr float kLift = 7.f, kRaise = 15.f;
 // Exponents between which a weight is too small for fp16's normal numbers, but not for 32 bits.
 constexpr float kLeast = -14.f, kNone = -126.f;
